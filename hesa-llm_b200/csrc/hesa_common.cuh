@@ -19,6 +19,7 @@ enum : int {
     kStatusDrainTimeout = 2,    // a copy still in flight during the error exit
     kStatusBadPosition = 3,     // a device-side position outside the cache / rope table
     kStatusPeerTimeout = 4,     // a peer rank did not reach the all-gather barrier in time
+    kStatusNoPages = 5,         // fewer free pages than a change of the page tables needs
 };
 
 constexpr unsigned long long HESA_WAIT_LIMIT_NS = 2000000000ull;  // 2 s

@@ -42,7 +42,44 @@ class Layer(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("wq", "wk", "wv", "wo", "w_gate", "w_up", "w_down", "attn_norm",
                                               "ffn_norm", "k_cache", "v_cache")]
 
+
+
+class PagedKVStruct(ctypes.Structure):
+    """hesa_cuda_paged_kv (include/hesa_cuda.h)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("page_stride", ctypes.c_int64),
+                ("layer_stride", ctypes.c_int64), ("n_layer", ctypes.c_int32), ("n_pages", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("n_kv_head", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("table", ctypes.c_void_p), ("seq_len", ctypes.c_void_p), ("page_refs", ctypes.c_void_p),
+                ("n_slots", ctypes.c_int32), ("max_pages", ctypes.c_int32)]
+
+
+class TokenBatchStruct(ctypes.Structure):
+    """hesa_cuda_token_batch (include/hesa_cuda.h)."""
+    _fields_ = [("slots", ctypes.c_void_p), ("q_start", ctypes.c_void_p), ("n_seq", ctypes.c_int32),
+                ("n_tokens", ctypes.c_int32), ("max_new", ctypes.c_int32), ("max_len", ctypes.c_int32)]
+
+
+class AttnOptionsStruct(ctypes.Structure):
+    """hesa_cuda_attn_options (include/hesa_cuda.h)."""
+    _fields_ = [("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("window", ctypes.c_int32),
+                ("slopes", ctypes.c_void_p), ("prefix", ctypes.c_void_p)]
+
+
+_kvp, _batchp, _optp = ctypes.POINTER(PagedKVStruct), ctypes.POINTER(TokenBatchStruct), ctypes.POINTER(AttnOptionsStruct)
+_i32 = ctypes.c_int32
+
 SIGNATURES = [
+    ("hesa_cuda_paged_attention_workspace_size", _sz, [_kvp, _batchp, _i64]),
+    ("hesa_cuda_paged_attention", _int, [_kvp, _i32, _batchp, _vp, _i64, _vp, _i64, _i64, _optp, _vp, _sz, _vp]),
+    ("hesa_cuda_rope_kv_paged", _int, [_kvp, _i32, _batchp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i32, _vp]),
+    ("hesa_cuda_kv_pages_workspace_size", _sz, [_kvp]),
+    ("hesa_cuda_kv_reserve", _int, [_kvp, _vp, _vp, _i32, _vp, _sz, _vp]),
+    ("hesa_cuda_kv_free", _int, [_kvp, _vp, _i32, _vp, _sz, _vp]),
+    ("hesa_cuda_kv_fork", _int, [_kvp, _vp, _vp, _i32, _vp, _sz, _vp]),
+    ("hesa_cuda_kv_compact", _int, [_kvp, _vp, _vp, _sz, _vp]),
+    ("hesa_cuda_kv_copy_pages", _int, [_kvp, _vp, _vp, _i32, _vp, _sz, _vp]),
+    ("hesa_cuda_token_logprobs_workspace_size", _sz, [_i64, _i64, _i32]),
+    ("hesa_cuda_token_logprobs", _int, [_vp, _i64, _i64, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     ("hesa_cuda_version", ctypes.c_char_p, []),
     ("hesa_cuda_row_bytes", _sz, [_int, _i64]),
     ("hesa_cuda_qmatvec_workspace_size", _sz, [_int, _i64, _i64, _i64]),
@@ -468,3 +505,275 @@ def make_layers(per_layer):
         for name, _ in Layer._fields_:
             setattr(arr[i], name, d[name].data_ptr())
     return arr
+
+
+# --------------------------------------------------------------------------
+# paged KV cache and token log probabilities
+# --------------------------------------------------------------------------
+
+def _want(t, dtype, what: str, device=None, dims: int | None = None):
+    """A CUDA tensor of this type on `device` (None: the current one); ValueError else."""
+    import torch
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or not t.is_cuda:
+        raise ValueError(f"{what} must be a CUDA tensor of {dtype}")
+    if t.device.index != (torch.cuda.current_device() if device is None else device):
+        raise ValueError(f"{what} is on {t.device}: every tensor must be on the current CUDA device, the cache's")
+    if dims is not None and t.dim() != dims:
+        raise ValueError(f"{what} must have {dims} dimensions")
+
+
+def _ints(t, what: str, n: int | None = None, device=None):
+    import torch
+    _want(t, torch.int32, what, device, 1)
+    if t.numel() > 1 and t.stride(0) != 1:
+        raise ValueError(f"{what} must be contiguous")
+    if n is not None and t.numel() != n:
+        raise ValueError(f"{what} must hold {n} values")
+    return t.data_ptr()
+
+
+def _new(make, stream):
+    """A tensor made for a call on `stream`: allocated and filled there, so that it may be freed in that stream's order."""
+    import torch
+    if stream is None:
+        return make()
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream) if stream else torch.cuda.default_stream()
+    with torch.cuda.stream(stream):
+        return make()
+
+
+class PagedKV:
+    """A paged fp16 KV cache (hesa_cuda_paged_kv): the page pools k, v
+    [n_layer, n_pages, page_size, n_kv_head, head_dim] (any layer and page
+    strides, the rest contiguous), the tables table [n_slots, max_pages],
+    seq_len [n_slots] and page_refs [n_pages] (int32; page_refs may be None
+    without page operations). Keeps the tensors and a scratch buffer for the
+    page operations; everything lies on one CUDA device."""
+
+    def __init__(self, k, v, table, seq_len, page_refs=None):
+        import torch
+        _want(k, torch.float16, "k", dims=5)
+        dev = k.device.index
+        _want(v, torch.float16, "v", dev, 5)
+        _want(table, torch.int32, "table", dev, 2)
+        if v.shape != k.shape or (v.stride(0), v.stride(1)) != (k.stride(0), k.stride(1)):
+            raise ValueError("k and v must have the same shape and strides")
+        n_layer, n_pages, page, n_kv, hd = k.shape
+        for t in (k, v):
+            if (t.stride(2), t.stride(3), t.stride(4)) != (n_kv * hd, hd, 1):
+                raise ValueError("places, heads and dims of a page must be contiguous")
+        if not table.is_contiguous():
+            raise ValueError("table must be contiguous")
+        _ints(seq_len, "seq_len", table.shape[0], dev)
+        if page_refs is not None:
+            _ints(page_refs, "page_refs", n_pages, dev)
+        self.device, self.n_slots, self.n_pages, self.n_kv_head, self.head_dim = dev, table.shape[0], n_pages, n_kv, hd
+        self.k, self.v, self.table, self.seq_len, self.page_refs = k, v, table, seq_len, page_refs
+        self.struct = PagedKVStruct(k.data_ptr(), v.data_ptr(), k.stride(1), k.stride(0), n_layer, n_pages, page, n_kv, hd,
+                                    table.data_ptr(), seq_len.data_ptr(), _ptr(page_refs), table.shape[0], table.shape[1])
+        self.ref = ctypes.byref(self.struct)
+        self.workspace = None
+
+    @classmethod
+    def empty(cls, n_layer: int, n_pages: int, page_size: int, n_kv_head: int, head_dim: int, n_slots: int, max_pages: int):
+        """A new cache on the current device with every page free and every slot empty."""
+        import torch
+        shape = (n_layer, n_pages, page_size, n_kv_head, head_dim)
+        return cls(torch.zeros(shape, dtype=torch.float16, device="cuda"), torch.zeros(shape, dtype=torch.float16, device="cuda"),
+                   torch.full((n_slots, max_pages), -1, dtype=torch.int32, device="cuda"),
+                   torch.zeros(n_slots, dtype=torch.int32, device="cuda"), torch.zeros(n_pages, dtype=torch.int32, device="cuda"))
+
+
+class TokenBatch:
+    """New tokens of several sequences (hesa_cuda_token_batch): q_start
+    [n_seq + 1] and slots [n_seq] (None: sequence i is in slot i), int32 on the
+    device; n_tokens rows in all, at most max_new new tokens and max_len tokens
+    for any sequence. The tensors may be refilled for every step within these
+    bounds."""
+
+    def __init__(self, q_start, n_tokens: int, max_new: int, max_len: int, slots=None):
+        _ints(q_start, "q_start")
+        n_seq = q_start.numel() - 1
+        if slots is not None:
+            _ints(slots, "slots", n_seq, q_start.device.index)
+        self.device, self.n_tokens, self.n_seq = q_start.device.index, n_tokens, n_seq
+        self.q_start, self.slots = q_start, slots
+        self.struct = TokenBatchStruct(_ptr(slots), q_start.data_ptr(), n_seq, n_tokens, max_new, max_len)
+        self.ref = ctypes.byref(self.struct)
+
+
+def _rows(t, n: int, width: int, what: str, device):
+    """Pointer and row stride of fp32 rows [n, width] (a column slice of a wider matrix is one)."""
+    import torch
+    _want(t, torch.float32, what, device, 2)
+    if t.shape[0] != n or t.shape[1] != width or (t.stride(1) != 1 and width > 1):
+        raise ValueError(f"{what} must be [{n}, {width}] with contiguous rows")
+    return t.data_ptr(), (t.stride(0) if n > 1 else width + (-width) % 4)
+
+
+def _same_device(cache, batch=None):
+    import torch
+    if torch.cuda.current_device() != cache.device or (batch is not None and batch.device != cache.device):
+        raise ValueError("the cache and the batch must be on the current CUDA device")
+
+
+def paged_attention_workspace(cache, batch, n_head: int):
+    """A zero-filled workspace for paged_attention of this batch's bounds (and of any smaller ones)."""
+    import torch
+    _same_device(cache, batch)
+    nb = int(lib().hesa_cuda_paged_attention_workspace_size(cache.ref, batch.ref, n_head))
+    if nb == 0:
+        raise HesaError(6, lib().hesa_cuda_last_error().decode())
+    return torch.zeros(nb, dtype=torch.uint8, device="cuda")
+
+
+def paged_attention(cache, layer: int, batch, q, n_head: int, out=None, scale: float | None = None, softcap: float = 0.0,
+                    window: int = 0, slopes=None, prefix=None, workspace=None, stream=None):
+    """Attention of the batch's new tokens, q [n_tokens, n_head * head_dim] fp32,
+    over layer `layer` of the cache (hesa_cuda_paged_attention); returns out."""
+    import torch
+    _same_device(cache, batch)
+    dev, n, width = cache.device, batch.n_tokens, n_head * cache.head_dim
+    qp, ldq = _rows(q, n, width, "q", dev)
+    if scale is not None and not scale > 0:
+        raise ValueError("scale must be positive")
+    opts = None
+    if scale is not None or softcap or window or slopes is not None or prefix is not None:
+        if slopes is not None:
+            _want(slopes, torch.float32, "slopes", dev, 1)
+            if slopes.numel() != n_head or not slopes.is_contiguous():
+                raise ValueError("slopes must hold n_head contiguous values")
+        if prefix is not None:
+            _ints(prefix, "prefix", batch.n_seq, dev)
+        opts = AttnOptionsStruct(scale or 0.0, softcap, window, _ptr(slopes), _ptr(prefix))
+    if out is None:
+        out = _new(lambda: torch.zeros((n, width), dtype=torch.float32, device="cuda"), stream)
+    op, ldo = _rows(out, n, width, "out", dev)
+    if workspace is None:
+        workspace = _new(lambda: paged_attention_workspace(cache, batch, n_head), stream)
+    else:
+        _want(workspace, torch.uint8, "workspace", dev)
+    _check(lib().hesa_cuda_paged_attention(cache.ref, layer, batch.ref, qp, ldq, op, ldo, n_head,
+                                           None if opts is None else ctypes.byref(opts), workspace.data_ptr(),
+                                           workspace.numel(), _stream_handle(stream)))
+    return out
+
+
+def rope_kv_paged(cache, layer: int, batch, q, k, v, n_head: int, rope_table=None, stream=None) -> None:
+    """The batch's new k, v [n_tokens, n_kv_head * head_dim] into layer `layer` of
+    the cache; with rope_table (a device copy of rope_table()) q is rotated in
+    place and k before it is stored (hesa_cuda_rope_kv_paged). q may be None
+    without a table."""
+    import torch
+    _same_device(cache, batch)
+    dev, n, width = cache.device, batch.n_tokens, cache.n_kv_head * cache.head_dim
+    qp, ldq = (None, 0) if q is None else _rows(q, n, n_head * cache.head_dim, "q", dev)
+    kp, ldk = _rows(k, n, width, "k", dev)
+    vp, ldv = _rows(v, n, width, "v", dev)
+    if rope_table is not None:
+        _want(rope_table, torch.float32, "rope_table", dev, 2)
+        if rope_table.shape[1] != cache.head_dim or not rope_table.is_contiguous():
+            raise ValueError("rope_table must be [rows, head_dim] and contiguous")
+    _check(lib().hesa_cuda_rope_kv_paged(cache.ref, layer, batch.ref, qp, ldq, kp, ldk, vp, ldv, n_head, _ptr(rope_table),
+                                         0 if rope_table is None else rope_table.shape[0], _stream_handle(stream)))
+
+
+def kv_pages_workspace(cache):
+    """Scratch for the page operations on this cache."""
+    import torch
+    _same_device(cache)
+    nb = int(lib().hesa_cuda_kv_pages_workspace_size(cache.ref))
+    if nb == 0:
+        raise HesaError(6, lib().hesa_cuda_last_error().decode() or "page operations take at most 2^20 pages")
+    return torch.empty(nb, dtype=torch.uint8, device="cuda")
+
+
+def _page_workspace(cache, workspace, stream):
+    import torch
+    _same_device(cache)
+    if workspace is None:
+        if cache.workspace is None:
+            cache.workspace = kv_pages_workspace(cache)
+        workspace = cache.workspace
+        if stream is not None and not isinstance(stream, int):
+            workspace.record_stream(stream)
+    else:
+        _want(workspace, torch.uint8, "workspace", cache.device)
+    return workspace
+
+
+def kv_reserve(cache, slots, n_new, workspace=None, stream=None) -> None:
+    """n_new[i] more tokens, and the pages for them, for slot slots[i] (hesa_cuda_kv_reserve)."""
+    ws = _page_workspace(cache, workspace, stream)
+    n = slots.numel()
+    _check(lib().hesa_cuda_kv_reserve(cache.ref, _ints(slots, "slots", n, cache.device), _ints(n_new, "n_new", n, cache.device), n,
+                                      ws.data_ptr(), ws.numel(), _stream_handle(stream)))
+
+
+def kv_free(cache, slots, workspace=None, stream=None) -> None:
+    """Give back the pages of these slots and empty them (hesa_cuda_kv_free)."""
+    ws = _page_workspace(cache, workspace, stream)
+    n = slots.numel()
+    _check(lib().hesa_cuda_kv_free(cache.ref, _ints(slots, "slots", n, cache.device), n, ws.data_ptr(), ws.numel(),
+                                   _stream_handle(stream)))
+
+
+def kv_fork(cache, src, dst, workspace=None, stream=None) -> None:
+    """The empty slots dst become copies of the slots src, sharing full pages (hesa_cuda_kv_fork)."""
+    ws = _page_workspace(cache, workspace, stream)
+    n = src.numel()
+    _check(lib().hesa_cuda_kv_fork(cache.ref, _ints(src, "src", n, cache.device), _ints(dst, "dst", n, cache.device), n,
+                                   ws.data_ptr(), ws.numel(), _stream_handle(stream)))
+
+
+def kv_compact(cache, n_live=None, workspace=None, stream=None) -> None:
+    """Move the pages in use to the front of the pool (hesa_cuda_kv_compact); n_live: int32 [1] for their count."""
+    ws = _page_workspace(cache, workspace, stream)
+    p = None if n_live is None else _ints(n_live, "n_live", 1, cache.device)
+    _check(lib().hesa_cuda_kv_compact(cache.ref, p, ws.data_ptr(), ws.numel(), _stream_handle(stream)))
+
+
+def kv_copy_pages(cache, src_pages, dst_pages, workspace=None, stream=None) -> None:
+    """Page dst_pages[i] becomes a copy of page src_pages[i] in every layer (hesa_cuda_kv_copy_pages)."""
+    ws = _page_workspace(cache, workspace, stream)
+    n = src_pages.numel()
+    _check(lib().hesa_cuda_kv_copy_pages(cache.ref, _ints(src_pages, "src_pages", n, cache.device),
+                                         _ints(dst_pages, "dst_pages", n, cache.device), n, ws.data_ptr(), ws.numel(),
+                                         _stream_handle(stream)))
+
+
+def token_logprobs_workspace(n_rows: int, vocab: int, top_k: int = 0):
+    """A zero-filled workspace for token_logprobs."""
+    import torch
+    nb = int(lib().hesa_cuda_token_logprobs_workspace_size(n_rows, vocab, top_k))
+    return torch.zeros(max(nb, 16), dtype=torch.uint8, device="cuda")
+
+
+def token_logprobs(logits, tokens=None, top_k: int = 0, workspace=None, stream=None):
+    """From logits [n_rows, vocab] fp32 (any row stride): the log probability of
+    each row's token (tokens [n_rows] int32; None: none), the row's entropy, and
+    the top_k most probable ids with their log probabilities
+    (hesa_cuda_token_logprobs). Returns (logprob or None, entropy, top_ids,
+    top_logprobs), the last two [n_rows, top_k]."""
+    import torch
+    _want(logits, torch.float32, "logits", dims=2)
+    n, vocab = logits.shape
+    if vocab > 1 and logits.stride(1) != 1:
+        raise ValueError("rows of logits must be contiguous")
+    dev = logits.device.index
+    tp = None if tokens is None else _ints(tokens, "tokens", n, dev)
+
+    def outputs():
+        f = torch.empty((2 + top_k, n), dtype=torch.float32, device="cuda")
+        return f[0], f[1], torch.empty((n, top_k), dtype=torch.int32, device="cuda"), f[2:].view(n, top_k)
+    logprob, entropy, ids, top = _new(outputs, stream)
+    if workspace is None:
+        workspace = _new(lambda: token_logprobs_workspace(n, vocab, top_k), stream)
+    else:
+        _want(workspace, torch.uint8, "workspace", dev)
+    _check(lib().hesa_cuda_token_logprobs(logits.data_ptr(), logits.stride(0) if n > 1 else vocab, n, vocab, tp, top_k,
+                                          None if tokens is None else logprob.data_ptr(), entropy.data_ptr(),
+                                          ids.data_ptr() if top_k else None, top.data_ptr() if top_k else None,
+                                          workspace.data_ptr(), workspace.numel(), _stream_handle(stream)))
+    return (None if tokens is None else logprob), entropy, ids, top

@@ -315,12 +315,162 @@ HESA_CUDA_API int hesa_cuda_decode_step_sharded(const hesa_cuda_model* model, co
                                                 const float* x_embed, const int32_t* pos_dev, float* logits,
                                                 void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------
+ * Paged KV cache: several sequences, chunks of new tokens, shared pages.
+ * The reference's design has one ring for one sequence
+ * (docs/architecture.md:287-338; hesa_cuda_kv_store, hesa_cuda_attention);
+ * no counterpart of pages in it.
+ * ------------------------------------------------------------------- */
+
+/* A cache: fp16 pools of pages for K and for V, and the tables of the slots
+ * that sequences live in. Element e of kv head h of the token in place s of
+ * page p of layer i is k[i * layer_stride + p * page_stride +
+ * (s * n_kv_head + h) * head_dim + e] (v the same); both strides count
+ * elements and are multiples of 8, layers and pages do not overlap, in
+ * either order of nesting. Token j of a slot lies in place j % page_size of
+ * page table[slot * max_pages + j / page_size]. page_refs[p] counts the slots
+ * that page p belongs to, 0: free. head_dim 64, 128 or 256; pools 16-byte
+ * aligned; at most 65536 slots, 2^20 pages and 2^30 tokens a slot. The struct
+ * is host memory; every pointer in it is a device pointer. page_refs may be
+ * NULL where no page operation is called. A new cache has seq_len and
+ * page_refs zero; table need not be set. */
+typedef struct {
+    void* k;
+    void* v;
+    int64_t page_stride, layer_stride;
+    int32_t n_layer, n_pages, page_size, n_kv_head, head_dim;
+    int32_t* table;      /* [n_slots, max_pages] */
+    int32_t* seq_len;    /* [n_slots] */
+    int32_t* page_refs;  /* [n_pages] */
+    int32_t n_slots, max_pages;
+} hesa_cuda_paged_kv;
+
+/* New tokens of n_seq sequences. Rows [q_start[i], q_start[i + 1]) of q, k, v
+ * and the output are sequence i's, the last ones of its slot's seq_len tokens
+ * (hesa_cuda_kv_reserve has counted them): row q_start[i] + t has position
+ * seq_len - (q_start[i + 1] - q_start[i]) + t. A sequence may have no new
+ * token; rows from q_start[n_seq] on are left as they are. The numbers are
+ * read on the device, so that a captured graph serves every step; the host
+ * gives their bounds: rows in all (n_tokens, the rows of the buffers), most
+ * new tokens (max_new) and most tokens (max_len) of a sequence. A sequence
+ * that exceeds a bound, or whose slot or length is not sound, is skipped (its
+ * output stays as it was) and device status 3 recorded; so is a page outside
+ * the pool, which reads as zeros. */
+typedef struct {
+    const int32_t* slots;    /* device [n_seq], or NULL: sequence i is in slot i */
+    const int32_t* q_start;  /* device [n_seq + 1], ascending from 0 */
+    int32_t n_seq, n_tokens, max_new, max_len;
+} hesa_cuda_token_batch;
+
+/* Scores: s = scale * q . k, then softcap * tanh(s / softcap), then minus
+ * slopes[head] * |position - j|. Key j is seen where j <= position and (window
+ * is 0 or j > position - window), and everywhere where j < prefix[i] for
+ * sequence i. Zeroed: the plain causal attention with scale 1/sqrt(head_dim). */
+typedef struct {
+    float scale;             /* 0: 1 / sqrt(head_dim) */
+    float softcap;           /* 0: not capped */
+    int32_t window;          /* 0: no window */
+    const float* slopes;     /* device [n_head] or NULL */
+    const int32_t* prefix;   /* device [n_seq] or NULL */
+} hesa_cuda_attn_options;
+
+/* out[r, h] = sum_j softmax_j(s) v_j over the keys that row r sees, for the
+ * n_head query heads of every row, kv head h / (n_head / n_kv_head): the
+ * attention of hesa_cuda_attention (CPU_Backend's SDPA,
+ * cpu_backend.cpp:225-294) for a chunk of new tokens, or one token of each
+ * sequence, over the pages. q and out are fp32 rows of n_head * head_dim with
+ * row strides ldq, ldo (multiples of 4), 16-byte aligned and not overlapping.
+ * A row that sees no key gives zeros. K and V at places that a row does not
+ * see (padding, other sequences, places past a slot's length) do not reach
+ * it, whatever they hold; a value that is not finite where it is seen gives a
+ * result that is not finite. A row of q that is not finite gives NaN.
+ * The workspace (16-byte aligned, zero-filled once before its first use;
+ * every successful call leaves it usable) can be shared by calls of any shape
+ * on one stream, up to the largest size that the shapes ask for, and not by
+ * calls that may overlap. Results do not depend on what else runs. */
+HESA_CUDA_API size_t hesa_cuda_paged_attention_workspace_size(const hesa_cuda_paged_kv* kv,
+                                                              const hesa_cuda_token_batch* batch, int64_t n_head);
+HESA_CUDA_API int hesa_cuda_paged_attention(const hesa_cuda_paged_kv* kv, int32_t layer,
+                                            const hesa_cuda_token_batch* batch, const float* q, int64_t ldq,
+                                            float* out, int64_t ldo, int64_t n_head,
+                                            const hesa_cuda_attn_options* options, void* workspace,
+                                            size_t workspace_bytes, void* stream);
+
+/* The new tokens' k and v into their pages, rounded to fp16 (nearest even),
+ * and, with a rope table (device copy of hesa_cuda_rope_table with rope_rows
+ * rows; NULL: no rotation, q is not touched), rotate-half rope of q in place
+ * and of k before it is stored, as hesa_cuda_rope and hesa_cuda_kv_store do for
+ * one token. q [n_tokens, n_head * head_dim], k and v [n_tokens, n_kv_head *
+ * head_dim], fp32 with row strides ldq, ldk, ldv (multiples of 4), 16-byte
+ * aligned: they may be columns of one joined projection. A row whose position
+ * is outside the rope table or whose page is outside the pool is skipped and
+ * device status 3 recorded. A batch names a slot once. */
+HESA_CUDA_API int hesa_cuda_rope_kv_paged(const hesa_cuda_paged_kv* kv, int32_t layer,
+                                          const hesa_cuda_token_batch* batch, float* q, int64_t ldq,
+                                          const float* k, int64_t ldk, const float* v, int64_t ldv, int64_t n_head,
+                                          const float* rope_table, int32_t rope_rows, void* stream);
+
+/* Page operations. Slots, counts and pages are device int32 arrays of n
+ * entries; n is at most n_slots (n_pages for copy_pages). New pages are the
+ * lowest free ones, in the order of the list, so results do not depend on
+ * scheduling. A call is carried out as a whole or not at all: a slot listed
+ * twice or outside the cache, a length or a page that is not sound records
+ * device status 3, and a pool with too few free pages status 5; then nothing
+ * has changed. The workspace (16-byte aligned, need not be set) is scratch
+ * that calls on one stream can share.
+ *   reserve: slot slots[i] gets n_new[i] more tokens and the pages for them.
+ *   free: the slots' pages lose a reference each (0: the page is free again),
+ *     their table entries become -1 and their lengths 0.
+ *   fork: the empty slot dst[i] becomes a copy of slot src[i] (which may be
+ *     named several times, but not as a dst): full pages are shared, and the
+ *     filled places of a last, partly filled page are copied, in all layers,
+ *     into a page of its own, so that both can be written on.
+ *   compact: pages in use become pages 0 .. n_live - 1: free pages below
+ *     n_live, ascending, take the pages in use from n_live on, ascending, in
+ *     all layers, and the tables follow. *n_live (device, or NULL) receives
+ *     the count. Every page with references moves with them, so a reference
+ *     that the caller holds outside the slots' tables goes stale.
+ *   copy_pages: page dst[i] becomes a copy of page src[i], in all layers; no
+ *     page is listed twice in dst, or in both lists. Tables are not touched. */
+HESA_CUDA_API size_t hesa_cuda_kv_pages_workspace_size(const hesa_cuda_paged_kv* kv);
+HESA_CUDA_API int hesa_cuda_kv_reserve(const hesa_cuda_paged_kv* kv, const int32_t* slots, const int32_t* n_new,
+                                       int32_t n, void* workspace, size_t workspace_bytes, void* stream);
+HESA_CUDA_API int hesa_cuda_kv_free(const hesa_cuda_paged_kv* kv, const int32_t* slots, int32_t n, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+HESA_CUDA_API int hesa_cuda_kv_fork(const hesa_cuda_paged_kv* kv, const int32_t* src, const int32_t* dst, int32_t n,
+                                    void* workspace, size_t workspace_bytes, void* stream);
+HESA_CUDA_API int hesa_cuda_kv_compact(const hesa_cuda_paged_kv* kv, int32_t* n_live, void* workspace,
+                                       size_t workspace_bytes, void* stream);
+HESA_CUDA_API int hesa_cuda_kv_copy_pages(const hesa_cuda_paged_kv* kv, const int32_t* src_pages,
+                                          const int32_t* dst_pages, int32_t n, void* workspace,
+                                          size_t workspace_bytes, void* stream);
+
+/* From n_rows rows of fp32 logits (row stride ld, any 4-byte alignment): the
+ * log softmax of each row's token, the entropy -sum p log p of the row in
+ * nats, and the top_k (0 .. 32, at most vocab) largest log probabilities with
+ * their ids, descending, equal logits by the lower id. Beside
+ * hesa_cuda_softmax (cpu_softmax_f32, cpu_backend.cpp:48-70). Outputs: logprob
+ * and entropy [n_rows], top_ids and top_logprobs [n_rows, top_k]; any may be
+ * NULL. A logit of -inf is a token that is ruled out: probability 0, nothing
+ * added to the entropy. A row of nothing else gives -inf, entropy 0 and the
+ * first ids; a row with NaN or +inf gives NaN (ids as if NaN were -inf). Token
+ * -1 asks for nothing and gives 0; another one outside [0, vocab) gives NaN
+ * and device status 3. The workspace is as hesa_cuda_paged_attention's (16-byte
+ * aligned, zero-filled once, shared by calls of any shape on one stream). */
+HESA_CUDA_API size_t hesa_cuda_token_logprobs_workspace_size(int64_t n_rows, int64_t vocab, int32_t top_k);
+HESA_CUDA_API int hesa_cuda_token_logprobs(const float* logits, int64_t ld, int64_t n_rows, int64_t vocab,
+                                           const int32_t* tokens, int32_t top_k, float* logprob, float* entropy,
+                                           int32_t* top_ids, float* top_logprobs, void* workspace,
+                                           size_t workspace_bytes, void* stream);
+
 /* Sticky device-side status of the kernels: 0 while nothing has gone wrong
  * in this process, else the first code recorded: 1 a bulk copy did not land
  * within the bounded wait, 2 a copy was still in flight when the kernel
  * gave up, 3 a device-side position outside the KV cache or the rope table,
  * 4 a peer rank did not reach hesa_cuda_peer_barrier, or did not deliver a
- * word of the sharded decode step, in time.
+ * word of the sharded decode step, in time, 5 too few free pages for a page
+ * operation. Status 3 also stands for a slot, length, page or token of the
+ * paged cache's and the log probabilities' device arrays that is not sound.
  * Reading synchronizes `stream`. hesa_cuda_clear_device_status resets it. */
 HESA_CUDA_API int hesa_cuda_device_status(void* stream, int* status_out);
 
