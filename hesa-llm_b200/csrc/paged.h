@@ -84,10 +84,19 @@ __device__ __forceinline__ void locate_tile(const BatchView& b, int g, int r, in
 
 // Key j is seen from position p: j < len and ((j <= p and (no window, or
 // j > p - window)) or j < prefix).
+struct RowKeys {
+    int32_t lo, hi, prefix;   // [lo, hi) and [0, prefix)
+    __device__ __forceinline__ bool sees(int32_t j) const {
+        return static_cast<uint32_t>(j - lo) < static_cast<uint32_t>(hi - lo) || j < prefix;
+    }
+};
+
 struct Mask {
-    int32_t len, window, prefix;
-    __device__ __forceinline__ bool sees(int32_t p, int32_t j) const {
-        return j < len && ((j <= p && (window == 0 || j > p - window)) || j < prefix);
+    int32_t len, window, prefix;   // prefix <= len
+    __device__ __forceinline__ RowKeys row(int32_t p) const {
+        const int32_t lo = window > 0 && p + 1 > window ? p + 1 - window : 0;
+        const int32_t hi = p + 1 < len ? p + 1 : len;
+        return RowKeys{lo, hi > lo ? hi : lo, prefix};
     }
     // every key of [j0, j1) is seen from every position of [p_lo, p_hi]
     __device__ __forceinline__ bool all(int32_t p_lo, int32_t p_hi, int32_t j0, int32_t j1) const {

@@ -27,6 +27,7 @@
 //   * the keys are split over CTAs in runs of whole blocks; the last CTA of a
 //     (tile, kv head) to arrive adds the parts in split order.
 #include "paged.h"
+#include "paged_tc.h"
 #include "abi_errors.h"
 #include "decode_ops.h"
 #include "qmatvec.h"
@@ -114,6 +115,7 @@ rows_kernel(const __grid_constant__ AttnArgs A) {
     const int32_t p_hi = base + min(r0 + kRowTile - 1, n_rows - 1) / A.group;
     Mask mask{sv.len, A.window, 0};
     if (A.prefix) mask.prefix = max(0, min(A.prefix[seq], sv.len));
+    const RowKeys keys = mask.row(pos);
     const KeyBlocks kb = key_blocks(mask, p_lo, p_hi, kKeyBlock);
     const int n_parts = max(1, (kb.n + A.blocks_per_split - 1) / A.blocks_per_split);
     if (split >= n_parts) return;
@@ -239,7 +241,7 @@ rows_kernel(const __grid_constant__ AttnArgs A) {
         if (!mask.all(p_lo, p_hi, j0, j0 + kKeyBlock)) {
 #pragma unroll
             for (int c = 0; c < 4; ++c)
-                if (!row_ok || !mask.sees(pos, jc + (c >> 1) * 8 + (c & 1))) s[c] = -INFINITY;
+                if (!keys.sees(jc + (c >> 1) * 8 + (c & 1))) s[c] = -INFINITY;
             // A key that some row does not see has P = 0 there, which would make
             // NaN of an infinite or NaN v. Such values (there are none in a sound
             // cache) are added where they are seen and then cleared, so that they
@@ -252,7 +254,7 @@ rows_kernel(const __grid_constant__ AttnArgs A) {
             if (__any_sync(0xffffffffu, odd)) {
                 __half* vb = reinterpret_cast<__half*>(smem + (sv_ - smem_addr(smem)));
                 for (int j = 0; j < kKeyBlock; ++j) {
-                    const bool seen = row_ok && mask.sees(pos, j0 + j);
+                    const bool seen = keys.sees(j0 + j);
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -386,7 +388,8 @@ rows_kernel(const __grid_constant__ AttnArgs A) {
 }
 
 struct Plan {
-    int per_seq, tiles, blocks_per_split, n_split;
+    bool tc;   // chunk_kernel of paged_attention_tc.cu
+    int rows, per_seq, tiles, blocks_per_split, n_split;
 };
 
 // How a call is cut: from the host's bounds alone, so that a captured graph
@@ -394,18 +397,23 @@ struct Plan {
 Plan make_plan(const hesa_cuda_paged_kv* kv, const hesa_cuda_token_batch* b, int64_t n_head) {
     Plan p{};
     const int g = static_cast<int>(n_head / kv->n_kv_head);
-    const int64_t most = (static_cast<int64_t>(b->max_new) * g + kRowTile - 1) / kRowTile;
-    const int64_t bound = tile_bound(b->n_tokens, b->n_seq, g, kRowTile);
+    const int64_t rows_a_seq = static_cast<int64_t>(b->max_new) * g;
+    p.tc = kv->head_dim <= 128 && rows_a_seq > 4 * kRowTile;
+    p.rows = p.tc ? kTcRows : kRowTile;
+    const int key_block = p.tc ? kTcKeys : kKeyBlock;
+    const int64_t most = (rows_a_seq + p.rows - 1) / p.rows;
+    const int64_t bound = tile_bound(b->n_tokens, b->n_seq, g, p.rows);
     p.per_seq = b->n_seq * most <= bound ? static_cast<int>(most) : 0;
     const int64_t tiles = p.per_seq ? b->n_seq * most : bound;
     p.tiles = static_cast<int>(tiles);
     const int64_t pairs = tiles * kv->n_kv_head;
-    const int64_t blocks = std::max<int64_t>(1, (b->max_len + kKeyBlock - 1) / kKeyBlock);
-    // about four CTAs an SM where there are keys enough, no split under 128 keys
+    const int64_t blocks = std::max<int64_t>(1, (b->max_len + key_block - 1) / key_block);
+    // rows_kernel: about four CTAs an SM where there are keys enough, no split under 128 keys;
+    // chunk_kernel: one CTA an SM, no split under 512 keys
     int64_t per = blocks;
     if (pairs <= kPagedPairs) {
-        const int64_t want = std::max<int64_t>(1, 148 * 4 / pairs);
-        per = std::max<int64_t>(8, (blocks + want - 1) / want);
+        const int64_t want = std::max<int64_t>(1, 148 * (p.tc ? 1 : 4) / pairs);
+        per = std::max<int64_t>(p.tc ? 4 : 8, (blocks + want - 1) / want);
     }
     p.blocks_per_split = static_cast<int>(std::min(per, blocks));
     p.n_split = static_cast<int>((blocks + p.blocks_per_split - 1) / p.blocks_per_split);
@@ -497,7 +505,7 @@ size_t hesa_cuda_paged_attention_workspace_size(const hesa_cuda_paged_kv* kv, co
     const Plan p = make_plan(kv, batch, n_head);
     size_t n = kPagedCounterBytes;
     if (p.n_split > 1)
-        n += static_cast<size_t>(p.tiles) * kv->n_kv_head * p.n_split * kRowTile * (kv->head_dim + 2) * sizeof(float);
+        n += static_cast<size_t>(p.tiles) * kv->n_kv_head * p.n_split * p.rows * (kv->head_dim + 2) * sizeof(float);
     return n;
 }
 
@@ -548,7 +556,9 @@ int hesa_cuda_paged_attention(const hesa_cuda_paged_kv* kv, int32_t layer, const
     a.n_split = p.n_split;
     cudaError_t e = status_word(&a.status);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (e == cudaSuccess) {
+    if (e == cudaSuccess && p.tc) {
+        e = paged_attention_tc(a, p.tiles, s);
+    } else if (e == cudaSuccess) {
         switch (kv->head_dim) {
             case 64: e = launch_rows<64>(a, p, s); break;
             case 128: e = launch_rows<128>(a, p, s); break;

@@ -1,0 +1,609 @@
+// paged_attention_tc.cu -- paged attention of chunks on the 5th-generation
+// tensor cores (tcgen05, TMEM): tiles of 128 rows (query heads of one kv head
+// times new tokens) over blocks of 128 keys.
+//
+// The formulas and the split of q and P into two fp16 halves are those of
+// paged_attention.cu. Here the halves are two products each: S = Q_lo K^T +
+// Q_hi K^T and O = P_hi V + P_lo V, four 128 x 128 x head_dim products a block
+// of keys, so the floor is twice that of fp16 attention's matrix work. It is
+// bound by the tensor cores.
+//
+// TMEM (512 columns): Q_hi | Q_lo (head_dim columns), two S buffers of 128
+// columns, O (head_dim columns). Q as a TMEM operand leaves all of shared memory
+// to a ring of K and V blocks and halves the operand reads of Q K^T. A buffer's
+// S is overwritten by its P where it lies: columns 64 h .. 64 h + 31 hold the
+// high halves of keys 64 h .. 64 h + 63, the next 32 columns the low halves.
+//
+// Warps 0-7 (compute): thread (row, h) has keys 64 h .. 64 h + 63 of its row's
+// scores, and dims h * head_dim / 2 .. of its output. It takes the maximum (the
+// two threads of a row exchange theirs through shared memory), makes P, and
+// then adds the previous block's O from TMEM to its fp32 registers, rescaling
+// with one fma. O is a fresh product for every block: only 16 products are
+// summed by the tensor core, and long sums round to nearest in fp32.
+// Warp 8 (one thread) issues the products. S buffer j & 1 is written for block
+// j + 2 in two halves of 64 keys, each as soon as the half of P V of block j
+// that read the same columns has completed, while the other half runs: no pair
+// of products relies on an order that the instruction set does not promise, and
+// the tensor core always has one queued.
+// Warps 9, 10 (producers): cp.async of K and V rows into the 128-byte swizzled
+// layout, page by page whatever the page size. Each thread waits for its own
+// copies, makes them visible to the async proxy and its warp arrives.
+#include "paged.h"
+#include "paged_tc.h"
+#include "qmatvec.h"
+
+#include <cuda/atomic>
+
+namespace hesa_cuda {
+namespace {
+
+constexpr int kM = kTcRows;                  // rows of a tile = TMEM lanes
+constexpr int kN = kTcKeys;                  // keys of a block
+constexpr int kComputeWarps = 8;
+constexpr int kMmaWarp = kComputeWarps;
+constexpr int kProducerWarps = 2;
+constexpr int kThreads = 384;                // three warpgroups; warp 11 is idle
+// Registers a thread after setmaxnreg: 256 x 208 + 128 x 88 = 384 x 168, what
+// the block is launched with.
+constexpr int kComputeRegs = 208, kOtherRegs = 88;
+constexpr int kInFlight = 3;                 // blocks that a producer has in flight
+
+template <int HD> struct TcShape {
+    static constexpr uint32_t slot = kN * HD * 2;            // one K or V block
+    static constexpr int slots = HD == 128 ? 6 : 8;
+    static constexpr uint32_t smem = slot * slots + 1024;    // + alignment of the swizzle
+    static constexpr uint32_t q_hi = 0, q_lo = HD / 2, s0 = HD, o = HD + 2 * kN;
+    static_assert(o + HD <= 512, "TMEM columns");
+};
+
+// ---- tcgen05 ----
+// D (+)= A B, A from TMEM, B from shared memory, fp16 in, fp32 out.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
+        "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate ? 1 : 0), "r"(0)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 16 / 32 consecutive columns of this warp's 32 lanes, one lane a thread
+__device__ __forceinline__ void st16(uint32_t t, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(t),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void ld32(uint32_t t, float* v) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(t));
+}
+// wait for this thread's tcgen05.ld; the registers are redefined after it so
+// that no use is scheduled before the wait
+template <int N>
+__device__ __forceinline__ void wait_ld(float* v) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+f"(v[i]));
+}
+
+// Shared-memory descriptors of 128-byte swizzled blocks: 64 fp16 (128 bytes) a
+// row, 8-row groups of 1024 bytes. K-major (K): the group stride is the second
+// offset, the first is not used. MN-major (V: a row is a key, its 64 values run
+// along N): the first offset is the stride to the next 64 of N, the second that
+// to the next 8 keys.
+__device__ __forceinline__ uint64_t desc(uint32_t saddr, uint32_t first, uint32_t second) {
+    return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (static_cast<uint64_t>((first >> 4) & 0x3FFFu) << 16) |
+           (static_cast<uint64_t>((second >> 4) & 0x3FFFu) << 32) | (1ull << 46) | (2ull << 61);
+}
+// fp32 accumulator, fp16 operands, M = 128; bit 16: B is MN-major
+constexpr uint32_t idesc_f16(int n, bool b_mn) {
+    return (1u << 4) | (b_mn ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kM >> 4) << 24);
+}
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool have) {
+    const int n = have ? 16 : 0;   // 0: sixteen zero bytes, src is not read
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+
+// Places in the ring: K0, K1, V0, K2, V1, ... , the order in which they are used.
+__device__ __forceinline__ int k_place(int j) { return j == 0 ? 0 : 2 * j - 1; }
+__device__ __forceinline__ int v_place(int j, int n) { return j + 1 < n ? 2 * j + 2 : 2 * n - 1; }
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 1)
+chunk_kernel(const __grid_constant__ AttnArgs A) {
+    using S = TcShape<HD>;
+    constexpr int HH = HD / 2;   // output dims of a thread
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t full[S::slots], empty[S::slots], s_full[2][2], p_full[2][2], pv_half, o_full, o_free;
+    __shared__ float s_max[2][2][kM];
+    __shared__ uint32_t tmem_base;
+    __shared__ int abort_flag, odd_block[2], s_last;
+
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int kvh = blockIdx.y, split = blockIdx.z;
+    int seq, tile;
+    locate_tile(A.b, A.group, kM, A.per_seq, static_cast<int>(blockIdx.x), seq, tile);
+    const SeqView sv = seq_view(A.c, A.b, seq);
+    if (!sv.ok) {
+        if (threadIdx.x == 0) record_status(A.status, kStatusBadPosition);
+        return;
+    }
+    const int n_rows = sv.n_new * A.group;
+    if (tile * kM >= n_rows) return;
+    // later rows see more keys: the longest tiles of a sequence start first
+    const int r0 = ((n_rows + kM - 1) / kM - 1 - tile) * kM;
+    const int base = sv.len - sv.n_new;
+    const int32_t p_lo = base + r0 / A.group;
+    const int32_t p_hi = base + min(r0 + kM - 1, n_rows - 1) / A.group;
+    Mask mask{sv.len, A.window, 0};
+    if (A.prefix) mask.prefix = max(0, min(A.prefix[seq], sv.len));
+    const KeyBlocks kb = key_blocks(mask, p_lo, p_hi, kN);
+    const int n_parts = max(1, (kb.n + A.blocks_per_split - 1) / A.blocks_per_split);
+    if (split >= n_parts) return;
+    const int i0 = split * A.blocks_per_split;
+    const int n = min(kb.n, i0 + A.blocks_per_split) - i0;   // blocks of this CTA; 0: the rows see nothing
+
+    const uint32_t ring = (smem_addr(smem_raw) + 1023u) & ~1023u;
+    uint8_t* ring_ptr = smem_raw + (ring - smem_addr(smem_raw));
+    volatile int* abort_v = &abort_flag;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::slots; ++i) {
+            mbar_init(&full[i], kProducerWarps);
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i)
+            for (int h = 0; h < 2; ++h) {
+                mbar_init(&s_full[i][h], 1);
+                mbar_init(&p_full[i][h], kComputeWarps / 2);
+            }
+        mbar_init(&pv_half, 1);
+        mbar_init(&o_full, 1);
+        mbar_init(&o_free, kComputeWarps);
+        abort_flag = 0;
+        odd_block[0] = odd_block[1] = -1;
+        fence_mbar_init();
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = tmem_base;
+
+    // ---- compute warps: q into TMEM ----
+    const int half = warp >> 2, wq = warp & 3;
+    const int row = 32 * wq + lane;                       // of the tile, = TMEM lane
+    const uint32_t tl = tmem + (static_cast<uint32_t>(32 * wq) << 16);
+    const int r = min(r0 + row, n_rows - 1);
+    const int t = r / A.group, h = kvh * A.group + r - t * A.group;
+    const int32_t pos = base + t;
+    float sc = 0.f;
+    if (warp < kComputeWarps) {
+        const float4* q = reinterpret_cast<const float4*>(A.q + static_cast<int64_t>(sv.q0 + t) * A.ldq + static_cast<int64_t>(h) * HD);
+        float mx = 0.f;
+#pragma unroll 8
+        for (int i = 0; i < HD / 4; ++i) {
+            const float4 v = q[i];
+            mx = fmax_nan(mx, fmax_nan(fmax_nan(fabsf(v.x), fabsf(v.y)), fmax_nan(fabsf(v.z), fabsf(v.w))));
+        }
+        // q = 2^e (hi + lo) with the largest |hi| in [2^14, 2^15)
+        const bool fin = mx < INFINITY;
+        int e = 0;
+        if (fin && mx > 0.f) e = max(ilogbf(mx) - 14, -120);
+        const float f1 = ldexpf(1.f, -(e / 2)), f2 = fin ? ldexpf(1.f, -(e - e / 2)) : 0.f;
+        sc = fin ? ldexpf(1.f, e) : NAN;
+#pragma unroll
+        for (int c = 0; c < HH / 32; ++c) {   // 32 dims of this thread's half: 16 columns
+            uint32_t hi[16], lo[16];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float4 v = q[half * HH / 4 + c * 8 + i];
+                if (!fin) v = make_float4(0.f, 0.f, 0.f, 0.f);
+                split_half2(v.x * f1 * f2, v.y * f1 * f2, hi[2 * i], lo[2 * i]);
+                split_half2(v.z * f1 * f2, v.w * f1 * f2, hi[2 * i + 1], lo[2 * i + 1]);
+            }
+            st16(tl + S::q_hi + half * HH / 2 + c * 16, hi);
+            st16(tl + S::q_lo + half * HH / 2 + c * 16, lo);
+        }
+        wait_st();
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+
+    if (warp >= kComputeWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (warp > kMmaWarp && warp <= kMmaWarp + kProducerWarps) {
+            // ---- producers: warp w of them copies keys 64 w .. 64 w + 63 of every block ----
+            const int pw = warp - kMmaWarp - 1;
+            constexpr int PIECES = HD / 8;          // 16-byte pieces of a row
+            constexpr int KEYS = kN / kProducerWarps, ROWS = 32 / PIECES;
+            const int32_t* table = A.c.table + static_cast<int64_t>(sv.slot) * A.c.max_pages;
+            const int64_t row_elems = static_cast<int64_t>(A.c.n_kv) * HD;
+            const int at = lane % PIECES, psz = A.c.page_size;
+            const uint32_t to = ring + static_cast<uint32_t>(at >> 3) * (kN * 128) + static_cast<uint32_t>(pw) * KEYS * 128;
+            bool dead = false;
+            // lane's keys lane, lane + 32 of block j: their pages, asked for one block ahead
+            int32_t pg[2];
+            auto ask = [&](int j) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int32_t key = j < n ? kb.at(i0 + j) * kN + pw * KEYS + u * 32 + lane : sv.len;
+                    pg[u] = key < sv.len ? table[key / psz] : -1;
+                }
+            };
+            // and where their rows lie; -1: nowhere, zeros are put there
+            auto find = [&](int j, int64_t (&off)[2]) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int32_t key = kb.at(i0 + j) * kN + pw * KEYS + u * 32 + lane;
+                    off[u] = -1;
+                    if (key < sv.len) {
+                        if (pg[u] >= 0 && pg[u] < A.c.n_pages) off[u] = pg[u] * A.c.page_stride + (key % psz) * row_elems + kvh * HD;
+                        else record_status(A.status, kStatusBadPosition);
+                    }
+                }
+            };
+            auto arrive = [&](int place) {   // this thread's copies into it have landed
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full[place % S::slots]);
+            };
+            auto put = [&](int place, const __half* pool, const int64_t (&off)[2]) {
+                const int slot = place % S::slots;
+                if (place >= S::slots && !dead)
+                    dead = !mbar_wait_bounded(&empty[slot], static_cast<uint32_t>(place / S::slots - 1) & 1u, A.status, kStatusWaitTimeout);
+                dead = __any_sync(0xffffffffu, dead);
+                if (!dead) {
+                    const uint32_t dst = to + static_cast<uint32_t>(slot) * S::slot;
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll 8
+                        for (int i = 0; i < 32; i += ROWS) {
+                            const int kr = i + lane / PIECES;   // of the 32 keys
+                            const int64_t o = __shfl_sync(0xffffffffu, off[u], kr);
+                            cp16(dst + (u * 32 + kr) * 128 + ((static_cast<uint32_t>(at & 7) ^ (kr & 7)) << 4), pool + (o < 0 ? 0 : o) + at * 8, o >= 0);
+                        }
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                if (place >= kInFlight) {
+                    asm volatile("cp.async.wait_group %0;" ::"n"(kInFlight) : "memory");
+                    arrive(place - kInFlight);
+                }
+            };
+            if (n > 0) {
+                int64_t cur[2], nxt[2];
+                ask(0);
+                find(0, cur);
+                ask(1);
+                put(0, A.c.k, cur);
+                for (int j = 0; j < n; ++j) {
+                    if (j + 1 < n) {
+                        find(j + 1, nxt);
+                        ask(j + 2);
+                        put(k_place(j + 1), A.c.k, nxt);
+                    }
+                    put(v_place(j, n), A.c.v, cur);
+                    cur[0] = nxt[0];
+                    cur[1] = nxt[1];
+                }
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                for (int p = max(0, 2 * n - kInFlight); p < 2 * n; ++p) arrive(p);
+            }
+        } else if (warp == kMmaWarp) {
+            // ---- products ----
+            if (lane == 0) {
+                constexpr uint32_t IQK = idesc_f16(kN / 2, false), IPV = idesc_f16(HD, true);
+                auto place = [&](int p) { return ring + static_cast<uint32_t>(p % S::slots) * S::slot; };
+                auto landed = [&](int p) { return mbar_wait_bounded(&full[p % S::slots], static_cast<uint32_t>(p / S::slots) & 1u, A.status, kStatusWaitTimeout); };
+                // the address field of a descriptor counts 16 bytes: k-steps are added to it
+                auto qk = [&](int j, int hf) {
+                    const uint32_t d = tmem + S::s0 + static_cast<uint32_t>((j & 1) * kN + hf * (kN / 2));
+                    const uint64_t b = desc(place(k_place(j)) + static_cast<uint32_t>(hf) * (kN / 2) * 128, 16, 1024);
+#pragma unroll 1
+                    for (int part = 0; part < 2; ++part) {   // the small products first
+                        const uint32_t a = tmem + (part == 0 ? S::q_lo : S::q_hi);
+#pragma unroll
+                        for (int k = 0; k < HD / 16; ++k) mma_ts(d, a + 8 * k, b + ((k >> 2) * (kN * 128) + (k & 3) * 32) / 16, IQK, part > 0 || k > 0);
+                    }
+                    commit(&s_full[j & 1][hf]);
+                };
+                auto pv = [&](int j, int hf) {
+                    const uint32_t p = tmem + S::s0 + static_cast<uint32_t>((j & 1) * kN + hf * (kN / 2));
+                    const uint64_t b = desc(place(v_place(j, n)) + static_cast<uint32_t>(hf) * (kN / 2) * 128, kN * 128, 1024);
+#pragma unroll 1
+                    for (int part = 0; part < 2; ++part) {
+                        const uint32_t a = p + (part == 0 ? 32 : 0);
+#pragma unroll
+                        for (int k = 0; k < kN / 32; ++k) mma_ts(tmem + S::o, a + 8 * k, b + k * 128, IPV, hf > 0 || part > 0 || k > 0);
+                    }
+                };
+                bool ok = true;
+                for (int j = 0; j < 2 && j < n && ok; ++j) {
+                    ok = landed(k_place(j));
+                    if (!ok) break;
+                    fence_after();
+                    qk(j, 0);
+                    qk(j, 1);
+                    commit(&empty[k_place(j) % S::slots]);
+                }
+                for (int j = 0; j < n && ok && !*abort_v; ++j) {
+                    const uint32_t ph = static_cast<uint32_t>(j >> 1) & 1u, each = static_cast<uint32_t>(j) & 1u;
+                    ok = landed(v_place(j, n)) && (j == 0 || mbar_wait_bounded(&o_free, each ^ 1u, A.status, kStatusWaitTimeout)) &&
+                         mbar_wait_bounded(&p_full[j & 1][0], ph, A.status, kStatusWaitTimeout);
+                    if (!ok) break;
+                    fence_after();
+                    pv(j, 0);
+                    commit(&pv_half);
+                    ok = mbar_wait_bounded(&p_full[j & 1][1], ph, A.status, kStatusWaitTimeout);
+                    if (!ok) break;
+                    fence_after();
+                    pv(j, 1);
+                    commit(&empty[v_place(j, n) % S::slots]);
+                    commit(&o_full);
+                    if (j + 2 < n) {
+                        // S half 0 of block j + 2 goes where P half 0 of block j has been read, while half 1 is
+                        ok = landed(k_place(j + 2)) && mbar_wait_bounded(&pv_half, each, A.status, kStatusWaitTimeout);
+                        if (!ok) break;
+                        fence_after();
+                        qk(j + 2, 0);
+                        ok = mbar_wait_bounded(&o_full, each, A.status, kStatusWaitTimeout);
+                        if (!ok) break;
+                        qk(j + 2, 1);
+                        commit(&empty[k_place(j + 2) % S::slots]);
+                    }
+                }
+                if (!ok) *abort_v = 1;
+            }
+            __syncwarp();
+        }
+    } else {
+        // ---- compute ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kComputeRegs));
+        if (A.cap2 == 0.f) sc *= A.scale2;
+        const float slope2 = A.slopes ? A.slopes[h] * 1.44269504088896341f : 0.f;
+        const bool plain = A.cap2 == 0.f && !A.slopes;
+        float m = -INFINITY, l = 0.f, alpha = 0.f;
+        float acc[HH];
+#pragma unroll
+        for (int i = 0; i < HH; ++i) acc[i] = 0.f;
+        bool ok = true;   // a wait that ran out is waited for no more; the loop goes on to its end
+        const RowKeys keys = mask.row(pos);
+
+        // acc = acc * alpha + O of block j
+        auto take = [&](int j) {
+            ok = ok && mbar_wait_bounded(&o_full, static_cast<uint32_t>(j) & 1u, A.status, kStatusWaitTimeout);
+            __syncwarp();
+            fence_after();
+#pragma unroll
+            for (int c = 0; c < HH / 32; ++c) {
+                float o[32];
+                ld32(tl + S::o + half * HH + c * 32, o);
+                wait_ld<32>(o);
+                if (c == HH / 32 - 1) {
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&o_free);
+                }
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    const float2 x = ffma2(make_float2(acc[c * 32 + i], acc[c * 32 + i + 1]), make_float2(alpha, alpha), make_float2(o[i], o[i + 1]));
+                    acc[c * 32 + i] = x.x;
+                    acc[c * 32 + i + 1] = x.y;
+                }
+            }
+        };
+
+        for (int j = 0; j < n; ++j) {
+            const int buf = j & 1;
+            const int32_t j0 = kb.at(i0 + j) * kN, jh = j0 + half * (kN / 2);
+            ok = ok && mbar_wait_bounded(&s_full[buf][half], static_cast<uint32_t>(j >> 1) & 1u, A.status, kStatusWaitTimeout);
+            __syncwarp();
+            fence_after();
+            const uint32_t sb = tl + S::s0 + buf * kN + half * (kN / 2);
+            float s[64];
+            ld32(sb, s);
+            ld32(sb + 32, s + 32);
+            wait_ld<64>(s);
+            float k = sc;   // s * k is the score in base 2
+            const bool whole = mask.all(p_lo, p_hi, j0, j0 + kN);
+            if (!plain) {
+                if (A.cap2 != 0.f) {
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) s[i] = capped(s[i] * sc, A.cap2, A.cap_in);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) s[i] *= sc;
+                }
+                if (A.slopes) {
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) s[i] -= slope2 * fabsf(static_cast<float>(pos - (jh + i)));
+                }
+                k = 1.f;
+            }
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < 64; ++i) s[i] = keys.sees(jh + i) ? s[i] * k : -INFINITY;
+                k = 1.f;
+                // values of V that are not finite and hidden from some row: added where they are seen, then
+                // cleared (paged_attention.cu). Keys past the sequence are zeros.
+                const int place = v_place(j, n);
+                uint8_t* vb = ring_ptr + static_cast<size_t>(place % S::slots) * S::slot;
+                ok = ok && mbar_wait_bounded(&full[place % S::slots], static_cast<uint32_t>(place / S::slots) & 1u, A.status, kStatusWaitTimeout);
+                bool odd = false;
+                for (uint32_t c = threadIdx.x * 16; c < S::slot; c += kComputeWarps * 32 * 16) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(vb + c);
+                    odd |= nonfinite_h2(w.x) || nonfinite_h2(w.y) || nonfinite_h2(w.z) || nonfinite_h2(w.w);
+                }
+                // a warp that is a block ahead writes the other word; none is two ahead (S of block j + 2 needs every P of j)
+                if (odd) odd_block[buf] = j;
+                named_barrier(5, kComputeWarps * 32);
+                if (*reinterpret_cast<volatile int*>(&odd_block[buf]) == j) {
+                    for (int kr = 0; kr < kN; ++kr) {
+                        if (!keys.sees(j0 + kr)) continue;
+#pragma unroll
+                        for (int d8 = 0; d8 < HH / 8; ++d8) {
+                            const int d = half * HH + d8 * 8;
+                            const uint4 w = *reinterpret_cast<const uint4*>(vb + (d >> 6) * (kN * 128) + kr * 128 + ((((d >> 3) & 7) ^ (kr & 7)) << 4));
+                            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const float x = half_bits_to_float(ws[i >> 1] >> (16 * (i & 1)));
+                                if (!isfinite(x)) acc[d8 * 8 + i] += x;
+                            }
+                        }
+                    }
+                    named_barrier(5, kComputeWarps * 32);
+                    for (uint32_t c = threadIdx.x * 2; c < S::slot; c += kComputeWarps * 32 * 2) {
+                        unsigned short& x = *reinterpret_cast<unsigned short*>(vb + c);
+                        if ((x & 0x7C00u) == 0x7C00u) x = 0;
+                    }
+                    fence_proxy_async_smem();
+                    named_barrier(5, kComputeWarps * 32);
+                }
+            }
+            float mx = s[0];
+#pragma unroll
+            for (int i = 1; i < 64; ++i) mx = fmaxf(mx, s[i]);
+            s_max[buf][half][row] = mx;
+            named_barrier(1 + wq, 64);   // the two warps of these rows
+            mx = fmaxf(mx, s_max[buf][half ^ 1][row]) * k;
+            // k is NaN for a row that is not finite: so are its maximum, its P and its result
+            mx = mx > m ? mx : (mx == mx ? m : mx);
+            const float ms = mx == -INFINITY ? 0.f : mx;
+            const float al = m == -INFINITY ? 0.f : ex2(m - ms);
+            m = mx;
+            const float off = kPShift - ms;
+            float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t hi[16], lo[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float2 x = ffma2(make_float2(s[c * 32 + 2 * i], s[c * 32 + 2 * i + 1]), make_float2(k, k), make_float2(off, off));
+                    const float2 p = make_float2(ex2(x.x), ex2(x.y));
+                    sum = fadd2(sum, p);
+                    split_half2(p.x, p.y, hi[i], lo[i]);
+                }
+                st16(sb + c * 16, hi);
+                st16(sb + 32 + c * 16, lo);
+            }
+            l = fmaf(l, al, sum.x + sum.y);
+            wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[buf][half]);
+            if (j > 0) take(j - 1);
+            alpha = al;
+        }
+        if (n > 0) take(n - 1);
+        if (!ok) *abort_v = 1;
+
+        // the row's sum over both halves of the keys
+        named_barrier(1 + wq, 64);
+        s_max[0][half][row] = l;
+        named_barrier(1 + wq, 64);
+        l = s_max[0][0][row] + s_max[0][1][row];
+        const int pair = static_cast<int>(blockIdx.x) * A.c.n_kv + kvh;
+        float* parts = A.part + static_cast<int64_t>(pair) * A.n_split * kM * (HD + 2);
+        float* o_row = A.out + static_cast<int64_t>(sv.q0 + t) * A.ldo + static_cast<int64_t>(h) * HD + half * HH;
+        const bool mine = r0 + row < n_rows;
+        if (n_parts == 1) {
+            if (mine && !*abort_v) {
+#pragma unroll
+                for (int i = 0; i < HH; i += 4)
+                    *reinterpret_cast<float4*>(o_row + i) = l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                                                     : make_float4(acc[i] / l, acc[i + 1] / l, acc[i + 2] / l, acc[i + 3] / l);
+            }
+        } else {
+            float* p = parts + (static_cast<int64_t>(split) * kM + row) * (HD + 2);
+            if (half == 0) *reinterpret_cast<float2*>(p) = make_float2(m, l);
+#pragma unroll
+            for (int i = 0; i < HH; i += 2) *reinterpret_cast<float2*>(p + 2 + half * HH + i) = make_float2(acc[i], acc[i + 1]);
+            named_barrier(5, kComputeWarps * 32);
+            if (threadIdx.x == 0) {
+                cuda::atomic_ref<int32_t, cuda::thread_scope_device> c(A.counters[pair]);
+                s_last = c.fetch_add(1, cuda::memory_order_acq_rel) == n_parts - 1;
+            }
+            named_barrier(5, kComputeWarps * 32);
+            if (s_last) {
+                cuda::atomic_thread_fence(cuda::memory_order_acquire, cuda::thread_scope_device);
+                // a warp takes 16 rows, one after another: lanes along the row
+                for (int rr = warp; rr < kM && r0 + rr < n_rows; rr += kComputeWarps) {
+                    const float* p0 = parts + static_cast<int64_t>(rr) * (HD + 2);
+                    constexpr int64_t step = kM * (HD + 2);
+                    float M = -INFINITY;
+                    for (int i = 0; i < n_parts; ++i) M = fmaxf(M, __ldcg(p0 + i * step));
+                    float L = 0.f, O[HD / 32];
+#pragma unroll
+                    for (int d = 0; d < HD / 32; ++d) O[d] = 0.f;
+                    for (int i = 0; i < n_parts; ++i) {
+                        const float mi = __ldcg(p0 + i * step);
+                        // a part that saw nothing adds zeros, or the NaN of a row that is not finite
+                        const float f = mi == -INFINITY ? 1.f : ex2(mi - M);
+                        L = fmaf(__ldcg(p0 + i * step + 1), f, L);
+#pragma unroll
+                        for (int d = 0; d < HD / 32; ++d) O[d] = fmaf(__ldcg(p0 + i * step + 2 + d * 32 + lane), f, O[d]);
+                    }
+                    const int rt = (r0 + rr) / A.group, rh = kvh * A.group + (r0 + rr) - rt * A.group;
+                    float* o = A.out + static_cast<int64_t>(sv.q0 + rt) * A.ldo + static_cast<int64_t>(rh) * HD;
+#pragma unroll
+                    for (int d = 0; d < HD / 32; ++d) o[d * 32 + lane] = L == 0.f ? 0.f : O[d] / L;
+                }
+                if (threadIdx.x == 0) {
+                    cuda::atomic_ref<int32_t, cuda::thread_scope_device> c(A.counters[pair]);
+                    c.store(0, cuda::memory_order_relaxed);
+                }
+            }
+        }
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    }
+}
+
+template <int HD>
+cudaError_t launch(const AttnArgs& a, int tiles, cudaStream_t s) {
+    static bool set[64] = {};   // per instance and device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!set[dev]) {
+        e = cudaFuncSetAttribute(chunk_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(TcShape<HD>::smem));
+        if (e != cudaSuccess) return e;
+        set[dev] = true;
+    }
+    const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(a.c.n_kv), static_cast<unsigned>(a.n_split));
+    chunk_kernel<HD><<<grid, kThreads, TcShape<HD>::smem, s>>>(a);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t paged_attention_tc(const AttnArgs& a, int tiles, cudaStream_t s) {
+    return a.c.head_dim == 64 ? launch<64>(a, tiles, s) : launch<128>(a, tiles, s);
+}
+
+}  // namespace hesa_cuda
