@@ -142,9 +142,10 @@ struct AttnArgs {
     const int32_t* prefix;         // [n_seq] or null
     int* status;
     int32_t* counters;             // [kAttnPairs], left at zero
-    float* part;                   // [pair][split][rows][head_dim + 2]
+    float* part;                   // m, l, acc of rows that are added up later
     int32_t per_seq;               // tiles of every sequence, 0: by q_start
-    int32_t blocks_per_split, n_split;
+    int32_t blocks_per_split;      // chunk_kernel: keys of a split
+    int32_t n_split;               // chunk_kernel: splits; rows_kernel: tiles of a balanced launch, 0: one CTA a tile
 };
 
 // (tile, kv head) pairs that may be split over the keys: one arrival counter
