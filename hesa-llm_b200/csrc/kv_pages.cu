@@ -136,6 +136,8 @@ __device__ __forceinline__ void refuse(const Tables& t, int code) {
 
 __global__ void __launch_bounds__(kPlanThreads)
 free_kernel(const Tables t, const int32_t* __restrict__ slots, int n) {
+    grid_dep_wait();
+    grid_dep_launch();
     __shared__ uint32_t bits[kMaxSlots / 32];
     if (!mark_slots(slots, n, t.n_slots, bits) || !slots_sound(t, slots, n)) return refuse(t, kStatusBadPosition);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -154,6 +156,8 @@ free_kernel(const Tables t, const int32_t* __restrict__ slots, int n) {
 
 __global__ void __launch_bounds__(kPlanThreads)
 reserve_kernel(const Tables t, const int32_t* __restrict__ slots, const int32_t* __restrict__ add, int n, PageWork w) {
+    grid_dep_wait();
+    grid_dep_launch();
     __shared__ uint32_t bits[kMaxSlots / 32];
     __shared__ int s[33];
     if (!mark_slots(slots, n, t.n_slots, bits)) return refuse(t, kStatusBadPosition);
@@ -195,6 +199,8 @@ reserve_kernel(const Tables t, const int32_t* __restrict__ slots, const int32_t*
 
 __global__ void __launch_bounds__(kPlanThreads)
 fork_plan_kernel(const Tables t, const int32_t* __restrict__ src, const int32_t* __restrict__ dst, int n, PageWork w) {
+    grid_dep_wait();
+    grid_dep_launch();
     __shared__ uint32_t bits[kMaxSlots / 32];
     __shared__ int s[33];
     if (threadIdx.x == 0) *w.n_items = 0;
@@ -244,6 +250,8 @@ fork_plan_kernel(const Tables t, const int32_t* __restrict__ src, const int32_t*
 // live pages to the front: free pages below n_live take the pages in use from n_live on
 __global__ void __launch_bounds__(kPlanThreads)
 compact_plan_kernel(const Tables t, PageWork w, int32_t* __restrict__ n_live_out) {
+    grid_dep_wait();
+    grid_dep_launch();
     __shared__ int s[33];
     if (threadIdx.x == 0) *w.n_items = 0;
     // a table entry outside the pool, or of a page that is free, would be lost: nothing is moved then
@@ -290,6 +298,8 @@ compact_plan_kernel(const Tables t, PageWork w, int32_t* __restrict__ n_live_out
 // The listed pairs of pages: in the pool, no page written twice or also read.
 __global__ void __launch_bounds__(kPlanThreads)
 copy_plan_kernel(const Tables t, const int32_t* __restrict__ src, const int32_t* __restrict__ dst, int n, PageWork w) {
+    grid_dep_wait();
+    grid_dep_launch();
     if (threadIdx.x == 0) *w.n_items = 0;
     for (int i = threadIdx.x; i < t.n_pages; i += kPlanThreads) w.map[i] = 0;
     __syncthreads();
@@ -323,6 +333,8 @@ __global__ void __launch_bounds__(256)
 copy_kernel(uint4* __restrict__ k, uint4* __restrict__ v, int64_t page_words, int64_t layer_words, int n_layer,
             int slot_words, const int32_t* __restrict__ n_items, const int32_t* __restrict__ items, const Tables t,
             const int32_t* __restrict__ map) {
+    grid_dep_wait();
+    grid_dep_launch();
     if (map) {
         const int64_t all = static_cast<int64_t>(t.n_slots) * t.max_pages;
         for (int64_t e = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; e < all; e += static_cast<int64_t>(gridDim.x) * blockDim.x) {
@@ -362,6 +374,8 @@ __global__ void __launch_bounds__(256)
 rope_kv_paged_kernel(PagedLayer c, BatchView b, float* __restrict__ q, int64_t ldq, const float* __restrict__ k, int64_t ldk,
                      const float* __restrict__ v, int64_t ldv, int n_head, const float* __restrict__ table, int table_rows,
                      int* __restrict__ status) {
+    grid_dep_wait();
+    grid_dep_launch();
     const int row = blockIdx.x;
     // the last sequence that starts at or before this row and is not empty there
     int lo = 0, hi = b.n_seq - 1;
@@ -459,10 +473,8 @@ cudaError_t launch_copy(const hesa_cuda_paged_kv* kv, const Tables& t, const Pag
     const int slot_words = kv->n_kv_head * kv->head_dim / 8;
     // eight blocks an SM keep enough loads in flight; fewer where fewer pages can move
     const int64_t blocks = std::min<int64_t>(148 * 8, std::max<int64_t>(1, most * kv->n_layer * 2));
-    copy_kernel<<<static_cast<unsigned>(blocks), 256, 0, s>>>(
-        static_cast<uint4*>(kv->k), static_cast<uint4*>(kv->v), kv->page_stride / 8, kv->layer_stride / 8, kv->n_layer,
-        slot_words, w.n_items, w.items, t, map);
-    return cudaGetLastError();
+    return launch_dep(copy_kernel, dim3(static_cast<unsigned>(blocks)), 256, 0, s, static_cast<uint4*>(kv->k), static_cast<uint4*>(kv->v),
+                      kv->page_stride / 8, kv->layer_stride / 8, kv->n_layer, slot_words, w.n_items, w.items, t, map);
 }
 
 }  // namespace
@@ -490,8 +502,7 @@ int hesa_cuda_kv_reserve(const hesa_cuda_paged_kv* kv, const int32_t* slots, con
     if (!slots || !n_new) return record_error(HESA_CUDA_INVALID_ARGUMENT, "null pointer");
     cudaError_t e = status_word(&t.status);
     if (e == cudaSuccess) {
-        reserve_kernel<<<1, kPlanThreads, 0, static_cast<cudaStream_t>(stream)>>>(t, slots, n_new, n, page_work(workspace, kv));
-        e = cudaGetLastError();
+        e = launch_dep(reserve_kernel, dim3(1), kPlanThreads, 0, static_cast<cudaStream_t>(stream), t, slots, n_new, n, page_work(workspace, kv));
     }
     return e == cudaSuccess ? HESA_CUDA_OK : record_cuda_error(e, "kv_reserve kernel");
 }
@@ -507,8 +518,7 @@ int hesa_cuda_kv_free(const hesa_cuda_paged_kv* kv, const int32_t* slots, int32_
     if (!slots) return record_error(HESA_CUDA_INVALID_ARGUMENT, "null pointer");
     cudaError_t e = status_word(&t.status);
     if (e == cudaSuccess) {
-        free_kernel<<<1, kPlanThreads, 0, static_cast<cudaStream_t>(stream)>>>(t, slots, n);
-        e = cudaGetLastError();
+        e = launch_dep(free_kernel, dim3(1), kPlanThreads, 0, static_cast<cudaStream_t>(stream), t, slots, n);
     }
     return e == cudaSuccess ? HESA_CUDA_OK : record_cuda_error(e, "kv_free kernel");
 }
@@ -526,8 +536,7 @@ int hesa_cuda_kv_fork(const hesa_cuda_paged_kv* kv, const int32_t* src, const in
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t e = status_word(&t.status);
     if (e == cudaSuccess) {
-        fork_plan_kernel<<<1, kPlanThreads, 0, s>>>(t, src, dst, n, w);
-        e = cudaGetLastError();
+        e = launch_dep(fork_plan_kernel, dim3(1), kPlanThreads, 0, s, t, src, dst, n, w);
     }
     if (e == cudaSuccess) e = launch_copy(kv, t, w, n, nullptr, s);
     return e == cudaSuccess ? HESA_CUDA_OK : record_cuda_error(e, "kv_fork kernels");
@@ -542,8 +551,7 @@ int hesa_cuda_kv_compact(const hesa_cuda_paged_kv* kv, int32_t* n_live, void* wo
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t e = status_word(&t.status);
     if (e == cudaSuccess) {
-        compact_plan_kernel<<<1, kPlanThreads, 0, s>>>(t, w, n_live);
-        e = cudaGetLastError();
+        e = launch_dep(compact_plan_kernel, dim3(1), kPlanThreads, 0, s, t, w, n_live);
     }
     if (e == cudaSuccess) e = launch_copy(kv, t, w, kv->n_pages / 2, w.map, s);
     return e == cudaSuccess ? HESA_CUDA_OK : record_cuda_error(e, "kv_compact kernels");
@@ -562,8 +570,7 @@ int hesa_cuda_kv_copy_pages(const hesa_cuda_paged_kv* kv, const int32_t* src_pag
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t e = status_word(&t.status);
     if (e == cudaSuccess) {
-        copy_plan_kernel<<<1, kPlanThreads, 0, s>>>(t, src_pages, dst_pages, n, w);
-        e = cudaGetLastError();
+        e = launch_dep(copy_plan_kernel, dim3(1), kPlanThreads, 0, s, t, src_pages, dst_pages, n, w);
     }
     if (e == cudaSuccess) e = launch_copy(kv, t, w, n, nullptr, s);
     return e == cudaSuccess ? HESA_CUDA_OK : record_cuda_error(e, "kv_copy_pages kernels");
@@ -591,9 +598,9 @@ int hesa_cuda_rope_kv_paged(const hesa_cuda_paged_kv* kv, int32_t layer, const h
         const int64_t units = (n_head + 2 * kv->n_kv_head) * (kv->head_dim / 16);
         // one block a token where tokens are many; few tokens are spread over more blocks
         const int64_t y = batch->n_tokens >= 148 * 4 ? 1 : std::min<int64_t>((units + 255) / 256, 1024);
-        rope_kv_paged_kernel<<<dim3(static_cast<unsigned>(batch->n_tokens), static_cast<unsigned>(y)), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-            layer_of(kv, layer), view_of(batch), q, ldq, k, ldk, v, ldv, static_cast<int>(n_head), rope_table, rope_rows, status);
-        e = cudaGetLastError();
+        e = launch_dep(rope_kv_paged_kernel, dim3(static_cast<unsigned>(batch->n_tokens), static_cast<unsigned>(y)), 256, 0,
+                       static_cast<cudaStream_t>(stream), layer_of(kv, layer), view_of(batch), q, ldq, k, ldk, v, ldv,
+                       static_cast<int>(n_head), rope_table, rope_rows, status);
     }
     return e == cudaSuccess ? HESA_CUDA_OK : record_cuda_error(e, "rope_kv_paged kernel");
 }

@@ -182,6 +182,24 @@ __device__ __forceinline__ void split_half2(float x0, float x1, uint32_t& hi, ui
     lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
+// Launch with programmatic stream serialization: the grid may be set up while
+// the previous kernel on the stream finishes. Every such kernel calls
+// grid_dep_wait before it reads or writes anything.
+template <typename... P, typename... T>
+cudaError_t launch_dep(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, T... args) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
 // The host's checks of a cache and a batch (paged_attention.cu): 0, or an error
 // code with its message recorded.
 int check_paged_kv(const hesa_cuda_paged_kv* kv);

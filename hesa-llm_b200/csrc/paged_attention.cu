@@ -398,12 +398,15 @@ __device__ __forceinline__ void rows_segment(const AttnArgs& A, uint8_t* smem, c
     }
 }
 
-// What combine_kernel does for the cut before CTA c's run: the parts of (tile,
-// grp) are `first`, then the first part of each of the next n - 1 CTAs. n = 0:
-// nothing (no cut inside it, or not the first).
+// What combine_kernel adds up: the parts of (tile, grp) are `first`, then the
+// first part of each of the next n - 1 CTAs. n < 2: nothing, it lies in one run.
+// Few (tile, group)s have an entry each; else there is one for each CTA, for
+// the cut before its run (if that is the first one of what it cuts).
 struct __align__(16) Cut {
     int32_t tile, grp, first, n;
 };
+
+__host__ __device__ inline bool by_tile(int tiles, const HeadGroups& hg) { return static_cast<int64_t>(tiles) * hg.groups <= kRowsCtas; }
 
 // A.n_split tiles in equal runs; 0: one CTA for each tile and group, where these are many.
 template <int HD>
@@ -415,6 +418,7 @@ rows_kernel(const __grid_constant__ AttnArgs A) {
     __shared__ int64_t s_sum[W];
     const HeadGroups hg(A.c.n_kv, W);
     const int tiles = A.n_split;
+    grid_dep_wait();
     if (tiles == 0) {
         const int nb = tile_blocks(A, static_cast<int>(blockIdx.x), threadIdx.x == 0);
         if (nb > 0) rows_segment<HD>(A, smem, hg, static_cast<int>(blockIdx.x), static_cast<int>(blockIdx.y), 0, nb, -1);
@@ -447,6 +451,11 @@ rows_kernel(const __grid_constant__ AttnArgs A) {
     Runs runs{before * hg.groups, 1};
     runs.n_cta = static_cast<int>(max(int64_t(1), min(static_cast<int64_t>(gridDim.x), runs.units / kLeastUnits)));
     const int cta = blockIdx.x;
+    const bool listed_by_tile = by_tile(tiles, hg);
+    Cut* cuts = reinterpret_cast<Cut*>(A.part);
+    if (listed_by_tile && cta == 0)   // those without rows
+        for (int i = threadIdx.x; i < tiles * hg.groups; i += W * 32)
+            if (s_pre[i / hg.groups + 1] == s_pre[i / hg.groups]) cuts[i] = Cut{0, 0, 0, 0};
     Cut cut{0, 0, 0, 0};
     if (runs.units > 0 && cta < runs.n_cta) {
         int64_t u = runs.start(cta);
@@ -467,16 +476,18 @@ rows_kernel(const __grid_constant__ AttnArgs A) {
                 const int64_t b0 = max(u, first + kSegCost) - first - kSegCost, b1 = stop - first - kSegCost;
                 const int c_first = runs.cta_of(first + kSegCost), c_last = runs.cta_of(first + n - 1);
                 const int which = begin >= first ? 0 : 1;
-                if (cta == c_first + 1) cut = Cut{lo, grp, 2 * c_first + (runs.start(c_first) >= first ? 0 : 1), c_last - c_first + 1};
+                const Cut all{lo, grp, 2 * c_first + (runs.start(c_first) >= first ? 0 : 1), c_last - c_first + 1};
+                if (cta == c_first + 1) cut = all;
+                if (listed_by_tile && cta == c_first && threadIdx.x == 0) cuts[lo * hg.groups + grp] = all;
                 rows_segment<HD>(A, smem, hg, lo, grp, static_cast<int>(b0), static_cast<int>(b1), c_first == c_last ? -1 : 2 * cta + which);
             }
             u = stop;
         }
     }
-    if (threadIdx.x == 0) reinterpret_cast<Cut*>(A.part)[cta] = cut;
+    if (!listed_by_tile && threadIdx.x == 0) cuts[cta] = cut;
 }
 
-// The parts of one row of what a cut runs through: block (cut, warp's head, row).
+// The parts of one row of what is cut: block (entry, head of the group, row).
 template <int HD>
 __global__ void __launch_bounds__(256)
 combine_kernel(const __grid_constant__ AttnArgs A) {
@@ -485,9 +496,10 @@ combine_kernel(const __grid_constant__ AttnArgs A) {
     __shared__ float s_red[2][8];
     __shared__ float4 s_o[256];
     grid_dep_wait();
-    const int4 c4 = __ldcg(reinterpret_cast<const int4*>(A.part) + blockIdx.x + 1);
+    grid_dep_launch();
+    const int4 c4 = __ldcg(reinterpret_cast<const int4*>(A.part) + blockIdx.x);
     const Cut cut{c4.x, c4.y, c4.z, c4.w};
-    if (cut.n == 0) return;
+    if (cut.n < 2) return;
     const HeadGroups hg(A.c.n_kv, S::warps);
     const int hl = blockIdx.y, row = blockIdx.z, kvh = cut.grp * hg.heads + hl;
     if (hl >= hg.heads || kvh >= A.c.n_kv) return;
@@ -607,24 +619,13 @@ cudaError_t launch_rows(const AttnArgs& a, const Plan& p, cudaStream_t s) {
         set[dev] = true;
     }
     using S = RowsShape<HD>;
-    if (!p.balanced) {
-        const HeadGroups hg(a.c.n_kv, S::warps);
-        rows_kernel<HD><<<dim3(static_cast<unsigned>(p.tiles), static_cast<unsigned>(hg.groups)), S::warps * 32, S::smem, s>>>(a);
-        return cudaGetLastError();
-    }
-    rows_kernel<HD><<<kRowsCtas, S::warps * 32, S::smem, s>>>(a);
-    e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(kRowsCtas - 1, S::warps, kRowTile);
-    cfg.blockDim = dim3(256);
-    cfg.stream = s;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, combine_kernel<HD>, a);
+    const HeadGroups hg(a.c.n_kv, S::warps);
+    const dim3 grid = p.balanced ? dim3(kRowsCtas) : dim3(static_cast<unsigned>(p.tiles), static_cast<unsigned>(hg.groups));
+    e = launch_dep(rows_kernel<HD>, grid, S::warps * 32, S::smem, s, a);
+    if (e != cudaSuccess || !p.balanced) return e;
+    const int cuts = by_tile(a.n_split, hg) ? a.n_split * hg.groups : kRowsCtas;
+    const int rows = std::min(kRowTile, a.b.max_new * a.group);
+    return launch_dep(combine_kernel<HD>, dim3(static_cast<unsigned>(cuts), static_cast<unsigned>(hg.heads), static_cast<unsigned>(rows)), 256, 0, s, a);
 }
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }

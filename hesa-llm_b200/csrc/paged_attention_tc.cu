@@ -136,6 +136,8 @@ chunk_kernel(const __grid_constant__ AttnArgs A) {
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int kvh = blockIdx.y, split = blockIdx.z;
+    grid_dep_wait();
+    grid_dep_launch();
     int seq, tile;
     locate_tile(A.b, A.group, kM, A.per_seq, static_cast<int>(blockIdx.x), seq, tile);
     const SeqView sv = seq_view(A.c, A.b, seq);
@@ -596,8 +598,7 @@ cudaError_t launch(const AttnArgs& a, int tiles, cudaStream_t s) {
         set[dev] = true;
     }
     const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(a.c.n_kv), static_cast<unsigned>(a.n_split));
-    chunk_kernel<HD><<<grid, kThreads, TcShape<HD>::smem, s>>>(a);
-    return cudaGetLastError();
+    return launch_dep(chunk_kernel<HD>, grid, kThreads, TcShape<HD>::smem, s, a);
 }
 
 }  // namespace

@@ -17,7 +17,7 @@
 // parts in split order.
 #include "../../include/hesa_cuda.h"
 #include "abi_errors.h"
-#include "hesa_common.cuh"
+#include "paged.h"
 #include "qmatvec.h"
 #include "trace.h"
 
@@ -144,6 +144,8 @@ token_logprobs_kernel(const float* __restrict__ logits, int64_t ld, int n_rows, 
     __shared__ int s_last;
     __shared__ unsigned s_thr;   // order bits of the largest k-th value that a warp holds
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    grid_dep_wait();
+    grid_dep_launch();
     const int64_t r = blockIdx.x;
     const int split = blockIdx.y;
     const float* row = logits + r * ld;
@@ -335,10 +337,9 @@ int hesa_cuda_token_logprobs(const float* logits, int64_t ld, int64_t n_rows, in
         uint8_t* ws = static_cast<uint8_t*>(workspace);
         LpPart* parts = reinterpret_cast<LpPart*>(ws + kLpCounterBytes);
         uint64_t* keys = reinterpret_cast<uint64_t*>(ws + kLpCounterBytes + static_cast<size_t>(n_rows) * s * sizeof(LpPart));
-        token_logprobs_kernel<<<dim3(static_cast<unsigned>(n_rows), static_cast<unsigned>(s)), kLpThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-            logits, ld, static_cast<int>(n_rows), static_cast<int>(vocab), tokens, top_k, s, LpOut{logprob, entropy, top_ids, top_logprobs},
-            reinterpret_cast<int32_t*>(ws), parts, keys, status);
-        e = cudaGetLastError();
+        e = launch_dep(token_logprobs_kernel, dim3(static_cast<unsigned>(n_rows), static_cast<unsigned>(s)), kLpThreads, 0,
+                       static_cast<cudaStream_t>(stream), logits, ld, static_cast<int>(n_rows), static_cast<int>(vocab), tokens, top_k, s,
+                       LpOut{logprob, entropy, top_ids, top_logprobs}, reinterpret_cast<int32_t*>(ws), parts, keys, status);
     }
     return e == cudaSuccess ? HESA_CUDA_OK : record_cuda_error(e, "token_logprobs kernel");
 }
