@@ -135,7 +135,7 @@ __device__ __forceinline__ void refuse(const Tables& t, int code) {
 }
 
 __global__ void __launch_bounds__(kPlanThreads)
-free_kernel(const Tables t, const int32_t* __restrict__ slots, int n) {
+free_kernel(const Tables t, const int32_t* slots, int n) {
     grid_dep_wait();
     grid_dep_launch();
     __shared__ uint32_t bits[kMaxSlots / 32];
@@ -155,7 +155,7 @@ free_kernel(const Tables t, const int32_t* __restrict__ slots, int n) {
 }
 
 __global__ void __launch_bounds__(kPlanThreads)
-reserve_kernel(const Tables t, const int32_t* __restrict__ slots, const int32_t* __restrict__ add, int n, PageWork w) {
+reserve_kernel(const Tables t, const int32_t* slots, const int32_t* add, int n, PageWork w) {
     grid_dep_wait();
     grid_dep_launch();
     __shared__ uint32_t bits[kMaxSlots / 32];
@@ -198,7 +198,7 @@ reserve_kernel(const Tables t, const int32_t* __restrict__ slots, const int32_t*
 }
 
 __global__ void __launch_bounds__(kPlanThreads)
-fork_plan_kernel(const Tables t, const int32_t* __restrict__ src, const int32_t* __restrict__ dst, int n, PageWork w) {
+fork_plan_kernel(const Tables t, const int32_t* src, const int32_t* dst, int n, PageWork w) {
     grid_dep_wait();
     grid_dep_launch();
     __shared__ uint32_t bits[kMaxSlots / 32];
@@ -249,7 +249,7 @@ fork_plan_kernel(const Tables t, const int32_t* __restrict__ src, const int32_t*
 
 // live pages to the front: free pages below n_live take the pages in use from n_live on
 __global__ void __launch_bounds__(kPlanThreads)
-compact_plan_kernel(const Tables t, PageWork w, int32_t* __restrict__ n_live_out) {
+compact_plan_kernel(const Tables t, PageWork w, int32_t* n_live_out) {
     grid_dep_wait();
     grid_dep_launch();
     __shared__ int s[33];
@@ -297,7 +297,7 @@ compact_plan_kernel(const Tables t, PageWork w, int32_t* __restrict__ n_live_out
 
 // The listed pairs of pages: in the pool, no page written twice or also read.
 __global__ void __launch_bounds__(kPlanThreads)
-copy_plan_kernel(const Tables t, const int32_t* __restrict__ src, const int32_t* __restrict__ dst, int n, PageWork w) {
+copy_plan_kernel(const Tables t, const int32_t* src, const int32_t* dst, int n, PageWork w) {
     grid_dep_wait();
     grid_dep_launch();
     if (threadIdx.x == 0) *w.n_items = 0;
@@ -330,9 +330,9 @@ copy_plan_kernel(const Tables t, const int32_t* __restrict__ src, const int32_t*
 // only). A page's filled slots are one contiguous range. With map, the tables'
 // entries are replaced by map[entry] in the same launch.
 __global__ void __launch_bounds__(256)
-copy_kernel(uint4* __restrict__ k, uint4* __restrict__ v, int64_t page_words, int64_t layer_words, int n_layer,
-            int slot_words, const int32_t* __restrict__ n_items, const int32_t* __restrict__ items, const Tables t,
-            const int32_t* __restrict__ map) {
+copy_kernel(uint4* k, uint4* v, int64_t page_words, int64_t layer_words, int n_layer,
+            int slot_words, const int32_t* n_items, const int32_t* items, const Tables t,
+            const int32_t* map) {
     grid_dep_wait();
     grid_dep_launch();
     if (map) {
@@ -371,9 +371,9 @@ copy_kernel(uint4* __restrict__ k, uint4* __restrict__ v, int64_t page_words, in
 // units (grid.y covers long rows); q, then k, then v. HBM-bound: each value is
 // read once and written once.
 __global__ void __launch_bounds__(256)
-rope_kv_paged_kernel(PagedLayer c, BatchView b, float* __restrict__ q, int64_t ldq, const float* __restrict__ k, int64_t ldk,
-                     const float* __restrict__ v, int64_t ldv, int n_head, const float* __restrict__ table, int table_rows,
-                     int* __restrict__ status) {
+rope_kv_paged_kernel(PagedLayer c, BatchView b, float* q, int64_t ldq, const float* k, int64_t ldk,
+                     const float* v, int64_t ldv, int n_head, const float* table, int table_rows,
+                     int* status) {
     grid_dep_wait();
     grid_dep_launch();
     const int row = blockIdx.x;
@@ -417,10 +417,10 @@ rope_kv_paged_kernel(PagedLayer c, BatchView b, float* __restrict__ q, int64_t l
         *reinterpret_cast<float4*>(y + 4) = *reinterpret_cast<const float4*>(src + half + d + 4);
         if (table && h < n_rot) {
             float co[8], si[8];
-            *reinterpret_cast<float4*>(co) = __ldg(reinterpret_cast<const float4*>(cs + d));
-            *reinterpret_cast<float4*>(co + 4) = __ldg(reinterpret_cast<const float4*>(cs + d + 4));
-            *reinterpret_cast<float4*>(si) = __ldg(reinterpret_cast<const float4*>(cs + half + d));
-            *reinterpret_cast<float4*>(si + 4) = __ldg(reinterpret_cast<const float4*>(cs + half + d + 4));
+            *reinterpret_cast<float4*>(co) = *reinterpret_cast<const float4*>(cs + d);
+            *reinterpret_cast<float4*>(co + 4) = *reinterpret_cast<const float4*>(cs + d + 4);
+            *reinterpret_cast<float4*>(si) = *reinterpret_cast<const float4*>(cs + half + d);
+            *reinterpret_cast<float4*>(si + 4) = *reinterpret_cast<const float4*>(cs + half + d + 4);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {   // each product and sum rounded by itself, as the library's other rope kernels
                 const float a = x[i], e = y[i];

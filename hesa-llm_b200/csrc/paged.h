@@ -23,6 +23,15 @@ struct PagedLayer {
     const int32_t* table;     // [n_slots][max_pages]
     const int32_t* seq_len;   // [n_slots]
     int32_t n_slots, max_pages;
+    // j / page_size for 0 <= j < 2^31 as the high word of j * mul, shifted: mul =
+    // ceil(2^(31 + b) / page_size), b = ceil(log2(page_size)); its excess of less
+    // than page_size over 2^(31 + b) adds less than one part in page_size.
+    uint32_t page_mul;
+    int32_t page_shift;       // b - 1; -1: pages of one token
+
+    __device__ __forceinline__ int32_t page_index(int32_t j) const {
+        return page_shift < 0 ? j : static_cast<int32_t>(__umulhi(static_cast<uint32_t>(j), page_mul) >> page_shift);
+    }
 };
 
 struct BatchView {
@@ -51,6 +60,7 @@ __device__ __forceinline__ SeqView seq_view(const PagedLayer& c, const BatchView
         r.len = c.seq_len[r.slot];
         r.ok = r.len >= 0 && r.len <= b.max_len && r.len <= static_cast<int64_t>(c.max_pages) * c.page_size;
     }
+    if (!r.ok) r.n_new = r.len = 0;
     return r;
 }
 
@@ -145,7 +155,8 @@ struct AttnArgs {
     float* part;                   // m, l, acc of rows that are added up later
     int32_t per_seq;               // tiles of every sequence, 0: by q_start
     int32_t blocks_per_split;      // chunk_kernel: keys of a split
-    int32_t n_split;               // chunk_kernel: splits; rows_kernel: tiles of a balanced launch, 0: one CTA a tile
+    int32_t n_split;               // chunk_kernel: splits; rows_kernel: tiles of this launch
+    int32_t tile0;                 // rows_kernel: the first of them
 };
 
 // (tile, kv head) pairs that may be split over the keys: one arrival counter
@@ -184,7 +195,8 @@ __device__ __forceinline__ void split_half2(float x0, float x1, uint32_t& hi, ui
 
 // Launch with programmatic stream serialization: the grid may be set up while
 // the previous kernel on the stream finishes. Every such kernel calls
-// grid_dep_wait before it reads or writes anything.
+// grid_dep_wait before it reads or writes anything, and reads what earlier kernels
+// wrote with plain loads (no read-only cache: the grid may be older than the data).
 template <typename... P, typename... T>
 cudaError_t launch_dep(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, T... args) {
     cudaLaunchAttribute attr[1];

@@ -17,15 +17,16 @@
 //     their low halves, so the split costs no product more: thread (row, 2
 //     columns) holds the high part in c0, c1 and the low part in c2, c3 and adds
 //     them. The same thread's scores become its A registers of P V.
-//   * a warp has a kv head of its own, and the eight warps of a CTA take the
-//     same blocks of 16 keys, so that the rows of all heads of a token, which
-//     lie side by side, are read at about the same time. (With a head a CTA the
-//     256-byte rows of a head were read 2 KB apart: 4.2 TB/s at two contexts of
-//     131072 and 100001.) With fewer than eight kv heads the warps share out
-//     the blocks. A warp has its own ring of cp.async stages and no block-wide
-//     barrier in its loop; rows are padded by 16 bytes so that ldmatrix reads
-//     different banks. Pages of any size: each lane looks up the page of one key
-//     of the next block ahead of its copies.
+//   * a warp has a kv head of its own, and the eight warps of a CTA work on the
+//     same blocks of 16 keys: K and V of all heads of a token lie side by side,
+//     and a producer warp copies them with one bulk copy a token and pool (2 KB
+//     for eight heads of 128) into a ring of stages. (A head a CTA read 256-byte
+//     rows 2 KB apart: 4.2 TB/s at two contexts of 131072 and 100001 tokens; 16
+//     bytes a thread with cp.async: 5.4; a 256-byte bulk copy a row and head:
+//     4.9, bound by the copies' number.) With fewer than eight kv heads the
+//     warps share out the blocks of a stage. Rows are padded by 16 bytes so that
+//     ldmatrix reads different banks; pages may have any size. The producer goes
+//     on to the next run of blocks while the warps finish the last one.
 //   * P V of a block starts at zero and is added with one fma that also
 //     rescales (acc = acc * 2^(m_old - m_new) + c): the running sums round to
 //     nearest in fp32 whatever the tensor core does.
@@ -50,23 +51,21 @@ namespace {
 
 constexpr int kRowTile = 8;
 constexpr int kKeyBlock = 16;
-constexpr int kRowsCtas = 148;       // of a balanced launch: one an SM
-constexpr int kMostTiles = 1024;     // of a balanced launch: the tiles' blocks are summed in shared memory
+constexpr int kRowsCtas = 148;       // one an SM
+constexpr int kMostTiles = 1024;     // of a launch: the tiles' blocks are summed in shared memory
 constexpr int kSegCost = 3;          // units for starting a (tile, group): about its time over that of a block
 constexpr int kLeastUnits = 4;       // of a run
 
 template <int HD> struct RowsShape {
-    static constexpr int warps = HD == 256 ? 4 : 8;
+    static constexpr int warps = HD == 256 ? 4 : 8;       // and one that copies
+    static constexpr int threads = (warps + 1) * 32;
     static constexpr int stages = HD == 64 ? 5 : 3;
-    static constexpr int row_halves = HD + 8;                      // padded by 16 bytes
-    static constexpr int stage_halves = 2 * kKeyBlock * row_halves;   // K, then V
-    static constexpr size_t warp_bytes = static_cast<size_t>(stages) * stage_halves * 2;
-    static constexpr size_t smem = warps * warp_bytes;
-    // after its loop a warp's ring holds its (m, l, acc) of 8 rows
-    static_assert(kRowTile * (HD + 2) * 4 <= warp_bytes, "merge region");
+    // a stage: K then V of `subs` blocks, rows of `heads` heads padded by 16 bytes; heads * subs <= warps
+    static constexpr size_t stage_bytes = 2 * kKeyBlock * (warps * HD * 2 + warps * 16);
+    static constexpr size_t smem = stages * stage_bytes;
     // parts: two a CTA, each [warps][rows]: (m, l), then acc[HD]
     static constexpr size_t part_rows = 2 * static_cast<size_t>(kRowsCtas) * warps * kRowTile;
-    static constexpr size_t cut_bytes = kRowsCtas * 16;
+    static constexpr size_t cut_bytes = kMostTiles * 16;   // of the list of what is to be added up
     static constexpr size_t part_bytes = cut_bytes + part_rows * (2 + HD) * 4;
 };
 
@@ -80,12 +79,10 @@ struct HeadGroups {
     }
 };
 
-__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool have) {
-    const int n = have ? 16 : 0;   // 0: sixteen zero bytes, src is not read
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+// Whether every (tile, group) has an entry in the list of what is to be added up.
+__host__ __device__ inline bool by_tile(int tiles, const HeadGroups& hg) {
+    return hg.subs > 1 || static_cast<int64_t>(tiles) * hg.groups <= kRowsCtas;   // (subs > 1: one group)
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -105,177 +102,228 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Blocks of a tile that has rows (one for a tile whose rows see nothing: its
-// zeros are written there), else 0.
-__device__ __forceinline__ int tile_blocks(const AttnArgs& A, int idx, bool report) {
-    int seq, tile;
-    locate_tile(A.b, A.group, kRowTile, A.per_seq, idx, seq, tile);
-    const SeqView sv = seq_view(A.c, A.b, seq);
-    if (!sv.ok) {
-        if (report) record_status(A.status, kStatusBadPosition);
-        return 0;
-    }
-    const int n_rows = sv.n_new * A.group, r0 = tile * kRowTile, base = sv.len - sv.n_new;
-    if (r0 >= n_rows) return 0;
-    Mask mask{sv.len, A.window, 0};
-    if (A.prefix) mask.prefix = max(0, min(A.prefix[seq], sv.len));
-    return max(1, key_blocks(mask, base + r0 / A.group, base + min(r0 + kRowTile - 1, n_rows - 1) / A.group, kKeyBlock).n);
+// 64-bit quotients of numbers that are small nearly always
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
 }
 
-// The runs: CTA c of n_cta has units [start(c), start(c + 1)).
+// The runs: CTA c of n_cta has units [start(c), start(c + 1)), `each` of them,
+// the first `more` CTAs one more.
 struct Runs {
-    int64_t units;
+    int64_t each, more;
     int n_cta;
-    __device__ __forceinline__ int64_t start(int c) const { return units * c / n_cta; }
+    __device__ __forceinline__ Runs(int64_t units, int most) {
+        n_cta = static_cast<int>(max(int64_t(1), min(static_cast<int64_t>(most), units / kLeastUnits)));
+        each = quotient(units, n_cta);
+        more = units - each * n_cta;
+    }
+    __device__ __forceinline__ int64_t start(int c) const { return each * c + min(static_cast<int64_t>(c), more); }
     __device__ __forceinline__ int cta_of(int64_t u) const {   // the last c with start(c) <= u
-        return static_cast<int>(((u + 1) * n_cta - 1) / units);
+        const int64_t head = more * (each + 1);
+        return static_cast<int>(u < head ? quotient(u, each + 1) : more + quotient(u - head, each));
     }
 };
 
-// Blocks [b0, b1) of tile idx for the heads of group grp. part < 0: they are all
-// of it, and the result goes to out; else (m, l, acc) go to that part.
+// What a CTA's run has of one (tile, group): blocks [b0, b1).
+struct Segment {
+    int tile, grp, b0, b1;
+    int64_t first;   // its first unit; the blocks' units start kSegCost later
+    int64_t units;
+};
+
+// The next segment with blocks of the run [u, end); u moves behind it. `lo` is a
+// tile that starts at or before u.
+__device__ __forceinline__ bool next_segment(const int64_t* pre, int groups, int64_t& u, int64_t end, int& lo, Segment& s) {
+    while (u < end) {
+        while (pre[lo + 1] * groups <= u) ++lo;   // tiles without rows have no units
+        s.tile = lo;
+        s.units = pre[lo + 1] - pre[lo];
+        s.grp = static_cast<int>(quotient(u - pre[lo] * groups, s.units));
+        s.first = pre[lo] * groups + s.grp * s.units;
+        const int64_t from = max(u, s.first + kSegCost), stop = min(end, s.first + s.units);
+        u = stop;
+        s.b0 = static_cast<int>(from - s.first - kSegCost);
+        s.b1 = static_cast<int>(stop - s.first - kSegCost);
+        if (s.b1 > s.b0) return true;
+    }
+    return false;
+}
+
+// The rows and keys of a tile.
+struct TileView {
+    SeqView sv;
+    int n_rows, r0, base;   // base: position of the sequence's first new token
+    int32_t p_lo, p_hi;
+    Mask mask;
+    KeyBlocks kb;
+};
+
+__device__ __forceinline__ TileView tile_view(const AttnArgs& A, int idx) {
+    TileView v;
+    int seq, tile;
+    locate_tile(A.b, A.group, kRowTile, A.per_seq, A.tile0 + idx, seq, tile);
+    v.sv = seq_view(A.c, A.b, seq);
+    v.n_rows = v.sv.n_new * A.group;
+    v.r0 = tile * kRowTile;
+    v.base = v.sv.len - v.sv.n_new;
+    v.p_lo = v.base + v.r0 / A.group;
+    v.p_hi = v.base + (min(v.r0 + kRowTile, v.n_rows) - 1) / A.group;
+    v.mask = Mask{v.sv.len, A.window, 0};
+    if (A.prefix && v.sv.ok) v.mask.prefix = max(0, min(A.prefix[seq], v.sv.len));
+    v.kb = key_blocks(v.mask, v.p_lo, v.p_hi, kKeyBlock);
+    return v;
+}
+
+// The ring between the producer and the consumer warps.
+struct Ring {
+    uint8_t* smem;
+    uint64_t *full, *empty;
+    uint32_t at;      // stages used so far (the same in every warp)
+    uint32_t row;     // bytes of a row
+    bool ok;          // no wait has run out
+};
+
+// Producer warp: a segment's blocks, `subs` a stage. Lane j < 16 copies K's row
+// of key j of a block (all heads of the group), lane 16 + j V's.
 template <int HD>
-__device__ __forceinline__ void rows_segment(const AttnArgs& A, uint8_t* smem, const HeadGroups& hg, int idx, int grp, int b0, int b1, int part) {
+__device__ __forceinline__ void copy_segment(const AttnArgs& A, Ring& ring, const HeadGroups& hg, const Segment& seg) {
+    using S = RowsShape<HD>;
+    const int lane = threadIdx.x & 31;
+    const TileView tv = tile_view(A, seg.tile);
+    const int i1 = min(tv.kb.n, seg.b1);
+    const int32_t* table = A.c.table + static_cast<int64_t>(tv.sv.slot) * A.c.max_pages;
+    const __half* pool = (lane < 16 ? A.c.k : A.c.v) + seg.grp * hg.heads * HD;
+    const int row_elems = A.c.n_kv * HD;
+    const uint32_t bytes = static_cast<uint32_t>(min(hg.heads, A.c.n_kv - seg.grp * hg.heads)) * HD * 2;
+    for (int i = seg.b0; i < i1; i += hg.subs) {
+        const uint32_t slot = ring.at % S::stages;
+        uint8_t* stage = ring.smem + slot * S::stage_bytes;
+        bool waited = false;
+#pragma unroll 1
+        for (int x = 0; x < hg.subs && i + x < i1; ++x) {
+            const int32_t j = tv.kb.at(i + x) * kKeyBlock + (lane & 15);
+            const int32_t pi = A.c.page_index(j);
+            const int32_t page = j < tv.sv.len ? table[pi] : -1;   // asked for before the wait
+            const bool good = page >= 0 && page < A.c.n_pages;
+            if (!waited) {
+                waited = true;
+                if (ring.at >= S::stages && ring.ok)
+                    ring.ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ring.empty[slot], (ring.at / S::stages - 1) & 1u, A.status, kStatusWaitTimeout));
+                if (!ring.ok) return;
+            }
+            uint8_t* dst = stage + ((lane >> 4) * hg.subs * kKeyBlock + x * kKeyBlock + (lane & 15)) * ring.row;
+            if (!good) {   // no token, or no page: zeros, in order before a later copy into the row
+                if (j < tv.sv.len) record_status(A.status, kStatusBadPosition);
+                for (uint32_t c = 0; c < bytes; c += 16) *reinterpret_cast<uint4*>(dst + c) = make_uint4(0u, 0u, 0u, 0u);
+                fence_proxy_async_smem();
+            }
+            const uint32_t rows = __popc(__ballot_sync(0xffffffffu, good));
+            __syncwarp();
+            // the stage's one arrival comes with its last block's bytes
+            if (lane == 0) {
+                if (x + 1 < hg.subs && i + x + 1 < i1) mbar_expect_tx(&ring.full[slot], rows * bytes);
+                else mbar_arrive_expect_tx(&ring.full[slot], rows * bytes);
+            }
+            __syncwarp();
+            if (good)
+                bulk_g2s(dst, pool + static_cast<int64_t>(page) * A.c.page_stride + static_cast<int64_t>(j - pi * A.c.page_size) * row_elems, bytes,
+                         &ring.full[slot]);
+        }
+        ++ring.at;
+    }
+}
+
+// Consumer warp: its head's attention over a segment's blocks. part < 0: they
+// are all that the rows see, and the result goes to out; else (m, l, acc) go to
+// that part.
+template <int HD>
+__device__ __forceinline__ void rows_segment(const AttnArgs& A, Ring& ring, const HeadGroups& hg, const Segment& seg, int part) {
     using S = RowsShape<HD>;
     constexpr int KS = HD / 16;                  // k-steps of Q K^T
     constexpr int NT = HD / 8;                   // column tiles of P V
-    constexpr int RH = S::row_halves;
-    constexpr int PIECES = HD / 8;               // 16-byte pieces of a row
-    constexpr int COPIES = kKeyBlock * PIECES / 32;   // of K (and of V) for each lane and block
-
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int sub = warp / hg.heads, kvh = grp * hg.heads + warp % hg.heads;
+    const int sub = warp / hg.heads, hl = warp % hg.heads, kvh = seg.grp * hg.heads + hl;
     const bool active = sub < hg.subs && kvh < A.c.n_kv;
-    uint8_t* my_smem = smem + warp * S::warp_bytes;
+    const TileView tv = tile_view(A, seg.tile);
+    const SeqView& sv = tv.sv;
+    const Mask& mask = tv.mask;
 
-    int seq, tile;
-    locate_tile(A.b, A.group, kRowTile, A.per_seq, idx, seq, tile);
-    const SeqView sv = seq_view(A.c, A.b, seq);   // sound: it has blocks
-    const int n_rows = sv.n_new * A.group;
-    const int r0 = tile * kRowTile;
+    // this thread's row and position
+    const int r = tv.r0 + (lane >> 2);
+    const bool row_ok = r < tv.n_rows && active;
+    const int rc = min(r, tv.n_rows - 1), t = rc / A.group, h = min(kvh, A.c.n_kv - 1) * A.group + rc - t * A.group;
+    const int32_t pos = tv.base + t;
+    const RowKeys keys = mask.row(pos);
+    const int i1 = min(tv.kb.n, seg.b1);
 
-    // this thread's row and position; the tile's positions
-    const int r = r0 + (lane >> 2);
-    const bool row_ok = r < n_rows;
-    const int t = (row_ok ? r : n_rows - 1) / A.group, h = kvh * A.group + (row_ok ? r : n_rows - 1) - t * A.group;
-    const int base = sv.len - sv.n_new;   // position of the sequence's first new token
-    const int32_t pos = base + t;
+    // ---- q as hi and lo halves of q * 2^-e, max |q| 2^-e in [2^14, 2^15) ----
+    uint32_t qa[KS][4];
+    float qscale;   // 2^e; NaN for a row that is not finite
+    {
+        const float* q = A.q + static_cast<int64_t>(sv.q0 + t) * A.ldq + static_cast<int64_t>(h) * HD;
+        float2 v[KS][2];
+        float mx = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) v[k][i] = row_ok ? *reinterpret_cast<const float2*>(q + k * 16 + i * 8 + 2 * (lane & 3)) : make_float2(0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) mx = fmax_nan(mx, fmax_nan(fabsf(v[k][i].x), fabsf(v[k][i].y)));
+        mx = fmax_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmax_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const bool fin = mx < INFINITY;
+        int e = 0;
+        if (fin && mx > 0.f) e = ilogbf(mx) - 14;
+        // two factors, so that 2^-e stays finite for the smallest subnormal q
+        const float f1 = ldexpf(1.f, -(e / 2)), f2 = fin ? ldexpf(1.f, -(e - e / 2)) : 0.f;
+        qscale = fin ? ldexpf(1.f, e) : NAN;
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float x = fin ? v[k][i].x * f1 * f2 : 0.f, y = fin ? v[k][i].y * f1 * f2 : 0.f;
+                split_half2(x, y, qa[k][2 * i], qa[k][2 * i + 1]);
+            }
+    }
+    const float sc = A.cap2 != 0.f ? qscale : qscale * A.scale2;
+    const float slope2 = A.slopes ? A.slopes[h] * 1.44269504088896341f : 0.f;
+
     float m = -INFINITY, l = 0.f;
     float acc[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = 0.f;
 
-    if (active) {
-        const int32_t p_lo = base + r0 / A.group;
-        const int32_t p_hi = base + min(r0 + kRowTile - 1, n_rows - 1) / A.group;
-        Mask mask{sv.len, A.window, 0};
-        if (A.prefix) mask.prefix = max(0, min(A.prefix[seq], sv.len));
-        const RowKeys keys = mask.row(pos);
-        const KeyBlocks kb = key_blocks(mask, p_lo, p_hi, kKeyBlock);
-        const int i0 = b0 + sub, i1 = min(kb.n, b1), step = hg.subs;
+    // ldmatrix row addresses: K matrices (keys 0-7 | 8-15) x (dims 0-7 | 8-15), V the same, transposed
+    const uint32_t mine = static_cast<uint32_t>(sub * kKeyBlock) * ring.row + hl * HD * 2;   // this warp's block and head in a stage
+    const uint32_t v_at = static_cast<uint32_t>(hg.subs * kKeyBlock) * ring.row;
+    const uint32_t k_row = ((lane & 7) + ((lane >> 4) << 3)) * ring.row + ((lane >> 3) & 1) * 16;
+    const uint32_t v_row = ((lane & 7) + (((lane >> 3) & 1) << 3)) * ring.row + (lane >> 4) * 16;
 
-        // ---- copies of this warp's blocks i0, i0 + step, ... ----
-        const int32_t* table = A.c.table + static_cast<int64_t>(sv.slot) * A.c.max_pages;
-        const int row_elems = A.c.n_kv * HD;
-        const uint32_t ring = smem_addr(my_smem);
-        const int psz = A.c.page_size;
-        // lane (key lane & 15 of block i): its page, -1 where it has none
-        auto page_of = [&](int i) -> int32_t {
-            if (i >= i1) return -1;
-            const int32_t j = kb.at(i) * kKeyBlock + (lane & 15);
-            return j < sv.len ? table[j / psz] : -1;
-        };
-        auto issue = [&](int i, int slot, int32_t page) {
-            if (i < i1) {
-                const int32_t j = kb.at(i) * kKeyBlock + (lane & 15);
-                const bool in = j < sv.len;
-                const bool good = in && page >= 0 && page < A.c.n_pages;
-                if (in && !good) record_status(A.status, kStatusBadPosition);   // not read: zeros in its place
-                const int64_t off = good ? static_cast<int64_t>(page) * A.c.page_stride +
-                                               static_cast<int64_t>(j % psz) * row_elems + kvh * HD
-                                         : -1;
-                const uint32_t dst = ring + static_cast<uint32_t>(slot) * S::stage_halves * 2;
-#pragma unroll
-                for (int c = 0; c < COPIES; ++c) {
-                    const int piece = c * 32 + lane, row = piece / PIECES, at = piece % PIECES;
-                    const int64_t o = __shfl_sync(0xffffffffu, off, row);
-                    const int64_t src = (o < 0 ? 0 : o) + at * 8;
-                    const uint32_t d = dst + static_cast<uint32_t>(row * RH + at * 8) * 2;
-                    cp_async16_zfill(d, A.c.k + src, o >= 0);
-                    cp_async16_zfill(d + kKeyBlock * RH * 2, A.c.v + src, o >= 0);
-                }
-            }
-            cp_commit();
-        };
-        int32_t next_page = page_of(i0);
-#pragma unroll
-        for (int s = 0; s < S::stages - 1; ++s) {
-            const int i = i0 + s * step;
-            const int32_t pg = next_page;
-            next_page = page_of(i + step);
-            issue(i, s, pg);
-        }
+    for (int i0 = seg.b0; i0 < i1; i0 += hg.subs, ++ring.at) {
+        const uint32_t slot = ring.at % S::stages;
+        if (ring.ok) ring.ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ring.full[slot], (ring.at / S::stages) & 1u, A.status, kStatusWaitTimeout));
+        if (!ring.ok) break;
+        const int i = i0 + sub;
+        if (active && i < i1) {
+            uint8_t* kp = ring.smem + slot * S::stage_bytes + mine;
+            uint8_t* vp = kp + v_at;
+            const uint32_t sk = smem_addr(kp), sv_ = smem_addr(vp);
+            const int32_t j0 = tv.kb.at(i) * kKeyBlock;
 
-        // ---- q as hi and lo halves of q * 2^-e, max |q| 2^-e in [2^14, 2^15) ----
-        uint32_t qa[KS][4];
-        float qscale;   // 2^e; NaN for a row that is not finite
-        {
-            const float* q = A.q + static_cast<int64_t>(sv.q0 + t) * A.ldq + static_cast<int64_t>(h) * HD;
-            float2 v[KS][2];
-            float mx = 0.f;
-#pragma unroll
-            for (int k = 0; k < KS; ++k)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    v[k][i] = row_ok ? *reinterpret_cast<const float2*>(q + k * 16 + i * 8 + 2 * (lane & 3)) : make_float2(0.f, 0.f);
-                    mx = fmax_nan(mx, fmax_nan(fabsf(v[k][i].x), fabsf(v[k][i].y)));
-                }
-            mx = fmax_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmax_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const bool fin = mx < INFINITY;
-            int e = 0;
-            if (fin && mx > 0.f) e = ilogbf(mx) - 14;
-            // two factors, so that 2^-e stays finite for the smallest subnormal q
-            const float f1 = ldexpf(1.f, -(e / 2)), f2 = fin ? ldexpf(1.f, -(e - e / 2)) : 0.f;
-            qscale = fin ? ldexpf(1.f, e) : NAN;
-#pragma unroll
-            for (int k = 0; k < KS; ++k)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float x = fin ? v[k][i].x * f1 * f2 : 0.f, y = fin ? v[k][i].y * f1 * f2 : 0.f;
-                    split_half2(x, y, qa[k][2 * i], qa[k][2 * i + 1]);
-                }
-        }
-        const float sc = A.cap2 != 0.f ? qscale : qscale * A.scale2;
-        const float slope2 = A.slopes ? A.slopes[h] * 1.44269504088896341f : 0.f;
-
-        // ldmatrix row addresses: K matrices (keys 0-7 | 8-15) x (dims 0-7 | 8-15), V the same, transposed
-        const uint32_t k_row = static_cast<uint32_t>(((lane & 7) + ((lane >> 4) << 3)) * RH + ((lane >> 3) & 1) * 8) * 2;
-        const uint32_t v_row = static_cast<uint32_t>(((lane & 7) + (((lane >> 3) & 1) << 3)) * RH + (lane >> 4) * 8) * 2;
-
-        int slot = 0;
-        for (int i = i0; i < i1; i += step) {
-            {
-                const int ahead = i + (S::stages - 1) * step;
-                const int32_t pg = next_page;
-                next_page = page_of(ahead + step);
-                issue(ahead, slot == 0 ? S::stages - 1 : slot - 1, pg);   // the stage read in the last round
-            }
-            cp_wait<S::stages - 1>();
-            __syncwarp();
-            const uint32_t sk = ring + static_cast<uint32_t>(slot) * S::stage_halves * 2, sv_ = sk + kKeyBlock * RH * 2;
-            __half* vb = reinterpret_cast<__half*>(my_smem + (sv_ - ring));
-            const int32_t j0 = kb.at(i) * kKeyBlock;
-
-            float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};   // keys 0-7, 8-15
+            // keys 0-7 and 8-15, each in two chains of products
+            float s0[2][4] = {}, s1[2][4] = {};
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
                 uint32_t b[4];
                 ldsm4(b, sk + k_row + k * 32);
-                mma16816(s0, qa[k], b[0], b[1]);
-                mma16816(s1, qa[k], b[2], b[3]);
+                mma16816(s0[k & 1], qa[k], b[0], b[1]);
+                mma16816(s1[k & 1], qa[k], b[2], b[3]);
             }
-            float s[4] = {s0[0] + s0[2], s0[1] + s0[3], s1[0] + s1[2], s1[1] + s1[3]};
+            float s[4] = {(s0[0][0] + s0[1][0]) + (s0[0][2] + s0[1][2]), (s0[0][1] + s0[1][1]) + (s0[0][3] + s0[1][3]),
+                          (s1[0][0] + s1[1][0]) + (s1[0][2] + s1[1][2]), (s1[0][1] + s1[1][1]) + (s1[0][3] + s1[1][3])};
 #pragma unroll
             for (int c = 0; c < 4; ++c) s[c] *= sc;
             if (A.cap2 != 0.f) {
@@ -287,7 +335,7 @@ __device__ __forceinline__ void rows_segment(const AttnArgs& A, uint8_t* smem, c
 #pragma unroll
                 for (int c = 0; c < 4; ++c) s[c] -= slope2 * fabsf(static_cast<float>(pos - (jc + (c >> 1) * 8 + (c & 1))));
             }
-            if (!mask.all(p_lo, p_hi, j0, j0 + kKeyBlock)) {
+            if (!mask.all(tv.p_lo, tv.p_hi, j0, j0 + kKeyBlock)) {
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
                     if (!keys.sees(jc + (c >> 1) * 8 + (c & 1))) s[c] = -INFINITY;
@@ -296,26 +344,28 @@ __device__ __forceinline__ void rows_segment(const AttnArgs& A, uint8_t* smem, c
                 // cache) are added where they are seen and then cleared, so that they
                 // reach no other row. Keys past the sequence are zeros.
                 bool odd = false;
-                for (int c = lane; c < kKeyBlock * PIECES; c += 32) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(vb + (c / PIECES) * RH + (c % PIECES) * 8);
+                for (int c = lane; c < kKeyBlock * HD / 8; c += 32) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(vp + (c / (HD / 8)) * ring.row + (c % (HD / 8)) * 16);
                     odd |= nonfinite_h2(w.x) || nonfinite_h2(w.y) || nonfinite_h2(w.z) || nonfinite_h2(w.w);
                 }
                 if (__any_sync(0xffffffffu, odd)) {
                     for (int j = 0; j < kKeyBlock; ++j) {
                         const bool seen = keys.sees(j0 + j);
+                        const __half* vr = reinterpret_cast<const __half*>(vp + j * ring.row) + 2 * (lane & 3);
 #pragma unroll
                         for (int n = 0; n < NT; ++n)
 #pragma unroll
                             for (int c = 0; c < 2; ++c) {
-                                const float x = __half2float(vb[j * RH + n * 8 + 2 * (lane & 3) + c]);
+                                const float x = __half2float(vr[n * 8 + c]);
                                 if (seen && !isfinite(x)) acc[n][c] += x;
                             }
                     }
                     __syncwarp();
                     for (int c = lane; c < kKeyBlock * HD; c += 32) {
-                        __half& x = vb[(c / HD) * RH + c % HD];
+                        __half& x = reinterpret_cast<__half*>(vp + (c / HD) * ring.row)[c % HD];
                         if (!isfinite(__half2float(x))) x = __float2half_rn(0.f);
                     }
+                    fence_proxy_async_smem();   // before the stage is filled again
                     __syncwarp();
                 }
             }
@@ -345,44 +395,13 @@ __device__ __forceinline__ void rows_segment(const AttnArgs& A, uint8_t* smem, c
                 acc[n + 1][0] = fmaf(acc[n + 1][0], corr, c1[0] + c1[2]);
                 acc[n + 1][1] = fmaf(acc[n + 1][1], corr, c1[1] + c1[3]);
             }
-            __syncwarp();   // the warp is done with this stage before it is refilled
-            slot = slot + 1 == S::stages ? 0 : slot + 1;
         }
-        cp_wait<0>();
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        __syncwarp();   // the warp is done with this stage
+        if (lane == 0) mbar_arrive(&ring.empty[slot]);
     }
-
-    if (hg.subs > 1) {
-        // the warps that share a head, in order
-        const int row = lane >> 2;
-        float* mine = reinterpret_cast<float*>(my_smem) + row * (HD + 2);
-        if (active && sub > 0) {
-            if ((lane & 3) == 0) *reinterpret_cast<float2*>(mine) = make_float2(m, l);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(mine + 2 + n * 8 + 2 * (lane & 3)) = make_float2(acc[n][0], acc[n][1]);
-        }
-        __syncthreads();
-        if (active && sub == 0) {
-            for (int s = 1; s < hg.subs; ++s) {
-                const float* o = reinterpret_cast<const float*>(my_smem + static_cast<size_t>(s) * hg.heads * S::warp_bytes) + row * (HD + 2);
-                const float2 ml = *reinterpret_cast<const float2*>(o);
-                const float M = fmaxf(m, ml.x);
-                // a side that saw nothing adds its l and acc too: zeros, or the NaN of a row that is not finite
-                const float fa = m == -INFINITY ? 1.f : ex2(m - M), fb = ml.x == -INFINITY ? 1.f : ex2(ml.x - M);
-                m = M;
-                l = fmaf(ml.y, fb, l * fa);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const float2 v = *reinterpret_cast<const float2*>(o + 2 + n * 8 + 2 * (lane & 3));
-                    acc[n][0] = fmaf(v.x, fb, acc[n][0] * fa);
-                    acc[n][1] = fmaf(v.y, fb, acc[n][1] * fa);
-                }
-            }
-        }
-        __syncthreads();   // shared memory is free again
-    }
-    if (!active || sub > 0 || !row_ok) return;
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if (!row_ok) return;
     if (part < 0) {
         float* o = A.out + static_cast<int64_t>(sv.q0 + t) * A.ldo + static_cast<int64_t>(h) * HD + 2 * (lane & 3);
         const float inv = l == 0.f ? 0.f : 1.f / l;   // nothing seen: zeros
@@ -399,39 +418,44 @@ __device__ __forceinline__ void rows_segment(const AttnArgs& A, uint8_t* smem, c
 }
 
 // What combine_kernel adds up: the parts of (tile, grp) are `first`, then the
-// first part of each of the next n - 1 CTAs. n < 2: nothing, it lies in one run.
-// Few (tile, group)s have an entry each; else there is one for each CTA, for
-// the cut before its run (if that is the first one of what it cuts).
+// first part of each of the next n - 1 CTAs, each of hg.subs warps. n = 0, or one
+// part of one warp: nothing. With by_tile every (tile, group) has an entry; else
+// there is one for each CTA, for the cut before its run (if it is the first one of
+// what it cuts).
 struct __align__(16) Cut {
     int32_t tile, grp, first, n;
 };
 
-__host__ __device__ inline bool by_tile(int tiles, const HeadGroups& hg) { return static_cast<int64_t>(tiles) * hg.groups <= kRowsCtas; }
-
-// A.n_split tiles in equal runs; 0: one CTA for each tile and group, where these are many.
 template <int HD>
-__global__ void __launch_bounds__(RowsShape<HD>::warps * 32, 1)
+__global__ void __launch_bounds__(RowsShape<HD>::threads, 1)
 rows_kernel(const __grid_constant__ AttnArgs A) {
-    constexpr int W = RowsShape<HD>::warps;
+    using S = RowsShape<HD>;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int64_t s_pre[kMostTiles + 1];
-    __shared__ int64_t s_sum[W];
-    const HeadGroups hg(A.c.n_kv, W);
-    const int tiles = A.n_split;
-    grid_dep_wait();
-    if (tiles == 0) {
-        const int nb = tile_blocks(A, static_cast<int>(blockIdx.x), threadIdx.x == 0);
-        if (nb > 0) rows_segment<HD>(A, smem, hg, static_cast<int>(blockIdx.x), static_cast<int>(blockIdx.y), 0, nb, -1);
-        return;
+    __shared__ int64_t s_sum[S::warps + 1];
+    __shared__ __align__(8) uint64_t s_full[S::stages], s_empty[S::stages];
+    const HeadGroups hg(A.c.n_kv, S::warps);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tiles = A.n_split, cta = blockIdx.x;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::stages; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&s_empty[i], S::warps);
+        }
+        s_pre[0] = 0;
+        fence_mbar_init();
     }
+    grid_dep_wait();
     grid_dep_launch();   // combine_kernel may be set up meanwhile; it waits for this grid's end
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int64_t before = 0;
-    if (threadIdx.x == 0) s_pre[0] = 0;
-    for (int i0 = 0; i0 < tiles; i0 += W * 32) {
+    for (int i0 = 0; i0 < tiles; i0 += S::threads) {
         const int i = i0 + threadIdx.x;
-        const int nb = i < tiles ? tile_blocks(A, i, blockIdx.x == 0) : 0;
-        int64_t v = nb > 0 ? nb + kSegCost : 0;
+        int64_t v = 0;
+        if (i < tiles) {
+            const TileView tv = tile_view(A, i);
+            if (!tv.sv.ok && cta == 0) record_status(A.status, kStatusBadPosition);
+            // a tile whose rows see nothing has one block too: its zeros are written there
+            if (tv.sv.ok && tv.r0 < tv.n_rows) v = max(1, tv.kb.n) + kSegCost;
+        }
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int64_t y = __shfl_up_sync(0xffffffffu, v, o);
@@ -440,7 +464,7 @@ rows_kernel(const __grid_constant__ AttnArgs A) {
         if (lane == 31) s_sum[warp] = v;
         __syncthreads();
         int64_t all = 0;
-        for (int w = 0; w < W; ++w) {
+        for (int w = 0; w <= S::warps; ++w) {
             if (w < warp) v += s_sum[w];
             all += s_sum[w];
         }
@@ -448,41 +472,41 @@ rows_kernel(const __grid_constant__ AttnArgs A) {
         before += all;
         __syncthreads();
     }
-    Runs runs{before * hg.groups, 1};
-    runs.n_cta = static_cast<int>(max(int64_t(1), min(static_cast<int64_t>(gridDim.x), runs.units / kLeastUnits)));
-    const int cta = blockIdx.x;
+    const int64_t units = before * hg.groups;
+    const Runs runs(units, gridDim.x);
     const bool listed_by_tile = by_tile(tiles, hg);
     Cut* cuts = reinterpret_cast<Cut*>(A.part);
+    int64_t u = 0, end = 0;
+    if (units > 0 && cta < runs.n_cta) {
+        u = runs.start(cta);
+        end = runs.start(cta + 1);
+    }
+    const int64_t begin = u;
+    int lo = 0, hi = tiles - 1;   // the last tile that starts at or before u
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (s_pre[mid] * hg.groups <= u) lo = mid;
+        else hi = mid - 1;
+    }
+    Ring ring{smem, s_full, s_empty, 0u, static_cast<uint32_t>(hg.heads * HD * 2 + 16), true};
+    Segment seg;
+    if (warp == S::warps) {
+        while (next_segment(s_pre, hg.groups, u, end, lo, seg)) copy_segment<HD>(A, ring, hg, seg);
+        // nothing may be in flight when the CTA ends
+        for (uint32_t i = ring.at > S::stages ? ring.at - S::stages : 0; i < ring.at; ++i)
+            if (!mbar_wait_bounded(&s_full[i % S::stages], (i / S::stages) & 1u, A.status, kStatusDrainTimeout)) break;
+        return;
+    }
     if (listed_by_tile && cta == 0)   // those without rows
-        for (int i = threadIdx.x; i < tiles * hg.groups; i += W * 32)
+        for (int i = threadIdx.x; i < tiles * hg.groups; i += S::warps * 32)
             if (s_pre[i / hg.groups + 1] == s_pre[i / hg.groups]) cuts[i] = Cut{0, 0, 0, 0};
     Cut cut{0, 0, 0, 0};
-    if (runs.units > 0 && cta < runs.n_cta) {
-        int64_t u = runs.start(cta);
-        const int64_t begin = u, end = runs.start(cta + 1);
-        int lo = 0, hi = tiles - 1;   // the last tile that starts at or before u
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (s_pre[mid] * hg.groups <= u) lo = mid;
-            else hi = mid - 1;
-        }
-        while (u < end) {
-            while (s_pre[lo + 1] * hg.groups <= u) ++lo;   // tiles without rows have no units
-            const int64_t n = s_pre[lo + 1] - s_pre[lo], off = u - s_pre[lo] * hg.groups;
-            const int grp = static_cast<int>(off / n);
-            const int64_t first = s_pre[lo] * hg.groups + grp * n;   // of kSegCost, then the blocks
-            const int64_t stop = min(end, first + n);
-            if (stop > first + kSegCost) {
-                const int64_t b0 = max(u, first + kSegCost) - first - kSegCost, b1 = stop - first - kSegCost;
-                const int c_first = runs.cta_of(first + kSegCost), c_last = runs.cta_of(first + n - 1);
-                const int which = begin >= first ? 0 : 1;
-                const Cut all{lo, grp, 2 * c_first + (runs.start(c_first) >= first ? 0 : 1), c_last - c_first + 1};
-                if (cta == c_first + 1) cut = all;
-                if (listed_by_tile && cta == c_first && threadIdx.x == 0) cuts[lo * hg.groups + grp] = all;
-                rows_segment<HD>(A, smem, hg, lo, grp, static_cast<int>(b0), static_cast<int>(b1), c_first == c_last ? -1 : 2 * cta + which);
-            }
-            u = stop;
-        }
+    while (next_segment(s_pre, hg.groups, u, end, lo, seg)) {
+        const int c_first = runs.cta_of(seg.first + kSegCost), c_last = runs.cta_of(seg.first + seg.units - 1);
+        const Cut all{seg.tile, seg.grp, 2 * c_first + (runs.start(c_first) >= seg.first ? 0 : 1), c_last - c_first + 1};
+        if (cta == c_first + 1) cut = all;
+        if (listed_by_tile && cta == c_first && threadIdx.x == 0) cuts[seg.tile * hg.groups + seg.grp] = all;
+        rows_segment<HD>(A, ring, hg, seg, c_first == c_last && hg.subs == 1 ? -1 : 2 * cta + (begin >= seg.first ? 0 : 1));
     }
     if (!listed_by_tile && threadIdx.x == 0) cuts[cta] = cut;
 }
@@ -492,42 +516,57 @@ template <int HD>
 __global__ void __launch_bounds__(256)
 combine_kernel(const __grid_constant__ AttnArgs A) {
     using S = RowsShape<HD>;
-    __shared__ float s_w[kRowsCtas];
+    __shared__ float s_w[kRowsCtas * S::warps];
     __shared__ float s_red[2][8];
     __shared__ float4 s_o[256];
+    // rows_kernel has waited for what came before it: the batch can be read already
+    const HeadGroups hg(A.c.n_kv, S::warps);
+    const bool listed_by_tile = by_tile(A.n_split, hg);
+    const int hl = blockIdx.y, row = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    TileView tv{};
+    if (listed_by_tile) tv = tile_view(A, static_cast<int>(blockIdx.x) / hg.groups);
     grid_dep_wait();
     grid_dep_launch();
     const int4 c4 = __ldcg(reinterpret_cast<const int4*>(A.part) + blockIdx.x);
     const Cut cut{c4.x, c4.y, c4.z, c4.w};
-    if (cut.n < 2) return;
-    const HeadGroups hg(A.c.n_kv, S::warps);
-    const int hl = blockIdx.y, row = blockIdx.z, kvh = cut.grp * hg.heads + hl;
-    if (hl >= hg.heads || kvh >= A.c.n_kv) return;
-    int seq, tile;
-    locate_tile(A.b, A.group, kRowTile, A.per_seq, cut.tile, seq, tile);
-    const SeqView sv = seq_view(A.c, A.b, seq);
-    const int r = tile * kRowTile + row;
-    if (r >= sv.n_new * A.group) return;
+    const int n = cut.n * hg.subs, kvh = cut.grp * hg.heads + hl;
+    if (n < 2 || kvh >= A.c.n_kv) return;
+    if (!listed_by_tile) tv = tile_view(A, cut.tile);
+    const int r = tv.r0 + row;
+    if (r >= tv.n_rows) return;
     const int t = r / A.group, h = kvh * A.group + r - t * A.group;
     const float* ml = A.part + S::cut_bytes / 4;
     const float* acc = ml + S::part_rows * 2;
-    // parts `first`, then slot 0 of the CTAs after it
-    auto at = [&](int i) { return (static_cast<int64_t>(i == 0 ? cut.first : 2 * ((cut.first >> 1) + i)) * S::warps + hl) * kRowTile + row; };
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    // every part's weight, and the sum (at most 148 parts: one a thread)
-    float2 p = make_float2(-INFINITY, 0.f);
-    if (static_cast<int>(threadIdx.x) < cut.n) p = __ldcg(reinterpret_cast<const float2*>(ml + at(threadIdx.x) * 2));
-    float M = p.x;
+    auto at = [&](int i) {
+        const int p = i / hg.subs, x = i - p * hg.subs;
+        return (static_cast<int64_t>(p == 0 ? cut.first : 2 * ((cut.first >> 1) + p)) * S::warps + x * hg.heads + hl) * kRowTile + row;
+    };
+    // thread (dims d .. d + 3, share of the parts): its first parts are on their way while the weights are made
+    constexpr int Q = HD / 4, SHARES = 256 / Q, AHEAD = 8;
+    const int d = threadIdx.x % Q, share = threadIdx.x / Q;
+    float4 a[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+        a[k] = share + k * SHARES < n ? __ldcg(reinterpret_cast<const float4*>(acc + at(share + k * SHARES) * HD) + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+    float M = -INFINITY;
+    for (int i = threadIdx.x; i < n; i += 256) {
+        const float mi = __ldcg(ml + at(i) * 2);
+        s_w[i] = mi;
+        M = fmaxf(M, mi);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     if (lane == 0) s_red[0][warp] = M;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < 8; ++w) M = fmaxf(M, s_red[0][w]);
-    // a part that saw nothing adds zeros, or the NaN of a row that is not finite
-    const float f = p.x == -INFINITY ? 1.f : ex2(p.x - M);
-    if (static_cast<int>(threadIdx.x) < cut.n) s_w[threadIdx.x] = f;
-    float L = p.y * f;
+    float L = 0.f;
+    for (int i = threadIdx.x; i < n; i += 256) {
+        const float mi = s_w[i];
+        const float f = mi == -INFINITY ? 1.f : ex2(mi - M);   // a part that saw nothing adds zeros, or the NaN of a row that is not finite
+        s_w[i] = f;
+        L = fmaf(__ldcg(ml + at(i) * 2 + 1), f, L);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
     if (lane == 0) s_red[1][warp] = L;
@@ -535,38 +574,37 @@ combine_kernel(const __grid_constant__ AttnArgs A) {
     L = 0.f;
 #pragma unroll
     for (int w = 0; w < 8; ++w) L += s_red[1][w];
-    // thread (dims d .. d + 3, share of the parts)
-    constexpr int Q = HD / 4, SHARES = 256 / Q;
-    const int d = threadIdx.x % Q, share = threadIdx.x / Q;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = share; i < cut.n; i += SHARES) {
-        const float4 a = __ldcg(reinterpret_cast<const float4*>(acc + at(i) * HD) + d);
+    auto add = [&](const float4& v, int i) {
         const float w = s_w[i];
-        o.x = fmaf(a.x, w, o.x);
-        o.y = fmaf(a.y, w, o.y);
-        o.z = fmaf(a.z, w, o.z);
-        o.w = fmaf(a.w, w, o.w);
-    }
+        o.x = fmaf(v.x, w, o.x);
+        o.y = fmaf(v.y, w, o.y);
+        o.z = fmaf(v.z, w, o.z);
+        o.w = fmaf(v.w, w, o.w);
+    };
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+        if (share + k * SHARES < n) add(a[k], share + k * SHARES);
+#pragma unroll 4
+    for (int i = share + AHEAD * SHARES; i < n; i += SHARES) add(__ldcg(reinterpret_cast<const float4*>(acc + at(i) * HD) + d), i);
     s_o[threadIdx.x] = o;
     __syncthreads();
     if (share == 0) {
         for (int s = 1; s < SHARES; ++s) {
-            const float4 a = s_o[s * Q + d];
-            o.x += a.x;
-            o.y += a.y;
-            o.z += a.z;
-            o.w += a.w;
+            const float4 v = s_o[s * Q + d];
+            o.x += v.x;
+            o.y += v.y;
+            o.z += v.z;
+            o.w += v.w;
         }
         const float inv = L == 0.f ? 0.f : 1.f / L;
-        reinterpret_cast<float4*>(A.out + static_cast<int64_t>(sv.q0 + t) * A.ldo + static_cast<int64_t>(h) * HD)[d] =
+        reinterpret_cast<float4*>(A.out + static_cast<int64_t>(tv.sv.q0 + t) * A.ldo + static_cast<int64_t>(h) * HD)[d] =
             make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
     }
 }
 
 struct Plan {
     bool tc;         // chunk_kernel of paged_attention_tc.cu
-    bool balanced;   // rows_kernel in equal runs
     int rows, per_seq, tiles, blocks_per_split, n_split;
 };
 
@@ -584,10 +622,7 @@ Plan make_plan(const hesa_cuda_paged_kv* kv, const hesa_cuda_token_batch* b, int
     const int64_t tiles = p.per_seq ? b->n_seq * most : bound;
     p.tiles = static_cast<int>(tiles);
     const int64_t pairs = tiles * kv->n_kv_head;
-    if (!p.tc) {
-        p.balanced = tiles <= kMostTiles;
-        return p;
-    }
+    if (!p.tc) return p;
     // one CTA an SM, no split under 512 keys
     const int64_t blocks = std::max<int64_t>(1, (b->max_len + kTcKeys - 1) / kTcKeys);
     int64_t per = blocks;
@@ -602,12 +637,12 @@ Plan make_plan(const hesa_cuda_paged_kv* kv, const hesa_cuda_token_batch* b, int
 
 size_t part_bytes(const Plan& p, const hesa_cuda_paged_kv* kv) {
     const size_t row = static_cast<size_t>(kv->head_dim + 2) * sizeof(float);
-    if (!p.tc) return !p.balanced ? 0 : kv->head_dim == 64 ? RowsShape<64>::part_bytes : kv->head_dim == 128 ? RowsShape<128>::part_bytes : RowsShape<256>::part_bytes;
+    if (!p.tc) return kv->head_dim == 64 ? RowsShape<64>::part_bytes : kv->head_dim == 128 ? RowsShape<128>::part_bytes : RowsShape<256>::part_bytes;
     return p.n_split > 1 ? static_cast<size_t>(p.tiles) * kv->n_kv_head * p.n_split * p.rows * row : 0;
 }
 
 template <int HD>
-cudaError_t launch_rows(const AttnArgs& a, const Plan& p, cudaStream_t s) {
+cudaError_t launch_rows(AttnArgs a, const Plan& p, cudaStream_t s) {
     static bool set[64] = {};   // per instance and device
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -620,12 +655,15 @@ cudaError_t launch_rows(const AttnArgs& a, const Plan& p, cudaStream_t s) {
     }
     using S = RowsShape<HD>;
     const HeadGroups hg(a.c.n_kv, S::warps);
-    const dim3 grid = p.balanced ? dim3(kRowsCtas) : dim3(static_cast<unsigned>(p.tiles), static_cast<unsigned>(hg.groups));
-    e = launch_dep(rows_kernel<HD>, grid, S::warps * 32, S::smem, s, a);
-    if (e != cudaSuccess || !p.balanced) return e;
-    const int cuts = by_tile(a.n_split, hg) ? a.n_split * hg.groups : kRowsCtas;
     const int rows = std::min(kRowTile, a.b.max_new * a.group);
-    return launch_dep(combine_kernel<HD>, dim3(static_cast<unsigned>(cuts), static_cast<unsigned>(hg.heads), static_cast<unsigned>(rows)), 256, 0, s, a);
+    for (a.tile0 = 0; a.tile0 < p.tiles && e == cudaSuccess; a.tile0 += kMostTiles) {
+        a.n_split = std::min(kMostTiles, p.tiles - a.tile0);
+        e = launch_dep(rows_kernel<HD>, dim3(kRowsCtas), S::threads, S::smem, s, a);
+        const int cuts = by_tile(a.n_split, hg) ? a.n_split * hg.groups : kRowsCtas;
+        if (e == cudaSuccess)
+            e = launch_dep(combine_kernel<HD>, dim3(static_cast<unsigned>(cuts), static_cast<unsigned>(hg.heads), static_cast<unsigned>(rows)), 256, 0, s, a);
+    }
+    return e;
 }
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -680,6 +718,10 @@ PagedLayer layer_of(const hesa_cuda_paged_kv* kv, int32_t layer) {
     c.seq_len = kv->seq_len;
     c.n_slots = kv->n_slots;
     c.max_pages = kv->max_pages;
+    int b = 0;
+    while ((1 << b) < kv->page_size) ++b;
+    c.page_mul = b == 0 ? 0u : static_cast<uint32_t>(((uint64_t(1) << (31 + b)) + kv->page_size - 1) / kv->page_size);
+    c.page_shift = b - 1;
     return c;
 }
 
@@ -741,7 +783,7 @@ int hesa_cuda_paged_attention(const hesa_cuda_paged_kv* kv, int32_t layer, const
     a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kPagedCounterBytes);
     a.per_seq = p.per_seq;
     a.blocks_per_split = p.blocks_per_split;
-    a.n_split = p.tc ? p.n_split : p.balanced ? p.tiles : 0;
+    a.n_split = p.n_split;
     cudaError_t e = status_word(&a.status);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (e == cudaSuccess && p.tc) {

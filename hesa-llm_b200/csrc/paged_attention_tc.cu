@@ -249,7 +249,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const int32_t key = j < n ? kb.at(i0 + j) * kN + pw * KEYS + u * 32 + lane : sv.len;
-                    pg[u] = key < sv.len ? table[key / psz] : -1;
+                    pg[u] = key < sv.len ? table[A.c.page_index(key)] : -1;
                 }
             };
             // and where their rows lie; -1: nowhere, zeros are put there
@@ -259,7 +259,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A) {
                     const int32_t key = kb.at(i0 + j) * kN + pw * KEYS + u * 32 + lane;
                     off[u] = -1;
                     if (key < sv.len) {
-                        if (pg[u] >= 0 && pg[u] < A.c.n_pages) off[u] = pg[u] * A.c.page_stride + (key % psz) * row_elems + kvh * HD;
+                        if (pg[u] >= 0 && pg[u] < A.c.n_pages) off[u] = pg[u] * A.c.page_stride + (key - A.c.page_index(key) * psz) * row_elems + kvh * HD;
                         else record_status(A.status, kStatusBadPosition);
                     }
                 }

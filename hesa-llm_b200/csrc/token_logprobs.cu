@@ -136,9 +136,9 @@ struct LpPart {
 };
 
 __global__ void __launch_bounds__(kLpThreads)
-token_logprobs_kernel(const float* __restrict__ logits, int64_t ld, int n_rows, int vocab, const int32_t* __restrict__ tokens,
-                      int top_k, int n_split, LpOut o, int32_t* __restrict__ counters, LpPart* __restrict__ parts,
-                      uint64_t* __restrict__ part_keys, int* __restrict__ status) {
+token_logprobs_kernel(const float* logits, int64_t ld, int n_rows, int vocab, const int32_t* tokens,
+                      int top_k, int n_split, LpOut o, int32_t* counters, LpPart* parts,
+                      uint64_t* part_keys, int* status) {
     __shared__ Sums s_sums[kLpWarps];
     __shared__ uint64_t s_keys[kLpWarps][kMaxTop];
     __shared__ int s_last;
