@@ -392,7 +392,7 @@ rope_kv_paged_kernel(PagedLayer c, BatchView b, float* q, int64_t ldq, const flo
     }
     if (t < 0 || t >= s.n_new) return;   // a row behind the last sequence
     const int pos = s.len - s.n_new + t;
-    const int page = pos >= 0 ? c.table[static_cast<int64_t>(s.slot) * c.max_pages + pos / c.page_size] : -1;
+    const int page = pos >= 0 ? c.table[static_cast<int64_t>(s.slot) * c.max_pages + c.page_div.div(pos)] : -1;
     if (pos < 0 || page < 0 || page >= c.n_pages || (table && pos >= table_rows)) {
         if (threadIdx.x == 0) record_status(status, kStatusBadPosition);
         return;
@@ -400,7 +400,7 @@ rope_kv_paged_kernel(PagedLayer c, BatchView b, float* q, int64_t ldq, const flo
     const int hd = c.head_dim, per = hd / 16, half = hd / 2;
     const int n_rot = n_head + c.n_kv;
     const int units = (n_rot + c.n_kv) * per;
-    const int64_t at = static_cast<int64_t>(page) * c.page_stride + static_cast<int64_t>(pos % c.page_size) * c.n_kv * hd;
+    const int64_t at = static_cast<int64_t>(page) * c.page_stride + static_cast<int64_t>(pos - c.page_div.div(pos) * c.page_size) * c.n_kv * hd;
     __half* kc = const_cast<__half*>(c.k) + at;
     __half* vc = const_cast<__half*>(c.v) + at;
     const float* cs = table ? table + static_cast<int64_t>(pos) * hd : nullptr;

@@ -13,6 +13,25 @@
 
 namespace hesa_cuda {
 
+// x / d for 0 <= x < 2^31 as the high word of x * mul, shifted: mul =
+// ceil(2^(31 + b) / d), b = ceil(log2(d)); its excess of less than d over
+// 2^(31 + b) adds less than 1 / d to the quotient.
+struct FastDiv {
+    uint32_t mul;
+    int32_t shift;   // b - 1; -1: d = 1
+    int32_t d;
+    FastDiv() = default;
+    __host__ explicit FastDiv(int32_t by) : mul(0), shift(-1), d(by) {
+        int b = 0;
+        while ((int64_t(1) << b) < by) ++b;
+        if (b > 0) mul = static_cast<uint32_t>(((uint64_t(1) << (31 + b)) + by - 1) / by);
+        shift = b - 1;
+    }
+    __device__ __forceinline__ int32_t div(int32_t x) const {
+        return shift < 0 ? x : static_cast<int32_t>(__umulhi(static_cast<uint32_t>(x), mul) >> shift);
+    }
+};
+
 // One layer of the cache. Element e of kv head h of the token in slot s of
 // page p lies at p * page_stride + (s * n_kv + h) * head_dim + e.
 struct PagedLayer {
@@ -23,15 +42,7 @@ struct PagedLayer {
     const int32_t* table;     // [n_slots][max_pages]
     const int32_t* seq_len;   // [n_slots]
     int32_t n_slots, max_pages;
-    // j / page_size for 0 <= j < 2^31 as the high word of j * mul, shifted: mul =
-    // ceil(2^(31 + b) / page_size), b = ceil(log2(page_size)); its excess of less
-    // than page_size over 2^(31 + b) adds less than one part in page_size.
-    uint32_t page_mul;
-    int32_t page_shift;       // b - 1; -1: pages of one token
-
-    __device__ __forceinline__ int32_t page_index(int32_t j) const {
-        return page_shift < 0 ? j : static_cast<int32_t>(__umulhi(static_cast<uint32_t>(j), page_mul) >> page_shift);
-    }
+    FastDiv page_div;         // by page_size
 };
 
 struct BatchView {
@@ -145,6 +156,7 @@ struct AttnArgs {
     float* out;
     int64_t ldo;
     int32_t n_head, group;         // group = n_head / n_kv
+    FastDiv group_div;             // by group
     float scale2;                  // scale * log2(e): scores are kept in base 2
     float cap2, cap_in;            // softcap * log2(e) and scale / softcap; 0: not capped
     int32_t window;

@@ -19,7 +19,7 @@
 //     them. The same thread's scores become its A registers of P V.
 //   * a warp has a kv head of its own, and the eight warps of a CTA work on the
 //     same blocks of 16 keys: K and V of all heads of a token lie side by side,
-//     and a producer warp copies them with one bulk copy a token and pool (2 KB
+//     and four producer warps copy them with one bulk copy a token and pool (2 KB
 //     for eight heads of 128) into a ring of stages. (A head a CTA read 256-byte
 //     rows 2 KB apart: 4.2 TB/s at two contexts of 131072 and 100001 tokens; 16
 //     bytes a thread with cp.async: 5.4; a 256-byte bulk copy a row and head:
@@ -31,7 +31,7 @@
 //     rescales (acc = acc * 2^(m_old - m_new) + c): the running sums round to
 //     nearest in fp32 whatever the tensor core does.
 //   * the work is a row of units, one for each block of keys of each (tile,
-//     group of heads) and kSegCost for starting one; a grid of one CTA an SM
+//     group of heads) and a few for starting one; a grid of one CTA an SM
 //     takes equal runs of it, cut anywhere, so that sequences of all lengths
 //     load every SM alike. The lengths are only known on the device: every CTA
 //     adds up the tiles' blocks itself. What lies in several runs leaves (m, l,
@@ -52,13 +52,14 @@ namespace {
 constexpr int kRowTile = 8;
 constexpr int kKeyBlock = 16;
 constexpr int kRowsCtas = 148;       // one an SM
+constexpr int kCopyWarps = 4;        // a warp gets no more than one bulk copy under way in about 45 ns
 constexpr int kMostTiles = 1024;     // of a launch: the tiles' blocks are summed in shared memory
-constexpr int kSegCost = 3;          // units for starting a (tile, group): about its time over that of a block
+constexpr int kSegCost = 5;          // stages that starting a (tile, group) takes the time of
 constexpr int kLeastUnits = 4;       // of a run
 
 template <int HD> struct RowsShape {
-    static constexpr int warps = HD == 256 ? 4 : 8;       // and one that copies
-    static constexpr int threads = (warps + 1) * 32;
+    static constexpr int warps = HD == 256 ? 4 : 8;       // and kCopyWarps that copy
+    static constexpr int threads = (warps + kCopyWarps) * 32;
     static constexpr int stages = HD == 64 ? 5 : 3;
     // a stage: K then V of `subs` blocks, rows of `heads` heads padded by 16 bytes; heads * subs <= warps
     static constexpr size_t stage_bytes = 2 * kKeyBlock * (warps * HD * 2 + warps * 16);
@@ -71,17 +72,22 @@ template <int HD> struct RowsShape {
 
 // Heads of a group (a CTA's warps have one each) and how many warps share a head.
 struct HeadGroups {
-    int groups, heads, subs;
-    __host__ __device__ HeadGroups(int n_kv, int warps) {
-        groups = (n_kv + warps - 1) / warps;
+    int groups, heads, subs, recip, cost, sub_bits;   // subs is a power of two, `warps` being one
+    // `most` heads a group at most, a power of two up to `warps`
+    HeadGroups(int n_kv, int warps, int most) {
+        groups = (n_kv + most - 1) / most;
         heads = (n_kv + groups - 1) / groups;
-        subs = warps / heads;
+        for (sub_bits = 0; (heads << (sub_bits + 1)) <= warps;) ++sub_bits;
+        subs = 1 << sub_bits;
+        recip = (256 + heads - 1) / heads;
+        cost = kSegCost * subs;
     }
+    __device__ __forceinline__ int sub_of(int warp) const { return warp * recip >> 8; }   // warp / heads for warp < 9
 };
 
 // Whether every (tile, group) has an entry in the list of what is to be added up.
 __host__ __device__ inline bool by_tile(int tiles, const HeadGroups& hg) {
-    return hg.subs > 1 || static_cast<int64_t>(tiles) * hg.groups <= kRowsCtas;   // (subs > 1: one group)
+    return hg.subs > 1 || static_cast<int64_t>(tiles) * hg.groups <= kRowsCtas;
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -128,23 +134,23 @@ struct Runs {
 // What a CTA's run has of one (tile, group): blocks [b0, b1).
 struct Segment {
     int tile, grp, b0, b1;
-    int64_t first;   // its first unit; the blocks' units start kSegCost later
+    int64_t first;   // its first unit; the blocks' units start hg.cost later
     int64_t units;
 };
 
 // The next segment with blocks of the run [u, end); u moves behind it. `lo` is a
 // tile that starts at or before u.
-__device__ __forceinline__ bool next_segment(const int64_t* pre, int groups, int64_t& u, int64_t end, int& lo, Segment& s) {
+__device__ __forceinline__ bool next_segment(const int64_t* pre, const HeadGroups& hg, int64_t& u, int64_t end, int& lo, Segment& s) {
     while (u < end) {
-        while (pre[lo + 1] * groups <= u) ++lo;   // tiles without rows have no units
+        while (pre[lo + 1] * hg.groups <= u) ++lo;   // tiles without rows have no units
         s.tile = lo;
         s.units = pre[lo + 1] - pre[lo];
-        s.grp = static_cast<int>(quotient(u - pre[lo] * groups, s.units));
-        s.first = pre[lo] * groups + s.grp * s.units;
-        const int64_t from = max(u, s.first + kSegCost), stop = min(end, s.first + s.units);
+        s.grp = static_cast<int>(quotient(u - pre[lo] * hg.groups, s.units));
+        s.first = pre[lo] * hg.groups + s.grp * s.units;
+        const int64_t from = max(u, s.first + hg.cost), stop = min(end, s.first + s.units);
         u = stop;
-        s.b0 = static_cast<int>(from - s.first - kSegCost);
-        s.b1 = static_cast<int>(stop - s.first - kSegCost);
+        s.b0 = static_cast<int>(from - s.first - hg.cost);
+        s.b1 = static_cast<int>(stop - s.first - hg.cost);
         if (s.b1 > s.b0) return true;
     }
     return false;
@@ -167,8 +173,8 @@ __device__ __forceinline__ TileView tile_view(const AttnArgs& A, int idx) {
     v.n_rows = v.sv.n_new * A.group;
     v.r0 = tile * kRowTile;
     v.base = v.sv.len - v.sv.n_new;
-    v.p_lo = v.base + v.r0 / A.group;
-    v.p_hi = v.base + (min(v.r0 + kRowTile, v.n_rows) - 1) / A.group;
+    v.p_lo = v.base + A.group_div.div(v.r0);
+    v.p_hi = v.base + A.group_div.div(max(min(v.r0 + kRowTile, v.n_rows), 1) - 1);
     v.mask = Mask{v.sv.len, A.window, 0};
     if (A.prefix && v.sv.ok) v.mask.prefix = max(0, min(A.prefix[seq], v.sv.len));
     v.kb = key_blocks(v.mask, v.p_lo, v.p_hi, kKeyBlock);
@@ -184,46 +190,53 @@ struct Ring {
     bool ok;          // no wait has run out
 };
 
-// Producer warp: a segment's blocks, `subs` a stage. Lane j < 16 copies K's row
-// of key j of a block (all heads of the group), lane 16 + j V's.
+// Copying warp pw: a segment's blocks, `subs` a stage. Of the 16 rows of K and 16
+// of V of a block (all heads of the group) it copies rows 8 pw .. 8 pw + 7, of
+// four blocks at once.
 template <int HD>
-__device__ __forceinline__ void copy_segment(const AttnArgs& A, Ring& ring, const HeadGroups& hg, const Segment& seg) {
+__device__ __forceinline__ void copy_segment(const AttnArgs& A, Ring& ring, const HeadGroups& hg, const Segment& seg, int pw) {
     using S = RowsShape<HD>;
     const int lane = threadIdx.x & 31;
     const TileView tv = tile_view(A, seg.tile);
     const int i1 = min(tv.kb.n, seg.b1);
     const int32_t* table = A.c.table + static_cast<int64_t>(tv.sv.slot) * A.c.max_pages;
-    const __half* pool = (lane < 16 ? A.c.k : A.c.v) + seg.grp * hg.heads * HD;
+    const int row = pw * 8 + (lane & 7), v = row >> 4;
+    const __half* pool = (v ? A.c.v : A.c.k) + seg.grp * hg.heads * HD;
     const int row_elems = A.c.n_kv * HD;
     const uint32_t bytes = static_cast<uint32_t>(min(hg.heads, A.c.n_kv - seg.grp * hg.heads)) * HD * 2;
     for (int i = seg.b0; i < i1; i += hg.subs) {
         const uint32_t slot = ring.at % S::stages;
         uint8_t* stage = ring.smem + slot * S::stage_bytes;
-        bool waited = false;
 #pragma unroll 1
-        for (int x = 0; x < hg.subs && i + x < i1; ++x) {
-            const int32_t j = tv.kb.at(i + x) * kKeyBlock + (lane & 15);
-            const int32_t pi = A.c.page_index(j);
+        for (int x0 = 0; x0 < hg.subs; x0 += 4) {
+            const int x = x0 + (lane >> 3);
+            const bool block = x < hg.subs && i + x < i1;
+            const int32_t j = block ? tv.kb.at(i + x) * kKeyBlock + (row & 15) : tv.sv.len;
+            const int32_t pi = A.c.page_div.div(j);
             const int32_t page = j < tv.sv.len ? table[pi] : -1;   // asked for before the wait
             const bool good = page >= 0 && page < A.c.n_pages;
-            if (!waited) {
-                waited = true;
+            if (x0 == 0) {
                 if (ring.at >= S::stages && ring.ok)
                     ring.ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ring.empty[slot], (ring.at / S::stages - 1) & 1u, A.status, kStatusWaitTimeout));
                 if (!ring.ok) return;
             }
-            uint8_t* dst = stage + ((lane >> 4) * hg.subs * kKeyBlock + x * kKeyBlock + (lane & 15)) * ring.row;
-            if (!good) {   // no token, or no page: zeros, in order before a later copy into the row
-                if (j < tv.sv.len) record_status(A.status, kStatusBadPosition);
-                for (uint32_t c = 0; c < bytes; c += 16) *reinterpret_cast<uint4*>(dst + c) = make_uint4(0u, 0u, 0u, 0u);
-                fence_proxy_async_smem();
+            uint8_t* dst = stage + ((v * hg.subs + x) * kKeyBlock + (row & 15)) * ring.row;
+            const unsigned have = __ballot_sync(0xffffffffu, good), lost = __ballot_sync(0xffffffffu, !good && j < tv.sv.len);
+            // zeros where there is no token's V (a K that no row sees may be anything) or no page
+            unsigned zero = __ballot_sync(0xffffffffu, block && !good && v) | lost;
+            if (zero) {
+                for (; zero; zero &= zero - 1) {
+                    uint8_t* to = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(dst), __ffs(zero) - 1));
+                    for (uint32_t c = lane * 16; c < bytes; c += 512) *reinterpret_cast<uint4*>(to + c) = make_uint4(0u, 0u, 0u, 0u);
+                }
+                fence_proxy_async_smem();   // in order before a later copy into the row
+                if (lost && lane == 0) record_status(A.status, kStatusBadPosition);
             }
-            const uint32_t rows = __popc(__ballot_sync(0xffffffffu, good));
             __syncwarp();
-            // the stage's one arrival comes with its last block's bytes
+            // the warp's one arrival at the stage comes with its last blocks' bytes
             if (lane == 0) {
-                if (x + 1 < hg.subs && i + x + 1 < i1) mbar_expect_tx(&ring.full[slot], rows * bytes);
-                else mbar_arrive_expect_tx(&ring.full[slot], rows * bytes);
+                if (x0 + 4 < hg.subs) mbar_expect_tx(&ring.full[slot], __popc(have) * bytes);
+                else mbar_arrive_expect_tx(&ring.full[slot], __popc(have) * bytes);
             }
             __syncwarp();
             if (good)
@@ -243,7 +256,7 @@ __device__ __forceinline__ void rows_segment(const AttnArgs& A, Ring& ring, cons
     constexpr int KS = HD / 16;                  // k-steps of Q K^T
     constexpr int NT = HD / 8;                   // column tiles of P V
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int sub = warp / hg.heads, hl = warp % hg.heads, kvh = seg.grp * hg.heads + hl;
+    const int sub = hg.sub_of(warp), hl = warp - sub * hg.heads, kvh = seg.grp * hg.heads + hl;
     const bool active = sub < hg.subs && kvh < A.c.n_kv;
     const TileView tv = tile_view(A, seg.tile);
     const SeqView& sv = tv.sv;
@@ -252,7 +265,7 @@ __device__ __forceinline__ void rows_segment(const AttnArgs& A, Ring& ring, cons
     // this thread's row and position
     const int r = tv.r0 + (lane >> 2);
     const bool row_ok = r < tv.n_rows && active;
-    const int rc = min(r, tv.n_rows - 1), t = rc / A.group, h = min(kvh, A.c.n_kv - 1) * A.group + rc - t * A.group;
+    const int rc = min(r, tv.n_rows - 1), t = A.group_div.div(rc), h = min(kvh, A.c.n_kv - 1) * A.group + rc - t * A.group;
     const int32_t pos = tv.base + t;
     const RowKeys keys = mask.row(pos);
     const int i1 = min(tv.kb.n, seg.b1);
@@ -428,17 +441,18 @@ struct __align__(16) Cut {
 
 template <int HD>
 __global__ void __launch_bounds__(RowsShape<HD>::threads, 1)
-rows_kernel(const __grid_constant__ AttnArgs A) {
+rows_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ HeadGroups hg) {
     using S = RowsShape<HD>;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int64_t s_pre[kMostTiles + 1];
-    __shared__ int64_t s_sum[S::warps + 1];
+    __shared__ int64_t s_sum[S::warps + kCopyWarps];
     __shared__ __align__(8) uint64_t s_full[S::stages], s_empty[S::stages];
-    const HeadGroups hg(A.c.n_kv, S::warps);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tiles = A.n_split, cta = blockIdx.x;
+    // the arguments come into the constant cache while the previous kernel ends
+    if (A.c.n_pages <= 0 || A.b.n_seq <= 0 || A.ldq <= 0 || A.group <= 0 || A.part == nullptr || hg.heads <= 0) return;
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::stages; ++i) {
-            mbar_init(&s_full[i], 1);
+            mbar_init(&s_full[i], kCopyWarps);
             mbar_init(&s_empty[i], S::warps);
         }
         s_pre[0] = 0;
@@ -454,7 +468,7 @@ rows_kernel(const __grid_constant__ AttnArgs A) {
             const TileView tv = tile_view(A, i);
             if (!tv.sv.ok && cta == 0) record_status(A.status, kStatusBadPosition);
             // a tile whose rows see nothing has one block too: its zeros are written there
-            if (tv.sv.ok && tv.r0 < tv.n_rows) v = max(1, tv.kb.n) + kSegCost;
+            if (tv.sv.ok && tv.r0 < tv.n_rows) v = max(1, tv.kb.n) + hg.cost;
         }
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -464,7 +478,7 @@ rows_kernel(const __grid_constant__ AttnArgs A) {
         if (lane == 31) s_sum[warp] = v;
         __syncthreads();
         int64_t all = 0;
-        for (int w = 0; w <= S::warps; ++w) {
+        for (int w = 0; w < S::warps + kCopyWarps; ++w) {
             if (w < warp) v += s_sum[w];
             all += s_sum[w];
         }
@@ -490,8 +504,8 @@ rows_kernel(const __grid_constant__ AttnArgs A) {
     }
     Ring ring{smem, s_full, s_empty, 0u, static_cast<uint32_t>(hg.heads * HD * 2 + 16), true};
     Segment seg;
-    if (warp == S::warps) {
-        while (next_segment(s_pre, hg.groups, u, end, lo, seg)) copy_segment<HD>(A, ring, hg, seg);
+    if (warp >= S::warps) {
+        while (next_segment(s_pre, hg, u, end, lo, seg)) copy_segment<HD>(A, ring, hg, seg, warp - S::warps);
         // nothing may be in flight when the CTA ends
         for (uint32_t i = ring.at > S::stages ? ring.at - S::stages : 0; i < ring.at; ++i)
             if (!mbar_wait_bounded(&s_full[i % S::stages], (i / S::stages) & 1u, A.status, kStatusDrainTimeout)) break;
@@ -501,8 +515,8 @@ rows_kernel(const __grid_constant__ AttnArgs A) {
         for (int i = threadIdx.x; i < tiles * hg.groups; i += S::warps * 32)
             if (s_pre[i / hg.groups + 1] == s_pre[i / hg.groups]) cuts[i] = Cut{0, 0, 0, 0};
     Cut cut{0, 0, 0, 0};
-    while (next_segment(s_pre, hg.groups, u, end, lo, seg)) {
-        const int c_first = runs.cta_of(seg.first + kSegCost), c_last = runs.cta_of(seg.first + seg.units - 1);
+    while (next_segment(s_pre, hg, u, end, lo, seg)) {
+        const int c_first = runs.cta_of(seg.first + hg.cost), c_last = runs.cta_of(seg.first + seg.units - 1);
         const Cut all{seg.tile, seg.grp, 2 * c_first + (runs.start(c_first) >= seg.first ? 0 : 1), c_last - c_first + 1};
         if (cta == c_first + 1) cut = all;
         if (listed_by_tile && cta == c_first && threadIdx.x == 0) cuts[seg.tile * hg.groups + seg.grp] = all;
@@ -511,18 +525,22 @@ rows_kernel(const __grid_constant__ AttnArgs A) {
     if (!listed_by_tile && threadIdx.x == 0) cuts[cta] = cut;
 }
 
-// The parts of one row of what is cut: block (entry, head of the group, row).
+// Adds up what is cut: block (entry, head of the group), or one for each row too
+// where these are few (then there are many parts). The rows are shared out over
+// the warps; where they are fewer than eight, several warps take every second,
+// fourth or eighth part of a row. Two contexts of 131072 and 100001 tokens with a
+// block for all eight rows: 180 us; with one for each: 163. A batch of 64 short
+// sequences: 13.7 us and 17.6.
 template <int HD>
 __global__ void __launch_bounds__(256)
-combine_kernel(const __grid_constant__ AttnArgs A) {
+combine_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ HeadGroups hg) {
     using S = RowsShape<HD>;
-    __shared__ float s_w[kRowsCtas * S::warps];
-    __shared__ float s_red[2][8];
-    __shared__ float4 s_o[256];
+    constexpr int V = HD / 32;     // values of a lane
+    constexpr int AHEAD = 32 / V;  // parts of which a warp has the loads under way
+    __shared__ float s_o[8][HD + 1];
     // rows_kernel has waited for what came before it: the batch can be read already
-    const HeadGroups hg(A.c.n_kv, S::warps);
     const bool listed_by_tile = by_tile(A.n_split, hg);
-    const int hl = blockIdx.y, row = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int hl = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     TileView tv{};
     if (listed_by_tile) tv = tile_view(A, static_cast<int>(blockIdx.x) / hg.groups);
     grid_dep_wait();
@@ -532,79 +550,79 @@ combine_kernel(const __grid_constant__ AttnArgs A) {
     const int n = cut.n * hg.subs, kvh = cut.grp * hg.heads + hl;
     if (n < 2 || kvh >= A.c.n_kv) return;
     if (!listed_by_tile) tv = tile_view(A, cut.tile);
-    const int r = tv.r0 + row;
-    if (r >= tv.n_rows) return;
-    const int t = r / A.group, h = kvh * A.group + r - t * A.group;
+    const int row0 = blockIdx.z, rows = min(gridDim.z > 1 ? 1 : kRowTile, tv.n_rows - tv.r0 - row0);
+    if (rows <= 0) return;
+    const int slots = rows > 4 ? 8 : rows > 2 ? 4 : rows;   // a power of two
+    const int row = warp & (slots - 1), share = warp / slots, shares = 8 / slots;   // row: of row0 ..
     const float* ml = A.part + S::cut_bytes / 4;
     const float* acc = ml + S::part_rows * 2;
-    auto at = [&](int i) {
-        const int p = i / hg.subs, x = i - p * hg.subs;
-        return (static_cast<int64_t>(p == 0 ? cut.first : 2 * ((cut.first >> 1) + p)) * S::warps + x * hg.heads + hl) * kRowTile + row;
+    auto at = [&](int i) {   // part i: sub-part i % subs of CTA part i / subs
+        const int p = i >> hg.sub_bits, x = i & (hg.subs - 1);
+        return (static_cast<int64_t>(p == 0 ? cut.first : 2 * ((cut.first >> 1) + p)) * S::warps + x * hg.heads + hl) * kRowTile + row0 + row;
     };
-    // thread (dims d .. d + 3, share of the parts): its first parts are on their way while the weights are made
-    constexpr int Q = HD / 4, SHARES = 256 / Q, AHEAD = 8;
-    const int d = threadIdx.x % Q, share = threadIdx.x / Q;
-    float4 a[AHEAD];
+    float L = 0.f, O[V];
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k)
-        a[k] = share + k * SHARES < n ? __ldcg(reinterpret_cast<const float4*>(acc + at(share + k * SHARES) * HD) + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-    float M = -INFINITY;
-    for (int i = threadIdx.x; i < n; i += 256) {
-        const float mi = __ldcg(ml + at(i) * 2);
-        s_w[i] = mi;
-        M = fmaxf(M, mi);
-    }
+    for (int k = 0; k < V; ++k) O[k] = 0.f;
+    if (row < rows) {
+        float2 p[AHEAD];
+        float v[AHEAD][V];
+        auto load = [&](int i0) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    if (lane == 0) s_red[0][warp] = M;
-    __syncthreads();
+            for (int k = 0; k < AHEAD; ++k) {
+                const int i = i0 + k * shares;
+                if (i >= n) break;
+                const int64_t a = at(i);
+                p[k] = __ldcg(reinterpret_cast<const float2*>(ml + a * 2));
+                const float* src = acc + a * HD + lane * V;
+                if constexpr (V == 2) *reinterpret_cast<float2*>(v[k]) = __ldcg(reinterpret_cast<const float2*>(src));
+                else
 #pragma unroll
-    for (int w = 0; w < 8; ++w) M = fmaxf(M, s_red[0][w]);
-    float L = 0.f;
-    for (int i = threadIdx.x; i < n; i += 256) {
-        const float mi = s_w[i];
-        const float f = mi == -INFINITY ? 1.f : ex2(mi - M);   // a part that saw nothing adds zeros, or the NaN of a row that is not finite
-        s_w[i] = f;
-        L = fmaf(__ldcg(ml + at(i) * 2 + 1), f, L);
-    }
+                    for (int c = 0; c < V; c += 4) *reinterpret_cast<float4*>(v[k] + c) = __ldcg(reinterpret_cast<const float4*>(src + c));
+            }
+        };
+        load(share);   // on their way while the maximum is found
+        float M = -INFINITY;
+#pragma unroll 8
+        for (int i = lane; i < n; i += 32) M = fmaxf(M, __ldcg(ml + at(i) * 2));
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-    if (lane == 0) s_red[1][warp] = L;
-    __syncthreads();
-    L = 0.f;
+        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        for (int i0 = share;;) {
 #pragma unroll
-    for (int w = 0; w < 8; ++w) L += s_red[1][w];
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](const float4& v, int i) {
-        const float w = s_w[i];
-        o.x = fmaf(v.x, w, o.x);
-        o.y = fmaf(v.y, w, o.y);
-        o.z = fmaf(v.z, w, o.z);
-        o.w = fmaf(v.w, w, o.w);
-    };
+            for (int k = 0; k < AHEAD; ++k) {
+                if (i0 + k * shares >= n) break;
+                // a part that saw nothing adds zeros, or the NaN of a row that is not finite
+                const float f = p[k].x == -INFINITY ? 1.f : ex2(p[k].x - M);
+                L = fmaf(p[k].y, f, L);
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k)
-        if (share + k * SHARES < n) add(a[k], share + k * SHARES);
-#pragma unroll 4
-    for (int i = share + AHEAD * SHARES; i < n; i += SHARES) add(__ldcg(reinterpret_cast<const float4*>(acc + at(i) * HD) + d), i);
-    s_o[threadIdx.x] = o;
-    __syncthreads();
-    if (share == 0) {
-        for (int s = 1; s < SHARES; ++s) {
-            const float4 v = s_o[s * Q + d];
-            o.x += v.x;
-            o.y += v.y;
-            o.z += v.z;
-            o.w += v.w;
+                for (int c = 0; c < V; ++c) O[c] = fmaf(v[k][c], f, O[c]);
+            }
+            i0 += AHEAD * shares;
+            if (i0 >= n) break;
+            load(i0);
         }
-        const float inv = L == 0.f ? 0.f : 1.f / L;
-        reinterpret_cast<float4*>(A.out + static_cast<int64_t>(tv.sv.q0 + t) * A.ldo + static_cast<int64_t>(h) * HD)[d] =
-            make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        if (shares > 1) {
+#pragma unroll
+            for (int c = 0; c < V; ++c) s_o[warp][lane * V + c] = O[c];
+            if (lane == 0) s_o[warp][HD] = L;
+        }
     }
+    if (shares > 1) __syncthreads();
+    if (row >= rows || share > 0) return;
+    for (int x = 1; x < shares; ++x) {
+        L += s_o[warp + x * slots][HD];
+#pragma unroll
+        for (int c = 0; c < V; ++c) O[c] += s_o[warp + x * slots][lane * V + c];
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    const int r = tv.r0 + row0 + row, t = A.group_div.div(r), h = kvh * A.group + r - t * A.group;
+    float* o = A.out + static_cast<int64_t>(tv.sv.q0 + t) * A.ldo + static_cast<int64_t>(h) * HD + lane * V;
+#pragma unroll
+    for (int c = 0; c < V; c += 2) *reinterpret_cast<float2*>(o + c) = make_float2(O[c] * inv, O[c + 1] * inv);
 }
 
 struct Plan {
     bool tc;         // chunk_kernel of paged_attention_tc.cu
+    int heads;       // rows_kernel: of a group at most
     int rows, per_seq, tiles, blocks_per_split, n_split;
 };
 
@@ -622,7 +640,16 @@ Plan make_plan(const hesa_cuda_paged_kv* kv, const hesa_cuda_token_batch* b, int
     const int64_t tiles = p.per_seq ? b->n_seq * most : bound;
     p.tiles = static_cast<int>(tiles);
     const int64_t pairs = tiles * kv->n_kv_head;
-    if (!p.tc) return p;
+    if (!p.tc) {
+        // All heads of a token at once read the longest rows, and an SM streams no
+        // more than about 44 GB/s: where that would leave SMs without work, groups
+        // of fewer heads. One context of 100 tokens, 64 heads on 8: 13.2 us with all
+        // heads together, 10.3 with two; one of 2048 tokens, 32 heads: 14.3 with eight, 16.5 with two.
+        const int64_t blocks = (b->max_len + kKeyBlock - 1) / kKeyBlock;
+        p.heads = kv->head_dim == 256 ? 4 : 8;
+        while (p.heads > 2 && tiles * ((kv->n_kv_head + p.heads - 1) / p.heads) * blocks < 2 * kRowsCtas) p.heads /= 2;
+        return p;
+    }
     // one CTA an SM, no split under 512 keys
     const int64_t blocks = std::max<int64_t>(1, (b->max_len + kTcKeys - 1) / kTcKeys);
     int64_t per = blocks;
@@ -654,14 +681,15 @@ cudaError_t launch_rows(AttnArgs a, const Plan& p, cudaStream_t s) {
         set[dev] = true;
     }
     using S = RowsShape<HD>;
-    const HeadGroups hg(a.c.n_kv, S::warps);
-    const int rows = std::min(kRowTile, a.b.max_new * a.group);
+    const HeadGroups hg(a.c.n_kv, S::warps, p.heads);
     for (a.tile0 = 0; a.tile0 < p.tiles && e == cudaSuccess; a.tile0 += kMostTiles) {
         a.n_split = std::min(kMostTiles, p.tiles - a.tile0);
-        e = launch_dep(rows_kernel<HD>, dim3(kRowsCtas), S::threads, S::smem, s, a);
+        e = launch_dep(rows_kernel<HD>, dim3(kRowsCtas), S::threads, S::smem, s, a, hg);
         const int cuts = by_tile(a.n_split, hg) ? a.n_split * hg.groups : kRowsCtas;
+        const int rows = std::min(kRowTile, a.b.max_new * a.group);
+        const unsigned z = static_cast<int64_t>(cuts) * hg.heads * rows <= 8 * kRowsCtas ? rows : 1;
         if (e == cudaSuccess)
-            e = launch_dep(combine_kernel<HD>, dim3(static_cast<unsigned>(cuts), static_cast<unsigned>(hg.heads), static_cast<unsigned>(rows)), 256, 0, s, a);
+            e = launch_dep(combine_kernel<HD>, dim3(static_cast<unsigned>(cuts), static_cast<unsigned>(hg.heads), z), 256, 0, s, a, hg);
     }
     return e;
 }
@@ -718,10 +746,7 @@ PagedLayer layer_of(const hesa_cuda_paged_kv* kv, int32_t layer) {
     c.seq_len = kv->seq_len;
     c.n_slots = kv->n_slots;
     c.max_pages = kv->max_pages;
-    int b = 0;
-    while ((1 << b) < kv->page_size) ++b;
-    c.page_mul = b == 0 ? 0u : static_cast<uint32_t>(((uint64_t(1) << (31 + b)) + kv->page_size - 1) / kv->page_size);
-    c.page_shift = b - 1;
+    c.page_div = FastDiv(kv->page_size);
     return c;
 }
 
@@ -771,6 +796,7 @@ int hesa_cuda_paged_attention(const hesa_cuda_paged_kv* kv, int32_t layer, const
     a.ldo = ldo;
     a.n_head = static_cast<int32_t>(n_head);
     a.group = static_cast<int32_t>(n_head / kv->n_kv_head);
+    a.group_div = FastDiv(a.group);
     const double log2e = 1.4426950408889634;
     const double scale = o.scale > 0.f ? o.scale : 1.0 / std::sqrt(static_cast<double>(kv->head_dim));
     a.scale2 = static_cast<float>(scale * log2e);

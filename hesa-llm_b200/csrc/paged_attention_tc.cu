@@ -150,8 +150,8 @@ chunk_kernel(const __grid_constant__ AttnArgs A) {
     // later rows see more keys: the longest tiles of a sequence start first
     const int r0 = ((n_rows + kM - 1) / kM - 1 - tile) * kM;
     const int base = sv.len - sv.n_new;
-    const int32_t p_lo = base + r0 / A.group;
-    const int32_t p_hi = base + min(r0 + kM - 1, n_rows - 1) / A.group;
+    const int32_t p_lo = base + A.group_div.div(r0);
+    const int32_t p_hi = base + A.group_div.div(min(r0 + kM - 1, n_rows - 1));
     Mask mask{sv.len, A.window, 0};
     if (A.prefix) mask.prefix = max(0, min(A.prefix[seq], sv.len));
     const KeyBlocks kb = key_blocks(mask, p_lo, p_hi, kN);
@@ -195,7 +195,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A) {
     const int row = 32 * wq + lane;                       // of the tile, = TMEM lane
     const uint32_t tl = tmem + (static_cast<uint32_t>(32 * wq) << 16);
     const int r = min(r0 + row, n_rows - 1);
-    const int t = r / A.group, h = kvh * A.group + r - t * A.group;
+    const int t = A.group_div.div(r), h = kvh * A.group + r - t * A.group;
     const int32_t pos = base + t;
     float sc = 0.f;
     if (warp < kComputeWarps) {
@@ -249,7 +249,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const int32_t key = j < n ? kb.at(i0 + j) * kN + pw * KEYS + u * 32 + lane : sv.len;
-                    pg[u] = key < sv.len ? table[A.c.page_index(key)] : -1;
+                    pg[u] = key < sv.len ? table[A.c.page_div.div(key)] : -1;
                 }
             };
             // and where their rows lie; -1: nowhere, zeros are put there
@@ -259,7 +259,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A) {
                     const int32_t key = kb.at(i0 + j) * kN + pw * KEYS + u * 32 + lane;
                     off[u] = -1;
                     if (key < sv.len) {
-                        if (pg[u] >= 0 && pg[u] < A.c.n_pages) off[u] = pg[u] * A.c.page_stride + (key - A.c.page_index(key) * psz) * row_elems + kvh * HD;
+                        if (pg[u] >= 0 && pg[u] < A.c.n_pages) off[u] = pg[u] * A.c.page_stride + (key - A.c.page_div.div(key) * psz) * row_elems + kvh * HD;
                         else record_status(A.status, kStatusBadPosition);
                     }
                 }
@@ -565,7 +565,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A) {
 #pragma unroll
                         for (int d = 0; d < HD / 32; ++d) O[d] = fmaf(__ldcg(p0 + i * step + 2 + d * 32 + lane), f, O[d]);
                     }
-                    const int rt = (r0 + rr) / A.group, rh = kvh * A.group + (r0 + rr) - rt * A.group;
+                    const int rt = A.group_div.div(r0 + rr), rh = kvh * A.group + (r0 + rr) - rt * A.group;
                     float* o = A.out + static_cast<int64_t>(sv.q0 + rt) * A.ldo + static_cast<int64_t>(rh) * HD;
 #pragma unroll
                     for (int d = 0; d < HD / 32; ++d) o[d * 32 + lane] = L == 0.f ? 0.f : O[d] / L;
