@@ -20,19 +20,26 @@
 // then adds the previous block's O from TMEM to its fp32 registers, rescaling
 // with one fma. O is a fresh product for every block: only 16 products are
 // summed by the tensor core, and long sums round to nearest in fp32.
-// Warp 8 (one thread) issues the products. S buffer j & 1 is written for block
-// j + 2 in two halves of 64 keys, each as soon as the half of P V of block j
-// that read the same columns has completed, while the other half runs: no pair
-// of products relies on an order that the instruction set does not promise, and
-// the tensor core always has one queued.
-// Warps 9, 10 (producers): cp.async of K and V rows into the 128-byte swizzled
-// layout, page by page whatever the page size. Each thread waits for its own
-// copies, makes them visible to the async proxy and its warp arrives.
+// Warp 8 (one thread) issues the products. S of block j + 2 goes into the buffer
+// that held P of block j once P V of block j has completed: no pair of products
+// relies on an order that the instruction set does not promise. (Writing it in
+// halves of 64 keys, each as soon as its half of P had been read, kept a product
+// queued at all times, but a product of 64 columns takes 56 of the 64 cycles that
+// one of 128 takes: 2.47 ms against XX for 2048 tokens at 16384, 64 heads on 8.)
+// Warps 9-11 (producers): K and V blocks into the 128-byte swizzled layout with
+// tiled copies (TMA) of boxes of gcd(page_size, 128) tokens by 64 dims; a page
+// that is not there is a coordinate past the pool, which reads as zeros. Pages
+// whose size is no multiple of 8 are copied with 16-byte cp.async by two of the
+// warps (a K block takes each of them about 1800 cycles: XX ms).
 #include "paged.h"
 #include "paged_tc.h"
 #include "qmatvec.h"
 
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda/atomic>
+
+#include <numeric>
 
 namespace hesa_cuda {
 namespace {
@@ -41,12 +48,12 @@ constexpr int kM = kTcRows;                  // rows of a tile = TMEM lanes
 constexpr int kN = kTcKeys;                  // keys of a block
 constexpr int kComputeWarps = 8;
 constexpr int kMmaWarp = kComputeWarps;
-constexpr int kProducerWarps = 2;
-constexpr int kThreads = 384;                // three warpgroups; warp 11 is idle
+constexpr int kProducerWarps = 3;            // 2 with cp.async
+constexpr int kThreads = 384;                // three warpgroups
 // Registers a thread after setmaxnreg: 256 x 208 + 128 x 88 = 384 x 168, what
 // the block is launched with.
 constexpr int kComputeRegs = 208, kOtherRegs = 88;
-constexpr int kInFlight = 3;                 // blocks that a producer has in flight
+constexpr int kInFlight = 3;                 // blocks that a producer has in flight with cp.async
 
 template <int HD> struct TcShape {
     static constexpr uint32_t slot = kN * HD * 2;            // one K or V block
@@ -119,17 +126,35 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool have) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 
+// 4-D tiled copy of the box at (x, head, place in page, page)
+__device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* map, int x, int head, int place, int page, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(head), "r"(place), "r"(page), "r"(smem_addr(bar))
+        : "memory");
+}
+
+// x = hi + lo to 22 bits for 0 <= x < 65504: hi is x cut to 11 bits, which costs no
+// conversion back and so has lo follow from x by one mask and one subtraction
+__device__ __forceinline__ void cut_half2(float2 x, uint32_t& hi, uint32_t& lo) {
+    const float2 h = make_float2(__uint_as_float(__float_as_uint(x.x) & 0xFFFFE000u), __uint_as_float(__float_as_uint(x.y) & 0xFFFFE000u));
+    const float2 l = ffma2(h, make_float2(-1.f, -1.f), x);
+    const __half2 a = __floats2half2_rn(h.x, h.y), b = __floats2half2_rn(l.x, l.y);
+    hi = *reinterpret_cast<const uint32_t*>(&a);
+    lo = *reinterpret_cast<const uint32_t*>(&b);
+}
+
 // Places in the ring: K0, K1, V0, K2, V1, ... , the order in which they are used.
 __device__ __forceinline__ int k_place(int j) { return j == 0 ? 0 : 2 * j - 1; }
 __device__ __forceinline__ int v_place(int j, int n) { return j + 1 < n ? 2 * j + 2 : 2 * n - 1; }
 
-template <int HD>
+template <int HD, bool TMA>
 __global__ void __launch_bounds__(kThreads, 1)
-chunk_kernel(const __grid_constant__ AttnArgs A) {
+chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, int box) {
     using S = TcShape<HD>;
     constexpr int HH = HD / 2;   // output dims of a thread
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t full[S::slots], empty[S::slots], s_full[2][2], p_full[2][2], pv_half, o_full, o_free;
+    __shared__ __align__(8) uint64_t full[S::slots], empty[S::slots], s_full[2], p_full[2][2], o_full, o_free;
     __shared__ float s_max[2][2][kM];
     __shared__ uint32_t tmem_base;
     __shared__ int abort_flag, odd_block[2], s_last;
@@ -166,15 +191,13 @@ chunk_kernel(const __grid_constant__ AttnArgs A) {
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::slots; ++i) {
-            mbar_init(&full[i], kProducerWarps);
+            mbar_init(&full[i], TMA ? kProducerWarps : 2);
             mbar_init(&empty[i], 1);
         }
-        for (int i = 0; i < 2; ++i)
-            for (int h = 0; h < 2; ++h) {
-                mbar_init(&s_full[i][h], 1);
-                mbar_init(&p_full[i][h], kComputeWarps / 2);
-            }
-        mbar_init(&pv_half, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_full[i], 1);
+            for (int h = 0; h < 2; ++h) mbar_init(&p_full[i][h], kComputeWarps / 2);
+        }
         mbar_init(&o_full, 1);
         mbar_init(&o_free, kComputeWarps);
         abort_flag = 0;
@@ -233,11 +256,59 @@ chunk_kernel(const __grid_constant__ AttnArgs A) {
 
     if (warp >= kComputeWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-        if (warp > kMmaWarp && warp <= kMmaWarp + kProducerWarps) {
+        if (TMA && warp > kMmaWarp) {
+            // ---- producers: copy c of a block (64 dims of `box` keys) is lane c / 3's of warp c % 3 ----
+            const int pw = warp - kMmaWarp - 1, c = lane * kProducerWarps + pw, copies = (kN / box) * (HD / 64);
+            const int g = c / (HD / 64), x = c % (HD / 64);   // which keys, which dims
+            const uint32_t mine = static_cast<uint32_t>((copies - pw + kProducerWarps - 1) / kProducerWarps) * box * 128;   // bytes of the warp
+            const int32_t* table = A.c.table + static_cast<int64_t>(sv.slot) * A.c.max_pages;
+            const uint32_t to = ring + static_cast<uint32_t>(x * kN + g * box) * 128;
+            bool dead = false;
+            // the page and the place in it of this lane's keys of block j; no page: one past the pool
+            auto find = [&](int j, int& page, int& at) {
+                page = A.c.n_pages;
+                at = 0;
+                if (j < n && c < copies) {
+                    const int32_t key = kb.at(i0 + j) * kN + g * box;
+                    const int32_t pi = A.c.page_div.div(key);
+                    at = key - pi * A.c.page_size;
+                    if (key < sv.len) {
+                        const int32_t p = table[pi];
+                        if (p >= 0 && p < A.c.n_pages) page = p;
+                        else record_status(A.status, kStatusBadPosition);
+                    }
+                }
+            };
+            auto put = [&](int place, const CUtensorMap* map, int page, int at) {
+                const int slot = place % S::slots;
+                if (place >= S::slots && !dead)
+                    dead = !mbar_wait_bounded(&empty[slot], static_cast<uint32_t>(place / S::slots - 1) & 1u, A.status, kStatusWaitTimeout);
+                dead = __any_sync(0xffffffffu, dead);
+                if (dead) return;
+                if (lane == 0) mbar_arrive_expect_tx(&full[slot], mine);
+                __syncwarp();
+                if (c < copies) tma_4d(to + static_cast<uint32_t>(slot) * S::slot, map, x * 64, kvh, at, page, &full[slot]);
+            };
+            if (n > 0) {
+                int page, at, page1, at1;
+                find(0, page, at);
+                put(0, &kmap, page, at);
+                for (int j = 0; j < n; ++j) {
+                    find(j + 1, page1, at1);
+                    if (j + 1 < n) put(k_place(j + 1), &kmap, page1, at1);
+                    put(v_place(j, n), &vmap, page, at);
+                    page = page1;
+                    at = at1;
+                }
+                // after a wait that ran out: nothing may be in flight when the CTA ends
+                for (int p = max(0, 2 * n - S::slots); dead && p < 2 * n; ++p)
+                    if (!mbar_wait_bounded(&full[p % S::slots], static_cast<uint32_t>(p / S::slots) & 1u, A.status, kStatusDrainTimeout)) break;
+            }
+        } else if (!TMA && warp > kMmaWarp && warp <= kMmaWarp + 2) {
             // ---- producers: warp w of them copies keys 64 w .. 64 w + 63 of every block ----
             const int pw = warp - kMmaWarp - 1;
             constexpr int PIECES = HD / 8;          // 16-byte pieces of a row
-            constexpr int KEYS = kN / kProducerWarps, ROWS = 32 / PIECES;
+            constexpr int KEYS = kN / 2, ROWS = 32 / PIECES;
             const int32_t* table = A.c.table + static_cast<int64_t>(sv.slot) * A.c.max_pages;
             const int64_t row_elems = static_cast<int64_t>(A.c.n_kv) * HD;
             const int at = lane % PIECES, psz = A.c.page_size;
@@ -313,20 +384,21 @@ chunk_kernel(const __grid_constant__ AttnArgs A) {
         } else if (warp == kMmaWarp) {
             // ---- products ----
             if (lane == 0) {
-                constexpr uint32_t IQK = idesc_f16(kN / 2, false), IPV = idesc_f16(HD, true);
+                constexpr uint32_t IQK = idesc_f16(kN, false), IPV = idesc_f16(HD, true);
                 auto place = [&](int p) { return ring + static_cast<uint32_t>(p % S::slots) * S::slot; };
                 auto landed = [&](int p) { return mbar_wait_bounded(&full[p % S::slots], static_cast<uint32_t>(p / S::slots) & 1u, A.status, kStatusWaitTimeout); };
                 // the address field of a descriptor counts 16 bytes: k-steps are added to it
-                auto qk = [&](int j, int hf) {
-                    const uint32_t d = tmem + S::s0 + static_cast<uint32_t>((j & 1) * kN + hf * (kN / 2));
-                    const uint64_t b = desc(place(k_place(j)) + static_cast<uint32_t>(hf) * (kN / 2) * 128, 16, 1024);
+                auto qk = [&](int j) {
+                    const uint32_t d = tmem + S::s0 + static_cast<uint32_t>((j & 1) * kN);
+                    const uint64_t b = desc(place(k_place(j)), 16, 1024);
 #pragma unroll 1
                     for (int part = 0; part < 2; ++part) {   // the small products first
                         const uint32_t a = tmem + (part == 0 ? S::q_lo : S::q_hi);
 #pragma unroll
                         for (int k = 0; k < HD / 16; ++k) mma_ts(d, a + 8 * k, b + ((k >> 2) * (kN * 128) + (k & 3) * 32) / 16, IQK, part > 0 || k > 0);
                     }
-                    commit(&s_full[j & 1][hf]);
+                    commit(&empty[k_place(j) % S::slots]);
+                    commit(&s_full[j & 1]);
                 };
                 auto pv = [&](int j, int hf) {
                     const uint32_t p = tmem + S::s0 + static_cast<uint32_t>((j & 1) * kN + hf * (kN / 2));
@@ -343,9 +415,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A) {
                     ok = landed(k_place(j));
                     if (!ok) break;
                     fence_after();
-                    qk(j, 0);
-                    qk(j, 1);
-                    commit(&empty[k_place(j) % S::slots]);
+                    qk(j);
                 }
                 for (int j = 0; j < n && ok && !*abort_v; ++j) {
                     const uint32_t ph = static_cast<uint32_t>(j >> 1) & 1u, each = static_cast<uint32_t>(j) & 1u;
@@ -354,7 +424,6 @@ chunk_kernel(const __grid_constant__ AttnArgs A) {
                     if (!ok) break;
                     fence_after();
                     pv(j, 0);
-                    commit(&pv_half);
                     ok = mbar_wait_bounded(&p_full[j & 1][1], ph, A.status, kStatusWaitTimeout);
                     if (!ok) break;
                     fence_after();
@@ -362,15 +431,11 @@ chunk_kernel(const __grid_constant__ AttnArgs A) {
                     commit(&empty[v_place(j, n) % S::slots]);
                     commit(&o_full);
                     if (j + 2 < n) {
-                        // S half 0 of block j + 2 goes where P half 0 of block j has been read, while half 1 is
-                        ok = landed(k_place(j + 2)) && mbar_wait_bounded(&pv_half, each, A.status, kStatusWaitTimeout);
+                        // S of block j + 2 goes where P of block j has been read
+                        ok = landed(k_place(j + 2)) && mbar_wait_bounded(&o_full, each, A.status, kStatusWaitTimeout);
                         if (!ok) break;
                         fence_after();
-                        qk(j + 2, 0);
-                        ok = mbar_wait_bounded(&o_full, each, A.status, kStatusWaitTimeout);
-                        if (!ok) break;
-                        qk(j + 2, 1);
-                        commit(&empty[k_place(j + 2) % S::slots]);
+                        qk(j + 2);
                     }
                 }
                 if (!ok) *abort_v = 1;
@@ -417,7 +482,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A) {
         for (int j = 0; j < n; ++j) {
             const int buf = j & 1;
             const int32_t j0 = kb.at(i0 + j) * kN, jh = j0 + half * (kN / 2);
-            ok = ok && mbar_wait_bounded(&s_full[buf][half], static_cast<uint32_t>(j >> 1) & 1u, A.status, kStatusWaitTimeout);
+            ok = ok && mbar_wait_bounded(&s_full[buf], static_cast<uint32_t>(j >> 1) & 1u, A.status, kStatusWaitTimeout);
             __syncwarp();
             fence_after();
             const uint32_t sb = tl + S::s0 + buf * kN + half * (kN / 2);
@@ -482,17 +547,18 @@ chunk_kernel(const __grid_constant__ AttnArgs A) {
                     named_barrier(5, kComputeWarps * 32);
                 }
             }
-            float mx = s[0];
+            float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int i = 1; i < 64; ++i) mx = fmaxf(mx, s[i]);
-            s_max[buf][half][row] = mx;
+            for (int i = 4; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
+            const float mh = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            s_max[buf][half][row] = mh;
             named_barrier(1 + wq, 64);   // the two warps of these rows
-            mx = fmaxf(mx, s_max[buf][half ^ 1][row]) * k;
+            float mn = fmaxf(mh, s_max[buf][half ^ 1][row]) * k;
             // k is NaN for a row that is not finite: so are its maximum, its P and its result
-            mx = mx > m ? mx : (mx == mx ? m : mx);
-            const float ms = mx == -INFINITY ? 0.f : mx;
+            mn = mn > m ? mn : (mn == mn ? m : mn);
+            const float ms = mn == -INFINITY ? 0.f : mn;
             const float al = m == -INFINITY ? 0.f : ex2(m - ms);
-            m = mx;
+            m = mn;
             const float off = kPShift - ms;
             float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
@@ -503,7 +569,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A) {
                     const float2 x = ffma2(make_float2(s[c * 32 + 2 * i], s[c * 32 + 2 * i + 1]), make_float2(k, k), make_float2(off, off));
                     const float2 p = make_float2(ex2(x.x), ex2(x.y));
                     sum = fadd2(sum, p);
-                    split_half2(p.x, p.y, hi[i], lo[i]);
+                    cut_half2(p, hi[i], lo[i]);
                 }
                 st16(sb + c * 16, hi);
                 st16(sb + 32 + c * 16, lo);
@@ -585,26 +651,54 @@ chunk_kernel(const __grid_constant__ AttnArgs A) {
     }
 }
 
-template <int HD>
-cudaError_t launch(const AttnArgs& a, int tiles, cudaStream_t s) {
+PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
+    static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q{};
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) f = nullptr;
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+    }();
+    return fn;
+}
+
+// One layer's pool as [page][place][head][dim]; the box: `box` places of one head, 64 dims (128 bytes, the swizzle's span).
+bool encode_pool(CUtensorMap* map, const void* pool, const PagedLayer& c, int box) {
+    const PFN_cuTensorMapEncodeTiled_v12000 encode = map_encoder();
+    if (!encode) return false;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.head_dim), static_cast<cuuint64_t>(c.n_kv), static_cast<cuuint64_t>(c.page_size), static_cast<cuuint64_t>(c.n_pages)};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(c.head_dim) * 2, static_cast<cuuint64_t>(c.n_kv) * c.head_dim * 2, static_cast<cuuint64_t>(c.page_stride) * 2};
+    const cuuint32_t boxes[4] = {64, 1, static_cast<cuuint32_t>(box), 1}, one[4] = {1, 1, 1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(pool), dims, strides, boxes, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int HD, bool TMA>
+cudaError_t launch(const AttnArgs& a, int tiles, int box, cudaStream_t s) {
     static bool set[64] = {};   // per instance and device
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     if (!set[dev]) {
-        e = cudaFuncSetAttribute(chunk_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(TcShape<HD>::smem));
+        e = cudaFuncSetAttribute(chunk_kernel<HD, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(TcShape<HD>::smem));
         if (e != cudaSuccess) return e;
         set[dev] = true;
     }
+    CUtensorMap k{}, v{};
+    if (TMA && (!encode_pool(&k, a.c.k, a.c, box) || !encode_pool(&v, a.c.v, a.c, box))) return cudaErrorInvalidValue;
     const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(a.c.n_kv), static_cast<unsigned>(a.n_split));
-    return launch_dep(chunk_kernel<HD>, grid, kThreads, TcShape<HD>::smem, s, a);
+    return launch_dep(chunk_kernel<HD, TMA>, grid, kThreads, TcShape<HD>::smem, s, a, k, v, box);
 }
 
 }  // namespace
 
 cudaError_t paged_attention_tc(const AttnArgs& a, int tiles, cudaStream_t s) {
-    return a.c.head_dim == 64 ? launch<64>(a, tiles, s) : launch<128>(a, tiles, s);
+    // a box of the tiled copies lies in one page and one block of keys, and its
+    // rows are whole groups of the swizzle; a tensor map's strides are below 2^40
+    const int box = std::gcd(a.c.page_size, kTcKeys);
+    const bool tma = box >= 8 && a.c.page_stride < (int64_t(1) << 39);
+    if (a.c.head_dim == 64) return tma ? launch<64, true>(a, tiles, box, s) : launch<64, false>(a, tiles, box, s);
+    return tma ? launch<128, true>(a, tiles, box, s) : launch<128, false>(a, tiles, box, s);
 }
 
 }  // namespace hesa_cuda
