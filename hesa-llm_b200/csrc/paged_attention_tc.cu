@@ -20,17 +20,18 @@
 // then adds the previous block's O from TMEM to its fp32 registers, rescaling
 // with one fma. O is a fresh product for every block: only 16 products are
 // summed by the tensor core, and long sums round to nearest in fp32.
-// Warp 8 (one thread) issues the products. S of block j + 2 goes into the buffer
+// One thread of warp 8 issues P V, one of warp 9 Q K^T, so that neither's waits
+// hold up the other's products. S of block j + 2 goes into the buffer
 // that held P of block j once P V of block j has completed: no pair of products
 // relies on an order that the instruction set does not promise. (Writing it in
 // halves of 64 keys, each as soon as its half of P had been read, kept a product
 // queued at all times, but a product of 64 columns takes 56 of the 64 cycles that
 // one of 128 takes: 2.47 ms against XX for 2048 tokens at 16384, 64 heads on 8.)
-// Warps 9-11 (producers): K and V blocks into the 128-byte swizzled layout with
+// Warps 10, 11 (producers): K and V blocks into the 128-byte swizzled layout with
 // tiled copies (TMA) of boxes of gcd(page_size, 128) tokens by 64 dims; a page
 // that is not there is a coordinate past the pool, which reads as zeros. Pages
-// whose size is no multiple of 8 are copied with 16-byte cp.async by two of the
-// warps (a K block takes each of them about 1800 cycles: XX ms).
+// whose size is no multiple of 8 are copied with 16-byte cp.async (a K block
+// takes each warp about 1800 cycles: XX ms).
 #include "paged.h"
 #include "paged_tc.h"
 #include "qmatvec.h"
@@ -47,8 +48,9 @@ namespace {
 constexpr int kM = kTcRows;                  // rows of a tile = TMEM lanes
 constexpr int kN = kTcKeys;                  // keys of a block
 constexpr int kComputeWarps = 8;
-constexpr int kMmaWarp = kComputeWarps;
-constexpr int kProducerWarps = 3;            // 2 with cp.async
+constexpr int kQkWarp = kComputeWarps + 1;   // issues Q K^T, the warp before it P V
+constexpr int kProducerWarps = 2;
+constexpr int kFirstProducer = kComputeWarps + 2;
 constexpr int kThreads = 384;                // three warpgroups
 // Registers a thread after setmaxnreg: 256 x 208 + 128 x 88 = 384 x 168, what
 // the block is launched with.
@@ -134,6 +136,12 @@ __device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* map, int
         : "memory");
 }
 
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // x = hi + lo to 22 bits for 0 <= x < 65504: hi is x cut to 11 bits, which costs no
 // conversion back and so has lo follow from x by one mask and one subtraction
 __device__ __forceinline__ void cut_half2(float2 x, uint32_t& hi, uint32_t& lo) {
@@ -154,7 +162,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
     using S = TcShape<HD>;
     constexpr int HH = HD / 2;   // output dims of a thread
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t full[S::slots], empty[S::slots], s_full[2], p_full[2][2], o_full, o_free;
+    __shared__ __align__(8) uint64_t full[S::slots], empty[S::slots], s_full[2], s_free[2], p_full[2][2], o_full, o_free;
     __shared__ float s_max[2][2][kM];
     __shared__ uint32_t tmem_base;
     __shared__ int abort_flag, odd_block[2], s_last;
@@ -191,11 +199,12 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::slots; ++i) {
-            mbar_init(&full[i], TMA ? kProducerWarps : 2);
+            mbar_init(&full[i], kProducerWarps);
             mbar_init(&empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
+            mbar_init(&s_free[i], 1);
             for (int h = 0; h < 2; ++h) mbar_init(&p_full[i][h], kComputeWarps / 2);
         }
         mbar_init(&o_full, 1);
@@ -256,9 +265,9 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
 
     if (warp >= kComputeWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-        if (TMA && warp > kMmaWarp) {
-            // ---- producers: copy c of a block (64 dims of `box` keys) is lane c / 3's of warp c % 3 ----
-            const int pw = warp - kMmaWarp - 1, c = lane * kProducerWarps + pw, copies = (kN / box) * (HD / 64);
+        if (TMA && warp >= kFirstProducer) {
+            // ---- producers: copy c of a block (64 dims of `box` keys) is lane c / 2's of warp c % 2 ----
+            const int pw = warp - kFirstProducer, c = lane * kProducerWarps + pw, copies = (kN / box) * (HD / 64);
             const int g = c / (HD / 64), x = c % (HD / 64);   // which keys, which dims
             const uint32_t mine = static_cast<uint32_t>((copies - pw + kProducerWarps - 1) / kProducerWarps) * box * 128;   // bytes of the warp
             const int32_t* table = A.c.table + static_cast<int64_t>(sv.slot) * A.c.max_pages;
@@ -304,11 +313,11 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
                 for (int p = max(0, 2 * n - S::slots); dead && p < 2 * n; ++p)
                     if (!mbar_wait_bounded(&full[p % S::slots], static_cast<uint32_t>(p / S::slots) & 1u, A.status, kStatusDrainTimeout)) break;
             }
-        } else if (!TMA && warp > kMmaWarp && warp <= kMmaWarp + 2) {
+        } else if (!TMA && warp >= kFirstProducer) {
             // ---- producers: warp w of them copies keys 64 w .. 64 w + 63 of every block ----
-            const int pw = warp - kMmaWarp - 1;
+            const int pw = warp - kFirstProducer;
             constexpr int PIECES = HD / 8;          // 16-byte pieces of a row
-            constexpr int KEYS = kN / 2, ROWS = 32 / PIECES;
+            constexpr int KEYS = kN / kProducerWarps, ROWS = 32 / PIECES;
             const int32_t* table = A.c.table + static_cast<int64_t>(sv.slot) * A.c.max_pages;
             const int64_t row_elems = static_cast<int64_t>(A.c.n_kv) * HD;
             const int at = lane % PIECES, psz = A.c.page_size;
@@ -381,67 +390,58 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
                 asm volatile("cp.async.wait_group 0;" ::: "memory");
                 for (int p = max(0, 2 * n - kInFlight); p < 2 * n; ++p) arrive(p);
             }
-        } else if (warp == kMmaWarp) {
+        } else if (lane == 0) {
             // ---- products ----
-            if (lane == 0) {
-                constexpr uint32_t IQK = idesc_f16(kN, false), IPV = idesc_f16(HD, true);
-                auto place = [&](int p) { return ring + static_cast<uint32_t>(p % S::slots) * S::slot; };
-                auto landed = [&](int p) { return mbar_wait_bounded(&full[p % S::slots], static_cast<uint32_t>(p / S::slots) & 1u, A.status, kStatusWaitTimeout); };
-                // the address field of a descriptor counts 16 bytes: k-steps are added to it
-                auto qk = [&](int j) {
+            auto place = [&](int p) { return ring + static_cast<uint32_t>(p % S::slots) * S::slot; };
+            auto landed = [&](int p) { return mbar_wait_bounded(&full[p % S::slots], static_cast<uint32_t>(p / S::slots) & 1u, A.status, kStatusWaitTimeout); };
+            bool ok = true;
+            // the address field of a descriptor counts 16 bytes: k-steps are added to it
+            if (warp == kQkWarp) {
+                for (int j = 0; j < n && ok && !*abort_v; ++j) {
+                    // S of block j goes where P of block j - 2 has been read. (Waiting for o_full here could miss
+                    // a phase: block j - 1 may be through by now. A buffer's own barrier waits for S of block j.)
+                    ok = landed(k_place(j)) && (j < 2 || mbar_wait_bounded(&s_free[j & 1], static_cast<uint32_t>((j >> 1) - 1) & 1u, A.status, kStatusWaitTimeout));
+                    if (!ok) break;
+                    fence_after();
                     const uint32_t d = tmem + S::s0 + static_cast<uint32_t>((j & 1) * kN);
                     const uint64_t b = desc(place(k_place(j)), 16, 1024);
 #pragma unroll 1
                     for (int part = 0; part < 2; ++part) {   // the small products first
                         const uint32_t a = tmem + (part == 0 ? S::q_lo : S::q_hi);
 #pragma unroll
-                        for (int k = 0; k < HD / 16; ++k) mma_ts(d, a + 8 * k, b + ((k >> 2) * (kN * 128) + (k & 3) * 32) / 16, IQK, part > 0 || k > 0);
+                        for (int k = 0; k < HD / 16; ++k)
+                            mma_ts(d, a + 8 * k, b + ((k >> 2) * (kN * 128) + (k & 3) * 32) / 16, idesc_f16(kN, false), part > 0 || k > 0);
                     }
-                    commit(&empty[k_place(j) % S::slots]);
                     commit(&s_full[j & 1]);
-                };
-                auto pv = [&](int j, int hf) {
-                    const uint32_t p = tmem + S::s0 + static_cast<uint32_t>((j & 1) * kN + hf * (kN / 2));
-                    const uint64_t b = desc(place(v_place(j, n)) + static_cast<uint32_t>(hf) * (kN / 2) * 128, kN * 128, 1024);
-#pragma unroll 1
-                    for (int part = 0; part < 2; ++part) {
-                        const uint32_t a = p + (part == 0 ? 32 : 0);
-#pragma unroll
-                        for (int k = 0; k < kN / 32; ++k) mma_ts(tmem + S::o, a + 8 * k, b + k * 128, IPV, hf > 0 || part > 0 || k > 0);
-                    }
-                };
-                bool ok = true;
-                for (int j = 0; j < 2 && j < n && ok; ++j) {
-                    ok = landed(k_place(j));
-                    if (!ok) break;
-                    fence_after();
-                    qk(j);
+                    commit(&empty[k_place(j) % S::slots]);
                 }
+            } else {
                 for (int j = 0; j < n && ok && !*abort_v; ++j) {
                     const uint32_t ph = static_cast<uint32_t>(j >> 1) & 1u, each = static_cast<uint32_t>(j) & 1u;
-                    ok = landed(v_place(j, n)) && (j == 0 || mbar_wait_bounded(&o_free, each ^ 1u, A.status, kStatusWaitTimeout)) &&
-                         mbar_wait_bounded(&p_full[j & 1][0], ph, A.status, kStatusWaitTimeout);
-                    if (!ok) break;
-                    fence_after();
-                    pv(j, 0);
-                    ok = mbar_wait_bounded(&p_full[j & 1][1], ph, A.status, kStatusWaitTimeout);
-                    if (!ok) break;
-                    fence_after();
-                    pv(j, 1);
-                    commit(&empty[v_place(j, n) % S::slots]);
-                    commit(&o_full);
-                    if (j + 2 < n) {
-                        // S of block j + 2 goes where P of block j has been read
-                        ok = landed(k_place(j + 2)) && mbar_wait_bounded(&o_full, each, A.status, kStatusWaitTimeout);
+                    const uint64_t b = desc(place(v_place(j, n)), kN * 128, 1024);
+                    ok = landed(v_place(j, n)) && (j == 0 || mbar_wait_bounded(&o_free, each ^ 1u, A.status, kStatusWaitTimeout));
+#pragma unroll 1
+                    for (int hf = 0; hf < 2 && ok; ++hf) {   // each half of the keys when its P is there
+                        ok = mbar_wait_bounded(&p_full[j & 1][hf], ph, A.status, kStatusWaitTimeout);
                         if (!ok) break;
                         fence_after();
-                        qk(j + 2);
+                        const uint32_t p = tmem + S::s0 + static_cast<uint32_t>((j & 1) * kN + hf * (kN / 2));
+#pragma unroll
+                        for (int part = 0; part < 2; ++part)
+#pragma unroll
+                            for (int k = 0; k < kN / 32; ++k)
+                                mma_ts(tmem + S::o, p + (part == 0 ? 32 : 0) + 8 * k, b + hf * (kN / 2) * 128 / 16 + k * 128, idesc_f16(HD, true),
+                                       hf > 0 || part > 0 || k > 0);
                     }
+                    if (!ok) break;
+                    commit(&o_full);
+                    commit(&s_free[j & 1]);
+                    commit(&empty[v_place(j, n) % S::slots]);
                 }
-                if (!ok) *abort_v = 1;
             }
-            __syncwarp();
+            if (!ok) *abort_v = 1;
         }
+        __syncwarp();
     } else {
         // ---- compute ----
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kComputeRegs));
@@ -460,22 +460,18 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
             ok = ok && mbar_wait_bounded(&o_full, static_cast<uint32_t>(j) & 1u, A.status, kStatusWaitTimeout);
             __syncwarp();
             fence_after();
+            float o[HH];
 #pragma unroll
-            for (int c = 0; c < HH / 32; ++c) {
-                float o[32];
-                ld32(tl + S::o + half * HH + c * 32, o);
-                wait_ld<32>(o);
-                if (c == HH / 32 - 1) {
-                    fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&o_free);
-                }
+            for (int c = 0; c < HH / 32; ++c) ld32(tl + S::o + half * HH + c * 32, o + c * 32);
+            wait_ld<HH>(o);
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&o_free);
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const float2 x = ffma2(make_float2(acc[c * 32 + i], acc[c * 32 + i + 1]), make_float2(alpha, alpha), make_float2(o[i], o[i + 1]));
-                    acc[c * 32 + i] = x.x;
-                    acc[c * 32 + i + 1] = x.y;
-                }
+            for (int i = 0; i < HH; i += 2) {
+                const float2 x = ffma2(make_float2(acc[i], acc[i + 1]), make_float2(alpha, alpha), make_float2(o[i], o[i + 1]));
+                acc[i] = x.x;
+                acc[i + 1] = x.y;
             }
         };
 
@@ -549,8 +545,8 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
             }
             float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int i = 4; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
-            const float mh = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            for (int i = 4; i < 60; i += 2) mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], s[i], s[i + 1]);
+            const float mh = fmax3(fmax3(mx[0], mx[1], mx[2]), fmax3(mx[3], s[60], s[61]), fmaxf(s[62], s[63]));
             s_max[buf][half][row] = mh;
             named_barrier(1 + wq, 64);   // the two warps of these rows
             float mn = fmaxf(mh, s_max[buf][half ^ 1][row]) * k;
