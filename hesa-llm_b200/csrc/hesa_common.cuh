@@ -163,6 +163,17 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
     }
 }
 
+// The same for a whole warp: one lane polls (each polling lane costs the barrier
+// a few cycles: 256 of them took 200 to 400), the others get its answer and see
+// what the barrier ordered.
+__device__ __forceinline__ bool mbar_warp_wait(uint64_t* bar, uint32_t parity, int* status, int code) {
+    int ok = 1;
+    if ((threadIdx.x & 31) == 0) ok = mbar_wait_bounded(bar, parity, status, code) ? 1 : 0;
+    ok = __shfl_sync(0xffffffffu, ok, 0);
+    __syncwarp();
+    return ok != 0;
+}
+
 __device__ __forceinline__ float half_bits_to_float(uint32_t h16) {
     return __half2float(__ushort_as_half(static_cast<unsigned short>(h16 & 0xFFFFu)));
 }

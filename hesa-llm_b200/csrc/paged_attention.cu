@@ -217,7 +217,7 @@ __device__ __forceinline__ void copy_segment(const AttnArgs& A, Ring& ring, cons
             const bool good = page >= 0 && page < A.c.n_pages;
             if (x0 == 0) {
                 if (ring.at >= S::stages && ring.ok)
-                    ring.ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ring.empty[slot], (ring.at / S::stages - 1) & 1u, A.status, kStatusWaitTimeout));
+                    ring.ok = mbar_warp_wait(&ring.empty[slot], (ring.at / S::stages - 1) & 1u, A.status, kStatusWaitTimeout);
                 if (!ring.ok) return;
             }
             uint8_t* dst = stage + ((v * hg.subs + x) * kKeyBlock + (row & 15)) * ring.row;
@@ -317,7 +317,7 @@ __device__ __forceinline__ void rows_segment(const AttnArgs& A, Ring& ring, cons
 
     for (int i0 = seg.b0; i0 < i1; i0 += hg.subs, ++ring.at) {
         const uint32_t slot = ring.at % S::stages;
-        if (ring.ok) ring.ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ring.full[slot], (ring.at / S::stages) & 1u, A.status, kStatusWaitTimeout));
+        if (ring.ok) ring.ok = mbar_warp_wait(&ring.full[slot], (ring.at / S::stages) & 1u, A.status, kStatusWaitTimeout);
         if (!ring.ok) break;
         const int i = i0 + sub;
         if (active && i < i1) {

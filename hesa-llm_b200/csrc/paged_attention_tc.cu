@@ -291,8 +291,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
             auto put = [&](int place, const CUtensorMap* map, int page, int at) {
                 const int slot = place % S::slots;
                 if (place >= S::slots && !dead)
-                    dead = !mbar_wait_bounded(&empty[slot], static_cast<uint32_t>(place / S::slots - 1) & 1u, A.status, kStatusWaitTimeout);
-                dead = __any_sync(0xffffffffu, dead);
+                    dead = !mbar_warp_wait(&empty[slot], static_cast<uint32_t>(place / S::slots - 1) & 1u, A.status, kStatusWaitTimeout);
                 if (dead) return;
                 if (lane == 0) mbar_arrive_expect_tx(&full[slot], mine);
                 __syncwarp();
@@ -352,8 +351,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
             auto put = [&](int place, const __half* pool, const int64_t (&off)[2]) {
                 const int slot = place % S::slots;
                 if (place >= S::slots && !dead)
-                    dead = !mbar_wait_bounded(&empty[slot], static_cast<uint32_t>(place / S::slots - 1) & 1u, A.status, kStatusWaitTimeout);
-                dead = __any_sync(0xffffffffu, dead);
+                    dead = !mbar_warp_wait(&empty[slot], static_cast<uint32_t>(place / S::slots - 1) & 1u, A.status, kStatusWaitTimeout);
                 if (!dead) {
                     const uint32_t dst = to + static_cast<uint32_t>(slot) * S::slot;
 #pragma unroll
@@ -457,8 +455,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
 
         // acc = acc * alpha + O of block j
         auto take = [&](int j) {
-            ok = ok && mbar_wait_bounded(&o_full, static_cast<uint32_t>(j) & 1u, A.status, kStatusWaitTimeout);
-            __syncwarp();
+            ok = ok && mbar_warp_wait(&o_full, static_cast<uint32_t>(j) & 1u, A.status, kStatusWaitTimeout);
             fence_after();
             float o[HH];
 #pragma unroll
@@ -478,8 +475,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
         for (int j = 0; j < n; ++j) {
             const int buf = j & 1;
             const int32_t j0 = kb.at(i0 + j) * kN, jh = j0 + half * (kN / 2);
-            ok = ok && mbar_wait_bounded(&s_full[buf], static_cast<uint32_t>(j >> 1) & 1u, A.status, kStatusWaitTimeout);
-            __syncwarp();
+            ok = ok && mbar_warp_wait(&s_full[buf], static_cast<uint32_t>(j >> 1) & 1u, A.status, kStatusWaitTimeout);
             fence_after();
             const uint32_t sb = tl + S::s0 + buf * kN + half * (kN / 2);
             float s[64];
@@ -510,7 +506,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
                 // cleared (paged_attention.cu). Keys past the sequence are zeros.
                 const int place = v_place(j, n);
                 uint8_t* vb = ring_ptr + static_cast<size_t>(place % S::slots) * S::slot;
-                ok = ok && mbar_wait_bounded(&full[place % S::slots], static_cast<uint32_t>(place / S::slots) & 1u, A.status, kStatusWaitTimeout);
+                ok = ok && mbar_warp_wait(&full[place % S::slots], static_cast<uint32_t>(place / S::slots) & 1u, A.status, kStatusWaitTimeout);
                 bool odd = false;
                 for (uint32_t c = threadIdx.x * 16; c < S::slot; c += kComputeWarps * 32 * 16) {
                     const uint4 w = *reinterpret_cast<const uint4*>(vb + c);
