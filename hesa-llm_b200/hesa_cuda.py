@@ -514,9 +514,13 @@ def make_layers(per_layer):
 def _want(t, dtype, what: str, device=None, dims: int | None = None):
     """A CUDA tensor of this type on `device` (None: the current one); ValueError else."""
     import torch
+    if device is None:
+        device = torch.cuda.current_device()
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == device and (dims is None or t.dim() == dims):
+        return
     if not isinstance(t, torch.Tensor) or t.dtype != dtype or not t.is_cuda:
         raise ValueError(f"{what} must be a CUDA tensor of {dtype}")
-    if t.device.index != (torch.cuda.current_device() if device is None else device):
+    if t.get_device() != device:
         raise ValueError(f"{what} is on {t.device}: every tensor must be on the current CUDA device, the cache's")
     if dims is not None and t.dim() != dims:
         raise ValueError(f"{what} must have {dims} dimensions")
@@ -530,6 +534,14 @@ def _ints(t, what: str, n: int | None = None, device=None):
     if n is not None and t.numel() != n:
         raise ValueError(f"{what} must hold {n} values")
     return t.data_ptr()
+
+
+def _stream_on(device: int, stream):
+    """The stream's handle for a call on `device`, which is the current one."""
+    if stream is None:
+        import torch
+        return torch._C._cuda_getCurrentRawStream(device) or None
+    return _stream_handle(stream)
 
 
 def _new(make, stream):
@@ -656,7 +668,7 @@ def paged_attention(cache, layer: int, batch, q, n_head: int, out=None, scale: f
         _want(workspace, torch.uint8, "workspace", dev)
     _check(lib().hesa_cuda_paged_attention(cache.ref, layer, batch.ref, qp, ldq, op, ldo, n_head,
                                            None if opts is None else ctypes.byref(opts), workspace.data_ptr(),
-                                           workspace.numel(), _stream_handle(stream)))
+                                           workspace.numel(), _stream_on(cache.device, stream)))
     return out
 
 
@@ -676,7 +688,7 @@ def rope_kv_paged(cache, layer: int, batch, q, k, v, n_head: int, rope_table=Non
         if rope_table.shape[1] != cache.head_dim or not rope_table.is_contiguous():
             raise ValueError("rope_table must be [rows, head_dim] and contiguous")
     _check(lib().hesa_cuda_rope_kv_paged(cache.ref, layer, batch.ref, qp, ldq, kp, ldk, vp, ldv, n_head, _ptr(rope_table),
-                                         0 if rope_table is None else rope_table.shape[0], _stream_handle(stream)))
+                                         0 if rope_table is None else rope_table.shape[0], _stream_on(cache.device, stream)))
 
 
 def kv_pages_workspace(cache):
@@ -708,7 +720,7 @@ def kv_reserve(cache, slots, n_new, workspace=None, stream=None) -> None:
     ws = _page_workspace(cache, workspace, stream)
     n = slots.numel()
     _check(lib().hesa_cuda_kv_reserve(cache.ref, _ints(slots, "slots", n, cache.device), _ints(n_new, "n_new", n, cache.device), n,
-                                      ws.data_ptr(), ws.numel(), _stream_handle(stream)))
+                                      ws.data_ptr(), ws.numel(), _stream_on(cache.device, stream)))
 
 
 def kv_free(cache, slots, workspace=None, stream=None) -> None:
@@ -716,7 +728,7 @@ def kv_free(cache, slots, workspace=None, stream=None) -> None:
     ws = _page_workspace(cache, workspace, stream)
     n = slots.numel()
     _check(lib().hesa_cuda_kv_free(cache.ref, _ints(slots, "slots", n, cache.device), n, ws.data_ptr(), ws.numel(),
-                                   _stream_handle(stream)))
+                                   _stream_on(cache.device, stream)))
 
 
 def kv_fork(cache, src, dst, workspace=None, stream=None) -> None:
@@ -724,14 +736,14 @@ def kv_fork(cache, src, dst, workspace=None, stream=None) -> None:
     ws = _page_workspace(cache, workspace, stream)
     n = src.numel()
     _check(lib().hesa_cuda_kv_fork(cache.ref, _ints(src, "src", n, cache.device), _ints(dst, "dst", n, cache.device), n,
-                                   ws.data_ptr(), ws.numel(), _stream_handle(stream)))
+                                   ws.data_ptr(), ws.numel(), _stream_on(cache.device, stream)))
 
 
 def kv_compact(cache, n_live=None, workspace=None, stream=None) -> None:
     """Move the pages in use to the front of the pool (hesa_cuda_kv_compact); n_live: int32 [1] for their count."""
     ws = _page_workspace(cache, workspace, stream)
     p = None if n_live is None else _ints(n_live, "n_live", 1, cache.device)
-    _check(lib().hesa_cuda_kv_compact(cache.ref, p, ws.data_ptr(), ws.numel(), _stream_handle(stream)))
+    _check(lib().hesa_cuda_kv_compact(cache.ref, p, ws.data_ptr(), ws.numel(), _stream_on(cache.device, stream)))
 
 
 def kv_copy_pages(cache, src_pages, dst_pages, workspace=None, stream=None) -> None:
@@ -740,7 +752,7 @@ def kv_copy_pages(cache, src_pages, dst_pages, workspace=None, stream=None) -> N
     n = src_pages.numel()
     _check(lib().hesa_cuda_kv_copy_pages(cache.ref, _ints(src_pages, "src_pages", n, cache.device),
                                          _ints(dst_pages, "dst_pages", n, cache.device), n, ws.data_ptr(), ws.numel(),
-                                         _stream_handle(stream)))
+                                         _stream_on(cache.device, stream)))
 
 
 def token_logprobs_workspace(n_rows: int, vocab: int, top_k: int = 0):
@@ -764,10 +776,12 @@ def token_logprobs(logits, tokens=None, top_k: int = 0, workspace=None, stream=N
     dev = logits.device.index
     tp = None if tokens is None else _ints(tokens, "tokens", n, dev)
 
+    where = logits.device
+
     def outputs():
-        f = torch.empty((2 + top_k, n), dtype=torch.float32, device="cuda")
-        return f[0], f[1], torch.empty((n, top_k), dtype=torch.int32, device="cuda"), f[2:].view(n, top_k)
-    logprob, entropy, ids, top = _new(outputs, stream)
+        return (None if tokens is None else torch.empty(n, dtype=torch.float32, device=where), torch.empty(n, dtype=torch.float32, device=where),
+                torch.empty((n, top_k), dtype=torch.int32, device=where), torch.empty((n, top_k), dtype=torch.float32, device=where))
+    logprob, entropy, ids, top = outputs() if stream is None else _new(outputs, stream)
     if workspace is None:
         workspace = _new(lambda: token_logprobs_workspace(n, vocab, top_k), stream)
     else:
@@ -775,5 +789,5 @@ def token_logprobs(logits, tokens=None, top_k: int = 0, workspace=None, stream=N
     _check(lib().hesa_cuda_token_logprobs(logits.data_ptr(), logits.stride(0) if n > 1 else vocab, n, vocab, tp, top_k,
                                           None if tokens is None else logprob.data_ptr(), entropy.data_ptr(),
                                           ids.data_ptr() if top_k else None, top.data_ptr() if top_k else None,
-                                          workspace.data_ptr(), workspace.numel(), _stream_handle(stream)))
-    return (None if tokens is None else logprob), entropy, ids, top
+                                          workspace.data_ptr(), workspace.numel(), _stream_on(dev, stream)))
+    return logprob, entropy, ids, top
