@@ -11,15 +11,18 @@
 // TMEM (512 columns): Q_hi | Q_lo (head_dim columns), two S buffers of 128
 // columns, O (head_dim columns). Q as a TMEM operand leaves all of shared memory
 // to a ring of K and V blocks and halves the operand reads of Q K^T. A buffer's
-// S is overwritten by its P where it lies: columns 64 h .. 64 h + 31 hold the
-// high halves of keys 64 h .. 64 h + 63, the next 32 columns the low halves.
+// S is overwritten by its P where it lies: columns 16 c .. 16 c + 7 hold the high
+// halves of keys 16 c .. 16 c + 15, the next 8 the low halves.
 //
-// Warps 0-7 (compute): thread (row, h) has keys 64 h .. 64 h + 63 of its row's
-// scores, and dims h * head_dim / 2 .. of its output. It takes the maximum (the
-// two threads of a row exchange theirs through shared memory), makes P, and
-// then adds the previous block's O from TMEM to its fp32 registers, rescaling
-// with one fma. O is a fresh product for every block: only 16 products are
-// summed by the tensor core, and long sums round to nearest in fp32.
+// Warps 0-3 and 4-7 (compute) take every second block each, a row a thread, with
+// their own maximum, sum and output registers, which meet at the end: while one
+// warpgroup waits for P V and adds the last O, the other makes its P. (With both
+// on the same block, 64 keys a thread, the rows' maxima had to be exchanged and
+// all eight warps wanted the same pipes at the same time: 3000 cycles a block,
+// 1.75 ms for 2048 tokens at 16384, 64 heads on 8.) A block's maximum is found in
+// a first pass over S in TMEM, P is made in a second. O is a fresh product for
+// every block, added to fp32 registers with one fma that rescales: only 16
+// products are summed by the tensor core, and long sums round to nearest.
 // One thread of warp 8 issues P V, one of warp 9 Q K^T, so that neither's waits
 // hold up the other's products. S of block j + 2 goes into the buffer
 // that held P of block j once P V of block j has completed: no pair of products
@@ -87,6 +90,29 @@ __device__ __forceinline__ void st16(uint32_t t, const uint32_t (&v)[16]) {
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(t),
         "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
         "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void st8(uint32_t t, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(t), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+__device__ __forceinline__ void ld16(uint32_t t, float* v) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(t));
+}
+__device__ __forceinline__ void st32(uint32_t t, const float* v) {
+    const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(t),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+        "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+        "r"(r[31])
         : "memory");
 }
 __device__ __forceinline__ void ld32(uint32_t t, float* v) {
@@ -162,8 +188,8 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
     using S = TcShape<HD>;
     constexpr int HH = HD / 2;   // output dims of a thread
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t full[S::slots], empty[S::slots], s_full[2], s_free[2], p_full[2][2], o_full, o_free;
-    __shared__ float s_max[2][2][kM];
+    __shared__ __align__(8) uint64_t full[S::slots], empty[S::slots], s_full[2], p_full[2][2], o_full[2], o_free;
+    __shared__ float2 s_ml[2][kM];
     __shared__ uint32_t tmem_base;
     __shared__ int abort_flag, odd_block[2], s_last;
 
@@ -204,11 +230,10 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&s_free[i], 1);
+            mbar_init(&o_full[i], 1);
             for (int h = 0; h < 2; ++h) mbar_init(&p_full[i][h], kComputeWarps / 2);
         }
-        mbar_init(&o_full, 1);
-        mbar_init(&o_free, kComputeWarps);
+        mbar_init(&o_free, kComputeWarps / 2);
         abort_flag = 0;
         odd_block[0] = odd_block[1] = -1;
         fence_mbar_init();
@@ -396,9 +421,9 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
             // the address field of a descriptor counts 16 bytes: k-steps are added to it
             if (warp == kQkWarp) {
                 for (int j = 0; j < n && ok && !*abort_v; ++j) {
-                    // S of block j goes where P of block j - 2 has been read. (Waiting for o_full here could miss
-                    // a phase: block j - 1 may be through by now. A buffer's own barrier waits for S of block j.)
-                    ok = landed(k_place(j)) && (j < 2 || mbar_wait_bounded(&s_free[j & 1], static_cast<uint32_t>((j >> 1) - 1) & 1u, A.status, kStatusWaitTimeout));
+                    // S of block j goes where P of block j - 2 has been read. (One barrier for all blocks could be a
+                    // phase ahead by now; each buffer's own is not: its next phase needs this S.)
+                    ok = landed(k_place(j)) && (j < 2 || mbar_wait_bounded(&o_full[j & 1], static_cast<uint32_t>((j >> 1) - 1) & 1u, A.status, kStatusWaitTimeout));
                     if (!ok) break;
                     fence_after();
                     const uint32_t d = tmem + S::s0 + static_cast<uint32_t>((j & 1) * kN);
@@ -428,12 +453,11 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
                         for (int part = 0; part < 2; ++part)
 #pragma unroll
                             for (int k = 0; k < kN / 32; ++k)
-                                mma_ts(tmem + S::o, p + (part == 0 ? 32 : 0) + 8 * k, b + hf * (kN / 2) * 128 / 16 + k * 128, idesc_f16(HD, true),
-                                       hf > 0 || part > 0 || k > 0);
+                                mma_ts(tmem + S::o, p + 16 * k + (part == 0 ? 8 : 0), b + hf * (kN / 2) * 128 / 16 + k * 128,
+                                       idesc_f16(HD, true), hf > 0 || part > 0 || k > 0);
                     }
                     if (!ok) break;
-                    commit(&o_full);
-                    commit(&s_free[j & 1]);
+                    commit(&o_full[j & 1]);
                     commit(&empty[v_place(j, n) % S::slots]);
                 }
             }
@@ -446,106 +470,101 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
         if (A.cap2 == 0.f) sc *= A.scale2;
         const float slope2 = A.slopes ? A.slopes[h] * 1.44269504088896341f : 0.f;
         const bool plain = A.cap2 == 0.f && !A.slopes;
-        float m = -INFINITY, l = 0.f, alpha = 0.f;
-        float acc[HH];
+        float m = -INFINITY, l = 0.f;
+        float acc[HD];
 #pragma unroll
-        for (int i = 0; i < HH; ++i) acc[i] = 0.f;
+        for (int i = 0; i < HD; ++i) acc[i] = 0.f;
         bool ok = true;   // a wait that ran out is waited for no more; the loop goes on to its end
         const RowKeys keys = mask.row(pos);
 
-        // acc = acc * alpha + O of block j
-        auto take = [&](int j) {
-            ok = ok && mbar_warp_wait(&o_full, static_cast<uint32_t>(j) & 1u, A.status, kStatusWaitTimeout);
+        for (int j = half; j < n; j += 2) {   // `half`: the warpgroup, and its S buffer
+            const int32_t j0 = kb.at(i0 + j) * kN;
+            ok = ok && mbar_warp_wait(&s_full[half], static_cast<uint32_t>(j >> 1) & 1u, A.status, kStatusWaitTimeout);
             fence_after();
-            float o[HH];
-#pragma unroll
-            for (int c = 0; c < HH / 32; ++c) ld32(tl + S::o + half * HH + c * 32, o + c * 32);
-            wait_ld<HH>(o);
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&o_free);
-#pragma unroll
-            for (int i = 0; i < HH; i += 2) {
-                const float2 x = ffma2(make_float2(acc[i], acc[i + 1]), make_float2(alpha, alpha), make_float2(o[i], o[i + 1]));
-                acc[i] = x.x;
-                acc[i + 1] = x.y;
-            }
-        };
-
-        for (int j = 0; j < n; ++j) {
-            const int buf = j & 1;
-            const int32_t j0 = kb.at(i0 + j) * kN, jh = j0 + half * (kN / 2);
-            ok = ok && mbar_warp_wait(&s_full[buf], static_cast<uint32_t>(j >> 1) & 1u, A.status, kStatusWaitTimeout);
-            fence_after();
-            const uint32_t sb = tl + S::s0 + buf * kN + half * (kN / 2);
-            float s[64];
-            ld32(sb, s);
-            ld32(sb + 32, s + 32);
-            wait_ld<64>(s);
+            const uint32_t sb = tl + S::s0 + half * kN;
             float k = sc;   // s * k is the score in base 2
             const bool whole = mask.all(p_lo, p_hi, j0, j0 + kN);
-            if (!plain) {
-                if (A.cap2 != 0.f) {
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            if (plain && whole) {
+                float s[2][32];
+                ld32(sb, s[0]);
+                wait_ld<32>(s[0]);
 #pragma unroll
-                    for (int i = 0; i < 64; ++i) s[i] = capped(s[i] * sc, A.cap2, A.cap_in);
-                } else {
+                for (int c = 0; c < 4; ++c) {
+                    if (c < 3) ld32(sb + (c + 1) * 32, s[(c + 1) & 1]);
 #pragma unroll
-                    for (int i = 0; i < 64; ++i) s[i] *= sc;
+                    for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], s[c & 1][i], s[c & 1][i + 1]);
+                    if (c < 3) wait_ld<32>(s[(c + 1) & 1]);
                 }
-                if (A.slopes) {
+            } else {
+                // the scores themselves go back into TMEM
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    float s[32];
+                    ld32(sb + c * 32, s);
+                    wait_ld<32>(s);
+                    const int32_t jc = j0 + c * 32;
+                    if (A.cap2 != 0.f) {
 #pragma unroll
-                    for (int i = 0; i < 64; ++i) s[i] -= slope2 * fabsf(static_cast<float>(pos - (jh + i)));
+                        for (int i = 0; i < 32; ++i) s[i] = capped(s[i] * sc, A.cap2, A.cap_in);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) s[i] *= sc;
+                    }
+                    if (A.slopes) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) s[i] -= slope2 * fabsf(static_cast<float>(pos - (jc + i)));
+                    }
+                    if (!whole) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) s[i] = keys.sees(jc + i) ? s[i] : -INFINITY;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], s[i], s[i + 1]);
+                    st32(sb + c * 32, s);
                 }
+                wait_st();
                 k = 1.f;
             }
             if (!whole) {
-#pragma unroll
-                for (int i = 0; i < 64; ++i) s[i] = keys.sees(jh + i) ? s[i] * k : -INFINITY;
-                k = 1.f;
                 // values of V that are not finite and hidden from some row: added where they are seen, then
-                // cleared (paged_attention.cu). Keys past the sequence are zeros.
+                // cleared (paged_attention.cu). Keys past the sequence are zeros, or what their page holds.
                 const int place = v_place(j, n);
                 uint8_t* vb = ring_ptr + static_cast<size_t>(place % S::slots) * S::slot;
                 ok = ok && mbar_warp_wait(&full[place % S::slots], static_cast<uint32_t>(place / S::slots) & 1u, A.status, kStatusWaitTimeout);
+                const uint32_t me = threadIdx.x & 127;
                 bool odd = false;
-                for (uint32_t c = threadIdx.x * 16; c < S::slot; c += kComputeWarps * 32 * 16) {
+                for (uint32_t c = me * 16; c < S::slot; c += 128 * 16) {
                     const uint4 w = *reinterpret_cast<const uint4*>(vb + c);
                     odd |= nonfinite_h2(w.x) || nonfinite_h2(w.y) || nonfinite_h2(w.z) || nonfinite_h2(w.w);
                 }
-                // a warp that is a block ahead writes the other word; none is two ahead (S of block j + 2 needs every P of j)
-                if (odd) odd_block[buf] = j;
-                named_barrier(5, kComputeWarps * 32);
-                if (*reinterpret_cast<volatile int*>(&odd_block[buf]) == j) {
+                // (no warp of the group is a block ahead: S of its next block needs every P of this one)
+                if (odd) odd_block[half] = j;
+                named_barrier(1 + half, 128);
+                if (*reinterpret_cast<volatile int*>(&odd_block[half]) == j) {
                     for (int kr = 0; kr < kN; ++kr) {
                         if (!keys.sees(j0 + kr)) continue;
 #pragma unroll
-                        for (int d8 = 0; d8 < HH / 8; ++d8) {
-                            const int d = half * HH + d8 * 8;
+                        for (int d = 0; d < HD; d += 8) {
                             const uint4 w = *reinterpret_cast<const uint4*>(vb + (d >> 6) * (kN * 128) + kr * 128 + ((((d >> 3) & 7) ^ (kr & 7)) << 4));
                             const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                             for (int i = 0; i < 8; ++i) {
                                 const float x = half_bits_to_float(ws[i >> 1] >> (16 * (i & 1)));
-                                if (!isfinite(x)) acc[d8 * 8 + i] += x;
+                                if (!isfinite(x)) acc[d + i] += x;
                             }
                         }
                     }
-                    named_barrier(5, kComputeWarps * 32);
-                    for (uint32_t c = threadIdx.x * 2; c < S::slot; c += kComputeWarps * 32 * 2) {
+                    named_barrier(1 + half, 128);
+                    for (uint32_t c = me * 2; c < S::slot; c += 128 * 2) {
                         unsigned short& x = *reinterpret_cast<unsigned short*>(vb + c);
                         if ((x & 0x7C00u) == 0x7C00u) x = 0;
                     }
                     fence_proxy_async_smem();
-                    named_barrier(5, kComputeWarps * 32);
+                    named_barrier(1 + half, 128);
                 }
             }
-            float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-            for (int i = 4; i < 60; i += 2) mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], s[i], s[i + 1]);
-            const float mh = fmax3(fmax3(mx[0], mx[1], mx[2]), fmax3(mx[3], s[60], s[61]), fmaxf(s[62], s[63]));
-            s_max[buf][half][row] = mh;
-            named_barrier(1 + wq, 64);   // the two warps of these rows
-            float mn = fmaxf(mh, s_max[buf][half ^ 1][row]) * k;
+            float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * k;
             // k is NaN for a row that is not finite: so are its maximum, its P and its result
             mn = mn > m ? mn : (mn == mn ? m : mn);
             const float ms = mn == -INFINITY ? 0.f : mn;
@@ -553,57 +572,98 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
             m = mn;
             const float off = kPShift - ms;
             float2 sum = make_float2(0.f, 0.f);
+            float s[2][16];   // the next 16 columns are on their way while these are made into P
+            ld16(sb, s[0]);
+            wait_ld<16>(s[0]);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                uint32_t hi[16], lo[16];
+            for (int c = 0; c < 8; ++c) {
+                if (c < 7) ld16(sb + (c + 1) * 16, s[(c + 1) & 1]);
+                uint32_t hi[8], lo[8];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float2 x = ffma2(make_float2(s[c * 32 + 2 * i], s[c * 32 + 2 * i + 1]), make_float2(k, k), make_float2(off, off));
+                for (int i = 0; i < 8; ++i) {
+                    const float2 x = ffma2(make_float2(s[c & 1][2 * i], s[c & 1][2 * i + 1]), make_float2(k, k), make_float2(off, off));
                     const float2 p = make_float2(ex2(x.x), ex2(x.y));
                     sum = fadd2(sum, p);
                     cut_half2(p, hi[i], lo[i]);
                 }
-                st16(sb + c * 16, hi);
-                st16(sb + 32 + c * 16, lo);
+                if (c < 7) wait_ld<16>(s[(c + 1) & 1]);   // before P goes over columns that are being read
+                st8(sb + c * 16, hi);
+                st8(sb + c * 16 + 8, lo);
+                if ((c & 3) == 3) {
+                    wait_st();
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[half][c >> 2]);
+                }
             }
             l = fmaf(l, al, sum.x + sum.y);
-            wait_st();
+            // acc = acc * al + O of this block
+            ok = ok && mbar_warp_wait(&o_full[half], static_cast<uint32_t>(j >> 1) & 1u, A.status, kStatusWaitTimeout);
+            fence_after();
+            float o[2][32];
+            ld32(tl + S::o, o[0]);
+            wait_ld<32>(o[0]);
+#pragma unroll
+            for (int c = 0; c < HD / 32; ++c) {
+                if (c + 1 < HD / 32) ld32(tl + S::o + (c + 1) * 32, o[(c + 1) & 1]);
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    const float2 x = ffma2(make_float2(acc[c * 32 + i], acc[c * 32 + i + 1]), make_float2(al, al), make_float2(o[c & 1][i], o[c & 1][i + 1]));
+                    acc[c * 32 + i] = x.x;
+                    acc[c * 32 + i + 1] = x.y;
+                }
+                if (c + 1 < HD / 32) wait_ld<32>(o[(c + 1) & 1]);
+            }
             fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[buf][half]);
-            if (j > 0) take(j - 1);
-            alpha = al;
+            if (lane == 0) mbar_arrive(&o_free);
         }
-        if (n > 0) take(n - 1);
         if (!ok) *abort_v = 1;
 
-        // the row's sum over both halves of the keys
-        named_barrier(1 + wq, 64);
-        s_max[0][half][row] = l;
-        named_barrier(1 + wq, 64);
-        l = s_max[0][0][row] + s_max[0][1][row];
+        // ---- the two warpgroups' results: each finishes half of the dims ----
+        named_barrier(3, kComputeWarps * 32);   // every block is through: the ring is read and written no more
+        s_ml[half][row] = make_float2(m, l);
+        float* xch = reinterpret_cast<float*>(ring_ptr) + static_cast<size_t>(half * kM + row) * (HH + 2);
+#pragma unroll
+        for (int i = 0; i < HH; i += 2)
+            *reinterpret_cast<float2*>(xch + i) = half == 0 ? make_float2(acc[HH + i], acc[HH + i + 1]) : make_float2(acc[i], acc[i + 1]);
+        named_barrier(3, kComputeWarps * 32);
+        const float2 other = s_ml[half ^ 1][row];
+        const float* theirs = reinterpret_cast<const float*>(ring_ptr) + static_cast<size_t>((half ^ 1) * kM + row) * (HH + 2);
+        const float M = fmaxf(m, other.x);
+        // a side that saw nothing adds zeros, or the NaN of a row that is not finite
+        const float fa = m == -INFINITY ? 1.f : ex2(m - M), fb = other.x == -INFINITY ? 1.f : ex2(other.x - M);
+        float res[HH];
+#pragma unroll
+        for (int i = 0; i < HH; i += 2) {
+            const float2 v = *reinterpret_cast<const float2*>(theirs + i);
+            res[i] = fmaf(v.x, fb, (half == 0 ? acc[i] : acc[HH + i]) * fa);
+            res[i + 1] = fmaf(v.y, fb, (half == 0 ? acc[i + 1] : acc[HH + i + 1]) * fa);
+        }
+        m = M;
+        l = fmaf(other.y, fb, l * fa);
         const int pair = static_cast<int>(blockIdx.x) * A.c.n_kv + kvh;
         float* parts = A.part + static_cast<int64_t>(pair) * A.n_split * kM * (HD + 2);
         float* o_row = A.out + static_cast<int64_t>(sv.q0 + t) * A.ldo + static_cast<int64_t>(h) * HD + half * HH;
         const bool mine = r0 + row < n_rows;
+        const float inv = l == 0.f ? 0.f : 1.f / l;   // nothing seen: zeros
         if (n_parts == 1) {
             if (mine && !*abort_v) {
 #pragma unroll
                 for (int i = 0; i < HH; i += 4)
-                    *reinterpret_cast<float4*>(o_row + i) = l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
-                                                                     : make_float4(acc[i] / l, acc[i + 1] / l, acc[i + 2] / l, acc[i + 3] / l);
+                    *reinterpret_cast<float4*>(o_row + i) = make_float4(res[i] * inv, res[i + 1] * inv, res[i + 2] * inv, res[i + 3] * inv);
             }
         } else {
             float* p = parts + (static_cast<int64_t>(split) * kM + row) * (HD + 2);
             if (half == 0) *reinterpret_cast<float2*>(p) = make_float2(m, l);
 #pragma unroll
-            for (int i = 0; i < HH; i += 2) *reinterpret_cast<float2*>(p + 2 + half * HH + i) = make_float2(acc[i], acc[i + 1]);
-            named_barrier(5, kComputeWarps * 32);
+            for (int i = 0; i < HH; i += 2) *reinterpret_cast<float2*>(p + 2 + half * HH + i) = make_float2(res[i], res[i + 1]);
+            named_barrier(3, kComputeWarps * 32);
             if (threadIdx.x == 0) {
                 cuda::atomic_ref<int32_t, cuda::thread_scope_device> c(A.counters[pair]);
                 s_last = c.fetch_add(1, cuda::memory_order_acq_rel) == n_parts - 1;
             }
-            named_barrier(5, kComputeWarps * 32);
+            named_barrier(3, kComputeWarps * 32);
             if (s_last) {
                 cuda::atomic_thread_fence(cuda::memory_order_acquire, cuda::thread_scope_device);
                 // a warp takes 16 rows, one after another: lanes along the row
