@@ -178,6 +178,23 @@ __device__ __forceinline__ void cut_half2(float2 x, uint32_t& hi, uint32_t& lo) 
     lo = *reinterpret_cast<const uint32_t*>(&b);
 }
 
+// cap2 tanh(x) for two |x| <= 0.6: tanh(x) = x + x u q(u), u = x^2, q of degree 4
+// fitted to (tanh(x) / x - 1) / u at Chebyshev nodes of u in [0, 0.36]; with its
+// coefficients in fp32 the relative error is below 1.5e-8.
+__device__ __forceinline__ float2 capped2_small(float2 x, float cap2) {
+    const float2 u = ffma2(x, x, make_float2(0.f, 0.f));
+    float2 q = make_float2(-0.006276387721f, -0.006276387721f);
+    q = ffma2(q, u, make_float2(0.021116213873f, 0.021116213873f));
+    q = ffma2(q, u, make_float2(-0.053875137120f, -0.053875137120f));
+    q = ffma2(q, u, make_float2(0.133329242468f, 0.133329242468f));
+    q = ffma2(q, u, make_float2(-0.333333313465f, -0.333333313465f));
+    const float2 y = ffma2(x, make_float2(cap2, cap2), make_float2(0.f, 0.f));
+    return ffma2(y, ffma2(u, q, make_float2(0.f, 0.f)), y);
+}
+
+// The low n bits set, 0 <= n <= 32 or clamped to that.
+__device__ __forceinline__ uint32_t low_bits(int32_t n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+
 // Places in the ring: K0, K1, V0, K2, V1, ... , the order in which they are used.
 __device__ __forceinline__ int k_place(int j) { return j == 0 ? 0 : 2 * j - 1; }
 __device__ __forceinline__ int v_place(int j, int n) { return j + 1 < n ? 2 * j + 2 : 2 * n - 1; }
@@ -188,7 +205,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
     using S = TcShape<HD>;
     constexpr int HH = HD / 2;   // output dims of a thread
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t full[S::slots], empty[S::slots], s_full[2], p_full[2][2], o_full[2], o_free;
+    __shared__ __align__(8) uint64_t full[S::slots], empty[S::slots], s_full[2], p_full[2][2], o_full[2], o_free, q_done;
     __shared__ float2 s_ml[2][kM];
     __shared__ uint32_t tmem_base;
     __shared__ int abort_flag, odd_block[2], s_last;
@@ -223,6 +240,23 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
     uint8_t* ring_ptr = smem_raw + (ring - smem_addr(smem_raw));
     volatile int* abort_v = &abort_flag;
 
+    // q comes through the last slots of the ring, whole rows at a time (a thread that
+    // read its own row from memory waited 7 us for rows 16 KB apart), 16-byte pieces
+    // swizzled by the row so that a row a thread is read without bank conflicts
+    constexpr int kQSlots = 2;
+    static_assert(kM * HD * 4 == kQSlots * S::slot, "q fills whole slots");
+    uint8_t* q_smem = ring_ptr + (S::slots - kQSlots) * S::slot;
+    if (warp < kComputeWarps) {
+        constexpr int PIECES = HD / 4;
+#pragma unroll
+        for (int i = 0; i < kM * PIECES / (kComputeWarps * 32); ++i) {
+            const int p = i * kComputeWarps * 32 + threadIdx.x, qr = p / PIECES, c = p % PIECES;
+            const int rr = min(r0 + qr, n_rows - 1), qt = A.group_div.div(rr);
+            const float* src = A.q + static_cast<int64_t>(sv.q0 + qt) * A.ldq + static_cast<int64_t>(kvh * A.group + rr - qt * A.group) * HD + c * 4;
+            cp16(smem_addr(q_smem) + qr * HD * 4 + ((c ^ (qr & 7)) << 4), src, true);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::slots; ++i) {
             mbar_init(&full[i], kProducerWarps);
@@ -234,6 +268,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
             for (int h = 0; h < 2; ++h) mbar_init(&p_full[i][h], kComputeWarps / 2);
         }
         mbar_init(&o_free, kComputeWarps / 2);
+        mbar_init(&q_done, kComputeWarps);
         abort_flag = 0;
         odd_block[0] = odd_block[1] = -1;
         fence_mbar_init();
@@ -247,46 +282,12 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
     fence_after();
     const uint32_t tmem = tmem_base;
 
-    // ---- compute warps: q into TMEM ----
     const int half = warp >> 2, wq = warp & 3;
     const int row = 32 * wq + lane;                       // of the tile, = TMEM lane
     const uint32_t tl = tmem + (static_cast<uint32_t>(32 * wq) << 16);
     const int r = min(r0 + row, n_rows - 1);
     const int t = A.group_div.div(r), h = kvh * A.group + r - t * A.group;
     const int32_t pos = base + t;
-    float sc = 0.f;
-    if (warp < kComputeWarps) {
-        const float4* q = reinterpret_cast<const float4*>(A.q + static_cast<int64_t>(sv.q0 + t) * A.ldq + static_cast<int64_t>(h) * HD);
-        float mx = 0.f;
-#pragma unroll 8
-        for (int i = 0; i < HD / 4; ++i) {
-            const float4 v = q[i];
-            mx = fmax_nan(mx, fmax_nan(fmax_nan(fabsf(v.x), fabsf(v.y)), fmax_nan(fabsf(v.z), fabsf(v.w))));
-        }
-        // q = 2^e (hi + lo) with the largest |hi| in [2^14, 2^15)
-        const bool fin = mx < INFINITY;
-        int e = 0;
-        if (fin && mx > 0.f) e = max(ilogbf(mx) - 14, -120);
-        const float f1 = ldexpf(1.f, -(e / 2)), f2 = fin ? ldexpf(1.f, -(e - e / 2)) : 0.f;
-        sc = fin ? ldexpf(1.f, e) : NAN;
-#pragma unroll
-        for (int c = 0; c < HH / 32; ++c) {   // 32 dims of this thread's half: 16 columns
-            uint32_t hi[16], lo[16];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float4 v = q[half * HH / 4 + c * 8 + i];
-                if (!fin) v = make_float4(0.f, 0.f, 0.f, 0.f);
-                split_half2(v.x * f1 * f2, v.y * f1 * f2, hi[2 * i], lo[2 * i]);
-                split_half2(v.z * f1 * f2, v.w * f1 * f2, hi[2 * i + 1], lo[2 * i + 1]);
-            }
-            st16(tl + S::q_hi + half * HH / 2 + c * 16, hi);
-            st16(tl + S::q_lo + half * HH / 2 + c * 16, lo);
-        }
-        wait_st();
-    }
-    fence_before();
-    __syncthreads();
-    fence_after();
 
     if (warp >= kComputeWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
@@ -317,6 +318,8 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
                 const int slot = place % S::slots;
                 if (place >= S::slots && !dead)
                     dead = !mbar_warp_wait(&empty[slot], static_cast<uint32_t>(place / S::slots - 1) & 1u, A.status, kStatusWaitTimeout);
+                else if (place >= S::slots - kQSlots && !dead)
+                    dead = !mbar_warp_wait(&q_done, 0u, A.status, kStatusWaitTimeout);
                 if (dead) return;
                 if (lane == 0) mbar_arrive_expect_tx(&full[slot], mine);
                 __syncwarp();
@@ -377,6 +380,8 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
                 const int slot = place % S::slots;
                 if (place >= S::slots && !dead)
                     dead = !mbar_warp_wait(&empty[slot], static_cast<uint32_t>(place / S::slots - 1) & 1u, A.status, kStatusWaitTimeout);
+                else if (place >= S::slots - kQSlots && !dead)
+                    dead = !mbar_warp_wait(&q_done, 0u, A.status, kStatusWaitTimeout);
                 if (!dead) {
                     const uint32_t dst = to + static_cast<uint32_t>(slot) * S::slot;
 #pragma unroll
@@ -420,6 +425,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
             bool ok = true;
             // the address field of a descriptor counts 16 bytes: k-steps are added to it
             if (warp == kQkWarp) {
+                if (n > 0) ok = mbar_wait_bounded(&q_done, 0u, A.status, kStatusWaitTimeout);
                 for (int j = 0; j < n && ok && !*abort_v; ++j) {
                     // S of block j goes where P of block j - 2 has been read. (One barrier for all blocks could be a
                     // phase ahead by now; each buffer's own is not: its next phase needs this S.)
@@ -467,6 +473,43 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
     } else {
         // ---- compute ----
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kComputeRegs));
+        // ---- q as hi and lo halves into TMEM ----
+        float sc;
+        {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            named_barrier(3, kComputeWarps * 32);
+            auto q4 = [&](int i) { return *reinterpret_cast<const float4*>(q_smem + row * HD * 4 + ((i ^ (row & 7)) << 4)); };
+            float mx = 0.f;
+#pragma unroll 8
+            for (int i = 0; i < HD / 4; ++i) {
+                const float4 v = q4(i);
+                mx = fmax_nan(mx, fmax_nan(fmax_nan(fabsf(v.x), fabsf(v.y)), fmax_nan(fabsf(v.z), fabsf(v.w))));
+            }
+            // q = 2^e (hi + lo) with the largest |hi| in [2^14, 2^15)
+            const bool fin = mx < INFINITY;
+            int e = 0;
+            if (fin && mx > 0.f) e = max(ilogbf(mx) - 14, -120);
+            const float f1 = ldexpf(1.f, -(e / 2)), f2 = fin ? ldexpf(1.f, -(e - e / 2)) : 0.f;
+            sc = fin ? ldexpf(1.f, e) : NAN;
+#pragma unroll
+            for (int c = 0; c < HH / 32; ++c) {   // 32 dims of this thread's half: 16 columns
+                uint32_t hi[16], lo[16];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float4 v = q4(half * HH / 4 + c * 8 + i);
+                    if (!fin) v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    split_half2(v.x * f1 * f2, v.y * f1 * f2, hi[2 * i], lo[2 * i]);
+                    split_half2(v.z * f1 * f2, v.w * f1 * f2, hi[2 * i + 1], lo[2 * i + 1]);
+                }
+                st16(tl + S::q_hi + half * HH / 2 + c * 16, hi);
+                st16(tl + S::q_lo + half * HH / 2 + c * 16, lo);
+            }
+            wait_st();
+            fence_before();
+            fence_proxy_async_smem();   // the slots are filled by the async proxy next
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_done);
+        }
         if (A.cap2 == 0.f) sc *= A.scale2;
         const float slope2 = A.slopes ? A.slopes[h] * 1.44269504088896341f : 0.f;
         const bool plain = A.cap2 == 0.f && !A.slopes;
@@ -504,20 +547,40 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
                     ld32(sb + c * 32, s);
                     wait_ld<32>(s);
                     const int32_t jc = j0 + c * 32;
+                    const float dist = static_cast<float>(pos - jc);   // exact below 2^24, else to 24 bits
                     if (A.cap2 != 0.f) {
+                        const float x1 = sc * A.cap_in;
+                        float far = 0.f;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) s[i] = capped(s[i] * sc, A.cap2, A.cap_in);
+                        for (int i = 0; i < 32; i += 2) {
+                            const float2 x = ffma2(make_float2(s[i], s[i + 1]), make_float2(x1, x1), make_float2(0.f, 0.f));
+                            s[i] = x.x;
+                            s[i + 1] = x.y;
+                            far = fmax3(far, fabsf(x.x), fabsf(x.y));
+                        }
+                        if (__any_sync(0xffffffffu, far > 0.6f)) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) s[i] = A.cap2 * tanhf(s[i]);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; i += 2) {
+                                const float2 y = capped2_small(make_float2(s[i], s[i + 1]), A.cap2);
+                                s[i] = y.x;
+                                s[i + 1] = y.y;
+                            }
+                        }
                     } else {
 #pragma unroll
                         for (int i = 0; i < 32; ++i) s[i] *= sc;
                     }
                     if (A.slopes) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) s[i] -= slope2 * fabsf(static_cast<float>(pos - (jc + i)));
+                        for (int i = 0; i < 32; ++i) s[i] = fmaf(-slope2, fabsf(dist - static_cast<float>(i)), s[i]);
                     }
                     if (!whole) {
+                        const uint32_t seen = (low_bits(keys.hi - jc) & ~low_bits(keys.lo - jc)) | low_bits(keys.prefix - jc);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) s[i] = keys.sees(jc + i) ? s[i] : -INFINITY;
+                        for (int i = 0; i < 32; ++i) s[i] = seen >> i & 1u ? s[i] : -INFINITY;
                     }
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], s[i], s[i + 1]);
@@ -643,21 +706,32 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
         m = M;
         l = fmaf(other.y, fb, l * fa);
         const int pair = static_cast<int>(blockIdx.x) * A.c.n_kv + kvh;
-        float* parts = A.part + static_cast<int64_t>(pair) * A.n_split * kM * (HD + 2);
-        float* o_row = A.out + static_cast<int64_t>(sv.q0 + t) * A.ldo + static_cast<int64_t>(h) * HD + half * HH;
-        const bool mine = r0 + row < n_rows;
-        const float inv = l == 0.f ? 0.f : 1.f / l;   // nothing seen: zeros
-        if (n_parts == 1) {
-            if (mine && !*abort_v) {
+        constexpr int64_t kPart = kM * (HD + 2);   // floats of a part: acc [kM][HD], then (m, l) [kM]
+        float* parts = A.part + static_cast<int64_t>(pair) * A.n_split * kPart;
+        const float inv = n_parts > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;   // nothing seen: zeros
+        // through shared memory, so that whole rows are written
+        uint8_t* o_smem = ring_ptr + ((2 * kM * (HH + 2) * 4 + 1023) & ~1023);
 #pragma unroll
-                for (int i = 0; i < HH; i += 4)
-                    *reinterpret_cast<float4*>(o_row + i) = make_float4(res[i] * inv, res[i + 1] * inv, res[i + 2] * inv, res[i + 3] * inv);
+        for (int i = 0; i < HH / 4; ++i)
+            *reinterpret_cast<float4*>(o_smem + row * HD * 4 + (((half * (HH / 4) + i) ^ (row & 7)) << 4)) =
+                make_float4(res[4 * i] * inv, res[4 * i + 1] * inv, res[4 * i + 2] * inv, res[4 * i + 3] * inv);
+        named_barrier(3, kComputeWarps * 32);
+        if (!*abort_v) {
+            constexpr int PIECES = HD / 4;
+            float* part = parts + split * kPart;
+#pragma unroll 4
+            for (int i = 0; i < kM * PIECES / (kComputeWarps * 32); ++i) {
+                const int p = i * kComputeWarps * 32 + threadIdx.x, orow = p / PIECES, c = p % PIECES, rr = r0 + orow;
+                if (rr >= n_rows) break;   // rows rise with i
+                const float4 v = *reinterpret_cast<const float4*>(o_smem + orow * HD * 4 + ((c ^ (orow & 7)) << 4));
+                const int ot = A.group_div.div(rr);
+                float* dst = n_parts > 1 ? part + orow * HD
+                                         : A.out + static_cast<int64_t>(sv.q0 + ot) * A.ldo + static_cast<int64_t>(kvh * A.group + rr - ot * A.group) * HD;
+                *reinterpret_cast<float4*>(dst + c * 4) = v;
             }
-        } else {
-            float* p = parts + (static_cast<int64_t>(split) * kM + row) * (HD + 2);
-            if (half == 0) *reinterpret_cast<float2*>(p) = make_float2(m, l);
-#pragma unroll
-            for (int i = 0; i < HH; i += 2) *reinterpret_cast<float2*>(p + 2 + half * HH + i) = make_float2(res[i], res[i + 1]);
+        }
+        if (n_parts > 1) {
+            if (half == 0) *reinterpret_cast<float2*>(parts + split * kPart + kM * HD + row * 2) = make_float2(m, l);
             named_barrier(3, kComputeWarps * 32);
             if (threadIdx.x == 0) {
                 cuda::atomic_ref<int32_t, cuda::thread_scope_device> c(A.counters[pair]);
@@ -668,20 +742,21 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
                 cuda::atomic_thread_fence(cuda::memory_order_acquire, cuda::thread_scope_device);
                 // a warp takes 16 rows, one after another: lanes along the row
                 for (int rr = warp; rr < kM && r0 + rr < n_rows; rr += kComputeWarps) {
-                    const float* p0 = parts + static_cast<int64_t>(rr) * (HD + 2);
-                    constexpr int64_t step = kM * (HD + 2);
+                    const float* ml = parts + kM * HD + rr * 2;
+                    const float* p0 = parts + static_cast<int64_t>(rr) * HD + lane;
                     float M = -INFINITY;
-                    for (int i = 0; i < n_parts; ++i) M = fmaxf(M, __ldcg(p0 + i * step));
+                    for (int i = 0; i < n_parts; ++i) M = fmaxf(M, __ldcg(ml + i * kPart));
                     float L = 0.f, O[HD / 32];
 #pragma unroll
                     for (int d = 0; d < HD / 32; ++d) O[d] = 0.f;
+#pragma unroll 4
                     for (int i = 0; i < n_parts; ++i) {
-                        const float mi = __ldcg(p0 + i * step);
+                        const float mi = __ldcg(ml + i * kPart);
                         // a part that saw nothing adds zeros, or the NaN of a row that is not finite
                         const float f = mi == -INFINITY ? 1.f : ex2(mi - M);
-                        L = fmaf(__ldcg(p0 + i * step + 1), f, L);
+                        L = fmaf(__ldcg(ml + i * kPart + 1), f, L);
 #pragma unroll
-                        for (int d = 0; d < HD / 32; ++d) O[d] = fmaf(__ldcg(p0 + i * step + 2 + d * 32 + lane), f, O[d]);
+                        for (int d = 0; d < HD / 32; ++d) O[d] = fmaf(__ldcg(p0 + i * kPart + d * 32), f, O[d]);
                     }
                     const int rt = A.group_div.div(r0 + rr), rh = kvh * A.group + (r0 + rr) - rt * A.group;
                     float* o = A.out + static_cast<int64_t>(sv.q0 + rt) * A.ldo + static_cast<int64_t>(rh) * HD;
