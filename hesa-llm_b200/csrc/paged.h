@@ -163,7 +163,6 @@ struct AttnArgs {
     const float* slopes;           // [n_head] or null
     const int32_t* prefix;         // [n_seq] or null
     int* status;
-    int32_t* counters;             // [kAttnPairs], left at zero
     float* part;                   // m, l, acc of rows that are added up later
     int32_t per_seq;               // tiles of every sequence, 0: by q_start
     int32_t blocks_per_split;      // chunk_kernel: keys of a split
@@ -171,11 +170,9 @@ struct AttnArgs {
     int32_t tile0;                 // rows_kernel: the first of them
 };
 
-// (tile, kv head) pairs that may be split over the keys: one arrival counter
-// each, in a region of the same size for every shape, so that calls of
-// different shapes can share a workspace.
+// (tile, kv head) pairs that may be split over the keys: more of them load every
+// SM as they are.
 constexpr int kPagedPairs = 4096;
-constexpr size_t kPagedCounterBytes = kPagedPairs * sizeof(int32_t);
 
 // The largest P is 2^kPShift before its split into fp16 halves: the low half of
 // a P down to 2^-28 of the row's largest is then still a normal or nearly

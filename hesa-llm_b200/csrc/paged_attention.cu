@@ -53,6 +53,11 @@ constexpr int kRowTile = 8;
 constexpr int kKeyBlock = 16;
 constexpr int kRowsCtas = 148;       // one an SM
 constexpr int kCopyWarps = 4;        // a warp gets no more than one bulk copy under way in about 45 ns
+// Rows of a sequence from which on 128-row tiles are used, though they may be
+// empty for the most part, rather than several tiles of 8 that each read K and V:
+// eight sequences of 4000 tokens (64 heads on 8) with 16 rows: 31 us here, 40
+// there; with 32 rows 45 and 43; with 64 82 and 48.
+constexpr int kMostRows = 16;
 constexpr int kMostTiles = 1024;     // of a launch: the tiles' blocks are summed in shared memory
 constexpr int kSegCost = 5;          // stages that starting a (tile, group) takes the time of
 constexpr int kLeastUnits = 4;       // of a run
@@ -632,7 +637,7 @@ Plan make_plan(const hesa_cuda_paged_kv* kv, const hesa_cuda_token_batch* b, int
     Plan p{};
     const int g = static_cast<int>(n_head / kv->n_kv_head);
     const int64_t rows_a_seq = static_cast<int64_t>(b->max_new) * g;
-    p.tc = kv->head_dim <= 128 && rows_a_seq > 4 * kRowTile;
+    p.tc = kv->head_dim <= 128 && rows_a_seq > kMostRows;
     p.rows = p.tc ? kTcRows : kRowTile;
     const int64_t most = (rows_a_seq + p.rows - 1) / p.rows;
     const int64_t bound = tile_bound(b->n_tokens, b->n_seq, g, p.rows);
@@ -650,12 +655,12 @@ Plan make_plan(const hesa_cuda_paged_kv* kv, const hesa_cuda_token_batch* b, int
         while (p.heads > 2 && tiles * ((kv->n_kv_head + p.heads - 1) / p.heads) * blocks < 2 * kRowsCtas) p.heads /= 2;
         return p;
     }
-    // one CTA an SM, no split under 512 keys
+    // one CTA an SM, no split under 256 keys
     const int64_t blocks = std::max<int64_t>(1, (b->max_len + kTcKeys - 1) / kTcKeys);
     int64_t per = blocks;
     if (pairs <= kPagedPairs) {
         const int64_t want = std::max<int64_t>(1, 148 / pairs);
-        per = std::max<int64_t>(4, (blocks + want - 1) / want);
+        per = std::max<int64_t>(2, (blocks + want - 1) / want);
     }
     p.blocks_per_split = static_cast<int>(std::min(per, blocks));
     p.n_split = static_cast<int>((blocks + p.blocks_per_split - 1) / p.blocks_per_split);
@@ -761,7 +766,7 @@ extern "C" {
 size_t hesa_cuda_paged_attention_workspace_size(const hesa_cuda_paged_kv* kv, const hesa_cuda_token_batch* batch, int64_t n_head) {
     if (check_paged_kv(kv) != HESA_CUDA_OK || check_batch(kv, 0, batch, n_head) != HESA_CUDA_OK) return 0;
     const Plan p = make_plan(kv, batch, n_head);
-    return kPagedCounterBytes + part_bytes(p, kv);
+    return std::max<size_t>(part_bytes(p, kv), 16);
 }
 
 int hesa_cuda_paged_attention(const hesa_cuda_paged_kv* kv, int32_t layer, const hesa_cuda_token_batch* batch, const float* q,
@@ -805,8 +810,7 @@ int hesa_cuda_paged_attention(const hesa_cuda_paged_kv* kv, int32_t layer, const
     a.window = o.window;
     a.slopes = o.slopes;
     a.prefix = o.prefix;
-    a.counters = static_cast<int32_t*>(workspace);
-    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kPagedCounterBytes);
+    a.part = static_cast<float*>(workspace);
     a.per_seq = p.per_seq;
     a.blocks_per_split = p.blocks_per_split;
     a.n_split = p.n_split;

@@ -41,8 +41,7 @@
 
 #include <cuda.h>
 #include <cudaTypedefs.h>
-#include <cuda/atomic>
-
+#include <algorithm>
 #include <numeric>
 
 namespace hesa_cuda {
@@ -208,7 +207,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
     __shared__ __align__(8) uint64_t full[S::slots], empty[S::slots], s_full[2], p_full[2][2], o_full[2], o_free, q_done;
     __shared__ float2 s_ml[2][kM];
     __shared__ uint32_t tmem_base;
-    __shared__ int abort_flag, odd_block[2], s_last;
+    __shared__ int abort_flag, odd_block[2];
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int kvh = blockIdx.y, split = blockIdx.z;
@@ -732,42 +731,6 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
         }
         if (n_parts > 1) {
             if (half == 0) *reinterpret_cast<float2*>(parts + split * kPart + kM * HD + row * 2) = make_float2(m, l);
-            named_barrier(3, kComputeWarps * 32);
-            if (threadIdx.x == 0) {
-                cuda::atomic_ref<int32_t, cuda::thread_scope_device> c(A.counters[pair]);
-                s_last = c.fetch_add(1, cuda::memory_order_acq_rel) == n_parts - 1;
-            }
-            named_barrier(3, kComputeWarps * 32);
-            if (s_last) {
-                cuda::atomic_thread_fence(cuda::memory_order_acquire, cuda::thread_scope_device);
-                // a warp takes 16 rows, one after another: lanes along the row
-                for (int rr = warp; rr < kM && r0 + rr < n_rows; rr += kComputeWarps) {
-                    const float* ml = parts + kM * HD + rr * 2;
-                    const float* p0 = parts + static_cast<int64_t>(rr) * HD + lane;
-                    float M = -INFINITY;
-                    for (int i = 0; i < n_parts; ++i) M = fmaxf(M, __ldcg(ml + i * kPart));
-                    float L = 0.f, O[HD / 32];
-#pragma unroll
-                    for (int d = 0; d < HD / 32; ++d) O[d] = 0.f;
-#pragma unroll 4
-                    for (int i = 0; i < n_parts; ++i) {
-                        const float mi = __ldcg(ml + i * kPart);
-                        // a part that saw nothing adds zeros, or the NaN of a row that is not finite
-                        const float f = mi == -INFINITY ? 1.f : ex2(mi - M);
-                        L = fmaf(__ldcg(ml + i * kPart + 1), f, L);
-#pragma unroll
-                        for (int d = 0; d < HD / 32; ++d) O[d] = fmaf(__ldcg(p0 + i * kPart + d * 32), f, O[d]);
-                    }
-                    const int rt = A.group_div.div(r0 + rr), rh = kvh * A.group + (r0 + rr) - rt * A.group;
-                    float* o = A.out + static_cast<int64_t>(sv.q0 + rt) * A.ldo + static_cast<int64_t>(rh) * HD;
-#pragma unroll
-                    for (int d = 0; d < HD / 32; ++d) o[d * 32 + lane] = L == 0.f ? 0.f : O[d] / L;
-                }
-                if (threadIdx.x == 0) {
-                    cuda::atomic_ref<int32_t, cuda::thread_scope_device> c(A.counters[pair]);
-                    c.store(0, cuda::memory_order_relaxed);
-                }
-            }
         }
     }
     fence_before();
@@ -776,6 +739,65 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
+}
+
+// Adds the parts of a tile that was split over the keys, in their order: a warp a
+// row, eight rows a block.
+template <int HD>
+__global__ void __launch_bounds__(256)
+combine_kernel(const __grid_constant__ AttnArgs A) {
+    constexpr int64_t kPart = kM * (HD + 2);
+    constexpr int V = HD / 32, AHEAD = 8;   // values of a lane; parts whose loads are under way
+    const int lane = threadIdx.x & 31, kvh = blockIdx.y;
+    int seq, tile;
+    locate_tile(A.b, A.group, kM, A.per_seq, static_cast<int>(blockIdx.x), seq, tile);   // chunk_kernel has waited for the batch
+    const SeqView sv = seq_view(A.c, A.b, seq);
+    const int n_rows = sv.n_new * A.group;
+    const int r0 = ((n_rows + kM - 1) / kM - 1 - tile) * kM, base = sv.len - sv.n_new;
+    const int row = blockIdx.z * 8 + (threadIdx.x >> 5), r = r0 + row;
+    if (!sv.ok || tile * kM >= n_rows || r >= n_rows) return;
+    Mask mask{sv.len, A.window, 0};
+    if (A.prefix) mask.prefix = max(0, min(A.prefix[seq], sv.len));
+    const KeyBlocks kb = key_blocks(mask, base + A.group_div.div(r0), base + A.group_div.div(min(r0 + kM - 1, n_rows - 1)), kN);
+    const int n = max(1, (kb.n + A.blocks_per_split - 1) / A.blocks_per_split);
+    if (n == 1) return;
+    grid_dep_wait();
+    const int64_t pair = static_cast<int64_t>(blockIdx.x) * A.c.n_kv + kvh;
+    const float* parts = A.part + pair * A.n_split * kPart;
+    const float* ml = parts + kM * HD + row * 2;
+    const float* acc = parts + static_cast<int64_t>(row) * HD + lane * V;
+    float M = -INFINITY;
+    for (int i = lane; i < n; i += 32) M = fmaxf(M, __ldcg(ml + i * kPart));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    float L = 0.f, O[V];
+#pragma unroll
+    for (int c = 0; c < V; ++c) O[c] = 0.f;
+    for (int i0 = 0; i0 < n; i0 += AHEAD) {
+        float2 p[AHEAD];
+        float v[AHEAD][V];
+#pragma unroll
+        for (int x = 0; x < AHEAD; ++x) {
+            if (i0 + x >= n) break;
+            p[x] = __ldcg(reinterpret_cast<const float2*>(ml + (i0 + x) * kPart));
+            if constexpr (V == 2) *reinterpret_cast<float2*>(v[x]) = __ldcg(reinterpret_cast<const float2*>(acc + (i0 + x) * kPart));
+            else *reinterpret_cast<float4*>(v[x]) = __ldcg(reinterpret_cast<const float4*>(acc + (i0 + x) * kPart));
+        }
+#pragma unroll
+        for (int x = 0; x < AHEAD; ++x) {
+            if (i0 + x >= n) break;
+            // a part that saw nothing adds zeros, or the NaN of a row that is not finite
+            const float f = p[x].x == -INFINITY ? 1.f : ex2(p[x].x - M);
+            L = fmaf(p[x].y, f, L);
+#pragma unroll
+            for (int c = 0; c < V; ++c) O[c] = fmaf(v[x][c], f, O[c]);
+        }
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    const int t = A.group_div.div(r);
+    float* o = A.out + static_cast<int64_t>(sv.q0 + t) * A.ldo + static_cast<int64_t>(kvh * A.group + r - t * A.group) * HD + lane * V;
+#pragma unroll
+    for (int c = 0; c < V; c += 2) *reinterpret_cast<float2*>(o + c) = make_float2(O[c] * inv, O[c + 1] * inv);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
@@ -814,7 +836,10 @@ cudaError_t launch(const AttnArgs& a, int tiles, int box, cudaStream_t s) {
     CUtensorMap k{}, v{};
     if (TMA && (!encode_pool(&k, a.c.k, a.c, box) || !encode_pool(&v, a.c.v, a.c, box))) return cudaErrorInvalidValue;
     const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(a.c.n_kv), static_cast<unsigned>(a.n_split));
-    return launch_dep(chunk_kernel<HD, TMA>, grid, kThreads, TcShape<HD>::smem, s, a, k, v, box);
+    e = launch_dep(chunk_kernel<HD, TMA>, grid, kThreads, TcShape<HD>::smem, s, a, k, v, box);
+    if (e != cudaSuccess || a.n_split == 1) return e;
+    const unsigned eights = static_cast<unsigned>((std::min(kM, a.b.max_new * a.group) + 7) / 8);
+    return launch_dep(combine_kernel<HD>, dim3(grid.x, grid.y, eights), 256, 0, s, a);
 }
 
 }  // namespace

@@ -631,13 +631,13 @@ def _same_device(cache, batch=None):
 
 
 def paged_attention_workspace(cache, batch, n_head: int):
-    """A zero-filled workspace for paged_attention of this batch's bounds (and of any smaller ones)."""
+    """A workspace for paged_attention of batches of these bounds."""
     import torch
     _same_device(cache, batch)
     nb = int(lib().hesa_cuda_paged_attention_workspace_size(cache.ref, batch.ref, n_head))
     if nb == 0:
         raise HesaError(6, lib().hesa_cuda_last_error().decode())
-    return torch.zeros(nb, dtype=torch.uint8, device="cuda")
+    return torch.empty(nb, dtype=torch.uint8, device="cuda")
 
 
 def paged_attention(cache, layer: int, batch, q, n_head: int, out=None, scale: float | None = None, softcap: float = 0.0,

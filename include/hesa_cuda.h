@@ -384,10 +384,9 @@ typedef struct {
  * see (padding, other sequences, places past a slot's length) do not reach
  * it, whatever they hold; a value that is not finite where it is seen gives a
  * result that is not finite. A row of q that is not finite gives NaN.
- * The workspace (16-byte aligned, zero-filled once before its first use;
- * every successful call leaves it usable) can be shared by calls of any shape
- * on one stream, up to the largest size that the shapes ask for, and not by
- * calls that may overlap. Results do not depend on what else runs. */
+ * The workspace (16-byte aligned, need not be set) is scratch: calls of any
+ * shape on one stream can share one of the largest size that they ask for,
+ * calls that may overlap cannot. Results do not depend on scheduling. */
 HESA_CUDA_API size_t hesa_cuda_paged_attention_workspace_size(const hesa_cuda_paged_kv* kv,
                                                               const hesa_cuda_token_batch* batch, int64_t n_head);
 HESA_CUDA_API int hesa_cuda_paged_attention(const hesa_cuda_paged_kv* kv, int32_t layer,
@@ -455,8 +454,9 @@ HESA_CUDA_API int hesa_cuda_kv_copy_pages(const hesa_cuda_paged_kv* kv, const in
  * added to the entropy. A row of nothing else gives -inf, entropy 0 and the
  * first ids; a row with NaN or +inf gives NaN (ids as if NaN were -inf). Token
  * -1 asks for nothing and gives 0; another one outside [0, vocab) gives NaN
- * and device status 3. The workspace is as hesa_cuda_paged_attention's (16-byte
- * aligned, zero-filled once, shared by calls of any shape on one stream). */
+ * and device status 3. The workspace (16-byte aligned, zero-filled once before
+ * its first use; every successful call leaves it usable) can be shared by
+ * calls of any shape on one stream, and not by calls that may overlap. */
 HESA_CUDA_API size_t hesa_cuda_token_logprobs_workspace_size(int64_t n_rows, int64_t vocab, int32_t top_k);
 HESA_CUDA_API int hesa_cuda_token_logprobs(const float* logits, int64_t ld, int64_t n_rows, int64_t vocab,
                                            const int32_t* tokens, int32_t top_k, float* logprob, float* entropy,

@@ -66,11 +66,13 @@ def test_nothing_to_attend_is_no_launch():
     assert attend(b=batch(n_tokens=0, max_new=0)) == 0
 
 
-def test_attention_workspace_grows_with_the_split_and_not_with_the_step():
+def test_attention_workspace_follows_the_cut():
+    """Next tokens: the parts of one grid, whatever the lengths. Chunks: parts where the keys are split, few bytes where not."""
     size = lambda **kw: H.lib().hesa_cuda_paged_attention_workspace_size(  # noqa: E731
         ctypes.byref(cache(max_pages=1 << 20)), ctypes.byref(batch(**kw)), 4)
-    one = size(n_seq=1, n_tokens=1, max_new=1, max_len=1 << 20)
-    assert size(n_seq=1, n_tokens=1, max_new=1, max_len=64) < one < 64 << 20
+    assert size(n_seq=1, n_tokens=1, max_new=1, max_len=64) == size(n_seq=3, n_tokens=3, max_new=1, max_len=1 << 20) < 16 << 20
+    assert size(n_seq=1, n_tokens=64, max_new=64, max_len=256) < size(n_seq=1, n_tokens=64, max_new=64, max_len=1 << 20) < 64 << 20
+    assert size(n_seq=3, n_tokens=1 << 16, max_new=1 << 16, max_len=1 << 20) == 16
 
 
 def store(c=None, b=None, layer=0, q=FAKE, ldq=256, k=FAKE, ldk=128, v=FAKE, ldv=128, n_head=4, table=FAKE, rows=128):
