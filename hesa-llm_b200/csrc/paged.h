@@ -203,9 +203,10 @@ __device__ __forceinline__ void split_half2(float x0, float x1, uint32_t& hi, ui
 }
 
 // Launch with programmatic stream serialization: the grid may be set up while
-// the previous kernel on the stream finishes. Every such kernel calls
-// grid_dep_wait before it reads or writes anything, and reads what earlier kernels
-// wrote with plain loads (no read-only cache: the grid may be older than the data).
+// the previous kernel on the stream finishes. Every block of such a kernel calls
+// grid_dep_wait, also one with nothing to do (the grid must not end before the one
+// it follows), before it writes anything, and reads what earlier kernels wrote with
+// plain loads (no read-only cache: the grid may be older than the data).
 template <typename... P, typename... T>
 cudaError_t launch_dep(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, T... args) {
     cudaLaunchAttribute attr[1];

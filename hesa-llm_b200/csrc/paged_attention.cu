@@ -69,10 +69,11 @@ template <int HD> struct RowsShape {
     // a stage: K then V of `subs` blocks, rows of `heads` heads padded by 16 bytes; heads * subs <= warps
     static constexpr size_t stage_bytes = 2 * kKeyBlock * (warps * HD * 2 + warps * 16);
     static constexpr size_t smem = stages * stage_bytes;
-    // parts: two a CTA, each [warps][rows]: (m, l), then acc[HD]
-    static constexpr size_t part_rows = 2 * static_cast<size_t>(kRowsCtas) * warps * kRowTile;
-    static constexpr size_t cut_bytes = kMostTiles * 16;   // of the list of what is to be added up
-    static constexpr size_t part_bytes = cut_bytes + part_rows * (2 + HD) * 4;
+    // workspace: the list of what is to be added up, then the parts' rows (m, l), then their acc[HD]; a part has
+    // [warps][rows] of them
+    static constexpr size_t cut_bytes = kMostTiles * 16;
+    static constexpr size_t part_rows(int64_t parts) { return static_cast<size_t>(parts) * warps * kRowTile; }
+    static constexpr size_t bytes(int64_t parts) { return cut_bytes + part_rows(parts) * (2 + HD) * 4; }
 };
 
 // Heads of a group (a CTA's warps have one each) and how many warps share a head.
@@ -89,6 +90,12 @@ struct HeadGroups {
     }
     __device__ __forceinline__ int sub_of(int warp) const { return warp * recip >> 8; }   // warp / heads for warp < 9
 };
+
+// Parts of a launch: two a CTA (its run's first (tile, group) and its last), and,
+// where several warps share a head, one for each (tile, group) that lies in one run.
+__host__ __device__ inline int64_t part_count(int tiles, const HeadGroups& hg) {
+    return 2 * kRowsCtas + (hg.subs > 1 ? static_cast<int64_t>(tiles) * hg.groups : 0);
+}
 
 // Whether every (tile, group) has an entry in the list of what is to be added up.
 __host__ __device__ inline bool by_tile(int tiles, const HeadGroups& hg) {
@@ -429,7 +436,7 @@ __device__ __forceinline__ void rows_segment(const AttnArgs& A, Ring& ring, cons
         const int64_t at = (static_cast<int64_t>(part) * S::warps + warp) * kRowTile + (lane >> 2);
         float* ml = A.part + S::cut_bytes / 4;
         if ((lane & 3) == 0) *reinterpret_cast<float2*>(ml + at * 2) = make_float2(m, l);
-        float* o = ml + S::part_rows * 2 + at * HD + 2 * (lane & 3);
+        float* o = ml + S::part_rows(part_count(A.n_split, hg)) * 2 + at * HD + 2 * (lane & 3);
 #pragma unroll
         for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(o + n * 8) = make_float2(acc[n][0], acc[n][1]);
     }
@@ -522,10 +529,12 @@ rows_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ HeadGrou
     Cut cut{0, 0, 0, 0};
     while (next_segment(s_pre, hg, u, end, lo, seg)) {
         const int c_first = runs.cta_of(seg.first + hg.cost), c_last = runs.cta_of(seg.first + seg.units - 1);
-        const Cut all{seg.tile, seg.grp, 2 * c_first + (runs.start(c_first) >= seg.first ? 0 : 1), c_last - c_first + 1};
+        const bool uncut = c_first == c_last;
+        const int own_part = 2 * kRowsCtas + seg.tile * hg.groups + seg.grp;   // of what several warps share, uncut
+        const Cut all{seg.tile, seg.grp, uncut ? own_part : 2 * c_first + (runs.start(c_first) >= seg.first ? 0 : 1), c_last - c_first + 1};
         if (cta == c_first + 1) cut = all;
         if (listed_by_tile && cta == c_first && threadIdx.x == 0) cuts[seg.tile * hg.groups + seg.grp] = all;
-        rows_segment<HD>(A, ring, hg, seg, c_first == c_last && hg.subs == 1 ? -1 : 2 * cta + (begin >= seg.first ? 0 : 1));
+        rows_segment<HD>(A, ring, hg, seg, !uncut ? 2 * cta + (begin >= seg.first ? 0 : 1) : hg.subs > 1 ? own_part : -1);
     }
     if (!listed_by_tile && threadIdx.x == 0) cuts[cta] = cut;
 }
@@ -560,7 +569,7 @@ combine_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ HeadG
     const int slots = rows > 4 ? 8 : rows > 2 ? 4 : rows;   // a power of two
     const int row = warp & (slots - 1), share = warp / slots, shares = 8 / slots;   // row: of row0 ..
     const float* ml = A.part + S::cut_bytes / 4;
-    const float* acc = ml + S::part_rows * 2;
+    const float* acc = ml + S::part_rows(part_count(A.n_split, hg)) * 2;
     auto at = [&](int i) {   // part i: sub-part i % subs of CTA part i / subs
         const int p = i >> hg.sub_bits, x = i & (hg.subs - 1);
         return (static_cast<int64_t>(p == 0 ? cut.first : 2 * ((cut.first >> 1) + p)) * S::warps + x * hg.heads + hl) * kRowTile + row0 + row;
@@ -669,7 +678,11 @@ Plan make_plan(const hesa_cuda_paged_kv* kv, const hesa_cuda_token_batch* b, int
 
 size_t part_bytes(const Plan& p, const hesa_cuda_paged_kv* kv) {
     const size_t row = static_cast<size_t>(kv->head_dim + 2) * sizeof(float);
-    if (!p.tc) return kv->head_dim == 64 ? RowsShape<64>::part_bytes : kv->head_dim == 128 ? RowsShape<128>::part_bytes : RowsShape<256>::part_bytes;
+    if (!p.tc) {
+        const HeadGroups hg(kv->n_kv_head, kv->head_dim == 256 ? RowsShape<256>::warps : RowsShape<128>::warps, p.heads);
+        const int64_t parts = part_count(std::min(p.tiles, kMostTiles), hg);
+        return kv->head_dim == 64 ? RowsShape<64>::bytes(parts) : kv->head_dim == 128 ? RowsShape<128>::bytes(parts) : RowsShape<256>::bytes(parts);
+    }
     return p.n_split > 1 ? static_cast<size_t>(p.tiles) * kv->n_kv_head * p.n_split * p.rows * row : 0;
 }
 
@@ -713,6 +726,7 @@ int check_paged_kv(const hesa_cuda_paged_kv* kv) {
         static_cast<int64_t>(kv->max_pages) * kv->page_size >= (int64_t(1) << 30))
         return record_error(HESA_CUDA_SHAPE_MISMATCH, "paged cache too large");
     const int64_t page = static_cast<int64_t>(kv->page_size) * kv->n_kv_head * kv->head_dim;
+    if (page > (int64_t(1) << 30)) return record_error(HESA_CUDA_SHAPE_MISMATCH, "pages of more than 2^30 values");
     const int64_t most = int64_t(1) << 50;
     if (kv->page_stride < page || kv->page_stride > most || kv->layer_stride < 0 || kv->layer_stride > most || (kv->page_stride & 7) || (kv->layer_stride & 7))
         return record_error(HESA_CUDA_SHAPE_MISMATCH, "page_stride and layer_stride must be multiples of 8, page_stride at least a page");
@@ -787,8 +801,10 @@ int hesa_cuda_paged_attention(const hesa_cuda_paged_kv* kv, int32_t layer, const
         return record_error(HESA_CUDA_INVALID_ARGUMENT, "workspace too small");
     hesa_cuda_attn_options o{};
     if (options) o = *options;
-    if (!(o.scale >= 0.f) || !std::isfinite(o.scale) || !(o.softcap >= 0.f) || !std::isfinite(o.softcap) || o.window < 0)
-        return record_error(HESA_CUDA_INVALID_ARGUMENT, "scale, softcap and window must be finite and not negative");
+    if (!(o.scale >= 0.f) || !std::isfinite(o.scale) || o.window < 0)
+        return record_error(HESA_CUDA_INVALID_ARGUMENT, "scale and window must be finite and not negative");
+    if (o.softcap != 0.f && !(o.softcap >= 1e-6f && o.softcap <= 1e6f))
+        return record_error(HESA_CUDA_INVALID_ARGUMENT, "softcap must be 0 or 1e-6 .. 1e6");
     if (batch->n_tokens == 0 || batch->max_new == 0) return HESA_CUDA_OK;
 
     const Plan p = make_plan(kv, batch, n_head);

@@ -750,7 +750,9 @@ combine_kernel(const __grid_constant__ AttnArgs A) {
     constexpr int V = HD / 32, AHEAD = 8;   // values of a lane; parts whose loads are under way
     const int lane = threadIdx.x & 31, kvh = blockIdx.y;
     int seq, tile;
-    locate_tile(A.b, A.group, kM, A.per_seq, static_cast<int>(blockIdx.x), seq, tile);   // chunk_kernel has waited for the batch
+    grid_dep_wait();
+    grid_dep_launch();
+    locate_tile(A.b, A.group, kM, A.per_seq, static_cast<int>(blockIdx.x), seq, tile);
     const SeqView sv = seq_view(A.c, A.b, seq);
     const int n_rows = sv.n_new * A.group;
     const int r0 = ((n_rows + kM - 1) / kM - 1 - tile) * kM, base = sv.len - sv.n_new;
@@ -761,7 +763,6 @@ combine_kernel(const __grid_constant__ AttnArgs A) {
     const KeyBlocks kb = key_blocks(mask, base + A.group_div.div(r0), base + A.group_div.div(min(r0 + kM - 1, n_rows - 1)), kN);
     const int n = max(1, (kb.n + A.blocks_per_split - 1) / A.blocks_per_split);
     if (n == 1) return;
-    grid_dep_wait();
     const int64_t pair = static_cast<int64_t>(blockIdx.x) * A.c.n_kv + kvh;
     const float* parts = A.part + pair * A.n_split * kPart;
     const float* ml = parts + kM * HD + row * 2;
@@ -847,8 +848,9 @@ cudaError_t launch(const AttnArgs& a, int tiles, int box, cudaStream_t s) {
 cudaError_t paged_attention_tc(const AttnArgs& a, int tiles, cudaStream_t s) {
     // a box of the tiled copies lies in one page and one block of keys, and its
     // rows are whole groups of the swizzle; a tensor map's strides are below 2^40
+    // bytes, each a multiple of the one before it
     const int box = std::gcd(a.c.page_size, kTcKeys);
-    const bool tma = box >= 8 && a.c.page_stride < (int64_t(1) << 39);
+    const bool tma = box >= 8 && a.c.page_stride < (int64_t(1) << 39) && a.c.page_stride % (static_cast<int64_t>(a.c.n_kv) * a.c.head_dim) == 0;
     if (a.c.head_dim == 64) return tma ? launch<64, true>(a, tiles, box, s) : launch<64, false>(a, tiles, box, s);
     return tma ? launch<128, true>(a, tiles, box, s) : launch<128, false>(a, tiles, box, s);
 }

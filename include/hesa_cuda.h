@@ -330,7 +330,8 @@ HESA_CUDA_API int hesa_cuda_decode_step_sharded(const hesa_cuda_model* model, co
  * either order of nesting. Token j of a slot lies in place j % page_size of
  * page table[slot * max_pages + j / page_size]. page_refs[p] counts the slots
  * that page p belongs to, 0: free. head_dim 64, 128 or 256; pools 16-byte
- * aligned; at most 65536 slots, 2^20 pages and 2^30 tokens a slot. The struct
+ * aligned; at most 65536 slots, 2^30 tokens a slot, 2^30 values a page, and for
+ * the page operations 2^20 pages. The struct
  * is host memory; every pointer in it is a device pointer. page_refs may be
  * NULL where no page operation is called. A new cache has seq_len and
  * page_refs zero; table need not be set. */
@@ -368,7 +369,7 @@ typedef struct {
  * sequence i. Zeroed: the plain causal attention with scale 1/sqrt(head_dim). */
 typedef struct {
     float scale;             /* 0: 1 / sqrt(head_dim) */
-    float softcap;           /* 0: not capped */
+    float softcap;           /* 0: not capped, else 1e-6 .. 1e6 */
     int32_t window;          /* 0: no window */
     const float* slopes;     /* device [n_head] or NULL */
     const int32_t* prefix;   /* device [n_seq] or NULL */

@@ -164,6 +164,43 @@ def test_options(T, shape, opts):
     check(c, **opts)
 
 
+@pytest.mark.parametrize("seed", range(100))
+def test_random_batches(T, seed):
+    """Ragged batches of all head layouts, with empty sequences, more new tokens than tokens, and any mask."""
+    import random
+    r = random.Random(1000 + seed)
+    n_kv = r.choice([1, 2, 3, 4, 5, 6, 8, 9, 12, 17])
+    group = r.choice([1, 1, 2, 3, 4, 7, 8, 16])
+    hd = r.choice([64, 128, 128, 256])
+    page = r.choice([1, 3, 8, 16, 24, 40, 64, 128, 200])
+    n_seq = r.choice([1, 2, 5, 23])
+    most = r.choice([40, 300, 3000]) if n_seq > 5 else r.choice([40, 700, 6000])
+    lens = [r.choice([0, 1, r.randrange(0, most), most]) for _ in range(n_seq)]
+    lens[0] = max(1, lens[0])
+    top = r.choice([1, 1, 3, 60])
+    news = [r.randrange(0, min(top, n + 2) + 1) for n in lens]
+    news[0] = max(1, news[0])
+    c = Case(T, n_kv * group, n_kv, hd, page, lens, news, seed=seed)
+    opts = {}
+    if r.random() < 0.4:
+        opts["window"] = r.choice([1, 5, 16, 130, 1000])
+    if r.random() < 0.3:
+        opts["softcap"] = r.choice([2.0, 30.0])
+    if r.random() < 0.3:
+        opts["slopes"] = T.exp2(-4.0 * T.rand(c.n_head, device="cuda"))
+    if r.random() < 0.3:
+        opts["prefix"] = T.tensor([r.randrange(0, n + 1) for n in lens], dtype=T.int32, device="cuda")
+    check(c, **opts)
+
+
+@pytest.mark.parametrize("n_head,n_kv,hd,news", [(8, 1, 64, [1]), (16, 8, 64, [1]), (34, 17, 64, [20, 0, 9])])
+def test_many_sequences(T, n_head, n_kv, hd, news):
+    """More tiles than one launch sums up (1024), and more than are worth splitting (4096 with their kv heads)."""
+    n = 1300
+    lens = [1 + (i * 37) % 61 for i in range(n)]
+    check(Case(T, n_head, n_kv, hd, 16, lens, [min(news[i % len(news)], lens[i]) for i in range(n)], seed=n_head))
+
+
 def test_rows_that_see_nothing_are_zero(T):
     """More new tokens than tokens: rows of negative positions see no key (or the prefix alone)."""
     c = Case(T, 4, 2, 64, 8, [5, 20], [9, 3], seed=3)
@@ -248,6 +285,22 @@ def test_page_and_layer_strides(T):
     k[1].copy_(c.k[0])
     v[1].copy_(c.v[0])
     c.cache, c.layer = c.H.PagedKV(k, v, c.cache.table, c.cache.seq_len), 1
+    assert float((c.run().double() - ref).abs().max()) <= tol
+
+
+@pytest.mark.parametrize("news", [[1, 1, 1], [5, 60, 3]])
+def test_pages_with_gaps(T, news):
+    """A page stride that is no multiple of a token's row."""
+    c = Case(T, 4, 2, 128, 16, [50, 200, 70], news, seed=19)
+    ref, tol = c.exact()
+    n = c.k.shape[1]
+    pools = []
+    for x in (c.k, c.v):
+        wide = T.full((1, n, 16 * 256 + 40), math.nan, dtype=T.float16, device="cuda")
+        p = wide.as_strided((1, n, 16, 2, 128), (wide.stride(0), wide.stride(1), 256, 128, 1))
+        p.copy_(x)
+        pools.append(p)
+    c.cache = c.H.PagedKV(pools[0], pools[1], c.cache.table, c.cache.seq_len)
     assert float((c.run().double() - ref).abs().max()) <= tol
 
 

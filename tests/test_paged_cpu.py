@@ -31,6 +31,7 @@ def attend(c=None, b=None, layer=0, q=FAKE, ldq=256, out=FAKE, ldo=256, n_head=4
 
 CACHES = [(dict(k=0), 2), (dict(v=0), 2), (dict(table=0), 2), (dict(seq_len=0), 2), (dict(k=FAKE + 8), 2), (dict(table=FAKE + 2), 2),
           (dict(head_dim=80), 6), (dict(n_pages=0), 6), (dict(page_size=0), 6), (dict(page_size=65537, page_stride=1 << 40), 6),
+          (dict(page_size=65536, n_kv_head=1024, page_stride=1 << 40, layer_stride=1 << 45), 6),
           (dict(n_slots=65537), 6), (dict(max_pages=1 << 27), 6), (dict(page_stride=2040), 6), (dict(page_stride=2052), 6),
           (dict(layer_stride=2048), 6), (dict(layer_stride=20484), 6), (dict(n_layer=0), 6), (dict(n_kv_head=-1), 6)]
 
@@ -56,7 +57,8 @@ def test_layers_inside_pages_are_a_sound_layout():
     (dict(b=batch(n_tokens=1 << 30, max_new=1)), 6), (dict(layer=2), 2), (dict(layer=-1), 2), (dict(n_head=3), 6), (dict(n_head=0), 6),
     (dict(q=0), 2), (dict(out=0), 2), (dict(ws=0), 2), (dict(q=FAKE + 4), 2), (dict(ldq=255), 6), (dict(ldo=258), 2), (dict(ws=FAKE + 8), 2),
     (dict(wsb=100), 2), (dict(opts=(-1.0, 0.0, 0, None, None)), 2), (dict(opts=(0.0, float("nan"), 0, None, None)), 2),
-    (dict(opts=(0.0, float("inf"), 0, None, None)), 2), (dict(opts=(0.0, 0.0, -1, None, None)), 2)])
+    (dict(opts=(0.0, float("inf"), 0, None, None)), 2), (dict(opts=(0.0, 0.0, -1, None, None)), 2),
+    (dict(opts=(0.0, -2.0, 0, None, None)), 2), (dict(opts=(0.0, 1e-9, 0, None, None)), 2)])
 def test_attention_refusals(kw, code):
     assert attend(**kw) == code
     assert H.lib().hesa_cuda_last_error()
@@ -67,10 +69,10 @@ def test_nothing_to_attend_is_no_launch():
 
 
 def test_attention_workspace_follows_the_cut():
-    """Next tokens: the parts of one grid, whatever the lengths. Chunks: parts where the keys are split, few bytes where not."""
+    """Next tokens: the parts of one grid and batch, whatever the lengths. Chunks: parts where the keys are split, few bytes where not."""
     size = lambda **kw: H.lib().hesa_cuda_paged_attention_workspace_size(  # noqa: E731
         ctypes.byref(cache(max_pages=1 << 20)), ctypes.byref(batch(**kw)), 4)
-    assert size(n_seq=1, n_tokens=1, max_new=1, max_len=64) == size(n_seq=3, n_tokens=3, max_new=1, max_len=1 << 20) < 16 << 20
+    assert size(n_seq=1, n_tokens=1, max_new=1, max_len=64) == size(n_seq=1, n_tokens=1, max_new=1, max_len=1 << 20) < 16 << 20
     assert size(n_seq=1, n_tokens=64, max_new=64, max_len=256) < size(n_seq=1, n_tokens=64, max_new=64, max_len=1 << 20) < 64 << 20
     assert size(n_seq=3, n_tokens=1 << 16, max_new=1 << 16, max_len=1 << 20) == 16
 
