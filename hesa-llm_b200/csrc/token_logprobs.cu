@@ -18,7 +18,8 @@
 // row's alignment (the first and the last quad of a row are read by the word), a
 // step ahead of its use. Few rows are split over blocks; the last block of a row
 // to arrive joins the parts.
-// 1024 rows of 131071, five alternatives: 111 us (537 MB, 4.8 TB/s), none: 85 us; one row of 32000: 10.4 us.
+// 1024 rows of 131071, five alternatives: 101 us (537 MB, 5.3 TB/s), 32: 150 us, none: 85 us; one row of 32000:
+// 9.9 us.
 #include "../../include/hesa_cuda.h"
 #include "abi_errors.h"
 #include "paged.h"
@@ -186,7 +187,7 @@ token_logprobs_kernel(const float* logits, int64_t ld, int n_rows, int vocab, co
     constexpr int kStep = kLpWarps * 32 * kUnroll;
     Sums s{-INFINITY, 0.f, 0.f};
     float4 nx[kUnroll];
-    int qb = q0 + warp * 32 * kUnroll + lane, best = qb;   // best: the step of the first maximum
+    int qb = q0 + warp * 32 * kUnroll + lane, best = qb;   // best: the quad of the first maximum
     if (qb < q1) {
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) nx[u] = quad(qb + u * 32);
@@ -199,15 +200,19 @@ token_logprobs_kernel(const float* logits, int64_t ld, int n_rows, int vocab, co
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) nx[u] = quad(qb + kStep + u * 32);
         }
-        float mx = -INFINITY;
+        float qm[kUnroll], mx = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) mx = fmaxf(mx, fmaxf(fmaxf(x[u].x, x[u].y), fmaxf(x[u].z, x[u].w)));
+        for (int u = 0; u < kUnroll; ++u) {
+            qm[u] = fmaxf(fmaxf(x[u].x, x[u].y), fmaxf(x[u].z, x[u].w));
+            mx = fmaxf(mx, qm[u]);
+        }
         if (mx > s.m) {
             const float d = s.m == -INFINITY ? 0.f : s.m - mx, f = lp_ex2(d * kLog2e);
             s.w = f > 0.f ? f * fmaf(s.z, d, s.w) : 0.f;
             s.z *= f;
             s.m = mx;
-            best = qb;
+#pragma unroll
+            for (int u = kUnroll - 1; u >= 0; --u) best = qm[u] == mx ? qb + u * 32 : best;
         }
         const float ms = s.m == -INFINITY ? 0.f : s.m;
         float2 z = make_float2(0.f, 0.f), w = make_float2(0.f, 0.f);
@@ -230,12 +235,11 @@ token_logprobs_kernel(const float* logits, int64_t ld, int n_rows, int vocab, co
     }
     if (TOP) {
         // the thread's largest key
-        uint64_t mine = 0;
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
+        uint64_t mine;
+        {
             uint64_t k[4];
-            keys(best + u * 32, quad(best + u * 32), k);
-            mine = max_key(mine, max_key(max_key(k[0], k[1]), max_key(k[2], k[3])));
+            keys(best, quad(best), k);
+            mine = max_key(max_key(k[0], k[1]), max_key(k[2], k[3]));
         }
         // each warp's ceil(k / 8)-th bounds the k-th of the block's from below; the threads above the least of them are ranked
         uint64_t rest = mine, nth = 0;

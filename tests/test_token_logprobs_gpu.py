@@ -145,3 +145,16 @@ def test_refusals_of_the_binding(T):
         H.token_logprobs(x, t, top_k=33)
     lp, ent, ids, top = H.token_logprobs(x)
     assert lp is None and ids.shape == (4, 0) and top.shape == (4, 0)
+
+
+@pytest.mark.parametrize("vocab,k", [(300000, 32), (131072, 7), (9000, 20)])
+def test_large_values_side_by_side(T, vocab, k):
+    """The largest values of a row all where one thread, or one block of a split row, reads; and everywhere but there."""
+    x = T.randn(4, vocab, device="cuda")
+    x[0, 128:640] += 50
+    x[1, ::256] += 50
+    x[2] = T.arange(vocab, device="cuda") % 251
+    x[3] = (T.arange(vocab, device="cuda") // 4 % 97).float()
+    check(T, x, T.tensor([130, 1, 250, 0], dtype=T.int32, device="cuda"), k)
+    wide = x.repeat(300, 1)      # whole rows a block
+    check(T, wide, T.zeros(1200, dtype=T.int32, device="cuda"), k)
