@@ -9,6 +9,11 @@
 // taken in ascending order, so results do not depend on scheduling. What is to
 // be copied goes into a list in the workspace, and a second kernel copies it for
 // all layers: whole 16-byte words of K and V, bound by HBM.
+// Measured: compaction that moves 240 pages of 32 layers 180 us (1.0 GB; the plan
+// takes 7 us of them, the copies run at 6 TB/s); free, fork and reserve of seven
+// slots of up to 44 pages 19 us for the four launches, which are chains of dependent
+// reads by one block; the cache write of 5296 tokens (32 heads) 67.8 us
+// (437 MB, 6.4 TB/s), of 32 tokens (64 heads on 8) 3.4 us.
 #include "paged.h"
 #include "abi_errors.h"
 #include "qmatvec.h"
@@ -500,6 +505,7 @@ int hesa_cuda_kv_reserve(const hesa_cuda_paged_kv* kv, const int32_t* slots, con
     if (n > kv->n_slots) return record_error(HESA_CUDA_SHAPE_MISMATCH, "more slots than the cache has");
     if (n == 0) return HESA_CUDA_OK;
     if (!slots || !n_new) return record_error(HESA_CUDA_INVALID_ARGUMENT, "null pointer");
+    if (!aligned(slots, 4) || !aligned(n_new, 4)) return record_error(HESA_CUDA_INVALID_ARGUMENT, "the lists must be 4-byte aligned");
     cudaError_t e = status_word(&t.status);
     if (e == cudaSuccess) {
         e = launch_dep(reserve_kernel, dim3(1), kPlanThreads, 0, static_cast<cudaStream_t>(stream), t, slots, n_new, n, page_work(workspace, kv));
@@ -516,6 +522,7 @@ int hesa_cuda_kv_free(const hesa_cuda_paged_kv* kv, const int32_t* slots, int32_
     if (n > kv->n_slots) return record_error(HESA_CUDA_SHAPE_MISMATCH, "more slots than the cache has");
     if (n == 0) return HESA_CUDA_OK;
     if (!slots) return record_error(HESA_CUDA_INVALID_ARGUMENT, "null pointer");
+    if (!aligned(slots, 4)) return record_error(HESA_CUDA_INVALID_ARGUMENT, "the lists must be 4-byte aligned");
     cudaError_t e = status_word(&t.status);
     if (e == cudaSuccess) {
         e = launch_dep(free_kernel, dim3(1), kPlanThreads, 0, static_cast<cudaStream_t>(stream), t, slots, n);
@@ -532,6 +539,7 @@ int hesa_cuda_kv_fork(const hesa_cuda_paged_kv* kv, const int32_t* src, const in
     if (n > kv->n_slots) return record_error(HESA_CUDA_SHAPE_MISMATCH, "more slots than the cache has");
     if (n == 0) return HESA_CUDA_OK;
     if (!src || !dst) return record_error(HESA_CUDA_INVALID_ARGUMENT, "null pointer");
+    if (!aligned(src, 4) || !aligned(dst, 4)) return record_error(HESA_CUDA_INVALID_ARGUMENT, "the lists must be 4-byte aligned");
     const PageWork w = page_work(workspace, kv);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t e = status_word(&t.status);
@@ -547,6 +555,7 @@ int hesa_cuda_kv_compact(const hesa_cuda_paged_kv* kv, int32_t* n_live, void* wo
     Tables t{};
     const int rc = page_op(kv, 0, workspace, workspace_bytes, &t);
     if (rc != HESA_CUDA_OK) return rc;
+    if (!aligned(n_live, 4)) return record_error(HESA_CUDA_INVALID_ARGUMENT, "n_live must be 4-byte aligned");
     const PageWork w = page_work(workspace, kv);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t e = status_word(&t.status);
@@ -566,6 +575,7 @@ int hesa_cuda_kv_copy_pages(const hesa_cuda_paged_kv* kv, const int32_t* src_pag
     if (n > kv->n_pages) return record_error(HESA_CUDA_SHAPE_MISMATCH, "more pairs than pages");
     if (n == 0) return HESA_CUDA_OK;
     if (!src_pages || !dst_pages) return record_error(HESA_CUDA_INVALID_ARGUMENT, "null pointer");
+    if (!aligned(src_pages, 4) || !aligned(dst_pages, 4)) return record_error(HESA_CUDA_INVALID_ARGUMENT, "the lists must be 4-byte aligned");
     const PageWork w = page_work(workspace, kv);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t e = status_word(&t.status);

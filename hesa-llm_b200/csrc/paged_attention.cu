@@ -36,6 +36,9 @@
 //     load every SM alike. The lengths are only known on the device: every CTA
 //     adds up the tiles' blocks itself. What lies in several runs leaves (m, l,
 //     acc) for each, which combine_kernel adds in the order of the runs.
+// Measured (both kernels): two contexts of 131072 and 100001 tokens, 64 heads on 8,
+// 167 us (6.4 TB/s); 32 of 1 to 8192 tokens 33.8 us (3.7 TB/s, the first copies and
+// the joining cost 10 of them); one of 2048 tokens, 32 heads, 14.7 us (2.3 TB/s).
 #include "paged.h"
 #include "paged_tc.h"
 #include "abi_errors.h"
@@ -71,7 +74,7 @@ template <int HD> struct RowsShape {
     static constexpr size_t smem = stages * stage_bytes;
     // workspace: the list of what is to be added up, then the parts' rows (m, l), then their acc[HD]; a part has
     // [warps][rows] of them
-    static constexpr size_t cut_bytes = kMostTiles * 16;
+    static constexpr size_t cut_bytes = kMostTiles * 32;
     static constexpr size_t part_rows(int64_t parts) { return static_cast<size_t>(parts) * warps * kRowTile; }
     static constexpr size_t bytes(int64_t parts) { return cut_bytes + part_rows(parts) * (2 + HD) * 4; }
 };
@@ -263,14 +266,13 @@ __device__ __forceinline__ void copy_segment(const AttnArgs& A, Ring& ring, cons
 // are all that the rows see, and the result goes to out; else (m, l, acc) go to
 // that part.
 template <int HD>
-__device__ __forceinline__ void rows_segment(const AttnArgs& A, Ring& ring, const HeadGroups& hg, const Segment& seg, int part) {
+__device__ __forceinline__ void rows_segment(const AttnArgs& A, Ring& ring, const HeadGroups& hg, const Segment& seg, const TileView& tv, int part) {
     using S = RowsShape<HD>;
     constexpr int KS = HD / 16;                  // k-steps of Q K^T
     constexpr int NT = HD / 8;                   // column tiles of P V
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int sub = hg.sub_of(warp), hl = warp - sub * hg.heads, kvh = seg.grp * hg.heads + hl;
     const bool active = sub < hg.subs && kvh < A.c.n_kv;
-    const TileView tv = tile_view(A, seg.tile);
     const SeqView& sv = tv.sv;
     const Mask& mask = tv.mask;
 
@@ -442,13 +444,16 @@ __device__ __forceinline__ void rows_segment(const AttnArgs& A, Ring& ring, cons
     }
 }
 
-// What combine_kernel adds up: the parts of (tile, grp) are `first`, then the
+// What combine_kernel adds up, and where it belongs: rows r0 .. r0 + rows - 1 of
+// the sequence whose first row of q is q0. The parts are `first`, then the
 // first part of each of the next n - 1 CTAs, each of hg.subs warps. n = 0, or one
-// part of one warp: nothing. With by_tile every (tile, group) has an entry; else
+// part of one warp: nothing. With by_tile every (tile, group) has an entry (groups
+// of fewer heads are only made of few tiles, so kMostTiles entries are enough); else
 // there is one for each CTA, for the cut before its run (if it is the first one of
 // what it cuts).
 struct __align__(16) Cut {
-    int32_t tile, grp, first, n;
+    int32_t grp, first, n, rows;
+    int32_t r0, q0, pad[2];
 };
 
 template <int HD>
@@ -525,16 +530,18 @@ rows_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ HeadGrou
     }
     if (listed_by_tile && cta == 0)   // those without rows
         for (int i = threadIdx.x; i < tiles * hg.groups; i += S::warps * 32)
-            if (s_pre[i / hg.groups + 1] == s_pre[i / hg.groups]) cuts[i] = Cut{0, 0, 0, 0};
-    Cut cut{0, 0, 0, 0};
+            if (s_pre[i / hg.groups + 1] == s_pre[i / hg.groups]) cuts[i] = Cut{};
+    Cut cut{};
     while (next_segment(s_pre, hg, u, end, lo, seg)) {
         const int c_first = runs.cta_of(seg.first + hg.cost), c_last = runs.cta_of(seg.first + seg.units - 1);
         const bool uncut = c_first == c_last;
         const int own_part = 2 * kRowsCtas + seg.tile * hg.groups + seg.grp;   // of what several warps share, uncut
-        const Cut all{seg.tile, seg.grp, uncut ? own_part : 2 * c_first + (runs.start(c_first) >= seg.first ? 0 : 1), c_last - c_first + 1};
+        const TileView tv = tile_view(A, seg.tile);
+        const Cut all{seg.grp, uncut ? own_part : 2 * c_first + (runs.start(c_first) >= seg.first ? 0 : 1), c_last - c_first + 1,
+                      min(kRowTile, tv.n_rows - tv.r0), tv.r0, tv.sv.q0};
         if (cta == c_first + 1) cut = all;
         if (listed_by_tile && cta == c_first && threadIdx.x == 0) cuts[seg.tile * hg.groups + seg.grp] = all;
-        rows_segment<HD>(A, ring, hg, seg, !uncut ? 2 * cta + (begin >= seg.first ? 0 : 1) : hg.subs > 1 ? own_part : -1);
+        rows_segment<HD>(A, ring, hg, seg, tv, !uncut ? 2 * cta + (begin >= seg.first ? 0 : 1) : hg.subs > 1 ? own_part : -1);
     }
     if (!listed_by_tile && threadIdx.x == 0) cuts[cta] = cut;
 }
@@ -552,19 +559,15 @@ combine_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ HeadG
     constexpr int V = HD / 32;     // values of a lane
     constexpr int AHEAD = 32 / V;  // parts of which a warp has the loads under way
     __shared__ float s_o[8][HD + 1];
-    // rows_kernel has waited for what came before it: the batch can be read already
-    const bool listed_by_tile = by_tile(A.n_split, hg);
     const int hl = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    TileView tv{};
-    if (listed_by_tile) tv = tile_view(A, static_cast<int>(blockIdx.x) / hg.groups);
     grid_dep_wait();
     grid_dep_launch();
-    const int4 c4 = __ldcg(reinterpret_cast<const int4*>(A.part) + blockIdx.x);
-    const Cut cut{c4.x, c4.y, c4.z, c4.w};
+    const int4* c4 = reinterpret_cast<const int4*>(A.part) + 2 * blockIdx.x;
+    const int4 ca = __ldcg(c4), cb = __ldcg(c4 + 1);
+    const Cut cut{ca.x, ca.y, ca.z, ca.w, cb.x, cb.y};
     const int n = cut.n * hg.subs, kvh = cut.grp * hg.heads + hl;
     if (n < 2 || kvh >= A.c.n_kv) return;
-    if (!listed_by_tile) tv = tile_view(A, cut.tile);
-    const int row0 = blockIdx.z, rows = min(gridDim.z > 1 ? 1 : kRowTile, tv.n_rows - tv.r0 - row0);
+    const int row0 = blockIdx.z, rows = min(gridDim.z > 1 ? 1 : kRowTile, cut.rows - row0);
     if (rows <= 0) return;
     const int slots = rows > 4 ? 8 : rows > 2 ? 4 : rows;   // a power of two
     const int row = warp & (slots - 1), share = warp / slots, shares = 8 / slots;   // row: of row0 ..
@@ -628,8 +631,8 @@ combine_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ HeadG
         for (int c = 0; c < V; ++c) O[c] += s_o[warp + x * slots][lane * V + c];
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
-    const int r = tv.r0 + row0 + row, t = A.group_div.div(r), h = kvh * A.group + r - t * A.group;
-    float* o = A.out + static_cast<int64_t>(tv.sv.q0 + t) * A.ldo + static_cast<int64_t>(h) * HD + lane * V;
+    const int r = cut.r0 + row0 + row, t = A.group_div.div(r), h = kvh * A.group + r - t * A.group;
+    float* o = A.out + static_cast<int64_t>(cut.q0 + t) * A.ldo + static_cast<int64_t>(h) * HD + lane * V;
 #pragma unroll
     for (int c = 0; c < V; c += 2) *reinterpret_cast<float2*>(o + c) = make_float2(O[c] * inv, O[c + 1] * inv);
 }
@@ -741,6 +744,7 @@ int check_paged_kv(const hesa_cuda_paged_kv* kv) {
 int check_batch(const hesa_cuda_paged_kv* kv, int32_t layer, const hesa_cuda_token_batch* b, int64_t n_head) {
     if (layer < 0 || layer >= kv->n_layer) return record_error(HESA_CUDA_INVALID_ARGUMENT, "no such layer");
     if (!b || !b->q_start) return record_error(HESA_CUDA_INVALID_ARGUMENT, "null pointer");
+    if (!aligned(b->q_start, 4) || !aligned(b->slots, 4)) return record_error(HESA_CUDA_INVALID_ARGUMENT, "q_start and slots must be 4-byte aligned");
     if (b->n_seq <= 0 || b->n_tokens < 0 || b->max_new < 0 || b->max_len < 0 || b->max_new > b->n_tokens)
         return record_error(HESA_CUDA_SHAPE_MISMATCH, "bad batch");
     if (b->n_seq > 65536 || (!b->slots && b->n_seq > kv->n_slots)) return record_error(HESA_CUDA_SHAPE_MISMATCH, "more sequences than slots");
@@ -805,6 +809,7 @@ int hesa_cuda_paged_attention(const hesa_cuda_paged_kv* kv, int32_t layer, const
         return record_error(HESA_CUDA_INVALID_ARGUMENT, "scale and window must be finite and not negative");
     if (o.softcap != 0.f && !(o.softcap >= 1e-6f && o.softcap <= 1e6f))
         return record_error(HESA_CUDA_INVALID_ARGUMENT, "softcap must be 0 or 1e-6 .. 1e6");
+    if (!aligned(o.slopes, 4) || !aligned(o.prefix, 4)) return record_error(HESA_CUDA_INVALID_ARGUMENT, "slopes and prefix must be 4-byte aligned");
     if (batch->n_tokens == 0 || batch->max_new == 0) return HESA_CUDA_OK;
 
     const Plan p = make_plan(kv, batch, n_head);

@@ -407,6 +407,9 @@ int hesa_cuda_token_logprobs(const float* logits, int64_t ld, int64_t n_rows, in
         return record_error(HESA_CUDA_INVALID_ARGUMENT, "null pointer");
     if ((reinterpret_cast<uintptr_t>(logits) & 3) || (reinterpret_cast<uintptr_t>(workspace) & 15))
         return record_error(HESA_CUDA_INVALID_ARGUMENT, "logits must be 4-byte and the workspace 16-byte aligned");
+    if ((reinterpret_cast<uintptr_t>(tokens) | reinterpret_cast<uintptr_t>(logprob) | reinterpret_cast<uintptr_t>(entropy) |
+         reinterpret_cast<uintptr_t>(top_ids) | reinterpret_cast<uintptr_t>(top_logprobs)) & 3)
+        return record_error(HESA_CUDA_INVALID_ARGUMENT, "tokens and outputs must be 4-byte aligned");
     if (workspace_bytes < hesa_cuda_token_logprobs_workspace_size(n_rows, vocab, top_k))
         return record_error(HESA_CUDA_INVALID_ARGUMENT, "workspace too small");
     int* status = nullptr;

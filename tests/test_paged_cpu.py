@@ -64,6 +64,23 @@ def test_attention_refusals(kw, code):
     assert H.lib().hesa_cuda_last_error()
 
 
+def test_words_of_the_device_arrays_are_aligned():
+    """A list or table of 4-byte words at an odd address is refused by every call that would read it."""
+    L, r = H.lib(), ctypes.byref(cache())
+    odd = FAKE + 2
+    for b in (batch(slots=odd), batch(q_start=odd)):
+        assert attend(b=b) == 2 and store(b=b) == 2
+    assert attend(opts=(0.0, 0.0, 0, odd, None)) == 2
+    assert attend(opts=(0.0, 0.0, 0, None, odd)) == 2
+    ws = (FAKE, 1 << 30, None)
+    assert L.hesa_cuda_kv_reserve(r, odd, FAKE, 1, *ws) == L.hesa_cuda_kv_reserve(r, FAKE, odd, 1, *ws) == 2
+    assert L.hesa_cuda_kv_fork(r, odd, FAKE, 1, *ws) == L.hesa_cuda_kv_fork(r, FAKE, odd, 1, *ws) == 2
+    assert L.hesa_cuda_kv_copy_pages(r, odd, FAKE, 1, *ws) == L.hesa_cuda_kv_copy_pages(r, FAKE, odd, 1, *ws) == 2
+    assert L.hesa_cuda_kv_free(r, odd, 1, *ws) == L.hesa_cuda_kv_compact(r, odd, *ws) == 2
+    for name in ("tokens", "lp", "ent", "ids", "top"):
+        assert logprobs(**{name: odd}) == 2
+
+
 def test_nothing_to_attend_is_no_launch():
     assert attend(b=batch(n_tokens=0, max_new=0)) == 0
 
