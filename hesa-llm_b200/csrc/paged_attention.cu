@@ -56,11 +56,12 @@ constexpr int kRowTile = 8;
 constexpr int kKeyBlock = 16;
 constexpr int kRowsCtas = 148;       // one an SM
 constexpr int kCopyWarps = 4;        // a warp gets no more than one bulk copy under way in about 45 ns
-// Rows of a sequence from which on 128-row tiles are used, though they may be
-// empty for the most part, rather than several tiles of 8 that each read K and V:
-// eight sequences of 4000 tokens (64 heads on 8) with 16 rows: 31 us here, 40
-// there; with 32 rows 45 and 43; with 64 82 and 48.
-constexpr int kMostRows = 16;
+// Rows of a sequence above which 128-row tiles are used, though they may be
+// empty for the most part, rather than several tiles of 8 that each read K and V.
+// Eight sequences of 4000 tokens, 64 heads of 128 on 8: 16 rows 31 us here, 38
+// there; 32 rows 45 and 39; 64 rows 82 and 39. 16 heads of 256 on 4: 32 rows 52 and
+// 74, 64 rows 89 and 75.
+constexpr int most_rows(int head_dim) { return head_dim == 256 ? 48 : 16; }
 constexpr int kMostTiles = 1024;     // of a launch: the tiles' blocks are summed in shared memory
 constexpr int kSegCost = 5;          // stages that starting a (tile, group) takes the time of
 constexpr int kLeastUnits = 4;       // of a run
@@ -649,14 +650,13 @@ Plan make_plan(const hesa_cuda_paged_kv* kv, const hesa_cuda_token_batch* b, int
     Plan p{};
     const int g = static_cast<int>(n_head / kv->n_kv_head);
     const int64_t rows_a_seq = static_cast<int64_t>(b->max_new) * g;
-    p.tc = kv->head_dim <= 128 && rows_a_seq > kMostRows;
+    p.tc = rows_a_seq > most_rows(kv->head_dim) && (kv->head_dim <= 128 || paged_attention_tiled(layer_of(kv, 0)));
     p.rows = p.tc ? kTcRows : kRowTile;
     const int64_t most = (rows_a_seq + p.rows - 1) / p.rows;
     const int64_t bound = tile_bound(b->n_tokens, b->n_seq, g, p.rows);
     p.per_seq = b->n_seq * most <= bound ? static_cast<int>(most) : 0;
     const int64_t tiles = p.per_seq ? b->n_seq * most : bound;
     p.tiles = static_cast<int>(tiles);
-    const int64_t pairs = tiles * kv->n_kv_head;
     if (!p.tc) {
         // All heads of a token at once read the longest rows, and an SM streams no
         // more than about 44 GB/s: where that would leave SMs without work, groups
@@ -668,11 +668,13 @@ Plan make_plan(const hesa_cuda_paged_kv* kv, const hesa_cuda_token_batch* b, int
         return p;
     }
     // one CTA an SM, no split under 256 keys
-    const int64_t blocks = std::max<int64_t>(1, (b->max_len + kTcKeys - 1) / kTcKeys);
+    const int keys = tc_keys(kv->head_dim);
+    const int64_t blocks = std::max<int64_t>(1, (b->max_len + keys - 1) / keys);
+    const int64_t pairs = tiles * kv->n_kv_head * (kv->head_dim / tc_dims(kv->head_dim));
     int64_t per = blocks;
     if (pairs <= kPagedPairs) {
         const int64_t want = std::max<int64_t>(1, 148 / pairs);
-        per = std::max<int64_t>(2, (blocks + want - 1) / want);
+        per = std::max<int64_t>(256 / keys, (blocks + want - 1) / want);
     }
     p.blocks_per_split = static_cast<int>(std::min(per, blocks));
     p.n_split = static_cast<int>((blocks + p.blocks_per_split - 1) / p.blocks_per_split);
@@ -680,13 +682,14 @@ Plan make_plan(const hesa_cuda_paged_kv* kv, const hesa_cuda_token_batch* b, int
 }
 
 size_t part_bytes(const Plan& p, const hesa_cuda_paged_kv* kv) {
-    const size_t row = static_cast<size_t>(kv->head_dim + 2) * sizeof(float);
     if (!p.tc) {
         const HeadGroups hg(kv->n_kv_head, kv->head_dim == 256 ? RowsShape<256>::warps : RowsShape<128>::warps, p.heads);
         const int64_t parts = part_count(std::min(p.tiles, kMostTiles), hg);
         return kv->head_dim == 64 ? RowsShape<64>::bytes(parts) : kv->head_dim == 128 ? RowsShape<128>::bytes(parts) : RowsShape<256>::bytes(parts);
     }
-    return p.n_split > 1 ? static_cast<size_t>(p.tiles) * kv->n_kv_head * p.n_split * p.rows * row : 0;
+    const int dims = tc_dims(kv->head_dim);
+    const size_t rows = static_cast<size_t>(p.tiles) * kv->n_kv_head * (kv->head_dim / dims) * p.n_split * p.rows;
+    return p.n_split > 1 ? rows * (dims + 2) * sizeof(float) : 0;
 }
 
 template <int HD>

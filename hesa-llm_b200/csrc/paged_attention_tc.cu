@@ -35,9 +35,14 @@
 // that is not there is a coordinate past the pool, which reads as zeros. Pages
 // whose size is no multiple of 8 are copied with 16-byte cp.async (a K block
 // takes each warp about 1800 cycles).
+// With head_dim 256 q alone takes half of TMEM: blocks have 64 keys, and two CTAs
+// share a tile, each with all of Q K^T and half of the dims of V. (Q K^T twice is
+// half as much work again; one CTA for both halves would need 256 output registers
+// a thread.)
 // Measured, 64 heads on 8: 2048 tokens at 16384 1.72 ms with pages of 64 (600
 // TFLOP/s, 1200 counting the halves' products; 88% of what the tensor cores keep
-// up at the clock that the power limit leaves), 2.58 ms with pages of 7.
+// up at the clock that the power limit leaves), 2.58 ms with pages of 7. 1024 tokens at
+// 4096, 4 heads of 256: 71 us, where tiles of 8 rows take 194.
 #include "paged.h"
 #include "paged_tc.h"
 #include "qmatvec.h"
@@ -51,7 +56,6 @@ namespace hesa_cuda {
 namespace {
 
 constexpr int kM = kTcRows;                  // rows of a tile = TMEM lanes
-constexpr int kN = kTcKeys;                  // keys of a block
 constexpr int kComputeWarps = 8;
 constexpr int kQkWarp = kComputeWarps + 1;   // issues Q K^T, the warp before it P V
 constexpr int kProducerWarps = 2;
@@ -63,11 +67,14 @@ constexpr int kComputeRegs = 208, kOtherRegs = 88;
 constexpr int kInFlight = 3;                 // blocks that a producer has in flight with cp.async
 
 template <int HD> struct TcShape {
-    static constexpr uint32_t slot = kN * HD * 2;            // one K or V block
-    static constexpr int slots = HD == 128 ? 6 : 8;
+    static constexpr int keys = tc_keys(HD), vd = tc_dims(HD);   // keys of a block, dims of V that a CTA works on
+    static constexpr int parts = HD / vd;                        // CTAs of a (tile, kv head, split)
+    static constexpr uint32_t slot = keys * HD * 2;          // one K block; a V block is no larger
+    static constexpr int slots = HD == 64 ? 8 : 6;
     static constexpr uint32_t smem = slot * slots + 1024;    // + alignment of the swizzle
-    static constexpr uint32_t q_hi = 0, q_lo = HD / 2, s0 = HD, o = HD + 2 * kN;
-    static_assert(o + HD <= 512, "TMEM columns");
+    static constexpr uint32_t q_hi = 0, q_lo = HD / 2, s0 = HD, o = HD + 2 * keys;
+    static_assert(o + vd <= 512, "TMEM columns");
+    static constexpr int64_t part = kM * (vd + 2);           // floats of a part: acc [kM][vd], then (m, l) [kM]
 };
 
 // ---- tcgen05 ----
@@ -205,7 +212,7 @@ template <int HD, bool TMA>
 __global__ void __launch_bounds__(kThreads, 1)
 chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, int box) {
     using S = TcShape<HD>;
-    constexpr int HH = HD / 2;   // output dims of a thread
+    constexpr int kN = S::keys, VD = S::vd, HH = VD / 2, HQ = HD / 2;   // HH, HQ: output dims and dims of q of a thread
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full[S::slots], empty[S::slots], s_full[2], p_full[2][2], o_full[2], o_free, q_done;
     __shared__ float2 s_ml[2][kM];
@@ -213,7 +220,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
     __shared__ int abort_flag, odd_block[2];
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int kvh = blockIdx.y, split = blockIdx.z;
+    const int kvh = blockIdx.y / S::parts, v0 = (blockIdx.y % S::parts) * VD, split = blockIdx.z;   // v0: its first dim of V
     grid_dep_wait();
     grid_dep_launch();
     int seq, tile;
@@ -245,8 +252,8 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
     // q comes through the last slots of the ring, whole rows at a time (a thread that
     // read its own row from memory waited 7 us for rows 16 KB apart), 16-byte pieces
     // swizzled by the row so that a row a thread is read without bank conflicts
-    constexpr int kQSlots = 2;
-    static_assert(kM * HD * 4 == kQSlots * S::slot, "q fills whole slots");
+    constexpr int kQSlots = kM * HD * 4 / S::slot;
+    static_assert(kM * HD * 4 == kQSlots * S::slot && kQSlots < S::slots, "q fills whole slots");
     uint8_t* q_smem = ring_ptr + (S::slots - kQSlots) * S::slot;
     if (warp < kComputeWarps) {
         constexpr int PIECES = HD / 4;
@@ -316,25 +323,26 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
                     }
                 }
             };
-            auto put = [&](int place, const CUtensorMap* map, int page, int at) {
+            // dims [from, from + 64 * wide) of the block's keys
+            auto put = [&](int place, const CUtensorMap* map, int page, int at, int from, int wide) {
                 const int slot = place % S::slots;
                 if (place >= S::slots && !dead)
                     dead = !mbar_warp_wait(&empty[slot], static_cast<uint32_t>(place / S::slots - 1) & 1u, A.status, kStatusWaitTimeout);
                 else if (place >= S::slots - kQSlots && !dead)
                     dead = !mbar_warp_wait(&q_done, 0u, A.status, kStatusWaitTimeout);
                 if (dead) return;
-                if (lane == 0) mbar_arrive_expect_tx(&full[slot], mine);
+                if (lane == 0) mbar_arrive_expect_tx(&full[slot], mine * wide / (HD / 64));   // a warp's dims are every second 64 of a box, or all
                 __syncwarp();
-                if (c < copies) tma_4d(to + static_cast<uint32_t>(slot) * S::slot, map, x * 64, kvh, at, page, &full[slot]);
+                if (c < copies && x < wide) tma_4d(to + static_cast<uint32_t>(slot) * S::slot, map, from + x * 64, kvh, at, page, &full[slot]);
             };
             if (n > 0) {
                 int page, at, page1, at1;
                 find(0, page, at);
-                put(0, &kmap, page, at);
+                put(0, &kmap, page, at, 0, HD / 64);
                 for (int j = 0; j < n; ++j) {
                     find(j + 1, page1, at1);
-                    if (j + 1 < n) put(k_place(j + 1), &kmap, page1, at1);
-                    put(v_place(j, n), &vmap, page, at);
+                    if (j + 1 < n) put(k_place(j + 1), &kmap, page1, at1, 0, HD / 64);
+                    put(v_place(j, n), &vmap, page, at, v0, VD / 64);
                     page = page1;
                     at = at1;
                 }
@@ -344,6 +352,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
             }
         } else if (!TMA && warp >= kFirstProducer) {
             // ---- producers: warp w of them copies keys 64 w .. 64 w + 63 of every block ----
+            static_assert(TMA || (VD == HD && kN == 128), "the shapes that are copied without TMA");
             const int pw = warp - kFirstProducer;
             constexpr int PIECES = HD / 8;          // 16-byte pieces of a row
             constexpr int KEYS = kN / kProducerWarps, ROWS = 32 / PIECES;
@@ -462,7 +471,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
 #pragma unroll
                             for (int k = 0; k < kN / 32; ++k)
                                 mma_ts(tmem + S::o, p + 16 * k + (part == 0 ? 8 : 0), b + hf * (kN / 2) * 128 / 16 + k * 128,
-                                       idesc_f16(HD, true), hf > 0 || part > 0 || k > 0);
+                                       idesc_f16(VD, true), hf > 0 || part > 0 || k > 0);
                     }
                     if (!ok) break;
                     commit(&o_full[j & 1]);
@@ -494,17 +503,17 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
             const float f1 = ldexpf(1.f, -(e / 2)), f2 = fin ? ldexpf(1.f, -(e - e / 2)) : 0.f;
             sc = fin ? ldexpf(1.f, e) : NAN;
 #pragma unroll
-            for (int c = 0; c < HH / 32; ++c) {   // 32 dims of this thread's half: 16 columns
+            for (int c = 0; c < HQ / 32; ++c) {   // 32 dims of this thread's half: 16 columns
                 uint32_t hi[16], lo[16];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    float4 v = q4(half * HH / 4 + c * 8 + i);
+                    float4 v = q4(half * HQ / 4 + c * 8 + i);
                     if (!fin) v = make_float4(0.f, 0.f, 0.f, 0.f);
                     split_half2(v.x * f1 * f2, v.y * f1 * f2, hi[2 * i], lo[2 * i]);
                     split_half2(v.z * f1 * f2, v.w * f1 * f2, hi[2 * i + 1], lo[2 * i + 1]);
                 }
-                st16(tl + S::q_hi + half * HH / 2 + c * 16, hi);
-                st16(tl + S::q_lo + half * HH / 2 + c * 16, lo);
+                st16(tl + S::q_hi + half * HQ / 2 + c * 16, hi);
+                st16(tl + S::q_lo + half * HQ / 2 + c * 16, lo);
             }
             wait_st();
             fence_before();
@@ -516,9 +525,9 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
         const float slope2 = A.slopes ? A.slopes[h] * 1.44269504088896341f : 0.f;
         const bool plain = A.cap2 == 0.f && !A.slopes;
         float m = -INFINITY, l = 0.f;
-        float acc[HD];
+        float acc[VD];
 #pragma unroll
-        for (int i = 0; i < HD; ++i) acc[i] = 0.f;
+        for (int i = 0; i < VD; ++i) acc[i] = 0.f;
         bool ok = true;   // a wait that ran out is waited for no more; the loop goes on to its end
         const RowKeys keys = mask.row(pos);
 
@@ -535,16 +544,16 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
                 ld32(sb, s[0]);
                 wait_ld<32>(s[0]);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    if (c < 3) ld32(sb + (c + 1) * 32, s[(c + 1) & 1]);
+                for (int c = 0; c < kN / 32; ++c) {
+                    if (c + 1 < kN / 32) ld32(sb + (c + 1) * 32, s[(c + 1) & 1]);
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], s[c & 1][i], s[c & 1][i + 1]);
-                    if (c < 3) wait_ld<32>(s[(c + 1) & 1]);
+                    if (c + 1 < kN / 32) wait_ld<32>(s[(c + 1) & 1]);
                 }
             } else {
                 // the scores themselves go back into TMEM
 #pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
+                for (int c = 0; c < kN / 32; ++c) {
                     float s[32];
                     ld32(sb + c * 32, s);
                     wait_ld<32>(s);
@@ -599,7 +608,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
                 ok = ok && mbar_warp_wait(&full[place % S::slots], static_cast<uint32_t>(place / S::slots) & 1u, A.status, kStatusWaitTimeout);
                 const uint32_t me = threadIdx.x & 127;
                 bool odd = false;
-                for (uint32_t c = me * 16; c < S::slot; c += 128 * 16) {
+                for (uint32_t c = me * 16; c < kN * VD * 2; c += 128 * 16) {
                     const uint4 w = *reinterpret_cast<const uint4*>(vb + c);
                     odd |= nonfinite_h2(w.x) || nonfinite_h2(w.y) || nonfinite_h2(w.z) || nonfinite_h2(w.w);
                 }
@@ -610,7 +619,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
                     for (int kr = 0; kr < kN; ++kr) {
                         if (!keys.sees(j0 + kr)) continue;
 #pragma unroll
-                        for (int d = 0; d < HD; d += 8) {
+                        for (int d = 0; d < VD; d += 8) {
                             const uint4 w = *reinterpret_cast<const uint4*>(vb + (d >> 6) * (kN * 128) + kr * 128 + ((((d >> 3) & 7) ^ (kr & 7)) << 4));
                             const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -621,7 +630,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
                         }
                     }
                     named_barrier(1 + half, 128);
-                    for (uint32_t c = me * 2; c < S::slot; c += 128 * 2) {
+                    for (uint32_t c = me * 2; c < kN * VD * 2; c += 128 * 2) {
                         unsigned short& x = *reinterpret_cast<unsigned short*>(vb + c);
                         if ((x & 0x7C00u) == 0x7C00u) x = 0;
                     }
@@ -641,8 +650,8 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
             ld16(sb, s[0]);
             wait_ld<16>(s[0]);
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                if (c < 7) ld16(sb + (c + 1) * 16, s[(c + 1) & 1]);
+            for (int c = 0; c < kN / 16; ++c) {
+                if (c + 1 < kN / 16) ld16(sb + (c + 1) * 16, s[(c + 1) & 1]);
                 uint32_t hi[8], lo[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -651,14 +660,14 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
                     sum = fadd2(sum, p);
                     cut_half2(p, hi[i], lo[i]);
                 }
-                if (c < 7) wait_ld<16>(s[(c + 1) & 1]);   // before P goes over columns that are being read
+                if (c + 1 < kN / 16) wait_ld<16>(s[(c + 1) & 1]);   // before P goes over columns that are being read
                 st8(sb + c * 16, hi);
                 st8(sb + c * 16 + 8, lo);
-                if ((c & 3) == 3) {
+                if (c % (kN / 32) == kN / 32 - 1) {   // half of the keys
                     wait_st();
                     fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&p_full[half][c >> 2]);
+                    if (lane == 0) mbar_arrive(&p_full[half][c / (kN / 32)]);
                 }
             }
             l = fmaf(l, al, sum.x + sum.y);
@@ -669,15 +678,15 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
             ld32(tl + S::o, o[0]);
             wait_ld<32>(o[0]);
 #pragma unroll
-            for (int c = 0; c < HD / 32; ++c) {
-                if (c + 1 < HD / 32) ld32(tl + S::o + (c + 1) * 32, o[(c + 1) & 1]);
+            for (int c = 0; c < VD / 32; ++c) {
+                if (c + 1 < VD / 32) ld32(tl + S::o + (c + 1) * 32, o[(c + 1) & 1]);
 #pragma unroll
                 for (int i = 0; i < 32; i += 2) {
                     const float2 x = ffma2(make_float2(acc[c * 32 + i], acc[c * 32 + i + 1]), make_float2(al, al), make_float2(o[c & 1][i], o[c & 1][i + 1]));
                     acc[c * 32 + i] = x.x;
                     acc[c * 32 + i + 1] = x.y;
                 }
-                if (c + 1 < HD / 32) wait_ld<32>(o[(c + 1) & 1]);
+                if (c + 1 < VD / 32) wait_ld<32>(o[(c + 1) & 1]);
             }
             fence_before();
             __syncwarp();
@@ -707,33 +716,30 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
         }
         m = M;
         l = fmaf(other.y, fb, l * fa);
-        const int pair = static_cast<int>(blockIdx.x) * A.c.n_kv + kvh;
-        constexpr int64_t kPart = kM * (HD + 2);   // floats of a part: acc [kM][HD], then (m, l) [kM]
-        float* parts = A.part + static_cast<int64_t>(pair) * A.n_split * kPart;
+        float* part = A.part + ((static_cast<int64_t>(blockIdx.x) * gridDim.y + blockIdx.y) * A.n_split + split) * S::part;
         const float inv = n_parts > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;   // nothing seen: zeros
         // through shared memory, so that whole rows are written
         uint8_t* o_smem = ring_ptr + ((2 * kM * (HH + 2) * 4 + 1023) & ~1023);
 #pragma unroll
         for (int i = 0; i < HH / 4; ++i)
-            *reinterpret_cast<float4*>(o_smem + row * HD * 4 + (((half * (HH / 4) + i) ^ (row & 7)) << 4)) =
+            *reinterpret_cast<float4*>(o_smem + row * VD * 4 + (((half * (HH / 4) + i) ^ (row & 7)) << 4)) =
                 make_float4(res[4 * i] * inv, res[4 * i + 1] * inv, res[4 * i + 2] * inv, res[4 * i + 3] * inv);
         named_barrier(3, kComputeWarps * 32);
         if (!*abort_v) {
-            constexpr int PIECES = HD / 4;
-            float* part = parts + split * kPart;
+            constexpr int PIECES = VD / 4;
 #pragma unroll 4
             for (int i = 0; i < kM * PIECES / (kComputeWarps * 32); ++i) {
                 const int p = i * kComputeWarps * 32 + threadIdx.x, orow = p / PIECES, c = p % PIECES, rr = r0 + orow;
                 if (rr >= n_rows) break;   // rows rise with i
-                const float4 v = *reinterpret_cast<const float4*>(o_smem + orow * HD * 4 + ((c ^ (orow & 7)) << 4));
+                const float4 v = *reinterpret_cast<const float4*>(o_smem + orow * VD * 4 + ((c ^ (orow & 7)) << 4));
                 const int ot = A.group_div.div(rr);
-                float* dst = n_parts > 1 ? part + orow * HD
-                                         : A.out + static_cast<int64_t>(sv.q0 + ot) * A.ldo + static_cast<int64_t>(kvh * A.group + rr - ot * A.group) * HD;
+                float* dst = n_parts > 1 ? part + orow * VD
+                                         : A.out + static_cast<int64_t>(sv.q0 + ot) * A.ldo + static_cast<int64_t>(kvh * A.group + rr - ot * A.group) * HD + v0;
                 *reinterpret_cast<float4*>(dst + c * 4) = v;
             }
         }
         if (n_parts > 1) {
-            if (half == 0) *reinterpret_cast<float2*>(parts + split * kPart + kM * HD + row * 2) = make_float2(m, l);
+            if (half == 0) *reinterpret_cast<float2*>(part + kM * VD + row * 2) = make_float2(m, l);
         }
     }
     fence_before();
@@ -749,9 +755,9 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
 template <int HD>
 __global__ void __launch_bounds__(256)
 combine_kernel(const __grid_constant__ AttnArgs A) {
-    constexpr int64_t kPart = kM * (HD + 2);
-    constexpr int V = HD / 32, AHEAD = 8;   // values of a lane; parts whose loads are under way
-    const int lane = threadIdx.x & 31, kvh = blockIdx.y;
+    using S = TcShape<HD>;
+    constexpr int V = S::vd / 32, AHEAD = 8;   // values of a lane; parts whose loads are under way
+    const int lane = threadIdx.x & 31, kvh = blockIdx.y / S::parts, v0 = (blockIdx.y % S::parts) * S::vd;
     int seq, tile;
     grid_dep_wait();
     grid_dep_launch();
@@ -763,15 +769,14 @@ combine_kernel(const __grid_constant__ AttnArgs A) {
     if (!sv.ok || tile * kM >= n_rows || r >= n_rows) return;
     Mask mask{sv.len, A.window, 0};
     if (A.prefix) mask.prefix = max(0, min(A.prefix[seq], sv.len));
-    const KeyBlocks kb = key_blocks(mask, base + A.group_div.div(r0), base + A.group_div.div(min(r0 + kM - 1, n_rows - 1)), kN);
+    const KeyBlocks kb = key_blocks(mask, base + A.group_div.div(r0), base + A.group_div.div(min(r0 + kM - 1, n_rows - 1)), S::keys);
     const int n = max(1, (kb.n + A.blocks_per_split - 1) / A.blocks_per_split);
     if (n == 1) return;
-    const int64_t pair = static_cast<int64_t>(blockIdx.x) * A.c.n_kv + kvh;
-    const float* parts = A.part + pair * A.n_split * kPart;
-    const float* ml = parts + kM * HD + row * 2;
-    const float* acc = parts + static_cast<int64_t>(row) * HD + lane * V;
+    const float* parts = A.part + (static_cast<int64_t>(blockIdx.x) * gridDim.y + blockIdx.y) * A.n_split * S::part;
+    const float* ml = parts + kM * S::vd + row * 2;
+    const float* acc = parts + static_cast<int64_t>(row) * S::vd + lane * V;
     float M = -INFINITY;
-    for (int i = lane; i < n; i += 32) M = fmaxf(M, __ldcg(ml + i * kPart));
+    for (int i = lane; i < n; i += 32) M = fmaxf(M, __ldcg(ml + i * S::part));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     float L = 0.f, O[V];
@@ -783,9 +788,9 @@ combine_kernel(const __grid_constant__ AttnArgs A) {
 #pragma unroll
         for (int x = 0; x < AHEAD; ++x) {
             if (i0 + x >= n) break;
-            p[x] = __ldcg(reinterpret_cast<const float2*>(ml + (i0 + x) * kPart));
-            if constexpr (V == 2) *reinterpret_cast<float2*>(v[x]) = __ldcg(reinterpret_cast<const float2*>(acc + (i0 + x) * kPart));
-            else *reinterpret_cast<float4*>(v[x]) = __ldcg(reinterpret_cast<const float4*>(acc + (i0 + x) * kPart));
+            p[x] = __ldcg(reinterpret_cast<const float2*>(ml + (i0 + x) * S::part));
+            if constexpr (V == 2) *reinterpret_cast<float2*>(v[x]) = __ldcg(reinterpret_cast<const float2*>(acc + (i0 + x) * S::part));
+            else *reinterpret_cast<float4*>(v[x]) = __ldcg(reinterpret_cast<const float4*>(acc + (i0 + x) * S::part));
         }
 #pragma unroll
         for (int x = 0; x < AHEAD; ++x) {
@@ -799,7 +804,7 @@ combine_kernel(const __grid_constant__ AttnArgs A) {
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
     const int t = A.group_div.div(r);
-    float* o = A.out + static_cast<int64_t>(sv.q0 + t) * A.ldo + static_cast<int64_t>(kvh * A.group + r - t * A.group) * HD + lane * V;
+    float* o = A.out + static_cast<int64_t>(sv.q0 + t) * A.ldo + static_cast<int64_t>(kvh * A.group + r - t * A.group) * HD + v0 + lane * V;
 #pragma unroll
     for (int c = 0; c < V; c += 2) *reinterpret_cast<float2*>(o + c) = make_float2(O[c] * inv, O[c + 1] * inv);
 }
@@ -839,7 +844,7 @@ cudaError_t launch(const AttnArgs& a, int tiles, int box, cudaStream_t s) {
     }
     CUtensorMap k{}, v{};
     if (TMA && (!encode_pool(&k, a.c.k, a.c, box) || !encode_pool(&v, a.c.v, a.c, box))) return cudaErrorInvalidValue;
-    const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(a.c.n_kv), static_cast<unsigned>(a.n_split));
+    const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(a.c.n_kv * TcShape<HD>::parts), static_cast<unsigned>(a.n_split));
     e = launch_dep(chunk_kernel<HD, TMA>, grid, kThreads, TcShape<HD>::smem, s, a, k, v, box);
     if (e != cudaSuccess || a.n_split == 1) return e;
     const unsigned eights = static_cast<unsigned>((std::min(kM, a.b.max_new * a.group) + 7) / 8);
@@ -848,14 +853,22 @@ cudaError_t launch(const AttnArgs& a, int tiles, int box, cudaStream_t s) {
 
 }  // namespace
 
+// A box of the tiled copies lies in one page and one block of keys, and its rows
+// are whole groups of the swizzle; a tensor map's strides are below 2^40 bytes,
+// each a multiple of the one before it.
+bool paged_attention_tiled(const PagedLayer& c) {
+    return std::gcd(c.page_size, tc_keys(c.head_dim)) >= 8 && c.page_stride < (int64_t(1) << 39) &&
+           c.page_stride % (static_cast<int64_t>(c.n_kv) * c.head_dim) == 0;
+}
+
 cudaError_t paged_attention_tc(const AttnArgs& a, int tiles, cudaStream_t s) {
-    // a box of the tiled copies lies in one page and one block of keys, and its
-    // rows are whole groups of the swizzle; a tensor map's strides are below 2^40
-    // bytes, each a multiple of the one before it
-    const int box = std::gcd(a.c.page_size, kTcKeys);
-    const bool tma = box >= 8 && a.c.page_stride < (int64_t(1) << 39) && a.c.page_stride % (static_cast<int64_t>(a.c.n_kv) * a.c.head_dim) == 0;
-    if (a.c.head_dim == 64) return tma ? launch<64, true>(a, tiles, box, s) : launch<64, false>(a, tiles, box, s);
-    return tma ? launch<128, true>(a, tiles, box, s) : launch<128, false>(a, tiles, box, s);
+    const int box = std::gcd(a.c.page_size, tc_keys(a.c.head_dim));
+    const bool tma = paged_attention_tiled(a.c);
+    switch (a.c.head_dim) {
+        case 64: return tma ? launch<64, true>(a, tiles, box, s) : launch<64, false>(a, tiles, box, s);
+        case 128: return tma ? launch<128, true>(a, tiles, box, s) : launch<128, false>(a, tiles, box, s);
+        default: return tma ? launch<256, true>(a, tiles, box, s) : cudaErrorInvalidValue;   // the caller asks first
+    }
 }
 
 }  // namespace hesa_cuda

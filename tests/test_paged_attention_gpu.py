@@ -142,6 +142,10 @@ def test_next_token(T, n_head, n_kv, hd, page, lens):
     (8, 1, 128, 32, [5000], [40]),                     # few rows, many keys
     (2, 2, 64, 16, [1, 1, 2], [1, 1, 2]),
     (64, 8, 128, 64, [2100], [200]),
+    (4, 1, 256, 16, [700, 64, 260], [70, 64, 255]),
+    (16, 2, 256, 64, [3000], [100]),
+    (8, 8, 256, 8, [1, 190, 65], [1, 190, 30]),
+    (4, 2, 256, 20, [150, 500], [70, 21]),             # wide heads in pages that are no multiple of 8
 ])
 def test_chunk(T, n_head, n_kv, hd, page, lens, news):
     check(Case(T, n_head, n_kv, hd, page, lens, news, seed=hd + len(lens)))
@@ -209,10 +213,10 @@ def test_rows_that_see_nothing_are_zero(T):
     check(c, prefix=T.tensor([2, 0], dtype=T.int32, device="cuda"))
 
 
-@pytest.mark.parametrize("new", [1, 40, 200])
-def test_hidden_values_do_not_leak(T, new):
+@pytest.mark.parametrize("new,hd", [(1, 128), (40, 128), (200, 128), (200, 64), (200, 256), (1, 256)])
+def test_hidden_values_do_not_leak(T, new, hd):
     """NaN and infinities in keys and values that a row does not see leave it as it was."""
-    c = Case(T, 8, 2, 128, 16, [333], [new], seed=11)
+    c = Case(T, 8, 2, hd, 16, [333], [new], seed=11)
     window = 50
     ref, tol = c.exact(window=window)
     first = 333 - new
@@ -227,10 +231,11 @@ def test_hidden_values_do_not_leak(T, new):
         # token first + 20 is hidden from the first 20 rows and seen by the next
         j = first + 20
         p, s = int(table[j // 16]), j % 16
-        c.v[0, p, s, 0, 5] = math.nan
+        d = hd - 59
+        c.v[0, p, s, 0, d] = math.nan
         out = c.run(window=window)
         ok = T.ones(new, c.n_head, c.hd, dtype=T.bool, device="cuda")
-        ok[20:20 + window, :4, 5] = False
+        ok[20:20 + window, :4, d] = False
         good = ok.view(new, -1)
         assert float((out.double() - ref).abs()[good].max()) <= tol
         assert T.isnan(out[~good]).all()
