@@ -384,7 +384,8 @@ typedef struct {
  * A row that sees no key gives zeros. K and V at places that a row does not
  * see (padding, other sequences, places past a slot's length) do not reach
  * it, whatever they hold; a value that is not finite where it is seen gives a
- * result that is not finite. A row of q that is not finite gives NaN.
+ * result that is not finite (softcap may make a score of an infinite k finite).
+ * A row of q that is not finite gives NaN.
  * The workspace (16-byte aligned, need not be set) is scratch: calls of any
  * shape on one stream can share one of the largest size that they ask for,
  * calls that may overlap cannot. Results do not depend on scheduling. */
