@@ -37,8 +37,8 @@
 //     adds up the tiles' blocks itself. What lies in several runs leaves (m, l,
 //     acc) for each, which combine_kernel adds in the order of the runs.
 // Measured (both kernels): two contexts of 131072 and 100001 tokens, 64 heads on 8,
-// 167 us (6.4 TB/s); 32 of 1 to 8192 tokens 33.8 us (3.7 TB/s, the first copies and
-// the joining cost 10 of them); one of 2048 tokens, 32 heads, 14.7 us (2.3 TB/s).
+// 167 us (6.4 TB/s); 32 of 1 to 8192 tokens 34.2 us (3.7 TB/s, the first copies and
+// the joining cost 10 of them); one of 2048 tokens, 32 heads, 15.4 us (2.2 TB/s).
 #include "paged.h"
 #include "paged_tc.h"
 #include "abi_errors.h"

@@ -544,14 +544,20 @@ def _stream_on(device: int, stream):
     return _stream_handle(stream)
 
 
+def _stream_object(stream):
+    """torch's object for a stream that is given as one or as a handle."""
+    import torch
+    if not isinstance(stream, int):
+        return stream
+    return torch.cuda.ExternalStream(stream) if stream else torch.cuda.default_stream()
+
+
 def _new(make, stream):
     """A tensor made for a call on `stream`: allocated and filled there, so that it may be freed in that stream's order."""
     import torch
     if stream is None:
         return make()
-    if isinstance(stream, int):
-        stream = torch.cuda.ExternalStream(stream) if stream else torch.cuda.default_stream()
-    with torch.cuda.stream(stream):
+    with torch.cuda.stream(_stream_object(stream)):
         return make()
 
 
@@ -708,8 +714,8 @@ def _page_workspace(cache, workspace, stream):
         if cache.workspace is None:
             cache.workspace = kv_pages_workspace(cache)
         workspace = cache.workspace
-        if stream is not None and not isinstance(stream, int):
-            workspace.record_stream(stream)
+        if stream is not None:
+            workspace.record_stream(_stream_object(stream))
     else:
         _want(workspace, torch.uint8, "workspace", cache.device)
     return workspace

@@ -199,6 +199,31 @@ def test_a_call_that_cannot_be_carried_out_changes_nothing(T):
     H.clear_device_status()
 
 
+@pytest.mark.parametrize("handle", [False, True], ids=("object", "handle"))
+def test_page_operations_on_another_stream(T, handle):
+    """A stream given as torch's object or as a handle, with the cache's own scratch: ordered there, results as ever."""
+    H, c, m = fresh(T)
+    lists = [ints(T, v) for v in ([0, 3], [20, 9], [3, 0], [1, 4], [3])]
+    k = c.k.clone()
+    T.cuda.synchronize()
+    side = T.cuda.Stream()
+    on = side.cuda_stream if handle else side
+    H.kv_reserve(c, lists[0], lists[1], stream=on)
+    H.kv_fork(c, lists[2], lists[3], stream=on)
+    H.kv_free(c, lists[4], stream=on)
+    H.kv_compact(c, stream=on)
+    side.synchronize()
+    m.reserve([0, 3], [20, 9])
+    pairs = m.fork([3, 0], [1, 4])
+    m.free([3])
+    for a, b, n in pairs:
+        k[:, b, :n] = k[:, a, :n]
+    for a, b in m.compact()[1]:
+        k[:, b] = k[:, a]
+    same(c, m)
+    assert T.equal(c.k, k) and H.device_status() == 0
+
+
 def test_copy_pages_and_empty_lists(T):
     H, c, _ = fresh(T, n_layer=3, page=5)
     k, v = c.k.clone(), c.v.clone()
