@@ -593,6 +593,7 @@ int hesa_cuda_rope_kv_paged(const hesa_cuda_paged_kv* kv, int32_t layer, const h
     int rc = check_paged_kv(kv);
     if (rc == HESA_CUDA_OK) rc = check_batch(kv, layer, batch, n_head);
     if (rc != HESA_CUDA_OK) return rc;
+    if (batch->n_tokens == 0) return HESA_CUDA_OK;   // no rows: their buffers may be null
     if (!k || !v || (rope_table && !q)) return record_error(HESA_CUDA_INVALID_ARGUMENT, "null pointer");
     const int64_t kv_width = static_cast<int64_t>(kv->n_kv_head) * kv->head_dim;
     if (ldk < kv_width || ldv < kv_width || (rope_table && (ldq < n_head * kv->head_dim || rope_rows <= 0)))
@@ -601,7 +602,6 @@ int hesa_cuda_rope_kv_paged(const hesa_cuda_paged_kv* kv, int32_t layer, const h
         return record_error(HESA_CUDA_SHAPE_MISMATCH, "leading dimension too large");
     if (!aligned(k, 16) || !aligned(v, 16) || (ldk & 3) || (ldv & 3) || (rope_table && (!aligned(q, 16) || !aligned(rope_table, 16) || (ldq & 3))))
         return record_error(HESA_CUDA_INVALID_ARGUMENT, "q, k, v and the rope table must be 16-byte aligned with leading dimensions multiples of 4");
-    if (batch->n_tokens == 0) return HESA_CUDA_OK;
     int* status = nullptr;
     cudaError_t e = status_word(&status);
     if (e == cudaSuccess) {

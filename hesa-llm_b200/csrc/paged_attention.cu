@@ -797,6 +797,7 @@ int hesa_cuda_paged_attention(const hesa_cuda_paged_kv* kv, int32_t layer, const
     int rc = check_paged_kv(kv);
     if (rc == HESA_CUDA_OK) rc = check_batch(kv, layer, batch, n_head);
     if (rc != HESA_CUDA_OK) return rc;
+    if (batch->n_tokens == 0) return HESA_CUDA_OK;   // no rows: their buffers may be null
     if (!q || !out || !workspace) return record_error(HESA_CUDA_INVALID_ARGUMENT, "null pointer");
     const int64_t width = n_head * kv->head_dim;
     if (ldq < width || ldo < width || ldq > (int64_t(1) << 40) || ldo > (int64_t(1) << 40))
@@ -813,7 +814,7 @@ int hesa_cuda_paged_attention(const hesa_cuda_paged_kv* kv, int32_t layer, const
     if (o.softcap != 0.f && !(o.softcap >= 1e-6f && o.softcap <= 1e6f))
         return record_error(HESA_CUDA_INVALID_ARGUMENT, "softcap must be 0 or 1e-6 .. 1e6");
     if (!aligned(o.slopes, 4) || !aligned(o.prefix, 4)) return record_error(HESA_CUDA_INVALID_ARGUMENT, "slopes and prefix must be 4-byte aligned");
-    if (batch->n_tokens == 0 || batch->max_new == 0) return HESA_CUDA_OK;
+    if (batch->max_new == 0) return HESA_CUDA_OK;
 
     const Plan p = make_plan(kv, batch, n_head);
     AttnArgs a{};

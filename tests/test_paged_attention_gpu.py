@@ -385,6 +385,17 @@ def test_workspace_shared_by_shapes_and_streams_of_their_own(T):
     assert all(T.equal(g, want[0]) for g in got1) and all(T.equal(g, want[1]) for g in got2)
 
 
+def test_a_batch_without_rows(T):
+    """A step in which nothing is new: no error, nothing written."""
+    c = Case(T, 4, 2, 64, 16, [50, 3], [1, 1], seed=18)
+    none = c.H.TokenBatch(T.zeros(3, dtype=T.int32, device="cuda"), 0, 0, 50)
+    k, v = c.k.clone(), c.v.clone()
+    q = T.zeros(0, 256, device="cuda")
+    assert c.H.paged_attention(c.cache, 0, none, q, 4).shape == (0, 256)
+    c.H.rope_kv_paged(c.cache, 0, none, q, q[:, :128], q[:, :128], 4, rope_table=T.zeros(60, 64, device="cuda"))
+    assert T.equal(c.k.view(T.int16), k.view(T.int16)) and T.equal(c.v.view(T.int16), v.view(T.int16)) and c.H.device_status() == 0
+
+
 def test_refusals_of_the_binding(T):
     c = Case(T, 4, 2, 64, 16, [50], [1], seed=17)
     H = c.H

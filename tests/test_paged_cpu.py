@@ -82,7 +82,11 @@ def test_words_of_the_device_arrays_are_aligned():
 
 
 def test_nothing_to_attend_is_no_launch():
-    assert attend(b=batch(n_tokens=0, max_new=0)) == 0
+    """Nor do tensors without rows, whose pointers are null, make an error."""
+    none = batch(n_tokens=0, max_new=0)
+    assert attend(b=none) == 0 and attend(b=none, q=0, out=0) == 0
+    assert store(b=none, q=0, k=0, v=0) == 0
+    assert attend(b=none, layer=2) == 2 and store(b=batch(q_start=0, n_tokens=0, max_new=0)) == 2
 
 
 def test_attention_workspace_follows_the_cut():
