@@ -179,10 +179,10 @@ constexpr int kPagedPairs = 4096;
 // normal fp16 number, and the factor cancels in P V / sum P.
 constexpr float kPShift = 14.0f;
 
-// fp16 bits with an all-ones exponent in either half of a word
-__device__ __forceinline__ bool nonfinite_h2(uint32_t w) {
-    return (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u;
-}
+// Two fp16 values: a bit of kNonfinite is set for each whose exponent is all ones
+// (one more in the exponent carries into the sign's place).
+constexpr uint32_t kNonfinite = 0x80008000u;
+__device__ __forceinline__ uint32_t nonfinite_mark(uint32_t w) { return (w & 0x7FFF7FFFu) + 0x04000400u; }
 
 __device__ __forceinline__ float ex2(float x) {
     float y;

@@ -371,12 +371,12 @@ __device__ __forceinline__ void rows_segment(const AttnArgs& A, Ring& ring, cons
                 // NaN of an infinite or NaN v. Such values (there are none in a sound
                 // cache) are added where they are seen and then cleared, so that they
                 // reach no other row. Keys past the sequence are zeros.
-                bool odd = false;
+                uint32_t odd = 0;
                 for (int c = lane; c < kKeyBlock * HD / 8; c += 32) {
                     const uint4 w = *reinterpret_cast<const uint4*>(vp + (c / (HD / 8)) * ring.row + (c % (HD / 8)) * 16);
-                    odd |= nonfinite_h2(w.x) || nonfinite_h2(w.y) || nonfinite_h2(w.z) || nonfinite_h2(w.w);
+                    odd |= nonfinite_mark(w.x) | nonfinite_mark(w.y) | nonfinite_mark(w.z) | nonfinite_mark(w.w);
                 }
-                if (__any_sync(0xffffffffu, odd)) {
+                if (__any_sync(0xffffffffu, (odd & kNonfinite) != 0)) {
                     for (int j = 0; j < kKeyBlock; ++j) {
                         const bool seen = keys.sees(j0 + j);
                         const __half* vr = reinterpret_cast<const __half*>(vp + j * ring.row) + 2 * (lane & 3);

@@ -533,11 +533,51 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
 
         for (int j = half; j < n; j += 2) {   // `half`: the warpgroup, and its S buffer
             const int32_t j0 = kb.at(i0 + j) * kN;
+            const bool whole = mask.all(p_lo, p_hi, j0, j0 + kN);
+            if (!whole) {
+                // values of V that are not finite and hidden from some row: added where they are seen, then
+                // cleared (paged_attention.cu). Keys past the sequence are zeros, or what their page holds. Looked for
+                // while S is being made.
+                const int place = v_place(j, n);
+                uint8_t* vb = ring_ptr + static_cast<size_t>(place % S::slots) * S::slot;
+                ok = ok && mbar_warp_wait(&full[place % S::slots], static_cast<uint32_t>(place / S::slots) & 1u, A.status, kStatusWaitTimeout);
+                const uint32_t me = threadIdx.x & 127;
+                uint32_t odd = 0;
+#pragma unroll 8
+                for (uint32_t c = me * 16; c < kN * VD * 2; c += 128 * 16) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(vb + c);
+                    odd |= nonfinite_mark(w.x) | nonfinite_mark(w.y) | nonfinite_mark(w.z) | nonfinite_mark(w.w);
+                }
+                // (no warp of the group is a block ahead: the O that it has added last needed every warp's P)
+                if (odd & kNonfinite) odd_block[half] = j;
+                named_barrier(1 + half, 128);
+                if (*reinterpret_cast<volatile int*>(&odd_block[half]) == j) {
+                    for (int kr = 0; kr < kN; ++kr) {
+                        if (!keys.sees(j0 + kr)) continue;
+#pragma unroll
+                        for (int d = 0; d < VD; d += 8) {
+                            const uint4 w = *reinterpret_cast<const uint4*>(vb + (d >> 6) * (kN * 128) + kr * 128 + ((((d >> 3) & 7) ^ (kr & 7)) << 4));
+                            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const float x = half_bits_to_float(ws[i >> 1] >> (16 * (i & 1)));
+                                if (!isfinite(x)) acc[d + i] += x;
+                            }
+                        }
+                    }
+                    named_barrier(1 + half, 128);
+                    for (uint32_t c = me * 2; c < kN * VD * 2; c += 128 * 2) {
+                        unsigned short& x = *reinterpret_cast<unsigned short*>(vb + c);
+                        if ((x & 0x7C00u) == 0x7C00u) x = 0;
+                    }
+                    fence_proxy_async_smem();
+                    named_barrier(1 + half, 128);
+                }
+            }
             ok = ok && mbar_warp_wait(&s_full[half], static_cast<uint32_t>(j >> 1) & 1u, A.status, kStatusWaitTimeout);
             fence_after();
             const uint32_t sb = tl + S::s0 + half * kN;
             float k = sc;   // s * k is the score in base 2
-            const bool whole = mask.all(p_lo, p_hi, j0, j0 + kN);
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
             if (plain && whole) {
                 float s[2][32];
@@ -599,44 +639,6 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
                 }
                 wait_st();
                 k = 1.f;
-            }
-            if (!whole) {
-                // values of V that are not finite and hidden from some row: added where they are seen, then
-                // cleared (paged_attention.cu). Keys past the sequence are zeros, or what their page holds.
-                const int place = v_place(j, n);
-                uint8_t* vb = ring_ptr + static_cast<size_t>(place % S::slots) * S::slot;
-                ok = ok && mbar_warp_wait(&full[place % S::slots], static_cast<uint32_t>(place / S::slots) & 1u, A.status, kStatusWaitTimeout);
-                const uint32_t me = threadIdx.x & 127;
-                bool odd = false;
-                for (uint32_t c = me * 16; c < kN * VD * 2; c += 128 * 16) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(vb + c);
-                    odd |= nonfinite_h2(w.x) || nonfinite_h2(w.y) || nonfinite_h2(w.z) || nonfinite_h2(w.w);
-                }
-                // (no warp of the group is a block ahead: S of its next block needs every P of this one)
-                if (odd) odd_block[half] = j;
-                named_barrier(1 + half, 128);
-                if (*reinterpret_cast<volatile int*>(&odd_block[half]) == j) {
-                    for (int kr = 0; kr < kN; ++kr) {
-                        if (!keys.sees(j0 + kr)) continue;
-#pragma unroll
-                        for (int d = 0; d < VD; d += 8) {
-                            const uint4 w = *reinterpret_cast<const uint4*>(vb + (d >> 6) * (kN * 128) + kr * 128 + ((((d >> 3) & 7) ^ (kr & 7)) << 4));
-                            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const float x = half_bits_to_float(ws[i >> 1] >> (16 * (i & 1)));
-                                if (!isfinite(x)) acc[d + i] += x;
-                            }
-                        }
-                    }
-                    named_barrier(1 + half, 128);
-                    for (uint32_t c = me * 2; c < kN * VD * 2; c += 128 * 2) {
-                        unsigned short& x = *reinterpret_cast<unsigned short*>(vb + c);
-                        if ((x & 0x7C00u) == 0x7C00u) x = 0;
-                    }
-                    fence_proxy_async_smem();
-                    named_barrier(1 + half, 128);
-                }
             }
             float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * k;
             // k is NaN for a row that is not finite: so are its maximum, its P and its result
