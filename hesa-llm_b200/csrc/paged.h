@@ -86,13 +86,15 @@ __host__ __device__ inline int64_t tile_bound(int64_t n_tokens, int64_t n_seq, i
     return n_tokens * g / r + n_seq;
 }
 
-__device__ __forceinline__ void locate_tile(const BatchView& b, int g, int r, int per_seq, int idx, int& seq, int& tile) {
+// Tile idx of the launch: tile `tile` (>= 0, and possibly behind its rows) of
+// sequence seq; false where it is no sequence's.
+__host__ __device__ __forceinline__ bool locate_tile(const BatchView& b, int g, int r, int per_seq, int idx, int& seq, int& tile) {
     if (per_seq > 0) {
         seq = idx / per_seq;
         tile = idx - seq * per_seq;
-        return;
+        return true;
     }
-    int lo = 0, hi = b.n_seq - 1;   // the last s with start(s) <= idx; in range whatever q_start holds
+    int lo = 0, hi = b.n_seq - 1;   // the last s with start(s) <= idx, or 0; in range whatever q_start holds
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         const int64_t at = static_cast<int64_t>(b.q_start[mid]) * g / r + mid;
@@ -100,7 +102,9 @@ __device__ __forceinline__ void locate_tile(const BatchView& b, int g, int r, in
         else hi = mid - 1;
     }
     seq = lo;
-    tile = idx - static_cast<int>(static_cast<int64_t>(b.q_start[lo]) * g / r + lo);
+    const int64_t behind = idx - (static_cast<int64_t>(b.q_start[lo]) * g / r + lo);
+    tile = behind < 0 ? 0 : behind < idx ? static_cast<int>(behind) : idx;   // more than idx: q_start[lo] < 0, which seq_view refuses
+    return behind >= 0;
 }
 
 // Key j is seen from position p: j < len and ((j <= p and (no window, or

@@ -184,9 +184,9 @@ struct TileView {
 __device__ __forceinline__ TileView tile_view(const AttnArgs& A, int idx) {
     TileView v;
     int seq, tile;
-    locate_tile(A.b, A.group, kRowTile, A.per_seq, A.tile0 + idx, seq, tile);
+    const bool some = locate_tile(A.b, A.group, kRowTile, A.per_seq, A.tile0 + idx, seq, tile);
     v.sv = seq_view(A.c, A.b, seq);
-    v.n_rows = v.sv.n_new * A.group;
+    v.n_rows = some ? v.sv.n_new * A.group : 0;
     v.r0 = tile * kRowTile;
     v.base = v.sv.len - v.sv.n_new;
     v.p_lo = v.base + A.group_div.div(v.r0);

@@ -224,7 +224,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
     grid_dep_wait();
     grid_dep_launch();
     int seq, tile;
-    locate_tile(A.b, A.group, kM, A.per_seq, static_cast<int>(blockIdx.x), seq, tile);
+    if (!locate_tile(A.b, A.group, kM, A.per_seq, static_cast<int>(blockIdx.x), seq, tile)) return;
     const SeqView sv = seq_view(A.c, A.b, seq);
     if (!sv.ok) {
         if (threadIdx.x == 0) record_status(A.status, kStatusBadPosition);
@@ -763,7 +763,7 @@ combine_kernel(const __grid_constant__ AttnArgs A) {
     int seq, tile;
     grid_dep_wait();
     grid_dep_launch();
-    locate_tile(A.b, A.group, kM, A.per_seq, static_cast<int>(blockIdx.x), seq, tile);
+    if (!locate_tile(A.b, A.group, kM, A.per_seq, static_cast<int>(blockIdx.x), seq, tile)) return;
     const SeqView sv = seq_view(A.c, A.b, seq);
     const int n_rows = sv.n_new * A.group;
     const int r0 = ((n_rows + kM - 1) / kM - 1 - tile) * kM, base = sv.len - sv.n_new;

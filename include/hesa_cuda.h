@@ -350,7 +350,8 @@ typedef struct {
  * and the output are sequence i's, the last ones of its slot's seq_len tokens
  * (hesa_cuda_kv_reserve has counted them): row q_start[i] + t has position
  * seq_len - (q_start[i + 1] - q_start[i]) + t. A sequence may have no new
- * token; rows from q_start[n_seq] on are left as they are. The numbers are
+ * token; rows before q_start[0] and from q_start[n_seq] on are left as they
+ * are, so that a part of a longer q_start is a batch too. The numbers are
  * read on the device, so that a captured graph serves every step; the host
  * gives their bounds: rows in all (n_tokens, the rows of the buffers), most
  * new tokens (max_new) and most tokens (max_len) of a sequence. A sequence
@@ -359,7 +360,7 @@ typedef struct {
  * the pool, which reads as zeros. */
 typedef struct {
     const int32_t* slots;    /* device [n_seq], or NULL: sequence i is in slot i */
-    const int32_t* q_start;  /* device [n_seq + 1], ascending from 0 */
+    const int32_t* q_start;  /* device [n_seq + 1], ascending from 0 or more */
     int32_t n_seq, n_tokens, max_new, max_len;
 } hesa_cuda_token_batch;
 
