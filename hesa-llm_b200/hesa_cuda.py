@@ -566,8 +566,9 @@ class PagedKV:
     [n_layer, n_pages, page_size, n_kv_head, head_dim] (any layer and page
     strides, the rest contiguous), the tables table [n_slots, max_pages],
     seq_len [n_slots] and page_refs [n_pages] (int32; page_refs may be None
-    without page operations). Keeps the tensors and a scratch buffer for the
-    page operations; everything lies on one CUDA device."""
+    without page operations). Keeps the tensors, and scratch of the page
+    operations for each stream that they ran on; everything lies on one CUDA
+    device."""
 
     def __init__(self, k, v, table, seq_len, page_refs=None):
         import torch
@@ -591,7 +592,7 @@ class PagedKV:
         self.struct = PagedKVStruct(k.data_ptr(), v.data_ptr(), k.stride(1), k.stride(0), n_layer, n_pages, page, n_kv, hd,
                                     table.data_ptr(), seq_len.data_ptr(), _ptr(page_refs), table.shape[0], table.shape[1])
         self.ref = ctypes.byref(self.struct)
-        self.workspace = None
+        self.scratch = {}   # of the page operations, by stream handle
 
     @classmethod
     def empty(cls, n_layer: int, n_pages: int, page_size: int, n_kv_head: int, head_dim: int, n_slots: int, max_pages: int):
@@ -708,16 +709,21 @@ def kv_pages_workspace(cache):
 
 
 def _page_workspace(cache, workspace, stream):
+    """The workspace of a page operation: the caller's, or scratch that was allocated on the very stream that the call
+    runs on (nothing else orders its kernels behind the memory's earlier use there). The cache keeps one for each stream
+    that was current at such a call; a given stream's, and a captured call's, lasts for the call alone (in a graph: is
+    the graph's own)."""
     import torch
     _same_device(cache)
-    if workspace is None:
-        if cache.workspace is None:
-            cache.workspace = kv_pages_workspace(cache)
-        workspace = cache.workspace
-        if stream is not None:
-            workspace.record_stream(_stream_object(stream))
-    else:
+    if workspace is not None:
         _want(workspace, torch.uint8, "workspace", cache.device)
+        return workspace
+    if stream is not None or torch.cuda.is_current_stream_capturing():
+        return _new(lambda: kv_pages_workspace(cache), stream)
+    handle = torch._C._cuda_getCurrentRawStream(cache.device)
+    workspace = cache.scratch.get(handle)
+    if workspace is None:
+        workspace = cache.scratch[handle] = kv_pages_workspace(cache)
     return workspace
 
 

@@ -6,6 +6,7 @@ import subprocess
 import pytest
 
 import hesa_build
+import hesa_cuda as H
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 OUT_DIR = os.path.join(ROOT, "tests", "cpp", "_build")
@@ -48,3 +49,63 @@ def test_starts_that_are_not_sound_stay_in_range(tiles_of):
     for starts in ([-4, 3, 9], [9, 3, 20], [2 ** 31 - 1, 5, 7], [-2 ** 31, -2 ** 31, 2 ** 31 - 1], [0, -4, 9]):
         got = tiles_of(8, 8, starts, 40)
         assert all(0 <= s < len(starts) - 1 and -1 <= at <= 8 * len(got) for s, at in got)
+
+
+class Streams:
+    """torch's streams as the binding uses them: which one is current, which ones capture."""
+
+    def __init__(self, monkeypatch):
+        import contextlib
+
+        import torch
+        self.now, self.capturing = 100, set()
+
+        @contextlib.contextmanager
+        def on(stream):
+            was, self.now = self.now, stream.cuda_stream
+            yield
+            self.now = was
+        monkeypatch.setattr(torch.cuda, "stream", on)
+        monkeypatch.setattr(torch.cuda, "ExternalStream", Stream)
+        monkeypatch.setattr(torch.cuda, "default_stream", lambda: Stream(0))
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: self.now in self.capturing)
+        monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: self.now)
+        monkeypatch.setattr(H, "_same_device", lambda cache, batch=None: None)
+        monkeypatch.setattr(H, "kv_pages_workspace", lambda cache: Scratch(self.now))
+
+
+class Stream:
+    def __init__(self, handle):
+        self.cuda_stream = handle
+
+
+class Scratch:
+    """A buffer that torch's allocator took from the memory of the stream that was current."""
+
+    def __init__(self, home):
+        self.home = home
+
+    def record_stream(self, stream):
+        pass
+
+
+class Cache:
+    def __init__(self):
+        self.scratch, self.workspace, self.device = {}, None, 0
+
+
+def test_scratch_of_page_operations_comes_from_the_calls_own_stream(monkeypatch):
+    """Whatever was current when the cache first needed some, and wherever the next call runs: memory of one stream is
+    never handed to kernels of another, and no captured graph shares it with eager calls or with another graph."""
+    s, c = Streams(monkeypatch), Cache()
+    for stream in (Stream(7), 7, None, Stream(8), 0, None):
+        want = s.now if stream is None else stream if isinstance(stream, int) else stream.cuda_stream
+        assert H._page_workspace(c, None, stream).home == want
+    s.now = 200
+    eager = H._page_workspace(c, None, None)
+    assert eager.home == 200 and H._page_workspace(c, None, None) is eager
+    s.capturing.add(200)
+    captured = [H._page_workspace(c, None, None) for _ in range(2)]
+    assert captured[0] is not captured[1] and eager not in captured and all(x.home == 200 for x in captured)
+    s.capturing.clear()
+    assert H._page_workspace(c, None, None) is eager

@@ -41,3 +41,49 @@ def test_a_batch_that_is_part_of_a_longer_one(T, n_head, n_kv, hd, before, news)
     at = c.cache.table[last, p // 16].item()
     assert T.equal(c.k[0, at, p % 16].reshape(-1), k[before + c.starts[last + 1] - 1, :n_kv * hd].half())
     assert c.H.device_status() == 0
+
+
+def test_page_operations_beside_a_busy_stream(T):
+    """Scratch for a call on another stream, while the current one still uses memory that it has given back; then by turns
+    on three streams, one of them current without being named, and captured."""
+    import hesa_cuda as H
+    from test_kv_pages_gpu import Model, fresh, ints, same
+    _, c, m = fresh(T, n_layer=3, n_pages=60)
+    assert isinstance(m, Model)
+    k, v = c.k.clone(), c.v.clone()
+    lists = {x: ints(T, x) for x in ((0,), (1,), (2,), (3,), (4,), (0, 1), (2, 3), (19, 30), (7,))}
+
+    def copied(pairs):
+        for a, b, n in pairs:
+            k[:, b, :n] = k[:, a, :n]
+            v[:, b, :n] = v[:, a, :n]
+    need = H.kv_pages_workspace(c).numel()
+    s1, s2 = T.cuda.Stream(), T.cuda.Stream()
+    T.cuda.synchronize()
+    T.cuda._sleep(20_000_000)                                   # about 10 ms
+    gone = [T.full((need,), 255, dtype=T.uint8, device="cuda") for _ in range(8)]   # written behind the sleep
+    del gone                                                    # to the allocator, while those writes are queued
+    H.kv_reserve(c, lists[0, 1], lists[19, 30], stream=s1)
+    H.kv_fork(c, lists[0, 1], lists[2, 3], stream=s1)
+    s2.wait_stream(s1)
+    with T.cuda.stream(s2):
+        H.kv_free(c, lists[1,])
+        H.kv_compact(c)
+    T.cuda.current_stream().wait_stream(s2)
+    H.kv_reserve(c, lists[4,], lists[7,])
+    m.reserve([0, 1], [19, 30])
+    copied(m.fork([0, 1], [2, 3]))
+    m.free([1])
+    copied([(a, b, m.page) for a, b in m.compact()[1]])
+    m.reserve([4], [7])
+    same(c, m)
+    assert T.equal(c.k, k) and T.equal(c.v, v)
+    g = T.cuda.CUDAGraph()
+    with T.cuda.graph(g):                                       # without a workspace: the graph has its own
+        H.kv_free(c, lists[3,])
+        H.kv_fork(c, lists[0,], lists[3,])
+    g.replay()
+    m.free([3])
+    copied(m.fork([0], [3]))
+    same(c, m)
+    assert T.equal(c.k, k) and T.equal(c.v, v) and H.device_status() == 0
