@@ -662,7 +662,10 @@ Plan make_plan(const hesa_cuda_paged_kv* kv, const hesa_cuda_token_batch* b, int
         // more than about 44 GB/s: where that would leave SMs without work, groups
         // of fewer heads. One context of 100 tokens, 64 heads on 8: 13.2 us with all
         // heads together, 10.3 with two; one of 2048 tokens, 32 heads: 14.3 with eight, 16.5 with two.
-        const int64_t blocks = (b->max_len + kKeyBlock - 1) / kKeyBlock;
+        // (A tile that sees no key is a block of work too. The loop ends with fewer
+        // than 4 kRowsCtas (tile, group)s, and kMostTiles of them can be listed.)
+        const int64_t blocks = std::max<int64_t>(1, (b->max_len + kKeyBlock - 1) / kKeyBlock);
+        static_assert(4 * kRowsCtas <= kMostTiles, "a list for every (tile, group) where groups are made smaller");
         p.heads = kv->head_dim == 256 ? 4 : 8;
         while (p.heads > 2 && tiles * ((kv->n_kv_head + p.heads - 1) / p.heads) * blocks < 2 * kRowsCtas) p.heads /= 2;
         return p;

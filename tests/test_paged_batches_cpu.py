@@ -1,4 +1,5 @@
 """How a ragged batch is cut into tiles, and the bindings' handling of streams, without a GPU."""
+import ctypes
 import os
 import random
 import subprocess
@@ -109,3 +110,16 @@ def test_scratch_of_page_operations_comes_from_the_calls_own_stream(monkeypatch)
     assert captured[0] is not captured[1] and eager not in captured and all(x.home == 200 for x in captured)
     s.capturing.clear()
     assert H._page_workspace(c, None, None) is eager
+
+
+@pytest.mark.parametrize("n_seq,n_kv,hd", [(1024, 32, 128), (1024, 8, 64), (200, 16, 64), (300, 17, 256), (1, 8, 128)])
+def test_lengths_of_no_token_are_cut_like_lengths_of_one(n_seq, n_kv, hd):
+    """A batch whose bound says that nobody has a key yet: a block a tile, as where everybody has one. (Cut into groups of
+    two heads whatever the number of tiles, the list of what is joined would be longer than its place.)"""
+    size = {}
+    for max_len in (0, 1, 16):
+        kv = H.PagedKVStruct(k=1 << 20, v=1 << 20, page_stride=16 * n_kv * hd, layer_stride=0, n_layer=1, n_pages=4, page_size=16, n_kv_head=n_kv,
+                             head_dim=hd, table=1 << 20, seq_len=1 << 20, page_refs=None, n_slots=n_seq, max_pages=4)
+        b = H.TokenBatchStruct(slots=None, q_start=1 << 20, n_seq=n_seq, n_tokens=n_seq, max_new=1, max_len=max_len)
+        size[max_len] = H.lib().hesa_cuda_paged_attention_workspace_size(ctypes.byref(kv), ctypes.byref(b), n_kv)
+    assert 0 < size[0] == size[1] == size[16]

@@ -87,3 +87,18 @@ def test_page_operations_beside_a_busy_stream(T):
     copied(m.fork([0], [3]))
     same(c, m)
     assert T.equal(c.k, k) and T.equal(c.v, v) and H.device_status() == 0
+
+
+@pytest.mark.parametrize("n_seq,n_head,n_kv,hd", [(1024, 32, 32, 128), (1024, 8, 8, 64), (200, 64, 16, 64), (300, 17, 17, 256), (3, 64, 8, 128),
+                                                  (5, 8, 2, 128)])
+@pytest.mark.parametrize("new", [1, 40])
+def test_nobody_has_a_key(T, n_seq, n_head, n_kv, hd, new):
+    """New rows of sequences without tokens see nothing: zeros, in every row."""
+    n_seq = min(n_seq, 60) if new > 1 else n_seq
+    c = Case(T, n_head, n_kv, hd, 16, [0] * n_seq, [new] * n_seq, seed=22)
+    out = T.full_like(c.q, 7.0)
+    ws = c.H.paged_attention_workspace(c.cache, c.batch, n_head).fill_(255)
+    for _ in range(3):
+        c.run(out=out, workspace=ws)
+        assert not out.any() and c.H.device_status() == 0
+        out.fill_(7.0)
