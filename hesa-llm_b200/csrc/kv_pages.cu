@@ -135,6 +135,19 @@ __device__ bool slots_sound(const Tables& t, const int32_t* slots, int n) {
     return !__syncthreads_or(bad);
 }
 
+// One reference more or less for every page of the (sound) slots; false when a
+// page had none left to take. All threads of the block; a barrier at its end.
+__device__ bool add_refs(const Tables& t, const int32_t* slots, int n, int by) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    bool bad = false;
+    for (int i = warp; i < n; i += kPlanThreads / 32) {
+        const int np = pages_for(t.seq_len[slots[i]], t.page_size);
+        const int32_t* row = t.table + static_cast<int64_t>(slots[i]) * t.max_pages;
+        for (int j = lane; j < np; j += 32) bad |= atomicAdd(&t.refs[row[j]], by) + by < 0;
+    }
+    return !__syncthreads_or(bad);
+}
+
 __device__ __forceinline__ void refuse(const Tables& t, int code) {
     if (threadIdx.x == 0) record_status(t.status, code);
 }
@@ -145,15 +158,17 @@ free_kernel(const Tables t, const int32_t* slots, int n) {
     grid_dep_launch();
     __shared__ uint32_t bits[kMaxSlots / 32];
     if (!mark_slots(slots, n, t.n_slots, bits) || !slots_sound(t, slots, n)) return refuse(t, kStatusBadPosition);
+    // A page that the slots hold more often than it has references would end below
+    // zero: the references are taken, and given back if one was not there.
+    if (!add_refs(t, slots, n, -1)) {
+        add_refs(t, slots, n, 1);
+        return refuse(t, kStatusBadPosition);
+    }
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int i = warp; i < n; i += kPlanThreads / 32) {
         const int s = slots[i];
         const int np = pages_for(t.seq_len[s], t.page_size);
-        for (int j = lane; j < np; j += 32) {
-            int32_t* e = t.table + static_cast<int64_t>(s) * t.max_pages + j;
-            atomicSub(&t.refs[*e], 1);
-            *e = -1;
-        }
+        for (int j = lane; j < np; j += 32) t.table[static_cast<int64_t>(s) * t.max_pages + j] = -1;
         __syncwarp();
         if (lane == 0) t.seq_len[s] = 0;
     }

@@ -102,3 +102,37 @@ def test_nobody_has_a_key(T, n_seq, n_head, n_kv, hd, new):
         c.run(out=out, workspace=ws)
         assert not out.any() and c.H.device_status() == 0
         out.fill_(7.0)
+
+
+@pytest.mark.parametrize("how", ["two slots", "one slot", "with a sound one"])
+def test_pages_held_more_often_than_they_have_references(T, how):
+    """Freeing what holds a page twice that has one reference: status 3, and nothing has changed."""
+    import hesa_cuda as H
+    from test_kv_pages_gpu import fresh, ints, same
+    _, c, m = fresh(T, n_pages=300, page=4, n_slots=6, max_pages=80)
+    H.kv_reserve(c, ints(T, [0, 1, 2, 5]), ints(T, [300, 33, 8, 9]))
+    m.reserve([0, 1, 2, 5], [300, 33, 8, 9])
+    if how == "one slot":
+        m.refs[m.rows[0][70]] = 0
+        m.rows[0][70] = m.rows[0][3]
+    else:
+        m.refs[m.rows[1][8]] = 0
+        m.rows[1][8] = m.rows[0][74]
+    c.table.copy_(T.tensor(m.rows, dtype=T.int32))
+    c.page_refs.copy_(T.tensor(m.refs, dtype=T.int32))
+    for _ in range(2):
+        H.kv_free(c, ints(T, {"two slots": [1, 0], "one slot": [0], "with a sound one": [2, 0, 5, 1]}[how]))
+        assert H.device_status() == 3
+        H.clear_device_status()
+        same(c, m)
+    H.kv_free(c, ints(T, [5, 2]))
+    m.free([5, 2])
+    same(c, m)
+    if how == "two slots":                       # with its second reference it goes
+        m.refs[m.rows[0][74]] += 1
+        c.page_refs.copy_(T.tensor(m.refs, dtype=T.int32))
+        H.kv_free(c, ints(T, [1, 0]))
+        m.free([1, 0])
+        same(c, m)
+    H.kv_compact(c)
+    assert H.device_status() == 0
