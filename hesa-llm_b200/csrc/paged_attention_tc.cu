@@ -609,9 +609,15 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
                             s[i + 1] = x.y;
                             far = fmax3(far, fabsf(x.x), fabsf(x.y));
                         }
+                        // which form a score takes goes by its own size alone, so that no other key or row changes it
                         if (__any_sync(0xffffffffu, far > 0.6f)) {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) s[i] = A.cap2 * tanhf(s[i]);
+                            for (int i = 0; i < 32; i += 2) {
+                                const float2 y = capped2_small(make_float2(s[i], s[i + 1]), A.cap2);
+                                const float t0 = A.cap2 * tanhf(s[i]), t1 = A.cap2 * tanhf(s[i + 1]);
+                                s[i] = fabsf(s[i]) > 0.6f ? t0 : y.x;
+                                s[i + 1] = fabsf(s[i + 1]) > 0.6f ? t1 : y.y;
+                            }
                         } else {
 #pragma unroll
                             for (int i = 0; i < 32; i += 2) {

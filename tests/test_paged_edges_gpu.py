@@ -136,3 +136,19 @@ def test_pages_held_more_often_than_they_have_references(T, how):
         same(c, m)
     H.kv_compact(c)
     assert H.device_status() == 0
+
+
+@pytest.mark.parametrize("n_head,n_kv,hd,page", [(8, 2, 128, 16), (8, 2, 64, 7), (4, 4, 256, 16)])
+def test_a_capped_row_depends_on_what_it_sees_alone(T, n_head, n_kv, hd, page):
+    """Scores far from zero, of hidden keys and of other rows, change no bit of a row whose own are near it."""
+    new, n, cap = 150, 400, 30.0
+    c = Case(T, n_head, n_kv, hd, page, [n], [new], seed=33)
+    was = c.run(softcap=cap)
+    j = n - 20
+    c.k[0, int(c.cache.table[0, j // page]), j % page] = 3000.0
+    out = c.run(softcap=cap)
+    assert T.equal(out[:new - 20], was[:new - 20]) and not T.equal(out[new - 20:], was[new - 20:])
+    c.q[37] *= 50.0
+    again = c.run(softcap=cap)
+    assert T.equal(again[:37], was[:37]) and T.equal(again[38:], out[38:]) and not T.equal(again[37], out[37])
+    assert T.isfinite(again).all() and c.H.device_status() == 0
