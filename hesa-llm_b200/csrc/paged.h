@@ -206,6 +206,20 @@ __device__ __forceinline__ void split_half2(float x0, float x1, uint32_t& hi, ui
     lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
+// x = hi + lo to 21 bits, |x| < 2^15, for q: hi is x taken away from zero to 11
+// bits, so that lo is zero or has the other sign. The score of an infinite k is then
+// inf - inf or 0 inf: NaN in every row that sees it, as for a k that is NaN,
+// whatever its sign and a cap on scores. (With hi to nearest, one bit more, it was
+// -inf, which is a weight of 0, or NaN, as q's low bits had it; looking for -inf in
+// the blocks' scores took 2 to 4% of a chunk's time.)
+__device__ __forceinline__ void split_away2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+    const float h0 = __uint_as_float((__float_as_uint(x0) + 0x1FFFu) & 0xFFFFE000u), h1 = __uint_as_float((__float_as_uint(x1) + 0x1FFFu) & 0xFFFFE000u);
+    const __half2 h = __floats2half2_rn(h0, h1);   // exact from 2^-14 on; below, lo is rounded to zero
+    const __half2 l = __floats2half2_rn(x0 - h0, x1 - h1);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
 // Launch with programmatic stream serialization: the grid may be set up while
 // the previous kernel on the stream finishes. Every block of such a kernel calls
 // grid_dep_wait, also one with nothing to do (the grid must not end before the one

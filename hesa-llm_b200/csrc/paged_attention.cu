@@ -12,7 +12,7 @@
 // <= 8 is one tile: every K and V byte is read once). Bound by HBM; the
 // tensor-core work is two m16n8k16 products a key and 128 dims.
 //   * fp32 accuracy from fp16 products: q and P are split into a high and a low
-//     fp16 half (22 bits; K and V are fp16 already, products are exact and sums
+//     fp16 half (21 and 22 bits; K and V are fp16 already, products are exact and sums
 //     are fp32). The 16 rows of the A operand are the 8 rows' high halves and
 //     their low halves, so the split costs no product more: thread (row, 2
 //     columns) holds the high part in c0, c1 and the low part in c2, c3 and adds
@@ -313,7 +313,7 @@ __device__ __forceinline__ void rows_segment(const AttnArgs& A, Ring& ring, cons
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const float x = fin ? v[k][i].x * f1 * f2 : 0.f, y = fin ? v[k][i].y * f1 * f2 : 0.f;
-                split_half2(x, y, qa[k][2 * i], qa[k][2 * i + 1]);
+                split_away2(x, y, qa[k][2 * i], qa[k][2 * i + 1]);
             }
     }
     const float sc = A.cap2 != 0.f ? qscale : qscale * A.scale2;

@@ -509,8 +509,8 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
                 for (int i = 0; i < 8; ++i) {
                     float4 v = q4(half * HQ / 4 + c * 8 + i);
                     if (!fin) v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    split_half2(v.x * f1 * f2, v.y * f1 * f2, hi[2 * i], lo[2 * i]);
-                    split_half2(v.z * f1 * f2, v.w * f1 * f2, hi[2 * i + 1], lo[2 * i + 1]);
+                    split_away2(v.x * f1 * f2, v.y * f1 * f2, hi[2 * i], lo[2 * i]);
+                    split_away2(v.z * f1 * f2, v.w * f1 * f2, hi[2 * i + 1], lo[2 * i + 1]);
                 }
                 st16(tl + S::q_hi + half * HQ / 2 + c * 16, hi);
                 st16(tl + S::q_lo + half * HQ / 2 + c * 16, lo);

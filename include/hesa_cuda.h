@@ -384,9 +384,9 @@ typedef struct {
  * row strides ldq, ldo (multiples of 4), 16-byte aligned and not overlapping.
  * A row that sees no key gives zeros. K and V at places that a row does not
  * see (padding, other sequences, places past a slot's length) do not reach
- * it, whatever they hold; a value that is not finite where it is seen gives a
- * result that is not finite (softcap may make a score of an infinite k finite).
- * A row of q that is not finite gives NaN.
+ * it, whatever they hold. A k that is not finite where a row sees it gives NaN
+ * in all of the row's dims, whatever its sign and the softcap; such a v gives a
+ * result that is not finite in its dim. A row of q that is not finite gives NaN.
  * The workspace (16-byte aligned, need not be set) is scratch: calls of any
  * shape on one stream can share one of the largest size that they ask for,
  * calls that may overlap cannot. Results do not depend on scheduling. */

@@ -152,3 +152,51 @@ def test_a_capped_row_depends_on_what_it_sees_alone(T, n_head, n_kv, hd, page):
     again = c.run(softcap=cap)
     assert T.equal(again[:37], was[:37]) and T.equal(again[38:], out[38:]) and not T.equal(again[37], out[37])
     assert T.isfinite(again).all() and c.H.device_status() == 0
+
+
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan], ids=("inf", "-inf", "nan"))
+@pytest.mark.parametrize("opts", [{}, dict(softcap=20.0), dict(window=60), dict(window=60, softcap=2.0, prefix=True), dict(slopes=True)],
+                         ids=lambda o: "-".join(o) or "plain")
+@pytest.mark.parametrize("n_head,n_kv,hd,page,n,new", [(8, 2, 128, 16, 333, 1), (8, 2, 64, 5, 700, 2), (4, 1, 256, 16, 333, 3), (2, 1, 128, 64, 20011, 1),
+                                                       (8, 2, 128, 16, 333, 200), (8, 2, 64, 7, 700, 65), (4, 4, 256, 16, 400, 100), (8, 1, 128, 32, 5000, 40)])
+def test_a_key_that_is_not_finite(T, n_head, n_kv, hd, page, n, new, opts, bad):
+    """One value of k of either sign: NaN for every row and head that sees its key, and no other row is any different."""
+    c = Case(T, n_head, n_kv, hd, page, [n], [new], seed=31)
+    opts = dict(opts)
+    if opts.get("slopes"):
+        opts["slopes"] = T.exp2(-8.0 * T.arange(1, n_head + 1, device="cuda") / n_head)
+    if opts.get("prefix"):
+        opts["prefix"] = T.tensor([4], dtype=T.int32, device="cuda")
+    was = c.run(**opts).view(new, n_head, hd)
+    assert T.isfinite(was).all()
+    first = n - new
+    pos = T.arange(first, n, device="cuda")
+    for j, d in ((first - 3, hd - 1), (n - 1, 0), (first + new // 2, 17), (2, 5)):
+        p, s = int(c.cache.table[0, j // page]), j % page
+        x = c.k[0, p, s, n_kv - 1, d].item()
+        c.k[0, p, s, n_kv - 1, d] = bad
+        out = c.run(**opts).view(new, n_head, hd)
+        c.k[0, p, s, n_kv - 1, d] = x
+        sees = (j <= pos) & (j > pos - opts["window"]) if "window" in opts else j <= pos
+        if "prefix" in opts:
+            sees = sees | (j < 4)
+        hit = T.zeros(new, n_head, dtype=T.bool, device="cuda")
+        hit[:, n_head - n_head // n_kv:] = sees[:, None]
+        assert T.isnan(out[hit]).all() and T.equal(out[~hit], was[~hit]), (j, d)
+    assert T.equal(c.run(**opts).view(new, n_head, hd), was) and c.H.device_status() == 0
+
+
+@pytest.mark.parametrize("news", [[2, 1], [150, 70]])
+def test_scores_past_the_range_of_floats_are_no_keys_that_are_not_finite(T, news):
+    """Finite q and k whose score is below the lowest float: the weight is 0, as it is for any score far below the best."""
+    c = Case(T, 4, 2, 128, 16, [300, 90], news, seed=32)
+    c.q.fill_(0.0)
+    c.q[:, ::128] = 3e38
+    c.k[0, :, :, :, 0] = -40000.0
+    for i in range(2):
+        c.k[0, int(c.cache.table[i, 0]), 1, :, 0] = 0.0     # the one key of each sequence that counts
+    out = c.run().view(-1, 4, 128)
+    for i in range(2):
+        want = c.values[i][1].float().repeat_interleave(2, 0)
+        assert T.equal(out[c.starts[i]:c.starts[i + 1]], want.expand(news[i], 4, 128))
+    assert c.H.device_status() == 0
