@@ -1,0 +1,73 @@
+"""The attention's results value by value, each within a bound of its own row, head and dim, and as a whole to a few
+2^-20: what a kernel that held q or P in one half would miss by far."""
+import pytest
+
+from paged_bounds import RMS, head, relative
+from test_paged_attention_gpu import Case, T  # noqa: F401  (T: the fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def definition(T, c, softcap=0.0, window=0, slopes=None, prefix=None, scale=None):
+    out = T.zeros(c.n_tokens, c.n_head, c.hd, dtype=T.float64, device="cuda")
+    bound = T.zeros_like(out)
+    q = c.q.view(c.n_tokens, c.n_head, c.hd)
+    for i in range(c.n_seq):
+        lo, hi, n = c.starts[i], c.starts[i + 1], c.lens[i]
+        pos = T.arange(n - (hi - lo), n, device="cuda")
+        for h in range(c.n_head if hi > lo else 0):
+            kv = h * c.n_kv // c.n_head
+            out[lo:hi, h], bound[lo:hi, h] = head(q[lo:hi, h], c.keys[i][:, kv], c.values[i][:, kv], pos, scale, softcap, window,
+                                                  0.0 if slopes is None else float(slopes[h]), 0 if prefix is None else int(prefix[i]))
+    return out, bound
+
+
+SHAPES = [
+    (8, 2, 64, 5, [700, 33], [1, 2]),                 # tiles of 8 rows
+    (8, 8, 128, 16, [2048], [1]),
+    (16, 2, 128, 16, [900, 5000], [1, 1]),            # cut over the keys
+    (4, 1, 256, 16, [333, 1200], [2, 1]),
+    (12, 3, 256, 24, [900], [4]),
+    (8, 2, 64, 16, [1000, 64], [100, 64]),            # tiles of 128 rows
+    (8, 2, 64, 7, [700], [65]),
+    (4, 4, 128, 16, [2048], [130]),
+    (8, 1, 128, 32, [5000], [40]),                    # cut over the keys
+    (6, 2, 128, 7, [400, 129], [129, 128]),
+    (4, 2, 256, 16, [600, 90], [100, 90]),
+    (4, 1, 256, 64, [3000], [70]),
+]
+
+
+@pytest.mark.parametrize("opts", [{}, dict(softcap=20.0), dict(softcap=1.5), dict(window=100, prefix=True), dict(slopes=True), dict(scale=0.02)],
+                         ids=lambda o: "-".join(map(str, o.items())) or "plain")
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "-".join(map(str, s[:4])))
+def test_every_value_and_the_whole(T, shape, opts):
+    c = Case(T, *shape, seed=41)
+    opts = dict(opts)
+    if opts.get("slopes"):
+        opts["slopes"] = T.exp2(-8.0 * T.arange(1, c.n_head + 1, device="cuda") / c.n_head)
+    if opts.get("prefix"):
+        opts["prefix"] = T.tensor([min(n, 40) for n in c.lens], dtype=T.int32, device="cuda")
+    ref, bound = definition(T, c, **opts)
+    out = c.run(**opts).view(c.n_tokens, c.n_head, c.hd)
+    over = ((out.double() - ref).abs() / bound).max()
+    assert float(over) <= 1, f"{float(over):.2f} times its bound"
+    rel = relative(out, ref)
+    assert rel <= RMS, f"{rel:.2e}"
+    assert c.H.device_status() == 0
+
+
+@pytest.mark.parametrize("shape", [(4, 2, 128, 16, [500], [37]), (4, 2, 64, 7, [500], [1]), (4, 1, 256, 16, [500], [20]), (4, 4, 128, 16, [500], [300])],
+                         ids=lambda s: "-".join(map(str, s[:3])))
+def test_each_row_has_its_own_scale(T, shape):
+    """Rows of q from 1e-38 to 1e4, side by side: each within its own bound, and the small ones to their last bits."""
+    c = Case(T, *shape, seed=42)
+    q = c.q.view(c.n_tokens, c.n_head, c.hd)
+    for i, f in enumerate((1e-38, 1e-30, 1e-3, 2000.0, 1e4)):
+        q[i % c.n_tokens, i % c.n_head] *= f
+    ref, bound = definition(T, c)
+    out = c.run().view(c.n_tokens, c.n_head, c.hd)
+    assert ((out.double() - ref).abs() <= bound).all() and c.H.device_status() == 0
+    for i in (0, 1, 2):
+        r, h = i % c.n_tokens, i % c.n_head
+        assert relative(out[r, h], ref[r, h]) <= RMS
