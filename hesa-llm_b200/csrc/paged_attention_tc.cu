@@ -652,7 +652,13 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
             const float ms = mn == -INFINITY ? 0.f : mn;
             const float al = m == -INFINITY ? 0.f : ex2(m - ms);
             m = mn;
-            const float off = kPShift - ms;
+            // P = 2^(14 + s k - ms), at most 2^14 and a rounding. From |ms| = 2^24 on that rounding would be past what a half
+            // holds, or all there is: scores then count in units that put ms back below 2^24, a float's precision still.
+            // (Subtracting ms from such rows' scores in a pass of their own took a vote a block: 512 tokens at 2048 0.5 us more.)
+            float unit = 1.f;
+            if (fabsf(ms) >= 0x1p24f) unit = __uint_as_float((277u - (__float_as_uint(ms) >> 23 & 255u)) << 23);   // 2^(23 - floor(log2 |ms|))
+            k *= unit;
+            const float off = fmaf(-ms, unit, kPShift);
             float2 sum = make_float2(0.f, 0.f);
             float s[2][16];   // the next 16 columns are on their way while these are made into P
             ld16(sb, s[0]);

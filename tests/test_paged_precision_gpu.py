@@ -71,3 +71,30 @@ def test_each_row_has_its_own_scale(T, shape):
     for i in (0, 1, 2):
         r, h = i % c.n_tokens, i % c.n_head
         assert relative(out[r, h], ref[r, h]) <= RMS
+
+
+@pytest.mark.parametrize("opts", [{}, dict(window=70, prefix=True), dict(slopes=True), dict(scale=1e3)], ids=lambda o: "-".join(o) or "plain")
+@pytest.mark.parametrize("shape", [(4, 2, 128, 16, [500], [50]), (2, 2, 64, 7, [500, 3], [2, 1]), (4, 1, 256, 16, [500], [40]), (4, 4, 64, 16, [500], [300]),
+                                   (8, 1, 128, 16, [4000], [32])], ids=lambda s: "-".join(map(str, s[:3])))
+def test_scores_of_any_size(T, shape, opts):
+    """Every row's scores at another power of two, up to 2^110: past 2^24 the shift of P and the maximum no longer fit into
+    one float. No infinite P and no row without one: every result is a mean of values, within its bound where that says
+    something."""
+    c = Case(T, *shape, seed=43)
+    opts = dict(opts)
+    if opts.get("slopes"):
+        opts["slopes"] = T.exp2(20 - 8.0 * T.arange(1, c.n_head + 1, device="cuda") / c.n_head)
+    if opts.get("prefix"):
+        opts["prefix"] = T.tensor([min(n, 40) for n in c.lens], dtype=T.int32, device="cuda")
+    q = c.q.view(c.n_tokens * c.n_head, c.hd)
+    top = 95 if "scale" in opts else 105
+    q *= T.exp2((T.arange(len(q), device="cuda") * 37 % 16 * (top / 15.0)).floor())[:, None] if len(q) < 100 else \
+        T.exp2((T.arange(len(q), device="cuda") * 37 % (top + 1)).float())[:, None]
+    ref, bound = definition(T, c, **opts)
+    out = c.run(**opts).view(c.n_tokens, c.n_head, c.hd)
+    assert T.isfinite(out).all()
+    small = bound < 8
+    assert ((out.double() - ref).abs() <= bound)[small].all()
+    vmax = float(max(v.abs().max() for v in c.values if len(v)))
+    assert float(out.abs().max()) <= vmax * (1 + 2.0 ** -10)      # always a mean of values
+    assert c.H.device_status() == 0
