@@ -835,6 +835,8 @@ int hesa_cuda_paged_attention(const hesa_cuda_paged_kv* kv, int32_t layer, const
     a.scale2 = static_cast<float>(scale * log2e);
     a.cap2 = static_cast<float>(o.softcap * log2e);
     a.cap_in = o.softcap > 0.f ? static_cast<float>(scale / o.softcap) : 0.f;
+    if (!std::isfinite(a.scale2) || !std::isfinite(a.cap_in))
+        return record_error(HESA_CUDA_INVALID_ARGUMENT, "scale is too large for a float, by itself or by softcap");
     a.window = o.window;
     a.slopes = o.slopes;
     a.prefix = o.prefix;

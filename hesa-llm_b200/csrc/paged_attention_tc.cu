@@ -600,7 +600,8 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
                     const int32_t jc = j0 + c * 32;
                     const float dist = static_cast<float>(pos - jc);   // exact below 2^24, else to 24 bits
                     if (A.cap2 != 0.f) {
-                        const float x1 = sc * A.cap_in;
+                        // 2^87 takes any S but 0 (at least 2^-48, below 2^40) past where tanh is 1, and none to infinity
+                        const float x1 = sc * A.cap_in > 0x1p87f ? 0x1p87f : sc * A.cap_in;
                         float far = 0.f;
 #pragma unroll
                         for (int i = 0; i < 32; i += 2) {

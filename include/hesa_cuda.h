@@ -369,7 +369,7 @@ typedef struct {
  * is 0 or j > position - window), and everywhere where j < prefix[i] for
  * sequence i. Zeroed: the plain causal attention with scale 1/sqrt(head_dim). */
 typedef struct {
-    float scale;             /* 0: 1 / sqrt(head_dim) */
+    float scale;             /* 0: 1 / sqrt(head_dim); 1.45 scale and scale / softcap are finite floats */
     float softcap;           /* 0: not capped, else 1e-6 .. 1e6 */
     int32_t window;          /* 0: no window */
     const float* slopes;     /* device [n_head] or NULL */

@@ -123,3 +123,14 @@ def test_lengths_of_no_token_are_cut_like_lengths_of_one(n_seq, n_kv, hd):
         b = H.TokenBatchStruct(slots=None, q_start=1 << 20, n_seq=n_seq, n_tokens=n_seq, max_new=1, max_len=max_len)
         size[max_len] = H.lib().hesa_cuda_paged_attention_workspace_size(ctypes.byref(kv), ctypes.byref(b), n_kv)
     assert 0 < size[0] == size[1] == size[16]
+
+
+@pytest.mark.parametrize("scale,softcap,code", [(3e38, 0.0, 2), (1e33, 1e-6, 2), (float("inf"), 0.0, 2), (float("nan"), 0.0, 2), (-1.0, 0.0, 2)])
+def test_scales_that_no_float_holds_are_refused(scale, softcap, code):
+    kv = H.PagedKVStruct(k=1 << 20, v=1 << 20, page_stride=16 * 64, layer_stride=0, n_layer=1, n_pages=4, page_size=16, n_kv_head=1,
+                         head_dim=64, table=1 << 20, seq_len=1 << 20, page_refs=None, n_slots=1, max_pages=4)
+    b = H.TokenBatchStruct(slots=None, q_start=1 << 20, n_seq=1, n_tokens=1, max_new=1, max_len=20)
+    o = H.AttnOptionsStruct(scale, softcap, 0, None, None)
+    assert H.lib().hesa_cuda_paged_attention(ctypes.byref(kv), 0, ctypes.byref(b), 1 << 20, 64, 1 << 20, 64, 1, ctypes.byref(o), 1 << 20,
+                                             1 << 30, None) == code
+    assert H.lib().hesa_cuda_last_error()

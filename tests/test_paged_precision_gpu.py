@@ -98,3 +98,19 @@ def test_scores_of_any_size(T, shape, opts):
     vmax = float(max(v.abs().max() for v in c.values if len(v)))
     assert float(out.abs().max()) <= vmax * (1 + 2.0 ** -10)      # always a mean of values
     assert c.H.device_status() == 0
+
+
+@pytest.mark.parametrize("new", [2, 80])
+def test_a_small_cap_on_scores_of_any_size(T, new):
+    """Keys of zeros beside scores near a float's end: a capped score of 0 stays 0, the others are the cap. All weights are
+    alike to 2^-19 then, and the sums round (n / 16 + 16) 2^-23: 6.1e-6 of values below 8, on both sides of the quotient."""
+    cap = 1e-6
+    c = Case(T, 4, 2, 128, 16, [300], [new], seed=44)
+    for j in (0, 17, 250):
+        c.k[0, int(c.cache.table[0, j // 16]), j % 16] = 0
+        c.keys[0][j] = 0
+    c.q *= 5e37
+    assert T.isfinite(c.q).all()
+    ref, bound = definition(T, c, softcap=cap)
+    out = c.run(softcap=cap).view(c.n_tokens, c.n_head, c.hd)
+    assert ((out.double() - ref).abs() <= bound.clamp(max=1e-4)).all() and c.H.device_status() == 0
