@@ -174,10 +174,6 @@ struct AttnArgs {
     int32_t tile0;                 // rows_kernel: the first of them
 };
 
-// (tile, kv head) pairs that may be split over the keys: more of them load every
-// SM as they are.
-constexpr int kPagedPairs = 4096;
-
 // The largest P is 2^kPShift before its split into fp16 halves: the low half of
 // a P down to 2^-28 of the row's largest is then still a normal or nearly
 // normal fp16 number, and the factor cancels in P V / sum P.

@@ -674,11 +674,8 @@ Plan make_plan(const hesa_cuda_paged_kv* kv, const hesa_cuda_token_batch* b, int
     const int keys = tc_keys(kv->head_dim);
     const int64_t blocks = std::max<int64_t>(1, (b->max_len + keys - 1) / keys);
     const int64_t pairs = tiles * kv->n_kv_head * (kv->head_dim / tc_dims(kv->head_dim));
-    int64_t per = blocks;
-    if (pairs <= kPagedPairs) {
-        const int64_t want = std::max<int64_t>(1, 148 / pairs);
-        per = std::max<int64_t>(256 / keys, (blocks + want - 1) / want);
-    }
+    const int64_t want = std::max<int64_t>(1, 148 / pairs);   // 1 from 75 pairs on: nothing is split
+    const int64_t per = std::max<int64_t>(256 / keys, (blocks + want - 1) / want);
     p.blocks_per_split = static_cast<int>(std::min(per, blocks));
     p.n_split = static_cast<int>((blocks + p.blocks_per_split - 1) / p.blocks_per_split);
     return p;
