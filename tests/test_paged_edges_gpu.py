@@ -3,6 +3,7 @@ import math  # noqa: F401
 
 import pytest
 
+from paged_bounds import RMS, relative
 from test_paged_attention_gpu import Case, T  # noqa: F401  (T: the fixture)
 
 pytestmark = pytest.mark.gpu
@@ -200,3 +201,67 @@ def test_scores_past_the_range_of_floats_are_no_keys_that_are_not_finite(T, news
         want = c.values[i][1].float().repeat_interleave(2, 0)
         assert T.equal(out[c.starts[i]:c.starts[i + 1]], want.expand(news[i], 4, 128))
     assert c.H.device_status() == 0
+
+
+def far_apart(T, pool, stride, buf, at):
+    """The pool's pages `stride` values apart in buf, layers side by side in each, from value `at` on."""
+    n_layer, n_pages, page, n_kv, hd = pool.shape
+    x = buf.as_strided(pool.shape, (page * n_kv * hd, stride, n_kv * hd, hd, 1), at)
+    x.copy_(pool)
+    return x
+
+
+@pytest.fixture
+def wide(T):
+    """2.9e9 values of fp16: offsets that neither 31 nor 32 bits of bytes, nor 31 of values, hold."""
+    buf = T.empty(11 * (1 << 28), dtype=T.float16, device="cuda")
+    yield buf
+    del buf
+    T.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("n_head,n_kv,hd,page,lens,news", [(16, 2, 128, 16, [70, 70], [1, 1]), (8, 2, 64, 7, [33, 29], [2, 1]), (4, 1, 256, 16, [70, 70], [1, 3]),
+                                                           (16, 2, 128, 16, [70, 70], [40, 33]), (8, 2, 64, 7, [33, 29], [33, 20]), (4, 1, 256, 16, [75, 70], [60, 70])])
+@pytest.mark.parametrize("odd", [0, 8], ids=("rows", "gaps"))
+def test_pages_beyond_two_to_the_31(T, wide, n_head, n_kv, hd, page, lens, news, odd):
+    """Cache write and attention over pages 2^28 values apart: as over the same pages side by side."""
+    c = Case(T, n_head, n_kv, hd, page, lens, news, seed=51, spare=0)
+    assert c.k.shape[1] == 10 and int(c.cache.table.max()) == 9
+    H, stride = c.H, (1 << 28) + odd
+    far = H.PagedKV(far_apart(T, c.k, stride, wide, 0), far_apart(T, c.v, stride, wide, 1 << 27), c.cache.table, c.cache.seq_len)
+    kv = T.randn(c.n_tokens, 2 * n_kv * hd, device="cuda")
+    got = []
+    for cache in (c.cache, far):
+        H.rope_kv_paged(cache, 0, c.batch, None, kv[:, :n_kv * hd], kv[:, n_kv * hd:], n_head)
+        got.append((H.paged_attention(cache, 0, c.batch, c.q, n_head), cache.k.clone(), cache.v.clone()))
+    (a, ka, va), (b, kb, vb) = got
+    assert T.equal(ka.view(T.int16), kb.view(T.int16)) and T.equal(va.view(T.int16), vb.view(T.int16))
+    if hd == 256 and odd and max(news) > 3:
+        # heads of 256 have chunk tiles for pages of whole rows apart only; with gaps tiles of 8 rows serve them: each is within RMS of 64 bits
+        assert relative(b, a.double()) <= 2 * RMS
+    else:
+        assert T.equal(a, b)
+    assert T.isfinite(a).all() and H.device_status() == 0
+
+
+def test_page_operations_beyond_two_to_the_31(T, wide):
+    import hesa_cuda as H
+    from test_kv_pages_gpu import Model, ints, same
+    near = H.PagedKV.empty(2, 11, 8, 2, 64, 6, 6)
+    near.k.normal_()
+    near.v.normal_()
+    far = H.PagedKV(far_apart(T, near.k, 1 << 28, wide, 0), far_apart(T, near.v, 1 << 28, wide, 1 << 27), near.table.clone(), near.seq_len.clone(),
+                    near.page_refs.clone())
+    m = Model(11, 8, 6, 6)
+    m.reserve([0, 1], [30, 35])
+    m.fork([1, 0], [2, 3])
+    m.free([0])
+    m.compact()
+    for c in (near, far):
+        H.kv_reserve(c, ints(T, [0, 1]), ints(T, [30, 35]))
+        H.kv_fork(c, ints(T, [1, 0]), ints(T, [2, 3]))
+        H.kv_free(c, ints(T, [0]))
+        H.kv_compact(c)
+        H.kv_copy_pages(c, ints(T, [1, 10]), ints(T, [9, 8]))
+        same(c, m)
+    assert T.equal(near.k, far.k) and T.equal(near.v, far.v) and H.device_status() == 0
