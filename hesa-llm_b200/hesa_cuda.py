@@ -561,6 +561,15 @@ def _new(make, stream):
         return make()
 
 
+def _page_strides(t) -> tuple:
+    """The strides of a pool; of a dimension of one entry, which may have any in torch, what a contiguous one would have."""
+    out = []
+    for size, stride in zip(reversed(t.shape), reversed(t.stride())):
+        out.append(stride if size != 1 else 1 if not out else out[-1] * below)
+        below = size
+    return tuple(reversed(out))
+
+
 class PagedKV:
     """A paged fp16 KV cache (hesa_cuda_paged_kv): the page pools k, v
     [n_layer, n_pages, page_size, n_kv_head, head_dim] (any layer and page
@@ -576,12 +585,12 @@ class PagedKV:
         dev = k.device.index
         _want(v, torch.float16, "v", dev, 5)
         _want(table, torch.int32, "table", dev, 2)
-        if v.shape != k.shape or (v.stride(0), v.stride(1)) != (k.stride(0), k.stride(1)):
-            raise ValueError("k and v must have the same shape and strides")
         n_layer, n_pages, page, n_kv, hd = k.shape
-        for t in (k, v):
-            if (t.stride(2), t.stride(3), t.stride(4)) != (n_kv * hd, hd, 1):
-                raise ValueError("places, heads and dims of a page must be contiguous")
+        strides = _page_strides(k)
+        if v.shape != k.shape or _page_strides(v) != strides:
+            raise ValueError("k and v must have the same shape and strides")
+        if strides[2:] != (n_kv * hd, hd, 1):
+            raise ValueError("places, heads and dims of a page must be contiguous")
         if not table.is_contiguous():
             raise ValueError("table must be contiguous")
         _ints(seq_len, "seq_len", table.shape[0], dev)
@@ -589,7 +598,7 @@ class PagedKV:
             _ints(page_refs, "page_refs", n_pages, dev)
         self.device, self.n_slots, self.n_pages, self.n_kv_head, self.head_dim = dev, table.shape[0], n_pages, n_kv, hd
         self.k, self.v, self.table, self.seq_len, self.page_refs = k, v, table, seq_len, page_refs
-        self.struct = PagedKVStruct(k.data_ptr(), v.data_ptr(), k.stride(1), k.stride(0), n_layer, n_pages, page, n_kv, hd,
+        self.struct = PagedKVStruct(k.data_ptr(), v.data_ptr(), strides[1], strides[0], n_layer, n_pages, page, n_kv, hd,
                                     table.data_ptr(), seq_len.data_ptr(), _ptr(page_refs), table.shape[0], table.shape[1])
         self.ref = ctypes.byref(self.struct)
         self.scratch = {}   # of the page operations, by stream handle

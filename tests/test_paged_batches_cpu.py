@@ -134,3 +134,26 @@ def test_scales_that_no_float_holds_are_refused(scale, softcap, code):
     assert H.lib().hesa_cuda_paged_attention(ctypes.byref(kv), 0, ctypes.byref(b), 1 << 20, 64, 1 << 20, 64, 1, ctypes.byref(o), 1 << 20,
                                              1 << 30, None) == code
     assert H.lib().hesa_cuda_last_error()
+
+
+def test_pools_with_dimensions_of_one_entry(monkeypatch):
+    """Such a dimension's stride says nothing: heads before places, one layer of many, one page, are sound pools."""
+    import torch
+    monkeypatch.setattr(H, "_want", lambda *a, **k: None)
+    table, seq_len = torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+
+    def strides(k, v=None):
+        s = H.PagedKV(k, k.clone(memory_format=torch.contiguous_format) if v is None else v, table, seq_len).struct
+        return s.layer_stride, s.page_stride
+    half = dict(dtype=torch.float16)
+    assert strides(torch.zeros(2, 5, 16, 4, 64, **half)) == (5 * 16 * 256, 16 * 256)
+    assert strides(torch.zeros(2, 5, 1, 16, 64, **half).transpose(2, 3)) == (5 * 16 * 64, 16 * 64)     # one head, heads outside
+    assert strides(torch.zeros(2, 5, 4, 1, 64, **half).transpose(2, 3)) == (5 * 256, 256)             # pages of one token
+    one = torch.zeros(5, 3, 16, 4, 64, **half).transpose(0, 1)
+    assert strides(one[1:2], one[2:3]) == (5 * 3 * 16 * 256, 3 * 16 * 256)                             # one layer of three
+    page = torch.zeros(7, 9, 16, 4, 64, **half).permute(1, 0, 2, 3, 4)
+    assert strides(page[:, 2:3], page[:, 4:5]) == (16 * 256, 16 * 256)                                 # one page, nine layers
+    for k, v in ((torch.zeros(2, 5, 4, 16, 64, **half).transpose(2, 3), None), (one, torch.zeros(3, 5, 16, 4, 64, **half)),
+                 (torch.zeros(2, 5, 16, 4, 128, **half)[..., :64], None), (one, one[:, :4])):
+        with pytest.raises(ValueError):
+            strides(k, v if v is not None else k)
