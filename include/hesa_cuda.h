@@ -330,8 +330,9 @@ HESA_CUDA_API int hesa_cuda_decode_step_sharded(const hesa_cuda_model* model, co
  * either order of nesting. Token j of a slot lies in place j % page_size of
  * page table[slot * max_pages + j / page_size]. page_refs[p] counts the slots
  * that page p belongs to, 0: free. head_dim 64, 128 or 256; pools 16-byte
- * aligned; at most 65536 slots, 2^30 tokens a slot, 2^30 values a page, and for
- * the page operations 2^20 pages. The struct
+ * aligned; at most 4096 layers, 1024 kv heads, 65536 places a page and 2^30
+ * values, 65536 slots of fewer than 2^30 tokens, strides of 2^50, and for the page
+ * operations 2^20 pages. The struct
  * is host memory; every pointer in it is a device pointer. page_refs may be
  * NULL where no page operation is called. A new cache has seq_len and
  * page_refs zero; table need not be set. */
@@ -357,7 +358,8 @@ typedef struct {
  * new tokens (max_new) and most tokens (max_len) of a sequence. A sequence
  * that exceeds a bound, or whose slot or length is not sound, is skipped (its
  * output stays as it was) and device status 3 recorded; so is a page outside
- * the pool, which reads as zeros. */
+ * the pool, which reads as zeros. At most 65536 sequences (n_slots without
+ * slots), and fewer than 2^31 - 2^20 rows times query heads. */
 typedef struct {
     const int32_t* slots;    /* device [n_seq], or NULL: sequence i is in slot i */
     const int32_t* q_start;  /* device [n_seq + 1], ascending from 0 or more */
@@ -377,11 +379,12 @@ typedef struct {
 } hesa_cuda_attn_options;
 
 /* out[r, h] = sum_j softmax_j(s) v_j over the keys that row r sees, for the
- * n_head query heads of every row, kv head h / (n_head / n_kv_head): the
- * attention of hesa_cuda_attention (CPU_Backend's SDPA,
- * cpu_backend.cpp:225-294) for a chunk of new tokens, or one token of each
- * sequence, over the pages. q and out are fp32 rows of n_head * head_dim with
- * row strides ldq, ldo (multiples of 4), 16-byte aligned and not overlapping.
+ * n_head query heads (a multiple of n_kv_head, at most 16384) of every row, kv
+ * head h / (n_head / n_kv_head): the attention of hesa_cuda_attention
+ * (CPU_Backend's SDPA, cpu_backend.cpp:225-294) for a chunk of new tokens, or
+ * one token of each sequence, over the pages. q and out are fp32 rows of
+ * n_head * head_dim with row strides ldq, ldo (multiples of 4), 16-byte aligned
+ * and not overlapping.
  * A row that sees no key gives zeros. K and V at places that a row does not
  * see (padding, other sequences, places past a slot's length) do not reach
  * it, whatever they hold. A k that is not finite where a row sees it gives NaN
