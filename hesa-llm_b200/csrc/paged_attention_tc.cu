@@ -214,7 +214,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
     using S = TcShape<HD>;
     constexpr int kN = S::keys, VD = S::vd, HH = VD / 2, HQ = HD / 2;   // HH, HQ: output dims and dims of q of a thread
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t full[S::slots], empty[S::slots], s_full[2], p_full[2][2], o_full[2], o_free, q_done;
+    __shared__ __align__(8) uint64_t full[S::slots], empty[S::slots], s_full[2], p_full[2][2], o_full[2], o_free, q_done, drained[2];
     __shared__ float2 s_ml[2][kM];
     __shared__ uint32_t tmem_base;
     __shared__ int abort_flag, odd_block[2];
@@ -274,6 +274,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
             mbar_init(&o_full[i], 1);
+            mbar_init(&drained[i], 1);
             for (int h = 0; h < 2; ++h) mbar_init(&p_full[i][h], kComputeWarps / 2);
         }
         mbar_init(&o_free, kComputeWarps / 2);
@@ -308,6 +309,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
             const int32_t* table = A.c.table + static_cast<int64_t>(sv.slot) * A.c.max_pages;
             const uint32_t to = ring + static_cast<uint32_t>(x * kN + g * box) * 128;
             bool dead = false;
+            int issued = 0;   // places that this warp has filled, in their order
             // the page and the place in it of this lane's keys of block j; no page: one past the pool
             auto find = [&](int j, int& page, int& at) {
                 page = A.c.n_pages;
@@ -333,6 +335,7 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
                 if (dead) return;
                 if (lane == 0) mbar_arrive_expect_tx(&full[slot], mine * wide / (HD / 64));   // a warp's dims are every second 64 of a box, or all
                 __syncwarp();
+                issued = place + 1;
                 if (c < copies && x < wide) tma_4d(to + static_cast<uint32_t>(slot) * S::slot, map, from + x * 64, kvh, at, page, &full[slot]);
             };
             if (n > 0) {
@@ -346,8 +349,8 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
                     page = page1;
                     at = at1;
                 }
-                // after a wait that ran out: nothing may be in flight when the CTA ends
-                for (int p = max(0, 2 * n - S::slots); dead && p < 2 * n; ++p)
+                // nothing may be in flight when the CTA ends, whoever gave up
+                for (int p = max(0, issued - S::slots); p < issued; ++p)
                     if (!mbar_wait_bounded(&full[p % S::slots], static_cast<uint32_t>(p / S::slots) & 1u, A.status, kStatusDrainTimeout)) break;
             }
         } else if (!TMA && warp >= kFirstProducer) {
@@ -479,6 +482,10 @@ chunk_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtenso
                 }
             }
             if (!ok) *abort_v = 1;
+            if (*abort_v) {   // its products may still read the ring and TMEM
+                commit(&drained[warp - kComputeWarps]);
+                mbar_wait_bounded(&drained[warp - kComputeWarps], 0u, A.status, kStatusDrainTimeout);
+            }
         }
         __syncwarp();
     } else {
