@@ -834,7 +834,7 @@ int hesa_cuda_paged_attention(const hesa_cuda_paged_kv* kv, int32_t layer, const
     a.cap_in = o.softcap > 0.f ? static_cast<float>(scale / o.softcap) : 0.f;
     if (!std::isfinite(a.scale2) || !std::isfinite(a.cap_in))
         return record_error(HESA_CUDA_INVALID_ARGUMENT, "scale is too large for a float, by itself or by softcap");
-    a.window = o.window;
+    a.window = std::min(o.window, 1 << 30);   // wider than any context; a position less a window stays in 32 bits
     a.slopes = o.slopes;
     a.prefix = o.prefix;
     a.part = static_cast<float*>(workspace);

@@ -265,3 +265,11 @@ def test_page_operations_beyond_two_to_the_31(T, wide):
         H.kv_copy_pages(c, ints(T, [1, 10]), ints(T, [9, 8]))
         same(c, m)
     assert T.equal(near.k, far.k) and T.equal(near.v, far.v) and H.device_status() == 0
+
+
+@pytest.mark.parametrize("window", [1 << 30, 2 ** 31 - 1])
+@pytest.mark.parametrize("news", [[9, 3], [70, 150]])
+def test_the_widest_window_is_none(T, window, news):
+    """Also where positions are negative (more new tokens than tokens)."""
+    c = Case(T, 4, 2, 64, 8, [5, 140], news, seed=52)
+    assert T.equal(c.run(window=window), c.run()) and c.H.device_status() == 0
