@@ -135,15 +135,26 @@ __device__ bool slots_sound(const Tables& t, const int32_t* slots, int n) {
     return !__syncthreads_or(bad);
 }
 
-// One reference more or less for every page of the (sound) slots; false when a
-// page had none left to take. All threads of the block; a barrier at its end.
+// One reference more or less for every page of the slots; false where a length or a
+// page is not sound (what is not has no reference changed, so that the opposite call
+// undoes this one), or a page had no reference left to take. All threads of the
+// block; a barrier at its end.
 __device__ bool add_refs(const Tables& t, const int32_t* slots, int n, int by) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     bool bad = false;
     for (int i = warp; i < n; i += kPlanThreads / 32) {
-        const int np = pages_for(t.seq_len[slots[i]], t.page_size);
+        const int len = t.seq_len[slots[i]];
+        if (len < 0 || len > static_cast<int64_t>(t.max_pages) * t.page_size) {
+            bad = true;
+            continue;
+        }
+        const int np = pages_for(len, t.page_size);
         const int32_t* row = t.table + static_cast<int64_t>(slots[i]) * t.max_pages;
-        for (int j = lane; j < np; j += 32) bad |= atomicAdd(&t.refs[row[j]], by) + by < 0;
+        for (int j = lane; j < np; j += 32) {
+            const int p = row[j];
+            if (p < 0 || p >= t.n_pages) bad = true;
+            else bad |= atomicAdd(&t.refs[p], by) + by < 0;
+        }
     }
     return !__syncthreads_or(bad);
 }
@@ -157,7 +168,7 @@ free_kernel(const Tables t, const int32_t* slots, int n) {
     grid_dep_wait();
     grid_dep_launch();
     __shared__ uint32_t bits[kMaxSlots / 32];
-    if (!mark_slots(slots, n, t.n_slots, bits) || !slots_sound(t, slots, n)) return refuse(t, kStatusBadPosition);
+    if (!mark_slots(slots, n, t.n_slots, bits)) return refuse(t, kStatusBadPosition);
     // A page that the slots hold more often than it has references would end below
     // zero: the references are taken, and given back if one was not there.
     if (!add_refs(t, slots, n, -1)) {

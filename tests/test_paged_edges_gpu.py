@@ -273,3 +273,33 @@ def test_the_widest_window_is_none(T, window, news):
     """Also where positions are negative (more new tokens than tokens)."""
     c = Case(T, 4, 2, 64, 8, [5, 140], news, seed=52)
     assert T.equal(c.run(window=window), c.run()) and c.H.device_status() == 0
+
+
+@pytest.mark.parametrize("what", ["below", "above", "free", "short", "long"])
+def test_freeing_slots_that_are_not_sound_changes_nothing(T, what):
+    """Sound slots beside one with a page outside the pool, a page that is free, or a length that its row cannot have."""
+    import hesa_cuda as H
+    from test_kv_pages_gpu import fresh, ints, same
+    _, c, m = fresh(T, n_pages=400, page=4, n_slots=60, max_pages=12)
+    slots = list(range(50))
+    m.reserve(slots, [1 + 7 * s % 40 for s in slots])
+    m.free([20])
+    m.reserve([20], [30])
+    if what in ("short", "long"):
+        m.len[20] = {"short": -1, "long": 49}[what]
+    else:
+        m.rows[20][5] = {"below": -1, "above": 400, "free": m.refs.index(0)}[what]
+    before = [x[:] for x in m.rows], m.refs[:], m.len[:]
+    c.table.copy_(T.tensor(m.rows, dtype=T.int32))
+    c.page_refs.copy_(T.tensor(m.refs, dtype=T.int32))
+    c.seq_len.copy_(T.tensor(m.len, dtype=T.int32))
+    H.kv_free(c, ints(T, slots))
+    assert H.device_status() == 3
+    H.clear_device_status()
+    same(c, m)
+    assert before == (m.rows, m.refs, m.len)
+    rest = [s for s in slots if s != 20]
+    H.kv_free(c, ints(T, rest))
+    m.free(rest)
+    same(c, m)
+    assert H.device_status() == 0
