@@ -12,6 +12,9 @@ taken to be cut, 2^-23):
            (2^-22) and the two halves of P (2^-21)
   sums     of p v and p: a rounding for every 16 keys and a few where parts are joined, (n / 16 + 16) 2^-23
 
+And a step of 2^-24 is the last that a half of P has, 2^-38 of the row's largest p, which the shift puts at 2^14: each p
+is off by that much beside its relative error (a weight of 10^-20 is none).
+
 A relative error e_j of p_j moves the result by at most sum_j w_j e_j (|v_j| + |out|), w the weights.
 
 Most of these are independent and of either sign, so a whole result is nearer. For scores of standard deviation 2 or
@@ -70,7 +73,7 @@ def head(q, k, v, pos, scale=None, softcap=0.0, window=0, slope=0.0, prefix=0, q
     w = torch.where(z > 0, (p_as(p) if p_as else p) / z, torch.zeros_like(p))
     out = w @ v
     e = torch.where(see, e + 2.0 ** -23 * (s.abs() + d.abs()) + 2.0 ** -19, torch.zeros_like(e))
-    we = torch.where(see, w * e, torch.zeros_like(e))
+    we = torch.where(see, w * e + 2.0 ** -38 / z, torch.zeros_like(e))
     bound = we @ v.abs() + we.sum(1, keepdim=True) * out.abs() + (n / 16 + 16) * 2.0 ** -23 * (w @ v.abs() + out.abs())
     return out, bound
 

@@ -15,7 +15,7 @@ def definition(T, c, softcap=0.0, window=0, slopes=None, prefix=None, scale=None
     for i in range(c.n_seq):
         lo, hi, n = c.starts[i], c.starts[i + 1], c.lens[i]
         pos = T.arange(n - (hi - lo), n, device="cuda")
-        for h in range(c.n_head if hi > lo else 0):
+        for h in range(c.n_head if hi > lo and n else 0):
             kv = h * c.n_kv // c.n_head
             out[lo:hi, h], bound[lo:hi, h] = head(q[lo:hi, h], c.keys[i][:, kv], c.values[i][:, kv], pos, scale, softcap, window,
                                                   0.0 if slopes is None else float(slopes[h]), 0 if prefix is None else int(prefix[i]))
