@@ -303,3 +303,41 @@ def test_freeing_slots_that_are_not_sound_changes_nothing(T, what):
     m.free(rest)
     same(c, m)
     assert H.device_status() == 0
+
+
+def test_two_host_threads_at_once(T):
+    """Attention, cache write, log probabilities and page operations from two threads, each on a stream of its own."""
+    import threading
+
+    import hesa_cuda as H
+    from test_kv_pages_gpu import ints
+    shapes = [(16, 2, 128, 16, [900, 70, 3], [1, 2, 1]), (8, 2, 64, 7, [700, 300], [65, 300])]
+    cases = [Case(T, *s, seed=61 + i) for i, s in enumerate(shapes)]
+    want = [c.run() for c in cases]
+    logits = [T.randn(2, 50001, device="cuda"), T.randn(1500, 321, device="cuda")]
+    top = [H.token_logprobs(x, top_k=7) for x in logits]
+    pages = [H.PagedKV.empty(2, 64, 8, 1, 64, 8, 16) for _ in cases]
+    lists = [ints(T, x) for x in ([0, 1], [20, 33], [2, 3], [1])]
+    T.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        c, cache, s = cases[i], pages[i], T.cuda.Stream()
+        with T.cuda.stream(s):
+            for _ in range(50):
+                out = c.run()
+                lp = H.token_logprobs(logits[i], top_k=7)
+                H.kv_reserve(cache, lists[0], lists[1])
+                H.kv_fork(cache, lists[0], lists[2])
+                H.kv_free(cache, lists[3])
+                H.kv_compact(cache)
+                H.kv_free(cache, ints(T, [0, 2, 3]))
+                s.synchronize()
+                if not T.equal(out, want[i]) or not all(a is None or T.equal(a, b) for a, b in zip(lp, top[i])) or bool(cache.page_refs.any()):
+                    wrong.append(i)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and H.device_status() == 0
