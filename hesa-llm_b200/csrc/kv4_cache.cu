@@ -1,0 +1,290 @@
+// kv4_cache.cu -- writing new tokens into the pages of a cache in 4 bits, and
+// reading them back.
+//
+//   m = the value of largest magnitude of 32 dims, d = round(m / -8) to 8
+//   significant bits, code = floor(x / d + 8.5) in 0 .. 15, value = d (code - 8)
+//
+// The 8 bits of a scale (a step of the code is off by at most 1 / 512 of itself,
+// and the codes are made for the scale as it is stored) and the 4 of a code make
+// 11: every value is an fp16 number exactly, so attention can take values as fp16
+// without another rounding. Scales below 2^-17 are multiples of 2^-24, fp16's
+// last step, for the same reason.
+//
+// Both kernels are bound by HBM: each value is read once and written once.
+#include "paged.h"
+#include "abi_errors.h"
+#include "qmatvec.h"
+#include "trace.h"
+
+#include <algorithm>
+
+namespace hesa_cuda {
+namespace {
+
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// The place of a row's token: group number of its first head's first group, or -1
+// (with a status recorded where the tables are not sound), and its position.
+struct Place {
+    int64_t group;
+    int32_t pos;
+    bool row;      // the row is a sequence's
+};
+
+__device__ __forceinline__ Place place_of(const PagedLayer& c, const BatchView& b, int row, int* status) {
+    // the last sequence that starts at or before this row and is not empty there
+    int lo = 0, hi = b.n_seq - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (b.q_start[mid] <= row) lo = mid;
+        else hi = mid - 1;
+    }
+    const SeqView s = seq_view(c, b, lo);
+    Place p{-1, 0, false};
+    if (!s.ok) {
+        if (threadIdx.x == 0) record_status(status, kStatusBadPosition);
+        return p;
+    }
+    const int t = row - s.q0;
+    if (t < 0 || t >= s.n_new) return p;   // a row behind the last sequence
+    p.row = true;
+    p.pos = s.len - s.n_new + t;
+    const int pi = p.pos >= 0 ? c.page_div.div(p.pos) : 0;
+    const int page = p.pos >= 0 ? c.table[static_cast<int64_t>(s.slot) * c.max_pages + pi] : -1;
+    if (page < 0 || page >= c.n_pages) {
+        if (threadIdx.x == 0) record_status(status, kStatusBadPosition);
+        return p;
+    }
+    p.group = static_cast<int64_t>(page) * c.page_stride + static_cast<int64_t>(p.pos - pi * c.page_size) * c.n_kv * (c.head_dim / kGroup);
+    return p;
+}
+
+// Eight values of a group whose other 24 the quad's other threads have (in order):
+// the group's scale, and this thread's word of codes.
+__device__ __forceinline__ uint32_t quantize8(const float (&x)[8], unsigned quad, float& scale) {
+    float m = x[0], a = fabsf(x[0]);
+    if (!(a < INFINITY)) a = INFINITY;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+        float ai = fabsf(x[i]);
+        if (!(ai < INFINITY)) ai = INFINITY;   // also NaN: such a group has no scale
+        if (ai > a) {
+            a = ai;
+            m = x[i];
+        }
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        const float ao = __shfl_xor_sync(quad, a, o), mo = __shfl_xor_sync(quad, m, o);
+        // equal magnitudes: the lower thread's value, on both sides
+        if (ao > a || (ao == a && (threadIdx.x & o))) {
+            a = ao;
+            m = mo;
+        }
+    }
+    const float s = m * -0.125f;
+    const uint32_t u = __float_as_uint(s);
+    float d = __uint_as_float((u + 0x7FFFu + ((u >> 16) & 1u)) & 0xFFFF0000u);   // 8 bits, ties to even
+    if (fabsf(s) < 0x1p-17f) d = rintf(s * 0x1p24f) * 0x1p-24f;
+    if (!(a < INFINITY) || !(fabsf(d) <= kMostScale)) d = NAN;
+    scale = d;
+    if (!(fabsf(d) > 0.f)) return 0x88888888u;
+    const float id = __frcp_rn(d);
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int c = static_cast<int>(__fadd_rn(__fmul_rn(x[i], id), 8.5f));   // toward zero: what is below 0 gives 0
+        w |= static_cast<uint32_t>(min(max(c, 0), 15)) << (4 * i);
+    }
+    return w;
+}
+
+// A unit is 16 values of one head of one token: 8 of the first half of the head
+// and the 8 that they are rotated with; four threads side by side have two whole
+// groups. A block takes one token's units (grid.y covers long rows); q, then k,
+// then v.
+__global__ void __launch_bounds__(256)
+rope_kv4_kernel(const PagedLayer c, const Pools4 pools, const BatchView b, float* q, int64_t ldq, const float* k, int64_t ldk,
+                const float* v, int64_t ldv, int n_head, const float* table, int table_rows, int* status) {
+    grid_dep_wait();
+    grid_dep_launch();
+    const int row = blockIdx.x;
+    const Place at = place_of(c, b, row, status);
+    if (at.group < 0) return;
+    if (table && at.pos >= table_rows) {
+        if (threadIdx.x == 0) record_status(status, kStatusBadPosition);
+        return;
+    }
+    const int hd = c.head_dim, per = hd / 16, half = hd / 2, groups = hd / kGroup;
+    const int n_rot = n_head + c.n_kv;
+    const int units = (n_rot + c.n_kv) * per;   // a multiple of 4, as `per` is: a quad works or none of its threads does
+    const float* cs = table ? table + static_cast<int64_t>(at.pos) * hd : nullptr;
+    const unsigned quad = 0xFu << (threadIdx.x & 28);
+    for (int u = blockIdx.y * blockDim.x + threadIdx.x; u < units; u += gridDim.y * blockDim.x) {
+        const int h = u / per, d = (u - h * per) * 8;
+        if (h < n_head && !table) continue;   // nothing to rotate: q stays as it is
+        const float* src = h < n_head ? q + row * ldq + static_cast<int64_t>(h) * hd
+                           : h < n_rot ? k + row * ldk + static_cast<int64_t>(h - n_head) * hd
+                                       : v + row * ldv + static_cast<int64_t>(h - n_rot) * hd;
+        float x[8], y[8];
+        *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(src + d);
+        *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(src + d + 4);
+        *reinterpret_cast<float4*>(y) = *reinterpret_cast<const float4*>(src + half + d);
+        *reinterpret_cast<float4*>(y + 4) = *reinterpret_cast<const float4*>(src + half + d + 4);
+        if (table && h < n_rot) {
+            float co[8], si[8];
+            *reinterpret_cast<float4*>(co) = *reinterpret_cast<const float4*>(cs + d);
+            *reinterpret_cast<float4*>(co + 4) = *reinterpret_cast<const float4*>(cs + d + 4);
+            *reinterpret_cast<float4*>(si) = *reinterpret_cast<const float4*>(cs + half + d);
+            *reinterpret_cast<float4*>(si + 4) = *reinterpret_cast<const float4*>(cs + half + d + 4);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {   // each product and sum rounded by itself, as the library's other rope kernels
+                const float a = x[i], e = y[i];
+                x[i] = __fsub_rn(__fmul_rn(a, co[i]), __fmul_rn(e, si[i]));
+                y[i] = __fadd_rn(__fmul_rn(a, si[i]), __fmul_rn(e, co[i]));
+            }
+        }
+        if (h < n_head) {
+            float* o = q + row * ldq + static_cast<int64_t>(h) * hd;
+            *reinterpret_cast<float4*>(o + d) = *reinterpret_cast<float4*>(x);
+            *reinterpret_cast<float4*>(o + d + 4) = *reinterpret_cast<float4*>(x + 4);
+            *reinterpret_cast<float4*>(o + half + d) = *reinterpret_cast<float4*>(y);
+            *reinterpret_cast<float4*>(o + half + d + 4) = *reinterpret_cast<float4*>(y + 4);
+        } else {
+            const bool is_k = h < n_rot;
+            const int64_t g = at.group + static_cast<int64_t>(is_k ? h - n_head : h - n_rot) * groups;
+            uint32_t* codes = reinterpret_cast<uint32_t*>(const_cast<uint4*>(is_k ? pools.k : pools.v) + g);
+            __half* scales = const_cast<__half*>(is_k ? pools.ks : pools.vs) + g;
+            float sx, sy;
+            const uint32_t wx = quantize8(x, quad, sx), wy = quantize8(y, quad, sy);
+            codes[d / 8] = wx;
+            codes[(half + d) / 8] = wy;
+            if ((threadIdx.x & 3) == 0) {
+                scales[d / kGroup] = __float2half_rn(sx);   // exact
+                scales[(half + d) / kGroup] = __float2half_rn(sy);
+            }
+        }
+    }
+}
+
+// A thread takes eight dims: a word of codes, 32 bytes of values.
+__global__ void __launch_bounds__(256)
+kv4_read_kernel(const PagedLayer c, const Pools4 pools, const BatchView b, float* k, int64_t ldk, float* v, int64_t ldv, int* status) {
+    grid_dep_wait();
+    grid_dep_launch();
+    const int row = blockIdx.x;
+    const Place at = place_of(c, b, row, status);
+    if (!at.row) return;
+    const int words = c.n_kv * c.head_dim / 8;
+    for (int u = blockIdx.y * blockDim.x + threadIdx.x; u < 2 * words; u += gridDim.y * blockDim.x) {
+        const bool is_k = u < words;
+        const int w = is_k ? u : u - words;
+        float* o = is_k ? k : v;
+        if (!o) continue;
+        o += row * (is_k ? ldk : ldv) + static_cast<int64_t>(w) * 8;
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = 0.f;
+        if (at.group >= 0) {
+            const uint32_t code = reinterpret_cast<const uint32_t*>((is_k ? pools.k : pools.v) + at.group)[w];
+            const float d = __half2float(((is_k ? pools.ks : pools.vs) + at.group)[w / 4]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = d * static_cast<float>(static_cast<int>((code >> (4 * i)) & 15u) - 8);
+        }
+        *reinterpret_cast<float4*>(o) = *reinterpret_cast<float4*>(x);
+        *reinterpret_cast<float4*>(o + 4) = *reinterpret_cast<float4*>(x + 4);
+    }
+}
+
+}  // namespace
+
+int check_paged_kv4(const hesa_cuda_paged_kv4* kv) {
+    if (!kv || !kv->k || !kv->v || !kv->k_scale || !kv->v_scale || !kv->table || !kv->seq_len)
+        return record_error(HESA_CUDA_INVALID_ARGUMENT, "null pointer");
+    const int rc = check_paged_shape({kv->table, kv->seq_len, kv->page_stride, kv->layer_stride, kGroup, kv->n_layer, kv->n_pages, kv->page_size, kv->n_kv_head,
+                                      kv->head_dim, kv->n_slots, kv->max_pages});
+    if (rc != HESA_CUDA_OK) return rc;
+    if (!aligned(kv->k, 16) || !aligned(kv->v, 16) || !aligned(kv->k_scale, 16) || !aligned(kv->v_scale, 16))
+        return record_error(HESA_CUDA_INVALID_ARGUMENT, "the page pools must be 16-byte aligned");
+    return HESA_CUDA_OK;
+}
+
+PagedLayer layer_of4(const hesa_cuda_paged_kv4* kv) {
+    PagedLayer c{};
+    c.page_stride = kv->page_stride;
+    c.n_pages = kv->n_pages;
+    c.page_size = kv->page_size;
+    c.n_kv = kv->n_kv_head;
+    c.head_dim = kv->head_dim;
+    c.table = kv->table;
+    c.seq_len = kv->seq_len;
+    c.n_slots = kv->n_slots;
+    c.max_pages = kv->max_pages;
+    c.page_div = FastDiv(kv->page_size);
+    return c;
+}
+
+Pools4 pools_of(const hesa_cuda_paged_kv4* kv, int32_t layer) {
+    const int64_t at = layer * kv->layer_stride;
+    return Pools4{static_cast<const uint4*>(kv->k) + at, static_cast<const uint4*>(kv->v) + at, static_cast<const __half*>(kv->k_scale) + at,
+                  static_cast<const __half*>(kv->v_scale) + at};
+}
+
+}  // namespace hesa_cuda
+
+using namespace hesa_cuda;
+
+extern "C" {
+
+int hesa_cuda_rope_kv4_paged(const hesa_cuda_paged_kv4* kv, int32_t layer, const hesa_cuda_token_batch* batch, float* q, int64_t ldq,
+                             const float* k, int64_t ldk, const float* v, int64_t ldv, int64_t n_head, const float* rope_table,
+                             int32_t rope_rows, void* stream) {
+    HESA_TRACE("hesa_cuda_rope_kv4_paged");
+    int rc = check_paged_kv4(kv);
+    if (rc == HESA_CUDA_OK) rc = check_batch4(kv, layer, batch, n_head);
+    if (rc != HESA_CUDA_OK) return rc;
+    if (batch->n_tokens == 0) return HESA_CUDA_OK;   // no rows: their buffers may be null
+    if (!k || !v || (rope_table && !q)) return record_error(HESA_CUDA_INVALID_ARGUMENT, "null pointer");
+    const int64_t kv_width = static_cast<int64_t>(kv->n_kv_head) * kv->head_dim;
+    if (ldk < kv_width || ldv < kv_width || (rope_table && (ldq < n_head * kv->head_dim || rope_rows <= 0)))
+        return record_error(HESA_CUDA_SHAPE_MISMATCH, "leading dimension or rope table too small");
+    if (ldq > (int64_t(1) << 40) || ldk > (int64_t(1) << 40) || ldv > (int64_t(1) << 40))
+        return record_error(HESA_CUDA_SHAPE_MISMATCH, "leading dimension too large");
+    if (!aligned(k, 16) || !aligned(v, 16) || (ldk & 3) || (ldv & 3) || (rope_table && (!aligned(q, 16) || !aligned(rope_table, 16) || (ldq & 3))))
+        return record_error(HESA_CUDA_INVALID_ARGUMENT, "q, k, v and the rope table must be 16-byte aligned with leading dimensions multiples of 4");
+    int* status = nullptr;
+    cudaError_t e = status_word(&status);
+    if (e == cudaSuccess) {
+        const int64_t units = (n_head + 2 * kv->n_kv_head) * (kv->head_dim / 16);
+        // one block a token where tokens are many; few tokens are spread over more blocks
+        const int64_t y = batch->n_tokens >= 148 * 4 ? 1 : std::min<int64_t>((units + 255) / 256, 1024);
+        e = launch_dep(rope_kv4_kernel, dim3(static_cast<unsigned>(batch->n_tokens), static_cast<unsigned>(y)), 256, 0, static_cast<cudaStream_t>(stream),
+                       layer_of4(kv), pools_of(kv, layer), view_of(batch), q, ldq, k, ldk, v, ldv, static_cast<int>(n_head), rope_table, rope_rows, status);
+    }
+    return e == cudaSuccess ? HESA_CUDA_OK : record_cuda_error(e, "rope_kv4_paged kernel");
+}
+
+int hesa_cuda_kv4_read(const hesa_cuda_paged_kv4* kv, int32_t layer, const hesa_cuda_token_batch* batch, float* k, int64_t ldk, float* v,
+                       int64_t ldv, void* stream) {
+    HESA_TRACE("hesa_cuda_kv4_read");
+    int rc = check_paged_kv4(kv);
+    if (rc == HESA_CUDA_OK) rc = check_batch4(kv, layer, batch, kv->n_kv_head);
+    if (rc != HESA_CUDA_OK) return rc;
+    if (batch->n_tokens == 0 || (!k && !v)) return HESA_CUDA_OK;
+    const int64_t width = static_cast<int64_t>(kv->n_kv_head) * kv->head_dim;
+    if ((k && (ldk < width || ldk > (int64_t(1) << 40))) || (v && (ldv < width || ldv > (int64_t(1) << 40))))
+        return record_error(HESA_CUDA_SHAPE_MISMATCH, "leading dimension too small or too large");
+    if (!aligned(k, 16) || !aligned(v, 16) || (k && (ldk & 3)) || (v && (ldv & 3)))
+        return record_error(HESA_CUDA_INVALID_ARGUMENT, "k and v must be 16-byte aligned with leading dimensions multiples of 4");
+    int* status = nullptr;
+    cudaError_t e = status_word(&status);
+    if (e == cudaSuccess) {
+        const int64_t units = 2 * width / 8;
+        const int64_t y = batch->n_tokens >= 148 * 4 ? 1 : std::min<int64_t>((units + 255) / 256, 1024);
+        e = launch_dep(kv4_read_kernel, dim3(static_cast<unsigned>(batch->n_tokens), static_cast<unsigned>(y)), 256, 0, static_cast<cudaStream_t>(stream),
+                       layer_of4(kv), pools_of(kv, layer), view_of(batch), k, ldk, v, ldv, status);
+    }
+    return e == cudaSuccess ? HESA_CUDA_OK : record_cuda_error(e, "kv4_read kernel");
+}
+
+}  // extern "C"

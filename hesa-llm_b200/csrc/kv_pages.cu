@@ -48,7 +48,8 @@ struct PageWork {
 
 __host__ __device__ inline int64_t most_items(int32_t n_pages, int32_t n_slots) { return n_pages > n_slots ? n_pages : n_slots; }
 
-PageWork page_work(void* ws, const hesa_cuda_paged_kv* kv) {
+template <typename KV>
+PageWork page_work(void* ws, const KV* kv) {
     const int64_t most = most_items(kv->n_pages, kv->n_slots);
     PageWork w;
     w.n_items = static_cast<int32_t*>(ws);
@@ -278,6 +279,101 @@ fork_plan_kernel(const Tables t, const int32_t* src, const int32_t* dst, int n, 
     if (threadIdx.x == 0) *w.n_items = n;
 }
 
+// Pages of the slots that no slot takes over lose a reference each (by = -1), or get it back (by = 1); false where a
+// page had none left to take. A warp a group, lane b has slot b of it. All threads of the block; a barrier at its end.
+__device__ bool drop_refs(const Tables& t, const int32_t* slots, const int32_t* parents, int n, int width, int by) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    bool bad = false;
+    for (int g = warp * width; g < n; g += kPlanThreads / 32 * width) {
+        const int par = lane < width ? parents[g + lane] : -1;
+        for (int b = 0; b < width; ++b) {
+            if (__any_sync(0xffffffffu, par == b)) continue;
+            const int slot = slots[g + b], np = pages_for(t.seq_len[slot], t.page_size);
+            for (int j = lane; j < np; j += 32) bad |= atomicAdd(&t.refs[t.table[static_cast<int64_t>(slot) * t.max_pages + j]], by) + by < 0;
+        }
+    }
+    return !__syncthreads_or(bad);
+}
+
+// Slot b of a group becomes what slot parents[b] of it was. References that go are taken first, so that the pages
+// they free can be taken for the copies, then those that come are added; the table's entries of a group are changed by
+// one warp, column by column, each lane holding an old entry of its slot when the first new one is written.
+__global__ void __launch_bounds__(kPlanThreads)
+reorder_plan_kernel(const Tables t, const int32_t* slots, const int32_t* parents, int n, int width, PageWork w) {
+    grid_dep_wait();
+    grid_dep_launch();
+    __shared__ uint32_t bits[kMaxSlots / 32];
+    __shared__ int s[33];
+    if (threadIdx.x == 0) *w.n_items = 0;
+    bool bad = !mark_slots(slots, n, t.n_slots, bits);
+    for (int i = threadIdx.x; i < n && !bad; i += kPlanThreads) bad = parents[i] < 0 || parents[i] >= width;
+    if (__syncthreads_or(bad) || !slots_sound(t, slots, n)) return refuse(t, kStatusBadPosition);
+    if (!drop_refs(t, slots, parents, n, width, -1)) {
+        drop_refs(t, slots, parents, n, width, 1);
+        return refuse(t, kStatusBadPosition);
+    }
+    // a slot whose parent has a partly filled page and an earlier child gets a page of its own
+    int total = 0;
+    for (int b = 0; b < n; b += kPlanThreads) {
+        const int i = b + threadIdx.x;
+        bool copy = false;
+        if (i < n) {
+            const int g = i - i % width, par = parents[i];
+            for (int x = g; x < i; ++x) copy |= parents[x] == par;
+            copy = copy && t.seq_len[slots[g + par]] % t.page_size != 0;
+        }
+        int all;
+        const int at = block_scan(copy ? 1 : 0, s, all);
+        if (i < n) w.start[i] = copy ? total + at : -1;
+        total += all;
+    }
+    if (total > t.n_pages || !lowest_free(t, total, w.list, s)) {
+        __syncthreads();
+        drop_refs(t, slots, parents, n, width, 1);
+        return refuse(t, kStatusNoPages);
+    }
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cols = 32 / width;   // columns of the table a warp has in hand
+    const int beam = lane % width, col = lane / width;
+    for (int g = warp * width; g < n; g += kPlanThreads / 32 * width) {
+        const int par = parents[g + beam], slot = slots[g + beam];
+        const int old_len = t.seq_len[slot], len = __shfl_sync(0xffffffffu, old_len, par);
+        const int old_pages = pages_for(old_len, t.page_size), pages = pages_for(len, t.page_size), full = len / t.page_size;
+        const int take = w.start[g + beam], fresh = take >= 0 ? w.list[take] : -1;
+        bool later = false;   // the parent has an earlier child
+        for (int x = 0; x < beam; ++x) later |= parents[g + x] == par;
+        int32_t* row = t.table + static_cast<int64_t>(slot) * t.max_pages;
+        int most = max(old_pages, pages);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+        for (int j0 = 0; j0 < most; j0 += cols) {
+            const int j = j0 + col;
+            const bool mine = col < cols && j < most;
+            const int old = mine && j < old_pages ? row[j] : -1;
+            const int from = __shfl_sync(0xffffffffu, old, col < cols ? col * width + par : lane);
+            if (mine) {
+                if (j < pages) {
+                    const bool copy = j == full && fresh >= 0;
+                    const int now = copy ? fresh : from;
+                    if (now != old) row[j] = now;
+                    if (copy) {
+                        int32_t* item = w.items + 3 * static_cast<int64_t>(take);
+                        item[0] = from;
+                        item[1] = fresh;
+                        item[2] = len % t.page_size;
+                        t.refs[fresh] = 1;
+                    }
+                } else if (j < old_pages) {
+                    row[j] = -1;
+                }
+            }
+            if (mine && later && j < full) atomicAdd(&t.refs[from], 1);   // for every child but the first
+        }
+        __syncwarp();
+        if (col == 0) t.seq_len[slot] = len;
+    }
+    if (threadIdx.x == 0) *w.n_items = total;
+}
+
 // live pages to the front: free pages below n_live take the pages in use from n_live on
 __global__ void __launch_bounds__(kPlanThreads)
 compact_plan_kernel(const Tables t, PageWork w, int32_t* n_live_out) {
@@ -356,13 +452,21 @@ copy_plan_kernel(const Tables t, const int32_t* src, const int32_t* dst, int n, 
     if (threadIdx.x == 0) *w.n_items = n;
 }
 
-// The copy list, for every layer and for K and V: item, layer and pool one
-// after another over a fixed grid (the list's length is known on the device
-// only). A page's filled slots are one contiguous range. With map, the tables'
-// entries are replaced by map[entry] in the same launch.
+// The pools whose pages go together: K and V, or the codes and scales of both. In bytes; a place of a pool of scales
+// may be no multiple of 16, a page's start is.
+struct CopyPools {
+    uint8_t* base[4];
+    int64_t page[4], layer[4];
+    int32_t place[4];
+    int32_t n;
+};
+
+// The copy list, for every layer and pool: item, layer and pool one after another
+// over a fixed grid (the list's length is known on the device only). A page's
+// filled slots are one contiguous range. With map, the tables' entries are replaced
+// by map[entry] in the same launch.
 __global__ void __launch_bounds__(256)
-copy_kernel(uint4* k, uint4* v, int64_t page_words, int64_t layer_words, int n_layer,
-            int slot_words, const int32_t* n_items, const int32_t* items, const Tables t,
+copy_kernel(const __grid_constant__ CopyPools pools, int n_layer, const int32_t* n_items, const int32_t* items, const Tables t,
             const int32_t* map) {
     grid_dep_wait();
     grid_dep_launch();
@@ -374,15 +478,16 @@ copy_kernel(uint4* k, uint4* v, int64_t page_words, int64_t layer_words, int n_l
             if (*n_items > 0 && j < pages_for(t.seq_len[slot], t.page_size)) t.table[e] = map[t.table[e]];
         }
     }
-    const int64_t n = static_cast<int64_t>(*n_items) * n_layer * 2;
+    const int64_t n = static_cast<int64_t>(*n_items) * n_layer * pools.n;
     for (int64_t x = blockIdx.x; x < n; x += gridDim.x) {
-        const int64_t it = x / (2 * n_layer);
-        const int lk = static_cast<int>(x - it * 2 * n_layer);
-        const int words = items[3 * it + 2] * slot_words;
-        if (words == 0) continue;
-        uint4* pool = (lk & 1) ? v : k;
-        const uint4* from = pool + (lk >> 1) * layer_words + items[3 * it] * page_words;
-        uint4* to = pool + (lk >> 1) * layer_words + items[3 * it + 1] * page_words;
+        const int64_t it = x / (pools.n * n_layer);
+        const int lk = static_cast<int>(x - it * pools.n * n_layer), layer = lk / pools.n, p = lk - layer * pools.n;
+        const int64_t bytes = static_cast<int64_t>(items[3 * it + 2]) * pools.place[p];
+        if (bytes == 0) continue;
+        const int words = static_cast<int>(bytes / 16);
+        const uint8_t* pool = pools.base[p] + layer * pools.layer[p];
+        const uint4* from = reinterpret_cast<const uint4*>(pool + items[3 * it] * pools.page[p]);
+        uint4* to = reinterpret_cast<uint4*>(const_cast<uint8_t*>(pool) + items[3 * it + 1] * pools.page[p]);
         for (int i = threadIdx.x; i < words; i += 4 * blockDim.x) {
             uint4 r[4];
 #pragma unroll
@@ -392,6 +497,8 @@ copy_kernel(uint4* k, uint4* v, int64_t page_words, int64_t layer_words, int n_l
             for (int u = 0; u < 4; ++u)
                 if (i + u * static_cast<int>(blockDim.x) < words) __stcs(to + i + u * blockDim.x, r[u]);
         }
+        if (threadIdx.x < (bytes & 15) / 4)
+            reinterpret_cast<uint32_t*>(to + words)[threadIdx.x] = reinterpret_cast<const uint32_t*>(from + words)[threadIdx.x];
     }
 }
 
@@ -481,15 +588,27 @@ rope_kv_paged_kernel(PagedLayer c, BatchView b, float* q, int64_t ldq, const flo
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
+int check(const hesa_cuda_paged_kv* kv) { return check_paged_kv(kv); }
+int check(const hesa_cuda_paged_kv4* kv) { return check_paged_kv4(kv); }
+
+template <typename KV>
+size_t pages_workspace(const KV* kv) {
+    if (check(kv) != HESA_CUDA_OK) return 0;
+    if (kv->n_pages > (1 << 20)) return 0;
+    const size_t most = static_cast<size_t>(most_items(kv->n_pages, kv->n_slots));
+    return (4 + 4 * most + static_cast<size_t>(kv->n_pages) + static_cast<size_t>(kv->n_slots) + 1) * sizeof(int32_t);
+}
+
 // Checks that every page operation shares, and its tables.
-int page_op(const hesa_cuda_paged_kv* kv, int32_t n, void* ws, size_t ws_bytes, Tables* t) {
-    const int rc = check_paged_kv(kv);
+template <typename KV>
+int page_op(const KV* kv, int32_t n, void* ws, size_t ws_bytes, Tables* t) {
+    const int rc = check(kv);
     if (rc != HESA_CUDA_OK) return rc;
     if (!kv->page_refs || !aligned(kv->page_refs, 4)) return record_error(HESA_CUDA_INVALID_ARGUMENT, "page operations need page_refs");
     if (n < 0) return record_error(HESA_CUDA_SHAPE_MISMATCH, "negative count");
     if (kv->n_pages > (1 << 20)) return record_error(HESA_CUDA_SHAPE_MISMATCH, "page operations take at most 2^20 pages");
     if (!ws || !aligned(ws, 16)) return record_error(HESA_CUDA_INVALID_ARGUMENT, "workspace must be 16-byte aligned");
-    if (ws_bytes < hesa_cuda_kv_pages_workspace_size(kv)) return record_error(HESA_CUDA_INVALID_ARGUMENT, "workspace too small");
+    if (ws_bytes < pages_workspace(kv)) return record_error(HESA_CUDA_INVALID_ARGUMENT, "workspace too small");
     t->table = kv->table;
     t->seq_len = kv->seq_len;
     t->refs = kv->page_refs;
@@ -500,31 +619,42 @@ int page_op(const hesa_cuda_paged_kv* kv, int32_t n, void* ws, size_t ws_bytes, 
     return HESA_CUDA_OK;
 }
 
-cudaError_t launch_copy(const hesa_cuda_paged_kv* kv, const Tables& t, const PageWork& w, int64_t most, const int32_t* map, cudaStream_t s) {
-    const int slot_words = kv->n_kv_head * kv->head_dim / 8;
+CopyPools copy_pools(const hesa_cuda_paged_kv* kv) {
+    CopyPools p{};
+    p.n = 2;
+    for (int i = 0; i < 2; ++i) {
+        p.base[i] = static_cast<uint8_t*>(i ? kv->v : kv->k);
+        p.page[i] = kv->page_stride * 2;
+        p.layer[i] = kv->layer_stride * 2;
+        p.place[i] = kv->n_kv_head * kv->head_dim * 2;
+    }
+    return p;
+}
+CopyPools copy_pools(const hesa_cuda_paged_kv4* kv) {
+    CopyPools p{};
+    p.n = 4;
+    void* const base[4] = {kv->k, kv->v, kv->k_scale, kv->v_scale};
+    for (int i = 0; i < 4; ++i) {
+        const int group = i < 2 ? 16 : 2;   // bytes
+        p.base[i] = static_cast<uint8_t*>(base[i]);
+        p.page[i] = kv->page_stride * group;
+        p.layer[i] = kv->layer_stride * group;
+        p.place[i] = kv->n_kv_head * (kv->head_dim / kGroup) * group;
+    }
+    return p;
+}
+
+template <typename KV>
+cudaError_t launch_copy(const KV* kv, const Tables& t, const PageWork& w, int64_t most, const int32_t* map, cudaStream_t s) {
+    const CopyPools pools = copy_pools(kv);
     // eight blocks an SM keep enough loads in flight; fewer where fewer pages can move
-    const int64_t blocks = std::min<int64_t>(148 * 8, std::max<int64_t>(1, most * kv->n_layer * 2));
-    return launch_dep(copy_kernel, dim3(static_cast<unsigned>(blocks)), 256, 0, s, static_cast<uint4*>(kv->k), static_cast<uint4*>(kv->v),
-                      kv->page_stride / 8, kv->layer_stride / 8, kv->n_layer, slot_words, w.n_items, w.items, t, map);
+    const int64_t blocks = std::min<int64_t>(148 * 8, std::max<int64_t>(1, most * kv->n_layer * pools.n));
+    return launch_dep(copy_kernel, dim3(static_cast<unsigned>(blocks)), 256, 0, s, pools, kv->n_layer, w.n_items, w.items, t, map);
 }
 
-}  // namespace
-}  // namespace hesa_cuda
-
-using namespace hesa_cuda;
-
-extern "C" {
-
-size_t hesa_cuda_kv_pages_workspace_size(const hesa_cuda_paged_kv* kv) {
-    if (check_paged_kv(kv) != HESA_CUDA_OK) return 0;
-    if (kv->n_pages > (1 << 20)) return 0;
-    const size_t most = static_cast<size_t>(most_items(kv->n_pages, kv->n_slots));
-    return (4 + 4 * most + static_cast<size_t>(kv->n_pages) + static_cast<size_t>(kv->n_slots) + 1) * sizeof(int32_t);
-}
-
-int hesa_cuda_kv_reserve(const hesa_cuda_paged_kv* kv, const int32_t* slots, const int32_t* n_new, int32_t n, void* workspace,
+template <typename KV>
+int kv_reserve(const KV* kv, const int32_t* slots, const int32_t* n_new, int32_t n, void* workspace,
                          size_t workspace_bytes, void* stream) {
-    HESA_TRACE("hesa_cuda_kv_reserve");
     Tables t{};
     const int rc = page_op(kv, n, workspace, workspace_bytes, &t);
     if (rc != HESA_CUDA_OK) return rc;
@@ -539,9 +669,9 @@ int hesa_cuda_kv_reserve(const hesa_cuda_paged_kv* kv, const int32_t* slots, con
     return e == cudaSuccess ? HESA_CUDA_OK : record_cuda_error(e, "kv_reserve kernel");
 }
 
-int hesa_cuda_kv_free(const hesa_cuda_paged_kv* kv, const int32_t* slots, int32_t n, void* workspace, size_t workspace_bytes,
+template <typename KV>
+int kv_free(const KV* kv, const int32_t* slots, int32_t n, void* workspace, size_t workspace_bytes,
                       void* stream) {
-    HESA_TRACE("hesa_cuda_kv_free");
     Tables t{};
     const int rc = page_op(kv, n, workspace, workspace_bytes, &t);
     if (rc != HESA_CUDA_OK) return rc;
@@ -556,9 +686,9 @@ int hesa_cuda_kv_free(const hesa_cuda_paged_kv* kv, const int32_t* slots, int32_
     return e == cudaSuccess ? HESA_CUDA_OK : record_cuda_error(e, "kv_free kernel");
 }
 
-int hesa_cuda_kv_fork(const hesa_cuda_paged_kv* kv, const int32_t* src, const int32_t* dst, int32_t n, void* workspace,
+template <typename KV>
+int kv_fork(const KV* kv, const int32_t* src, const int32_t* dst, int32_t n, void* workspace,
                       size_t workspace_bytes, void* stream) {
-    HESA_TRACE("hesa_cuda_kv_fork");
     Tables t{};
     const int rc = page_op(kv, n, workspace, workspace_bytes, &t);
     if (rc != HESA_CUDA_OK) return rc;
@@ -576,8 +706,8 @@ int hesa_cuda_kv_fork(const hesa_cuda_paged_kv* kv, const int32_t* src, const in
     return e == cudaSuccess ? HESA_CUDA_OK : record_cuda_error(e, "kv_fork kernels");
 }
 
-int hesa_cuda_kv_compact(const hesa_cuda_paged_kv* kv, int32_t* n_live, void* workspace, size_t workspace_bytes, void* stream) {
-    HESA_TRACE("hesa_cuda_kv_compact");
+template <typename KV>
+int kv_compact(const KV* kv, int32_t* n_live, void* workspace, size_t workspace_bytes, void* stream) {
     Tables t{};
     const int rc = page_op(kv, 0, workspace, workspace_bytes, &t);
     if (rc != HESA_CUDA_OK) return rc;
@@ -592,9 +722,9 @@ int hesa_cuda_kv_compact(const hesa_cuda_paged_kv* kv, int32_t* n_live, void* wo
     return e == cudaSuccess ? HESA_CUDA_OK : record_cuda_error(e, "kv_compact kernels");
 }
 
-int hesa_cuda_kv_copy_pages(const hesa_cuda_paged_kv* kv, const int32_t* src_pages, const int32_t* dst_pages, int32_t n,
+template <typename KV>
+int kv_copy_pages(const KV* kv, const int32_t* src_pages, const int32_t* dst_pages, int32_t n,
                             void* workspace, size_t workspace_bytes, void* stream) {
-    HESA_TRACE("hesa_cuda_kv_copy_pages");
     Tables t{};
     const int rc = page_op(kv, n, workspace, workspace_bytes, &t);
     if (rc != HESA_CUDA_OK) return rc;
@@ -610,6 +740,98 @@ int hesa_cuda_kv_copy_pages(const hesa_cuda_paged_kv* kv, const int32_t* src_pag
     }
     if (e == cudaSuccess) e = launch_copy(kv, t, w, n, nullptr, s);
     return e == cudaSuccess ? HESA_CUDA_OK : record_cuda_error(e, "kv_copy_pages kernels");
+}
+
+template <typename KV>
+int kv_reorder(const KV* kv, const int32_t* slots, const int32_t* parents, int32_t n, int32_t width, void* workspace, size_t workspace_bytes,
+               void* stream) {
+    Tables t{};
+    const int rc = page_op(kv, n, workspace, workspace_bytes, &t);
+    if (rc != HESA_CUDA_OK) return rc;
+    if (n > kv->n_slots) return record_error(HESA_CUDA_SHAPE_MISMATCH, "more slots than the cache has");
+    if (width < 1 || width > 32 || n % width != 0) return record_error(HESA_CUDA_SHAPE_MISMATCH, "width must be 1 .. 32 and divide n");
+    if (n == 0) return HESA_CUDA_OK;
+    if (!slots || !parents) return record_error(HESA_CUDA_INVALID_ARGUMENT, "null pointer");
+    if (!aligned(slots, 4) || !aligned(parents, 4)) return record_error(HESA_CUDA_INVALID_ARGUMENT, "the lists must be 4-byte aligned");
+    const PageWork w = page_work(workspace, kv);
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    cudaError_t e = status_word(&t.status);
+    if (e == cudaSuccess) {
+        e = launch_dep(reorder_plan_kernel, dim3(1), kPlanThreads, 0, s, t, slots, parents, n, width, w);
+    }
+    if (e == cudaSuccess) e = launch_copy(kv, t, w, n, nullptr, s);
+    return e == cudaSuccess ? HESA_CUDA_OK : record_cuda_error(e, "kv_reorder kernels");
+}
+
+}  // namespace
+}  // namespace hesa_cuda
+
+using namespace hesa_cuda;
+
+extern "C" {
+
+size_t hesa_cuda_kv_pages_workspace_size(const hesa_cuda_paged_kv* kv) { return pages_workspace(kv); }
+
+int hesa_cuda_kv_reserve(const hesa_cuda_paged_kv* kv, const int32_t* slots, const int32_t* n_new, int32_t n, void* workspace, size_t workspace_bytes, void* stream) {
+    HESA_TRACE("hesa_cuda_kv_reserve");
+    return kv_reserve(kv, slots, n_new, n, workspace, workspace_bytes, stream);
+}
+
+int hesa_cuda_kv_free(const hesa_cuda_paged_kv* kv, const int32_t* slots, int32_t n, void* workspace, size_t workspace_bytes, void* stream) {
+    HESA_TRACE("hesa_cuda_kv_free");
+    return kv_free(kv, slots, n, workspace, workspace_bytes, stream);
+}
+
+int hesa_cuda_kv_fork(const hesa_cuda_paged_kv* kv, const int32_t* src, const int32_t* dst, int32_t n, void* workspace, size_t workspace_bytes, void* stream) {
+    HESA_TRACE("hesa_cuda_kv_fork");
+    return kv_fork(kv, src, dst, n, workspace, workspace_bytes, stream);
+}
+
+int hesa_cuda_kv_compact(const hesa_cuda_paged_kv* kv, int32_t* n_live, void* workspace, size_t workspace_bytes, void* stream) {
+    HESA_TRACE("hesa_cuda_kv_compact");
+    return kv_compact(kv, n_live, workspace, workspace_bytes, stream);
+}
+
+int hesa_cuda_kv_copy_pages(const hesa_cuda_paged_kv* kv, const int32_t* src_pages, const int32_t* dst_pages, int32_t n, void* workspace, size_t workspace_bytes, void* stream) {
+    HESA_TRACE("hesa_cuda_kv_copy_pages");
+    return kv_copy_pages(kv, src_pages, dst_pages, n, workspace, workspace_bytes, stream);
+}
+
+int hesa_cuda_kv_reorder(const hesa_cuda_paged_kv* kv, const int32_t* slots, const int32_t* parents, int32_t n, int32_t width, void* workspace, size_t workspace_bytes, void* stream) {
+    HESA_TRACE("hesa_cuda_kv_reorder");
+    return kv_reorder(kv, slots, parents, n, width, workspace, workspace_bytes, stream);
+}
+
+size_t hesa_cuda_kv4_pages_workspace_size(const hesa_cuda_paged_kv4* kv) { return pages_workspace(kv); }
+
+int hesa_cuda_kv4_reserve(const hesa_cuda_paged_kv4* kv, const int32_t* slots, const int32_t* n_new, int32_t n, void* workspace, size_t workspace_bytes, void* stream) {
+    HESA_TRACE("hesa_cuda_kv4_reserve");
+    return kv_reserve(kv, slots, n_new, n, workspace, workspace_bytes, stream);
+}
+
+int hesa_cuda_kv4_free(const hesa_cuda_paged_kv4* kv, const int32_t* slots, int32_t n, void* workspace, size_t workspace_bytes, void* stream) {
+    HESA_TRACE("hesa_cuda_kv4_free");
+    return kv_free(kv, slots, n, workspace, workspace_bytes, stream);
+}
+
+int hesa_cuda_kv4_fork(const hesa_cuda_paged_kv4* kv, const int32_t* src, const int32_t* dst, int32_t n, void* workspace, size_t workspace_bytes, void* stream) {
+    HESA_TRACE("hesa_cuda_kv4_fork");
+    return kv_fork(kv, src, dst, n, workspace, workspace_bytes, stream);
+}
+
+int hesa_cuda_kv4_compact(const hesa_cuda_paged_kv4* kv, int32_t* n_live, void* workspace, size_t workspace_bytes, void* stream) {
+    HESA_TRACE("hesa_cuda_kv4_compact");
+    return kv_compact(kv, n_live, workspace, workspace_bytes, stream);
+}
+
+int hesa_cuda_kv4_copy_pages(const hesa_cuda_paged_kv4* kv, const int32_t* src_pages, const int32_t* dst_pages, int32_t n, void* workspace, size_t workspace_bytes, void* stream) {
+    HESA_TRACE("hesa_cuda_kv4_copy_pages");
+    return kv_copy_pages(kv, src_pages, dst_pages, n, workspace, workspace_bytes, stream);
+}
+
+int hesa_cuda_kv4_reorder(const hesa_cuda_paged_kv4* kv, const int32_t* slots, const int32_t* parents, int32_t n, int32_t width, void* workspace, size_t workspace_bytes, void* stream) {
+    HESA_TRACE("hesa_cuda_kv4_reorder");
+    return kv_reorder(kv, slots, parents, n, width, workspace, workspace_bytes, stream);
 }
 
 int hesa_cuda_rope_kv_paged(const hesa_cuda_paged_kv* kv, int32_t layer, const hesa_cuda_token_batch* batch, float* q, int64_t ldq,

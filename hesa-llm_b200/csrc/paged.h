@@ -240,7 +240,50 @@ cudaError_t launch_dep(void (*kernel)(P...), dim3 grid, int threads, size_t smem
 // code with its message recorded.
 int check_paged_kv(const hesa_cuda_paged_kv* kv);
 int check_batch(const hesa_cuda_paged_kv* kv, int32_t layer, const hesa_cuda_token_batch* b, int64_t n_head);
+// The checks of strides, tables and counts that caches of both kinds share; strides count units of `unit` values.
+struct PagedShape {
+    const int32_t *table, *seq_len;
+    int64_t page_stride, layer_stride;
+    int32_t unit, n_layer, n_pages, page_size, n_kv_head, head_dim, n_slots, max_pages;
+};
+int check_paged_shape(const PagedShape& c);
+
+// ---- the cache in 4 bits (paged_attention4.cu, kv4_cache.cu) ----
+constexpr int kGroup = 32;          // values of a group: 16 bytes of codes, one scale
+constexpr float kMostScale = 2720.f;   // 24 of it is an fp16 number
+
+// One layer: group (s * n_kv + h) * (head_dim / 32) + g of page p lies p * page_stride groups behind the pools' starts.
+struct Pools4 {
+    const uint4* k;
+    const uint4* v;
+    const __half* ks;
+    const __half* vs;
+};
+int check_paged_kv4(const hesa_cuda_paged_kv4* kv);
+int check_batch4(const hesa_cuda_paged_kv4* kv, int32_t layer, const hesa_cuda_token_batch* b, int64_t n_head);
+// The tables and the shape, strides in groups; k and v are null.
+PagedLayer layer_of4(const hesa_cuda_paged_kv4* kv);
+Pools4 pools_of(const hesa_cuda_paged_kv4* kv, int32_t layer);
+
+// Eight codes of a word as four pairs of values, (e, e + 4) for e = 0 .. 3: a code
+// put behind the leading bit of an fp16 number is 16 + code, and (16 + code) d - 24 d
+// = (code - 8) d takes one fma, exact because d has 8 bits. m = -24 d.
+__device__ __forceinline__ __half2 code_pair(uint32_t shifted, __half2 d, __half2 m) {
+    uint32_t x = (shifted & 0x03C003C0u) | 0x4C004C00u;
+    return __hfma2(*reinterpret_cast<__half2*>(&x), d, m);
+}
+__device__ __forceinline__ void code_pairs(uint32_t w, __half2 d, __half2 m, uint32_t (&p)[4]) {
+    const __half2 a = code_pair(w << 6, d, m), b = code_pair(w << 2, d, m), c = code_pair(w >> 2, d, m), e = code_pair(w >> 6, d, m);
+    p[0] = *reinterpret_cast<const uint32_t*>(&a);
+    p[1] = *reinterpret_cast<const uint32_t*>(&b);
+    p[2] = *reinterpret_cast<const uint32_t*>(&c);
+    p[3] = *reinterpret_cast<const uint32_t*>(&e);
+}
 PagedLayer layer_of(const hesa_cuda_paged_kv* kv, int32_t layer);
 BatchView view_of(const hesa_cuda_token_batch* b);
+// The checks of attention's other arguments, and those that do not depend on the cache's kind in *args: b, q, out, the
+// options and part.
+int attention_args(int32_t head_dim, int32_t n_kv_head, const hesa_cuda_token_batch* batch, const float* q, int64_t ldq, float* out, int64_t ldo,
+                   int64_t n_head, const hesa_cuda_attn_options* options, void* workspace, AttnArgs* args);
 
 }  // namespace hesa_cuda

@@ -40,6 +40,7 @@
 // 167 us (6.4 TB/s); 32 of 1 to 8192 tokens 34.2 us (3.7 TB/s, the first copies and
 // the joining cost 10 of them); one of 2048 tokens, 32 heads, 15.4 us (2.2 TB/s).
 #include "paged.h"
+#include "paged_rows.cuh"
 #include "paged_tc.h"
 #include "abi_errors.h"
 #include "decode_ops.h"
@@ -52,9 +53,7 @@
 namespace hesa_cuda {
 namespace {
 
-constexpr int kRowTile = 8;
 constexpr int kKeyBlock = 16;
-constexpr int kRowsCtas = 148;       // one an SM
 constexpr int kCopyWarps = 4;        // a warp gets no more than one bulk copy under way in about 45 ns
 // Rows of a sequence above which 128-row tiles are used, though they may be
 // empty for the most part, rather than several tiles of 8 that each read K and V.
@@ -62,49 +61,17 @@ constexpr int kCopyWarps = 4;        // a warp gets no more than one bulk copy u
 // there; 32 rows 45 and 39; 64 rows 82 and 39. 16 heads of 256 on 4: 32 rows 52 and
 // 74, 64 rows 89 and 75.
 constexpr int most_rows(int head_dim) { return head_dim == 256 ? 48 : 16; }
-constexpr int kMostTiles = 1024;     // of a launch: the tiles' blocks are summed in shared memory
 constexpr int kSegCost = 5;          // stages that starting a (tile, group) takes the time of
-constexpr int kLeastUnits = 4;       // of a run
 
-template <int HD> struct RowsShape {
-    static constexpr int warps = HD == 256 ? 4 : 8;       // and kCopyWarps that copy
+// 8 warps (4 with head_dim 256) and kCopyWarps that copy
+template <int HD> struct RowsShape : RowParts<HD, (HD == 256 ? 4 : 8)> {
+    using RowParts<HD, (HD == 256 ? 4 : 8)>::warps;
     static constexpr int threads = (warps + kCopyWarps) * 32;
     static constexpr int stages = HD == 64 ? 5 : 3;
     // a stage: K then V of `subs` blocks, rows of `heads` heads padded by 16 bytes; heads * subs <= warps
     static constexpr size_t stage_bytes = 2 * kKeyBlock * (warps * HD * 2 + warps * 16);
     static constexpr size_t smem = stages * stage_bytes;
-    // workspace: the list of what is to be added up, then the parts' rows (m, l), then their acc[HD]; a part has
-    // [warps][rows] of them
-    static constexpr size_t cut_bytes = kMostTiles * 32;
-    static constexpr size_t part_rows(int64_t parts) { return static_cast<size_t>(parts) * warps * kRowTile; }
-    static constexpr size_t bytes(int64_t parts) { return cut_bytes + part_rows(parts) * (2 + HD) * 4; }
 };
-
-// Heads of a group (a CTA's warps have one each) and how many warps share a head.
-struct HeadGroups {
-    int groups, heads, subs, recip, cost, sub_bits;   // subs is a power of two, `warps` being one
-    // `most` heads a group at most, a power of two up to `warps`
-    HeadGroups(int n_kv, int warps, int most) {
-        groups = (n_kv + most - 1) / most;
-        heads = (n_kv + groups - 1) / groups;
-        for (sub_bits = 0; (heads << (sub_bits + 1)) <= warps;) ++sub_bits;
-        subs = 1 << sub_bits;
-        recip = (256 + heads - 1) / heads;
-        cost = kSegCost * subs;
-    }
-    __device__ __forceinline__ int sub_of(int warp) const { return warp * recip >> 8; }   // warp / heads for warp < 9
-};
-
-// Parts of a launch: two a CTA (its run's first (tile, group) and its last), and,
-// where several warps share a head, one for each (tile, group) that lies in one run.
-__host__ __device__ inline int64_t part_count(int tiles, const HeadGroups& hg) {
-    return 2 * kRowsCtas + (hg.subs > 1 ? static_cast<int64_t>(tiles) * hg.groups : 0);
-}
-
-// Whether every (tile, group) has an entry in the list of what is to be added up.
-__host__ __device__ inline bool by_tile(int tiles, const HeadGroups& hg) {
-    return hg.subs > 1 || static_cast<int64_t>(tiles) * hg.groups <= kRowsCtas;
-}
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -118,85 +85,6 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
                  : "r"(addr)
                  : "memory");
 }
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// 64-bit quotients of numbers that are small nearly always
-__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
-    if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
-    return a / b;
-}
-
-// The runs: CTA c of n_cta has units [start(c), start(c + 1)), `each` of them,
-// the first `more` CTAs one more.
-struct Runs {
-    int64_t each, more;
-    int n_cta;
-    __device__ __forceinline__ Runs(int64_t units, int most) {
-        n_cta = static_cast<int>(max(int64_t(1), min(static_cast<int64_t>(most), units / kLeastUnits)));
-        each = quotient(units, n_cta);
-        more = units - each * n_cta;
-    }
-    __device__ __forceinline__ int64_t start(int c) const { return each * c + min(static_cast<int64_t>(c), more); }
-    __device__ __forceinline__ int cta_of(int64_t u) const {   // the last c with start(c) <= u
-        const int64_t head = more * (each + 1);
-        return static_cast<int>(u < head ? quotient(u, each + 1) : more + quotient(u - head, each));
-    }
-};
-
-// What a CTA's run has of one (tile, group): blocks [b0, b1).
-struct Segment {
-    int tile, grp, b0, b1;
-    int64_t first;   // its first unit; the blocks' units start hg.cost later
-    int64_t units;
-};
-
-// The next segment with blocks of the run [u, end); u moves behind it. `lo` is a
-// tile that starts at or before u.
-__device__ __forceinline__ bool next_segment(const int64_t* pre, const HeadGroups& hg, int64_t& u, int64_t end, int& lo, Segment& s) {
-    while (u < end) {
-        while (pre[lo + 1] * hg.groups <= u) ++lo;   // tiles without rows have no units
-        s.tile = lo;
-        s.units = pre[lo + 1] - pre[lo];
-        s.grp = static_cast<int>(quotient(u - pre[lo] * hg.groups, s.units));
-        s.first = pre[lo] * hg.groups + s.grp * s.units;
-        const int64_t from = max(u, s.first + hg.cost), stop = min(end, s.first + s.units);
-        u = stop;
-        s.b0 = static_cast<int>(from - s.first - hg.cost);
-        s.b1 = static_cast<int>(stop - s.first - hg.cost);
-        if (s.b1 > s.b0) return true;
-    }
-    return false;
-}
-
-// The rows and keys of a tile.
-struct TileView {
-    SeqView sv;
-    int n_rows, r0, base;   // base: position of the sequence's first new token
-    int32_t p_lo, p_hi;
-    Mask mask;
-    KeyBlocks kb;
-};
-
-__device__ __forceinline__ TileView tile_view(const AttnArgs& A, int idx) {
-    TileView v;
-    int seq, tile;
-    const bool some = locate_tile(A.b, A.group, kRowTile, A.per_seq, A.tile0 + idx, seq, tile);
-    v.sv = seq_view(A.c, A.b, seq);
-    v.n_rows = some ? v.sv.n_new * A.group : 0;
-    v.r0 = tile * kRowTile;
-    v.base = v.sv.len - v.sv.n_new;
-    v.p_lo = v.base + A.group_div.div(v.r0);
-    v.p_hi = v.base + A.group_div.div(max(min(v.r0 + kRowTile, v.n_rows), 1) - 1);
-    v.mask = Mask{v.sv.len, A.window, 0};
-    if (A.prefix && v.sv.ok) v.mask.prefix = max(0, min(A.prefix[seq], v.sv.len));
-    v.kb = key_blocks(v.mask, v.p_lo, v.p_hi, kKeyBlock);
-    return v;
-}
-
 // The ring between the producer and the consumer warps.
 struct Ring {
     uint8_t* smem;
@@ -213,7 +101,7 @@ template <int HD>
 __device__ __forceinline__ void copy_segment(const AttnArgs& A, Ring& ring, const HeadGroups& hg, const Segment& seg, int pw) {
     using S = RowsShape<HD>;
     const int lane = threadIdx.x & 31;
-    const TileView tv = tile_view(A, seg.tile);
+    const TileView tv = tile_view<kKeyBlock>(A, seg.tile);
     const int i1 = min(tv.kb.n, seg.b1);
     const int32_t* table = A.c.table + static_cast<int64_t>(tv.sv.slot) * A.c.max_pages;
     const int row = pw * 8 + (lane & 7), v = row >> 4;
@@ -445,18 +333,6 @@ __device__ __forceinline__ void rows_segment(const AttnArgs& A, Ring& ring, cons
     }
 }
 
-// What combine_kernel adds up, and where it belongs: rows r0 .. r0 + rows - 1 of
-// the sequence whose first row of q is q0. The parts are `first`, then the
-// first part of each of the next n - 1 CTAs, each of hg.subs warps. n = 0, or one
-// part of one warp: nothing. With by_tile every (tile, group) has an entry (groups
-// of fewer heads are only made of few tiles, so kMostTiles entries are enough); else
-// there is one for each CTA, for the cut before its run (if it is the first one of
-// what it cuts).
-struct __align__(16) Cut {
-    int32_t grp, first, n, rows;
-    int32_t r0, q0, pad[2];
-};
-
 template <int HD>
 __global__ void __launch_bounds__(RowsShape<HD>::threads, 1)
 rows_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ HeadGroups hg) {
@@ -478,33 +354,7 @@ rows_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ HeadGrou
     }
     grid_dep_wait();
     grid_dep_launch();   // combine_kernel may be set up meanwhile; it waits for this grid's end
-    int64_t before = 0;
-    for (int i0 = 0; i0 < tiles; i0 += S::threads) {
-        const int i = i0 + threadIdx.x;
-        int64_t v = 0;
-        if (i < tiles) {
-            const TileView tv = tile_view(A, i);
-            if (!tv.sv.ok && cta == 0) record_status(A.status, kStatusBadPosition);
-            // a tile whose rows see nothing has one block too: its zeros are written there
-            if (tv.sv.ok && tv.r0 < tv.n_rows) v = max(1, tv.kb.n) + hg.cost;
-        }
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t y = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= o) v += y;
-        }
-        if (lane == 31) s_sum[warp] = v;
-        __syncthreads();
-        int64_t all = 0;
-        for (int w = 0; w < S::warps + kCopyWarps; ++w) {
-            if (w < warp) v += s_sum[w];
-            all += s_sum[w];
-        }
-        if (i < tiles) s_pre[i + 1] = before + v;
-        before += all;
-        __syncthreads();
-    }
-    const int64_t units = before * hg.groups;
+    const int64_t units = tile_units<S::warps + kCopyWarps, kKeyBlock>(A, hg, tiles, s_pre, s_sum) * hg.groups;
     const Runs runs(units, gridDim.x);
     const bool listed_by_tile = by_tile(tiles, hg);
     Cut* cuts = reinterpret_cast<Cut*>(A.part);
@@ -514,12 +364,7 @@ rows_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ HeadGrou
         end = runs.start(cta + 1);
     }
     const int64_t begin = u;
-    int lo = 0, hi = tiles - 1;   // the last tile that starts at or before u
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (s_pre[mid] * hg.groups <= u) lo = mid;
-        else hi = mid - 1;
-    }
+    int lo = tile_at(s_pre, hg, tiles, u);
     Ring ring{smem, s_full, s_empty, 0u, static_cast<uint32_t>(hg.heads * HD * 2 + 16), true};
     Segment seg;
     if (warp >= S::warps) {
@@ -537,7 +382,7 @@ rows_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ HeadGrou
         const int c_first = runs.cta_of(seg.first + hg.cost), c_last = runs.cta_of(seg.first + seg.units - 1);
         const bool uncut = c_first == c_last;
         const int own_part = 2 * kRowsCtas + seg.tile * hg.groups + seg.grp;   // of what several warps share, uncut
-        const TileView tv = tile_view(A, seg.tile);
+        const TileView tv = tile_view<kKeyBlock>(A, seg.tile);
         const Cut all{seg.grp, uncut ? own_part : 2 * c_first + (runs.start(c_first) >= seg.first ? 0 : 1), c_last - c_first + 1,
                       min(kRowTile, tv.n_rows - tv.r0), tv.r0, tv.sv.q0};
         if (cta == c_first + 1) cut = all;
@@ -545,97 +390,6 @@ rows_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ HeadGrou
         rows_segment<HD>(A, ring, hg, seg, tv, !uncut ? 2 * cta + (begin >= seg.first ? 0 : 1) : hg.subs > 1 ? own_part : -1);
     }
     if (!listed_by_tile && threadIdx.x == 0) cuts[cta] = cut;
-}
-
-// Adds up what is cut: block (entry, head of the group), or one for each row too
-// where these are few (then there are many parts). The rows are shared out over
-// the warps; where they are fewer than eight, several warps take every second,
-// fourth or eighth part of a row. Two contexts of 131072 and 100001 tokens with a
-// block for all eight rows: 180 us; with one for each: 163. A batch of 64 short
-// sequences: 13.7 us and 17.6.
-template <int HD>
-__global__ void __launch_bounds__(256)
-combine_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ HeadGroups hg) {
-    using S = RowsShape<HD>;
-    constexpr int V = HD / 32;     // values of a lane
-    constexpr int AHEAD = 32 / V;  // parts of which a warp has the loads under way
-    __shared__ float s_o[8][HD + 1];
-    const int hl = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    grid_dep_wait();
-    grid_dep_launch();
-    const int4* c4 = reinterpret_cast<const int4*>(A.part) + 2 * blockIdx.x;
-    const int4 ca = __ldcg(c4), cb = __ldcg(c4 + 1);
-    const Cut cut{ca.x, ca.y, ca.z, ca.w, cb.x, cb.y};
-    const int n = cut.n * hg.subs, kvh = cut.grp * hg.heads + hl;
-    if (n < 2 || kvh >= A.c.n_kv) return;
-    const int row0 = blockIdx.z, rows = min(gridDim.z > 1 ? 1 : kRowTile, cut.rows - row0);
-    if (rows <= 0) return;
-    const int slots = rows > 4 ? 8 : rows > 2 ? 4 : rows;   // a power of two
-    const int row = warp & (slots - 1), share = warp / slots, shares = 8 / slots;   // row: of row0 ..
-    const float* ml = A.part + S::cut_bytes / 4;
-    const float* acc = ml + S::part_rows(part_count(A.n_split, hg)) * 2;
-    auto at = [&](int i) {   // part i: sub-part i % subs of CTA part i / subs
-        const int p = i >> hg.sub_bits, x = i & (hg.subs - 1);
-        return (static_cast<int64_t>(p == 0 ? cut.first : 2 * ((cut.first >> 1) + p)) * S::warps + x * hg.heads + hl) * kRowTile + row0 + row;
-    };
-    float L = 0.f, O[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) O[k] = 0.f;
-    if (row < rows) {
-        float2 p[AHEAD];
-        float v[AHEAD][V];
-        auto load = [&](int i0) {
-#pragma unroll
-            for (int k = 0; k < AHEAD; ++k) {
-                const int i = i0 + k * shares;
-                if (i >= n) break;
-                const int64_t a = at(i);
-                p[k] = __ldcg(reinterpret_cast<const float2*>(ml + a * 2));
-                const float* src = acc + a * HD + lane * V;
-                if constexpr (V == 2) *reinterpret_cast<float2*>(v[k]) = __ldcg(reinterpret_cast<const float2*>(src));
-                else
-#pragma unroll
-                    for (int c = 0; c < V; c += 4) *reinterpret_cast<float4*>(v[k] + c) = __ldcg(reinterpret_cast<const float4*>(src + c));
-            }
-        };
-        load(share);   // on their way while the maximum is found
-        float M = -INFINITY;
-#pragma unroll 8
-        for (int i = lane; i < n; i += 32) M = fmaxf(M, __ldcg(ml + at(i) * 2));
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-        for (int i0 = share;;) {
-#pragma unroll
-            for (int k = 0; k < AHEAD; ++k) {
-                if (i0 + k * shares >= n) break;
-                // a part that saw nothing adds zeros, or the NaN of a row that is not finite
-                const float f = p[k].x == -INFINITY ? 1.f : ex2(p[k].x - M);
-                L = fmaf(p[k].y, f, L);
-#pragma unroll
-                for (int c = 0; c < V; ++c) O[c] = fmaf(v[k][c], f, O[c]);
-            }
-            i0 += AHEAD * shares;
-            if (i0 >= n) break;
-            load(i0);
-        }
-        if (shares > 1) {
-#pragma unroll
-            for (int c = 0; c < V; ++c) s_o[warp][lane * V + c] = O[c];
-            if (lane == 0) s_o[warp][HD] = L;
-        }
-    }
-    if (shares > 1) __syncthreads();
-    if (row >= rows || share > 0) return;
-    for (int x = 1; x < shares; ++x) {
-        L += s_o[warp + x * slots][HD];
-#pragma unroll
-        for (int c = 0; c < V; ++c) O[c] += s_o[warp + x * slots][lane * V + c];
-    }
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    const int r = cut.r0 + row0 + row, t = A.group_div.div(r), h = kvh * A.group + r - t * A.group;
-    float* o = A.out + static_cast<int64_t>(cut.q0 + t) * A.ldo + static_cast<int64_t>(h) * HD + lane * V;
-#pragma unroll
-    for (int c = 0; c < V; c += 2) *reinterpret_cast<float2*>(o + c) = make_float2(O[c] * inv, O[c + 1] * inv);
 }
 
 struct Plan {
@@ -683,7 +437,7 @@ Plan make_plan(const hesa_cuda_paged_kv* kv, const hesa_cuda_token_batch* b, int
 
 size_t part_bytes(const Plan& p, const hesa_cuda_paged_kv* kv) {
     if (!p.tc) {
-        const HeadGroups hg(kv->n_kv_head, kv->head_dim == 256 ? RowsShape<256>::warps : RowsShape<128>::warps, p.heads);
+        const HeadGroups hg(kv->n_kv_head, kv->head_dim == 256 ? RowsShape<256>::warps : RowsShape<128>::warps, p.heads, kSegCost);
         const int64_t parts = part_count(std::min(p.tiles, kMostTiles), hg);
         return kv->head_dim == 64 ? RowsShape<64>::bytes(parts) : kv->head_dim == 128 ? RowsShape<128>::bytes(parts) : RowsShape<256>::bytes(parts);
     }
@@ -705,7 +459,7 @@ cudaError_t launch_rows(AttnArgs a, const Plan& p, cudaStream_t s) {
         set[dev] = true;
     }
     using S = RowsShape<HD>;
-    const HeadGroups hg(a.c.n_kv, S::warps, p.heads);
+    const HeadGroups hg(a.c.n_kv, S::warps, p.heads, kSegCost);
     for (a.tile0 = 0; a.tile0 < p.tiles && e == cudaSuccess; a.tile0 += kMostTiles) {
         a.n_split = std::min(kMostTiles, p.tiles - a.tile0);
         e = launch_dep(rows_kernel<HD>, dim3(kRowsCtas), S::threads, S::smem, s, a, hg);
@@ -713,7 +467,7 @@ cudaError_t launch_rows(AttnArgs a, const Plan& p, cudaStream_t s) {
         const int rows = std::min(kRowTile, a.b.max_new * a.group);
         const unsigned z = static_cast<int64_t>(cuts) * hg.heads * rows <= 8 * kRowsCtas ? rows : 1;
         if (e == cudaSuccess)
-            e = launch_dep(combine_kernel<HD>, dim3(static_cast<unsigned>(cuts), static_cast<unsigned>(hg.heads), z), 256, 0, s, a, hg);
+            e = launch_dep(combine_kernel<HD, S::warps>, dim3(static_cast<unsigned>(cuts), static_cast<unsigned>(hg.heads), z), 256, 0, s, a, hg);
     }
     return e;
 }
@@ -722,29 +476,37 @@ bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p
 
 }  // namespace
 
-int check_paged_kv(const hesa_cuda_paged_kv* kv) {
-    if (!kv || !kv->k || !kv->v || !kv->table || !kv->seq_len) return record_error(HESA_CUDA_INVALID_ARGUMENT, "null pointer");
-    if (kv->n_layer <= 0 || kv->n_pages <= 0 || kv->page_size <= 0 || kv->n_kv_head <= 0 || kv->n_slots <= 0 || kv->max_pages <= 0)
+int check_paged_shape(const PagedShape& c) {
+    if (c.n_layer <= 0 || c.n_pages <= 0 || c.page_size <= 0 || c.n_kv_head <= 0 || c.n_slots <= 0 || c.max_pages <= 0)
         return record_error(HESA_CUDA_SHAPE_MISMATCH, "non-positive dimension");
-    if (kv->head_dim != 64 && kv->head_dim != 128 && kv->head_dim != 256)
+    if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256)
         return record_error(HESA_CUDA_SHAPE_MISMATCH, "head_dim must be 64, 128 or 256");
-    if (kv->page_size > 65536 || kv->n_kv_head > 1024 || kv->n_slots > 65536 || kv->n_layer > 4096 ||
-        static_cast<int64_t>(kv->max_pages) * kv->page_size >= (int64_t(1) << 30))
+    if (c.page_size > 65536 || c.n_kv_head > 1024 || c.n_slots > 65536 || c.n_layer > 4096 ||
+        static_cast<int64_t>(c.max_pages) * c.page_size >= (int64_t(1) << 30))
         return record_error(HESA_CUDA_SHAPE_MISMATCH, "paged cache too large");
-    const int64_t page = static_cast<int64_t>(kv->page_size) * kv->n_kv_head * kv->head_dim;
-    if (page > (int64_t(1) << 30)) return record_error(HESA_CUDA_SHAPE_MISMATCH, "pages of more than 2^30 values");
+    const int64_t values = static_cast<int64_t>(c.page_size) * c.n_kv_head * c.head_dim, page = values / c.unit;
+    if (values > (int64_t(1) << 30)) return record_error(HESA_CUDA_SHAPE_MISMATCH, "pages of more than 2^30 values");
     const int64_t most = int64_t(1) << 50;
-    if (kv->page_stride < page || kv->page_stride > most || kv->layer_stride < 0 || kv->layer_stride > most || (kv->page_stride & 7) || (kv->layer_stride & 7))
+    if (c.page_stride < page || c.page_stride > most || c.layer_stride < 0 || c.layer_stride > most || (c.page_stride & 7) || (c.layer_stride & 7))
         return record_error(HESA_CUDA_SHAPE_MISMATCH, "page_stride and layer_stride must be multiples of 8, page_stride at least a page");
-    if (kv->n_layer > 1 && kv->layer_stride < (static_cast<int64_t>(kv->n_pages) - 1) * kv->page_stride + page &&
-        (kv->layer_stride < page || kv->page_stride < (static_cast<int64_t>(kv->n_layer) - 1) * kv->layer_stride + page))
+    if (c.n_layer > 1 && c.layer_stride < (static_cast<int64_t>(c.n_pages) - 1) * c.page_stride + page &&
+        (c.layer_stride < page || c.page_stride < (static_cast<int64_t>(c.n_layer) - 1) * c.layer_stride + page))
         return record_error(HESA_CUDA_SHAPE_MISMATCH, "the pages of two layers overlap");
-    if (!aligned(kv->k, 16) || !aligned(kv->v, 16)) return record_error(HESA_CUDA_INVALID_ARGUMENT, "the page pools must be 16-byte aligned");
-    if (!aligned(kv->table, 4) || !aligned(kv->seq_len, 4)) return record_error(HESA_CUDA_INVALID_ARGUMENT, "the tables must be 4-byte aligned");
+    if (!aligned(c.table, 4) || !aligned(c.seq_len, 4)) return record_error(HESA_CUDA_INVALID_ARGUMENT, "the tables must be 4-byte aligned");
     return HESA_CUDA_OK;
 }
 
-int check_batch(const hesa_cuda_paged_kv* kv, int32_t layer, const hesa_cuda_token_batch* b, int64_t n_head) {
+int check_paged_kv(const hesa_cuda_paged_kv* kv) {
+    if (!kv || !kv->k || !kv->v || !kv->table || !kv->seq_len) return record_error(HESA_CUDA_INVALID_ARGUMENT, "null pointer");
+    const int rc = check_paged_shape({kv->table, kv->seq_len, kv->page_stride, kv->layer_stride, 1, kv->n_layer, kv->n_pages, kv->page_size, kv->n_kv_head,
+                                      kv->head_dim, kv->n_slots, kv->max_pages});
+    if (rc != HESA_CUDA_OK) return rc;
+    if (!aligned(kv->k, 16) || !aligned(kv->v, 16)) return record_error(HESA_CUDA_INVALID_ARGUMENT, "the page pools must be 16-byte aligned");
+    return HESA_CUDA_OK;
+}
+
+template <typename KV>
+static int check_rows(const KV* kv, int32_t layer, const hesa_cuda_token_batch* b, int64_t n_head) {
     if (layer < 0 || layer >= kv->n_layer) return record_error(HESA_CUDA_INVALID_ARGUMENT, "no such layer");
     if (!b || !b->q_start) return record_error(HESA_CUDA_INVALID_ARGUMENT, "null pointer");
     if (!aligned(b->q_start, 4) || !aligned(b->slots, 4)) return record_error(HESA_CUDA_INVALID_ARGUMENT, "q_start and slots must be 4-byte aligned");
@@ -758,6 +520,8 @@ int check_batch(const hesa_cuda_paged_kv* kv, int32_t layer, const hesa_cuda_tok
         return record_error(HESA_CUDA_SHAPE_MISMATCH, "too many rows");
     return HESA_CUDA_OK;
 }
+int check_batch(const hesa_cuda_paged_kv* kv, int32_t layer, const hesa_cuda_token_batch* b, int64_t n_head) { return check_rows(kv, layer, b, n_head); }
+int check_batch4(const hesa_cuda_paged_kv4* kv, int32_t layer, const hesa_cuda_token_batch* b, int64_t n_head) { return check_rows(kv, layer, b, n_head); }
 
 PagedLayer layer_of(const hesa_cuda_paged_kv* kv, int32_t layer) {
     PagedLayer c{};
@@ -777,6 +541,46 @@ PagedLayer layer_of(const hesa_cuda_paged_kv* kv, int32_t layer) {
 }
 
 BatchView view_of(const hesa_cuda_token_batch* b) { return BatchView{b->slots, b->q_start, b->n_seq, b->n_tokens, b->max_new, b->max_len}; }
+
+int attention_args(int32_t head_dim, int32_t n_kv_head, const hesa_cuda_token_batch* batch, const float* q, int64_t ldq, float* out, int64_t ldo,
+                   int64_t n_head, const hesa_cuda_attn_options* options, void* workspace, AttnArgs* args) {
+    AttnArgs& a = *args;
+    if (!q || !out || !workspace) return record_error(HESA_CUDA_INVALID_ARGUMENT, "null pointer");
+    const int64_t width = n_head * head_dim;
+    if (ldq < width || ldo < width || ldq > (int64_t(1) << 40) || ldo > (int64_t(1) << 40))
+        return record_error(HESA_CUDA_SHAPE_MISMATCH, "leading dimension too small");
+    if (!aligned(q, 16) || !aligned(out, 16) || (ldq & 3) || (ldo & 3))
+        return record_error(HESA_CUDA_INVALID_ARGUMENT, "q / out must be 16-byte aligned with ldq, ldo multiples of 4");
+    if (!aligned(workspace, 16)) return record_error(HESA_CUDA_INVALID_ARGUMENT, "workspace must be 16-byte aligned");
+    hesa_cuda_attn_options o{};
+    if (options) o = *options;
+    if (!(o.scale >= 0.f) || !std::isfinite(o.scale) || o.window < 0)
+        return record_error(HESA_CUDA_INVALID_ARGUMENT, "scale and window must be finite and not negative");
+    if (o.softcap != 0.f && !(o.softcap >= 1e-6f && o.softcap <= 1e6f))
+        return record_error(HESA_CUDA_INVALID_ARGUMENT, "softcap must be 0 or 1e-6 .. 1e6");
+    if (!aligned(o.slopes, 4) || !aligned(o.prefix, 4)) return record_error(HESA_CUDA_INVALID_ARGUMENT, "slopes and prefix must be 4-byte aligned");
+    if (batch->max_new == 0) return HESA_CUDA_OK;   // nothing will run
+    a.b = view_of(batch);
+    a.q = q;
+    a.ldq = ldq;
+    a.out = out;
+    a.ldo = ldo;
+    a.n_head = static_cast<int32_t>(n_head);
+    a.group = static_cast<int32_t>(n_head / n_kv_head);
+    a.group_div = FastDiv(a.group);
+    const double log2e = 1.4426950408889634;
+    const double scale = o.scale > 0.f ? o.scale : 1.0 / std::sqrt(static_cast<double>(head_dim));
+    a.scale2 = static_cast<float>(scale * log2e);
+    a.cap2 = static_cast<float>(o.softcap * log2e);
+    a.cap_in = o.softcap > 0.f ? static_cast<float>(scale / o.softcap) : 0.f;
+    if (!std::isfinite(a.scale2) || !std::isfinite(a.cap_in))
+        return record_error(HESA_CUDA_INVALID_ARGUMENT, "scale is too large for a float, by itself or by softcap");
+    a.window = std::min(o.window, 1 << 30);   // wider than any context; a position less a window stays in 32 bits
+    a.slopes = o.slopes;
+    a.prefix = o.prefix;
+    a.part = static_cast<float*>(workspace);
+    return HESA_CUDA_OK;
+}
 
 }  // namespace hesa_cuda
 
@@ -798,46 +602,15 @@ int hesa_cuda_paged_attention(const hesa_cuda_paged_kv* kv, int32_t layer, const
     if (rc == HESA_CUDA_OK) rc = check_batch(kv, layer, batch, n_head);
     if (rc != HESA_CUDA_OK) return rc;
     if (batch->n_tokens == 0) return HESA_CUDA_OK;   // no rows: their buffers may be null
-    if (!q || !out || !workspace) return record_error(HESA_CUDA_INVALID_ARGUMENT, "null pointer");
-    const int64_t width = n_head * kv->head_dim;
-    if (ldq < width || ldo < width || ldq > (int64_t(1) << 40) || ldo > (int64_t(1) << 40))
-        return record_error(HESA_CUDA_SHAPE_MISMATCH, "leading dimension too small");
-    if (!aligned(q, 16) || !aligned(out, 16) || (ldq & 3) || (ldo & 3))
-        return record_error(HESA_CUDA_INVALID_ARGUMENT, "q / out must be 16-byte aligned with ldq, ldo multiples of 4");
-    if (!aligned(workspace, 16)) return record_error(HESA_CUDA_INVALID_ARGUMENT, "workspace must be 16-byte aligned");
+    AttnArgs a{};
+    rc = attention_args(kv->head_dim, kv->n_kv_head, batch, q, ldq, out, ldo, n_head, options, workspace, &a);
+    if (rc != HESA_CUDA_OK) return rc;
     if (workspace_bytes < hesa_cuda_paged_attention_workspace_size(kv, batch, n_head))
         return record_error(HESA_CUDA_INVALID_ARGUMENT, "workspace too small");
-    hesa_cuda_attn_options o{};
-    if (options) o = *options;
-    if (!(o.scale >= 0.f) || !std::isfinite(o.scale) || o.window < 0)
-        return record_error(HESA_CUDA_INVALID_ARGUMENT, "scale and window must be finite and not negative");
-    if (o.softcap != 0.f && !(o.softcap >= 1e-6f && o.softcap <= 1e6f))
-        return record_error(HESA_CUDA_INVALID_ARGUMENT, "softcap must be 0 or 1e-6 .. 1e6");
-    if (!aligned(o.slopes, 4) || !aligned(o.prefix, 4)) return record_error(HESA_CUDA_INVALID_ARGUMENT, "slopes and prefix must be 4-byte aligned");
     if (batch->max_new == 0) return HESA_CUDA_OK;
 
     const Plan p = make_plan(kv, batch, n_head);
-    AttnArgs a{};
     a.c = layer_of(kv, layer);
-    a.b = view_of(batch);
-    a.q = q;
-    a.ldq = ldq;
-    a.out = out;
-    a.ldo = ldo;
-    a.n_head = static_cast<int32_t>(n_head);
-    a.group = static_cast<int32_t>(n_head / kv->n_kv_head);
-    a.group_div = FastDiv(a.group);
-    const double log2e = 1.4426950408889634;
-    const double scale = o.scale > 0.f ? o.scale : 1.0 / std::sqrt(static_cast<double>(kv->head_dim));
-    a.scale2 = static_cast<float>(scale * log2e);
-    a.cap2 = static_cast<float>(o.softcap * log2e);
-    a.cap_in = o.softcap > 0.f ? static_cast<float>(scale / o.softcap) : 0.f;
-    if (!std::isfinite(a.scale2) || !std::isfinite(a.cap_in))
-        return record_error(HESA_CUDA_INVALID_ARGUMENT, "scale is too large for a float, by itself or by softcap");
-    a.window = std::min(o.window, 1 << 30);   // wider than any context; a position less a window stays in 32 bits
-    a.slopes = o.slopes;
-    a.prefix = o.prefix;
-    a.part = static_cast<float*>(workspace);
     a.per_seq = p.per_seq;
     a.blocks_per_split = p.blocks_per_split;
     a.n_split = p.n_split;

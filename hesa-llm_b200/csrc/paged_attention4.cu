@@ -1,0 +1,695 @@
+// paged_attention4.cu -- attention of new tokens over a paged cache in 4 bits.
+//
+// The formulas, rows, tiles, masks and the equal runs of work are those of
+// paged_attention.cu; a value is d (code - 8), an fp16 number exactly.
+//
+// rows4_kernel: tiles of 8 rows, for the next tokens of a decode step. A warp has
+// a kv head of its own and takes blocks of 32 keys of it: their codes and scales
+// come by 16-byte asynchronous copies into a ring of the warp's own (no barrier
+// between warps), a few blocks ahead, also of the next run.
+//   * codes become fp16 pairs in registers, in the places of the operands of
+//     m16n8k16 products: the order of dims within a sum is free, so the thread
+//     that needs keys of column n and dims of quarter c takes 16 consecutive bytes
+//     of key n (head_dim 128: a whole group, one scale), and q is read in that
+//     order. For P V a pair has two keys: one byte permutation of two keys' words
+//     brings them together, and the thread of column n takes head_dim / 8
+//     consecutive dims. Half an instruction a value puts the codes in place, half
+//     one puts them behind the bits of 16, half one is the exact fma by the scale.
+//   * q and P are split into fp16 halves that are the two halves of the A operand
+//     (16 rows), as in paged_attention.cu.
+//   * rows of a warp's block are stored so that eight (or 16, 32) threads read
+//     different banks: see k_at and v_at.
+//
+// Chunks: the tokens of a few sequences at a time are laid out in fp16 in the
+// workspace (values are fp16 numbers, nothing is rounded) as a cache of their own,
+// and the kernel of paged_attention_tc.cu reads that. A chunk's keys are read once
+// for each of its many tiles, so the pass before costs a few percent.
+#include "paged.h"
+#include "paged_rows.cuh"
+#include "paged_tc.h"
+#include "abi_errors.h"
+#include "qmatvec.h"
+#include "trace.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace hesa_cuda {
+namespace {
+
+constexpr int kKeys4 = 32;           // of a block
+constexpr int kSegCost4 = 3;         // blocks that starting a (tile, group) takes the time of
+constexpr int kScratchPage = 128;    // tokens of a page of the fp16 copy
+constexpr int64_t kScratchBytes = int64_t(1) << 30;
+
+// Rows of a sequence above which the chunk kernel takes over.
+constexpr int most_rows4(int head_dim) { return head_dim == 256 ? 48 : 16; }
+
+template <int HD> struct Rows4Shape : RowParts<HD, (HD == 256 ? 8 : 16)> {
+    using RowParts<HD, (HD == 256 ? 8 : 16)>::warps;
+    static constexpr int threads = warps * 32;
+    static constexpr int groups = HD / kGroup;             // of a head: 16-byte pieces of a key's codes
+    static constexpr int row = HD / 2, srow = groups * 2;  // bytes of a key's codes and scales
+    static constexpr int v = kKeys4 * row, ks = 2 * v, vs = ks + kKeys4 * srow;   // K's codes, V's, then the scales
+    static constexpr int stage = vs + kKeys4 * srow;       // a warp's
+    static constexpr int stages = HD == 64 ? 5 : 3;
+    static constexpr size_t smem = static_cast<size_t>(stage) * stages * warps;
+};
+
+// Where piece ch (16 bytes) of key j lies in a block. K: a thread (n, c) of a warp
+// reads quarter c of key n; eight threads side by side cover 128 bytes that differ
+// in their banks: two keys of 64 bytes; of 128-byte rows the lower half of an even
+// key and the upper half of an odd one.
+template <int HD> __device__ __forceinline__ int k_at(int j, int ch) {
+    if constexpr (HD == 256) ch ^= (j & 1) << 2;
+    return j * (HD / 2) + ch * 16;
+}
+// V: thread (n, c) reads dims of column n of keys 2 c and 2 c + 1. Keys 0, 2, 4, 6
+// lie side by side, and pieces change places so that those of the four keys that
+// are read together differ.
+__device__ __forceinline__ int v_row(int j) { return (j & ~7) | ((j & 1) << 2) | ((j >> 1) & 3); }
+template <int HD> __device__ __forceinline__ int v_at(int j, int ch) {
+    const int r = v_row(j);
+    if constexpr (HD == 128) ch ^= r & 2;
+    if constexpr (HD == 256) ch ^= (r & 3) << 1;
+    return r * (HD / 2) + ch * 16;
+}
+
+// BYTES (4, 8 or 16) from global to shared memory, zeros where !ok
+template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool ok) {
+    const int n = ok ? BYTES : 0;
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// A warp's way through its blocks of the CTA's run, ahead of the products.
+struct Ahead {
+    int64_t u, end;
+    int lo, i, i1, kvh;
+    int32_t len;
+    const int32_t* table;
+    KeyBlocks kb;
+    int32_t page;   // of key `lane` of block i; -1: none
+    bool any;       // there is a block i
+};
+
+__device__ __forceinline__ int32_t page_of(const AttnArgs& A, const Ahead& h) {
+    const int32_t j = h.kb.at(h.i) * kKeys4 + (threadIdx.x & 31);
+    return j < h.len ? h.table[A.c.page_div.div(j)] : -1;
+}
+
+// The next segment with a block for this warp, if i has come to the end of one.
+__device__ __forceinline__ void go_on(const AttnArgs& A, const HeadGroups& hg, const int64_t* pre, int sub, int hl, Ahead& h) {
+    while (h.i >= h.i1) {
+        Segment seg;
+        if (!next_segment(pre, hg, h.u, h.end, h.lo, seg)) {
+            h.any = false;
+            return;
+        }
+        h.kvh = seg.grp * hg.heads + hl;
+        if (h.kvh >= A.c.n_kv) continue;
+        const TileView tv = tile_view<kKeys4>(A, seg.tile);
+        h.i = seg.b0 + sub;
+        h.i1 = min(tv.kb.n, seg.b1);
+        h.len = tv.sv.len;
+        h.table = A.c.table + static_cast<int64_t>(tv.sv.slot) * A.c.max_pages;
+        h.kb = tv.kb;
+    }
+    h.page = page_of(A, h);
+}
+
+// Block h.i into a stage, and h to the block after it. One group of copies, empty where there is none.
+template <int HD>
+__device__ __forceinline__ void copy_block(const AttnArgs& A, const Pools4& pools, const HeadGroups& hg, const int64_t* pre, int sub, int hl, uint32_t stage,
+                                           Ahead& h) {
+    using S = Rows4Shape<HD>;
+    if (h.any) {
+        const int lane = threadIdx.x & 31;
+        const int32_t j = h.kb.at(h.i) * kKeys4 + lane;
+        const bool good = h.page >= 0 && h.page < A.c.n_pages;
+        if (!good && j < h.len) record_status(A.status, kStatusBadPosition);
+        // of this lane's key
+        const int64_t at = good ? h.page * A.c.page_stride + static_cast<int64_t>((j - A.c.page_div.div(j) * A.c.page_size) * A.c.n_kv + h.kvh) * S::groups : -1;
+        const int64_t from = good ? at : 0;
+        copy_async<S::srow>(stage + S::ks + lane * S::srow, pools.ks + from, good);
+        copy_async<S::srow>(stage + S::vs + lane * S::srow, pools.vs + from, good);
+        const int ch = lane % S::groups;
+#pragma unroll
+        for (int x = 0; x < S::groups; ++x) {
+            const int key = lane / S::groups + x * (32 / S::groups);
+            const int64_t a = __shfl_sync(0xffffffffu, at, key);
+            copy_async<16>(stage + k_at<HD>(key, ch), pools.k + (a >= 0 ? a + ch : 0), a >= 0);
+            copy_async<16>(stage + S::v + v_at<HD>(key, ch), pools.v + (a >= 0 ? a + ch : 0), a >= 0);
+        }
+        h.i += hg.subs;
+        if (h.i < h.i1) h.page = page_of(A, h);
+        else go_on(A, hg, pre, sub, hl, h);
+    }
+    copy_commit();
+}
+
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+    uint32_t v;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+    uint2 v;
+    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t a) {
+    unsigned short v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
+
+// This warp's head's attention over its blocks of a segment. part < 0: they are
+// all that the rows see, and the result goes to out; else (m, l, acc) go to that
+// part. `at`: stages used so far.
+template <int HD>
+__device__ __forceinline__ void rows4_segment(const AttnArgs& A, const Pools4& pools, const HeadGroups& hg, const int64_t* pre, uint8_t* ring, Ahead& ahead,
+                                              uint32_t& at, const Segment& seg, const TileView& tv, int part) {
+    using S = Rows4Shape<HD>;
+    constexpr int KW = HD / 32;                  // words of codes of a key's quarter: two k-steps of Q K^T each
+    constexpr int VW = HD / 64;                  // words of codes of a column's dims
+    constexpr int NT = HD / 8;                   // column tiles of P V
+    constexpr int KT = kKeys4 / 8;               // column tiles of Q K^T
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = lane >> 2, c = lane & 3;
+    const int sub = hg.sub_of(warp), hl = warp - sub * hg.heads, kvh = seg.grp * hg.heads + hl;
+    const SeqView& sv = tv.sv;
+    const Mask& mask = tv.mask;
+    if (sub >= hg.subs || kvh >= A.c.n_kv) return;
+
+    // this thread's row and position
+    const int r = tv.r0 + n;
+    const bool row_ok = r < tv.n_rows;
+    const int rc = min(r, tv.n_rows - 1), t = A.group_div.div(rc), h = kvh * A.group + rc - t * A.group;
+    const int32_t pos = tv.base + t;
+    const RowKeys keys = mask.row(pos);
+    const int i1 = min(tv.kb.n, seg.b1);
+
+    // ---- q as hi and lo halves of q * 2^-e, max |q| 2^-e in [2^14, 2^15), in the order of the codes' pairs ----
+    uint32_t qa[2 * KW][4];
+    float qscale;   // 2^e; NaN for a row that is not finite
+    {
+        const float* q = A.q + static_cast<int64_t>(sv.q0 + t) * A.ldq + static_cast<int64_t>(h) * HD;
+        float v[KW][8];
+        float mx = 0.f;
+#pragma unroll
+        for (int w = 0; w < KW; ++w) {
+            const int d = HD == 256 ? 32 * (c + (w & 4)) + 8 * (w & 3) : (HD / 4) * c + 8 * w;
+#pragma unroll
+            for (int i = 0; i < 8; i += 4)
+                *reinterpret_cast<float4*>(v[w] + i) = row_ok ? *reinterpret_cast<const float4*>(q + d + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) mx = fmax_nan(mx, fabsf(v[w][i]));
+        }
+        mx = fmax_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmax_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const bool fin = mx < INFINITY;
+        int e = 0;
+        if (fin && mx > 0.f) e = ilogbf(mx) - 14;
+        // two factors, so that 2^-e stays finite for the smallest subnormal q
+        const float f1 = ldexpf(1.f, -(e / 2)), f2 = fin ? ldexpf(1.f, -(e - e / 2)) : 0.f;
+        qscale = fin ? ldexpf(1.f, e) : NAN;
+#pragma unroll
+        for (int w = 0; w < KW; ++w)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = fin ? v[w][i] * f1 * f2 : 0.f, y = fin ? v[w][i + 4] * f1 * f2 : 0.f;
+                split_half2(x, y, qa[2 * w + (i >> 1)][2 * (i & 1)], qa[2 * w + (i >> 1)][2 * (i & 1) + 1]);
+            }
+    }
+    const float sc = A.cap2 != 0.f ? qscale : qscale * A.scale2;
+    const float slope2 = A.slopes ? A.slopes[h] * 1.44269504088896341f : 0.f;
+
+    float m = -INFINITY, l = 0.f;
+    float acc[NT][2];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = 0.f;
+    const int vg = n * HD / 256;   // the group of this thread's column's dims
+
+    for (int i = seg.b0 + sub; i < i1; i += hg.subs, ++at) {
+        copy_wait<S::stages - 2>();
+        __syncwarp();   // the block has landed for every lane, and the one before it has been read
+        const uint32_t base = smem_addr(ring);
+        copy_block<HD>(A, pools, hg, pre, sub, hl, base + (at + S::stages - 1) % S::stages * S::stage, ahead);
+        const uint32_t st = base + at % S::stages * S::stage;
+        const int32_t j0 = tv.kb.at(i) * kKeys4;
+
+        // ---- scores of keys 8 t + 2 c, + 1 ----
+        float s[KT][4];
+#pragma unroll
+        for (int x = 0; x < KT; ++x) s[x][0] = s[x][1] = s[x][2] = s[x][3] = 0.f;
+#pragma unroll
+        for (int x = 0; x < KT; ++x) {
+            const int key = 8 * x + n;
+#pragma unroll
+            for (int p = 0; p < (HD == 256 ? 2 : 1); ++p) {
+                uint32_t w[4];
+                if constexpr (HD == 64) {
+                    const uint2 y = lds64(st + k_at<HD>(key, 0) + c * 8);
+                    w[0] = y.x;
+                    w[1] = y.y;
+                } else {
+                    const uint4 y = lds128(st + k_at<HD>(key, c + 4 * p));
+                    w[0] = y.x;
+                    w[1] = y.y;
+                    w[2] = y.z;
+                    w[3] = y.w;
+                }
+                const uint32_t d16 = lds16(st + S::ks + key * S::srow + (HD == 64 ? c >> 1 : c + 4 * p) * 2);
+                const __half2 d = as_half2(d16 | d16 << 16), dm = __hmul2(d, __float2half2_rn(-24.f));
+#pragma unroll
+                for (int y = 0; y < (HD == 64 ? 2 : 4); ++y) {
+                    uint32_t b[4];
+                    code_pairs(w[y], d, dm, b);
+                    mma16816(s[x], qa[2 * (4 * p + y)], b[0], b[1]);
+                    mma16816(s[x], qa[2 * (4 * p + y) + 1], b[2], b[3]);
+                }
+            }
+        }
+        float sx[KT][2];
+#pragma unroll
+        for (int x = 0; x < KT; ++x)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                sx[x][k] = (s[x][k] + s[x][k + 2]) * sc;
+                if (A.cap2 != 0.f) sx[x][k] = capped(sx[x][k], A.cap2, A.cap_in);
+            }
+        const int32_t jc = j0 + 2 * c;   // this thread's keys: jc + 8 x + k
+        if (A.slopes) {
+#pragma unroll
+            for (int x = 0; x < KT; ++x)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) sx[x][k] -= slope2 * fabsf(static_cast<float>(pos - (jc + 8 * x + k)));
+        }
+        if (!mask.all(tv.p_lo, tv.p_hi, j0, j0 + kKeys4)) {
+#pragma unroll
+            for (int x = 0; x < KT; ++x)
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    if (!keys.sees(jc + 8 * x + k)) sx[x][k] = -INFINITY;
+            // A key that some row does not see has P = 0 there, which would make NaN of a
+            // scale that is not finite. Such groups (there are none in a sound cache) are
+            // added where they are seen and then cleared, so that they reach no other row.
+            uint32_t odd = 0;
+#pragma unroll
+            for (int x = 0; x < S::srow / 4; ++x) odd |= nonfinite_mark(lds32(st + S::vs + lane * S::srow + 4 * x));
+            if (__any_sync(0xffffffffu, (odd & kNonfinite) != 0)) {
+                __half* vs = reinterpret_cast<__half*>(ring + at % S::stages * S::stage + S::vs);
+                for (int j = 0; j < kKeys4; ++j) {
+                    if (!keys.sees(j0 + j)) continue;
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)   // the columns 2 c + k of this thread's sums
+                        if (!isfinite(__half2float(vs[j * S::groups + (2 * c + k) * HD / 256]))) {
+#pragma unroll
+                            for (int x = 0; x < NT; ++x) acc[x][k] = NAN;
+                        }
+                }
+                __syncwarp();
+                for (int x = lane; x < kKeys4 * S::groups; x += 32)
+                    if (!isfinite(__half2float(vs[x]))) vs[x] = __float2half_rn(0.f);
+                __syncwarp();
+            }
+        }
+        float mx = m;
+#pragma unroll
+        for (int x = 0; x < KT; ++x) mx = fmaxf(mx, fmaxf(sx[x][0], sx[x][1]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float ms = mx == -INFINITY ? 0.f : mx;   // nothing seen yet: P = 2^-inf = 0
+        const float corr = m == -INFINITY ? 0.f : ex2(m - ms);
+        m = mx;
+        uint32_t pa[KT / 2][4];
+        float sum = 0.f;
+#pragma unroll
+        for (int x = 0; x < KT; ++x) {
+            const float p0 = ex2(sx[x][0] - ms + kPShift), p1 = ex2(sx[x][1] - ms + kPShift);
+            sum += p0 + p1;
+            split_half2(p0, p1, pa[x >> 1][2 * (x & 1)], pa[x >> 1][2 * (x & 1) + 1]);
+        }
+        l = fmaf(l, corr, sum);
+
+        // ---- P V: keys 2 c, + 1, + 8, + 9 of each 16, dims of column n ----
+        uint32_t vw[kKeys4 / 4][VW];   // [k-step, + 8, second of the pair]
+        __half2 vd[KT], vm[KT];
+#pragma unroll
+        for (int x = 0; x < KT; ++x) {
+            uint32_t d16[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int key = 8 * x + 2 * c + k;
+                if constexpr (HD == 64) vw[2 * x + k][0] = lds32(st + S::v + v_at<HD>(key, n >> 2) + (n & 3) * 4);
+                if constexpr (HD == 128) {
+                    const uint2 y = lds64(st + S::v + v_at<HD>(key, n >> 1) + (n & 1) * 8);
+                    vw[2 * x + k][0] = y.x;
+                    vw[2 * x + k][1] = y.y;
+                }
+                if constexpr (HD == 256) {
+                    const uint4 y = lds128(st + S::v + v_at<HD>(key, n));
+                    vw[2 * x + k][0] = y.x;
+                    vw[2 * x + k][1] = y.y;
+                    vw[2 * x + k][2] = y.z;
+                    vw[2 * x + k][3] = y.w;
+                }
+                d16[k] = lds16(st + S::vs + key * S::srow + vg * 2);
+            }
+            vd[x] = as_half2(d16[0] | d16[1] << 16);
+            vm[x] = __hmul2(vd[x], __float2half2_rn(-24.f));
+        }
+#pragma unroll
+        for (int y = 0; y < 2 * VW; ++y) {   // four dims of the column
+            float o[4][4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k][0] = o[k][1] = o[k][2] = o[k][3] = 0.f;
+#pragma unroll
+            for (int x = 0; x < KT; x += 2) {
+                uint32_t b0[4], b1[4];
+                code_pairs(prmt(vw[2 * x][y >> 1], vw[2 * x + 1][y >> 1], (y & 1) ? 0x7632u : 0x5410u), vd[x], vm[x], b0);
+                code_pairs(prmt(vw[2 * x + 2][y >> 1], vw[2 * x + 3][y >> 1], (y & 1) ? 0x7632u : 0x5410u), vd[x + 1], vm[x + 1], b1);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) mma16816(o[k], pa[x >> 1], b0[k], b1[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                acc[4 * y + k][0] = fmaf(acc[4 * y + k][0], corr, o[k][0] + o[k][2]);
+                acc[4 * y + k][1] = fmaf(acc[4 * y + k][1], corr, o[k][1] + o[k][3]);
+            }
+        }
+    }
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if (!row_ok) return;
+    float* o;
+    float inv = 1.f;
+    if (part < 0) {
+        o = A.out + static_cast<int64_t>(sv.q0 + t) * A.ldo + static_cast<int64_t>(h) * HD;
+        inv = l == 0.f ? 0.f : 1.f / l;   // nothing seen: zeros
+    } else {
+        const int64_t at_row = (static_cast<int64_t>(part) * S::warps + warp) * kRowTile + n;
+        float* ml = A.part + S::cut_bytes / 4;
+        if (c == 0) *reinterpret_cast<float2*>(ml + at_row * 2) = make_float2(m, l);
+        o = ml + S::part_rows(part_count(A.n_split, hg)) * 2 + at_row * HD;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int x = 0; x < NT; x += 4)
+            *reinterpret_cast<float4*>(o + (2 * c + k) * NT + x) = make_float4(acc[x][k] * inv, acc[x + 1][k] * inv, acc[x + 2][k] * inv, acc[x + 3][k] * inv);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(Rows4Shape<HD>::threads, 1)
+rows4_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ Pools4 pools, const __grid_constant__ HeadGroups hg) {
+    using S = Rows4Shape<HD>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int64_t s_pre[kMostTiles + 1];
+    __shared__ int64_t s_sum[S::warps];
+    const int warp = threadIdx.x >> 5, tiles = A.n_split, cta = blockIdx.x;
+    if (threadIdx.x == 0) s_pre[0] = 0;
+    grid_dep_wait();
+    grid_dep_launch();   // combine_kernel may be set up meanwhile; it waits for this grid's end
+    const int64_t units = tile_units<S::warps, kKeys4>(A, hg, tiles, s_pre, s_sum) * hg.groups;
+    const Runs runs(units, gridDim.x);
+    const bool listed_by_tile = by_tile(tiles, hg);
+    Cut* cuts = reinterpret_cast<Cut*>(A.part);
+    int64_t u = 0, end = 0;
+    if (units > 0 && cta < runs.n_cta) {
+        u = runs.start(cta);
+        end = runs.start(cta + 1);
+    }
+    const int64_t begin = u;
+    int lo = tile_at(s_pre, hg, tiles, u);
+    if (listed_by_tile && cta == 0)   // those without rows
+        for (int i = threadIdx.x; i < tiles * hg.groups; i += S::threads)
+            if (s_pre[i / hg.groups + 1] == s_pre[i / hg.groups]) cuts[i] = Cut{};
+
+    const int sub = hg.sub_of(warp), hl = warp - sub * hg.heads;
+    uint8_t* ring = smem + static_cast<size_t>(warp) * S::stage * S::stages;
+    Ahead ahead{};
+    ahead.u = u;
+    ahead.end = end;
+    ahead.lo = lo;
+    ahead.any = sub < hg.subs;
+    if (ahead.any) go_on(A, hg, s_pre, sub, hl, ahead);
+    for (int i = 0; i < S::stages - 1; ++i) copy_block<HD>(A, pools, hg, s_pre, sub, hl, smem_addr(ring) + i * S::stage, ahead);
+
+    uint32_t at = 0;
+    Segment seg;
+    Cut cut{};
+    while (next_segment(s_pre, hg, u, end, lo, seg)) {
+        const int c_first = runs.cta_of(seg.first + hg.cost), c_last = runs.cta_of(seg.first + seg.units - 1);
+        const bool uncut = c_first == c_last;
+        const int own_part = 2 * kRowsCtas + seg.tile * hg.groups + seg.grp;   // of what several warps share, uncut
+        const TileView tv = tile_view<kKeys4>(A, seg.tile);
+        const Cut all{seg.grp, uncut ? own_part : 2 * c_first + (runs.start(c_first) >= seg.first ? 0 : 1), c_last - c_first + 1,
+                      min(kRowTile, tv.n_rows - tv.r0), tv.r0, tv.sv.q0};
+        if (cta == c_first + 1) cut = all;
+        if (listed_by_tile && cta == c_first && threadIdx.x == 0) cuts[seg.tile * hg.groups + seg.grp] = all;
+        rows4_segment<HD>(A, pools, hg, s_pre, ring, ahead, at, seg, tv, !uncut ? 2 * cta + (begin >= seg.first ? 0 : 1) : hg.subs > 1 ? own_part : -1);
+    }
+    if (!listed_by_tile && threadIdx.x == 0) cuts[cta] = cut;
+    copy_wait<0>();   // nothing may be in flight when the CTA ends
+}
+
+// ---- chunks: a cache of fp16 pages, sequence i in slot i ----
+
+struct Scratch {
+    __half* k;
+    __half* v;
+    int32_t* table;     // [n_seq][pages]: page i * pages + x of slot i
+    int32_t* seq_len;   // -1 for a sequence that is not sound
+    int32_t pages;
+};
+
+// A block writes kScratchPage tokens of one sequence, those that its rows see, and
+// their entry of the table. A warp takes a token's row: a lane four codes' words of
+// K, then of V.
+__global__ void __launch_bounds__(256)
+expand_kernel(const AttnArgs A, const Pools4 pools, const Scratch w) {
+    grid_dep_wait();
+    grid_dep_launch();
+    const int seq = blockIdx.y, x = blockIdx.x;
+    const SeqView sv = seq_view(A.c, A.b, seq);
+    if (threadIdx.x == 0) {
+        w.table[static_cast<int64_t>(seq) * w.pages + x] = seq * w.pages + x;
+        if (x == 0) w.seq_len[seq] = sv.ok ? sv.len : -1;
+    }
+    if (!sv.ok || sv.n_new == 0) return;
+    const int32_t prefix = A.prefix ? max(0, min(A.prefix[seq], sv.len)) : 0;
+    const int32_t first = A.window > 0 ? max(0, sv.len - sv.n_new + 1 - A.window) : 0;   // the first key in a window
+    const int row_words = A.c.n_kv * A.c.head_dim / 8, lane = threadIdx.x & 31;
+    const int32_t* table = A.c.table + static_cast<int64_t>(sv.slot) * A.c.max_pages;
+    const int32_t j1 = min((x + 1) * kScratchPage, sv.len);
+    for (int32_t j = x * kScratchPage + (threadIdx.x >> 5); j < j1; j += 8) {
+        if (j < first && j >= prefix) continue;
+        const int32_t pi = A.c.page_div.div(j), page = table[pi];
+        const bool good = page >= 0 && page < A.c.n_pages;
+        if (!good && lane == 0) record_status(A.status, kStatusBadPosition);
+        const int64_t from = good ? page * A.c.page_stride + static_cast<int64_t>(j - pi * A.c.page_size) * (row_words / 4) : 0;
+        const int64_t to = (static_cast<int64_t>(seq) * w.pages * kScratchPage + j) * row_words;
+        for (int u = lane; u < 2 * row_words; u += 32) {
+            const bool is_k = u < row_words;
+            const int at = is_k ? u : u - row_words;
+            uint32_t b[4] = {0u, 0u, 0u, 0u};
+            if (good) {
+                const uint32_t code = reinterpret_cast<const uint32_t*>((is_k ? pools.k : pools.v) + from)[at];
+                const __half2 d = __half2half2(((is_k ? pools.ks : pools.vs) + from)[at / 4]);
+                uint32_t p[4];
+                code_pairs(code, d, __hmul2(d, __float2half2_rn(-24.f)), p);   // (0, 4) (1, 5) (2, 6) (3, 7)
+                b[0] = prmt(p[0], p[1], 0x5410u);
+                b[1] = prmt(p[2], p[3], 0x5410u);
+                b[2] = prmt(p[0], p[1], 0x7632u);
+                b[3] = prmt(p[2], p[3], 0x7632u);
+            }
+            reinterpret_cast<uint4*>(is_k ? w.k : w.v)[to + at] = make_uint4(b[0], b[1], b[2], b[3]);
+        }
+    }
+}
+
+struct Plan4 {
+    bool chunk;
+    int heads, per_seq, tiles;   // rows4_kernel
+    int n_seq, pages;            // chunk: sequences at a time, pages of each
+};
+
+int warps4(int head_dim) { return head_dim == 256 ? Rows4Shape<256>::warps : Rows4Shape<128>::warps; }
+
+// How a call is cut: from the host's bounds alone, so that a captured graph
+// serves every later length within them.
+Plan4 make_plan4(const hesa_cuda_paged_kv4* kv, const hesa_cuda_token_batch* b, int64_t n_head) {
+    Plan4 p{};
+    const int g = static_cast<int>(n_head / kv->n_kv_head);
+    const int64_t rows_a_seq = static_cast<int64_t>(b->max_new) * g;
+    p.chunk = rows_a_seq > most_rows4(kv->head_dim);
+    if (p.chunk) {
+        p.pages = std::max(1, (b->max_len + kScratchPage - 1) / kScratchPage);
+        const int64_t bytes = static_cast<int64_t>(p.pages) * kScratchPage * kv->n_kv_head * kv->head_dim * 4;
+        p.n_seq = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(b->n_seq, kScratchBytes / bytes)));
+        return p;
+    }
+    const int64_t most = (rows_a_seq + kRowTile - 1) / kRowTile;
+    const int64_t bound = tile_bound(b->n_tokens, b->n_seq, g, kRowTile);
+    p.per_seq = b->n_seq * most <= bound ? static_cast<int>(most) : 0;
+    const int64_t tiles = p.per_seq ? b->n_seq * most : bound;
+    p.tiles = static_cast<int>(tiles);
+    const int64_t blocks = std::max<int64_t>(1, (b->max_len + kKeys4 - 1) / kKeys4);
+    static_assert(4 * kRowsCtas <= kMostTiles, "a list for every (tile, group) where groups are made smaller");
+    p.heads = warps4(kv->head_dim);
+    while (p.heads > 2 && tiles * ((kv->n_kv_head + p.heads - 1) / p.heads) * blocks < 2 * kRowsCtas) p.heads /= 2;
+    return p;
+}
+
+size_t round16(size_t n) { return (n + 15) & ~static_cast<size_t>(15); }
+
+// The chunk's scratch in the workspace: pools, table, lengths, then the chunk kernel's own.
+struct ScratchSizes {
+    size_t pool, table, len;
+    size_t all() const { return 2 * pool + table + len; }
+};
+ScratchSizes scratch_sizes(const hesa_cuda_paged_kv4* kv, const Plan4& p) {
+    const size_t pages = static_cast<size_t>(p.n_seq) * p.pages;
+    return {pages * kScratchPage * kv->n_kv_head * kv->head_dim * 2, round16(pages * 4), round16(static_cast<size_t>(p.n_seq) * 4)};
+}
+hesa_cuda_paged_kv scratch_kv(const hesa_cuda_paged_kv4* kv, const Plan4& p, uint8_t* ws) {
+    const ScratchSizes z = scratch_sizes(kv, p);
+    hesa_cuda_paged_kv s{};
+    s.k = ws;
+    s.v = ws + z.pool;
+    s.table = reinterpret_cast<int32_t*>(ws + 2 * z.pool);
+    s.seq_len = reinterpret_cast<int32_t*>(ws + 2 * z.pool + z.table);
+    s.page_stride = static_cast<int64_t>(kScratchPage) * kv->n_kv_head * kv->head_dim;
+    s.n_layer = 1;
+    s.n_pages = p.n_seq * p.pages;
+    s.page_size = kScratchPage;
+    s.n_kv_head = kv->n_kv_head;
+    s.head_dim = kv->head_dim;
+    s.n_slots = p.n_seq;
+    s.max_pages = p.pages;
+    return s;
+}
+
+size_t rows4_bytes(const Plan4& p, const hesa_cuda_paged_kv4* kv) {
+    const HeadGroups hg(kv->n_kv_head, warps4(kv->head_dim), p.heads, kSegCost4);
+    const int64_t parts = part_count(std::min(p.tiles, kMostTiles), hg);
+    return kv->head_dim == 64 ? Rows4Shape<64>::bytes(parts) : kv->head_dim == 128 ? Rows4Shape<128>::bytes(parts) : Rows4Shape<256>::bytes(parts);
+}
+
+template <int HD>
+cudaError_t launch_rows4(AttnArgs a, const Pools4& pools, const Plan4& p, cudaStream_t s) {
+    static bool set[64] = {};   // per instance and device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    using S = Rows4Shape<HD>;
+    if (!set[dev]) {
+        e = cudaFuncSetAttribute(rows4_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::smem));
+        if (e != cudaSuccess) return e;
+        set[dev] = true;
+    }
+    const HeadGroups hg(a.c.n_kv, S::warps, p.heads, kSegCost4);
+    for (a.tile0 = 0; a.tile0 < p.tiles && e == cudaSuccess; a.tile0 += kMostTiles) {
+        a.n_split = std::min(kMostTiles, p.tiles - a.tile0);
+        e = launch_dep(rows4_kernel<HD>, dim3(kRowsCtas), S::threads, S::smem, s, a, pools, hg);
+        const int cuts = by_tile(a.n_split, hg) ? a.n_split * hg.groups : kRowsCtas;
+        const int rows = std::min(kRowTile, a.b.max_new * a.group);
+        const unsigned z = static_cast<int64_t>(cuts) * hg.heads * rows <= 8 * kRowsCtas ? rows : 1;
+        if (e == cudaSuccess)
+            e = launch_dep(combine_kernel<HD, S::warps>, dim3(static_cast<unsigned>(cuts), static_cast<unsigned>(hg.heads), z), 256, 0, s, a, hg);
+    }
+    return e;
+}
+
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+}  // namespace
+}  // namespace hesa_cuda
+
+using namespace hesa_cuda;
+
+extern "C" {
+
+size_t hesa_cuda_paged_attention_kv4_workspace_size(const hesa_cuda_paged_kv4* kv, const hesa_cuda_token_batch* batch, int64_t n_head) {
+    if (check_paged_kv4(kv) != HESA_CUDA_OK || check_batch4(kv, 0, batch, n_head) != HESA_CUDA_OK) return 0;
+    const Plan4 p = make_plan4(kv, batch, n_head);
+    if (!p.chunk) return std::max<size_t>(rows4_bytes(p, kv), 16);
+    const hesa_cuda_paged_kv s = scratch_kv(kv, p, reinterpret_cast<uint8_t*>(uintptr_t(16)));   // not looked into
+    hesa_cuda_token_batch b = *batch;
+    b.n_seq = p.n_seq;
+    b.slots = nullptr;
+    const size_t inner = hesa_cuda_paged_attention_workspace_size(&s, &b, n_head);
+    return inner ? scratch_sizes(kv, p).all() + inner : 0;
+}
+
+int hesa_cuda_paged_attention_kv4(const hesa_cuda_paged_kv4* kv, int32_t layer, const hesa_cuda_token_batch* batch, const float* q,
+                                  int64_t ldq, float* out, int64_t ldo, int64_t n_head, const hesa_cuda_attn_options* options,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+    HESA_TRACE("hesa_cuda_paged_attention_kv4");
+    int rc = check_paged_kv4(kv);
+    if (rc == HESA_CUDA_OK) rc = check_batch4(kv, layer, batch, n_head);
+    if (rc != HESA_CUDA_OK) return rc;
+    if (batch->n_tokens == 0) return HESA_CUDA_OK;   // no rows: their buffers may be null
+    hesa_cuda_attn_options o{};
+    if (options) o = *options;
+    AttnArgs a{};
+    rc = attention_args(kv->head_dim, kv->n_kv_head, batch, q, ldq, out, ldo, n_head, options, workspace, &a);
+    if (rc != HESA_CUDA_OK) return rc;
+    const size_t need = hesa_cuda_paged_attention_kv4_workspace_size(kv, batch, n_head);
+    if (need == 0) return HESA_CUDA_SHAPE_MISMATCH;   // a chunk's copy that would be no cache; the message is there
+    if (workspace_bytes < need) return record_error(HESA_CUDA_INVALID_ARGUMENT, "workspace too small");
+    if (batch->max_new == 0) return HESA_CUDA_OK;
+
+    const Plan4 p = make_plan4(kv, batch, n_head);
+    const Pools4 pools = pools_of(kv, layer);
+    a.c = layer_of4(kv);
+    a.per_seq = p.per_seq;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    cudaError_t e = status_word(&a.status);
+    if (e == cudaSuccess && p.chunk) {
+        uint8_t* ws = static_cast<uint8_t*>(workspace);
+        hesa_cuda_paged_kv c = scratch_kv(kv, p, ws);
+        const size_t used = scratch_sizes(kv, p).all();
+        hesa_cuda_token_batch b = *batch;
+        b.slots = nullptr;
+        for (int i = 0; i < batch->n_seq; i += p.n_seq) {
+            b.n_seq = std::min(p.n_seq, batch->n_seq - i);
+            b.q_start = batch->q_start + i;
+            a.b.n_seq = b.n_seq;
+            a.b.q_start = b.q_start;
+            a.b.slots = batch->slots ? batch->slots + i : nullptr;
+            PagedLayer& l = a.c;
+            if (!batch->slots) {   // sequence i is in slot i
+                l.table = kv->table + static_cast<int64_t>(i) * kv->max_pages;
+                l.seq_len = kv->seq_len + i;
+                l.n_slots = kv->n_slots - i;
+            }
+            o.prefix = options && options->prefix ? options->prefix + i : nullptr;
+            a.prefix = o.prefix;
+            e = launch_dep(expand_kernel, dim3(static_cast<unsigned>(p.pages), static_cast<unsigned>(b.n_seq)), 256, 0, s, a, pools,
+                           Scratch{static_cast<__half*>(c.k), static_cast<__half*>(c.v), c.table, c.seq_len, p.pages});
+            if (e != cudaSuccess) break;
+            rc = hesa_cuda_paged_attention(&c, 0, &b, q, ldq, out, ldo, n_head, &o, ws + used, workspace_bytes - used, stream);
+            if (rc != HESA_CUDA_OK) return rc;
+        }
+    } else if (e == cudaSuccess) {
+        switch (kv->head_dim) {
+            case 64: e = launch_rows4<64>(a, pools, p, s); break;
+            case 128: e = launch_rows4<128>(a, pools, p, s); break;
+            default: e = launch_rows4<256>(a, pools, p, s); break;
+        }
+    }
+    return e == cudaSuccess ? HESA_CUDA_OK : record_cuda_error(e, "paged attention kernel");
+}
+
+}  // extern "C"

@@ -53,6 +53,11 @@ class PagedKVStruct(ctypes.Structure):
                 ("n_slots", ctypes.c_int32), ("max_pages", ctypes.c_int32)]
 
 
+class PagedKV4Struct(ctypes.Structure):
+    """hesa_cuda_paged_kv4 (include/hesa_cuda.h)."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + PagedKVStruct._fields_[2:]
+
+
 class TokenBatchStruct(ctypes.Structure):
     """hesa_cuda_token_batch (include/hesa_cuda.h)."""
     _fields_ = [("slots", ctypes.c_void_p), ("q_start", ctypes.c_void_p), ("n_seq", ctypes.c_int32),
@@ -66,9 +71,24 @@ class AttnOptionsStruct(ctypes.Structure):
 
 
 _kvp, _batchp, _optp = ctypes.POINTER(PagedKVStruct), ctypes.POINTER(TokenBatchStruct), ctypes.POINTER(AttnOptionsStruct)
+_kv4p = ctypes.POINTER(PagedKV4Struct)
 _i32 = ctypes.c_int32
 
 SIGNATURES = [
+    ("hesa_cuda_kv_reorder", _int, [_kvp, _vp, _vp, _i32, _i32, _vp, _sz, _vp]),
+    ("hesa_cuda_paged_attention_kv4_workspace_size", _sz, [_kv4p, _batchp, _i64]),
+    ("hesa_cuda_paged_attention_kv4", _int, [_kv4p, _i32, _batchp, _vp, _i64, _vp, _i64, _i64, _optp, _vp, _sz, _vp]),
+    ("hesa_cuda_rope_kv4_paged", _int, [_kv4p, _i32, _batchp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i32, _vp]),
+    ("hesa_cuda_kv4_read", _int, [_kv4p, _i32, _batchp, _vp, _i64, _vp, _i64, _vp]),
+    ("hesa_cuda_kv4_pages_workspace_size", _sz, [_kv4p]),
+    ("hesa_cuda_kv4_reserve", _int, [_kv4p, _vp, _vp, _i32, _vp, _sz, _vp]),
+    ("hesa_cuda_kv4_free", _int, [_kv4p, _vp, _i32, _vp, _sz, _vp]),
+    ("hesa_cuda_kv4_fork", _int, [_kv4p, _vp, _vp, _i32, _vp, _sz, _vp]),
+    ("hesa_cuda_kv4_compact", _int, [_kv4p, _vp, _vp, _sz, _vp]),
+    ("hesa_cuda_kv4_copy_pages", _int, [_kv4p, _vp, _vp, _i32, _vp, _sz, _vp]),
+    ("hesa_cuda_kv4_reorder", _int, [_kv4p, _vp, _vp, _i32, _i32, _vp, _sz, _vp]),
+    ("hesa_cuda_beam_select_workspace_size", _sz, [_i64, _i32, _i64]),
+    ("hesa_cuda_beam_select", _int, [_vp, _i64, _i64, _i32, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     ("hesa_cuda_paged_attention_workspace_size", _sz, [_kvp, _batchp, _i64]),
     ("hesa_cuda_paged_attention", _int, [_kvp, _i32, _batchp, _vp, _i64, _vp, _i64, _i64, _optp, _vp, _sz, _vp]),
     ("hesa_cuda_rope_kv_paged", _int, [_kvp, _i32, _batchp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i32, _vp]),
@@ -579,6 +599,10 @@ class PagedKV:
     operations for each stream that they ran on; everything lies on one CUDA
     device."""
 
+    # the library's functions for a cache of this kind
+    calls = {n: f"hesa_cuda_{n}" for n in ("paged_attention", "paged_attention_workspace_size", "rope_kv_paged", "kv_pages_workspace_size",
+                                           "kv_reserve", "kv_free", "kv_fork", "kv_compact", "kv_copy_pages", "kv_reorder")}
+
     def __init__(self, k, v, table, seq_len, page_refs=None):
         import torch
         _want(k, torch.float16, "k", dims=5)
@@ -591,17 +615,25 @@ class PagedKV:
             raise ValueError("k and v must have the same shape and strides")
         if strides[2:] != (n_kv * hd, hd, 1):
             raise ValueError("places, heads and dims of a page must be contiguous")
+        self.k, self.v = k, v
+        self._tables(dev, n_layer, n_pages, page, n_kv, hd, table, seq_len, page_refs)
+        self._struct(PagedKVStruct(k.data_ptr(), v.data_ptr(), strides[1], strides[0], n_layer, n_pages, page, n_kv, hd,
+                                   table.data_ptr(), seq_len.data_ptr(), _ptr(page_refs), table.shape[0], table.shape[1]))
+
+    def _tables(self, dev, n_layer, n_pages, page, n_kv, hd, table, seq_len, page_refs):
+        """The checks of the tables, and what every cache keeps."""
         if not table.is_contiguous():
             raise ValueError("table must be contiguous")
         _ints(seq_len, "seq_len", table.shape[0], dev)
         if page_refs is not None:
             _ints(page_refs, "page_refs", n_pages, dev)
         self.device, self.n_slots, self.n_pages, self.n_kv_head, self.head_dim = dev, table.shape[0], n_pages, n_kv, hd
-        self.k, self.v, self.table, self.seq_len, self.page_refs = k, v, table, seq_len, page_refs
-        self.struct = PagedKVStruct(k.data_ptr(), v.data_ptr(), strides[1], strides[0], n_layer, n_pages, page, n_kv, hd,
-                                    table.data_ptr(), seq_len.data_ptr(), _ptr(page_refs), table.shape[0], table.shape[1])
-        self.ref = ctypes.byref(self.struct)
+        self.table, self.seq_len, self.page_refs = table, seq_len, page_refs
+
+    def _struct(self, struct):
+        self.struct, self.ref = struct, ctypes.byref(struct)
         self.scratch = {}   # of the page operations, by stream handle
+        self.fn = {n: getattr(lib(), f) for n, f in self.calls.items()}
 
     @classmethod
     def empty(cls, n_layer: int, n_pages: int, page_size: int, n_kv_head: int, head_dim: int, n_slots: int, max_pages: int):
@@ -609,6 +641,66 @@ class PagedKV:
         import torch
         shape = (n_layer, n_pages, page_size, n_kv_head, head_dim)
         return cls(torch.zeros(shape, dtype=torch.float16, device="cuda"), torch.zeros(shape, dtype=torch.float16, device="cuda"),
+                   torch.full((n_slots, max_pages), -1, dtype=torch.int32, device="cuda"),
+                   torch.zeros(n_slots, dtype=torch.int32, device="cuda"), torch.zeros(n_pages, dtype=torch.int32, device="cuda"))
+
+
+class PagedKV4(PagedKV):
+    """A paged KV cache in 4 bits (hesa_cuda_paged_kv4): codes k, v [n_layer,
+    n_pages, page_size, n_kv_head, head_dim / 2] (uint8) and scales k_scale,
+    v_scale [..., head_dim / 32] (fp16), in groups of 32 dims; any layer and page
+    strides, the same for all four pools when counted in groups, the rest
+    contiguous. Tables, batches and every function that takes a PagedKV are the
+    same."""
+
+    calls = {"paged_attention": "hesa_cuda_paged_attention_kv4", "paged_attention_workspace_size": "hesa_cuda_paged_attention_kv4_workspace_size",
+             "rope_kv_paged": "hesa_cuda_rope_kv4_paged", "kv_pages_workspace_size": "hesa_cuda_kv4_pages_workspace_size", "kv_reserve": "hesa_cuda_kv4_reserve",
+             "kv_free": "hesa_cuda_kv4_free", "kv_fork": "hesa_cuda_kv4_fork", "kv_compact": "hesa_cuda_kv4_compact",
+             "kv_copy_pages": "hesa_cuda_kv4_copy_pages", "kv_reorder": "hesa_cuda_kv4_reorder"}
+
+    def __init__(self, k, v, k_scale, v_scale, table, seq_len, page_refs=None):
+        import torch
+        _want(k, torch.uint8, "k", dims=5)
+        dev = k.device.index
+        _want(v, torch.uint8, "v", dev, 5)
+        _want(k_scale, torch.float16, "k_scale", dev, 5)
+        _want(v_scale, torch.float16, "v_scale", dev, 5)
+        _want(table, torch.int32, "table", dev, 2)
+        n_layer, n_pages, page, n_kv, half = k.shape
+        if half % 16:
+            raise ValueError("head_dim must be a multiple of 32")
+        groups = half // 16
+        strides = _page_strides(k)
+        if v.shape != k.shape or _page_strides(v) != strides:
+            raise ValueError("k and v must have the same shape and strides")
+        if strides[2:] != (n_kv * half, half, 1):
+            raise ValueError("places, heads and dims of a page must be contiguous")
+        if strides[0] % 16 or strides[1] % 16:
+            raise ValueError("layer and page strides must be whole groups")
+        of_scales = (strides[0] // 16, strides[1] // 16, n_kv * groups, groups, 1)
+        for t, what in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+            if t.shape != (n_layer, n_pages, page, n_kv, groups):
+                raise ValueError(f"{what} must be {[n_layer, n_pages, page, n_kv, groups]}")
+            # the stride of a dimension of one entry is not looked at
+            if any(n > 1 and a != b for n, a, b in zip(t.shape, t.stride(), of_scales)):
+                raise ValueError(f"{what} must have the strides of k and v, counted in groups")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._tables(dev, n_layer, n_pages, page, n_kv, 2 * half, table, seq_len, page_refs)
+        self._struct(PagedKV4Struct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), of_scales[1], of_scales[0], n_layer, n_pages,
+                                    page, n_kv, 2 * half, table.data_ptr(), seq_len.data_ptr(), _ptr(page_refs), table.shape[0], table.shape[1]))
+
+    @classmethod
+    def empty(cls, n_layer: int, n_pages: int, page_size: int, n_kv_head: int, head_dim: int, n_slots: int, max_pages: int):
+        """A new cache on the current device with every page free and every slot empty."""
+        import torch
+        # pages start at multiples of 8 groups, whatever a page holds
+        per = page_size * n_kv_head * (head_dim // 32)
+        stride = -(-per // 8) * 8
+
+        def pool(width, dtype):
+            flat = torch.zeros((n_layer, n_pages, stride * width), dtype=dtype, device="cuda")
+            return flat[:, :, : per * width].unflatten(2, (page_size, n_kv_head, head_dim // 32 * width))
+        return cls(pool(16, torch.uint8), pool(16, torch.uint8), pool(1, torch.float16), pool(1, torch.float16),
                    torch.full((n_slots, max_pages), -1, dtype=torch.int32, device="cuda"),
                    torch.zeros(n_slots, dtype=torch.int32, device="cuda"), torch.zeros(n_pages, dtype=torch.int32, device="cuda"))
 
@@ -650,7 +742,7 @@ def paged_attention_workspace(cache, batch, n_head: int):
     """A workspace for paged_attention of batches of these bounds."""
     import torch
     _same_device(cache, batch)
-    nb = int(lib().hesa_cuda_paged_attention_workspace_size(cache.ref, batch.ref, n_head))
+    nb = int(cache.fn["paged_attention_workspace_size"](cache.ref, batch.ref, n_head))
     if nb == 0:
         raise HesaError(6, lib().hesa_cuda_last_error().decode())
     return torch.empty(nb, dtype=torch.uint8, device="cuda")
@@ -682,7 +774,7 @@ def paged_attention(cache, layer: int, batch, q, n_head: int, out=None, scale: f
         workspace = _new(lambda: paged_attention_workspace(cache, batch, n_head), stream)
     else:
         _want(workspace, torch.uint8, "workspace", dev)
-    _check(lib().hesa_cuda_paged_attention(cache.ref, layer, batch.ref, qp, ldq, op, ldo, n_head,
+    _check(cache.fn["paged_attention"](cache.ref, layer, batch.ref, qp, ldq, op, ldo, n_head,
                                            None if opts is None else ctypes.byref(opts), workspace.data_ptr(),
                                            workspace.numel(), _stream_on(cache.device, stream)))
     return out
@@ -703,7 +795,7 @@ def rope_kv_paged(cache, layer: int, batch, q, k, v, n_head: int, rope_table=Non
         _want(rope_table, torch.float32, "rope_table", dev, 2)
         if rope_table.shape[1] != cache.head_dim or not rope_table.is_contiguous():
             raise ValueError("rope_table must be [rows, head_dim] and contiguous")
-    _check(lib().hesa_cuda_rope_kv_paged(cache.ref, layer, batch.ref, qp, ldq, kp, ldk, vp, ldv, n_head, _ptr(rope_table),
+    _check(cache.fn["rope_kv_paged"](cache.ref, layer, batch.ref, qp, ldq, kp, ldk, vp, ldv, n_head, _ptr(rope_table),
                                          0 if rope_table is None else rope_table.shape[0], _stream_on(cache.device, stream)))
 
 
@@ -711,7 +803,7 @@ def kv_pages_workspace(cache):
     """Scratch for the page operations on this cache."""
     import torch
     _same_device(cache)
-    nb = int(lib().hesa_cuda_kv_pages_workspace_size(cache.ref))
+    nb = int(cache.fn["kv_pages_workspace_size"](cache.ref))
     if nb == 0:
         raise HesaError(6, lib().hesa_cuda_last_error().decode() or "page operations take at most 2^20 pages")
     return torch.empty(nb, dtype=torch.uint8, device="cuda")
@@ -740,7 +832,7 @@ def kv_reserve(cache, slots, n_new, workspace=None, stream=None) -> None:
     """n_new[i] more tokens, and the pages for them, for slot slots[i] (hesa_cuda_kv_reserve)."""
     ws = _page_workspace(cache, workspace, stream)
     n = slots.numel()
-    _check(lib().hesa_cuda_kv_reserve(cache.ref, _ints(slots, "slots", n, cache.device), _ints(n_new, "n_new", n, cache.device), n,
+    _check(cache.fn["kv_reserve"](cache.ref, _ints(slots, "slots", n, cache.device), _ints(n_new, "n_new", n, cache.device), n,
                                       ws.data_ptr(), ws.numel(), _stream_on(cache.device, stream)))
 
 
@@ -748,7 +840,7 @@ def kv_free(cache, slots, workspace=None, stream=None) -> None:
     """Give back the pages of these slots and empty them (hesa_cuda_kv_free)."""
     ws = _page_workspace(cache, workspace, stream)
     n = slots.numel()
-    _check(lib().hesa_cuda_kv_free(cache.ref, _ints(slots, "slots", n, cache.device), n, ws.data_ptr(), ws.numel(),
+    _check(cache.fn["kv_free"](cache.ref, _ints(slots, "slots", n, cache.device), n, ws.data_ptr(), ws.numel(),
                                    _stream_on(cache.device, stream)))
 
 
@@ -756,7 +848,7 @@ def kv_fork(cache, src, dst, workspace=None, stream=None) -> None:
     """The empty slots dst become copies of the slots src, sharing full pages (hesa_cuda_kv_fork)."""
     ws = _page_workspace(cache, workspace, stream)
     n = src.numel()
-    _check(lib().hesa_cuda_kv_fork(cache.ref, _ints(src, "src", n, cache.device), _ints(dst, "dst", n, cache.device), n,
+    _check(cache.fn["kv_fork"](cache.ref, _ints(src, "src", n, cache.device), _ints(dst, "dst", n, cache.device), n,
                                    ws.data_ptr(), ws.numel(), _stream_on(cache.device, stream)))
 
 
@@ -764,16 +856,85 @@ def kv_compact(cache, n_live=None, workspace=None, stream=None) -> None:
     """Move the pages in use to the front of the pool (hesa_cuda_kv_compact); n_live: int32 [1] for their count."""
     ws = _page_workspace(cache, workspace, stream)
     p = None if n_live is None else _ints(n_live, "n_live", 1, cache.device)
-    _check(lib().hesa_cuda_kv_compact(cache.ref, p, ws.data_ptr(), ws.numel(), _stream_on(cache.device, stream)))
+    _check(cache.fn["kv_compact"](cache.ref, p, ws.data_ptr(), ws.numel(), _stream_on(cache.device, stream)))
 
 
 def kv_copy_pages(cache, src_pages, dst_pages, workspace=None, stream=None) -> None:
     """Page dst_pages[i] becomes a copy of page src_pages[i] in every layer (hesa_cuda_kv_copy_pages)."""
     ws = _page_workspace(cache, workspace, stream)
     n = src_pages.numel()
-    _check(lib().hesa_cuda_kv_copy_pages(cache.ref, _ints(src_pages, "src_pages", n, cache.device),
+    _check(cache.fn["kv_copy_pages"](cache.ref, _ints(src_pages, "src_pages", n, cache.device),
                                          _ints(dst_pages, "dst_pages", n, cache.device), n, ws.data_ptr(), ws.numel(),
                                          _stream_on(cache.device, stream)))
+
+
+def kv_reorder(cache, slots, parents, width: int, workspace=None, stream=None) -> None:
+    """Slots in groups of `width`: slots[i] takes over what slot parents[i] of its
+    group held, sharing full pages (hesa_cuda_kv_reorder)."""
+    ws = _page_workspace(cache, workspace, stream)
+    n = slots.numel()
+    _check(cache.fn["kv_reorder"](cache.ref, _ints(slots, "slots", n, cache.device), _ints(parents, "parents", n, cache.device), n, width,
+                                  ws.data_ptr(), ws.numel(), _stream_on(cache.device, stream)))
+
+
+def kv_read(cache, layer: int, batch, k=None, v=None, stream=None):
+    """What layer `layer` of a cache in 4 bits holds for the batch's new tokens:
+    k, v [n_tokens, n_kv_head * head_dim] fp32 (hesa_cuda_kv4_read); without k
+    and v new tensors, zero where no sequence has a row. Returns (k, v)."""
+    import torch
+    if not isinstance(cache, PagedKV4):
+        raise ValueError("kv_read is for a PagedKV4: a PagedKV's values lie in its pools")
+    _same_device(cache, batch)
+    n, width = batch.n_tokens, cache.n_kv_head * cache.head_dim
+
+    def new():
+        return torch.zeros((n, width), dtype=torch.float32, device="cuda")
+    k = _new(new, stream) if k is None else k
+    v = _new(new, stream) if v is None else v
+    kp, ldk = _rows(k, n, width, "k", cache.device)
+    vp, ldv = _rows(v, n, width, "v", cache.device)
+    _check(lib().hesa_cuda_kv4_read(cache.ref, layer, batch.ref, kp, ldk, vp, ldv, _stream_on(cache.device, stream)))
+    return k, v
+
+
+def beam_select_workspace(n_seq: int, width: int, vocab: int):
+    """A workspace for beam_select."""
+    import torch
+    nb = int(lib().hesa_cuda_beam_select_workspace_size(n_seq, width, vocab))
+    return torch.empty(max(nb, 16), dtype=torch.uint8, device="cuda")
+
+
+def beam_select(logits, scores, width: int, ended=None, workspace=None, stream=None):
+    """The `width` best next beams of each sequence from its beams' logits
+    [n_seq * width, vocab] fp32 (any row stride) and scores [n_seq * width] fp32;
+    ended [n_seq * width] int32: beams that only go on as they are
+    (hesa_cuda_beam_select). Returns (scores, parents, tokens), each
+    [n_seq * width]."""
+    import torch
+    _want(logits, torch.float32, "logits", dims=2)
+    n, vocab = logits.shape
+    if vocab > 1 and logits.stride(1) != 1:
+        raise ValueError("rows of logits must be contiguous")
+    if not 1 <= width <= 32 or n % width:
+        raise ValueError("width must be 1 .. 32 and divide the rows of logits")
+    dev = logits.device.index
+    _want(scores, torch.float32, "scores", dev, 1)
+    if scores.numel() != n or not scores.is_contiguous():
+        raise ValueError(f"scores must hold {n} contiguous values")
+    ep = None if ended is None else _ints(ended, "ended", n, dev)
+
+    def outputs():
+        return (torch.empty(n, dtype=torch.float32, device=logits.device), torch.empty(n, dtype=torch.int32, device=logits.device),
+                torch.empty(n, dtype=torch.int32, device=logits.device))
+    best, parents, tokens = outputs() if stream is None else _new(outputs, stream)
+    if workspace is None:
+        workspace = _new(lambda: beam_select_workspace(n // width, width, vocab), stream)
+    else:
+        _want(workspace, torch.uint8, "workspace", dev)
+    _check(lib().hesa_cuda_beam_select(logits.data_ptr(), logits.stride(0) if n > 1 else vocab, n // width, width, vocab, scores.data_ptr(), ep,
+                                       best.data_ptr(), parents.data_ptr(), tokens.data_ptr(), workspace.data_ptr(), workspace.numel(),
+                                       _stream_on(dev, stream)))
+    return best, parents, tokens
 
 
 def token_logprobs_workspace(n_rows: int, vocab: int, top_k: int = 0):

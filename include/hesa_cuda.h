@@ -450,6 +450,125 @@ HESA_CUDA_API int hesa_cuda_kv_copy_pages(const hesa_cuda_paged_kv* kv, const in
                                           const int32_t* dst_pages, int32_t n, void* workspace,
                                           size_t workspace_bytes, void* stream);
 
+/* n slots in groups of `width` (1 .. 32; n a multiple of it), as the beams of a
+ * search change places: slot slots[i] takes over what slot
+ * slots[i - i % width + parents[i]] held, all at once; parents[i] lies in
+ * 0 .. width - 1 and may be named several times or not at all. Full pages are
+ * shared. A partly filled last page goes to the first slot in the list that
+ * takes it over; the others get copies of its filled places, in all layers. What
+ * no slot takes over is given back first, and may be taken again by the copies:
+ * new pages are the lowest free ones, in the order of the list. Table entries
+ * that were in use and lie behind a slot's new pages become -1. No counterpart in
+ * the reference. A page operation like those above: workspace of
+ * hesa_cuda_kv_pages_workspace_size, at most n_slots slots, carried out as a
+ * whole or not at all (status 3 also for a parent outside its group). */
+HESA_CUDA_API int hesa_cuda_kv_reorder(const hesa_cuda_paged_kv* kv, const int32_t* slots, const int32_t* parents,
+                                       int32_t n, int32_t width, void* workspace, size_t workspace_bytes,
+                                       void* stream);
+
+/* ---- the paged cache in 4 bits ----
+ * The values of a head come in groups of 32 consecutive dims: 16 bytes of codes
+ * (byte b of a group holds dim 2 b in its low and dim 2 b + 1 in its high nibble)
+ * and one fp16 scale d; a value is d * (code - 8), 4.5 bits in all. Group g of kv
+ * head h of the token in place s of page p of layer i is number
+ *   i * layer_stride + p * page_stride + (s * n_kv_head + h) * (head_dim / 32) + g
+ * of its pool: both strides count groups, are multiples of 8, and hold for the
+ * pools of codes (16 bytes a group) and of scales (2 bytes a group) alike. Scales
+ * have at most 8 significant bits, are multiples of 2^-24 and at most 2720 in
+ * magnitude, or NaN, so that every value is an fp16 number exactly: what
+ * hesa_cuda_rope_kv4_paged writes. With other scales values are not what the
+ * formula says. Everything else, the tables, their limits and their meaning, is
+ * as in hesa_cuda_paged_kv; all four pools are 16-byte aligned. A new cache has
+ * seq_len and page_refs zero. */
+typedef struct {
+    void* k;             /* codes */
+    void* v;
+    void* k_scale;       /* fp16 */
+    void* v_scale;
+    int64_t page_stride, layer_stride;
+    int32_t n_layer, n_pages, page_size, n_kv_head, head_dim;
+    int32_t* table;      /* [n_slots, max_pages] */
+    int32_t* seq_len;    /* [n_slots] */
+    int32_t* page_refs;  /* [n_pages] */
+    int32_t n_slots, max_pages;
+} hesa_cuda_paged_kv4;
+
+/* hesa_cuda_rope_kv_paged for a cache in 4 bits: the same rotation, arguments
+ * and refusals. A group's scale is m / -8, m its value of the largest magnitude
+ * (the first such), rounded to nearest even to 8 significant bits (to a multiple of
+ * 2^-24 where it is smaller than 2^-17); a group with a magnitude above 21824
+ * (its scale would be above 2720), or a value that is not finite, gets the scale
+ * NaN and codes 8. A code is floor(x * (1 / scale) + 8.5) limited to 0 .. 15, each
+ * operation rounded to fp32, the rounding of Q4_0; 8 where the scale is zero. */
+HESA_CUDA_API int hesa_cuda_rope_kv4_paged(const hesa_cuda_paged_kv4* kv, int32_t layer,
+                                           const hesa_cuda_token_batch* batch, float* q, int64_t ldq, const float* k,
+                                           int64_t ldk, const float* v, int64_t ldv, int64_t n_head,
+                                           const float* rope_table, int32_t rope_rows, void* stream);
+
+/* The other way: the values that the pages of one layer hold for the batch's new
+ * tokens, as fp32 rows k and v [n_tokens, n_kv_head * head_dim] with row strides
+ * ldk, ldv (multiples of 4), 16-byte aligned; either may be NULL. A token whose
+ * page is outside the pool gives zeros and device status 3; rows of no sequence
+ * stay as they are. The counterpart of hesa_cuda_dequantize for a cache. */
+HESA_CUDA_API int hesa_cuda_kv4_read(const hesa_cuda_paged_kv4* kv, int32_t layer, const hesa_cuda_token_batch* batch,
+                                     float* k, int64_t ldk, float* v, int64_t ldv, void* stream);
+
+/* hesa_cuda_paged_attention over a cache in 4 bits: the same formula, options,
+ * limits and treatment of rows, masks and numbers that are not finite, with the
+ * values that the cache holds. (A group with scale NaN is a k or v that is not
+ * finite.) Next tokens are read from the codes; for chunks (more rows a kv head
+ * and sequence than tiles of 8 are worth) the tokens of as many sequences at a
+ * time as fit into 1 GB, at least one, are laid out in fp16 in the workspace, which
+ * is large then: 4 * n_kv_head * head_dim bytes for each of max_len tokens. */
+HESA_CUDA_API size_t hesa_cuda_paged_attention_kv4_workspace_size(const hesa_cuda_paged_kv4* kv,
+                                                                  const hesa_cuda_token_batch* batch, int64_t n_head);
+HESA_CUDA_API int hesa_cuda_paged_attention_kv4(const hesa_cuda_paged_kv4* kv, int32_t layer,
+                                                const hesa_cuda_token_batch* batch, const float* q, int64_t ldq,
+                                                float* out, int64_t ldo, int64_t n_head,
+                                                const hesa_cuda_attn_options* options, void* workspace,
+                                                size_t workspace_bytes, void* stream);
+
+/* The page operations (hesa_cuda_kv_reserve and the others) on a cache in 4 bits. */
+HESA_CUDA_API size_t hesa_cuda_kv4_pages_workspace_size(const hesa_cuda_paged_kv4* kv);
+HESA_CUDA_API int hesa_cuda_kv4_reserve(const hesa_cuda_paged_kv4* kv, const int32_t* slots, const int32_t* n_new,
+                                        int32_t n, void* workspace, size_t workspace_bytes, void* stream);
+HESA_CUDA_API int hesa_cuda_kv4_free(const hesa_cuda_paged_kv4* kv, const int32_t* slots, int32_t n, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+HESA_CUDA_API int hesa_cuda_kv4_fork(const hesa_cuda_paged_kv4* kv, const int32_t* src, const int32_t* dst, int32_t n,
+                                     void* workspace, size_t workspace_bytes, void* stream);
+HESA_CUDA_API int hesa_cuda_kv4_compact(const hesa_cuda_paged_kv4* kv, int32_t* n_live, void* workspace,
+                                        size_t workspace_bytes, void* stream);
+HESA_CUDA_API int hesa_cuda_kv4_copy_pages(const hesa_cuda_paged_kv4* kv, const int32_t* src_pages,
+                                           const int32_t* dst_pages, int32_t n, void* workspace,
+                                           size_t workspace_bytes, void* stream);
+HESA_CUDA_API int hesa_cuda_kv4_reorder(const hesa_cuda_paged_kv4* kv, const int32_t* slots, const int32_t* parents,
+                                        int32_t n, int32_t width, void* workspace, size_t workspace_bytes,
+                                        void* stream);
+
+/* The next beams of n_seq sequences with `width` (1 .. 32) beams each, from the
+ * beams' logits [n_seq * width, vocab] fp32 (row stride ld, any 4-byte alignment)
+ * and their scores (sums of log probabilities, [n_seq * width]): of all
+ *   scores[b] + log softmax(logits[b])[token]
+ * of a sequence's beams, and scores[b] itself, with token -1, for each beam that
+ * has ended (ended[b] != 0; NULL: none has; its logits are not looked at), the
+ * `width` largest, descending, equal ones by the lower beam and then the lower
+ * token: next_scores, parents (0 .. width - 1, the beam within the sequence) and
+ * tokens, each [n_seq * width]. Candidates of one beam are ordered by their
+ * logits; those of different beams by sums in 64 bits, each beam's log of a sum
+ * having fp32 terms (1e-7 or so).
+ * A logit or score of -inf is ruled out: such candidates are taken when there is
+ * nothing else, with score -inf. (At its start a search has scores 0, -inf, ...,
+ * -inf.) A beam whose score is NaN or +inf, or whose logits hold one of these, ranks
+ * as -inf with all its candidates, which have the score NaN. next_scores may be
+ * scores; the other buffers do not overlap. The workspace (16-byte aligned, need
+ * not be set) is scratch. With hesa_cuda_token_logprobs this is the search's half
+ * of cpu_softmax_f32 (cpu_backend.cpp:48-70); no beam search in the reference. */
+HESA_CUDA_API size_t hesa_cuda_beam_select_workspace_size(int64_t n_seq, int32_t width, int64_t vocab);
+HESA_CUDA_API int hesa_cuda_beam_select(const float* logits, int64_t ld, int64_t n_seq, int32_t width, int64_t vocab,
+                                        const float* scores, const int32_t* ended, float* next_scores,
+                                        int32_t* parents, int32_t* tokens, void* workspace, size_t workspace_bytes,
+                                        void* stream);
+
 /* From n_rows rows of fp32 logits (row stride ld, any 4-byte alignment): the
  * log softmax of each row's token, the entropy -sum p log p of the row in
  * nats, and the top_k (0 .. 32, at most vocab) largest log probabilities with
