@@ -52,8 +52,9 @@ template <int HD> struct Rows4Shape : RowParts<HD, (HD == 256 ? 8 : 16)> {
     static constexpr int row = HD / 2, srow = groups * 2;  // bytes of a key's codes and scales
     static constexpr int v = kKeys4 * row, ks = 2 * v, vs = ks + kKeys4 * srow;   // K's codes, V's, then the scales
     static constexpr int stage = vs + kKeys4 * srow;       // a warp's
-    static constexpr int stages = HD == 64 ? 5 : 3;
-    static constexpr size_t smem = static_cast<size_t>(stage) * stages * warps;
+    static constexpr int stages = HD == 64 ? 4 : 2;
+    static constexpr int q = HD / 16 * 512;                // a warp's q: a k-step's operand is 16 bytes a lane
+    static constexpr size_t smem = static_cast<size_t>(stage * stages + q) * warps;
 };
 
 // Where piece ch (16 bytes) of key j lies in a block. K: a thread (n, c) of a warp
@@ -165,12 +166,16 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
     return v;
 }
+__device__ __forceinline__ void sts128(uint32_t a, const uint32_t (&v)[4]) {
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
 __device__ __forceinline__ uint32_t lds16(uint32_t a) {
     unsigned short v;
     asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
     return v;
 }
 __device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
+__device__ __forceinline__ __half2 half2_of(uint32_t x) { return as_half2(prmt(x, x, 0x1010u)); }
 
 // This warp's head's attention over its blocks of a segment. part < 0: they are
 // all that the rows see, and the result goes to out; else (m, l, acc) go to that
@@ -198,7 +203,7 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const Pools4& p
     const int i1 = min(tv.kb.n, seg.b1);
 
     // ---- q as hi and lo halves of q * 2^-e, max |q| 2^-e in [2^14, 2^15), in the order of the codes' pairs ----
-    uint32_t qa[2 * KW][4];
+    const uint32_t qs = smem_addr(ring) + S::stage * S::stages + lane * 16;
     float qscale;   // 2^e; NaN for a row that is not finite
     {
         const float* q = A.q + static_cast<int64_t>(sv.q0 + t) * A.ldq + static_cast<int64_t>(h) * HD;
@@ -224,18 +229,23 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const Pools4& p
 #pragma unroll
         for (int w = 0; w < KW; ++w)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float x = fin ? v[w][i] * f1 * f2 : 0.f, y = fin ? v[w][i + 4] * f1 * f2 : 0.f;
-                split_half2(x, y, qa[2 * w + (i >> 1)][2 * (i & 1)], qa[2 * w + (i >> 1)][2 * (i & 1) + 1]);
+            for (int i = 0; i < 4; i += 2) {
+                uint32_t a[4];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const float x = fin ? v[w][i + k] * f1 * f2 : 0.f, y = fin ? v[w][i + k + 4] * f1 * f2 : 0.f;
+                    split_half2(x, y, a[2 * k], a[2 * k + 1]);
+                }
+                sts128(qs + (2 * w + (i >> 1)) * 512, a);   // read by this lane alone
             }
     }
     const float sc = A.cap2 != 0.f ? qscale : qscale * A.scale2;
     const float slope2 = A.slopes ? A.slopes[h] * 1.44269504088896341f : 0.f;
 
     float m = -INFINITY, l = 0.f;
-    float acc[NT][2];
+    float2 acc[NT];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = 0.f;
+    for (int i = 0; i < NT; ++i) acc[i] = make_float2(0.f, 0.f);
     const int vg = n * HD / 256;   // the group of this thread's column's dims
 
     for (int i = seg.b0 + sub; i < i1; i += hg.subs, ++at) {
@@ -246,35 +256,40 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const Pools4& p
         const uint32_t st = base + at % S::stages * S::stage;
         const int32_t j0 = tv.kb.at(i) * kKeys4;
 
-        // ---- scores of keys 8 t + 2 c, + 1 ----
+        // ---- scores of keys 8 x + 2 c, + 1 ----
         float s[KT][4];
 #pragma unroll
         for (int x = 0; x < KT; ++x) s[x][0] = s[x][1] = s[x][2] = s[x][3] = 0.f;
 #pragma unroll
-        for (int x = 0; x < KT; ++x) {
-            const int key = 8 * x + n;
+        for (int p = 0; p < (HD == 256 ? 2 : 1); ++p) {
+            uint32_t w[KT][HD == 64 ? 2 : 4];
+            __half2 d[KT];
 #pragma unroll
-            for (int p = 0; p < (HD == 256 ? 2 : 1); ++p) {
-                uint32_t w[4];
+            for (int x = 0; x < KT; ++x) {
+                const int key = 8 * x + n;
                 if constexpr (HD == 64) {
                     const uint2 y = lds64(st + k_at<HD>(key, 0) + c * 8);
-                    w[0] = y.x;
-                    w[1] = y.y;
+                    w[x][0] = y.x;
+                    w[x][1] = y.y;
                 } else {
                     const uint4 y = lds128(st + k_at<HD>(key, c + 4 * p));
-                    w[0] = y.x;
-                    w[1] = y.y;
-                    w[2] = y.z;
-                    w[3] = y.w;
+                    w[x][0] = y.x;
+                    w[x][1] = y.y;
+                    w[x][2] = y.z;
+                    w[x][3] = y.w;
                 }
-                const uint32_t d16 = lds16(st + S::ks + key * S::srow + (HD == 64 ? c >> 1 : c + 4 * p) * 2);
-                const __half2 d = as_half2(d16 | d16 << 16), dm = __hmul2(d, __float2half2_rn(-24.f));
+                d[x] = half2_of(lds16(st + S::ks + key * S::srow + (HD == 64 ? c >> 1 : c + 4 * p) * 2));
+            }
 #pragma unroll
-                for (int y = 0; y < (HD == 64 ? 2 : 4); ++y) {
+            for (int y = 0; y < (HD == 64 ? 2 : 4); ++y) {
+                const uint4 a0 = lds128(qs + 2 * (4 * p + y) * 512), a1 = lds128(qs + (2 * (4 * p + y) + 1) * 512);
+                const uint32_t q0[4] = {a0.x, a0.y, a0.z, a0.w}, q1[4] = {a1.x, a1.y, a1.z, a1.w};
+#pragma unroll
+                for (int x = 0; x < KT; ++x) {
                     uint32_t b[4];
-                    code_pairs(w[y], d, dm, b);
-                    mma16816(s[x], qa[2 * (4 * p + y)], b[0], b[1]);
-                    mma16816(s[x], qa[2 * (4 * p + y) + 1], b[2], b[3]);
+                    code_pairs(w[x][y], d[x], b);
+                    mma16816(s[x], q0, b[0], b[1]);
+                    mma16816(s[x], q1, b[2], b[3]);
                 }
             }
         }
@@ -313,7 +328,7 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const Pools4& p
                     for (int k = 0; k < 2; ++k)   // the columns 2 c + k of this thread's sums
                         if (!isfinite(__half2float(vs[j * S::groups + (2 * c + k) * HD / 256]))) {
 #pragma unroll
-                            for (int x = 0; x < NT; ++x) acc[x][k] = NAN;
+                            for (int x = 0; x < NT; ++x) (k ? acc[x].y : acc[x].x) = NAN;
                         }
                 }
                 __syncwarp();
@@ -342,7 +357,7 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const Pools4& p
 
         // ---- P V: keys 2 c, + 1, + 8, + 9 of each 16, dims of column n ----
         uint32_t vw[kKeys4 / 4][VW];   // [k-step, + 8, second of the pair]
-        __half2 vd[KT], vm[KT];
+        __half2 vd[KT];
 #pragma unroll
         for (int x = 0; x < KT; ++x) {
             uint32_t d16[2];
@@ -364,8 +379,7 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const Pools4& p
                 }
                 d16[k] = lds16(st + S::vs + key * S::srow + vg * 2);
             }
-            vd[x] = as_half2(d16[0] | d16[1] << 16);
-            vm[x] = __hmul2(vd[x], __float2half2_rn(-24.f));
+            vd[x] = as_half2(prmt(d16[0], d16[1], 0x5410u));
         }
 #pragma unroll
         for (int y = 0; y < 2 * VW; ++y) {   // four dims of the column
@@ -375,15 +389,14 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const Pools4& p
 #pragma unroll
             for (int x = 0; x < KT; x += 2) {
                 uint32_t b0[4], b1[4];
-                code_pairs(prmt(vw[2 * x][y >> 1], vw[2 * x + 1][y >> 1], (y & 1) ? 0x7632u : 0x5410u), vd[x], vm[x], b0);
-                code_pairs(prmt(vw[2 * x + 2][y >> 1], vw[2 * x + 3][y >> 1], (y & 1) ? 0x7632u : 0x5410u), vd[x + 1], vm[x + 1], b1);
+                code_pairs(prmt(vw[2 * x][y >> 1], vw[2 * x + 1][y >> 1], (y & 1) ? 0x7632u : 0x5410u), vd[x], b0);
+                code_pairs(prmt(vw[2 * x + 2][y >> 1], vw[2 * x + 3][y >> 1], (y & 1) ? 0x7632u : 0x5410u), vd[x + 1], b1);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) mma16816(o[k], pa[x >> 1], b0[k], b1[k]);
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                acc[4 * y + k][0] = fmaf(acc[4 * y + k][0], corr, o[k][0] + o[k][2]);
-                acc[4 * y + k][1] = fmaf(acc[4 * y + k][1], corr, o[k][1] + o[k][3]);
+                acc[4 * y + k] = ffma2(acc[4 * y + k], make_float2(corr, corr), fadd2(make_float2(o[k][0], o[k][1]), make_float2(o[k][2], o[k][3])));
             }
         }
     }
@@ -402,10 +415,10 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const Pools4& p
         o = ml + S::part_rows(part_count(A.n_split, hg)) * 2 + at_row * HD;
     }
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int x = 0; x < NT; x += 4)
-            *reinterpret_cast<float4*>(o + (2 * c + k) * NT + x) = make_float4(acc[x][k] * inv, acc[x + 1][k] * inv, acc[x + 2][k] * inv, acc[x + 3][k] * inv);
+    for (int x = 0; x < NT; x += 4) {
+        *reinterpret_cast<float4*>(o + 2 * c * NT + x) = make_float4(acc[x].x * inv, acc[x + 1].x * inv, acc[x + 2].x * inv, acc[x + 3].x * inv);
+        *reinterpret_cast<float4*>(o + (2 * c + 1) * NT + x) = make_float4(acc[x].y * inv, acc[x + 1].y * inv, acc[x + 2].y * inv, acc[x + 3].y * inv);
+    }
 }
 
 template <int HD>
@@ -435,7 +448,7 @@ rows4_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ Pools4 
             if (s_pre[i / hg.groups + 1] == s_pre[i / hg.groups]) cuts[i] = Cut{};
 
     const int sub = hg.sub_of(warp), hl = warp - sub * hg.heads;
-    uint8_t* ring = smem + static_cast<size_t>(warp) * S::stage * S::stages;
+    uint8_t* ring = smem + static_cast<size_t>(warp) * (S::stage * S::stages + S::q);
     Ahead ahead{};
     ahead.u = u;
     ahead.end = end;
@@ -472,47 +485,67 @@ struct Scratch {
     int32_t pages;
 };
 
-// A block writes kScratchPage tokens of one sequence, those that its rows see, and
-// their entry of the table. A warp takes a token's row: a lane four codes' words of
-// K, then of V.
+// Blocks x of gridDim.x share out one sequence's tokens that its rows see, kExpandTokens
+// at a time, and write the sequence's entries of the tables. A thread takes a word
+// of codes (16 bytes of fp16) of K or V at a time, four of them under way.
+constexpr int kExpandTokens = 8;
+
 __global__ void __launch_bounds__(256)
-expand_kernel(const AttnArgs A, const Pools4 pools, const Scratch w) {
+expand_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ Pools4 pools, const __grid_constant__ Scratch w, const FastDiv words_div) {
+    __shared__ int64_t s_from[kExpandTokens];   // first group of the token's K, -1: no page
     grid_dep_wait();
     grid_dep_launch();
-    const int seq = blockIdx.y, x = blockIdx.x;
+    const int seq = blockIdx.y;
     const SeqView sv = seq_view(A.c, A.b, seq);
-    if (threadIdx.x == 0) {
+    for (int x = blockIdx.x * blockDim.x + threadIdx.x; x < w.pages; x += gridDim.x * blockDim.x)
         w.table[static_cast<int64_t>(seq) * w.pages + x] = seq * w.pages + x;
-        if (x == 0) w.seq_len[seq] = sv.ok ? sv.len : -1;
-    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) w.seq_len[seq] = sv.ok ? sv.len : -1;
     if (!sv.ok || sv.n_new == 0) return;
     const int32_t prefix = A.prefix ? max(0, min(A.prefix[seq], sv.len)) : 0;
     const int32_t first = A.window > 0 ? max(0, sv.len - sv.n_new + 1 - A.window) : 0;   // the first key in a window
-    const int row_words = A.c.n_kv * A.c.head_dim / 8, lane = threadIdx.x & 31;
+    const int row_words = A.c.n_kv * A.c.head_dim / 8;
     const int32_t* table = A.c.table + static_cast<int64_t>(sv.slot) * A.c.max_pages;
-    const int32_t j1 = min((x + 1) * kScratchPage, sv.len);
-    for (int32_t j = x * kScratchPage + (threadIdx.x >> 5); j < j1; j += 8) {
-        if (j < first && j >= prefix) continue;
-        const int32_t pi = A.c.page_div.div(j), page = table[pi];
-        const bool good = page >= 0 && page < A.c.n_pages;
-        if (!good && lane == 0) record_status(A.status, kStatusBadPosition);
-        const int64_t from = good ? page * A.c.page_stride + static_cast<int64_t>(j - pi * A.c.page_size) * (row_words / 4) : 0;
-        const int64_t to = (static_cast<int64_t>(seq) * w.pages * kScratchPage + j) * row_words;
-        for (int u = lane; u < 2 * row_words; u += 32) {
-            const bool is_k = u < row_words;
-            const int at = is_k ? u : u - row_words;
-            uint32_t b[4] = {0u, 0u, 0u, 0u};
-            if (good) {
-                const uint32_t code = reinterpret_cast<const uint32_t*>((is_k ? pools.k : pools.v) + from)[at];
-                const __half2 d = __half2half2(((is_k ? pools.ks : pools.vs) + from)[at / 4]);
-                uint32_t p[4];
-                code_pairs(code, d, __hmul2(d, __float2half2_rn(-24.f)), p);   // (0, 4) (1, 5) (2, 6) (3, 7)
-                b[0] = prmt(p[0], p[1], 0x5410u);
-                b[1] = prmt(p[2], p[3], 0x5410u);
-                b[2] = prmt(p[0], p[1], 0x7632u);
-                b[3] = prmt(p[2], p[3], 0x7632u);
+    const int64_t base = static_cast<int64_t>(seq) * w.pages * kScratchPage;
+    for (int32_t j0 = blockIdx.x * kExpandTokens; j0 < sv.len; j0 += gridDim.x * kExpandTokens) {
+        const int n = min(kExpandTokens, sv.len - j0);
+        if (j0 + n <= first && j0 >= prefix) continue;
+        __syncthreads();
+        if (static_cast<int>(threadIdx.x) < n) {
+            const int32_t j = j0 + threadIdx.x, pi = A.c.page_div.div(j);
+            // what no row sees is not looked at
+            const int32_t page = j >= first || j < prefix ? table[pi] : 0;
+            const bool good = page >= 0 && page < A.c.n_pages;
+            if (!good) record_status(A.status, kStatusBadPosition);
+            s_from[threadIdx.x] = good ? page * A.c.page_stride + static_cast<int64_t>(j - pi * A.c.page_size) * (row_words / 4) : -1;
+        }
+        __syncthreads();
+        const int all = n * 2 * row_words;
+        for (int u0 = threadIdx.x; u0 < all; u0 += 4 * blockDim.x) {
+            uint32_t code[4];
+            __half d[4];
+            uint4* to[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int u = u0 + x * static_cast<int>(blockDim.x);
+                if (u >= all) break;
+                const int half = words_div.div(u), t = half >> 1, at = u - half * row_words;   // K, then V of each token
+                const bool is_k = !(half & 1);
+                const int64_t from = s_from[t];
+                code[x] = 0x88888888u;
+                d[x] = __half(__float2half_rn(0.f));
+                if (from >= 0) {
+                    code[x] = __ldcs(reinterpret_cast<const uint32_t*>((is_k ? pools.k : pools.v) + from) + at);
+                    d[x] = ((is_k ? pools.ks : pools.vs) + from)[at / 4];
+                }
+                to[x] = reinterpret_cast<uint4*>(is_k ? w.k : w.v) + (base + j0 + t) * row_words + at;
             }
-            reinterpret_cast<uint4*>(is_k ? w.k : w.v)[to + at] = make_uint4(b[0], b[1], b[2], b[3]);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                if (u0 + x * static_cast<int>(blockDim.x) >= all) break;
+                uint32_t p[4];
+                code_pairs(code[x], __half2half2(d[x]), p);   // (0, 4) (1, 5) (2, 6) (3, 7)
+                *to[x] = make_uint4(prmt(p[0], p[1], 0x5410u), prmt(p[2], p[3], 0x5410u), prmt(p[0], p[1], 0x7632u), prmt(p[2], p[3], 0x7632u));
+            }
         }
     }
 }
@@ -676,8 +709,10 @@ int hesa_cuda_paged_attention_kv4(const hesa_cuda_paged_kv4* kv, int32_t layer, 
             }
             o.prefix = options && options->prefix ? options->prefix + i : nullptr;
             a.prefix = o.prefix;
-            e = launch_dep(expand_kernel, dim3(static_cast<unsigned>(p.pages), static_cast<unsigned>(b.n_seq)), 256, 0, s, a, pools,
-                           Scratch{static_cast<__half*>(c.k), static_cast<__half*>(c.v), c.table, c.seq_len, p.pages});
+            // blocks for every SM, as far as the sequences have tokens for them
+            const int share = std::max(1, std::min((batch->max_len + kExpandTokens - 1) / kExpandTokens, (148 * 16 + b.n_seq - 1) / b.n_seq));
+            e = launch_dep(expand_kernel, dim3(static_cast<unsigned>(share), static_cast<unsigned>(b.n_seq)), 256, 0, s, a, pools,
+                           Scratch{static_cast<__half*>(c.k), static_cast<__half*>(c.v), c.table, c.seq_len, p.pages}, FastDiv(kv->n_kv_head * kv->head_dim / 8));
             if (e != cudaSuccess) break;
             rc = hesa_cuda_paged_attention(&c, 0, &b, q, ldq, out, ldo, n_head, &o, ws + used, workspace_bytes - used, stream);
             if (rc != HESA_CUDA_OK) return rc;
