@@ -32,6 +32,7 @@
 #include "trace.h"
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 namespace hesa_cuda {
@@ -75,15 +76,29 @@ template <int HD> __device__ __forceinline__ int v_at(int j, int ch) {
     if constexpr (HD == 256) ch ^= (r & 3) << 1;
     return r * (HD / 2) + ch * 16;
 }
+// In a loop over x, what v_at makes of key lane / groups + x * (32 / groups): that of x = 0 and a number of its own.
+template <int HD> __device__ __forceinline__ uint32_t v_step(uint32_t at0, int x) {
+    if constexpr (HD == 256) return ((x & 1) ? at0 ^ 64u : at0) + (x >> 1) * 8 * 128 + (x & 1) * 2 * 128;
+    return at0 + x * 512;   // 8 keys of 64 bytes, 16 of 32
+}
 
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 // BYTES (4, 8 or 16) from global to shared memory, zeros where !ok
 template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool ok) {
     const int n = ok ? BYTES : 0;
-    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// d = a b, in fp32 from zero
+__device__ __forceinline__ void mma16816_0(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 
 // A warp's way through its blocks of the CTA's run, ahead of the products.
 struct Ahead {
@@ -121,7 +136,9 @@ __device__ __forceinline__ void go_on(const AttnArgs& A, const HeadGroups& hg, c
     h.page = page_of(A, h);
 }
 
-// Block h.i into a stage, and h to the block after it. One group of copies, empty where there is none.
+// Block h.i into a stage, and h to the block after it. One group of copies, empty
+// where there is none. Where there is no key, or no page, the scales are zeros and
+// the codes any.
 template <int HD>
 __device__ __forceinline__ void copy_block(const AttnArgs& A, const Pools4& pools, const HeadGroups& hg, const int64_t* pre, int sub, int hl, uint32_t stage,
                                            Ahead& h) {
@@ -132,17 +149,18 @@ __device__ __forceinline__ void copy_block(const AttnArgs& A, const Pools4& pool
         const bool good = h.page >= 0 && h.page < A.c.n_pages;
         if (!good && j < h.len) record_status(A.status, kStatusBadPosition);
         // of this lane's key
-        const int64_t at = good ? h.page * A.c.page_stride + static_cast<int64_t>((j - A.c.page_div.div(j) * A.c.page_size) * A.c.n_kv + h.kvh) * S::groups : -1;
-        const int64_t from = good ? at : 0;
-        copy_async<S::srow>(stage + S::ks + lane * S::srow, pools.ks + from, good);
-        copy_async<S::srow>(stage + S::vs + lane * S::srow, pools.vs + from, good);
-        const int ch = lane % S::groups;
+        int64_t at = static_cast<int64_t>(((j - A.c.page_div.div(j) * A.c.page_size) * A.c.n_kv + h.kvh) * S::groups) + h.page * A.c.page_stride;
+        if (!good) at = 0;
+        copy_async<S::srow>(stage + S::ks + lane * S::srow, pools.ks + at, good);
+        copy_async<S::srow>(stage + S::vs + lane * S::srow, pools.vs + at, good);
+        const int ch = lane % S::groups, key = lane / S::groups;
+        const uint32_t kd = stage + k_at<HD>(key, ch), vd = stage + S::v + v_at<HD>(key, ch);
+        const uint4 *const kp = pools.k + ch, *const vp = pools.v + ch;
 #pragma unroll
         for (int x = 0; x < S::groups; ++x) {
-            const int key = lane / S::groups + x * (32 / S::groups);
-            const int64_t a = __shfl_sync(0xffffffffu, at, key);
-            copy_async<16>(stage + k_at<HD>(key, ch), pools.k + (a >= 0 ? a + ch : 0), a >= 0);
-            copy_async<16>(stage + S::v + v_at<HD>(key, ch), pools.v + (a >= 0 ? a + ch : 0), a >= 0);
+            const int64_t a = __shfl_sync(0xffffffffu, at, key + x * (32 / S::groups));
+            copy_async16(kd + x * 512, kp + a);   // 32 / groups keys of 16 * groups bytes
+            copy_async16(v_step<HD>(vd, x), vp + a);
         }
         h.i += hg.subs;
         if (h.i < h.i1) h.page = page_of(A, h);
@@ -241,6 +259,10 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const Pools4& p
     }
     const float sc = A.cap2 != 0.f ? qscale : qscale * A.scale2;
     const float slope2 = A.slopes ? A.slopes[h] * 1.44269504088896341f : 0.f;
+    // Scores and their maximum are kept as the products come out, a score being `unit` of them; with a cap or a bias they
+    // are scaled first, and the unit is 1.
+    const bool plain = A.cap2 == 0.f && A.slopes == nullptr;
+    const float unit = plain ? (sc == 0.f ? FLT_MIN : sc) : 1.f;   // a unit of 0 would make NaN of a hidden key's -inf
 
     float m = -INFINITY, l = 0.f;
     float2 acc[NT];
@@ -258,8 +280,6 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const Pools4& p
 
         // ---- scores of keys 8 x + 2 c, + 1 ----
         float s[KT][4];
-#pragma unroll
-        for (int x = 0; x < KT; ++x) s[x][0] = s[x][1] = s[x][2] = s[x][3] = 0.f;
 #pragma unroll
         for (int p = 0; p < (HD == 256 ? 2 : 1); ++p) {
             uint32_t w[KT][HD == 64 ? 2 : 4];
@@ -288,32 +308,40 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const Pools4& p
                 for (int x = 0; x < KT; ++x) {
                     uint32_t b[4];
                     code_pairs(w[x][y], d[x], b);
-                    mma16816(s[x], q0, b[0], b[1]);
+                    if (p == 0 && y == 0) mma16816_0(s[x], q0, b[0], b[1]);
+                    else mma16816(s[x], q0, b[0], b[1]);
                     mma16816(s[x], q1, b[2], b[3]);
                 }
             }
         }
-        float sx[KT][2];
+        float2 sx[KT];
 #pragma unroll
-        for (int x = 0; x < KT; ++x)
+        for (int x = 0; x < KT; ++x) sx[x] = fadd2(make_float2(s[x][0], s[x][1]), make_float2(s[x][2], s[x][3]));
+        if (!plain) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                sx[x][k] = (s[x][k] + s[x][k + 2]) * sc;
-                if (A.cap2 != 0.f) sx[x][k] = capped(sx[x][k], A.cap2, A.cap_in);
+            for (int x = 0; x < KT; ++x) {
+                sx[x].x *= sc;
+                sx[x].y *= sc;
+                if (A.cap2 != 0.f) {
+                    sx[x].x = capped(sx[x].x, A.cap2, A.cap_in);
+                    sx[x].y = capped(sx[x].y, A.cap2, A.cap_in);
+                }
             }
+        }
         const int32_t jc = j0 + 2 * c;   // this thread's keys: jc + 8 x + k
         if (A.slopes) {
 #pragma unroll
-            for (int x = 0; x < KT; ++x)
-#pragma unroll
-                for (int k = 0; k < 2; ++k) sx[x][k] -= slope2 * fabsf(static_cast<float>(pos - (jc + 8 * x + k)));
+            for (int x = 0; x < KT; ++x) {
+                sx[x].x -= slope2 * fabsf(static_cast<float>(pos - (jc + 8 * x)));
+                sx[x].y -= slope2 * fabsf(static_cast<float>(pos - (jc + 8 * x + 1)));
+            }
         }
         if (!mask.all(tv.p_lo, tv.p_hi, j0, j0 + kKeys4)) {
 #pragma unroll
-            for (int x = 0; x < KT; ++x)
-#pragma unroll
-                for (int k = 0; k < 2; ++k)
-                    if (!keys.sees(jc + 8 * x + k)) sx[x][k] = -INFINITY;
+            for (int x = 0; x < KT; ++x) {
+                if (!keys.sees(jc + 8 * x)) sx[x].x = -INFINITY;
+                if (!keys.sees(jc + 8 * x + 1)) sx[x].y = -INFINITY;
+            }
             // A key that some row does not see has P = 0 there, which would make NaN of a
             // scale that is not finite. Such groups (there are none in a sound cache) are
             // added where they are seen and then cleared, so that they reach no other row.
@@ -339,21 +367,22 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const Pools4& p
         }
         float mx = m;
 #pragma unroll
-        for (int x = 0; x < KT; ++x) mx = fmaxf(mx, fmaxf(sx[x][0], sx[x][1]));
+        for (int x = 0; x < KT; ++x) mx = fmaxf(mx, fmaxf(sx[x].x, sx[x].y));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         const float ms = mx == -INFINITY ? 0.f : mx;   // nothing seen yet: P = 2^-inf = 0
-        const float corr = m == -INFINITY ? 0.f : ex2(m - ms);
+        const float corr = m == -INFINITY ? 0.f : ex2((m - ms) * unit);
         m = mx;
+        const float2 less = make_float2(-ms, -ms), by = make_float2(unit, unit), up = make_float2(kPShift, kPShift);
         uint32_t pa[KT / 2][4];
-        float sum = 0.f;
+        float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
         for (int x = 0; x < KT; ++x) {
-            const float p0 = ex2(sx[x][0] - ms + kPShift), p1 = ex2(sx[x][1] - ms + kPShift);
-            sum += p0 + p1;
-            split_half2(p0, p1, pa[x >> 1][2 * (x & 1)], pa[x >> 1][2 * (x & 1) + 1]);
+            const float2 e = ffma2(fadd2(sx[x], less), by, up), pr = make_float2(ex2(e.x), ex2(e.y));
+            sum = fadd2(sum, pr);
+            split_half2(pr.x, pr.y, pa[x >> 1][2 * (x & 1)], pa[x >> 1][2 * (x & 1) + 1]);
         }
-        l = fmaf(l, corr, sum);
+        l = fmaf(l, corr, sum.x + sum.y);
 
         // ---- P V: keys 2 c, + 1, + 8, + 9 of each 16, dims of column n ----
         uint32_t vw[kKeys4 / 4][VW];   // [k-step, + 8, second of the pair]
@@ -385,14 +414,15 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const Pools4& p
         for (int y = 0; y < 2 * VW; ++y) {   // four dims of the column
             float o[4][4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) o[k][0] = o[k][1] = o[k][2] = o[k][3] = 0.f;
-#pragma unroll
             for (int x = 0; x < KT; x += 2) {
                 uint32_t b0[4], b1[4];
                 code_pairs(prmt(vw[2 * x][y >> 1], vw[2 * x + 1][y >> 1], (y & 1) ? 0x7632u : 0x5410u), vd[x], b0);
                 code_pairs(prmt(vw[2 * x + 2][y >> 1], vw[2 * x + 3][y >> 1], (y & 1) ? 0x7632u : 0x5410u), vd[x + 1], b1);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) mma16816(o[k], pa[x >> 1], b0[k], b1[k]);
+                for (int k = 0; k < 4; ++k) {
+                    if (x == 0) mma16816_0(o[k], pa[0], b0[k], b1[k]);
+                    else mma16816(o[k], pa[x >> 1], b0[k], b1[k]);
+                }
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -411,7 +441,7 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const Pools4& p
     } else {
         const int64_t at_row = (static_cast<int64_t>(part) * S::warps + warp) * kRowTile + n;
         float* ml = A.part + S::cut_bytes / 4;
-        if (c == 0) *reinterpret_cast<float2*>(ml + at_row * 2) = make_float2(m, l);
+        if (c == 0) *reinterpret_cast<float2*>(ml + at_row * 2) = make_float2(m == -INFINITY ? m : m * unit, l);
         o = ml + S::part_rows(part_count(A.n_split, hg)) * 2 + at_row * HD;
     }
 #pragma unroll
