@@ -39,6 +39,7 @@ namespace hesa_cuda {
 namespace {
 
 constexpr int kKeys4 = 32;           // of a block
+constexpr int kCopyWarps4 = 4;
 constexpr int kSegCost4 = 3;         // blocks that starting a (tile, group) takes the time of
 constexpr int kScratchPage = 128;    // tokens of a page of the fp16 copy
 constexpr int64_t kScratchBytes = int64_t(1) << 30;
@@ -46,16 +47,21 @@ constexpr int64_t kScratchBytes = int64_t(1) << 30;
 // Rows of a sequence above which the chunk kernel takes over.
 constexpr int most_rows4(int head_dim) { return head_dim == 256 ? 48 : 16; }
 
+// 16 warps (8 with head_dim 256) and a warpgroup that copies. Registers a thread
+// after setmaxnreg: 512 x 112 + 128 x 32 = 640 x 96, and 256 x 232 + 128 x 40 = 384 x 168,
+// what the block is launched with.
 template <int HD> struct Rows4Shape : RowParts<HD, (HD == 256 ? 8 : 16)> {
     using RowParts<HD, (HD == 256 ? 8 : 16)>::warps;
-    static constexpr int threads = warps * 32;
+    static constexpr int threads = (warps + kCopyWarps4) * 32;
+    static constexpr int regs = HD == 256 ? 232 : 112, copy_regs = HD == 256 ? 40 : 32;
     static constexpr int groups = HD / kGroup;             // of a head: 16-byte pieces of a key's codes
     static constexpr int row = HD / 2, srow = groups * 2;  // bytes of a key's codes and scales
     static constexpr int v = kKeys4 * row, ks = 2 * v, vs = ks + kKeys4 * srow;   // K's codes, V's, then the scales
-    static constexpr int stage = vs + kKeys4 * srow;       // a warp's
-    static constexpr int stages = HD == 64 ? 4 : 2;
-    static constexpr int q = HD / 16 * 512;                // a warp's q: a k-step's operand is 16 bytes a lane
-    static constexpr size_t smem = static_cast<size_t>(stage * stages + q) * warps;
+    static constexpr int block = vs + kKeys4 * srow;       // bytes of a block of one head
+    static constexpr int depth = HD == 64 ? 4 : 2;         // blocks of a warp in the ring
+    static constexpr int q = HD / 16 * 512;                // a warp's q: a k-step's operand is 16 bytes a lane; also its sums
+    static constexpr size_t smem = static_cast<size_t>(block * depth + q) * warps;
+    static_assert(q == kRowTile * HD * 4, "a warp's sums fit where its q was");
 };
 
 // Where piece ch (16 bytes) of key j lies in a block. K: a thread (n, c) of a warp
@@ -76,12 +82,6 @@ template <int HD> __device__ __forceinline__ int v_at(int j, int ch) {
     if constexpr (HD == 256) ch ^= (r & 3) << 1;
     return r * (HD / 2) + ch * 16;
 }
-// In a loop over x, what v_at makes of key lane / groups + x * (32 / groups): that of x = 0 and a number of its own.
-template <int HD> __device__ __forceinline__ uint32_t v_step(uint32_t at0, int x) {
-    if constexpr (HD == 256) return ((x & 1) ? at0 ^ 64u : at0) + (x >> 1) * 8 * 128 + (x & 1) * 2 * 128;
-    return at0 + x * 512;   // 8 keys of 64 bytes, 16 of 32
-}
-
 __device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -90,8 +90,10 @@ template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t dst, co
     const int n = ok ? BYTES : 0;
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
 }
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// An arrival at `bar` once this thread's copies so far have landed
+__device__ __forceinline__ void copy_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
 
 // d = a b, in fp32 from zero
 __device__ __forceinline__ void mma16816_0(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -100,73 +102,75 @@ __device__ __forceinline__ void mma16816_0(float (&d)[4], const uint32_t (&a)[4]
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
-// A warp's way through its blocks of the CTA's run, ahead of the products.
-struct Ahead {
-    int64_t u, end;
-    int lo, i, i1, kvh;
-    int32_t len;
-    const int32_t* table;
-    KeyBlocks kb;
-    int32_t page;   // of key `lane` of block i; -1: none
-    bool any;       // there is a block i
+// The ring: `depth` blocks for each of the CTA's hg.subs sets of warps (one warp a
+// head), which take the blocks of a segment in turn. Block k of set x lies in place
+// x * depth + k % depth, as S::block bytes for each head.
+template <int HD> struct Ring4 {
+    uint8_t* smem;
+    uint64_t *full, *empty;   // [subs * depth]: 128 copying threads arrive at full, hg.heads warps at empty
+    uint32_t stage;           // bytes of a place
+    bool ok;                  // no wait has run out
+    __device__ __forceinline__ int place(int x, uint32_t k) const { return x * Rows4Shape<HD>::depth + k % Rows4Shape<HD>::depth; }
+    __device__ __forceinline__ uint32_t phase(uint32_t k) const { return (k / Rows4Shape<HD>::depth) & 1u; }
 };
 
-__device__ __forceinline__ int32_t page_of(const AttnArgs& A, const Ahead& h) {
-    const int32_t j = h.kb.at(h.i) * kKeys4 + (threadIdx.x & 31);
-    return j < h.len ? h.table[A.c.page_div.div(j)] : -1;
-}
-
-// The next segment with a block for this warp, if i has come to the end of one.
-__device__ __forceinline__ void go_on(const AttnArgs& A, const HeadGroups& hg, const int64_t* pre, int sub, int hl, Ahead& h) {
-    while (h.i >= h.i1) {
-        Segment seg;
-        if (!next_segment(pre, hg, h.u, h.end, h.lo, seg)) {
-            h.any = false;
-            return;
-        }
-        h.kvh = seg.grp * hg.heads + hl;
-        if (h.kvh >= A.c.n_kv) continue;
-        const TileView tv = tile_view<kKeys4>(A, seg.tile);
-        h.i = seg.b0 + sub;
-        h.i1 = min(tv.kb.n, seg.b1);
-        h.len = tv.sv.len;
-        h.table = A.c.table + static_cast<int64_t>(tv.sv.slot) * A.c.max_pages;
-        h.kb = tv.kb;
-    }
-    h.page = page_of(A, h);
-}
-
-// Block h.i into a stage, and h to the block after it. One group of copies, empty
-// where there is none. Where there is no key, or no page, the scales are zeros and
-// the codes any.
+// Copying warp pw: keys 8 pw .. 8 pw + 7 of every block of a segment, for all heads of the group. Lane x has `used`, the
+// blocks of set x so far. Where there is no key, or no page, the scales are zeros and the codes any.
 template <int HD>
-__device__ __forceinline__ void copy_block(const AttnArgs& A, const Pools4& pools, const HeadGroups& hg, const int64_t* pre, int sub, int hl, uint32_t stage,
-                                           Ahead& h) {
+__device__ __forceinline__ void copy_segment4(const AttnArgs& A, const Pools4& pools, const HeadGroups& hg, Ring4<HD>& ring, const Segment& seg, int pw,
+                                              uint32_t& used) {
     using S = Rows4Shape<HD>;
-    if (h.any) {
-        const int lane = threadIdx.x & 31;
-        const int32_t j = h.kb.at(h.i) * kKeys4 + lane;
-        const bool good = h.page >= 0 && h.page < A.c.n_pages;
-        if (!good && j < h.len) record_status(A.status, kStatusBadPosition);
-        // of this lane's key
-        int64_t at = static_cast<int64_t>(((j - A.c.page_div.div(j) * A.c.page_size) * A.c.n_kv + h.kvh) * S::groups) + h.page * A.c.page_stride;
+    const int lane = threadIdx.x & 31, h0 = seg.grp * hg.heads, heads = min(hg.heads, A.c.n_kv - h0);
+    const TileView tv = tile_view<kKeys4>(A, seg.tile);
+    const int i1 = min(tv.kb.n, seg.b1);
+    const int32_t* table = A.c.table + static_cast<int64_t>(tv.sv.slot) * A.c.max_pages;
+    const int my_key = pw * 8 + (lane & 7);   // whose place this lane looks up
+    auto page_of = [&](int i) {
+        const int32_t j = tv.kb.at(i) * kKeys4 + my_key;
+        return j < tv.sv.len ? table[A.c.page_div.div(j)] : -1;
+    };
+    int32_t page = seg.b0 < i1 ? page_of(seg.b0) : -1;
+    for (int i = seg.b0; i < i1; ++i) {
+        const int x = (i - seg.b0) & (hg.subs - 1);
+        const uint32_t k = __shfl_sync(0xffffffffu, used, x);
+        const int at_place = ring.place(x, k);
+        const int32_t j = tv.kb.at(i) * kKeys4 + my_key;
+        const bool good = page >= 0 && page < A.c.n_pages;
+        if (!good && j < tv.sv.len) record_status(A.status, kStatusBadPosition);
+        int64_t at = static_cast<int64_t>(((j - A.c.page_div.div(j) * A.c.page_size) * A.c.n_kv + h0) * S::groups) + page * A.c.page_stride;
         if (!good) at = 0;
-        copy_async<S::srow>(stage + S::ks + lane * S::srow, pools.ks + at, good);
-        copy_async<S::srow>(stage + S::vs + lane * S::srow, pools.vs + at, good);
-        const int ch = lane % S::groups, key = lane / S::groups;
-        const uint32_t kd = stage + k_at<HD>(key, ch), vd = stage + S::v + v_at<HD>(key, ch);
-        const uint4 *const kp = pools.k + ch, *const vp = pools.v + ch;
+        const unsigned goods = __ballot_sync(0xffffffffu, good);
+        if (i + 1 < i1) page = page_of(i + 1);   // on its way meanwhile
+        if (k >= S::depth && ring.ok) ring.ok = mbar_warp_wait(&ring.empty[at_place], ring.phase(k) ^ 1u, A.status, kStatusWaitTimeout);
+        if (!ring.ok) return;
+        const uint32_t to = smem_addr(ring.smem) + at_place * ring.stage;
+        // codes: a lane takes 16 bytes of a key's row
+        for (int u0 = 0; u0 < heads * S::groups; u0 += 32) {
+            const int u = u0 + lane;
+            const bool some = u < heads * S::groups;
+            const uint32_t head = to + u / S::groups * S::block;
+            const uint4 *const kp = pools.k + u, *const vp = pools.v + u;
 #pragma unroll
-        for (int x = 0; x < S::groups; ++x) {
-            const int64_t a = __shfl_sync(0xffffffffu, at, key + x * (32 / S::groups));
-            copy_async16(kd + x * 512, kp + a);   // 32 / groups keys of 16 * groups bytes
-            copy_async16(v_step<HD>(vd, x), vp + a);
+            for (int t = 0; t < 8; ++t) {
+                const int64_t a = __shfl_sync(0xffffffffu, at, t);
+                if (some) {
+                    copy_async16(head + pw * 8 * S::row + k_at<HD>(t, u % S::groups), kp + a);   // key 8 pw + t: eight keys on, the pattern is the same
+                    copy_async16(head + S::v + pw * 8 * S::row + v_at<HD>(t, u % S::groups), vp + a);
+                }
+            }
         }
-        h.i += hg.subs;
-        if (h.i < h.i1) h.page = page_of(A, h);
-        else go_on(A, hg, pre, sub, hl, h);
+        // scales: a lane takes a key's of one head, the lanes eight keys of four heads
+        const int64_t mine = __shfl_sync(0xffffffffu, at, lane & 7);
+        const bool there = (goods >> (lane & 7)) & 1u;
+        for (int h = lane >> 3; h < heads; h += 4) {
+            const int64_t from = mine + h * S::groups;   // of a place that is there, or of the first page
+            const uint32_t head = to + h * S::block + my_key * S::srow;
+            copy_async<S::srow>(head + S::ks, pools.ks + from, there);
+            copy_async<S::srow>(head + S::vs, pools.vs + from, there);
+        }
+        copy_arrive(&ring.full[at_place]);
+        if (lane == x) ++used;
     }
-    copy_commit();
 }
 
 __device__ __forceinline__ uint32_t lds32(uint32_t a) {
@@ -195,12 +199,13 @@ __device__ __forceinline__ uint32_t lds16(uint32_t a) {
 __device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
 __device__ __forceinline__ __half2 half2_of(uint32_t x) { return as_half2(prmt(x, x, 0x1010u)); }
 
-// This warp's head's attention over its blocks of a segment. part < 0: they are
-// all that the rows see, and the result goes to out; else (m, l, acc) go to that
-// part. `at`: stages used so far.
+// This warp's head's attention over its blocks of a segment; the first of the
+// head's warps adds up what they have. part < 0: these are all blocks that the rows
+// see, and the result goes to out; else (m, l, acc) go to that part. `used`: blocks
+// of the warp's set so far.
 template <int HD>
-__device__ __forceinline__ void rows4_segment(const AttnArgs& A, const Pools4& pools, const HeadGroups& hg, const int64_t* pre, uint8_t* ring, Ahead& ahead,
-                                              uint32_t& at, const Segment& seg, const TileView& tv, int part) {
+__device__ __forceinline__ void rows4_segment(const AttnArgs& A, const HeadGroups& hg, Ring4<HD>& ring, uint32_t& used, uint8_t* own, float2 (*s_ml)[kRowTile],
+                                              const Segment& seg, const TileView& tv, int part) {
     using S = Rows4Shape<HD>;
     constexpr int KW = HD / 32;                  // words of codes of a key's quarter: two k-steps of Q K^T each
     constexpr int VW = HD / 64;                  // words of codes of a column's dims
@@ -210,7 +215,16 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const Pools4& p
     const int sub = hg.sub_of(warp), hl = warp - sub * hg.heads, kvh = seg.grp * hg.heads + hl;
     const SeqView& sv = tv.sv;
     const Mask& mask = tv.mask;
-    if (sub >= hg.subs || kvh >= A.c.n_kv) return;
+    const int i1 = min(tv.kb.n, seg.b1);
+    if (kvh >= A.c.n_kv) {   // a head that the last group does not have: nothing but to keep the ring going
+        for (int i = seg.b0 + sub; i < i1; i += hg.subs, ++used) {
+            const int at = ring.place(sub, used);
+            if (ring.ok) ring.ok = mbar_warp_wait(&ring.full[at], ring.phase(used), A.status, kStatusWaitTimeout);
+            if (!ring.ok) return;
+            if (lane == 0) mbar_arrive(&ring.empty[at]);
+        }
+        return;
+    }
 
     // this thread's row and position
     const int r = tv.r0 + n;
@@ -218,10 +232,11 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const Pools4& p
     const int rc = min(r, tv.n_rows - 1), t = A.group_div.div(rc), h = kvh * A.group + rc - t * A.group;
     const int32_t pos = tv.base + t;
     const RowKeys keys = mask.row(pos);
-    const int i1 = min(tv.kb.n, seg.b1);
+    // a block [j0, j0 + kKeys4) is seen by every row where it lies in [all_lo, all_hi) or before the prefix's end
+    const int32_t all_hi = min(mask.len, tv.p_lo + 1), all_lo = mask.window > 0 ? tv.p_hi - mask.window + 1 : 0;
 
     // ---- q as hi and lo halves of q * 2^-e, max |q| 2^-e in [2^14, 2^15), in the order of the codes' pairs ----
-    const uint32_t qs = smem_addr(ring) + S::stage * S::stages + lane * 16;
+    const uint32_t qs = smem_addr(own) + lane * 16;
     float qscale;   // 2^e; NaN for a row that is not finite
     {
         const float* q = A.q + static_cast<int64_t>(sv.q0 + t) * A.ldq + static_cast<int64_t>(h) * HD;
@@ -270,12 +285,12 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const Pools4& p
     for (int i = 0; i < NT; ++i) acc[i] = make_float2(0.f, 0.f);
     const int vg = n * HD / 256;   // the group of this thread's column's dims
 
-    for (int i = seg.b0 + sub; i < i1; i += hg.subs, ++at) {
-        copy_wait<S::stages - 2>();
-        __syncwarp();   // the block has landed for every lane, and the one before it has been read
-        const uint32_t base = smem_addr(ring);
-        copy_block<HD>(A, pools, hg, pre, sub, hl, base + (at + S::stages - 1) % S::stages * S::stage, ahead);
-        const uint32_t st = base + at % S::stages * S::stage;
+    for (int i = seg.b0 + sub; i < i1; i += hg.subs, ++used) {
+        const int at = ring.place(sub, used);
+        if (ring.ok) ring.ok = mbar_warp_wait(&ring.full[at], ring.phase(used), A.status, kStatusWaitTimeout);
+        if (!ring.ok) break;
+        uint8_t* const block = ring.smem + at * ring.stage + hl * S::block;
+        const uint32_t st = smem_addr(block);
         const int32_t j0 = tv.kb.at(i) * kKeys4;
 
         // ---- scores of keys 8 x + 2 c, + 1 ----
@@ -336,7 +351,7 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const Pools4& p
                 sx[x].y -= slope2 * fabsf(static_cast<float>(pos - (jc + 8 * x + 1)));
             }
         }
-        if (!mask.all(tv.p_lo, tv.p_hi, j0, j0 + kKeys4)) {
+        if (!((j0 >= all_lo && j0 + kKeys4 <= all_hi) || j0 + kKeys4 <= mask.prefix)) {
 #pragma unroll
             for (int x = 0; x < KT; ++x) {
                 if (!keys.sees(jc + 8 * x)) sx[x].x = -INFINITY;
@@ -349,7 +364,7 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const Pools4& p
 #pragma unroll
             for (int x = 0; x < S::srow / 4; ++x) odd |= nonfinite_mark(lds32(st + S::vs + lane * S::srow + 4 * x));
             if (__any_sync(0xffffffffu, (odd & kNonfinite) != 0)) {
-                __half* vs = reinterpret_cast<__half*>(ring + at % S::stages * S::stage + S::vs);
+                __half* vs = reinterpret_cast<__half*>(block + S::vs);
                 for (int j = 0; j < kKeys4; ++j) {
                     if (!keys.sees(j0 + j)) continue;
 #pragma unroll
@@ -429,9 +444,44 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const Pools4& p
                 acc[4 * y + k] = ffma2(acc[4 * y + k], make_float2(corr, corr), fadd2(make_float2(o[k][0], o[k][1]), make_float2(o[k][2], o[k][3])));
             }
         }
+        __syncwarp();   // every lane has read the block
+        if (lane == 0) mbar_arrive(&ring.empty[at]);
     }
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
+    m = m == -INFINITY ? m : m * unit;
+    if (hg.subs > 1) {
+        // the other warps' sums in the place of their q, 16 bytes a lane at a time
+        float4* mine = reinterpret_cast<float4*>(own) + lane;
+        if (sub > 0) {
+#pragma unroll
+            for (int x = 0; x < NT; x += 2) mine[x * 16] = make_float4(acc[x].x, acc[x].y, acc[x + 1].x, acc[x + 1].y);
+            if (c == 0) s_ml[warp][n] = make_float2(m, l);
+        }
+        named_barrier(1 + hl, hg.subs * 32);
+        if (sub == 0) {
+            for (int y = 1; y < hg.subs; ++y) {
+                const int w = y * hg.heads + hl;
+                const float2 ml = s_ml[w][n];
+                const float4* theirs = mine + (w - hl) * (S::q / 16);
+                const float top = fmaxf(m, ml.x);
+                // a part that saw nothing adds zeros, or the NaN of a row that is not finite
+                const float f0 = m == -INFINITY ? 1.f : ex2(m - top), f1 = ml.x == -INFINITY ? 1.f : ex2(ml.x - top);
+                m = top;
+                l = fmaf(l, f0, ml.y * f1);
+                const float2 g0 = make_float2(f0, f0), g1 = make_float2(f1, f1);
+#pragma unroll
+                for (int x = 0; x < NT; x += 2) {
+                    const float4 v = theirs[x * 16];
+                    const float2 z = make_float2(0.f, 0.f);
+                    acc[x] = ffma2(make_float2(v.x, v.y), g1, ffma2(acc[x], g0, z));
+                    acc[x + 1] = ffma2(make_float2(v.z, v.w), g1, ffma2(acc[x + 1], g0, z));
+                }
+            }
+        }
+        named_barrier(1 + hl, hg.subs * 32);   // read: q may be written again
+        if (sub > 0) return;
+    }
     if (!row_ok) return;
     float* o;
     float inv = 1.f;
@@ -439,10 +489,10 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const Pools4& p
         o = A.out + static_cast<int64_t>(sv.q0 + t) * A.ldo + static_cast<int64_t>(h) * HD;
         inv = l == 0.f ? 0.f : 1.f / l;   // nothing seen: zeros
     } else {
-        const int64_t at_row = (static_cast<int64_t>(part) * S::warps + warp) * kRowTile + n;
+        const int64_t at_row = (static_cast<int64_t>(part) * S::warps + hl) * kRowTile + n;
         float* ml = A.part + S::cut_bytes / 4;
-        if (c == 0) *reinterpret_cast<float2*>(ml + at_row * 2) = make_float2(m == -INFINITY ? m : m * unit, l);
-        o = ml + S::part_rows(part_count(A.n_split, hg)) * 2 + at_row * HD;
+        if (c == 0) *reinterpret_cast<float2*>(ml + at_row * 2) = make_float2(m, l);
+        o = ml + S::part_rows(2 * kRowsCtas) * 2 + at_row * HD;
     }
 #pragma unroll
     for (int x = 0; x < NT; x += 4) {
@@ -451,20 +501,32 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const Pools4& p
     }
 }
 
+// hg: heads and sets of warps. What is added up later has one part a head (its warps have added up theirs), as if one
+// warp had it: `whole`.
 template <int HD>
 __global__ void __launch_bounds__(Rows4Shape<HD>::threads, 1)
-rows4_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ Pools4 pools, const __grid_constant__ HeadGroups hg) {
+rows4_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ Pools4 pools, const __grid_constant__ HeadGroups hg,
+             const __grid_constant__ HeadGroups whole) {
     using S = Rows4Shape<HD>;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int64_t s_pre[kMostTiles + 1];
-    __shared__ int64_t s_sum[S::warps];
+    __shared__ int64_t s_sum[S::warps + kCopyWarps4];
+    __shared__ __align__(8) uint64_t s_full[S::warps * S::depth], s_empty[S::warps * S::depth];
+    __shared__ float2 s_ml[S::warps][kRowTile];
     const int warp = threadIdx.x >> 5, tiles = A.n_split, cta = blockIdx.x;
-    if (threadIdx.x == 0) s_pre[0] = 0;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < hg.subs * S::depth; ++i) {
+            mbar_init(&s_full[i], kCopyWarps4 * 32);
+            mbar_init(&s_empty[i], hg.heads);
+        }
+        s_pre[0] = 0;
+        fence_mbar_init();
+    }
     grid_dep_wait();
     grid_dep_launch();   // combine_kernel may be set up meanwhile; it waits for this grid's end
-    const int64_t units = tile_units<S::warps, kKeys4>(A, hg, tiles, s_pre, s_sum) * hg.groups;
+    const int64_t units = tile_units<S::warps + kCopyWarps4, kKeys4>(A, hg, tiles, s_pre, s_sum) * hg.groups;
     const Runs runs(units, gridDim.x);
-    const bool listed_by_tile = by_tile(tiles, hg);
+    const bool listed_by_tile = by_tile(tiles, whole);
     Cut* cuts = reinterpret_cast<Cut*>(A.part);
     int64_t u = 0, end = 0;
     if (units > 0 && cta < runs.n_cta) {
@@ -473,36 +535,31 @@ rows4_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ Pools4 
     }
     const int64_t begin = u;
     int lo = tile_at(s_pre, hg, tiles, u);
-    if (listed_by_tile && cta == 0)   // those without rows
-        for (int i = threadIdx.x; i < tiles * hg.groups; i += S::threads)
-            if (s_pre[i / hg.groups + 1] == s_pre[i / hg.groups]) cuts[i] = Cut{};
-
-    const int sub = hg.sub_of(warp), hl = warp - sub * hg.heads;
-    uint8_t* ring = smem + static_cast<size_t>(warp) * (S::stage * S::stages + S::q);
-    Ahead ahead{};
-    ahead.u = u;
-    ahead.end = end;
-    ahead.lo = lo;
-    ahead.any = sub < hg.subs;
-    if (ahead.any) go_on(A, hg, s_pre, sub, hl, ahead);
-    for (int i = 0; i < S::stages - 1; ++i) copy_block<HD>(A, pools, hg, s_pre, sub, hl, smem_addr(ring) + i * S::stage, ahead);
-
-    uint32_t at = 0;
+    Ring4<HD> ring{smem + S::q * S::warps, s_full, s_empty, static_cast<uint32_t>(hg.heads * S::block), true};
     Segment seg;
+    if (warp >= S::warps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::copy_regs));
+        uint32_t used = 0;
+        while (ring.ok && next_segment(s_pre, hg, u, end, lo, seg)) copy_segment4<HD>(A, pools, hg, ring, seg, warp - S::warps, used);
+        asm volatile("cp.async.wait_all;" ::: "memory");   // nothing may be in flight when the CTA ends
+        return;
+    }
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::regs));
+    if (listed_by_tile && cta == 0)   // those without rows
+        for (int i = threadIdx.x; i < tiles * hg.groups; i += S::warps * 32)
+            if (s_pre[i / hg.groups + 1] == s_pre[i / hg.groups]) cuts[i] = Cut{};
+    const int sub = hg.sub_of(warp);
+    uint32_t used = 0;
     Cut cut{};
     while (next_segment(s_pre, hg, u, end, lo, seg)) {
         const int c_first = runs.cta_of(seg.first + hg.cost), c_last = runs.cta_of(seg.first + seg.units - 1);
-        const bool uncut = c_first == c_last;
-        const int own_part = 2 * kRowsCtas + seg.tile * hg.groups + seg.grp;   // of what several warps share, uncut
         const TileView tv = tile_view<kKeys4>(A, seg.tile);
-        const Cut all{seg.grp, uncut ? own_part : 2 * c_first + (runs.start(c_first) >= seg.first ? 0 : 1), c_last - c_first + 1,
-                      min(kRowTile, tv.n_rows - tv.r0), tv.r0, tv.sv.q0};
+        const Cut all{seg.grp, 2 * c_first + (runs.start(c_first) >= seg.first ? 0 : 1), c_last - c_first + 1, min(kRowTile, tv.n_rows - tv.r0), tv.r0, tv.sv.q0};
         if (cta == c_first + 1) cut = all;
         if (listed_by_tile && cta == c_first && threadIdx.x == 0) cuts[seg.tile * hg.groups + seg.grp] = all;
-        rows4_segment<HD>(A, pools, hg, s_pre, ring, ahead, at, seg, tv, !uncut ? 2 * cta + (begin >= seg.first ? 0 : 1) : hg.subs > 1 ? own_part : -1);
+        if (sub < hg.subs) rows4_segment<HD>(A, hg, ring, used, smem + warp * S::q, s_ml, seg, tv, c_first == c_last ? -1 : 2 * cta + (begin >= seg.first ? 0 : 1));
     }
     if (!listed_by_tile && threadIdx.x == 0) cuts[cta] = cut;
-    copy_wait<0>();   // nothing may be in flight when the CTA ends
 }
 
 // ---- chunks: a cache of fp16 pages, sequence i in slot i ----
@@ -642,9 +699,15 @@ hesa_cuda_paged_kv scratch_kv(const hesa_cuda_paged_kv4* kv, const Plan4& p, uin
     return s;
 }
 
-size_t rows4_bytes(const Plan4& p, const hesa_cuda_paged_kv4* kv) {
-    const HeadGroups hg(kv->n_kv_head, warps4(kv->head_dim), p.heads, kSegCost4);
-    const int64_t parts = part_count(std::min(p.tiles, kMostTiles), hg);
+// As what is added up later sees them: a head's warps have added up theirs.
+HeadGroups one_warp_a_head(HeadGroups hg) {
+    hg.subs = 1;
+    hg.sub_bits = 0;
+    return hg;
+}
+
+size_t rows4_bytes(const hesa_cuda_paged_kv4* kv) {
+    const int64_t parts = 2 * kRowsCtas;
     return kv->head_dim == 64 ? Rows4Shape<64>::bytes(parts) : kv->head_dim == 128 ? Rows4Shape<128>::bytes(parts) : Rows4Shape<256>::bytes(parts);
 }
 
@@ -661,20 +724,18 @@ cudaError_t launch_rows4(AttnArgs a, const Pools4& pools, const Plan4& p, cudaSt
         if (e != cudaSuccess) return e;
         set[dev] = true;
     }
-    const HeadGroups hg(a.c.n_kv, S::warps, p.heads, kSegCost4);
+    const HeadGroups hg(a.c.n_kv, S::warps, p.heads, kSegCost4), whole = one_warp_a_head(hg);
     for (a.tile0 = 0; a.tile0 < p.tiles && e == cudaSuccess; a.tile0 += kMostTiles) {
         a.n_split = std::min(kMostTiles, p.tiles - a.tile0);
-        e = launch_dep(rows4_kernel<HD>, dim3(kRowsCtas), S::threads, S::smem, s, a, pools, hg);
-        const int cuts = by_tile(a.n_split, hg) ? a.n_split * hg.groups : kRowsCtas;
+        e = launch_dep(rows4_kernel<HD>, dim3(kRowsCtas), S::threads, S::smem, s, a, pools, hg, whole);
+        const int cuts = by_tile(a.n_split, whole) ? a.n_split * hg.groups : kRowsCtas;
         const int rows = std::min(kRowTile, a.b.max_new * a.group);
         const unsigned z = static_cast<int64_t>(cuts) * hg.heads * rows <= 8 * kRowsCtas ? rows : 1;
         if (e == cudaSuccess)
-            e = launch_dep(combine_kernel<HD, S::warps>, dim3(static_cast<unsigned>(cuts), static_cast<unsigned>(hg.heads), z), 256, 0, s, a, hg);
+            e = launch_dep(combine_kernel<HD, S::warps>, dim3(static_cast<unsigned>(cuts), static_cast<unsigned>(hg.heads), z), 256, 0, s, a, whole);
     }
     return e;
 }
-
-bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 }  // namespace
 }  // namespace hesa_cuda
@@ -686,7 +747,7 @@ extern "C" {
 size_t hesa_cuda_paged_attention_kv4_workspace_size(const hesa_cuda_paged_kv4* kv, const hesa_cuda_token_batch* batch, int64_t n_head) {
     if (check_paged_kv4(kv) != HESA_CUDA_OK || check_batch4(kv, 0, batch, n_head) != HESA_CUDA_OK) return 0;
     const Plan4 p = make_plan4(kv, batch, n_head);
-    if (!p.chunk) return std::max<size_t>(rows4_bytes(p, kv), 16);
+    if (!p.chunk) return std::max<size_t>(rows4_bytes(kv), 16);
     const hesa_cuda_paged_kv s = scratch_kv(kv, p, reinterpret_cast<uint8_t*>(uintptr_t(16)));   // not looked into
     hesa_cuda_token_batch b = *batch;
     b.n_seq = p.n_seq;
