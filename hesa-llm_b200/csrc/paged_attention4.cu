@@ -82,13 +82,13 @@ template <int HD> __device__ __forceinline__ int v_at(int j, int ch) {
     if constexpr (HD == 256) ch ^= (r & 3) << 1;
     return r * (HD / 2) + ch * 16;
 }
-__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+// 16 bytes from global to shared memory, both addresses with a constant in the instruction
+template <int DST, int SRC> __device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0+%2], [%1+%3], 16;" ::"r"(dst), "l"(src), "n"(DST), "n"(SRC) : "memory");
 }
-// BYTES (4, 8 or 16) from global to shared memory, zeros where !ok
-template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool ok) {
-    const int n = ok ? BYTES : 0;
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
+// BYTES (4, 8 or 16), of which n come from src and the others are zeros
+template <int BYTES, int DST, int SRC> __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, int n) {
+    asm volatile("cp.async.ca.shared.global [%0+%4], [%1+%5], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n), "n"(DST), "n"(SRC) : "memory");
 }
 // An arrival at `bar` once this thread's copies so far have landed
 __device__ __forceinline__ void copy_arrive(uint64_t* bar) {
@@ -107,15 +107,42 @@ __device__ __forceinline__ void mma16816_0(float (&d)[4], const uint32_t (&a)[4]
 // x * depth + k % depth, as S::block bytes for each head.
 template <int HD> struct Ring4 {
     uint8_t* smem;
-    uint64_t *full, *empty;   // [subs * depth]: 128 copying threads arrive at full, hg.heads warps at empty
+    uint64_t *full, *empty;   // [subs * depth]: every copying thread arrives at full, hg.heads warps at empty
     uint32_t stage;           // bytes of a place
     bool ok;                  // no wait has run out
     __device__ __forceinline__ int place(int x, uint32_t k) const { return x * Rows4Shape<HD>::depth + k % Rows4Shape<HD>::depth; }
     __device__ __forceinline__ uint32_t phase(uint32_t k) const { return (k / Rows4Shape<HD>::depth) & 1u; }
 };
 
-// Copying warp pw: keys 8 pw .. 8 pw + 7 of every block of a segment, for all heads of the group. Lane x has `used`, the
-// blocks of set x so far. Where there is no key, or no page, the scales are zeros and the codes any.
+// Pieces Y, Y + 1, .. 3 of four, of K and V: piece l + 4 y of a key's row in the pools lies 64 y bytes on, in the ring
+// with the head that it is of.
+template <int HD, int Y = 0> __device__ __forceinline__ void copy_four(uint32_t k0, uint32_t k1, uint32_t v0, uint32_t v1, const uint4* kp, const uint4* vp, int n) {
+    using S = Rows4Shape<HD>;
+    if constexpr (Y < 4) {
+        constexpr int head = (HD == 64 ? 2 * Y : HD == 128 ? Y : Y / 2) * S::block;
+        if (Y < n) {
+            copy_async16<head, 64 * Y>(HD == 256 && (Y & 1) ? k1 : k0, kp);
+            copy_async16<head, 64 * Y>(HD == 256 && (Y & 1) ? v1 : v0, vp);
+        }
+        copy_four<HD, Y + 1>(k0, k1, v0, v1, kp, vp, n);
+    }
+}
+// The scales of heads l + 4 Y, .. of a key, up to four.
+template <int HD, int Y = 0> __device__ __forceinline__ void copy_scales(uint32_t to, const __half* kp, const __half* vp, int n, int heads) {
+    using S = Rows4Shape<HD>;
+    if constexpr (Y < 4) {
+        if (4 * Y < heads) {
+            copy_async<S::srow, 4 * Y * S::block + S::ks, 4 * Y * S::srow>(to, kp, n);
+            copy_async<S::srow, 4 * Y * S::block + S::vs, 4 * Y * S::srow>(to, vp, n);
+            copy_scales<HD, Y + 1>(to, kp, vp, n, heads);
+        }
+    }
+}
+
+// Copying warp pw: eight keys of every block of a segment, for all heads of the group;
+// four lanes a key, so that a copy's addresses are a lane's own plus constants. Lane x
+// has `used`, the blocks of set x so far. Where there is no key, or no page, the scales
+// are zeros and the codes any.
 template <int HD>
 __device__ __forceinline__ void copy_segment4(const AttnArgs& A, const Pools4& pools, const HeadGroups& hg, Ring4<HD>& ring, const Segment& seg, int pw,
                                               uint32_t& used) {
@@ -124,50 +151,38 @@ __device__ __forceinline__ void copy_segment4(const AttnArgs& A, const Pools4& p
     const TileView tv = tile_view<kKeys4>(A, seg.tile);
     const int i1 = min(tv.kb.n, seg.b1);
     const int32_t* table = A.c.table + static_cast<int64_t>(tv.sv.slot) * A.c.max_pages;
-    const int my_key = pw * 8 + (lane & 7);   // whose place this lane looks up
+    const int key = pw * 8 + (lane >> 2), l = lane & 3;
     auto page_of = [&](int i) {
-        const int32_t j = tv.kb.at(i) * kKeys4 + my_key;
+        const int32_t j = tv.kb.at(i) * kKeys4 + key;
         return j < tv.sv.len ? table[A.c.page_div.div(j)] : -1;
     };
     int32_t page = seg.b0 < i1 ? page_of(seg.b0) : -1;
+    // this lane's pieces of a row, l, l + 4, ..: with head_dim 64 and an odd head left over, lanes 2 and 3 have one less
+    const int pieces = (heads * S::groups + 3 - l) / 4;
+    const int my_heads = heads - l;   // scales of heads l, l + 4, ..
+    const uint32_t base = smem_addr(ring.smem) + (HD == 64 ? l / 2 * S::block : 0);
+    const uint32_t k0 = base + k_at<HD>(key, l % S::groups), v0 = base + S::v + v_at<HD>(key, l % S::groups);
+    const uint32_t k1 = HD == 256 ? base + k_at<HD>(key, l + 4) : 0, v1 = HD == 256 ? base + S::v + v_at<HD>(key, l + 4) : 0;
+    const uint32_t s0 = smem_addr(ring.smem) + l * S::block + key * S::srow;
+    constexpr int four = (HD == 64 ? 8 : HD == 128 ? 4 : 2) * S::block;   // four pieces on in the ring
     for (int i = seg.b0; i < i1; ++i) {
         const int x = (i - seg.b0) & (hg.subs - 1);
         const uint32_t k = __shfl_sync(0xffffffffu, used, x);
         const int at_place = ring.place(x, k);
-        const int32_t j = tv.kb.at(i) * kKeys4 + my_key;
+        const int32_t j = tv.kb.at(i) * kKeys4 + key;
         const bool good = page >= 0 && page < A.c.n_pages;
         if (!good && j < tv.sv.len) record_status(A.status, kStatusBadPosition);
         int64_t at = static_cast<int64_t>(((j - A.c.page_div.div(j) * A.c.page_size) * A.c.n_kv + h0) * S::groups) + page * A.c.page_stride;
         if (!good) at = 0;
-        const unsigned goods = __ballot_sync(0xffffffffu, good);
         if (i + 1 < i1) page = page_of(i + 1);   // on its way meanwhile
         if (k >= S::depth && ring.ok) ring.ok = mbar_warp_wait(&ring.empty[at_place], ring.phase(k) ^ 1u, A.status, kStatusWaitTimeout);
         if (!ring.ok) return;
-        const uint32_t to = smem_addr(ring.smem) + at_place * ring.stage;
-        // codes: a lane takes 16 bytes of a key's row
-        for (int u0 = 0; u0 < heads * S::groups; u0 += 32) {
-            const int u = u0 + lane;
-            const bool some = u < heads * S::groups;
-            const uint32_t head = to + u / S::groups * S::block;
-            const uint4 *const kp = pools.k + u, *const vp = pools.v + u;
-#pragma unroll
-            for (int t = 0; t < 8; ++t) {
-                const int64_t a = __shfl_sync(0xffffffffu, at, t);
-                if (some) {
-                    copy_async16(head + pw * 8 * S::row + k_at<HD>(t, u % S::groups), kp + a);   // key 8 pw + t: eight keys on, the pattern is the same
-                    copy_async16(head + S::v + pw * 8 * S::row + v_at<HD>(t, u % S::groups), vp + a);
-                }
-            }
-        }
-        // scales: a lane takes a key's of one head, the lanes eight keys of four heads
-        const int64_t mine = __shfl_sync(0xffffffffu, at, lane & 7);
-        const bool there = (goods >> (lane & 7)) & 1u;
-        for (int h = lane >> 3; h < heads; h += 4) {
-            const int64_t from = mine + h * S::groups;   // of a place that is there, or of the first page
-            const uint32_t head = to + h * S::block + my_key * S::srow;
-            copy_async<S::srow>(head + S::ks, pools.ks + from, there);
-            copy_async<S::srow>(head + S::vs, pools.vs + from, there);
-        }
+        uint32_t to = at_place * ring.stage;
+        copy_scales<HD>(s0 + to, pools.ks + at + l * S::groups, pools.vs + at + l * S::groups, good ? S::srow : 0, my_heads);
+        const uint4 *kp = pools.k + at + l, *vp = pools.v + at + l;
+        int y = pieces;
+        for (; y >= 4; y -= 4, to += four, kp += 16, vp += 16) copy_four<HD>(k0 + to, k1 + to, v0 + to, v1 + to, kp, vp, 4);
+        if (y > 0) copy_four<HD>(k0 + to, k1 + to, v0 + to, v1 + to, kp, vp, y);
         copy_arrive(&ring.full[at_place]);
         if (lane == x) ++used;
     }
