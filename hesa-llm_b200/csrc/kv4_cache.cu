@@ -167,7 +167,10 @@ rope_kv4_kernel(const PagedLayer c, const Pools4 pools, const BatchView b, float
     }
 }
 
-// A thread takes eight dims: a word of codes, 32 bytes of values.
+// A thread takes four dims, half a word of codes, so that a warp writes 512 bytes in
+// a row, of kReadAhead words at a time.
+constexpr int kReadAhead = 4;
+
 __global__ void __launch_bounds__(256)
 kv4_read_kernel(const PagedLayer c, const Pools4 pools, const BatchView b, float* k, int64_t ldk, float* v, int64_t ldv, int* status) {
     grid_dep_wait();
@@ -175,24 +178,36 @@ kv4_read_kernel(const PagedLayer c, const Pools4 pools, const BatchView b, float
     const int row = blockIdx.x;
     const Place at = place_of(c, b, row, status);
     if (!at.row) return;
-    const int words = c.n_kv * c.head_dim / 8;
-    for (int u = blockIdx.y * blockDim.x + threadIdx.x; u < 2 * words; u += gridDim.y * blockDim.x) {
-        const bool is_k = u < words;
-        const int w = is_k ? u : u - words;
-        float* o = is_k ? k : v;
-        if (!o) continue;
-        o += row * (is_k ? ldk : ldv) + static_cast<int64_t>(w) * 8;
-        float x[8];
+    const int quads = c.n_kv * c.head_dim / 4;
+    const int step = gridDim.y * blockDim.x;
+    for (int u0 = blockIdx.y * blockDim.x + threadIdx.x; u0 < 2 * quads; u0 += kReadAhead * step) {
+        uint32_t code[kReadAhead];
+        float d[kReadAhead];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = 0.f;
-        if (at.group >= 0) {
-            const uint32_t code = reinterpret_cast<const uint32_t*>((is_k ? pools.k : pools.v) + at.group)[w];
-            const float d = __half2float(((is_k ? pools.ks : pools.vs) + at.group)[w / 4]);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = d * static_cast<float>(static_cast<int>((code >> (4 * i)) & 15u) - 8);
+        for (int x = 0; x < kReadAhead; ++x) {
+            const int u = u0 + x * step;
+            const bool is_k = u < quads;
+            const int w = (is_k ? u : u - quads) / 2;
+            code[x] = 0x88888888u;
+            d[x] = 0.f;
+            if (u < 2 * quads && at.group >= 0 && (is_k ? k : v)) {
+                code[x] = __ldcs(reinterpret_cast<const uint32_t*>((is_k ? pools.k : pools.v) + at.group) + w);
+                d[x] = __half2float(((is_k ? pools.ks : pools.vs) + at.group)[w / 4]);
+            }
         }
-        *reinterpret_cast<float4*>(o) = *reinterpret_cast<float4*>(x);
-        *reinterpret_cast<float4*>(o + 4) = *reinterpret_cast<float4*>(x + 4);
+#pragma unroll
+        for (int x = 0; x < kReadAhead; ++x) {
+            const int u = u0 + x * step;
+            const bool is_k = u < quads;
+            float* o = is_k ? k : v;
+            if (u >= 2 * quads || !o) continue;
+            o += row * (is_k ? ldk : ldv) + static_cast<int64_t>(is_k ? u : u - quads) * 4;
+            const uint32_t four = code[x] >> ((u & 1) * 16);
+            float y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = d[x] * static_cast<float>(static_cast<int>((four >> (4 * i)) & 15u) - 8);
+            __stcs(reinterpret_cast<float4*>(o), make_float4(y[0], y[1], y[2], y[3]));
+        }
     }
 }
 
@@ -279,7 +294,7 @@ int hesa_cuda_kv4_read(const hesa_cuda_paged_kv4* kv, int32_t layer, const hesa_
     int* status = nullptr;
     cudaError_t e = status_word(&status);
     if (e == cudaSuccess) {
-        const int64_t units = 2 * width / 8;
+        const int64_t units = 2 * width / 4;
         const int64_t y = batch->n_tokens >= 148 * 4 ? 1 : std::min<int64_t>((units + 255) / 256, 1024);
         e = launch_dep(kv4_read_kernel, dim3(static_cast<unsigned>(batch->n_tokens), static_cast<unsigned>(y)), 256, 0, static_cast<cudaStream_t>(stream),
                        layer_of4(kv), pools_of(kv, layer), view_of(batch), k, ldk, v, ldv, status);

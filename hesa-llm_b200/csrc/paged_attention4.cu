@@ -587,13 +587,14 @@ struct Scratch {
     int32_t pages;
 };
 
-// Blocks x of gridDim.x share out one sequence's tokens that its rows see, kExpandTokens
-// at a time, and write the sequence's entries of the tables. A thread takes a word
-// of codes (16 bytes of fp16) of K or V at a time, four of them under way.
-constexpr int kExpandTokens = 8;
+// Blocks x of gridDim.x share out one sequence's tokens that its rows see, `tokens`
+// (at most 16) at a time, and write the sequence's entries of the tables. A thread
+// takes a word of codes (16 bytes of fp16) of K or V at a time, eight of them under way.
+constexpr int kExpandWords = 8;
+constexpr int kExpandTokens = 16;
 
 __global__ void __launch_bounds__(256)
-expand_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ Pools4 pools, const __grid_constant__ Scratch w, const FastDiv words_div) {
+expand_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ Pools4 pools, const __grid_constant__ Scratch w, const FastDiv words_div, int tokens) {
     __shared__ int64_t s_from[kExpandTokens];   // first group of the token's K, -1: no page
     grid_dep_wait();
     grid_dep_launch();
@@ -608,8 +609,8 @@ expand_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ Pools4
     const int row_words = A.c.n_kv * A.c.head_dim / 8;
     const int32_t* table = A.c.table + static_cast<int64_t>(sv.slot) * A.c.max_pages;
     const int64_t base = static_cast<int64_t>(seq) * w.pages * kScratchPage;
-    for (int32_t j0 = blockIdx.x * kExpandTokens; j0 < sv.len; j0 += gridDim.x * kExpandTokens) {
-        const int n = min(kExpandTokens, sv.len - j0);
+    for (int64_t start = static_cast<int64_t>(blockIdx.x) * tokens; start < sv.len; start += static_cast<int64_t>(gridDim.x) * tokens) {
+        const int j0 = static_cast<int>(start), n = min(tokens, sv.len - j0);
         if (j0 + n <= first && j0 >= prefix) continue;
         __syncthreads();
         if (static_cast<int>(threadIdx.x) < n) {
@@ -622,31 +623,31 @@ expand_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ Pools4
         }
         __syncthreads();
         const int all = n * 2 * row_words;
-        for (int u0 = threadIdx.x; u0 < all; u0 += 4 * blockDim.x) {
-            uint32_t code[4];
-            __half d[4];
-            uint4* to[4];
+        for (int u0 = threadIdx.x; u0 < all; u0 += kExpandWords * blockDim.x) {
+            uint32_t code[kExpandWords];
+            __half d[kExpandWords];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
+            for (int x = 0; x < kExpandWords; ++x) {
                 const int u = u0 + x * static_cast<int>(blockDim.x);
                 if (u >= all) break;
-                const int half = words_div.div(u), t = half >> 1, at = u - half * row_words;   // K, then V of each token
-                const bool is_k = !(half & 1);
-                const int64_t from = s_from[t];
+                const int half = words_div.div(u), at = u - half * row_words;   // K, then V of each token
+                const int64_t from = s_from[half >> 1];
                 code[x] = 0x88888888u;
-                d[x] = __half(__float2half_rn(0.f));
+                d[x] = __float2half_rn(0.f);
                 if (from >= 0) {
-                    code[x] = __ldcs(reinterpret_cast<const uint32_t*>((is_k ? pools.k : pools.v) + from) + at);
-                    d[x] = ((is_k ? pools.ks : pools.vs) + from)[at / 4];
+                    code[x] = __ldcs(reinterpret_cast<const uint32_t*>((half & 1 ? pools.v : pools.k) + from) + at);
+                    d[x] = ((half & 1 ? pools.vs : pools.ks) + from)[at / 4];
                 }
-                to[x] = reinterpret_cast<uint4*>(is_k ? w.k : w.v) + (base + j0 + t) * row_words + at;
             }
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                if (u0 + x * static_cast<int>(blockDim.x) >= all) break;
+            for (int x = 0; x < kExpandWords; ++x) {
+                const int u = u0 + x * static_cast<int>(blockDim.x);
+                if (u >= all) break;
+                const int half = words_div.div(u), at = u - half * row_words;
                 uint32_t p[4];
                 code_pairs(code[x], __half2half2(d[x]), p);   // (0, 4) (1, 5) (2, 6) (3, 7)
-                *to[x] = make_uint4(prmt(p[0], p[1], 0x5410u), prmt(p[2], p[3], 0x5410u), prmt(p[0], p[1], 0x7632u), prmt(p[2], p[3], 0x7632u));
+                reinterpret_cast<uint4*>(half & 1 ? w.v : w.k)[(base + j0 + (half >> 1)) * row_words + at] =
+                    make_uint4(prmt(p[0], p[1], 0x5410u), prmt(p[2], p[3], 0x5410u), prmt(p[0], p[1], 0x7632u), prmt(p[2], p[3], 0x7632u));
             }
         }
     }
@@ -815,10 +816,11 @@ int hesa_cuda_paged_attention_kv4(const hesa_cuda_paged_kv4* kv, int32_t layer, 
             }
             o.prefix = options && options->prefix ? options->prefix + i : nullptr;
             a.prefix = o.prefix;
-            // blocks for every SM, as far as the sequences have tokens for them
-            const int share = std::max(1, std::min((batch->max_len + kExpandTokens - 1) / kExpandTokens, (148 * 16 + b.n_seq - 1) / b.n_seq));
+            // as many tokens a block as its threads have words under way for; blocks for every SM, as far as there are tokens for them
+            const int row_words = kv->n_kv_head * kv->head_dim / 8, tokens = std::max(1, std::min(kExpandTokens, kExpandWords * 256 / (2 * row_words)));
+            const int share = std::max(1, std::min((batch->max_len + tokens - 1) / tokens, (148 * 16 + b.n_seq - 1) / b.n_seq));
             e = launch_dep(expand_kernel, dim3(static_cast<unsigned>(share), static_cast<unsigned>(b.n_seq)), 256, 0, s, a, pools,
-                           Scratch{static_cast<__half*>(c.k), static_cast<__half*>(c.v), c.table, c.seq_len, p.pages}, FastDiv(kv->n_kv_head * kv->head_dim / 8));
+                           Scratch{static_cast<__half*>(c.k), static_cast<__half*>(c.v), c.table, c.seq_len, p.pages}, FastDiv(row_words), tokens);
             if (e != cudaSuccess) break;
             rc = hesa_cuda_paged_attention(&c, 0, &b, q, ldq, out, ldo, n_head, &o, ws + used, workspace_bytes - used, stream);
             if (rc != HESA_CUDA_OK) return rc;
