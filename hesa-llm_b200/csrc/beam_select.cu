@@ -89,15 +89,21 @@ beam_join_kernel(const float* scores, const int32_t* ended, int width, int vocab
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-            // the parts' lists joined: each descends, so the first key that is too small ends it
+            // the parts' lists joined: a lane has the heads of two of them (and what comes behind these on its way), the
+            // largest of all heads is the next one
             const unsigned long long* lists = reinterpret_cast<const unsigned long long*>(keys + r * n_split * top);
-            uint64_t best = lane < top ? __ldcg(lists + lane) : 0;
-            for (int l = 1; l < n_split; ++l) {
-                const uint64_t theirs = lane < top ? __ldcg(lists + static_cast<int64_t>(l) * top + lane) : 0;
-                for (int i = 0; i < top; ++i) {
-                    const uint64_t c = __shfl_sync(0xffffffffu, theirs, i);
-                    if (c <= __shfl_sync(0xffffffffu, best, top - 1)) break;
-                    insert(best, c, lane);
+            auto key_of = [&](int l, int i) -> uint64_t { return l < n_split && i < top ? __ldcg(lists + static_cast<int64_t>(l) * top + i) : 0; };
+            uint64_t head0 = key_of(lane, 0), head1 = key_of(lane + 32, 0), next0 = key_of(lane, 1), next1 = key_of(lane + 32, 1), best = 0;
+            int at0 = 1, at1 = 1;
+            for (int i = 0; i < top; ++i) {
+                const uint64_t c = warp_max_key(max_key(head0, head1));
+                if (lane == i) best = c;
+                if (head0 == c) {
+                    head0 = next0;
+                    next0 = key_of(lane, ++at0);
+                } else if (head1 == c) {
+                    head1 = next1;
+                    next1 = key_of(lane + 32, ++at1);
                 }
             }
             if (isfinite(z)) {
@@ -141,9 +147,12 @@ beam_join_kernel(const float* scores, const int32_t* ended, int width, int vocab
     }
 }
 
-// Parts of a row: about three blocks an SM, at least a quad for each thread a block.
+// Parts of a row: blocks enough that the SMs end together though some beams have ended, at least a quad for each thread a block.
+#ifndef WANT
+#define WANT 12
+#endif
 int parts_of(int64_t n_rows, int64_t vocab) {
-    const int64_t want = std::max<int64_t>(1, 148 * 3 / n_rows), most = std::max<int64_t>(1, vocab / (4 * kLpThreads));
+    const int64_t want = (148 * WANT + n_rows - 1) / n_rows, most = std::max<int64_t>(1, vocab / (4 * kLpThreads));
     return static_cast<int>(std::min(std::min(want, most), static_cast<int64_t>(kMostParts)));
 }
 

@@ -279,25 +279,58 @@ fork_plan_kernel(const Tables t, const int32_t* src, const int32_t* dst, int n, 
     if (threadIdx.x == 0) *w.n_items = n;
 }
 
-// Pages of the slots that no slot takes over lose a reference each (by = -1), or get it back (by = 1); false where a
-// page had none left to take. A warp a group, lane b has slot b of it. All threads of the block; a barrier at its end.
-__device__ bool drop_refs(const Tables& t, const int32_t* slots, const int32_t* parents, int n, int width, int by) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// The pages of the listed slots, by what becomes of them. kDrop: those of slots that no
+// slot takes over lose a reference each; kGiveBack undoes that (what is not sound has
+// no reference changed); kKept: those of the other slots have references left. False
+// where a length or a page is not sound, or there is no reference to take or left.
+// A warp takes kSlotsAhead slots at a time, whose reads go side by side, its lanes
+// their pages. All threads of the block; a barrier at the end.
+enum Refs { kDrop, kGiveBack, kKept };
+constexpr int kSlotsAhead = 4;
+
+template <Refs MODE>
+__device__ bool slot_refs(const Tables& t, const int32_t* slots, const int32_t* parents, int n, int width) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, step = kPlanThreads / 32;
     bool bad = false;
-    for (int g = warp * width; g < n; g += kPlanThreads / 32 * width) {
-        const int par = lane < width ? parents[g + lane] : -1;
-        for (int b = 0; b < width; ++b) {
-            if (__any_sync(0xffffffffu, par == b)) continue;
-            const int slot = slots[g + b], np = pages_for(t.seq_len[slot], t.page_size);
-            for (int j = lane; j < np; j += 32) bad |= atomicAdd(&t.refs[t.table[static_cast<int64_t>(slot) * t.max_pages + j]], by) + by < 0;
+    auto look = [&](int p, bool mine) {
+        if (p < 0 || p >= t.n_pages) bad = true;
+        else if (!mine) return;
+        else if (MODE == kDrop) bad |= atomicAdd(&t.refs[p], -1) <= 0;
+        else if (MODE == kGiveBack) atomicAdd(&t.refs[p], 1);
+        else bad |= t.refs[p] <= 0;
+    };
+    for (int i0 = warp; i0 < n; i0 += kSlotsAhead * step) {
+        const int32_t* row[kSlotsAhead];
+        int np[kSlotsAhead], first[kSlotsAhead];
+        bool mine[kSlotsAhead];
+#pragma unroll
+        for (int k = 0; k < kSlotsAhead; ++k) {
+            const int i = i0 + k * step, b = i % width;
+            const int slot = i < n ? slots[i] : 0, par = i < n && lane < width ? parents[i - b + lane] : -1;
+            const int len = i < n ? t.seq_len[slot] : 0;
+            const bool ok = len >= 0 && len <= static_cast<int64_t>(t.max_pages) * t.page_size;
+            bad |= !ok;
+            np[k] = ok ? pages_for(len, t.page_size) : 0;
+            row[k] = t.table + static_cast<int64_t>(slot) * t.max_pages;
+            mine[k] = __any_sync(0xffffffffu, par == b) == (MODE == kKept);
+        }
+#pragma unroll
+        for (int k = 0; k < kSlotsAhead; ++k) first[k] = lane < np[k] ? row[k][lane] : 0;
+#pragma unroll
+        for (int k = 0; k < kSlotsAhead; ++k) {
+            if (lane < np[k]) look(first[k], mine[k]);
+            for (int j = lane + 32; j < np[k]; j += 32) look(row[k][j], mine[k]);
         }
     }
     return !__syncthreads_or(bad);
 }
 
 // Slot b of a group becomes what slot parents[b] of it was. References that go are taken first, so that the pages
-// they free can be taken for the copies, then those that come are added; the table's entries of a group are changed by
-// one warp, column by column, each lane holding an old entry of its slot when the first new one is written.
+// they free can be taken for the copies, then those that come are added. The table's entries of a group are changed by
+// one warp: a lane has one slot's in some columns, and a slot's new entries are the old ones of its parent's lane; a
+// column is read before it is written, by the same warp. Bound by latency: a chain of dependent reads in one block.
+constexpr int kColumnSteps = 8;   // reads of a row that a lane has under way
+
 __global__ void __launch_bounds__(kPlanThreads)
 reorder_plan_kernel(const Tables t, const int32_t* slots, const int32_t* parents, int n, int width, PageWork w) {
     grid_dep_wait();
@@ -307,9 +340,9 @@ reorder_plan_kernel(const Tables t, const int32_t* slots, const int32_t* parents
     if (threadIdx.x == 0) *w.n_items = 0;
     bool bad = !mark_slots(slots, n, t.n_slots, bits);
     for (int i = threadIdx.x; i < n && !bad; i += kPlanThreads) bad = parents[i] < 0 || parents[i] >= width;
-    if (__syncthreads_or(bad) || !slots_sound(t, slots, n)) return refuse(t, kStatusBadPosition);
-    if (!drop_refs(t, slots, parents, n, width, -1)) {
-        drop_refs(t, slots, parents, n, width, 1);
+    if (__syncthreads_or(bad)) return refuse(t, kStatusBadPosition);
+    if (!slot_refs<kDrop>(t, slots, parents, n, width) || !slot_refs<kKept>(t, slots, parents, n, width)) {
+        slot_refs<kGiveBack>(t, slots, parents, n, width);
         return refuse(t, kStatusBadPosition);
     }
     // a slot whose parent has a partly filled page and an earlier child gets a page of its own
@@ -328,11 +361,10 @@ reorder_plan_kernel(const Tables t, const int32_t* slots, const int32_t* parents
         total += all;
     }
     if (total > t.n_pages || !lowest_free(t, total, w.list, s)) {
-        __syncthreads();
-        drop_refs(t, slots, parents, n, width, 1);
+        slot_refs<kGiveBack>(t, slots, parents, n, width);
         return refuse(t, kStatusNoPages);
     }
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cols = 32 / width;   // columns of the table a warp has in hand
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cols = 32 / width;   // columns of the table a warp has in hand at a time
     const int beam = lane % width, col = lane / width;
     for (int g = warp * width; g < n; g += kPlanThreads / 32 * width) {
         const int par = parents[g + beam], slot = slots[g + beam];
@@ -345,16 +377,22 @@ reorder_plan_kernel(const Tables t, const int32_t* slots, const int32_t* parents
         int most = max(old_pages, pages);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-        for (int j0 = 0; j0 < most; j0 += cols) {
-            const int j = j0 + col;
-            const bool mine = col < cols && j < most;
-            const int old = mine && j < old_pages ? row[j] : -1;
-            const int from = __shfl_sync(0xffffffffu, old, col < cols ? col * width + par : lane);
-            if (mine) {
+        for (int j0 = 0; j0 < most; j0 += kColumnSteps * cols) {
+            int old[kColumnSteps];
+#pragma unroll
+            for (int k = 0; k < kColumnSteps; ++k) {
+                const int j = j0 + k * cols + col;
+                old[k] = col < cols && j < old_pages ? row[j] : -1;
+            }
+#pragma unroll
+            for (int k = 0; k < kColumnSteps; ++k) {
+                const int j = j0 + k * cols + col;
+                const int from = __shfl_sync(0xffffffffu, old[k], col < cols ? col * width + par : lane);
+                if (col >= cols || j >= most) continue;
                 if (j < pages) {
                     const bool copy = j == full && fresh >= 0;
                     const int now = copy ? fresh : from;
-                    if (now != old) row[j] = now;
+                    if (now != old[k]) row[j] = now;
                     if (copy) {
                         int32_t* item = w.items + 3 * static_cast<int64_t>(take);
                         item[0] = from;
@@ -362,11 +400,11 @@ reorder_plan_kernel(const Tables t, const int32_t* slots, const int32_t* parents
                         item[2] = len % t.page_size;
                         t.refs[fresh] = 1;
                     }
+                    if (later && j < full) atomicAdd(&t.refs[from], 1);   // for every child but the first
                 } else if (j < old_pages) {
                     row[j] = -1;
                 }
             }
-            if (mine && later && j < full) atomicAdd(&t.refs[from], 1);   // for every child but the first
         }
         __syncwarp();
         if (col == 0) t.seq_len[slot] = len;

@@ -13,6 +13,7 @@ constexpr int kLpThreads = 256;
 constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kMaxTop = 32;
 constexpr int kUnroll = 4;           // quads a thread has in flight
+constexpr int kAgain = 4;            // and when a few are read again
 
 constexpr float kLog2e = 1.44269504088896341f;
 
@@ -215,25 +216,35 @@ __device__ __forceinline__ Sums row_part(const float* row, int vocab, int split,
             const int f = f0 + warp < n_from ? sh.from[f0 + warp] : -1;
             const int base = q0 + (f >> 5) * 32 * kUnroll + (f & 31);
             const int n_mine = (q1 - q0 + kStep - 1) / kStep * kUnroll;   // quads of a thread at most
-            for (int i0 = 0; i0 < n_mine; i0 += 32) {
-                if (f >= 0 && i0 + lane < n_mine) {
-                    const int q = base + ((i0 + lane) / kUnroll) * kStep + ((i0 + lane) % kUnroll) * 32;
+            for (int i1 = 0; i1 < n_mine; i1 += 32 * kAgain) {
+                // their reads side by side
+                float4 v[kAgain];
+                int q[kAgain];
+#pragma unroll
+                for (int a = 0; a < kAgain; ++a) {
+                    const int i = i1 + a * 32 + lane;
+                    q[a] = f >= 0 && i < n_mine ? base + (i / kUnroll) * kStep + (i % kUnroll) * 32 : q1;
+                    v[a] = quad(q[a]);
+                }
+#pragma unroll
+                for (int a = 0; a < kAgain; ++a) {
+                    if (i1 + a * 32 >= n_mine) break;
                     uint64_t k[4];
-                    keys(q, quad(q), k);
+                    keys(q[a], v[a], k);
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         if (k[i] != 0 && k[i] >= bound) sh.cand[atomicAdd(&sh.n, 1)] = k[i];
-                }
-                __syncthreads();
-                // 1024 more may come: keep the k largest, the k-th is the new bound
-                const int n = sh.n;
-                __syncthreads();
-                if (n > kCand - 4 * kLpThreads) {
-                    select(sh.cand, n, top_k, sh.top);
-                    if (static_cast<int>(threadIdx.x) < top_k) sh.cand[threadIdx.x] = sh.top[threadIdx.x];
-                    bound = sh.top[top_k - 1];
-                    if (threadIdx.x == 0) sh.n = top_k;
                     __syncthreads();
+                    // 1024 more may come: keep the k largest, the k-th is the new bound
+                    const int n = sh.n;
+                    __syncthreads();
+                    if (n > kCand - 4 * kLpThreads) {
+                        select(sh.cand, n, top_k, sh.top);
+                        if (static_cast<int>(threadIdx.x) < top_k) sh.cand[threadIdx.x] = sh.top[threadIdx.x];
+                        bound = sh.top[top_k - 1];
+                        if (threadIdx.x == 0) sh.n = top_k;
+                        __syncthreads();
+                    }
                 }
             }
         }
