@@ -265,6 +265,37 @@ def test_reorder(H, kind, seed):
             assert torch.equal(p, want)
 
 
+def test_reorder_of_many_slots(H):
+    """More slots than the planning block has threads, groups that lie across its ends, pages beyond a thousand."""
+    r = random.Random(77)
+    for width, groups in ((7, 400), (32, 70), (1, 1500)):
+        n = width * groups
+        cache, pools, t, m = random_cache(H, r, "kv4", n, 4, layers=1, n_kv=1, most=23, spare=n)
+        slots = r.sample(range(n), n)
+        for step in range(2):
+            parents = [r.randrange(width) for _ in slots]
+            before = [p.clone() for p in pools]
+            copies = m.reorder(slots, parents, width)
+            assert copies is not None
+            H.kv_reorder(cache, torch.tensor(slots, dtype=torch.int32, device="cuda"), torch.tensor(parents, dtype=torch.int32, device="cuda"), width)
+            assert H.device_status() == 0
+            same_tables(t, m)
+            for p, b in zip(pools, before):
+                want = b.clone()
+                for frm, to, places in copies:
+                    want[:, to, :places] = b[:, frm, :places]
+                assert torch.equal(p, want)
+        # the last slot of all is not sound: nothing changes
+        kept = [x.clone() for x in t]
+        t[1][slots[-1]] = 10 ** 6
+        now = [x.clone() for x in t]
+        H.kv_reorder(cache, torch.tensor(slots, dtype=torch.int32, device="cuda"), torch.tensor(parents, dtype=torch.int32, device="cuda"), width)
+        assert H.device_status() == 3 and all(torch.equal(a, b) for a, b in zip(t, now))
+        H.clear_device_status()
+        for x, k in zip(t, kept):
+            x.copy_(k)
+
+
 @pytest.mark.parametrize("kind", ["fp16", "kv4"])
 def test_reorder_refusals_change_nothing(H, kind):
     r = random.Random(3)
