@@ -148,11 +148,8 @@ beam_join_kernel(const float* scores, const int32_t* ended, int width, int vocab
 }
 
 // Parts of a row: blocks enough that the SMs end together though some beams have ended, at least a quad for each thread a block.
-#ifndef WANT
-#define WANT 12
-#endif
 int parts_of(int64_t n_rows, int64_t vocab) {
-    const int64_t want = (148 * WANT + n_rows - 1) / n_rows, most = std::max<int64_t>(1, vocab / (4 * kLpThreads));
+    const int64_t want = (148 * 8 + n_rows - 1) / n_rows, most = std::max<int64_t>(1, vocab / (4 * kLpThreads));
     return static_cast<int>(std::min(std::min(want, most), static_cast<int64_t>(kMostParts)));
 }
 

@@ -341,7 +341,7 @@ rows_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ HeadGrou
     __shared__ int64_t s_pre[kMostTiles + 1];
     __shared__ int64_t s_sum[S::warps + kCopyWarps];
     __shared__ __align__(8) uint64_t s_full[S::stages], s_empty[S::stages];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tiles = A.n_split, cta = blockIdx.x;
+    const int warp = threadIdx.x >> 5, tiles = A.n_split, cta = blockIdx.x;
     // the arguments come into the constant cache while the previous kernel ends
     if (A.c.n_pages <= 0 || A.b.n_seq <= 0 || A.ldq <= 0 || A.group <= 0 || A.part == nullptr || hg.heads <= 0) return;
     if (threadIdx.x == 0) {

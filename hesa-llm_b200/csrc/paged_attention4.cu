@@ -40,7 +40,7 @@ namespace {
 
 constexpr int kKeys4 = 32;           // of a block
 constexpr int kCopyWarps4 = 4;
-constexpr int kSegCost4 = 3;         // blocks that starting a (tile, group) takes the time of
+constexpr int kSegCost4 = 2;         // blocks that starting a (tile, group) takes the time of
 constexpr int kScratchPage = 128;    // tokens of a page of the fp16 copy
 constexpr int64_t kScratchBytes = int64_t(1) << 30;
 
@@ -211,8 +211,7 @@ __device__ __forceinline__ uint32_t lds16(uint32_t a) {
     asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
     return v;
 }
-__device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
-__device__ __forceinline__ __half2 half2_of(uint32_t x) { return as_half2(prmt(x, x, 0x1010u)); }
+__device__ __forceinline__ __half2 half2_of(uint32_t x) { return half2_bits(prmt(x, x, 0x1010u)); }
 
 // This warp's head's attention over its blocks of a segment; the first of the
 // head's warps adds up what they have. part < 0: these are all blocks that the rows
@@ -416,7 +415,7 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const HeadGroup
 
         // ---- P V: keys 2 c, + 1, + 8, + 9 of each 16, dims of column n ----
         uint32_t vw[kKeys4 / 4][VW];   // [k-step, + 8, second of the pair]
-        __half2 vd[KT];
+        __half2 vd[KT], vm[KT];
 #pragma unroll
         for (int x = 0; x < KT; ++x) {
             uint32_t d16[2];
@@ -438,7 +437,8 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const HeadGroup
                 }
                 d16[k] = lds16(st + S::vs + key * S::srow + vg * 2);
             }
-            vd[x] = as_half2(prmt(d16[0], d16[1], 0x5410u));
+            vd[x] = half2_bits(prmt(d16[0], d16[1], 0x5410u));
+            vm[x] = __hmul2(vd[x], __float2half2_rn(-24.f));
         }
 #pragma unroll
         for (int y = 0; y < 2 * VW; ++y) {   // four dims of the column
@@ -446,8 +446,8 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const HeadGroup
 #pragma unroll
             for (int x = 0; x < KT; x += 2) {
                 uint32_t b0[4], b1[4];
-                code_pairs(prmt(vw[2 * x][y >> 1], vw[2 * x + 1][y >> 1], (y & 1) ? 0x7632u : 0x5410u), vd[x], b0);
-                code_pairs(prmt(vw[2 * x + 2][y >> 1], vw[2 * x + 3][y >> 1], (y & 1) ? 0x7632u : 0x5410u), vd[x + 1], b1);
+                code_pairs_fma(prmt(vw[2 * x][y >> 1], vw[2 * x + 1][y >> 1], (y & 1) ? 0x7632u : 0x5410u), vd[x], vm[x], b0);
+                code_pairs_fma(prmt(vw[2 * x + 2][y >> 1], vw[2 * x + 3][y >> 1], (y & 1) ? 0x7632u : 0x5410u), vd[x + 1], vm[x + 1], b1);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     if (x == 0) mma16816_0(o[k], pa[0], b0[k], b1[k]);
