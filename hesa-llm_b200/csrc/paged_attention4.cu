@@ -44,8 +44,13 @@ constexpr int kSegCost4 = 2;         // blocks that starting a (tile, group) tak
 constexpr int kScratchPage = 128;    // tokens of a page of the fp16 copy
 constexpr int64_t kScratchBytes = int64_t(1) << 30;
 
-// Rows of a sequence above which the chunk kernel takes over.
-constexpr int most_rows4(int head_dim) { return head_dim == 256 ? 48 : 16; }
+// Rows of a kv head and sequence above which the chunk kernel takes over, rather than
+// tiles of 8 that each read the codes again (of the chunk, the codes are read once,
+// and fp16 is written and read). Eight sequences of 4000 tokens, 64 heads on 8: 32 rows
+// 36 us in tiles, 61 as a chunk; 64 rows 57 and 65; 96 rows 93 and 72. Two of 60000: 64
+// rows 186 and 238, 96 rows 462 and 239. 16 heads of 256 on 4, eight of 4000: 64 rows 61
+// and 85, 128 rows 104 and 91. 32 heads of 64 on 8: 64 rows 37 and 46, 96 rows 59 and 50.
+constexpr int kMostRows4 = 64;
 
 // 16 warps (8 with head_dim 256) and a warpgroup that copies. Registers a thread
 // after setmaxnreg: 512 x 112 + 128 x 32 = 640 x 96, and 256 x 232 + 128 x 40 = 384 x 168,
@@ -667,7 +672,7 @@ Plan4 make_plan4(const hesa_cuda_paged_kv4* kv, const hesa_cuda_token_batch* b, 
     Plan4 p{};
     const int g = static_cast<int>(n_head / kv->n_kv_head);
     const int64_t rows_a_seq = static_cast<int64_t>(b->max_new) * g;
-    p.chunk = rows_a_seq > most_rows4(kv->head_dim);
+    p.chunk = rows_a_seq > kMostRows4;
     if (p.chunk) {
         p.pages = std::max(1, (b->max_len + kScratchPage - 1) / kScratchPage);
         const int64_t bytes = static_cast<int64_t>(p.pages) * kScratchPage * kv->n_kv_head * kv->head_dim * 4;

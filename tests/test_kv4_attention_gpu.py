@@ -44,6 +44,11 @@ def test_next_token(n_head, n_kv, hd, page, lens):
     (16, 4, 64, 24, [301, 7, 1000], [100, 7, 333]),
     (4, 2, 256, 16, [150, 90], [70, 90]),
     (6, 2, 64, 7, [130, 129, 128], [5, 3, 2]),
+    (6, 2, 64, 7, [130, 129, 128], [50, 3, 2]),
+    (32, 1, 128, 16, [300, 40], [1, 1]),               # 32 heads on one: four tiles of rows
+    (65, 1, 64, 16, [300, 1], [1, 1]),                 # and so many that they are a chunk
+    (2, 2, 256, 16, [700, 300], [64, 3]),              # the most rows that are tiles of eight
+    (2, 2, 256, 16, [700, 300], [65, 3]),
     (2, 2, 128, 5, [400], [8]),                        # eight new tokens are rows of one tile
     (4, 1, 128, 16, [400, 1], [3, 1]),
 ])
@@ -56,7 +61,7 @@ OPTIONS = [dict(softcap=20.0), dict(window=50), dict(window=1), dict(scale=0.3),
 
 
 @pytest.mark.parametrize("opts", OPTIONS)
-@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("new", [1, 10, 40])
 @pytest.mark.parametrize("hd", [64, 128, 256])
 def test_options(opts, new, hd):
     lens = [333, 300, 41]
@@ -75,7 +80,7 @@ def test_options(opts, new, hd):
     assert c.H.device_status() == 0
 
 
-@pytest.mark.parametrize("new", [1, 30])
+@pytest.mark.parametrize("new", [1, 7, 64])
 def test_layers_strides_slots_and_gaps(new):
     for kw in (dict(layers=3), dict(layers=2, inside=True), dict(gap=24), dict(slots=[4, 0, 2]), dict(layers=2, gap=8, inside=True, slots=[1, 3, 0])):
         c = Case(6, 3, 64, 7, [100, 33, 64], [new, 1, new], seed=new, **kw)
@@ -88,7 +93,7 @@ def test_layers_strides_slots_and_gaps(new):
 
 
 @pytest.mark.parametrize("hd", [64, 128, 256])
-@pytest.mark.parametrize("new", [1, 24])
+@pytest.mark.parametrize("new", [1, 24, 40])
 def test_what_is_not_finite_stays_where_it_is_seen(hd, new):
     """A k group with scale NaN makes the rows that see it NaN, a v group its 32 dims of those rows; nothing else."""
     c = Case(4, 2, hd, 16, [100, 70], [new, new], seed=hd)
@@ -117,7 +122,7 @@ def test_what_is_not_finite_stays_where_it_is_seen(hd, new):
         assert bool(((out.double() - ref).abs()[: new - 1] <= bound[: new - 1]).all())
 
 
-@pytest.mark.parametrize("new", [1, 24])
+@pytest.mark.parametrize("new", [1, 24, 40])
 def test_rows_of_q_that_are_not_finite_and_of_any_size(new):
     c = Case(4, 2, 128, 16, [90, 60], [new, new], seed=3)
     c.q[0] *= 2.0 ** 90
@@ -134,8 +139,8 @@ def test_rows_of_q_that_are_not_finite_and_of_any_size(new):
 
 
 def test_empty_sequences_rows_that_see_nothing_and_parts_of_a_batch(H):
-    for new in (1, 20):
-        c = Case(4, 2, 64, 8, [50, 30, 25], [new, 0, new], seed=new)
+    for new, g in ((1, 2), (20, 2), (20, 8)):
+        c = Case(2 * g, 2, 64, 8, [50, 30, 25], [new, 0, new], seed=new)
         c.check()
         # shorter than its new tokens: positions below 0 see nothing and give zeros
         if new > 1:
@@ -146,15 +151,15 @@ def test_empty_sequences_rows_that_see_nothing_and_parts_of_a_batch(H):
         # rows in front of the first and behind the last sequence of a part stay
         out = torch.full_like(c.q, 5.0)
         part = H.TokenBatch(c.q_start[2:], c.n_tokens, max(c.news), 50, slots=torch.tensor([2], dtype=torch.int32, device="cuda"))
-        H.paged_attention(c.cache, 0, part, c.q, 4, out=out)
+        H.paged_attention(c.cache, 0, part, c.q, 2 * g, out=out)
         assert bool((out[:new] == 5).all()) and bool((out[new:] != 5).any())
     empty = H.TokenBatch(torch.zeros(2, dtype=torch.int32, device="cuda"), 0, 0, 5)
-    assert H.paged_attention(c.cache, 0, empty, c.q[:0], 4).shape == (0, 256)
+    assert H.paged_attention(c.cache, 0, empty, c.q[:0], 16).shape == (0, 1024)
 
 
-@pytest.mark.parametrize("new", [1, 20])
-def test_tables_that_are_not_sound(H, new):
-    c = Case(4, 2, 64, 8, [50, 30], [new, new], seed=5)
+@pytest.mark.parametrize("new,g", [(1, 2), (20, 2), (20, 4)])
+def test_tables_that_are_not_sound(H, new, g):
+    c = Case(2 * g, 2, 64, 8, [50, 30], [new, new], seed=5)
     ref, bound = c.exact()
     good = int(c.table[0, 3])
     for bad in (-1, c.cache.n_pages, 1 << 30):
@@ -225,14 +230,14 @@ def test_streams_repeats_and_shared_workspaces(H):
 def test_more_sequences_than_the_scratch_holds(H):
     """Chunks of sequences whose fp16 copies take more than 1 GB: a few at a time, the workspace bounded."""
     lens = [40000, 3, 39000, 500, 40000, 40000, 1]
-    c = Case(16, 16, 128, 64, lens, [2, 3, 20, 20, 0, 1, 1], seed=4)
+    c = Case(16, 16, 128, 64, lens, [2, 3, 70, 70, 0, 1, 1], seed=4)
     nb = H.paged_attention_workspace(c.cache, c.batch, 16).numel()
     assert (1 << 29) < nb < (1 << 30) + (64 << 20)
     slopes = torch.full((16,), 0.01, device="cuda")
     prefix = torch.tensor([0, 1, 50, 0, 7, 3000, 0], dtype=torch.int32, device="cuda")
     c.check(window=3000, slopes=slopes, prefix=prefix)
     c.slots = torch.tensor([6, 5, 4, 3, 2, 1, 0], dtype=torch.int32, device="cuda")
-    c.batch = H.TokenBatch(c.q_start, c.n_tokens, 20, 40000, slots=c.slots)
+    c.batch = H.TokenBatch(c.q_start, c.n_tokens, 70, 40000, slots=c.slots)
     c.lens, c.keys, c.values = c.lens[::-1], c.keys[::-1], c.values[::-1]
     c.check(window=3000, slopes=slopes)
 
@@ -251,22 +256,22 @@ def test_pools_of_more_than_4_gb(H):
         big[3, pages[3]] = few[0, int(small.table[1, 0])]
     small.cache, small.layer = H.PagedKV4(k, v, ks, vs, table, small.seq_len), 3
     small.check()
-    small.news, small.starts, small.n_tokens = [30, 20], [0, 30, 50], 50
-    small.q_start.copy_(torch.tensor([0, 30, 50], dtype=torch.int32))
-    small.q = torch.randn(50, 16 * hd, device="cuda")
-    small.batch = H.TokenBatch(small.q_start, 50, 30, 300)
+    small.news, small.starts, small.n_tokens = [40, 20], [0, 40, 60], 60
+    small.q_start.copy_(torch.tensor([0, 40, 60], dtype=torch.int32))
+    small.q = torch.randn(60, 16 * hd, device="cuda")
+    small.batch = H.TokenBatch(small.q_start, 60, 40, 300)
     small.check()
 
 
 def test_random_ragged_batches(H):
     import random
     r = random.Random(11)
-    for i in range(25):
+    for i in range(40):
         kv = r.choice((1, 2, 3, 5, 8, 17))
         g = r.choice((1, 1, 2, 3, 8, 9))
         hd = r.choice((64, 128, 256))
         n = r.randrange(1, 9)
-        new = r.choice((1, 1, 1, 2, 7, 33))
+        new = r.choice((1, 1, 2, 7, 33, 66))
         lens = [r.randrange(1, r.choice((3, 70, 900))) for _ in range(n)]
         news = [min(x, r.randrange(0, new + 1)) for x in lens]
         if not any(news):

@@ -155,7 +155,7 @@ def test_workspaces_grow_with_the_batch_and_are_bounded():
         nb = size(ctypes.byref(c), ctypes.byref(b), 4)
         assert held * one <= nb < held * one + (256 << 20)
     wide = cache(n_kv_head=64, head_dim=256, page_stride=16 * 64 * 8, layer_stride=160 * 64 * 8, n_slots=2, max_pages=1 << 16, page_size=16)
-    b = batch(n_seq=2, n_tokens=100, max_new=50, max_len=1 << 20)
+    b = batch(n_seq=2, n_tokens=200, max_new=100, max_len=1 << 20)
     assert size(ctypes.byref(wide), ctypes.byref(b), 64) >= (1 << 20) * 64 * 256 * 4
 
 
