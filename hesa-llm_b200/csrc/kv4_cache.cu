@@ -31,7 +31,7 @@ struct Place {
     bool row;      // the row is a sequence's
 };
 
-__device__ __forceinline__ Place place_of(const PagedLayer& c, const BatchView& b, int row, int* status) {
+__device__ __forceinline__ Place find_place(const PagedLayer& c, const BatchView& b, int row, int* status) {
     // the last sequence that starts at or before this row and is not empty there
     int lo = 0, hi = b.n_seq - 1;
     while (lo < hi) {
@@ -42,7 +42,7 @@ __device__ __forceinline__ Place place_of(const PagedLayer& c, const BatchView& 
     const SeqView s = seq_view(c, b, lo);
     Place p{-1, 0, false};
     if (!s.ok) {
-        if (threadIdx.x == 0) record_status(status, kStatusBadPosition);
+        record_status(status, kStatusBadPosition);
         return p;
     }
     const int t = row - s.q0;
@@ -52,7 +52,7 @@ __device__ __forceinline__ Place place_of(const PagedLayer& c, const BatchView& 
     const int pi = p.pos >= 0 ? c.page_div.div(p.pos) : 0;
     const int page = p.pos >= 0 ? c.table[static_cast<int64_t>(s.slot) * c.max_pages + pi] : -1;
     if (page < 0 || page >= c.n_pages) {
-        if (threadIdx.x == 0) record_status(status, kStatusBadPosition);
+        record_status(status, kStatusBadPosition);
         return p;
     }
     p.group = static_cast<int64_t>(page) * c.page_stride + static_cast<int64_t>(p.pos - pi * c.page_size) * c.n_kv * (c.head_dim / kGroup);
@@ -62,41 +62,46 @@ __device__ __forceinline__ Place place_of(const PagedLayer& c, const BatchView& 
 // Eight values of a group whose other 24 the quad's other threads have (in order):
 // the group's scale, and this thread's word of codes.
 __device__ __forceinline__ uint32_t quantize8(const float (&x)[8], unsigned quad, float& scale) {
-    float m = x[0], a = fabsf(x[0]);
-    if (!(a < INFINITY)) a = INFINITY;
+    // the largest and the smallest value: the one of larger magnitude makes the scale; NaN stays
+    float hi = x[0], lo = x[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) {
-        float ai = fabsf(x[i]);
-        if (!(ai < INFINITY)) ai = INFINITY;   // also NaN: such a group has no scale
-        if (ai > a) {
-            a = ai;
-            m = x[i];
-        }
+        hi = fmax_nan(hi, x[i]);
+        lo = fmin_nan(lo, x[i]);
     }
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
-        const float ao = __shfl_xor_sync(quad, a, o), mo = __shfl_xor_sync(quad, m, o);
-        // equal magnitudes: the lower thread's value, on both sides
-        if (ao > a || (ao == a && (threadIdx.x & o))) {
-            a = ao;
-            m = mo;
-        }
+        hi = fmax_nan(hi, __shfl_xor_sync(quad, hi, o));
+        lo = fmin_nan(lo, __shfl_xor_sync(quad, lo, o));
+    }
+    float m = hi > -lo ? hi : lo;
+    if (hi == -lo) {   // as large on either side: the first of them
+        const int lane = threadIdx.x & 31;
+        unsigned first = 8;
+#pragma unroll
+        for (int i = 7; i >= 0; --i) first = fabsf(x[i]) == hi ? i : first;
+        const unsigned have = __ballot_sync(quad, first < 8) & quad;
+        float mine = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mine = static_cast<int>(first) == i ? x[i] : mine;
+        m = __shfl_sync(quad, mine, have ? __ffs(have) - 1 : lane);
     }
     const float s = m * -0.125f;
     const uint32_t u = __float_as_uint(s);
     float d = __uint_as_float((u + 0x7FFFu + ((u >> 16) & 1u)) & 0xFFFF0000u);   // 8 bits, ties to even
     if (fabsf(s) < 0x1p-17f) d = rintf(s * 0x1p24f) * 0x1p-24f;
-    if (!(a < INFINITY) || !(fabsf(d) <= kMostScale)) d = NAN;
+    if (!(hi - lo < INFINITY) || !(fabsf(d) <= kMostScale)) d = NAN;   // hi - lo: not finite where a value is not, or the scale is too large
     scale = d;
     if (!(fabsf(d) > 0.f)) return 0x88888888u;
     const float id = __frcp_rn(d);
+    // a number of 0 .. 15.9 rounded down behind 2^23 has its whole part in the low bits
     uint32_t w = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const int c = static_cast<int>(__fadd_rn(__fmul_rn(x[i], id), 8.5f));   // toward zero: what is below 0 gives 0
-        w |= static_cast<uint32_t>(min(max(c, 0), 15)) << (4 * i);
+        const float c = fminf(fmaxf(__fadd_rn(__fmul_rn(x[i], id), 8.5f), 0.f), 15.f);
+        w += __float_as_uint(__fadd_rd(c, 0x1p23f)) << (4 * i);
     }
-    return w;
+    return w - (0x4B000000u * 0x11111111u);
 }
 
 // A unit is 16 values of one head of one token: 8 of the first half of the head
@@ -109,19 +114,22 @@ rope_kv4_kernel(const PagedLayer c, const Pools4 pools, const BatchView b, float
     grid_dep_wait();
     grid_dep_launch();
     const int row = blockIdx.x;
-    const Place at = place_of(c, b, row, status);
+    __shared__ Place s_at;
+    if (threadIdx.x == 0) s_at = find_place(c, b, row, status);
+    __syncthreads();
+    const Place at = s_at;
     if (at.group < 0) return;
     if (table && at.pos >= table_rows) {
         if (threadIdx.x == 0) record_status(status, kStatusBadPosition);
         return;
     }
-    const int hd = c.head_dim, per = hd / 16, half = hd / 2, groups = hd / kGroup;
+    const int hd = c.head_dim, per = hd / 16, per_bits = __ffs(per) - 1, half = hd / 2, groups = hd / kGroup;   // head_dim is a power of two
     const int n_rot = n_head + c.n_kv;
     const int units = (n_rot + c.n_kv) * per;   // a multiple of 4, as `per` is: a quad works or none of its threads does
     const float* cs = table ? table + static_cast<int64_t>(at.pos) * hd : nullptr;
     const unsigned quad = 0xFu << (threadIdx.x & 28);
     for (int u = blockIdx.y * blockDim.x + threadIdx.x; u < units; u += gridDim.y * blockDim.x) {
-        const int h = u / per, d = (u - h * per) * 8;
+        const int h = u >> per_bits, d = (u - (h << per_bits)) * 8;
         if (h < n_head && !table) continue;   // nothing to rotate: q stays as it is
         const float* src = h < n_head ? q + row * ldq + static_cast<int64_t>(h) * hd
                            : h < n_rot ? k + row * ldk + static_cast<int64_t>(h - n_head) * hd
@@ -167,45 +175,74 @@ rope_kv4_kernel(const PagedLayer c, const Pools4 pools, const BatchView b, float
     }
 }
 
-// A thread takes four dims, half a word of codes, so that a warp writes 512 bytes in
-// a row, of kReadAhead words at a time.
-constexpr int kReadAhead = 4;
+// A block takes `rows` tokens' K and V, kReadChunk quads of dims at a time, and reads
+// the codes of the next chunk before it writes the values of one: writing, which is
+// nearly all of the traffic, does not wait for reads. A thread's quad is half a word
+// of codes, so that a warp writes 512 bytes in a row. Without the reads ahead 5296
+// tokens of 32 heads took 45 us, without reads at all 26.
+constexpr int kReadQuads = 8;                      // of a thread and chunk
+constexpr int kReadChunk = kReadQuads * 256;
+constexpr int kMostRows = 8;
 
 __global__ void __launch_bounds__(256)
-kv4_read_kernel(const PagedLayer c, const Pools4 pools, const BatchView b, float* k, int64_t ldk, float* v, int64_t ldv, int* status) {
+kv4_read_kernel(const PagedLayer c, const Pools4 pools, const BatchView b, float* k, int64_t ldk, float* v, int64_t ldv, int rows, int* status) {
+    __shared__ Place s_at[kMostRows];
     grid_dep_wait();
     grid_dep_launch();
-    const int row = blockIdx.x;
-    const Place at = place_of(c, b, row, status);
-    if (!at.row) return;
-    const int quads = c.n_kv * c.head_dim / 4;
-    const int step = gridDim.y * blockDim.x;
-    for (int u0 = blockIdx.y * blockDim.x + threadIdx.x; u0 < 2 * quads; u0 += kReadAhead * step) {
-        uint32_t code[kReadAhead];
-        float d[kReadAhead];
+    const int row0 = blockIdx.x * rows;
+    rows = min(rows, b.n_tokens - row0);
+    if (static_cast<int>(threadIdx.x) < rows) s_at[threadIdx.x] = find_place(c, b, row0 + threadIdx.x, status);
+    __syncthreads();
+    const int quads = c.n_kv * c.head_dim / 4, chunks = (2 * quads + kReadChunk - 1) / kReadChunk;   // K's, then V's
+    uint32_t code[kReadQuads];
+    __half d[kReadQuads];
+    // the grid's y shares out the chunks
+    auto load = [&](int r, int ch) {
+        const Place at = s_at[r];
 #pragma unroll
-        for (int x = 0; x < kReadAhead; ++x) {
-            const int u = u0 + x * step;
+        for (int x = 0; x < kReadQuads; ++x) {
+            const int u = ch * kReadChunk + x * 256 + threadIdx.x;
             const bool is_k = u < quads;
             const int w = (is_k ? u : u - quads) / 2;
             code[x] = 0x88888888u;
-            d[x] = 0.f;
+            d[x] = __float2half_rn(0.f);
             if (u < 2 * quads && at.group >= 0 && (is_k ? k : v)) {
                 code[x] = __ldcs(reinterpret_cast<const uint32_t*>((is_k ? pools.k : pools.v) + at.group) + w);
-                d[x] = __half2float(((is_k ? pools.ks : pools.vs) + at.group)[w / 4]);
+                d[x] = ((is_k ? pools.ks : pools.vs) + at.group)[w / 4];
             }
         }
+    };
+    int r = 0, ch = blockIdx.y;
+    if (rows > 0 && ch < chunks) load(r, ch);
+    while (r < rows && ch < chunks) {
+        uint32_t now[kReadQuads];
+        __half scale[kReadQuads];
 #pragma unroll
-        for (int x = 0; x < kReadAhead; ++x) {
-            const int u = u0 + x * step;
+        for (int x = 0; x < kReadQuads; ++x) {
+            now[x] = code[x];
+            scale[x] = d[x];
+        }
+        const int row = row0 + r, at = ch;
+        const bool some = s_at[r].row;
+        ch += gridDim.y;
+        if (ch >= chunks) {
+            ch = blockIdx.y;
+            ++r;
+        }
+        if (r < rows) load(r, ch);
+        if (!some) continue;
+#pragma unroll
+        for (int x = 0; x < kReadQuads; ++x) {
+            const int u = at * kReadChunk + x * 256 + threadIdx.x;
             const bool is_k = u < quads;
             float* o = is_k ? k : v;
             if (u >= 2 * quads || !o) continue;
             o += row * (is_k ? ldk : ldv) + static_cast<int64_t>(is_k ? u : u - quads) * 4;
-            const uint32_t four = code[x] >> ((u & 1) * 16);
+            const uint32_t four = now[x] >> ((u & 1) * 16);
+            const float f = __half2float(scale[x]);
             float y[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = d[x] * static_cast<float>(static_cast<int>((four >> (4 * i)) & 15u) - 8);
+            for (int i = 0; i < 4; ++i) y[i] = f * static_cast<float>(static_cast<int>((four >> (4 * i)) & 15u) - 8);
             __stcs(reinterpret_cast<float4*>(o), make_float4(y[0], y[1], y[2], y[3]));
         }
     }
@@ -294,10 +331,12 @@ int hesa_cuda_kv4_read(const hesa_cuda_paged_kv4* kv, int32_t layer, const hesa_
     int* status = nullptr;
     cudaError_t e = status_word(&status);
     if (e == cudaSuccess) {
-        const int64_t units = 2 * width / 4;
-        const int64_t y = batch->n_tokens >= 148 * 4 ? 1 : std::min<int64_t>((units + 255) / 256, 1024);
-        e = launch_dep(kv4_read_kernel, dim3(static_cast<unsigned>(batch->n_tokens), static_cast<unsigned>(y)), 256, 0, static_cast<cudaStream_t>(stream),
-                       layer_of4(kv), pools_of(kv, layer), view_of(batch), k, ldk, v, ldv, status);
+        // rows for one block after another only where there are blocks for every SM several times over
+        const int64_t chunks = (2 * width / 4 + kReadChunk - 1) / kReadChunk;
+        const int rows = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMostRows, batch->n_tokens / (148 * 6))));
+        const int64_t y = rows > 1 ? 1 : std::min<int64_t>(chunks, 1024);
+        e = launch_dep(kv4_read_kernel, dim3(static_cast<unsigned>((batch->n_tokens + rows - 1) / rows), static_cast<unsigned>(y)), 256, 0, static_cast<cudaStream_t>(stream),
+                       layer_of4(kv), pools_of(kv, layer), view_of(batch), k, ldk, v, ldv, rows, status);
     }
     return e == cudaSuccess ? HESA_CUDA_OK : record_cuda_error(e, "kv4_read kernel");
 }
