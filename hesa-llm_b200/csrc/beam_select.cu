@@ -7,10 +7,14 @@
 // pass over every beam's logits (a block a beam, or a part of one where beams are
 // few) for its sums and its `width` largest logits; the second, a block a sequence,
 // joins the parts of each beam and gives every candidate that is left its rank.
+// Where a cluster of eight blocks is enough for a sequence, one kernel does both.
 // Between beams it is the sums that decide, and they may be very close: they are
 // made in 64 bits from z's fp32 terms.
 // HBM-bound: every logit is read once (those of ended and ruled-out beams not at
-// all); a few beams are bound by the latency of the two launches.
+// all); a few beams, and many short rows, are bound by the chain of waits at a row's
+// end. 64 sequences of 8 beams, 131071 tokens, 355 of the beams alive: 49 us (186 MB,
+// 3.8 TB/s; without finding the largest 43, and the same with 1 to 5 parts a beam);
+// 128 of 16 beams, 3000 tokens 21 us; one of 4 beams, 32000 tokens 10.7 us.
 #include "../../include/hesa_cuda.h"
 #include "abi_errors.h"
 #include "paged.h"
@@ -25,6 +29,7 @@ namespace {
 
 constexpr int kMaxWidth = kMaxTop;
 constexpr int kMostParts = 64;   // of a row
+constexpr int kSmallWarps = 2;
 
 struct RowPart {
     float m, z;
@@ -35,15 +40,16 @@ __device__ __forceinline__ bool counts(const float* scores, const int32_t* ended
     return !(ended && ended[r] != 0) && scores[r] > -INFINITY && scores[r] < INFINITY;
 }
 
-__global__ void __launch_bounds__(kLpThreads, 4)
+template <int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 4 * kLpWarps / WARPS)
 beam_rows_kernel(const float* logits, int64_t ld, int vocab, const float* scores, const int32_t* ended, int top, int n_split, RowPart* parts,
                  uint64_t* keys) {
-    __shared__ TopShared<true> sh;
+    __shared__ TopShared<true, WARPS> sh;
     grid_dep_wait();
     grid_dep_launch();
     const int64_t r = blockIdx.x;
     if (!counts(scores, ended, r)) return;
-    const Sums s = row_part<true>(logits + r * ld, vocab, blockIdx.y, n_split, top, sh);
+    const Sums s = row_part<true, WARPS>(logits + r * ld, vocab, blockIdx.y, n_split, top, sh);
     const int64_t at = r * n_split + blockIdx.y;
     if (threadIdx.x == 0) parts[at] = RowPart{s.m, s.z};
     if (static_cast<int>(threadIdx.x) < top) keys[at * top + threadIdx.x] = sh.top[threadIdx.x];
@@ -56,19 +62,28 @@ __device__ __forceinline__ uint64_t order_of(double x) {
     return u >> 63 ? ~u : u | (uint64_t(1) << 63);
 }
 
-__global__ void __launch_bounds__(kLpThreads)
-beam_join_kernel(const float* scores, const int32_t* ended, int width, int vocab, int top, int n_split, const RowPart* parts, const uint64_t* keys,
-                 float* next_scores, int32_t* parents, int32_t* tokens) {
-    // candidate b * kMaxWidth + i: the i-th of beam b
-    __shared__ uint64_t s_key[kMaxWidth * kMaxWidth];
-    __shared__ double s_score[kMaxWidth * kMaxWidth];
-    __shared__ int s_token[kMaxWidth * kMaxWidth];
-    __shared__ int s_n[kMaxWidth];
-    grid_dep_wait();
-    grid_dep_launch();
+struct BeamOut {
+    float* scores;
+    int32_t* parents;
+    int32_t* tokens;
+};
+
+// Candidates of a sequence: b * kMaxWidth + i is the i-th of beam b.
+struct JoinShared {
+    uint64_t key[kMaxWidth * kMaxWidth];
+    double score[kMaxWidth * kMaxWidth];
+    int token[kMaxWidth * kMaxWidth];
+    int n[kMaxWidth];
+};
+
+// The next beams of the sequence whose first beam is row r0, from the n_split (at most
+// kMostParts) parts of each of its beams: part(b, l) and key_of(b, l, i), the i-th key
+// of part l of beam b. All threads of a block.
+template <int WARPS, typename PartOf, typename KeyOf>
+__device__ __forceinline__ void join_beams(const float* scores, const int32_t* ended, int64_t r0, int width, int top, int n_split, const PartOf& part,
+                                           const KeyOf& key_of, JoinShared& sh, const BeamOut& out) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t r0 = static_cast<int64_t>(blockIdx.x) * width;
-    for (int b = warp; b < width; b += kLpWarps) {
+    for (int b = warp; b < width; b += WARPS) {
         const int64_t r = r0 + b;
         const float score = scores[r];
         const bool end = ended && ended[r] != 0, nan = !(score < INFINITY), dead = !end && !counts(scores, ended, r);
@@ -76,34 +91,37 @@ beam_join_kernel(const float* scores, const int32_t* ended, int width, int vocab
         uint64_t order = order_of(nan ? -INFINITY : score);
         int token = end ? -1 : lane;   // the lowest tokens of a beam whose candidates are all alike
         if (!end && !dead) {
-            const RowPart* p = parts + r * n_split;
             float m = -INFINITY;
-            for (int i = lane; i < n_split; i += 32) m = fmaxf(m, __ldcg(&p[i].m));
+            for (int i = lane; i < n_split; i += 32) m = fmaxf(m, part(b, i).m);
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
             const float ms = m == -INFINITY ? 0.f : m;
             double z = 0.0;
             for (int i = lane; i < n_split; i += 32) {
-                const float pm = __ldcg(&p[i].m), pz = __ldcg(&p[i].z);
-                z += pm == -INFINITY ? pz : pz * exp(static_cast<double>(pm) - ms);   // a part of nothing but NaN has m -inf and z NaN
+                const RowPart p = part(b, i);
+                z += p.m == -INFINITY ? p.z : p.z * exp(static_cast<double>(p.m) - ms);   // a part of nothing but NaN has m -inf and z NaN
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
             // the parts' lists joined: a lane has the heads of two of them (and what comes behind these on its way), the
             // largest of all heads is the next one
-            const unsigned long long* lists = reinterpret_cast<const unsigned long long*>(keys + r * n_split * top);
-            auto key_of = [&](int l, int i) -> uint64_t { return l < n_split && i < top ? __ldcg(lists + static_cast<int64_t>(l) * top + i) : 0; };
-            uint64_t head0 = key_of(lane, 0), head1 = key_of(lane + 32, 0), next0 = key_of(lane, 1), next1 = key_of(lane + 32, 1), best = 0;
-            int at0 = 1, at1 = 1;
-            for (int i = 0; i < top; ++i) {
-                const uint64_t c = warp_max_key(max_key(head0, head1));
-                if (lane == i) best = c;
-                if (head0 == c) {
-                    head0 = next0;
-                    next0 = key_of(lane, ++at0);
-                } else if (head1 == c) {
-                    head1 = next1;
-                    next1 = key_of(lane + 32, ++at1);
+            auto at = [&](int l, int i) -> uint64_t { return l < n_split && i < top ? key_of(b, l, i) : 0; };
+            uint64_t best = 0;
+            if (n_split == 1) {
+                best = at(0, lane);
+            } else {
+                uint64_t head0 = at(lane, 0), head1 = at(lane + 32, 0), next0 = at(lane, 1), next1 = at(lane + 32, 1);
+                int at0 = 1, at1 = 1;
+                for (int i = 0; i < top; ++i) {
+                    const uint64_t c = warp_max_key(max_key(head0, head1));
+                    if (lane == i) best = c;
+                    if (head0 == c) {
+                        head0 = next0;
+                        next0 = at(lane, ++at0);
+                    } else if (head1 == c) {
+                        head1 = next1;
+                        next1 = at(lane + 32, ++at1);
+                    }
                 }
             }
             if (isfinite(z)) {
@@ -118,39 +136,141 @@ beam_join_kernel(const float* scores, const int32_t* ended, int width, int vocab
             }
         }
         const int n = end ? 1 : top;
-        if (lane == 0) s_n[b] = n;
+        if (lane == 0) sh.n[b] = n;
         if (lane < n) {
-            s_key[b * kMaxWidth + lane] = order;
-            s_score[b * kMaxWidth + lane] = mine;
-            s_token[b * kMaxWidth + lane] = token;
+            sh.key[b * kMaxWidth + lane] = order;
+            sh.score[b * kMaxWidth + lane] = mine;
+            sh.token[b * kMaxWidth + lane] = token;
         }
     }
     __syncthreads();
     // the rank of each: how many are larger, or equal with a lower number
-    for (int c = threadIdx.x; c < width * kMaxWidth; c += kLpThreads) {
+    for (int c = threadIdx.x; c < width * kMaxWidth; c += WARPS * 32) {
         const int b = c / kMaxWidth, i = c % kMaxWidth;
-        if (i >= s_n[b]) continue;
-        const uint64_t key = s_key[c];
+        if (i >= sh.n[b]) continue;
+        const uint64_t key = sh.key[c];
         int rank = 0;
         for (int y = 0; y < width && rank < width; ++y)
-            for (int x = 0; x < s_n[y]; ++x) {   // a beam's candidates descend
-                const uint64_t k = s_key[y * kMaxWidth + x];
+            for (int x = 0; x < sh.n[y]; ++x) {   // a beam's candidates descend
+                const uint64_t k = sh.key[y * kMaxWidth + x];
                 if (k < key || (k == key && y * kMaxWidth + x >= c)) break;
                 ++rank;
             }
         if (rank < width) {
             const int64_t o = r0 + rank;
-            next_scores[o] = static_cast<float>(s_score[c]);
-            parents[o] = b;
-            tokens[o] = s_token[c];
+            out.scores[o] = static_cast<float>(sh.score[c]);
+            out.parents[o] = b;
+            out.tokens[o] = sh.token[c];
         }
     }
 }
 
-// Parts of a row: blocks enough that the SMs end together though some beams have ended, at least a quad for each thread a block.
+constexpr int kJoinWarps = 16;
+
+__global__ void __launch_bounds__(kJoinWarps * 32)
+beam_join_kernel(const float* scores, const int32_t* ended, int width, int top, int n_split, const RowPart* parts, const uint64_t* keys, BeamOut out) {
+    __shared__ JoinShared sh;
+    grid_dep_wait();
+    grid_dep_launch();
+    const int64_t r0 = static_cast<int64_t>(blockIdx.x) * width;
+    const unsigned long long* lists = reinterpret_cast<const unsigned long long*>(keys);
+    join_beams<kJoinWarps>(
+        scores, ended, r0, width, top, n_split,
+        [&](int b, int l) {
+            const float2 p = __ldcg(reinterpret_cast<const float2*>(parts + (r0 + b) * n_split + l));
+            return RowPart{p.x, p.y};
+        },
+        [&](int b, int l, int i) -> uint64_t { return __ldcg(lists + ((r0 + b) * n_split + l) * top + i); }, sh, out);
+}
+
+// Both in one launch, a cluster of eight blocks a sequence: each takes a beam or a
+// part of one, and the first joins what the others have in their shared memory. For
+// few sequences, rows that a few blocks are quick with, and no more beams than blocks:
+// 64 sequences of 8 beams, 24000 tokens 20 us (two kernels 25), 16 of them 12.7 (15.5);
+// one sequence of 4 beams, 32000 tokens 10.7 (9.6), but 3 us less of the host's time;
+// 128 sequences of 2 beams, 24000 tokens 24 (14), one of 16 beams 25 (16).
+constexpr int kCluster = 8;
+constexpr int64_t kClusterElems = 24576;                               // logits of a part
+constexpr int64_t kClusterSeqs = 148 * 4 / kCluster;                   // that are on the SMs at a time
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t in_block(const void* p, int rank) {   // the address of the same thing in block `rank` of the cluster
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ uint64_t lds_cluster(uint32_t a) {
+    unsigned long long v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
+    return v;
+}
+
+__global__ void __launch_bounds__(kLpThreads, 4)
+beam_cluster_kernel(const float* logits, int64_t ld, int vocab, const float* scores, const int32_t* ended, int width, int top, int n_split, BeamOut out) {
+    __shared__ union {   // the join follows the last row
+        TopShared<true> rows;
+        JoinShared join;
+    } sh;
+    __shared__ __align__(8) RowPart s_part;
+    __shared__ uint64_t s_keys[kMaxTop];
+    grid_dep_wait();
+    grid_dep_launch();
+    const int rank = blockIdx.x % kCluster;
+    const int64_t r0 = static_cast<int64_t>(blockIdx.x / kCluster) * width;
+    // part `rank` of them all
+    const int64_t r = r0 + rank / n_split;
+    if (rank < width * n_split && counts(scores, ended, r)) {
+        const Sums s = row_part<true>(logits + r * ld, vocab, rank % n_split, n_split, top, sh.rows);
+        if (threadIdx.x == 0) s_part = RowPart{s.m, s.z};
+        if (static_cast<int>(threadIdx.x) < top) s_keys[threadIdx.x] = sh.rows.top[threadIdx.x];
+    }
+    __syncthreads();   // sh is the join's from here
+    cluster_sync();
+    if (rank == 0) {
+        join_beams<kLpWarps>(
+            scores, ended, r0, width, top, n_split,
+            [&](int b, int l) {
+                const uint64_t p = lds_cluster(in_block(&s_part, b * n_split + l));
+                return RowPart{__uint_as_float(static_cast<uint32_t>(p)), __uint_as_float(static_cast<uint32_t>(p >> 32))};
+            },
+            [&](int b, int l, int i) -> uint64_t { return lds_cluster(in_block(&s_keys[i], b * n_split + l)); },
+            sh.join, out);
+    }
+    cluster_sync();   // the others' shared memory has been read
+}
+
+// Parts of a row: what fits on the SMs at a time (four blocks each), none below
+// kPartElems logits; where there are rows for more than that, about two rounds of
+// blocks, so that SMs end together though some beams have ended.
+constexpr int kPartElems = 4096;
 int parts_of(int64_t n_rows, int64_t vocab) {
-    const int64_t want = (148 * 8 + n_rows - 1) / n_rows, most = std::max<int64_t>(1, vocab / (4 * kLpThreads));
+    const int64_t one = 148 * 4, want = n_rows <= one / 2 ? one / n_rows : (2 * one + n_rows - 1) / n_rows, most = std::max<int64_t>(1, vocab / kPartElems);
     return static_cast<int>(std::min(std::min(want, most), static_cast<int64_t>(kMostParts)));
+}
+
+// Parts of a row of a cluster's; 0: the two kernels.
+int cluster_parts(int64_t n_seq, int32_t width, int64_t vocab) {
+    const int parts = std::max(1, kCluster / width);
+    return width <= kCluster && n_seq <= kClusterSeqs && vocab <= parts * kClusterElems ? parts : 0;
+}
+
+cudaError_t launch_clusters(int64_t n_seq, cudaStream_t s, const float* logits, int64_t ld, int vocab, const float* scores, const int32_t* ended, int width, int top,
+                            int n_split, const BeamOut& out) {
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = kCluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(n_seq * kCluster));
+    cfg.blockDim = dim3(kLpThreads);
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, beam_cluster_kernel, logits, ld, vocab, scores, ended, width, top, n_split, out);
 }
 
 bool shape_ok(int64_t n_seq, int32_t width, int64_t vocab) {
@@ -184,15 +304,21 @@ int hesa_cuda_beam_select(const float* logits, int64_t ld, int64_t n_seq, int32_
     if (workspace_bytes < hesa_cuda_beam_select_workspace_size(n_seq, width, vocab))
         return record_error(HESA_CUDA_INVALID_ARGUMENT, "workspace too small");
     const int64_t rows = n_seq * width;
-    const int top = static_cast<int>(std::min<int64_t>(width, vocab)), n_split = parts_of(rows, vocab);
+    const int top = static_cast<int>(std::min<int64_t>(width, vocab)), n_split = parts_of(rows, vocab), in_cluster = cluster_parts(n_seq, width, vocab);
+    const BeamOut out{next_scores, parents, tokens};
+    if (in_cluster > 0) {
+        const cudaError_t e = launch_clusters(n_seq, static_cast<cudaStream_t>(stream), logits, ld, static_cast<int>(vocab), scores, ended, width, top, in_cluster, out);
+        return e == cudaSuccess ? HESA_CUDA_OK : record_cuda_error(e, "beam_select kernel");
+    }
     RowPart* parts = static_cast<RowPart*>(workspace);
     uint64_t* keys = reinterpret_cast<uint64_t*>(parts + rows * n_split);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    cudaError_t e = launch_dep(beam_rows_kernel, dim3(static_cast<unsigned>(rows), static_cast<unsigned>(n_split)), kLpThreads, 0, s, logits, ld,
-                               static_cast<int>(vocab), scores, ended, top, n_split, parts, keys);
+    // many short rows: small blocks, so that more of them, and of the waits at a row's end, go side by side
+    const bool small = vocab <= kPartElems && rows > 148 * 2;
+    cudaError_t e = launch_dep(small ? beam_rows_kernel<kSmallWarps> : beam_rows_kernel<kLpWarps>, dim3(static_cast<unsigned>(rows), static_cast<unsigned>(n_split)),
+                               (small ? kSmallWarps : kLpWarps) * 32, 0, s, logits, ld, static_cast<int>(vocab), scores, ended, top, n_split, parts, keys);
     if (e == cudaSuccess)
-        e = launch_dep(beam_join_kernel, dim3(static_cast<unsigned>(n_seq)), kLpThreads, 0, s, scores, ended, width, static_cast<int>(vocab), top, n_split, parts,
-                       keys, next_scores, parents, tokens);
+        e = launch_dep(beam_join_kernel, dim3(static_cast<unsigned>(n_seq)), kJoinWarps * 32, 0, s, scores, ended, width, top, n_split, parts, keys, out);
     return e == cudaSuccess ? HESA_CUDA_OK : record_cuda_error(e, "beam_select kernels");
 }
 

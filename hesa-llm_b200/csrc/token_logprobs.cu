@@ -121,7 +121,7 @@ token_logprobs_kernel(const float* logits, int64_t ld, int n_rows, int vocab, co
         }
         if (lane < top_k) s_cand[warp * top_k + lane] = mine;
         __syncthreads();
-        select(s_cand, kLpWarps * top_k, top_k, s_top);
+        select<kLpWarps>(s_cand, kLpWarps * top_k, top_k, s_top);
     }
     if (warp == 0) {
         // the parts' sums: at most 64, two a lane, joined in a fixed tree

@@ -1,6 +1,6 @@
 // top_rows.cuh -- one pass over (a part of) a row of logits: its softmax sums, its
 // entropy's sum and its largest values with their ids (token_logprobs.cu says how
-// and why), for a block of kLpThreads.
+// and why), for a block of WARPS warps.
 #pragma once
 
 #include <cstdint>
@@ -63,14 +63,16 @@ __device__ __forceinline__ void insert(uint64_t& mine, uint64_t c, int lane) {
     else if (lane == at) mine = c;
 }
 
-constexpr int kCand = 2 * 1024 + kMaxTop;   // keys that are gathered before the k largest of them are kept
+// Keys that are gathered before the k largest of them are kept: twice what may come in one step.
+constexpr int cand_of(int warps) { return 2 * 4 * 32 * warps + kMaxTop; }
 
 // The k largest of the n keys in cand (distinct; fewer than k are followed by
 // zeros), descending, into out. All threads of the block.
+template <int WARPS>
 __device__ __forceinline__ void select(const uint64_t* cand, int n, int k, uint64_t* out) {
     if (static_cast<int>(threadIdx.x) < k) out[threadIdx.x] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kLpThreads) {
+    for (int i = threadIdx.x; i < n; i += WARPS * 32) {
         const uint64_t c = cand[i];
         int rank = 0;
         for (int j = 0; j < n; ++j) rank += cand[j] > c;
@@ -81,23 +83,23 @@ __device__ __forceinline__ void select(const uint64_t* cand, int n, int k, uint6
 
 __device__ __forceinline__ uint64_t max_key(uint64_t a, uint64_t b) { return a > b ? a : b; }
 __device__ __forceinline__ uint64_t warp_max_key(uint64_t v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = max_key(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(v >> 32));
+    const uint32_t lo = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(v >> 32) == hi ? static_cast<uint32_t>(v) : 0u);
+    return static_cast<uint64_t>(hi) << 32 | lo;
 }
 
 // Shared memory of a block.
-template <bool TOP> struct TopShared {
-    Sums sums[kLpWarps];
-    uint64_t cand[TOP ? kCand : 1], top[kMaxTop], key[kLpWarps];
-    int from[TOP ? kLpThreads : 1];   // the threads in cand, then those whose values are read again
+template <bool TOP, int WARPS = kLpWarps> struct TopShared {
+    Sums sums[WARPS];
+    uint64_t cand[TOP ? cand_of(WARPS) : 1], top[kMaxTop], key[WARPS];
+    int from[TOP ? WARPS * 32 : 1];   // the threads in cand, then those whose values are read again
     int n;
 };
 
 // Part `split` of n_split of a row: its sums, in every thread, and with TOP its
 // top_k largest keys, descending, in sh.top (zeros behind them).
-template <bool TOP>
-__device__ __forceinline__ Sums row_part(const float* row, int vocab, int split, int n_split, int top_k, TopShared<TOP>& sh) {
+template <bool TOP, int WARPS = kLpWarps>
+__device__ __forceinline__ Sums row_part(const float* row, int vocab, int split, int n_split, int top_k, TopShared<TOP, WARPS>& sh) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int mis = static_cast<int>((reinterpret_cast<uintptr_t>(row) >> 2) & 3);
     // quad q holds elements 4 q - mis .. + 3
@@ -121,7 +123,7 @@ __device__ __forceinline__ Sums row_part(const float* row, int vocab, int split,
         for (int i = 0; i < 4; ++i) k[i] = q < q1 && e + i >= 0 && e + i < vocab ? make_key(v[i], e + i) : 0;
     };
     // the thread's quads: qb + u * 32 for u < kUnroll, then kStep further on
-    constexpr int kStep = kLpWarps * 32 * kUnroll;
+    constexpr int kStep = WARPS * 32 * kUnroll;
     Sums s{-INFINITY, 0.f, 0.f};
     float4 nx[kUnroll];
     int qb = q0 + warp * 32 * kUnroll + lane, best = qb;   // best: the quad of the first maximum
@@ -171,16 +173,26 @@ __device__ __forceinline__ Sums row_part(const float* row, int vocab, int split,
         s.w += w.x + w.y;
     }
     if (TOP) {
-        // the thread's largest key
+        // the thread's largest key; a thread that has read its quads at once still has them
+        const bool once = q1 - q0 <= kStep;
+        const int mine0 = q0 + warp * 32 * kUnroll + lane;
         uint64_t mine;
         {
+            float4 v;
+            if (once) {
+#pragma unroll
+                for (int u = 0; u < kUnroll; ++u)
+                    if (u == 0 || best == mine0 + u * 32) v = nx[u];
+            } else {
+                v = quad(best);
+            }
             uint64_t k[4];
-            keys(best, quad(best), k);
+            keys(best, v, k);
             mine = max_key(max_key(k[0], k[1]), max_key(k[2], k[3]));
         }
         // each warp's ceil(k / 8)-th bounds the k-th of the block's from below; the threads above the least of them are ranked
         uint64_t rest = mine, nth = 0;
-        for (int i = 0; i < (top_k + kLpWarps - 1) / kLpWarps; ++i) {
+        for (int i = 0; i < (top_k + WARPS - 1) / WARPS; ++i) {
             nth = warp_max_key(rest);
             if (rest == nth) rest = 0;
         }
@@ -189,7 +201,7 @@ __device__ __forceinline__ Sums row_part(const float* row, int vocab, int split,
         __syncthreads();
         uint64_t least = sh.key[0];
 #pragma unroll
-        for (int w2 = 1; w2 < kLpWarps; ++w2) least = least < sh.key[w2] ? least : sh.key[w2];
+        for (int w2 = 1; w2 < WARPS; ++w2) least = least < sh.key[w2] ? least : sh.key[w2];
         if (mine != 0 && mine >= least) {
             const int at = atomicAdd(&sh.n, 1);
             sh.cand[at] = mine;
@@ -211,8 +223,21 @@ __device__ __forceinline__ Sums row_part(const float* row, int vocab, int split,
         uint64_t bound = n_max >= top_k ? sh.top[top_k - 1] : 0;
         if (threadIdx.x == 0) sh.n = 0;
         __syncthreads();
+        if (once) {   // at most kMaxTop threads, 16 values each
+            if (mine != 0 && mine >= bound) {
+#pragma unroll
+                for (int u = 0; u < kUnroll; ++u) {
+                    uint64_t k[4];
+                    keys(mine0 + u * 32, nx[u], k);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (k[i] != 0 && k[i] >= bound) sh.cand[atomicAdd(&sh.n, 1)] = k[i];
+                }
+            }
+            __syncthreads();
+        }
         // their values again: a warp takes one thread's quads, a quad a lane at a time
-        for (int f0 = 0; f0 < n_from; f0 += kLpWarps) {
+        for (int f0 = once ? n_from : 0; f0 < n_from; f0 += kLpWarps) {
             const int f = f0 + warp < n_from ? sh.from[f0 + warp] : -1;
             const int base = q0 + (f >> 5) * 32 * kUnroll + (f & 31);
             const int n_mine = (q1 - q0 + kStep - 1) / kStep * kUnroll;   // quads of a thread at most
@@ -235,11 +260,11 @@ __device__ __forceinline__ Sums row_part(const float* row, int vocab, int split,
                     for (int i = 0; i < 4; ++i)
                         if (k[i] != 0 && k[i] >= bound) sh.cand[atomicAdd(&sh.n, 1)] = k[i];
                     __syncthreads();
-                    // 1024 more may come: keep the k largest, the k-th is the new bound
+                    // as many more may come: keep the k largest, the k-th is the new bound
                     const int n = sh.n;
                     __syncthreads();
-                    if (n > kCand - 4 * kLpThreads) {
-                        select(sh.cand, n, top_k, sh.top);
+                    if (n > cand_of(WARPS) - 4 * 32 * WARPS) {
+                        select<WARPS>(sh.cand, n, top_k, sh.top);
                         if (static_cast<int>(threadIdx.x) < top_k) sh.cand[threadIdx.x] = sh.top[threadIdx.x];
                         bound = sh.top[top_k - 1];
                         if (threadIdx.x == 0) sh.n = top_k;
@@ -248,7 +273,7 @@ __device__ __forceinline__ Sums row_part(const float* row, int vocab, int split,
                 }
             }
         }
-        select(sh.cand, sh.n, top_k, sh.top);
+        select<WARPS>(sh.cand, sh.n, top_k, sh.top);
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) {
@@ -258,7 +283,7 @@ __device__ __forceinline__ Sums row_part(const float* row, int vocab, int split,
     if (lane == 0) sh.sums[warp] = s;
     __syncthreads();
     s = sh.sums[0];
-    for (int w2 = 1; w2 < kLpWarps; ++w2) s = merge(s, sh.sums[w2]);
+    for (int w2 = 1; w2 < WARPS; ++w2) s = merge(s, sh.sums[w2]);
     return s;
 }
 
