@@ -107,7 +107,8 @@ __device__ __forceinline__ uint32_t quantize8(const float (&x)[8], unsigned quad
 // A unit is 16 values of one head of one token: 8 of the first half of the head
 // and the 8 that they are rotated with; four threads side by side have two whole
 // groups. A block takes one token's units (grid.y covers long rows); q, then k,
-// then v.
+// then v. 5296 tokens of 32 heads: 65 us (371 MB, 5.7 TB/s); with four and four values a
+// thread, sixteen-byte accesses side by side but more shuffles a value, 71.
 __global__ void __launch_bounds__(256)
 rope_kv4_kernel(const PagedLayer c, const Pools4 pools, const BatchView b, float* q, int64_t ldq, const float* k, int64_t ldk,
                 const float* v, int64_t ldv, int n_head, const float* table, int table_rows, int* status) {
@@ -177,9 +178,9 @@ rope_kv4_kernel(const PagedLayer c, const Pools4 pools, const BatchView b, float
 
 // A block takes `rows` tokens' K and V, kReadChunk quads of dims at a time, and reads
 // the codes of the next chunk before it writes the values of one: writing, which is
-// nearly all of the traffic, does not wait for reads. A thread's quad is half a word
-// of codes, so that a warp writes 512 bytes in a row. Without the reads ahead 5296
-// tokens of 32 heads took 45 us, without reads at all 26.
+// nearly all of the traffic, does not wait for reads. (5296 tokens of 32 heads: 45 us
+// without that, 26 without reading.) A thread's quad is half a word of codes, so that
+// a warp writes 512 bytes in a row; with a word a thread, two stores 32 bytes apart, 55.
 constexpr int kReadQuads = 8;                      // of a thread and chunk
 constexpr int kReadChunk = kReadQuads * 256;
 constexpr int kMostRows = 8;
@@ -193,28 +194,29 @@ kv4_read_kernel(const PagedLayer c, const Pools4 pools, const BatchView b, float
     rows = min(rows, b.n_tokens - row0);
     if (static_cast<int>(threadIdx.x) < rows) s_at[threadIdx.x] = find_place(c, b, row0 + threadIdx.x, status);
     __syncthreads();
-    const int quads = c.n_kv * c.head_dim / 4, chunks = (2 * quads + kReadChunk - 1) / kReadChunk;   // K's, then V's
+    const int quads = c.n_kv * c.head_dim / 4, chunks = (quads + kReadChunk - 1) / kReadChunk;   // of K, and as many of V
     uint32_t code[kReadQuads];
     __half d[kReadQuads];
-    // the grid's y shares out the chunks
+    // chunk ch: of K where it is even, of V where it is odd; the grid's y shares them out
     auto load = [&](int r, int ch) {
-        const Place at = s_at[r];
+        const int64_t group = s_at[r].group;
+        const uint32_t* from = reinterpret_cast<const uint32_t*>((ch & 1 ? pools.v : pools.k) + group);
+        const __half* scales = (ch & 1 ? pools.vs : pools.ks) + group;
+        const bool some = group >= 0 && (ch & 1 ? v : k) != nullptr;
 #pragma unroll
         for (int x = 0; x < kReadQuads; ++x) {
-            const int u = ch * kReadChunk + x * 256 + threadIdx.x;
-            const bool is_k = u < quads;
-            const int w = (is_k ? u : u - quads) / 2;
+            const int u = (ch >> 1) * kReadChunk + x * 256 + threadIdx.x;
             code[x] = 0x88888888u;
             d[x] = __float2half_rn(0.f);
-            if (u < 2 * quads && at.group >= 0 && (is_k ? k : v)) {
-                code[x] = __ldcs(reinterpret_cast<const uint32_t*>((is_k ? pools.k : pools.v) + at.group) + w);
-                d[x] = ((is_k ? pools.ks : pools.vs) + at.group)[w / 4];
+            if (some && u < quads) {
+                code[x] = __ldcs(from + u / 2);
+                d[x] = scales[u / 8];
             }
         }
     };
     int r = 0, ch = blockIdx.y;
-    if (rows > 0 && ch < chunks) load(r, ch);
-    while (r < rows && ch < chunks) {
+    if (rows > 0 && ch < 2 * chunks) load(r, ch);
+    while (r < rows && ch < 2 * chunks) {
         uint32_t now[kReadQuads];
         __half scale[kReadQuads];
 #pragma unroll
@@ -222,28 +224,28 @@ kv4_read_kernel(const PagedLayer c, const Pools4 pools, const BatchView b, float
             now[x] = code[x];
             scale[x] = d[x];
         }
-        const int row = row0 + r, at = ch;
-        const bool some = s_at[r].row;
+        const int64_t row = row0 + r;
+        const int at = ch;
+        float* o = ch & 1 ? v : k;
+        const bool some = s_at[r].row && o;
         ch += gridDim.y;
-        if (ch >= chunks) {
+        if (ch >= 2 * chunks) {
             ch = blockIdx.y;
             ++r;
         }
         if (r < rows) load(r, ch);
         if (!some) continue;
+        o += row * (at & 1 ? ldv : ldk);
 #pragma unroll
         for (int x = 0; x < kReadQuads; ++x) {
-            const int u = at * kReadChunk + x * 256 + threadIdx.x;
-            const bool is_k = u < quads;
-            float* o = is_k ? k : v;
-            if (u >= 2 * quads || !o) continue;
-            o += row * (is_k ? ldk : ldv) + static_cast<int64_t>(is_k ? u : u - quads) * 4;
-            const uint32_t four = now[x] >> ((u & 1) * 16);
-            const float f = __half2float(scale[x]);
-            float y[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = f * static_cast<float>(static_cast<int>((four >> (4 * i)) & 15u) - 8);
-            __stcs(reinterpret_cast<float4*>(o), make_float4(y[0], y[1], y[2], y[3]));
+            const int u = (at >> 1) * kReadChunk + x * 256 + threadIdx.x;
+            if (u >= quads) break;
+            // the quad's two bytes apart: codes 0 and 2 in the low nibbles, 1 and 3 in the next ones
+            const uint32_t bytes = prmt(now[x], 0u, threadIdx.x & 1 ? 0x4342u : 0x4140u);
+            const __half2 sc = __half2half2(scale[x]);
+            const float2 even = __half22float2(__hmul2(__hadd2(half2_bits(and_or(bytes, 0x000F000Fu, 0x64006400u)), half2_bits(0xE408E408u)), sc));
+            const float2 odd = __half22float2(__hmul2(__hadd2(half2_bits(and_or(bytes, 0x00F000F0u, 0x54005400u)), half2_bits(0xD480D480u)), sc));
+            __stcs(reinterpret_cast<float4*>(o) + u, make_float4(even.x, odd.x, even.y, odd.y));   // exact, see code_pairs
         }
     }
 }
@@ -332,7 +334,7 @@ int hesa_cuda_kv4_read(const hesa_cuda_paged_kv4* kv, int32_t layer, const hesa_
     cudaError_t e = status_word(&status);
     if (e == cudaSuccess) {
         // rows for one block after another only where there are blocks for every SM several times over
-        const int64_t chunks = (2 * width / 4 + kReadChunk - 1) / kReadChunk;
+        const int64_t chunks = 2 * ((width / 4 + kReadChunk - 1) / kReadChunk);
         const int rows = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMostRows, batch->n_tokens / (148 * 6))));
         const int64_t y = rows > 1 ? 1 : std::min<int64_t>(chunks, 1024);
         e = launch_dep(kv4_read_kernel, dim3(static_cast<unsigned>((batch->n_tokens + rows - 1) / rows), static_cast<unsigned>(y)), 256, 0, static_cast<cudaStream_t>(stream),
