@@ -593,13 +593,15 @@ struct Scratch {
 };
 
 // Blocks x of gridDim.x share out one sequence's tokens that its rows see, `tokens`
-// (at most 16) at a time, and write the sequence's entries of the tables. A thread
-// takes a word of codes (16 bytes of fp16) of K or V at a time, eight of them under way.
-constexpr int kExpandWords = 8;
+// (at most 16) at a time, and write the sequence's entries of the tables. A thread has
+// a word of the row (or several, 256 apart; where rows are short, that word of every
+// second, third .. token), and takes it of K and of V, kExpandSteps tokens or words
+// under way.
+constexpr int kExpandSteps = 4;
 constexpr int kExpandTokens = 16;
 
 __global__ void __launch_bounds__(256)
-expand_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ Pools4 pools, const __grid_constant__ Scratch w, const FastDiv words_div, int tokens) {
+expand_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ Pools4 pools, const __grid_constant__ Scratch w, int tokens) {
     __shared__ int64_t s_from[kExpandTokens];   // first group of the token's K, -1: no page
     grid_dep_wait();
     grid_dep_launch();
@@ -612,6 +614,8 @@ expand_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ Pools4
     const int32_t prefix = A.prefix ? max(0, min(A.prefix[seq], sv.len)) : 0;
     const int32_t first = A.window > 0 ? max(0, sv.len - sv.n_new + 1 - A.window) : 0;   // the first key in a window
     const int row_words = A.c.n_kv * A.c.head_dim / 8;
+    const int abreast = max(1, 256 / row_words);                        // tokens that the block's threads take at a time
+    const int tok = row_words < 256 ? threadIdx.x / row_words : 0, word = threadIdx.x - tok * row_words;
     const int32_t* table = A.c.table + static_cast<int64_t>(sv.slot) * A.c.max_pages;
     const int64_t base = static_cast<int64_t>(seq) * w.pages * kScratchPage;
     for (int64_t start = static_cast<int64_t>(blockIdx.x) * tokens; start < sv.len; start += static_cast<int64_t>(gridDim.x) * tokens) {
@@ -627,32 +631,43 @@ expand_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ Pools4
             s_from[threadIdx.x] = good ? page * A.c.page_stride + static_cast<int64_t>(j - pi * A.c.page_size) * (row_words / 4) : -1;
         }
         __syncthreads();
-        const int all = n * 2 * row_words;
-        for (int u0 = threadIdx.x; u0 < all; u0 += kExpandWords * blockDim.x) {
-            uint32_t code[kExpandWords];
-            __half d[kExpandWords];
+        if (tok >= abreast) continue;
+        int t = tok, at = word;   // the next token and word
+        while (t < n) {
+            uint32_t code[2][kExpandSteps];
+            __half d[2][kExpandSteps];
+            int64_t to[kExpandSteps];
 #pragma unroll
-            for (int x = 0; x < kExpandWords; ++x) {
-                const int u = u0 + x * static_cast<int>(blockDim.x);
-                if (u >= all) break;
-                const int half = words_div.div(u), at = u - half * row_words;   // K, then V of each token
-                const int64_t from = s_from[half >> 1];
-                code[x] = 0x88888888u;
-                d[x] = __float2half_rn(0.f);
-                if (from >= 0) {
-                    code[x] = __ldcs(reinterpret_cast<const uint32_t*>((half & 1 ? pools.v : pools.k) + from) + at);
-                    d[x] = ((half & 1 ? pools.vs : pools.ks) + from)[at / 4];
+            for (int x = 0; x < kExpandSteps; ++x) {
+                to[x] = -1;
+                if (t >= n) continue;
+                const int64_t from = s_from[t];
+                to[x] = (base + j0 + t) * row_words + at;
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    code[p][x] = 0x88888888u;
+                    d[p][x] = __float2half_rn(0.f);
+                    if (from >= 0) {
+                        code[p][x] = __ldcs(reinterpret_cast<const uint32_t*>((p ? pools.v : pools.k) + from) + at);
+                        d[p][x] = ((p ? pools.vs : pools.ks) + from)[at / 4];
+                    }
+                }
+                at += 256;
+                if (at >= row_words) {
+                    at = word;
+                    t += abreast;
                 }
             }
 #pragma unroll
-            for (int x = 0; x < kExpandWords; ++x) {
-                const int u = u0 + x * static_cast<int>(blockDim.x);
-                if (u >= all) break;
-                const int half = words_div.div(u), at = u - half * row_words;
-                uint32_t p[4];
-                code_pairs(code[x], __half2half2(d[x]), p);   // (0, 4) (1, 5) (2, 6) (3, 7)
-                reinterpret_cast<uint4*>(half & 1 ? w.v : w.k)[(base + j0 + (half >> 1)) * row_words + at] =
-                    make_uint4(prmt(p[0], p[1], 0x5410u), prmt(p[2], p[3], 0x5410u), prmt(p[0], p[1], 0x7632u), prmt(p[2], p[3], 0x7632u));
+            for (int x = 0; x < kExpandSteps; ++x) {
+                if (to[x] < 0) continue;
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    uint32_t v[4];
+                    code_pairs(code[p][x], __half2half2(d[p][x]), v);   // (0, 4) (1, 5) (2, 6) (3, 7)
+                    reinterpret_cast<uint4*>(p ? w.v : w.k)[to[x]] = make_uint4(prmt(v[0], v[1], 0x5410u), prmt(v[2], v[3], 0x5410u),
+                                                                               prmt(v[0], v[1], 0x7632u), prmt(v[2], v[3], 0x7632u));
+                }
             }
         }
     }
@@ -822,10 +837,10 @@ int hesa_cuda_paged_attention_kv4(const hesa_cuda_paged_kv4* kv, int32_t layer, 
             o.prefix = options && options->prefix ? options->prefix + i : nullptr;
             a.prefix = o.prefix;
             // as many tokens a block as its threads have words under way for; blocks for every SM, as far as there are tokens for them
-            const int row_words = kv->n_kv_head * kv->head_dim / 8, tokens = std::max(1, std::min(kExpandTokens, kExpandWords * 256 / (2 * row_words)));
+            const int row_words = kv->n_kv_head * kv->head_dim / 8, tokens = std::max(1, std::min(kExpandTokens, kExpandSteps * 256 / row_words));
             const int share = std::max(1, std::min((batch->max_len + tokens - 1) / tokens, (148 * 16 + b.n_seq - 1) / b.n_seq));
             e = launch_dep(expand_kernel, dim3(static_cast<unsigned>(share), static_cast<unsigned>(b.n_seq)), 256, 0, s, a, pools,
-                           Scratch{static_cast<__half*>(c.k), static_cast<__half*>(c.v), c.table, c.seq_len, p.pages}, FastDiv(row_words), tokens);
+                           Scratch{static_cast<__half*>(c.k), static_cast<__half*>(c.v), c.table, c.seq_len, p.pages}, tokens);
             if (e != cudaSuccess) break;
             rc = hesa_cuda_paged_attention(&c, 0, &b, q, ldq, out, ldo, n_head, &o, ws + used, workspace_bytes - used, stream);
             if (rc != HESA_CUDA_OK) return rc;
