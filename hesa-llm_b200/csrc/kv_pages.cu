@@ -12,7 +12,9 @@
 // Measured: compaction that moves 240 pages of 32 layers 180 us (1.0 GB; the plan
 // takes 7 us of them, the copies run at 6 TB/s); free, fork and reserve of seven
 // slots of up to 44 pages 19 us for the four launches, which are chains of dependent
-// reads by one block; the cache write of 5296 tokens (32 heads) 67.8 us
+// reads by one block; reordering the beams of 32 sequences of 4 (32 layers, 50 to 400
+// tokens) 34 us, 17 of them the copies (117 MB, 6.8 TB/s) and 14 the plan, of one
+// sequence 14 us; the cache write of 5296 tokens (32 heads) 67.8 us
 // (437 MB, 6.4 TB/s), of 32 tokens (64 heads on 8) 3.4 us.
 #include "paged.h"
 #include "abi_errors.h"

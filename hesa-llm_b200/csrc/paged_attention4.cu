@@ -3,27 +3,44 @@
 // The formulas, rows, tiles, masks and the equal runs of work are those of
 // paged_attention.cu; a value is d (code - 8), an fp16 number exactly.
 //
-// rows4_kernel: tiles of 8 rows, for the next tokens of a decode step. A warp has
-// a kv head of its own and takes blocks of 32 keys of it: their codes and scales
-// come by 16-byte asynchronous copies into a ring of the warp's own (no barrier
-// between warps), a few blocks ahead, also of the next run.
+// rows4_kernel: tiles of 8 rows, for the next tokens of a decode step. A warp has a
+// kv head of its own and takes blocks of 32 keys of it. Four more warps copy codes and
+// scales of all heads of the block's tokens (they lie side by side) into a ring, with
+// 16-byte asynchronous copies that put every key's row where the warps' reads meet no
+// bank twice (k_at, v_at), and run ahead across sequences. (When every warp copied
+// its own head's blocks, copies were a sixth of its instructions: two contexts of
+// 131072 and 100001 tokens, 64 heads on 8, 110 us and 103.)
 //   * codes become fp16 pairs in registers, in the places of the operands of
 //     m16n8k16 products: the order of dims within a sum is free, so the thread
 //     that needs keys of column n and dims of quarter c takes 16 consecutive bytes
 //     of key n (head_dim 128: a whole group, one scale), and q is read in that
-//     order. For P V a pair has two keys: one byte permutation of two keys' words
+//     order, from shared memory (in registers it made the warps spill: 196 us and
+//     112). For P V a pair has two keys: one byte permutation of two keys' words
 //     brings them together, and the thread of column n takes head_dim / 8
-//     consecutive dims. Half an instruction a value puts the codes in place, half
-//     one puts them behind the bits of 16, half one is the exact fma by the scale.
+//     consecutive dims. code_pairs and code_pairs_fma (paged.h) are the two ways from
+//     codes to values; K takes one, V the other, which loads the pipes most evenly
+//     (both alike: 102 us; so: 100).
 //   * q and P are split into fp16 halves that are the two halves of the A operand
 //     (16 rows), as in paged_attention.cu.
-//   * rows of a warp's block are stored so that eight (or 16, 32) threads read
-//     different banks: see k_at and v_at.
+//   * with fewer heads than warps several warps have a head, take its blocks in turn
+//     and add their sums up in shared memory at a segment's end, so that a sequence
+//     that lies in one CTA's run is written at once.
+// Bound by the warps' instructions and their waits for one another's pipes, not by
+// HBM: a block of 32 keys of one head is 730 instructions of a warp (K 235, V 300,
+// softmax 66), 40% of the time each of the tensor, fp16 and integer pipes; without
+// the copies the kernel takes 90 us, without the products 65. More warps would fill
+// the pipes, but their registers are all taken (32 of a thread's are sums).
+// Measured (with combine_kernel): two contexts of 131072 and 100001 tokens, 64 heads on
+// 8, 100 us (301 MB, 3.0 TB/s; the fp16 cache 167); 32 of 1 to 8192 tokens 30.6 us (34);
+// one of 2048 tokens, 32 heads, 14.5 us (15.4): 5.4 us until the first products, 3 a
+// block, 4 to join the parts.
 //
 // Chunks: the tokens of a few sequences at a time are laid out in fp16 in the
 // workspace (values are fp16 numbers, nothing is rounded) as a cache of their own,
 // and the kernel of paged_attention_tc.cu reads that. A chunk's keys are read once
-// for each of its many tiles, so the pass before costs a few percent.
+// for each of its many tiles, so the pass before costs little: 2048 tokens at 16384, 64
+// heads on 8, 1.76 ms (fp16 1.75); 512 at 2048, 32 heads, 48 us (41); 12 mixed chunks 40
+// us (36).
 #include "paged.h"
 #include "paged_rows.cuh"
 #include "paged_tc.h"
