@@ -193,14 +193,6 @@ constexpr int kCluster = 8;
 constexpr int64_t kClusterElems = 24576;                               // logits of a part
 constexpr int64_t kClusterSeqs = 148 * 4 / kCluster;                   // that are on the SMs at a time
 
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t in_block(const void* p, int rank) {   // the address of the same thing in block `rank` of the cluster
-    uint32_t a;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
-    return a;
-}
 __device__ __forceinline__ uint64_t lds_cluster(uint32_t a) {
     unsigned long long v;
     asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
@@ -256,23 +248,6 @@ int cluster_parts(int64_t n_seq, int32_t width, int64_t vocab) {
     return width <= kCluster && n_seq <= kClusterSeqs && vocab <= parts * kClusterElems ? parts : 0;
 }
 
-cudaError_t launch_clusters(int64_t n_seq, cudaStream_t s, const float* logits, int64_t ld, int vocab, const float* scores, const int32_t* ended, int width, int top,
-                            int n_split, const BeamOut& out) {
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = kCluster;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(n_seq * kCluster));
-    cfg.blockDim = dim3(kLpThreads);
-    cfg.stream = s;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, beam_cluster_kernel, logits, ld, vocab, scores, ended, width, top, n_split, out);
-}
-
 bool shape_ok(int64_t n_seq, int32_t width, int64_t vocab) {
     return n_seq >= 0 && width >= 1 && width <= kMaxWidth && vocab > 0 && vocab < (int64_t(1) << 30) && n_seq < (int64_t(1) << 31) / kMaxWidth;
 }
@@ -307,7 +282,8 @@ int hesa_cuda_beam_select(const float* logits, int64_t ld, int64_t n_seq, int32_
     const int top = static_cast<int>(std::min<int64_t>(width, vocab)), n_split = parts_of(rows, vocab), in_cluster = cluster_parts(n_seq, width, vocab);
     const BeamOut out{next_scores, parents, tokens};
     if (in_cluster > 0) {
-        const cudaError_t e = launch_clusters(n_seq, static_cast<cudaStream_t>(stream), logits, ld, static_cast<int>(vocab), scores, ended, width, top, in_cluster, out);
+        const cudaError_t e = launch_clusters(beam_cluster_kernel, kCluster, dim3(static_cast<unsigned>(n_seq * kCluster)), kLpThreads, 0, static_cast<cudaStream_t>(stream),
+                                              logits, ld, static_cast<int>(vocab), scores, ended, width, top, in_cluster, out);
         return e == cudaSuccess ? HESA_CUDA_OK : record_cuda_error(e, "beam_select kernel");
     }
     RowPart* parts = static_cast<RowPart*>(workspace);

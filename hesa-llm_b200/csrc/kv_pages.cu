@@ -3,7 +3,7 @@
 //
 // The tables (pages of each slot, tokens of each slot, references of each page)
 // live on the device, so a serving loop changes them between two steps without
-// reading anything back. One block plans a change: it checks every slot, page
+// reading anything back. One block (or one cluster of blocks) plans a change: it checks every slot, page
 // and length that the change touches, and only when all are sound writes the
 // tables; else it records a device status and changes nothing. Free pages are
 // taken in ascending order, so results do not depend on scheduling. What is to
@@ -13,7 +13,7 @@
 // takes 7 us of them, the copies run at 6 TB/s); free, fork and reserve of seven
 // slots of up to 44 pages 19 us for the four launches, which are chains of dependent
 // reads by one block; reordering the beams of 32 sequences of 4 (32 layers, 50 to 400
-// tokens) 34 us, 17 of them the copies (117 MB, 6.8 TB/s) and 14 the plan, of one
+// tokens) 35 us, 19 of them the copies (117 MB, 6.2 TB/s) and 14 the plan, of one
 // sequence 14 us; the cache write of 5296 tokens (32 heads) 67.8 us
 // (437 MB, 6.4 TB/s), of 32 tokens (64 heads on 8) 3.4 us.
 #include "paged.h"
@@ -28,6 +28,13 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kMaxSlots = 65536;
+
+// Reordering n slots is planned by one block up to this many table entries (n times max_pages),
+// and by a cluster of kPlanBlocks beyond: 32 slots of 126 entries 19.7 us (cluster 21.0), 64 of
+// them 24.6 (22.5), 128 of them 33 (25), 576 of 251 170 (50; a cluster of four 75). The barriers
+// and the start of a cluster cost 3 us of the smallest call.
+constexpr int kPlanBlocks = 8;
+constexpr int64_t kMostEntries = 6000;
 
 struct Tables {
     int32_t* table;      // [n_slots][max_pages]
@@ -76,26 +83,28 @@ __device__ __forceinline__ int block_scan(int x, int* s, int& total) {
     }
     if (lane == 31) s[warp] = v;
     __syncthreads();
-    int before = 0, all = 0;
-    for (int w = 0; w < n_warp; ++w) {
-        const int y = s[w];
-        before += w < warp ? y : 0;
-        all += y;
-    }
+    const int y = lane < n_warp ? s[lane] : 0;
+    const int before = __reduce_add_sync(0xffffffffu, lane < warp ? y : 0);
+    total = __reduce_add_sync(0xffffffffu, y);
     __syncthreads();
-    total = all;
     return before + v - x;
 }
 
-// The lowest `want` free pages into list, ascending; false when there are fewer.
+// The lowest `want` free pages into list, ascending; false when there are fewer. A thread looks at several
+// pages side by side: a pass over the block costs a read's latency, a scan and three barriers.
+constexpr int kFreeAhead = 8;
+
 __device__ bool lowest_free(const Tables& t, int want, int32_t* list, int* s) {
     int found = 0;
-    for (int b = 0; b < t.n_pages && found < want; b += kPlanThreads) {
-        const int i = b + threadIdx.x;
-        const bool is_free = i < t.n_pages && t.refs[i] == 0;
+    for (int64_t b = 0; b < t.n_pages && found < want; b += kPlanThreads * kFreeAhead) {
+        const int64_t first = b + threadIdx.x * kFreeAhead;
+        uint32_t is_free = 0;
+#pragma unroll
+        for (int k = 0; k < kFreeAhead; ++k)
+            if (first + k < t.n_pages && t.refs[first + k] == 0) is_free |= 1u << k;
         int total;
-        const int at = found + block_scan(is_free ? 1 : 0, s, total);
-        if (is_free && at < want) list[at] = i;
+        int at = found + block_scan(__popc(is_free), s, total);
+        for (; is_free && at < want; is_free &= is_free - 1) list[at++] = static_cast<int32_t>(first) + __ffs(is_free) - 1;
         found += total;
     }
     __syncthreads();
@@ -281,18 +290,40 @@ fork_plan_kernel(const Tables t, const int32_t* src, const int32_t* dst, int n, 
     if (threadIdx.x == 0) *w.n_items = n;
 }
 
+// The blocks that plan together: one, or a cluster. `mine` of `all` warps.
+template <int BLOCKS> struct Team {
+    int rank, mine;
+    static constexpr int all = kPlanThreads / 32 * BLOCKS;
+    int* flags;   // a word for each vote, zeros, in every block
+    __device__ explicit Team(int* votes) : rank(BLOCKS > 1 ? blockIdx.x : 0), mine(rank * (kPlanThreads / 32) + (threadIdx.x >> 5)), flags(votes) {}
+    __device__ __forceinline__ void sync() const {
+        if constexpr (BLOCKS > 1) cluster_sync();
+        else __syncthreads();
+    }
+    // x of any thread; what they wrote before is seen after it
+    __device__ __forceinline__ bool any(bool x, int vote) const {
+        x = __syncthreads_or(x);
+        if constexpr (BLOCKS > 1) {
+            if (x && threadIdx.x < BLOCKS) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(in_block(flags + vote, threadIdx.x)), "r"(1) : "memory");
+            cluster_sync();
+            x = *static_cast<volatile int*>(flags + vote) != 0;
+        }
+        return x;
+    }
+};
+
 // The pages of the listed slots, by what becomes of them. kDrop: those of slots that no
 // slot takes over lose a reference each; kGiveBack undoes that (what is not sound has
-// no reference changed); kKept: those of the other slots have references left. False
+// no reference changed); kKept: those of the other slots have references left. True
 // where a length or a page is not sound, or there is no reference to take or left.
 // A warp takes kSlotsAhead slots at a time, whose reads go side by side, its lanes
-// their pages. All threads of the block; a barrier at the end.
+// their pages; with few slots 2^share warps have a slot.
 enum Refs { kDrop, kGiveBack, kKept };
 constexpr int kSlotsAhead = 4;
 
-template <Refs MODE>
-__device__ bool slot_refs(const Tables& t, const int32_t* slots, const int32_t* parents, int n, int width) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, step = kPlanThreads / 32;
+template <Refs MODE, typename T>
+__device__ bool slot_refs(const Tables& t, const T& team, int share, const int32_t* slots, const int32_t* parents, int n, int width) {
+    const int lane = threadIdx.x & 31, step = T::all >> share, cols = 32 << share, col = (team.mine * 32 + lane) & (cols - 1);
     bool bad = false;
     auto look = [&](int p, bool mine) {
         if (p < 0 || p >= t.n_pages) bad = true;
@@ -301,9 +332,10 @@ __device__ bool slot_refs(const Tables& t, const int32_t* slots, const int32_t* 
         else if (MODE == kGiveBack) atomicAdd(&t.refs[p], 1);
         else bad |= t.refs[p] <= 0;
     };
-    for (int i0 = warp; i0 < n; i0 += kSlotsAhead * step) {
+    for (int i0 = team.mine >> share; i0 < n; i0 += kSlotsAhead * step) {
         const int32_t* row[kSlotsAhead];
-        int np[kSlotsAhead], first[kSlotsAhead];
+        uint32_t np[kSlotsAhead];
+        int first[kSlotsAhead];
         bool mine[kSlotsAhead];
 #pragma unroll
         for (int k = 0; k < kSlotsAhead; ++k) {
@@ -317,78 +349,91 @@ __device__ bool slot_refs(const Tables& t, const int32_t* slots, const int32_t* 
             mine[k] = __any_sync(0xffffffffu, par == b) == (MODE == kKept);
         }
 #pragma unroll
-        for (int k = 0; k < kSlotsAhead; ++k) first[k] = lane < np[k] ? row[k][lane] : 0;
+        for (int k = 0; k < kSlotsAhead; ++k) first[k] = col < np[k] ? row[k][col] : 0;
 #pragma unroll
         for (int k = 0; k < kSlotsAhead; ++k) {
-            if (lane < np[k]) look(first[k], mine[k]);
-            for (int j = lane + 32; j < np[k]; j += 32) look(row[k][j], mine[k]);
+            if (col < np[k]) look(first[k], mine[k]);
+            for (uint32_t j = col + cols; j < np[k]; j += cols) look(row[k][j], mine[k]);
         }
     }
-    return !__syncthreads_or(bad);
+    return bad;
 }
 
 // Slot b of a group becomes what slot parents[b] of it was. References that go are taken first, so that the pages
-// they free can be taken for the copies, then those that come are added. The table's entries of a group are changed by
-// one warp: a lane has one slot's in some columns, and a slot's new entries are the old ones of its parent's lane; a
-// column is read before it is written, by the same warp. Bound by latency: a chain of dependent reads in one block.
+// they free can be taken for the copies, then those that come are added. The table's entries of a group's columns are
+// changed by one warp: a lane has one slot's in some columns, and a slot's new entries are the old ones of its parent's
+// lane; a column is read before it is written, by the same warp. Bound by latency: a chain of dependent reads.
 constexpr int kColumnSteps = 8;   // reads of a row that a lane has under way
 
+template <int BLOCKS>
 __global__ void __launch_bounds__(kPlanThreads)
-reorder_plan_kernel(const Tables t, const int32_t* slots, const int32_t* parents, int n, int width, PageWork w) {
+reorder_plan_kernel(const Tables t, const int32_t* slots, const int32_t* parents, int n, int width, int slot_share, int group_share, PageWork w) {
+    __shared__ uint32_t bits[kMaxSlots / 32];
+    __shared__ int s[33], votes[4];
+    const Team<BLOCKS> team(votes);
+    if (BLOCKS > 1) {
+        if (threadIdx.x < 4) votes[threadIdx.x] = 0;
+        team.sync();   // every block is there, with its votes at 0
+    }
     grid_dep_wait();
     grid_dep_launch();
-    __shared__ uint32_t bits[kMaxSlots / 32];
-    __shared__ int s[33];
-    if (threadIdx.x == 0) *w.n_items = 0;
-    bool bad = !mark_slots(slots, n, t.n_slots, bits);
+    const bool lead = team.rank == 0;
+    if (lead && threadIdx.x == 0) *w.n_items = 0;
+    bool bad = !mark_slots(slots, n, t.n_slots, bits);   // each block all of them, and the parents
     for (int i = threadIdx.x; i < n && !bad; i += kPlanThreads) bad = parents[i] < 0 || parents[i] >= width;
-    if (__syncthreads_or(bad)) return refuse(t, kStatusBadPosition);
-    if (!slot_refs<kDrop>(t, slots, parents, n, width) || !slot_refs<kKept>(t, slots, parents, n, width)) {
-        slot_refs<kGiveBack>(t, slots, parents, n, width);
-        return refuse(t, kStatusBadPosition);
+    const bool listed = !__syncthreads_or(bad);
+    if (team.any(!listed || slot_refs<kDrop>(t, team, slot_share, slots, parents, n, width), 0) ||
+        team.any(slot_refs<kKept>(t, team, slot_share, slots, parents, n, width), 1)) {
+        if (listed) slot_refs<kGiveBack>(t, team, slot_share, slots, parents, n, width);
+        if (lead) refuse(t, kStatusBadPosition);
+        return;
     }
     // a slot whose parent has a partly filled page and an earlier child gets a page of its own
     int total = 0;
-    for (int b = 0; b < n; b += kPlanThreads) {
-        const int i = b + threadIdx.x;
-        bool copy = false;
-        if (i < n) {
-            const int g = i - i % width, par = parents[i];
-            for (int x = g; x < i; ++x) copy |= parents[x] == par;
-            copy = copy && t.seq_len[slots[g + par]] % t.page_size != 0;
+    if (lead) {
+        for (int b = 0; b < n; b += kPlanThreads) {
+            const int i = b + threadIdx.x;
+            bool copy = false;
+            if (i < n) {
+                const int g = i - i % width, par = parents[i];
+                for (int x = g; x < i; ++x) copy |= parents[x] == par;
+                copy = copy && t.seq_len[slots[g + par]] % t.page_size != 0;
+            }
+            int all;
+            const int at = block_scan(copy ? 1 : 0, s, all);
+            if (i < n) w.start[i] = copy ? total + at : -1;
+            total += all;
         }
-        int all;
-        const int at = block_scan(copy ? 1 : 0, s, all);
-        if (i < n) w.start[i] = copy ? total + at : -1;
-        total += all;
+        bad = total > t.n_pages || !lowest_free(t, total, w.list, s);
     }
-    if (total > t.n_pages || !lowest_free(t, total, w.list, s)) {
-        slot_refs<kGiveBack>(t, slots, parents, n, width);
-        return refuse(t, kStatusNoPages);
+    if (team.any(bad, 2)) {
+        slot_refs<kGiveBack>(t, team, slot_share, slots, parents, n, width);
+        if (lead) refuse(t, kStatusNoPages);
+        return;
     }
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cols = 32 / width;   // columns of the table a warp has in hand at a time
+    const int lane = threadIdx.x & 31, cols = 32 / width;   // columns of the table a warp has in hand at a time
+    const int part = team.mine & ((1 << group_share) - 1), step = kColumnSteps * cols;   // of the 2^group_share warps of a group
     const int beam = lane % width, col = lane / width;
-    for (int g = warp * width; g < n; g += kPlanThreads / 32 * width) {
+    int new_slot = -1, new_len = 0;
+    for (int g = (team.mine >> group_share) * width; g < n; g += (team.all >> group_share) * width) {
         const int par = parents[g + beam], slot = slots[g + beam];
         const int old_len = t.seq_len[slot], len = __shfl_sync(0xffffffffu, old_len, par);
-        const int old_pages = pages_for(old_len, t.page_size), pages = pages_for(len, t.page_size), full = len / t.page_size;
+        const uint32_t old_pages = pages_for(old_len, t.page_size), pages = pages_for(len, t.page_size), full = len / t.page_size;
         const int take = w.start[g + beam], fresh = take >= 0 ? w.list[take] : -1;
         bool later = false;   // the parent has an earlier child
         for (int x = 0; x < beam; ++x) later |= parents[g + x] == par;
         int32_t* row = t.table + static_cast<int64_t>(slot) * t.max_pages;
-        int most = max(old_pages, pages);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-        for (int j0 = 0; j0 < most; j0 += kColumnSteps * cols) {
+        const uint32_t most = __reduce_max_sync(0xffffffffu, max(old_pages, pages));
+        for (uint32_t j0 = part * step; j0 < most; j0 += step << group_share) {
             int old[kColumnSteps];
 #pragma unroll
             for (int k = 0; k < kColumnSteps; ++k) {
-                const int j = j0 + k * cols + col;
+                const uint32_t j = j0 + k * cols + col;
                 old[k] = col < cols && j < old_pages ? row[j] : -1;
             }
 #pragma unroll
             for (int k = 0; k < kColumnSteps; ++k) {
-                const int j = j0 + k * cols + col;
+                const uint32_t j = j0 + k * cols + col;
                 const int from = __shfl_sync(0xffffffffu, old[k], col < cols ? col * width + par : lane);
                 if (col >= cols || j >= most) continue;
                 if (j < pages) {
@@ -409,9 +454,16 @@ reorder_plan_kernel(const Tables t, const int32_t* slots, const int32_t* parents
             }
         }
         __syncwarp();
-        if (col == 0) t.seq_len[slot] = len;
+        if (col == 0 && part == 0) {
+            if (group_share == 0) t.seq_len[slot] = len;
+            else new_slot = slot, new_len = len;   // once the group's other warps have read it
+        }
     }
-    if (threadIdx.x == 0) *w.n_items = total;
+    if (group_share > 0) {   // each warp has had one group at most
+        team.sync();
+        if (new_slot >= 0) t.seq_len[new_slot] = new_len;
+    }
+    if (lead && threadIdx.x == 0) *w.n_items = total;
 }
 
 // live pages to the front: free pages below n_live take the pages in use from n_live on
@@ -782,6 +834,13 @@ int kv_copy_pages(const KV* kv, const int32_t* src_pages, const int32_t* dst_pag
     return e == cudaSuccess ? HESA_CUDA_OK : record_cuda_error(e, "kv_copy_pages kernels");
 }
 
+// Warps that share one of n things, none with less than a step of `columns` of the table: the logarithm of a power of two
+int share_of(int warps, int n, int32_t max_pages, int columns) {
+    int x = 0;
+    while ((warps >> (x + 1)) >= n && max_pages > static_cast<int64_t>(columns) << x) ++x;
+    return x;
+}
+
 template <typename KV>
 int kv_reorder(const KV* kv, const int32_t* slots, const int32_t* parents, int32_t n, int32_t width, void* workspace, size_t workspace_bytes,
                void* stream) {
@@ -797,7 +856,11 @@ int kv_reorder(const KV* kv, const int32_t* slots, const int32_t* parents, int32
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t e = status_word(&t.status);
     if (e == cudaSuccess) {
-        e = launch_dep(reorder_plan_kernel, dim3(1), kPlanThreads, 0, s, t, slots, parents, n, width, w);
+        const bool wide = static_cast<int64_t>(n) * kv->max_pages > kMostEntries;
+        const int blocks = wide ? kPlanBlocks : 1, warps = kPlanThreads / 32 * blocks;
+        e = launch_clusters(wide ? reorder_plan_kernel<kPlanBlocks> : reorder_plan_kernel<1>, blocks, dim3(blocks), kPlanThreads, 0, s, t, slots, parents, n, width,
+                            share_of(warps, n, kv->max_pages, 32),
+                            share_of(warps, n / width, kv->max_pages, kColumnSteps * (32 / width)), w);
     }
     if (e == cudaSuccess) e = launch_copy(kv, t, w, n, nullptr, s);
     return e == cudaSuccess ? HESA_CUDA_OK : record_cuda_error(e, "kv_reorder kernels");

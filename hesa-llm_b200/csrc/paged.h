@@ -221,19 +221,27 @@ __device__ __forceinline__ void split_away2(float x0, float x1, uint32_t& hi, ui
 // grid_dep_wait, also one with nothing to do (the grid must not end before the one
 // it follows), before it writes anything, and reads what earlier kernels wrote with
 // plain loads (no read-only cache: the grid may be older than the data).
+// cluster: blocks of a cluster, 1 for none.
 template <typename... P, typename... T>
-cudaError_t launch_dep(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, T... args) {
-    cudaLaunchAttribute attr[1];
+cudaError_t launch_clusters(void (*kernel)(P...), int cluster, dim3 grid, int threads, size_t smem, cudaStream_t s, T... args) {
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(static_cast<unsigned>(threads));
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+template <typename... P, typename... T>
+cudaError_t launch_dep(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, T... args) {
+    return launch_clusters(kernel, 1, grid, threads, smem, s, args...);
 }
 
 // The host's checks of a cache and a batch (paged_attention.cu): 0, or an error

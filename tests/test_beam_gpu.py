@@ -296,6 +296,58 @@ def test_reorder_of_many_slots(H):
             x.copy_(k)
 
 
+@pytest.mark.parametrize("width,groups,most,page", [(12, 1, 300, 1), (5, 4, 300, 1), (12, 4, 300, 1), (32, 1, 900, 1), (2, 40, 333, 2), (1, 30, 400, 1), (7, 3, 4097, 3)])
+def test_reorder_of_long_rows(H, width, groups, most, page):
+    """Rows that several warps share, and enough entries for several blocks; then a row that is not sound, and too few pages."""
+    r = random.Random(most + width)
+    n = width * groups
+    cache, pools, t, m = random_cache(H, r, "kv4", n + 3, page, layers=2, n_kv=1, most=most, spare=2 * n)
+    slots = r.sample(range(n + 3), n)
+
+    def call(parents):
+        H.kv_reorder(cache, torch.tensor(slots, dtype=torch.int32, device="cuda"), torch.tensor(parents, dtype=torch.int32, device="cuda"), width)
+    for step in range(3):
+        parents = [r.randrange(width) for _ in slots]
+        before = [p.clone() for p in pools]
+        copies = m.reorder(slots, parents, width)
+        assert copies is not None
+        call(parents)
+        assert H.device_status() == 0
+        same_tables(t, m)
+        for p, b in zip(pools, before):
+            want = b.clone()
+            for frm, to, places in copies:
+                want[:, to, :places] = b[:, frm, :places]
+            assert torch.equal(p, want)
+    slot = max(slots, key=lambda x: m.lens[x])   # the last page of the longest row
+    at = m.used(m.lens[slot]) - 1
+    kept = t[0][slot, at].item()
+    for bad in (-1, cache.n_pages):
+        t[0][slot, at] = bad
+        now = [x.clone() for x in t]
+        call([0] * n)
+        assert H.device_status() == 3 and all(torch.equal(a, b) for a, b in zip(t, now))
+        H.clear_device_status()
+    t[0][slot, at] = kept
+    if page > 1 and width > 1:   # pages are partly filled, and none is free
+        first = slots[0]
+        t[1][first] -= 1 if m.lens[first] % page != 1 else 0
+        t[2].add_(1)
+        now = [x.clone() for x in t]
+        call([0] * n)
+        lens = [t[1][x].item() for x in slots]
+        assert any(x % page for x in lens[::width])
+        assert H.device_status() == (3 if min(lens) < 0 else 5) and all(torch.equal(a, b) for a, b in zip(t, now))
+        H.clear_device_status()
+        slot = max(slots, key=lambda x: m.lens[x])   # the same with no length below zero
+        t[1][first] = m.lens[first]
+        t[1][slot] -= 1 if m.lens[slot] % page != 1 else 0
+        now = [x.clone() for x in t]
+        call([slots.index(slot) % width] * n)
+        assert H.device_status() == 5 and all(torch.equal(a, b) for a, b in zip(t, now))
+        H.clear_device_status()
+
+
 @pytest.mark.parametrize("kind", ["fp16", "kv4"])
 def test_reorder_refusals_change_nothing(H, kind):
     r = random.Random(3)
