@@ -562,7 +562,7 @@ rows4_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ Pools4 
     grid_dep_wait();
     grid_dep_launch();   // combine_kernel may be set up meanwhile; it waits for this grid's end
     const int64_t units = tile_units<S::warps + kCopyWarps4, kKeys4>(A, hg, tiles, s_pre, s_sum) * hg.groups;
-    const Runs runs(units, gridDim.x);
+    const Runs runs(units, gridDim.x, hg.least);
     const bool listed_by_tile = by_tile(tiles, whole);
     Cut* cuts = reinterpret_cast<Cut*>(A.part);
     int64_t u = 0, end = 0;
@@ -705,6 +705,19 @@ struct Plan4 {
 
 int warps4(int head_dim) { return head_dim == 256 ? Rows4Shape<256>::warps : Rows4Shape<128>::warps; }
 
+// Whether groups of half as many heads, with `subs` warps a head, are better: for few
+// segments, (tile, group)s, since each costs a start, and few blocks, since copies of
+// fewer heads are narrower. 8 heads of 128 a group and 4: one sequence of 30000
+// tokens, 64 heads on 8, 32 us and 27, two of 131072 and 100001 100 and 104, eight of
+// up to 8192 22.5 and 19.1, 32 of them 33.5 and 33.2, 32 of 8192 99.8 and 106; 32 heads, ten of up to 1000 22.1
+// and 23.1, 14 of 2 tokens 11.7 and 13.2 (16 heads: 14.2, 2: 18.1). Groups of 2: one of
+// 2048, 64 heads on 8, 15.8 and 15.0, 32 heads 14.6 and 15.5.
+bool halve_heads(int64_t segments, int64_t blocks, int subs) {
+    const int64_t work = segments * blocks;
+    if (subs > 4) return segments <= 16 && work <= 1000;
+    return (segments <= 32 && work <= 8192) || (segments <= 64 && (work <= kRowsCtas));
+}
+
 // How a call is cut: from the host's bounds alone, so that a captured graph
 // serves every later length within them.
 Plan4 make_plan4(const hesa_cuda_paged_kv4* kv, const hesa_cuda_token_batch* b, int64_t n_head) {
@@ -726,7 +739,7 @@ Plan4 make_plan4(const hesa_cuda_paged_kv4* kv, const hesa_cuda_token_batch* b, 
     const int64_t blocks = std::max<int64_t>(1, (b->max_len + kKeys4 - 1) / kKeys4);
     static_assert(4 * kRowsCtas <= kMostTiles, "a list for every (tile, group) where groups are made smaller");
     p.heads = warps4(kv->head_dim);
-    while (p.heads > 2 && tiles * ((kv->n_kv_head + p.heads - 1) / p.heads) * blocks < 2 * kRowsCtas) p.heads /= 2;
+    while (p.heads > 2 && halve_heads(tiles * ((kv->n_kv_head + p.heads / 2 - 1) / (p.heads / 2)), blocks, warps4(kv->head_dim) / (p.heads / 2))) p.heads /= 2;
     return p;
 }
 
@@ -784,7 +797,9 @@ cudaError_t launch_rows4(AttnArgs a, const Pools4& pools, const Plan4& p, cudaSt
         if (e != cudaSuccess) return e;
         set[dev] = true;
     }
-    const HeadGroups hg(a.c.n_kv, S::warps, p.heads, kSegCost4), whole = one_warp_a_head(hg);
+    HeadGroups hg(a.c.n_kv, S::warps, p.heads, kSegCost4);
+    if (hg.subs < 4) hg.least = 2;   // a start and a block are few units: 40 sequences of 2 tokens, 32 heads 16.9 us, with 4 22.8
+    const HeadGroups whole = one_warp_a_head(hg);
     for (a.tile0 = 0; a.tile0 < p.tiles && e == cudaSuccess; a.tile0 += kMostTiles) {
         a.n_split = std::min(kMostTiles, p.tiles - a.tile0);
         e = launch_dep(rows4_kernel<HD>, dim3(kRowsCtas), S::threads, S::smem, s, a, pools, hg, whole);

@@ -24,6 +24,7 @@ template <int HD, int WARPS> struct RowParts {
 // Heads of a group (a CTA's warps have one each) and how many warps share a head.
 struct HeadGroups {
     int groups, heads, subs, recip, cost, sub_bits;   // subs is a power of two, `warps` being one
+    int least = kLeastUnits;                          // units of a run
     // `most` heads a group at most, a power of two up to `warps`; starting a (tile, group) takes as long as seg_cost blocks of every warp
     HeadGroups(int n_kv, int warps, int most, int seg_cost) {
         groups = (n_kv + most - 1) / most;
@@ -64,8 +65,8 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
 struct Runs {
     int64_t each, more;
     int n_cta;
-    __device__ __forceinline__ Runs(int64_t units, int most) {
-        n_cta = static_cast<int>(max(int64_t(1), min(static_cast<int64_t>(most), units / kLeastUnits)));
+    __device__ __forceinline__ Runs(int64_t units, int most, int least) {
+        n_cta = static_cast<int>(max(int64_t(1), min(static_cast<int64_t>(most), units / least)));
         each = quotient(units, n_cta);
         more = units - each * n_cta;
     }
