@@ -202,7 +202,7 @@ __device__ __forceinline__ void copy_segment4(const AttnArgs& A, const Pools4& p
         uint32_t to = at_place * ring.stage;
         copy_scales<HD>(s0 + to, pools.ks + at + l * S::groups, pools.vs + at + l * S::groups, good ? S::srow : 0, my_heads);
         const uint4 *kp = pools.k + at + l, *vp = pools.v + at + l;
-        int y = pieces;
+        int y = good ? pieces : 0;   // no reads of any one place in its stead: 148 CTAs' would meet there (74 sequences of 2 tokens, 32 heads: 23 us)
         for (; y >= 4; y -= 4, to += four, kp += 16, vp += 16) copy_four<HD>(k0 + to, k1 + to, v0 + to, v1 + to, kp, vp, 4);
         if (y > 0) copy_four<HD>(k0 + to, k1 + to, v0 + to, v1 + to, kp, vp, y);
         copy_arrive(&ring.full[at_place]);
@@ -315,7 +315,7 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const HeadGroup
     const bool plain = A.cap2 == 0.f && A.slopes == nullptr;
     const float unit = plain ? (sc == 0.f ? FLT_MIN : sc) : 1.f;   // a unit of 0 would make NaN of a hidden key's -inf
 
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = -0.f;   // l stays -0 until there is a block, whose sums are never below +0
     float2 acc[NT];
 #pragma unroll
     for (int i = 0; i < NT; ++i) acc[i] = make_float2(0.f, 0.f);
@@ -500,6 +500,7 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const HeadGroup
             for (int y = 1; y < hg.subs; ++y) {
                 const int w = y * hg.heads + hl;
                 const float2 ml = s_ml[w][n];
+                if (__float_as_uint(ml.y) == 0x80000000u) break;   // a warp without a block, and so are those behind it
                 const float4* theirs = mine + (w - hl) * (S::q / 16);
                 const float top = fmaxf(m, ml.x);
                 // a part that saw nothing adds zeros, or the NaN of a row that is not finite
