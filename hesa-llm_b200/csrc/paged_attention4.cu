@@ -611,12 +611,12 @@ struct Scratch {
 };
 
 // Blocks x of gridDim.x share out one sequence's tokens that its rows see, `tokens`
-// (at most 16) at a time, and write the sequence's entries of the tables. A thread has
+// (at most 64) at a time, and write the sequence's entries of the tables. A thread has
 // a word of the row (or several, 256 apart; where rows are short, that word of every
 // second, third .. token), and takes it of K and of V, kExpandSteps tokens or words
 // under way.
 constexpr int kExpandSteps = 4;
-constexpr int kExpandTokens = 16;
+constexpr int kExpandTokens = 64;
 
 __global__ void __launch_bounds__(256)
 expand_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ Pools4 pools, const __grid_constant__ Scratch w, int tokens) {
@@ -876,8 +876,11 @@ int hesa_cuda_paged_attention_kv4(const hesa_cuda_paged_kv4* kv, int32_t layer, 
             }
             o.prefix = options && options->prefix ? options->prefix + i : nullptr;
             a.prefix = o.prefix;
-            // as many tokens a block as its threads have words under way for; blocks for every SM, as far as there are tokens for them
-            const int row_words = kv->n_kv_head * kv->head_dim / 8, tokens = std::max(1, std::min(kExpandTokens, kExpandSteps * 256 / row_words));
+            // as many tokens a block as its threads have words under way for, but fewer, down to four, where there are not four
+            // blocks for every SM: 49 tokens of eight sequences of up to 262, 64 heads on 8, 22.0 us (up to 16 tokens whatever
+            // their number 24.6), one sequence of 45194, 8 heads on 1, 36.2 (39.1)
+            const int row_words = kv->n_kv_head * kv->head_dim / 8, most = std::max(1, std::min(kExpandTokens, kExpandSteps * 256 / row_words));
+            const int tokens = static_cast<int>(std::min<int64_t>(most, std::max<int64_t>(4, static_cast<int64_t>(b.n_seq) * batch->max_len / (148 * 4))));
             const int share = std::max(1, std::min((batch->max_len + tokens - 1) / tokens, (148 * 16 + b.n_seq - 1) / b.n_seq));
             e = launch_dep(expand_kernel, dim3(static_cast<unsigned>(share), static_cast<unsigned>(b.n_seq)), 256, 0, s, a, pools,
                            Scratch{static_cast<__half*>(c.k), static_cast<__half*>(c.v), c.table, c.seq_len, p.pages}, tokens);
