@@ -564,3 +564,61 @@ def test_a_beam_search(H, kind):
     refs = cache.page_refs.tolist()
     held = [p for s in range(n) for p in cache.table[s, : -(-len(hist[s]) // page)].tolist()]
     assert refs == [held.count(p) for p in range(200)]
+
+
+def test_two_host_threads_at_once(H):
+    """Writes, reads, attention, selection and reordering from two threads, each on a stream of its own with a cache of its own."""
+    import threading
+    r = random.Random(5)
+    work = []
+    for i in range(2):
+        kv, hd, page, vocab = ((2, 64, 4, 5003), (1, 128, 16, 40))[i]
+        n, width = 8, 4
+        cache, pools, t, m = random_cache(H, r, "kv4", n, page, layers=1, n_kv=kv, hd=hd, most=40, spare=40)
+        t[1].fill_(1)
+        t[0].fill_(-1)
+        t[0][:, 0] = torch.arange(n, dtype=torch.int32)
+        t[2].fill_(0)
+        t[2][:n] = 1
+        first = [x.clone() for x in t]
+        for p in pools:   # values that are sound
+            p.zero_()
+        g = torch.Generator(device="cuda").manual_seed(i)
+        batch = H.TokenBatch(torch.arange(n + 1, dtype=torch.int32, device="cuda"), n, 1, 20)
+        work.append(dict(cache=cache, pools=pools, t=t, first=first, batch=batch, n=n, width=width, kv=kv, hd=hd, vocab=vocab, slots=torch.arange(n, dtype=torch.int32, device="cuda"),
+                         one=torch.ones(n, dtype=torch.int32, device="cuda"), x=torch.randn(12, 3, n, kv * hd, generator=g, device="cuda"),
+                         logits=torch.randn(12, n, vocab, generator=g, device="cuda")))
+
+    def search(w):
+        for a, b in zip(w["t"], w["first"]):
+            a.copy_(b)
+        for p in w["pools"]:
+            p.zero_()
+        scores, seen = torch.zeros(w["n"], device="cuda"), []
+        for step in range(12):
+            scores, parents, tokens = H.beam_select(w["logits"][step], scores, w["width"])
+            H.kv_reorder(w["cache"], w["slots"], parents, w["width"])
+            H.kv_reserve(w["cache"], w["slots"], w["one"])
+            q, k, v = w["x"][step]
+            H.rope_kv_paged(w["cache"], 0, w["batch"], None, k, v, w["kv"])
+            seen += [scores, parents, tokens, *H.kv_read(w["cache"], 0, w["batch"]), H.paged_attention(w["cache"], 0, w["batch"], q, w["kv"])]
+        return [x.clone() for x in seen + w["t"]]
+    want = [search(w) for w in work]
+    assert H.device_status() == 0
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(15):
+                got = search(work[i])
+                s.synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    wrong.append(i)
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and H.device_status() == 0

@@ -38,6 +38,37 @@ def test_next_token(n_head, n_kv, hd, page, lens):
     Case(n_head, n_kv, hd, page, lens, [1] * len(lens), seed=n_head + hd).check()
 
 
+@pytest.mark.parametrize("n_head,n_kv,hd,page,lens", [
+    (32, 32, 128, 16, [2] * 74),            # a CTA for each (sequence, group of heads)
+    (32, 32, 128, 16, [1, 2, 3, 40, 33] * 3),
+    (32, 32, 64, 16, [7] * 40),
+    (32, 32, 128, 16, [9001]),
+    (64, 8, 128, 16, [30000]),
+    (64, 8, 128, 16, [8000, 3, 300, 77, 1, 5000, 64, 20]),
+    (4, 4, 256, 16, [2] * 148),
+    (4, 4, 256, 16, [12000]),
+    (12, 12, 128, 24, [300, 1, 33]),        # heads that are no power of two, in groups of six and three
+    (8, 1, 128, 24, [2, 3, 40]),            # a warp with a block, and fifteen of its head without one
+])
+def test_groups_of_heads(n_head, n_kv, hd, page, lens):
+    Case(n_head, n_kv, hd, page, lens, [1] * len(lens), seed=len(lens) + hd).check()
+
+
+@pytest.mark.parametrize("n_head,n_kv,hd", [(8, 2, 64), (12, 2, 128), (8, 4, 256)])
+def test_scratch_may_hold_anything(H, n_head, n_kv, hd):
+    """What the workspace of a chunk holds, NaN among it, changes no bit: places of the fp16 copy that no row sees are zeros."""
+    c = Case(n_head, n_kv, hd, 24, [301, 90, 1000, 129], [70, 90, 100, 1], seed=hd)
+    ws = H.paged_attention_workspace(c.cache, c.batch, n_head)
+    prefix = torch.tensor([3, 0, 200, 40], dtype=torch.int32, device="cuda")
+    for o in (dict(), dict(window=40, prefix=prefix), dict(window=1)):
+        outs = []
+        for byte in (0, 0x7e, 0xfc):   # fp16 0x7e7e is NaN
+            ws.fill_(byte)
+            outs.append(c.run(workspace=ws, **o).clone())
+        assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2]) and bool(torch.isfinite(outs[0]).all())
+    assert H.device_status() == 0
+
+
 @pytest.mark.parametrize("n_head,n_kv,hd,page,lens,news", [
     (4, 4, 128, 16, [512], [512]),                     # a whole prompt
     (8, 2, 128, 16, [700, 50, 33, 257], [130, 50, 0, 1]),
