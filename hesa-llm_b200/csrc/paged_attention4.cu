@@ -31,8 +31,8 @@
 // the copies the kernel takes 90 us, without the products 65. More warps would fill
 // the pipes, but their registers are all taken (32 of a thread's are sums).
 // Measured (with combine_kernel): two contexts of 131072 and 100001 tokens, 64 heads on
-// 8, 100 us (301 MB, 3.0 TB/s; the fp16 cache 167); 32 of 1 to 8192 tokens 30.6 us (34);
-// one of 2048 tokens, 32 heads, 14.5 us (15.4): 5.4 us until the first products, 3 a
+// 8, 100 us (301 MB, 3.0 TB/s; the fp16 cache 167); 32 of 1 to 8192 tokens 29.9 us (34);
+// one of 2048 tokens, 32 heads, 14.3 us (15.4): 5.4 us until the first products, 3 a
 // block, 4 to join the parts.
 //
 // Chunks: the tokens of a few sequences at a time are laid out in fp16 in the
@@ -235,11 +235,17 @@ __device__ __forceinline__ uint32_t lds16(uint32_t a) {
 }
 __device__ __forceinline__ __half2 half2_of(uint32_t x) { return half2_bits(prmt(x, x, 0x1010u)); }
 
+// Where 16-byte piece p of row n of q lies among a warp's eight rows: written by the row and read by the thread (n, c)
+// of a quarter, both without bank conflicts.
+template <int HD> __device__ __forceinline__ int stage_at(int n, int p) {
+    return n * (HD / 4) + (p ^ (HD == 64 ? (n & 1) * 2 + (p >> 3) : (n & 1) * 4 + ((p >> 3) & 3)));
+}
+
 // This warp's head's attention over its blocks of a segment; the first of the
 // head's warps adds up what they have. part < 0: these are all blocks that the rows
 // see, and the result goes to out; else (m, l, acc) go to that part. `used`: blocks
-// of the warp's set so far.
-template <int HD>
+// of the warp's set so far. ONE: no tile has more than one row.
+template <int HD, bool ONE>
 __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const HeadGroups& hg, Ring4<HD>& ring, uint32_t& used, uint8_t* own, float2 (*s_ml)[kRowTile],
                                               const Segment& seg, const TileView& tv, int part) {
     using S = Rows4Shape<HD>;
@@ -247,6 +253,8 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const HeadGroup
     constexpr int VW = HD / 64;                  // words of codes of a column's dims
     constexpr int NT = HD / 8;                   // column tiles of P V
     constexpr int KT = kKeys4 / 8;               // column tiles of Q K^T
+    constexpr int PIECES = HD / 4, STEPS = kRowTile * PIECES / 32;   // 16-byte pieces of a row of q; what a lane has of the warp's eight rows
+    float4* const stage = reinterpret_cast<float4*>(own);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = lane >> 2, c = lane & 3;
     const int sub = hg.sub_of(warp), hl = warp - sub * hg.heads, kvh = seg.grp * hg.heads + hl;
     const SeqView& sv = tv.sv;
@@ -276,6 +284,18 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const HeadGroup
     float qscale;   // 2^e; NaN for a row that is not finite
     {
         const float* q = A.q + static_cast<int64_t>(sv.q0 + t) * A.ldq + static_cast<int64_t>(h) * HD;
+        if constexpr (!ONE) {   // whole rows at a time: a thread's own dims are a line of their own in each load, 1 us for eight heads of eight rows
+            float4 y[STEPS];
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k) {
+                const int row = (k * 32 + lane) / PIECES, piece = (k * 32 + lane) % PIECES;
+                const float* from = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(q), 4 * row));
+                y[k] = tv.r0 + row < tv.n_rows ? reinterpret_cast<const float4*>(from)[piece] : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k) stage[stage_at<HD>((k * 32 + lane) / PIECES, (k * 32 + lane) % PIECES)] = y[k];
+            __syncwarp();
+        }
         float v[KW][8];
         float mx = 0.f;
 #pragma unroll
@@ -283,12 +303,15 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const HeadGroup
             const int d = HD == 256 ? 32 * (c + (w & 4)) + 8 * (w & 3) : (HD / 4) * c + 8 * w;
 #pragma unroll
             for (int i = 0; i < 8; i += 4)
-                *reinterpret_cast<float4*>(v[w] + i) = row_ok ? *reinterpret_cast<const float4*>(q + d + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                *reinterpret_cast<float4*>(v[w] + i) = !ONE     ? stage[stage_at<HD>(n, (d + i) / 4)]
+                                                       : row_ok ? *reinterpret_cast<const float4*>(q + d + i)
+                                                                : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int i = 0; i < 8; ++i) mx = fmax_nan(mx, fabsf(v[w][i]));
         }
         mx = fmax_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmax_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        if (!ONE) __syncwarp();   // every lane has its dims
         const bool fin = mx < INFINITY;
         int e = 0;
         if (fin && mx > 0.f) e = ilogbf(mx) - 14;
@@ -541,7 +564,7 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const HeadGroup
 
 // hg: heads and sets of warps. What is added up later has one part a head (its warps have added up theirs), as if one
 // warp had it: `whole`.
-template <int HD>
+template <int HD, bool ONE>
 __global__ void __launch_bounds__(Rows4Shape<HD>::threads, 1)
 rows4_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ Pools4 pools, const __grid_constant__ HeadGroups hg,
              const __grid_constant__ HeadGroups whole) {
@@ -595,7 +618,7 @@ rows4_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ Pools4 
         const Cut all{seg.grp, 2 * c_first + (runs.start(c_first) >= seg.first ? 0 : 1), c_last - c_first + 1, min(kRowTile, tv.n_rows - tv.r0), tv.r0, tv.sv.q0};
         if (cta == c_first + 1) cut = all;
         if (listed_by_tile && cta == c_first && threadIdx.x == 0) cuts[seg.tile * hg.groups + seg.grp] = all;
-        if (sub < hg.subs) rows4_segment<HD>(A, hg, ring, used, smem + warp * S::q, s_ml, seg, tv, c_first == c_last ? -1 : 2 * cta + (begin >= seg.first ? 0 : 1));
+        if (sub < hg.subs) rows4_segment<HD, ONE>(A, hg, ring, used, smem + warp * S::q, s_ml, seg, tv, c_first == c_last ? -1 : 2 * cta + (begin >= seg.first ? 0 : 1));
     }
     if (!listed_by_tile && threadIdx.x == 0) cuts[cta] = cut;
 }
@@ -785,7 +808,7 @@ size_t rows4_bytes(const hesa_cuda_paged_kv4* kv) {
     return kv->head_dim == 64 ? Rows4Shape<64>::bytes(parts) : kv->head_dim == 128 ? Rows4Shape<128>::bytes(parts) : Rows4Shape<256>::bytes(parts);
 }
 
-template <int HD>
+template <int HD, bool ONE>
 cudaError_t launch_rows4(AttnArgs a, const Pools4& pools, const Plan4& p, cudaStream_t s) {
     static bool set[64] = {};   // per instance and device
     int dev = 0;
@@ -794,7 +817,7 @@ cudaError_t launch_rows4(AttnArgs a, const Pools4& pools, const Plan4& p, cudaSt
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     using S = Rows4Shape<HD>;
     if (!set[dev]) {
-        e = cudaFuncSetAttribute(rows4_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::smem));
+        e = cudaFuncSetAttribute(rows4_kernel<HD, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::smem));
         if (e != cudaSuccess) return e;
         set[dev] = true;
     }
@@ -803,7 +826,7 @@ cudaError_t launch_rows4(AttnArgs a, const Pools4& pools, const Plan4& p, cudaSt
     const HeadGroups whole = one_warp_a_head(hg);
     for (a.tile0 = 0; a.tile0 < p.tiles && e == cudaSuccess; a.tile0 += kMostTiles) {
         a.n_split = std::min(kMostTiles, p.tiles - a.tile0);
-        e = launch_dep(rows4_kernel<HD>, dim3(kRowsCtas), S::threads, S::smem, s, a, pools, hg, whole);
+        e = launch_dep(rows4_kernel<HD, ONE>, dim3(kRowsCtas), S::threads, S::smem, s, a, pools, hg, whole);
         const int cuts = by_tile(a.n_split, whole) ? a.n_split * hg.groups : kRowsCtas;
         const int rows = std::min(kRowTile, a.b.max_new * a.group);
         const unsigned z = static_cast<int64_t>(cuts) * hg.heads * rows <= 8 * kRowsCtas ? rows : 1;
@@ -889,10 +912,11 @@ int hesa_cuda_paged_attention_kv4(const hesa_cuda_paged_kv4* kv, int32_t layer, 
             if (rc != HESA_CUDA_OK) return rc;
         }
     } else if (e == cudaSuccess) {
+        const bool one = batch->max_new == 1 && a.group == 1;   // 74 sequences of 2 tokens, 32 heads: 14.2 us, with the code for eight rows 14.7
         switch (kv->head_dim) {
-            case 64: e = launch_rows4<64>(a, pools, p, s); break;
-            case 128: e = launch_rows4<128>(a, pools, p, s); break;
-            default: e = launch_rows4<256>(a, pools, p, s); break;
+            case 64: e = one ? launch_rows4<64, true>(a, pools, p, s) : launch_rows4<64, false>(a, pools, p, s); break;
+            case 128: e = one ? launch_rows4<128, true>(a, pools, p, s) : launch_rows4<128, false>(a, pools, p, s); break;
+            default: e = one ? launch_rows4<256, true>(a, pools, p, s) : launch_rows4<256, false>(a, pools, p, s); break;
         }
     }
     return e == cudaSuccess ? HESA_CUDA_OK : record_cuda_error(e, "paged attention kernel");
