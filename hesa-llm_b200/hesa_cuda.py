@@ -726,10 +726,13 @@ class TokenBatch:
 def _rows(t, n: int, width: int, what: str, device):
     """Pointer and row stride of fp32 rows [n, width] (a column slice of a wider matrix is one)."""
     import torch
-    _want(t, torch.float32, what, device, 2)
-    if t.shape[0] != n or t.shape[1] != width or (t.stride(1) != 1 and width > 1):
+    if not (isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.get_device() == device and t.dim() == 2):
+        _want(t, torch.float32, what, device, 2)
+    rows, cols = t.shape
+    ld, step = t.stride()
+    if rows != n or cols != width or (step != 1 and width > 1):
         raise ValueError(f"{what} must be [{n}, {width}] with contiguous rows")
-    return t.data_ptr(), (t.stride(0) if n > 1 else width + (-width) % 4)
+    return t.data_ptr(), (ld if n > 1 else width + (-width) % 4)
 
 
 def _same_device(cache, batch=None):
@@ -924,8 +927,7 @@ def beam_select(logits, scores, width: int, ended=None, workspace=None, stream=N
     ep = None if ended is None else _ints(ended, "ended", n, dev)
 
     def outputs():
-        return (torch.empty(n, dtype=torch.float32, device=logits.device), torch.empty(n, dtype=torch.int32, device=logits.device),
-                torch.empty(n, dtype=torch.int32, device=logits.device))
+        return torch.empty_like(scores), torch.empty_like(scores, dtype=torch.int32), torch.empty_like(scores, dtype=torch.int32)
     best, parents, tokens = outputs() if stream is None else _new(outputs, stream)
     if workspace is None:
         workspace = _new(lambda: beam_select_workspace(n // width, width, vocab), stream)
