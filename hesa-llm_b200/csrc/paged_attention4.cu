@@ -31,7 +31,7 @@
 // the copies the kernel takes 90 us, without the products 65. More warps would fill
 // the pipes, but their registers are all taken (32 of a thread's are sums).
 // Measured (with combine_kernel): two contexts of 131072 and 100001 tokens, 64 heads on
-// 8, 100 us (301 MB, 3.0 TB/s; the fp16 cache 167); 32 of 1 to 8192 tokens 29.9 us (34);
+// 8, 100 us (301 MB, 3.0 TB/s; the fp16 cache 167); 32 of 1 to 8192 tokens 29.7 us (34);
 // one of 2048 tokens, 32 heads, 14.3 us (15.4): 5.4 us until the first products, 3 a
 // block, 4 to join the parts.
 //
@@ -57,7 +57,8 @@ namespace {
 
 constexpr int kKeys4 = 32;           // of a block
 constexpr int kCopyWarps4 = 4;
-constexpr int kSegCost4 = 2;         // blocks that starting a (tile, group) takes the time of
+constexpr int kSegCost4 = 2;         // blocks of every warp that starting a (tile, group) takes the time of,
+constexpr int kSegCostMost4 = 8;     // and blocks of a head: 100 sequences of 1 to 3000 tokens, 8 heads on 1, 21.2 us (32: 27.6, 16: 22.9), 12 on 2 21.8 (16: 24.1, 4: 25.5)
 constexpr int kScratchPage = 128;    // tokens of a page of the fp16 copy
 constexpr int64_t kScratchBytes = int64_t(1) << 30;
 
@@ -822,6 +823,7 @@ cudaError_t launch_rows4(AttnArgs a, const Pools4& pools, const Plan4& p, cudaSt
         set[dev] = true;
     }
     HeadGroups hg(a.c.n_kv, S::warps, p.heads, kSegCost4);
+    hg.cost = std::min(hg.cost, kSegCostMost4);
     if (hg.subs < 4) hg.least = 2;   // a start and a block are few units: 40 sequences of 2 tokens, 32 heads 16.9 us, with 4 22.8
     const HeadGroups whole = one_warp_a_head(hg);
     for (a.tile0 = 0; a.tile0 < p.tiles && e == cudaSuccess; a.tile0 += kMostTiles) {
