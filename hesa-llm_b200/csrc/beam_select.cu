@@ -14,7 +14,7 @@
 // all); a few beams, and many short rows, are bound by the chain of waits at a row's
 // end. 64 sequences of 8 beams, 131071 tokens, 355 of the beams alive: 49 us (186 MB,
 // 3.8 TB/s; without finding the largest 43, and the same with 1 to 5 parts a beam);
-// 128 of 16 beams, 3000 tokens 21 us; one of 4 beams, 32000 tokens 10.7 us.
+// 128 of 16 beams, 3000 tokens 39 us; one of 4 beams, 32000 tokens 10.7 us.
 #include "../../include/hesa_cuda.h"
 #include "abi_errors.h"
 #include "paged.h"

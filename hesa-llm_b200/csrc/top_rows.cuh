@@ -223,6 +223,7 @@ __device__ __forceinline__ Sums row_part(const float* row, int vocab, int split,
         uint64_t bound = n_max >= top_k ? sh.top[top_k - 1] : 0;
         if (threadIdx.x == 0) sh.n = 0;
         __syncthreads();
+        static_assert(cand_of(WARPS) >= kMaxTop * 4 * kUnroll, "what is read once fits");
         if (once) {   // at most kMaxTop threads, 16 values each
             if (mine != 0 && mine >= bound) {
 #pragma unroll
@@ -237,7 +238,7 @@ __device__ __forceinline__ Sums row_part(const float* row, int vocab, int split,
             __syncthreads();
         }
         // their values again: a warp takes one thread's quads, a quad a lane at a time
-        for (int f0 = once ? n_from : 0; f0 < n_from; f0 += kLpWarps) {
+        for (int f0 = once ? n_from : 0; f0 < n_from; f0 += WARPS) {
             const int f = f0 + warp < n_from ? sh.from[f0 + warp] : -1;
             const int base = q0 + (f >> 5) * 32 * kUnroll + (f & 31);
             const int n_mine = (q1 - q0 + kStep - 1) / kStep * kUnroll;   // quads of a thread at most

@@ -622,3 +622,29 @@ def test_two_host_threads_at_once(H):
     for t in threads:
         t.join()
     assert not wrong and H.device_status() == 0
+
+
+# The branches of the selection's dispatch: a cluster a sequence, two kernels with blocks of eight warps, and with blocks
+# of two; each with parts that a block reads in one pass, and longer ones whose largest values it reads again.
+BRANCHES = [
+    (3, 8, 4000), (2, 3, 5001), (5, 5, 3999), (3, 8, 20001), (2, 3, 40002), (74, 4, 9003),          # clusters
+    (10, 16, 4000), (4, 32, 3001), (75, 3, 2002), (20, 16, 9001), (80, 3, 9002), (80, 8, 12003), (5, 32, 20001),   # eight warps
+    (100, 3, 1001), (75, 8, 517), (30, 16, 1024), (12, 32, 899),                                    # two warps, one pass
+    (80, 5, 1023), (100, 3, 1030), (80, 4, 2050), (76, 8, 1025), (128, 16, 3000), (40, 16, 4095), (100, 32, 4096), (20, 32, 1537),
+]
+
+
+@pytest.mark.parametrize("n_seq,width,vocab", BRANCHES)
+def test_select_of_every_branch(H, n_seq, width, vocab):
+    """Rows of odd lengths begin at every alignment. Random values, ascending ones (the largest with the last threads),
+    and rows with their largest side by side (all with one thread)."""
+    g = torch.Generator(device="cuda").manual_seed(vocab * 33 + width)
+    n = n_seq * width
+    x = torch.randn(n, vocab, generator=g, device="cuda") * 3
+    x[1::3] = torch.linspace(-4, 4, vocab, device="cuda")
+    at = int(torch.randint(0, max(1, vocab - 16), (1,), generator=g, device="cuda"))
+    x[2::3, at:at + 16] += 9
+    scores = -torch.rand(n, generator=g, device="cuda") * 5
+    check(H, x, scores, width)
+    check(H, x, scores, width, (torch.rand(n, generator=g, device="cuda") < 0.3).int())
+    assert H.device_status() == 0
