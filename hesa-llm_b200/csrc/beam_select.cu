@@ -29,7 +29,13 @@ namespace {
 
 constexpr int kMaxWidth = kMaxTop;
 constexpr int kMostParts = 64;   // of a row
+
+// Blocks of two warps, against eight. What a row's largest are found in again takes them top / 2 steps instead of
+// top / 8, so that wide searches need more rows to gain: 128 sequences of 16 beams, 3000 tokens 38.6 us and 47.7, 62 of 16,
+// 1500 tokens 25.9 and 22.6, 100 of 32, 4096 tokens 91 and 77, 333 of 3, 3000 tokens 14.6 and 25.7. Rows of up to
+// kSmallOnce logits are read once at any address: 16 of 20, 1000 tokens 21.5 and 23.2, 200 of 16 25.4 and 49.8.
 constexpr int kSmallWarps = 2;
+constexpr int kSmallOnce = kSmallWarps * 32 * kUnroll * 4 - 3;
 
 struct RowPart {
     float m, z;
@@ -290,7 +296,7 @@ int hesa_cuda_beam_select(const float* logits, int64_t ld, int64_t n_seq, int32_
     uint64_t* keys = reinterpret_cast<uint64_t*>(parts + rows * n_split);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     // many short rows: small blocks, so that more of them, and of the waits at a row's end, go side by side
-    const bool small = vocab <= kPartElems && rows > 148 * 2;
+    const bool small = vocab <= kPartElems && rows > 148 * 2 && (vocab <= kSmallOnce || n_seq > 4 * width);
     cudaError_t e = launch_dep(small ? beam_rows_kernel<kSmallWarps> : beam_rows_kernel<kLpWarps>, dim3(static_cast<unsigned>(rows), static_cast<unsigned>(n_split)),
                                (small ? kSmallWarps : kLpWarps) * 32, 0, s, logits, ld, static_cast<int>(vocab), scores, ended, top, n_split, parts, keys);
     if (e == cudaSuccess)
