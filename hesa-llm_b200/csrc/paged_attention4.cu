@@ -797,6 +797,23 @@ hesa_cuda_paged_kv scratch_kv(const hesa_cuda_paged_kv4* kv, const Plan4& p, uin
     return s;
 }
 
+// What the chunk kernel needs beside the scratch: the most that any of the passes over the batch takes. The last pass may
+// have fewer sequences than the others, whose keys are then split over more CTAs, in parts that take room. 0: the copy would be no cache.
+size_t inner_bytes(const hesa_cuda_paged_kv4* kv, const Plan4& p, const hesa_cuda_token_batch* batch, int64_t n_head) {
+    const hesa_cuda_paged_kv s = scratch_kv(kv, p, reinterpret_cast<uint8_t*>(uintptr_t(16)));   // not looked into
+    hesa_cuda_token_batch b = *batch;
+    b.slots = nullptr;
+    size_t most = 0;
+    for (const int n : {p.n_seq, batch->n_seq % p.n_seq}) {
+        if (n == 0) continue;
+        b.n_seq = n;
+        const size_t need = hesa_cuda_paged_attention_workspace_size(&s, &b, n_head);
+        if (need == 0) return 0;
+        most = std::max(most, need);
+    }
+    return most;
+}
+
 // As what is added up later sees them: a head's warps have added up theirs.
 HeadGroups one_warp_a_head(HeadGroups hg) {
     hg.subs = 1;
@@ -849,11 +866,7 @@ size_t hesa_cuda_paged_attention_kv4_workspace_size(const hesa_cuda_paged_kv4* k
     if (check_paged_kv4(kv) != HESA_CUDA_OK || check_batch4(kv, 0, batch, n_head) != HESA_CUDA_OK) return 0;
     const Plan4 p = make_plan4(kv, batch, n_head);
     if (!p.chunk) return std::max<size_t>(rows4_bytes(kv), 16);
-    const hesa_cuda_paged_kv s = scratch_kv(kv, p, reinterpret_cast<uint8_t*>(uintptr_t(16)));   // not looked into
-    hesa_cuda_token_batch b = *batch;
-    b.n_seq = p.n_seq;
-    b.slots = nullptr;
-    const size_t inner = hesa_cuda_paged_attention_workspace_size(&s, &b, n_head);
+    const size_t inner = inner_bytes(kv, p, batch, n_head);
     return inner ? scratch_sizes(kv, p).all() + inner : 0;
 }
 

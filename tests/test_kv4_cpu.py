@@ -187,3 +187,40 @@ def test_values_are_fp16_numbers():
 def test_python_refusals():
     with pytest.raises((ValueError, RuntimeError, AssertionError)):
         H.beam_select(torch.zeros(4, 10), torch.zeros(4), 2)   # not on a GPU
+
+
+def test_workspaces_hold_every_pass_of_a_chunk():
+    """The fp16 copies of as many sequences as fit into 1 GB go at a time, as a cache of pages of 128 tokens; the last pass may
+    have fewer, and what the attention over each of them asks for is there."""
+    import random
+    r = random.Random(5)
+    L = H.lib()
+    several = more = 0
+    for i in range(3000):
+        n_kv, hd = r.choice((1, 2, 4, 8, 16, 32, 64)), r.choice((64, 128, 256))
+        g = r.choice((1, 2, 4, 8))
+        n_seq = r.randrange(1, r.choice((3, 10, 60)))
+        max_len = int(2 ** r.uniform(7, 19))
+        max_new = min(max_len, r.randrange(1, r.choice((100, 3000))))
+        tokens = min(max_new * n_seq, (1 << 31) // (2 * n_kv * g))
+        if max_new * g <= 64 or max_new > tokens:
+            continue
+        c = cache(n_kv_head=n_kv, head_dim=hd, page_stride=16 * n_kv * hd // 32, layer_stride=0, n_layer=1, n_slots=64, max_pages=1 << 15)
+        b = batch(n_seq=n_seq, n_tokens=r.randrange(max_new, tokens + 1), max_new=max_new, max_len=max_len)
+        size = L.hesa_cuda_paged_attention_kv4_workspace_size(ctypes.byref(c), ctypes.byref(b), n_kv * g)
+        pages = -(-max_len // 128)
+        token = 4 * n_kv * hd
+        at_a_time = max(1, min(n_seq, (1 << 30) // (pages * 128 * token)))
+        needs = []
+        for n in [at_a_time] * (n_seq // at_a_time) + [n_seq % at_a_time]:
+            if n == 0:
+                continue
+            inner = fp16_cache(n_kv_head=n_kv, head_dim=hd, page_size=128, page_stride=128 * n_kv * hd, layer_stride=0, n_layer=1,
+                               n_slots=at_a_time, max_pages=pages, n_pages=at_a_time * pages)
+            part = batch(n_seq=n, n_tokens=b.n_tokens, max_new=max_new, max_len=max_len)
+            needs.append(L.hesa_cuda_paged_attention_workspace_size(ctypes.byref(inner), ctypes.byref(part), n_kv * g))
+            assert needs[-1] > 0
+        assert size >= at_a_time * pages * 128 * token + max(needs), (n_kv, hd, g, n_seq, max_len, max_new)
+        several += len(needs) > 1
+        more += needs[-1] > needs[0]
+    assert several > 200 and more > 50

@@ -1,0 +1,43 @@
+"""Edges of attention over a cache in 4 bits: chunks that take several passes."""
+import pytest
+import torch
+
+from kv4_model import Case
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def H():
+    assert torch.cuda.is_available()
+    import hesa_cuda
+    hesa_cuda.lib()
+    hesa_cuda.clear_device_status()
+    return hesa_cuda
+
+
+def bounded(c, max_len):
+    """The case with tables and a batch for sequences of up to max_len tokens."""
+    H = c.H
+    pages = -(-max_len // c.page)
+    c.table = torch.nn.functional.pad(c.table, (0, pages - c.table.shape[1]), value=-1).contiguous()
+    c.cache = H.PagedKV4(*c.pools, c.table, c.seq_len, c.refs)
+    c.batch = H.TokenBatch(c.q_start, c.n_tokens, max(c.news), max_len, slots=c.slots)
+    return c
+
+
+@pytest.mark.parametrize("n_head,n_kv,hd,max_len,lens,news", [
+    (64, 8, 128, 131072, [300, 100, 2111], [100, 100, 100]),                                      # 2 + 1 sequences
+    (64, 8, 128, 30000, [500, 64, 70, 90, 64, 333, 80, 64, 1500], [64] * 9),                       # 8 + 1
+    (32, 32, 128, 32768, [300, 256, 257, 512, 700], [256, 256, 1, 30, 256]),                       # 2 + 2 + 1
+    (64, 8, 128, 16384, [70 + 13 * i for i in range(16)] + [900], [64] * 17),                      # 16 + 1
+    (16, 4, 256, 131072, [600, 100, 300], [200, 40, 130]),                                         # 2 + 1, in 64 keys a block
+])
+def test_the_last_pass_of_a_chunk_is_split_over_more_keys(n_head, n_kv, hd, max_len, lens, news):
+    """Sequences whose fp16 copies take more than 1 GB by the host's bound: the last pass has fewer of them, so that their keys
+    are split, which needs room in the workspace."""
+    c = bounded(Case(n_head, n_kv, hd, 64, lens, news, seed=len(lens)), max_len)
+    c.check()
+    ws = c.H.paged_attention_workspace(c.cache, c.batch, n_head)
+    ws.fill_(0x7e)
+    c.check(run=lambda **o: c.run(workspace=ws, **o), window=50)
