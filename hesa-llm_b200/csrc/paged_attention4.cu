@@ -282,7 +282,7 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const HeadGroup
 
     // ---- q as hi and lo halves of q * 2^-e, max |q| 2^-e in [2^14, 2^15), in the order of the codes' pairs ----
     const uint32_t qs = smem_addr(own) + lane * 16;
-    float qscale;   // 2^e; NaN for a row that is not finite
+    float qscale;   // 2^e; NaN for a row that is not finite, unless it sees no key: its zeros have no q
     {
         const float* q = A.q + static_cast<int64_t>(sv.q0 + t) * A.ldq + static_cast<int64_t>(h) * HD;
         if constexpr (!ONE) {   // whole rows at a time: a thread's own dims are a line of their own in each load, 1 us for eight heads of eight rows
@@ -318,7 +318,7 @@ __device__ __forceinline__ void rows4_segment(const AttnArgs& A, const HeadGroup
         if (fin && mx > 0.f) e = ilogbf(mx) - 14;
         // two factors, so that 2^-e stays finite for the smallest subnormal q
         const float f1 = ldexpf(1.f, -(e / 2)), f2 = fin ? ldexpf(1.f, -(e - e / 2)) : 0.f;
-        qscale = fin ? ldexpf(1.f, e) : NAN;
+        qscale = fin || (keys.hi <= keys.lo && keys.prefix <= 0) ? ldexpf(1.f, e) : NAN;
 #pragma unroll
         for (int w = 0; w < KW; ++w)
 #pragma unroll

@@ -389,7 +389,8 @@ typedef struct {
  * see (padding, other sequences, places past a slot's length) do not reach
  * it, whatever they hold. A k that is not finite where a row sees it gives NaN
  * in all of the row's dims, whatever its sign and the softcap; such a v gives a
- * result that is not finite in its dim. A row of q that is not finite gives NaN.
+ * result that is not finite in its dim. A row of q that is not finite gives NaN
+ * where it sees a key.
  * The workspace (16-byte aligned, need not be set) is scratch: calls of any
  * shape on one stream can share one of the largest size that they ask for,
  * calls that may overlap cannot. Results do not depend on scheduling. */

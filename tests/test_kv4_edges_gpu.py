@@ -1,4 +1,6 @@
-"""Edges of attention over a cache in 4 bits: chunks that take several passes."""
+"""Edges of attention over a cache in 4 bits: chunks that take several passes, rows that see nothing."""
+import math
+
 import pytest
 import torch
 
@@ -41,3 +43,21 @@ def test_the_last_pass_of_a_chunk_is_split_over_more_keys(n_head, n_kv, hd, max_
     ws = c.H.paged_attention_workspace(c.cache, c.batch, n_head)
     ws.fill_(0x7e)
     c.check(run=lambda **o: c.run(workspace=ws, **o), window=50)
+
+
+@pytest.mark.parametrize("n_head,new", [(2, 9), (4, 9), (4, 30), (16, 20)])
+def test_a_row_that_sees_nothing_gives_zeros_whatever_its_q(H, n_head, new):
+    """Rows of negative positions, some not finite, beside rows of the same tile that see keys."""
+    c = Case(n_head, 2, 128, 8, [5, 40], [new, 3], seed=new)
+    want = c.run().clone()
+    for bad in (math.nan, math.inf, -math.inf):
+        c.q[: new - 5: 2, ::7] = bad
+        c.q[new - 4, 0] = bad     # this one sees two keys
+        for o in (dict(), dict(softcap=9.0), dict(slopes=torch.ones(n_head, device="cuda"))):
+            out = c.run(**o)
+            assert not bool(out[: new - 5].any())
+            assert bool(torch.isnan(out[new - 4, :128]).all()) and bool(torch.isfinite(out[new - 4, 128:]).all())
+            assert bool(torch.isfinite(out[new - 3:]).all())
+            if not o:
+                assert torch.equal(out[new - 3:], want[new - 3:])
+    assert H.device_status() == 0
