@@ -684,9 +684,11 @@ class PagedKV4(PagedKV):
             # the stride of a dimension of one entry is not looked at
             if any(n > 1 and a != b for n, a, b in zip(t.shape, t.stride(), of_scales)):
                 raise ValueError(f"{what} must have the strides of k and v, counted in groups")
+        # and goes to the library as a multiple of 8, which it does not use
+        layer, stride = (s if n > 1 else s + -s % 8 for n, s in zip(k.shape, of_scales[:2]))
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self._tables(dev, n_layer, n_pages, page, n_kv, 2 * half, table, seq_len, page_refs)
-        self._struct(PagedKV4Struct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), of_scales[1], of_scales[0], n_layer, n_pages,
+        self._struct(PagedKV4Struct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), stride, layer, n_layer, n_pages,
                                     page, n_kv, 2 * half, table.data_ptr(), seq_len.data_ptr(), _ptr(page_refs), table.shape[0], table.shape[1]))
 
     @classmethod

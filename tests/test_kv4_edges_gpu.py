@@ -1,9 +1,10 @@
-"""Edges of attention over a cache in 4 bits: chunks that take several passes, rows that see nothing."""
+"""Edges of the cache in 4 bits: chunks that take several passes, rows that see nothing, pools of one page."""
 import math
 
 import pytest
 import torch
 
+import kv4_model
 from kv4_model import Case
 
 pytestmark = pytest.mark.gpu
@@ -60,4 +61,25 @@ def test_a_row_that_sees_nothing_gives_zeros_whatever_its_q(H, n_head, new):
             assert bool(torch.isfinite(out[new - 3:]).all())
             if not o:
                 assert torch.equal(out[new - 3:], want[new - 3:])
+    assert H.device_status() == 0
+
+
+@pytest.mark.parametrize("layers,page,n_kv,hd", [(1, 1, 1, 64), (3, 1, 1, 64), (2, 5, 1, 128), (1, 3, 3, 64), (2, 1, 1, 256)])
+@pytest.mark.parametrize("inside", [False, True])
+def test_a_pool_of_one_page(H, layers, page, n_kv, hd, inside):
+    """Its pages need no stride: a page whose groups are no multiple of 8 is one all the same."""
+    c = Case(2 * n_kv, n_kv, hd, page, [page], [1], seed=page, layers=layers, spare=0, inside=inside)
+    assert c.cache.n_pages == 1
+    c.check()
+    for cache in (H.PagedKV4.empty(layers, 1, page, n_kv, hd, 2, 1), c.cache):
+        cache.seq_len.zero_()
+        cache.page_refs.zero_()
+        H.kv_reserve(cache, torch.zeros(1, dtype=torch.int32, device="cuda"), torch.full((1,), page, dtype=torch.int32, device="cuda"))
+        batch = H.TokenBatch(torch.tensor([0, page], dtype=torch.int32, device="cuda"), page, page, page)
+        g = torch.Generator(device="cuda").manual_seed(1)
+        k, v = (torch.randn(page, n_kv * hd, generator=g, device="cuda") for _ in range(2))
+        for layer in range(layers):
+            H.rope_kv_paged(cache, layer, batch, None, k, v, 2 * n_kv)
+            for got, x in zip(H.kv_read(cache, layer, batch), (k, v)):
+                assert torch.equal(got, kv4_model.values(*kv4_model.quantize(x.view(page, n_kv, hd))).view(page, -1))
     assert H.device_status() == 0
