@@ -695,6 +695,8 @@ class PagedKV4(PagedKV):
     def empty(cls, n_layer: int, n_pages: int, page_size: int, n_kv_head: int, head_dim: int, n_slots: int, max_pages: int):
         """A new cache on the current device with every page free and every slot empty."""
         import torch
+        if head_dim % 32:
+            raise ValueError("head_dim must be a multiple of 32")
         # pages start at multiples of 8 groups, whatever a page holds
         per = page_size * n_kv_head * (head_dim // 32)
         stride = -(-per // 8) * 8

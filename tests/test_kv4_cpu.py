@@ -224,3 +224,9 @@ def test_workspaces_hold_every_pass_of_a_chunk():
         several += len(needs) > 1
         more += needs[-1] > needs[0]
     assert several > 200 and more > 50
+
+
+@pytest.mark.parametrize("head_dim", [48, 80, 100, 144, 1])
+def test_an_empty_cache_has_whole_groups(head_dim):
+    with pytest.raises(ValueError, match="multiple of 32"):
+        H.PagedKV4.empty(1, 4, 16, 2, head_dim, 2, 2)
