@@ -1,4 +1,5 @@
-"""Edges of the cache in 4 bits: chunks that take several passes, rows that see nothing, pools of one page."""
+"""Edges of the cache in 4 bits: chunks that take several passes, rows that see nothing, pools of one page,
+windows near 2^31, scales at ties."""
 import math
 
 import pytest
@@ -82,4 +83,37 @@ def test_a_pool_of_one_page(H, layers, page, n_kv, hd, inside):
             H.rope_kv_paged(cache, layer, batch, None, k, v, 2 * n_kv)
             for got, x in zip(H.kv_read(cache, layer, batch), (k, v)):
                 assert torch.equal(got, kv4_model.values(*kv4_model.quantize(x.view(page, n_kv, hd))).view(page, -1))
+    assert H.device_status() == 0
+
+
+@pytest.mark.parametrize("window", [1 << 30, 2 ** 31 - 1])
+@pytest.mark.parametrize("n_head,news", [(4, [9, 3]), (4, [70, 150]), (16, [20, 20])])
+def test_the_widest_window_is_none(H, window, n_head, news):
+    """Also where positions are negative (more new tokens than tokens), whatever scratch holds."""
+    c = Case(n_head, 2, 64, 8, [5, 140], news, seed=52)
+    ws = H.paged_attention_workspace(c.cache, c.batch, n_head)
+    ws.fill_(0x7e)   # fp16 0x7e7e is NaN
+    want = c.run()
+    assert bool(torch.isfinite(want).all()) and torch.equal(c.run(window=window, workspace=ws), want) and H.device_status() == 0
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_scales_between_two_numbers_go_to_the_even_one(H, hd):
+    """m / -8 half a step above 128 .. 255 in the last of 8 bits, of all sizes; the format's model on the CPU, where powers of
+    two are exact."""
+    rows = []
+    g = torch.Generator().manual_seed(3)
+    for e in list(range(-24, 5)) + [-30, -17]:
+        for n in (128, 129, 130, 200, 201, 254, 255):
+            x = (torch.rand(hd, generator=g) * 1.9 - 0.95) * n * 2.0 ** e
+            x[int(torch.randint(0, hd, (1,), generator=g))] = -8 * (n + 0.5) * 2.0 ** e * (1 - 2 * (n & 1))
+            x[int(torch.randint(0, hd, (1,), generator=g))] = 8 * (n + 0.5) * 2.0 ** e * (1 - 2 * (n & 1))
+            rows.append(x)
+    x = torch.stack(rows)
+    n = len(rows)
+    c = Case(1, 1, hd, 16, [n], [n], seed=0)
+    H.rope_kv_paged(c.cache, 0, c.batch, None, x.cuda(), -x.cuda(), 1)
+    for got, y in zip(H.kv_read(c.cache, 0, c.batch), (x, -x)):
+        # the largest, above 2720, are NaN
+        assert torch.allclose(got.cpu(), kv4_model.values(*kv4_model.quantize(y)), rtol=0, atol=0, equal_nan=True)
     assert H.device_status() == 0
