@@ -12,9 +12,10 @@
 // made in 64 bits from z's fp32 terms.
 // HBM-bound: every logit is read once (those of ended and ruled-out beams not at
 // all); a few beams are bound by the chain of waits at a row's end, many short rows by
-// what is done there (128 of 16 beams, 3000 tokens: 61% of issue slots, 10% of DRAM). 64 sequences of 8 beams, 131071 tokens, 355 of the beams alive: 49 us (186 MB,
-// 3.8 TB/s; without finding the largest 43, and the same with 1 to 5 parts a beam);
-// 128 of 16 beams, 3000 tokens 39 us; one of 4 beams, 32000 tokens 10.7 us.
+// what is done there. 64 sequences of 8 beams, 131071 tokens, 355 of the beams alive:
+// 49 us (186 MB, 3.8 TB/s; without finding the largest 43, and the same with 1 to 5
+// parts a beam); 128 of 16 beams, 3000 tokens 39 us (61% of issue slots, 10% of DRAM);
+// one of 4 beams, 32000 tokens 10.7 us.
 #include "../../include/hesa_cuda.h"
 #include "abi_errors.h"
 #include "paged.h"
