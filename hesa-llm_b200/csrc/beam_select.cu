@@ -14,7 +14,7 @@
 // all); a few beams are bound by the chain of waits at a row's end, many short rows by
 // what is done there. 64 sequences of 8 beams, 131071 tokens, 355 of the beams alive:
 // 49 us (186 MB, 3.8 TB/s; without finding the largest 43, and the same with 1 to 5
-// parts a beam); 128 of 16 beams, 3000 tokens 39 us (61% of issue slots, 10% of DRAM);
+// parts a beam); 128 of 16 beams, 3000 tokens 32 us (the first kernel 58% of issue slots, 13% of DRAM);
 // one of 4 beams, 32000 tokens 10.7 us.
 #include "../../include/hesa_cuda.h"
 #include "abi_errors.h"
@@ -32,9 +32,9 @@ constexpr int kMaxWidth = kMaxTop;
 constexpr int kMostParts = 64;   // of a row
 
 // Blocks of two warps, against eight. What a row's largest are found in again takes them top / 2 steps instead of
-// top / 8, so that wide searches need more rows to gain: 128 sequences of 16 beams, 3000 tokens 38.6 us and 47.7, 62 of 16,
-// 1500 tokens 25.9 and 22.6, 100 of 32, 4096 tokens 91 and 77, 333 of 3, 3000 tokens 14.6 and 25.7. Rows of up to
-// kSmallOnce logits are read once at any address: 16 of 20, 1000 tokens 21.5 and 23.2, 200 of 16 25.4 and 49.8.
+// top / 8, so that wide searches need more rows to gain: 62 sequences of 16 beams, 3000 tokens 22.6 us and 29.5, 31 of 32,
+// 1500 tokens 48 and 42, 100 of 32 71 and 72, 333 of 3, 3000 tokens 13.7 and 24.7. Rows of up to kSmallOnce logits are read
+// once at any address: 16 of 20, 1000 tokens 21.9 and 23.3, 200 of 16 25.2 and 49.2.
 constexpr int kSmallWarps = 2;
 constexpr int kSmallOnce = kSmallWarps * 32 * kUnroll * 4 - 3;
 
@@ -297,7 +297,7 @@ int hesa_cuda_beam_select(const float* logits, int64_t ld, int64_t n_seq, int32_
     uint64_t* keys = reinterpret_cast<uint64_t*>(parts + rows * n_split);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     // many short rows: small blocks, so that more of them, and of the waits at a row's end, go side by side
-    const bool small = vocab <= kPartElems && rows > 148 * 2 && (vocab <= kSmallOnce || n_seq > 4 * width);
+    const bool small = vocab <= kPartElems && rows > 148 * 2 && (vocab <= kSmallOnce || n_seq > 2 * width);
     cudaError_t e = launch_dep(small ? beam_rows_kernel<kSmallWarps> : beam_rows_kernel<kLpWarps>, dim3(static_cast<unsigned>(rows), static_cast<unsigned>(n_split)),
                                (small ? kSmallWarps : kLpWarps) * 32, 0, s, logits, ld, static_cast<int>(vocab), scores, ended, top, n_split, parts, keys);
     if (e == cudaSuccess)

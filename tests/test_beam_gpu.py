@@ -630,9 +630,9 @@ BRANCHES = [
     (3, 8, 4000), (2, 3, 5001), (5, 5, 3999), (3, 8, 20001), (2, 3, 40002), (74, 4, 9003),          # clusters
     (10, 16, 4000), (4, 32, 3001), (75, 3, 2002), (20, 16, 9001), (80, 3, 9002), (80, 8, 12003), (5, 32, 20001),   # eight warps
     (100, 3, 1001), (75, 8, 517), (30, 16, 1020), (12, 32, 899), (300, 4, 1021),                    # two warps, one pass
-    # short rows that are read again: two warps where there are more than 4 * width sequences
+    # short rows that are read again: two warps where there are more than 2 * width sequences
     (80, 5, 1023), (100, 3, 1030), (80, 4, 2050), (76, 8, 1025), (128, 16, 3000), (40, 16, 4095), (100, 32, 4096), (20, 32, 1537),
-    (65, 16, 1022), (131, 32, 1537), (64, 16, 1022), (30, 16, 1024),
+    (65, 16, 1022), (131, 32, 1537), (64, 16, 1022), (33, 16, 1022), (32, 16, 1022), (65, 32, 1537), (64, 32, 1537), (30, 16, 1024),
 ]
 
 
