@@ -355,7 +355,7 @@ rows_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ HeadGrou
     grid_dep_wait();
     grid_dep_launch();   // combine_kernel may be set up meanwhile; it waits for this grid's end
     const int64_t units = tile_units<S::warps + kCopyWarps, kKeyBlock>(A, hg, tiles, s_pre, s_sum) * hg.groups;
-    const Runs runs(units, gridDim.x, hg.least);
+    const Runs runs(units, gridDim.x, kLeastUnits);   // a constant: 0.15 us less than from hg
     const bool listed_by_tile = by_tile(tiles, hg);
     Cut* cuts = reinterpret_cast<Cut*>(A.part);
     int64_t u = 0, end = 0;
