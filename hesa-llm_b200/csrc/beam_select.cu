@@ -14,7 +14,7 @@
 // all); a few beams are bound by the chain of waits at a row's end, many short rows by
 // what is done there. 64 sequences of 8 beams, 131071 tokens, 355 of the beams alive:
 // 49 us (186 MB, 3.8 TB/s; without finding the largest 43, and the same with 1 to 5
-// parts a beam); 128 of 16 beams, 3000 tokens 32 us (the first kernel 58% of issue slots, 13% of DRAM);
+// parts a beam); 128 of 16 beams, 3000 tokens 30 us (the first kernel 58% of issue slots, 13% of DRAM);
 // one of 4 beams, 32000 tokens 10.7 us.
 #include "../../include/hesa_cuda.h"
 #include "abi_errors.h"
@@ -32,7 +32,7 @@ constexpr int kMaxWidth = kMaxTop;
 constexpr int kMostParts = 64;   // of a row
 
 // Blocks of two warps, against eight. What a row's largest are found in again takes them top / 2 steps instead of
-// top / 8, so that wide searches need more rows to gain: 62 sequences of 16 beams, 3000 tokens 22.6 us and 29.5, 31 of 32,
+// top / 8, so that wide searches need more rows to gain: 62 sequences of 16 beams, 3000 tokens 22.1 us and 29.5, 31 of 32,
 // 1500 tokens 48 and 42, 100 of 32 71 and 72, 333 of 3, 3000 tokens 13.7 and 24.7. Rows of up to kSmallOnce logits are read
 // once at any address: 16 of 20, 1000 tokens 21.9 and 23.3, 200 of 16 25.2 and 49.2.
 constexpr int kSmallWarps = 2;

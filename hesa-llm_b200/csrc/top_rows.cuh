@@ -249,19 +249,21 @@ __device__ __forceinline__ Sums row_part(const float* row, int vocab, int split,
                 int q[kAgain];
 #pragma unroll
                 for (int a = 0; a < kAgain; ++a) {
-                    if (i1 + a * 32 >= n_mine) break;   // (100 rows of 32000, 32 alternatives: 20.7 us, with reads of nothing 24.1)
+                    if (i1 + a * 32 >= n_mine) break;   // (100 rows of 32000, 32 alternatives: 19.9 us, with reads of nothing 24.1)
                     const int i = i1 + a * 32 + lane;
                     q[a] = f >= 0 && i < n_mine ? base + (i / kUnroll) * kStep + (i % kUnroll) * 32 : q1;
-                    v[a] = quad(q[a]);
+                    if (q[a] < q1) v[a] = quad(q[a]);
                 }
 #pragma unroll
                 for (int a = 0; a < kAgain; ++a) {
                     if (i1 + a * 32 >= n_mine) break;
-                    uint64_t k[4];
-                    keys(q[a], v[a], k);
+                    if (q[a] < q1) {
+                        uint64_t k[4];
+                        keys(q[a], v[a], k);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (k[i] != 0 && k[i] >= bound) sh.cand[atomicAdd(&sh.n, 1)] = k[i];
+                        for (int i = 0; i < 4; ++i)
+                            if (k[i] != 0 && k[i] >= bound) sh.cand[atomicAdd(&sh.n, 1)] = k[i];
+                    }
                     __syncthreads();
                     // as many more may come: keep the k largest, the k-th is the new bound
                     const int n = sh.n;
