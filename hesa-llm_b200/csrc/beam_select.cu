@@ -15,7 +15,7 @@
 // what is done there. 64 sequences of 8 beams, 131071 tokens, 355 of the beams alive:
 // 49 us (186 MB, 3.8 TB/s; without finding the largest 43, and the same with 1 to 5
 // parts a beam); 128 of 16 beams, 3000 tokens 30 us (the first kernel 58% of issue slots, 13% of DRAM);
-// one of 4 beams, 32000 tokens 10.7 us.
+// one of 4 beams, 32000 tokens 9.8 us.
 #include "../../include/hesa_cuda.h"
 #include "abi_errors.h"
 #include "paged.h"

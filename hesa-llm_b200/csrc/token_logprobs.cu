@@ -18,8 +18,8 @@
 // row's alignment (the first and the last quad of a row are read by the word), a
 // step ahead of its use. Few rows are split over blocks; the last block of a row
 // to arrive joins the parts.
-// 1024 rows of 131071, five alternatives: 101 us (537 MB, 5.3 TB/s), 32: 150 us, none: 85 us; one row of 32000:
-// 9.9 us.
+// 1024 rows of 131071, five alternatives: 99 us (537 MB, 5.4 TB/s), 32: 149 us, none: 85 us; one row of 32000:
+// 9.2 us.
 #include "../../include/hesa_cuda.h"
 #include "abi_errors.h"
 #include "paged.h"
